@@ -708,6 +708,69 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
     return router_launch(logits, l_dt, tokens, n_experts, k, h, h_dt, hidden, gate, g_dt, shared_id, ids, w, stream);
 }
 
+int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t tokens, int64_t n_experts, int k, int scoring,
+                      const float* bias, int n_groups, int topk_groups, int group_score, int renormalise, float scale,
+                      const void* h, int h_dt, int64_t hidden, const void* gate, int g_dt, int64_t shared_id,
+                      int32_t* ids, float* w, void* stream)
+{
+    clear_error();
+    CHECK(tokens >= 0, "vq2_router_select: bad token count");
+    CHECK(n_experts >= 1 && n_experts <= VQ2_ROUTER_MAX_EXPERTS, "vq2_router_select: n_experts=%lld not in [1, %d]",
+          (long long)n_experts, VQ2_ROUTER_MAX_EXPERTS);
+    CHECK(k >= 1 && k <= VQ2_ROUTER_MAX_TOPK && k <= n_experts, "vq2_router_select: k=%d out of range", k);
+    CHECK(scoring == VQ2_SCORE_SOFTMAX || scoring == VQ2_SCORE_SIGMOID, "vq2_router_select: scoring %d invalid", scoring);
+    CHECK(n_groups >= 1 && n_groups <= VQ2_ROUTER_MAX_GROUPS && n_experts % n_groups == 0,
+          "vq2_router_select: n_groups=%d must be at most %d and divide n_experts=%lld", n_groups, VQ2_ROUTER_MAX_GROUPS,
+          (long long)n_experts);
+    CHECK(topk_groups >= 1 && topk_groups <= n_groups && topk_groups * (n_experts / n_groups) >= k,
+          "vq2_router_select: topk_groups=%d out of range (1..%d, with k=%d experts among them)", topk_groups, n_groups, k);
+    CHECK(group_score == VQ2_GROUP_MAX || group_score == VQ2_GROUP_TOP2, "vq2_router_select: group_score %d invalid",
+          group_score);
+    CHECK(scale == scale, "vq2_router_select: scale is NaN");
+    CHECK(shared_id <= 0x7FFFFFFF, "vq2_router_select: shared_id does not fit int32");
+    if (tokens == 0) return VQ2_OK;
+    if (tokens > 0x7FFFFFFF) return set_error(VQ2_ERR_UNSUPPORTED, "vq2_router_select: too many tokens");
+    CHECK(logits && ids && w, "vq2_router_select: NULL pointer argument");
+    CHECK(dt_ok(l_dt), "vq2_router_select: bad logits dtype");
+    CHECK(l_stride >= n_experts || tokens == 1, "vq2_router_select: l_stride < n_experts");
+    if (shared_id >= 0 && gate) {
+        CHECK(h && hidden > 0, "vq2_router_select: shared gate needs h and hidden");
+        CHECK(dt_ok(h_dt) && dt_ok(g_dt), "vq2_router_select: bad h/gate dtype");
+    }
+    return router_select_launch(RouterSelectCall{logits, l_dt, l_stride, tokens, n_experts, k, scoring, bias, n_groups,
+                                                 topk_groups, group_score, renormalise != 0, scale, h, h_dt, hidden, gate,
+                                                 g_dt, shared_id < 0 ? -1 : shared_id, ids, w, stream});
+}
+
+size_t vq2_sample_workspace(int64_t rows, int64_t vocab) { return sample_workspace_bytes(rows, vocab); }
+
+int vq2_sample(const void* logits, int l_dt, int64_t l_stride, int64_t rows, int64_t vocab, const float* u,
+               float temperature, const float* temperature_rows, int64_t top_k, const int32_t* top_k_rows, float top_p,
+               const float* top_p_rows, float min_p, const float* min_p_rows, int64_t* out_idx, float* out_logprob,
+               void* workspace, size_t ws_bytes, void* stream)
+{
+    clear_error();
+    CHECK(rows >= 0, "vq2_sample: bad row count");
+    CHECK(vocab >= 1 && vocab <= VQ2_SAMPLE_MAX_VOCAB, "vq2_sample: vocab=%lld not in [1, %d]", (long long)vocab,
+          VQ2_SAMPLE_MAX_VOCAB);
+    CHECK(temperature_rows || temperature >= 0.0f, "vq2_sample: temperature %g is negative or NaN", (double)temperature);
+    CHECK(top_p_rows || (top_p >= 0.0f), "vq2_sample: top_p %g is negative or NaN", (double)top_p);
+    CHECK(min_p_rows || (min_p >= 0.0f && min_p <= 1.0f), "vq2_sample: min_p %g not in [0, 1]", (double)min_p);
+    CHECK(top_k_rows || top_k >= 0, "vq2_sample: top_k %lld is negative", (long long)top_k);
+    if (rows == 0) return VQ2_OK;
+    if (rows > VQ2_SAMPLE_MAX_ROWS)
+        return set_error(VQ2_ERR_UNSUPPORTED, "vq2_sample: rows=%lld > %d", (long long)rows, VQ2_SAMPLE_MAX_ROWS);
+    CHECK(logits && u && out_idx && out_logprob, "vq2_sample: NULL pointer argument");
+    CHECK(dt_ok(l_dt), "vq2_sample: bad logits dtype");
+    CHECK(l_stride >= vocab || rows == 1, "vq2_sample: l_stride < vocab");
+    CHECK((uintptr_t)out_idx % 8 == 0, "vq2_sample: out_idx must be 8-byte aligned");
+    const size_t need = sample_workspace_bytes(rows, vocab);
+    CHECK(need == 0 || (workspace && ws_bytes >= need), "vq2_sample: workspace of %zu bytes needed, got %zu", need, ws_bytes);
+    CHECK((uintptr_t)workspace % 256 == 0, "vq2_sample: workspace must be 256-byte aligned");
+    return sample_launch(SampleCall{logits, l_dt, l_stride, rows, vocab, u, temperature, temperature_rows, top_k, top_k_rows,
+                                    top_p, top_p_rows, min_p, min_p_rows, out_idx, out_logprob, workspace, ws_bytes, stream});
+}
+
 int vq2_argmax_rows(const void* v, int v_dt, int64_t rows, int64_t cols, int64_t* out_idx, float* out_val,
                     void* stream)
 {

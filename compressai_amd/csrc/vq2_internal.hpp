@@ -347,6 +347,61 @@ int router_launch(const void* logits, int l_dt, int64_t tokens, int64_t n_expert
                   int h_dt, int64_t hidden, const void* gate, int g_dt, int64_t shared_id, int32_t* ids, float* w,
                   void* stream);
 
+// Expert routing with scores, bias and groups (vq2_select.hip).
+struct RouterSelectCall {
+    const void* logits;
+    int l_dt;
+    int64_t l_stride;  // elements between the tokens' logits
+    int64_t tokens;
+    int64_t n_experts;
+    int k;
+    int scoring;
+    const float* bias;  // null: none
+    int n_groups;
+    int keep;
+    int group_score;
+    int renorm;
+    float scale;
+    const void* h;
+    int h_dt;
+    int64_t hidden;
+    const void* gate;  // null: the shared expert weighs 1
+    int g_dt;
+    int64_t shared_id;  // < 0: none
+    int32_t* ids;
+    float* w;
+    void* stream;
+};
+
+int router_select_launch(const RouterSelectCall& c);
+
+// The next token of each row (vq2_sample.hip).  A setting's `_rows` pointer,
+// where not null, holds one value per row in place of the common one.
+struct SampleCall {
+    const void* logits;
+    int l_dt;
+    int64_t l_stride;  // elements between rows
+    int64_t rows;
+    int64_t vocab;
+    const float* u;
+    float temperature;
+    const float* temperature_rows;
+    int64_t top_k;
+    const int32_t* top_k_rows;
+    float top_p;
+    const float* top_p_rows;
+    float min_p;
+    const float* min_p_rows;
+    int64_t* out_idx;
+    float* out_logprob;
+    void* workspace;
+    size_t ws_bytes;
+    void* stream;
+};
+
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab);  // 0 for sizes that vq2_sample refuses
+int sample_launch(const SampleCall& c);
+
 int dequant_launch(const int16_t* idx0, const void* idx1, int s2, const void* cb0, const void* cb1, int cb_dt,
                    const void* scale, int s_dt, int64_t r0, int64_t r1, int64_t n, float* out, void* stream);
 

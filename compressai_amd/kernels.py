@@ -13,8 +13,8 @@ Kept names and signatures (reference: vq2/kernels.py):
   attention / DeltaNet fusions they install are outside this library)
 
 Additive entry points: vq_gemv_16_16 (4 bpw), batched GEMV (x of shape
-[B, n]), vq_rht, vq_swiglu_rht, vq_router_topk, vq_moe_down_combine,
-vq_gemv_argmax, vq_argmax, vq_dequant_rows, vq_decode_idx.
+[B, n]), vq_rht, vq_swiglu_rht, vq_router_topk, vq_router_select,
+vq_moe_down_combine, vq_gemv_argmax, vq_sample, vq_argmax, vq_dequant_rows, vq_decode_idx.
 
 The entries of the small calls (vq_sorted_gemv, vq_gemv_rht, vq_rows_gemm,
 vq_sorted_moe) hand the calls without given outputs to their native twins
@@ -31,6 +31,7 @@ is selectable (``out_dtype``; bf16 by default, as in the reference).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import weakref
@@ -46,7 +47,7 @@ __all__ = [
     "vq_moe_parallel_gate_up", "vq_moe_parallel_down", "vq_moe_down_combine", "vq_moe_grouped",
     "vq_gemv_rht", "vq_moe_gate_up_rht", "vq_moe_down_swiglu_combine", "vq_gemm_small_m",
     "vq_moe_router_gate_up_rht", "vq_unpack_fixed", "SortedPlanes", "vq_sorted_gemv", "vq_sorted_gemv_argmax",
-    "vq_rht", "vq_swiglu_rht", "vq_router_topk", "vq_gemv_argmax", "vq_argmax",
+    "vq_rht", "vq_swiglu_rht", "vq_router_topk", "vq_router_select", "vq_sample", "vq_gemv_argmax", "vq_argmax",
     "vq_dequant_rows", "vq_decode_idx", "patch_transformers_kernels",
     "optimize_deltanet_layers", "Vq2Error",
 ]
@@ -1443,6 +1444,106 @@ def vq_router_topk(logits, k=8, h=None, shared_gate=None, shared_id=-1, *, ids=N
               _dt(h, "h") if extra else 0, hid, _p(shared_gate) if extra else None,
               _dt(shared_gate, "gate") if extra else 0, int(shared_id), _p(ids), _p(w), _stream(dev))
     return ids, w
+
+
+def _rows2d(t, what):
+    """t [..., n] as rows [R, n] of unit stride, without a copy, and the
+    elements between them."""
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise Vq2Error(f"{what} must be [..., n], got {tuple(t.shape)}")
+    if t.dim() != 2:
+        t = _contig(t, what).reshape(-1, t.shape[-1])
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise Vq2Error(f"{what} must have a unit-stride last dim")
+    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if stride < t.shape[1]:
+        raise Vq2Error(f"{what}: rows overlap (stride {stride} of {t.shape[1]} columns)")
+    return t, stride
+
+
+def _on_device(dev):
+    """Makes dev current for a launch on its stream (it nearly always is)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, topk_groups=None, group_score="max",
+                     renormalise=True, scale=1.0, h=None, shared_gate=None, shared_id=-1, ids=None, w=None):
+    """The router's further forms, per token: scores s = softmax(logits) or
+    sigmoid(logits) (``scoring``), choices c = s + bias (fp32 [E], a balance
+    bias that chooses but does not weigh); of n_groups groups of consecutive
+    experts the topk_groups (None: all) with the largest best c ("max") or sum of
+    their two best ("top2") stay; the k largest c among them in descending
+    order, ties to the lower id, weigh s / (sum of the k s if renormalise
+    else 1) * scale.  Experts with logit -inf or NaN (or bias) are masked:
+    last, weight 0.  With shared_id >= 0 an extra slot k carries the shared
+    expert with weight sigmoid(shared_gate . h), or 1 without a gate.
+    logits [..., E] (2-D: any row stride).  Returns (ids int32 [T, k(+1)],
+    w float32 [T, k(+1)]).  ``vq_router_topk`` is the softmax, renormalised
+    form without bias and groups."""
+    k, n_groups, shared_id = int(k), int(n_groups), int(shared_id)
+    topk_groups = n_groups if topk_groups is None else int(topk_groups)
+    if scoring not in _lib.SCORING or group_score not in _lib.GROUP_SCORE:
+        raise Vq2Error(f"vq_router_select: scoring {scoring!r} (softmax/sigmoid), group_score {group_score!r} (max/top2)")
+    dev = _dev(logits, bias, h, shared_gate, ids, w)
+    lg, stride = _rows2d(logits, "logits")
+    T, E = lg.shape
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != E or not bias.is_contiguous()):
+        raise Vq2Error(f"bias must be a contiguous float32 [{E}]")
+    slots = k + (1 if shared_id >= 0 else 0)
+    gate, hid = None, 0
+    if shared_id >= 0 and shared_gate is not None:
+        if h is None:
+            raise Vq2Error("shared expert gate needs h")
+        gate = _gate_vec(shared_gate, shared_gate.numel())
+        hid = gate.numel()
+        if h.numel() != T * hid:
+            raise Vq2Error(f"h must hold {T} x {hid} values, got {tuple(h.shape)}")
+        _contig(h, "h")
+    for t, nm, dt in ((ids, "ids", torch.int32), (w, "w", torch.float32)):
+        if t is not None and (t.dtype != dt or t.numel() != T * slots or not t.is_contiguous()):
+            raise Vq2Error(f"{nm} must be a contiguous {dt} [{T}, {slots}]")
+    if ids is None:
+        ids = torch.empty((T, slots), dtype=torch.int32, device=dev)
+    if w is None:
+        w = torch.empty((T, slots), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        _lib.call("vq2_router_select", _p(lg), _dt(lg, "logits"), stride, T, E, k, _lib.SCORING[scoring], _p(bias),
+                  n_groups, topk_groups, _lib.GROUP_SCORE[group_score], 1 if renormalise else 0, float(scale),
+                  _p(h) if gate is not None else None, _dt(h, "h") if gate is not None else 0, hid, _p(gate),
+                  _dt(gate, "gate") if gate is not None else 0, shared_id, _p(ids), _p(w), _stream(dev))
+    return ids, w
+
+
+def vq_sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of each row of logits [..., V] (2-D: any row stride) at
+    the given random numbers u (fp32 [rows], in [0, 1)): weights
+    exp((l - max) / temperature); the top_k largest (0: all); of those, in
+    descending order, entries while the ones before weigh less than top_p of
+    them; of those, the ones of weight >= min_p times the largest; the first
+    column at which their running sum exceeds u times the total.  Ties go to
+    the lower column; temperature 0 takes the first maximum; -inf and NaN
+    columns are absent, and a row of nothing else gives token -1 and a NaN
+    logprob.  Each setting is a number for all rows or a tensor [rows] (fp32;
+    top_k int32).  Returns (idx int64 [rows], logprob fp32 [rows]: the log of
+    the probability the token was drawn with)."""
+    rows_of = [t if torch.is_tensor(t) else None for t in (temperature, top_k, top_p, min_p)]
+    dev = _dev(logits, u, *rows_of)
+    lg, stride = _rows2d(logits, "logits")
+    B, V = lg.shape
+    for t, nm, dt in ((u, "u", torch.float32), (rows_of[0], "temperature", torch.float32), (rows_of[1], "top_k", torch.int32),
+                      (rows_of[2], "top_p", torch.float32), (rows_of[3], "min_p", torch.float32)):
+        if t is not None and (t.dtype != dt or t.numel() != B or not t.is_contiguous()):
+            raise Vq2Error(f"{nm} must be a contiguous {dt} [{B}]")
+    one = [0.0 if r is not None else v for r, v in zip(rows_of, (temperature, top_k, top_p, min_p))]
+    idx = torch.empty(B, dtype=torch.int64, device=dev)
+    logprob = torch.empty(B, dtype=torch.float32, device=dev)
+    nbytes = int(_lib.load().vq2_sample_workspace(B, V))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on_device(dev):
+        _lib.call("vq2_sample", _p(lg), _dt(lg, "logits"), stride, B, V, _p(u), float(one[0]), _p(rows_of[0]), int(one[1]),
+                  _p(rows_of[1]), float(one[2]), _p(rows_of[2]), float(one[3]), _p(rows_of[3]), _p(idx), _p(logprob),
+                  _p(ws), nbytes, _stream(dev))
+    return idx, logprob
 
 
 def vq_argmax(v):

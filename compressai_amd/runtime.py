@@ -9,7 +9,8 @@ runs the fused VQ GEMV (batch <= 2) or the matrix-core product of all rows
 (batch >= 3, ``kernels.vq_rows_gemm``) for every cfg in (16,), (16, 8), (16, 16) -- the reference
 fuses only batch 1 of (16,) and (16, 8) and otherwise re-materialises the
 dequantized matrix (runtime.py:91-110).
-``PackedLMHead`` (runtime.py:136-144) wraps it and adds ``argmax``.
+``PackedLMHead`` (runtime.py:136-144) wraps it and adds ``argmax`` and
+``sample`` (the next token under temperature, top-k, top-p and min-p).
 ``PackedProjections`` runs projections of one activation (q, k, v) in one
 launch.
 
@@ -318,6 +319,13 @@ class PackedLMHead(nn.Module):
 
     def forward(self, x):
         return self.lin(x)
+
+    def sample(self, x, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """The next token per row of x at the random numbers u (fp32 [rows]),
+        drawn from the head's fp32 logits (kernels.vq_sample, whose settings
+        these are): (idx int64 [B], logprob fp32 [B])."""
+        logits = self.lin(x.reshape(-1, self.lin.n), out_dtype=torch.float32)
+        return K.vq_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     def argmax(self, x):
         """Top-1 token per row of x without materialising bf16 logits:

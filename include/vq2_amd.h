@@ -326,6 +326,67 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
                     const void* h, int h_dt, int64_t hidden, const void* gate, int g_dt, int64_t shared_id,
                     int32_t* ids, float* w, void* stream);
 
+/* The router's further forms, per token, on given logits [tokens, l_stride]
+ * (n_experts of each row used):
+ *   s_e = softmax(l)_e over the n_experts, or sigmoid(l_e)   (scoring)
+ *   c_e = s_e + bias[e]                    (bias fp32 [n_experts] or NULL)
+ * The experts are cut into n_groups groups of n_experts / n_groups consecutive
+ * ones (1: no groups); the topk_groups groups of the largest group score --
+ * their best c or the sum of their two best -- stay, ties to the lower group.
+ *   ids[t, j] (int32), j < k: the k largest c of the groups that stay, in
+ *     descending order (ties toward the lower id)
+ *   w[t, j] (fp32) = s_ids[t, j] / (renormalise ? sum_j s_ids[t, j] : 1) * scale
+ * Without a bias c orders as the logits do, which are compared themselves;
+ * else choices are made in 64-bit arithmetic, c that agree to 42 bits as ties.
+ * An expert whose logit is -inf or NaN, or whose bias is, is masked: behind
+ * every other of its group, weight 0 (a token whose experts are all masked
+ * gets ids of weight 0).  If shared_id >= 0, slot k of each row is the shared
+ * expert: ids[t, k] = shared_id, w[t, k] = sigmoid(sum_i gate[i] * h[t, i]), or
+ * 1 with a NULL gate.  Row stride of ids / w is k (+ 1).  k <=
+ * VQ2_ROUTER_MAX_TOPK.  Beside the reference's router (vq2_router_topk), for
+ * checkpoints that route otherwise; no counterpart in the reference. */
+#define VQ2_SCORE_SOFTMAX 0
+#define VQ2_SCORE_SIGMOID 1
+#define VQ2_GROUP_MAX 0
+#define VQ2_GROUP_TOP2 1
+#define VQ2_ROUTER_MAX_EXPERTS 1024
+#define VQ2_ROUTER_MAX_GROUPS 64
+int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t tokens, int64_t n_experts, int k, int scoring,
+                      const float* bias, int n_groups, int topk_groups, int group_score, int renormalise, float scale,
+                      const void* h, int h_dt, int64_t hidden, const void* gate, int g_dt, int64_t shared_id,
+                      int32_t* ids, float* w, void* stream);
+
+/* The next token of each row of logits [rows, l_stride] (vocab of each row
+ * used) from a given random number u[row] in [0, 1):
+ *   weights w_i = exp((l_i - max l) / temperature); order: logit descending,
+ *   ties toward the lower column
+ *   top_k > 0: the first top_k entries of the order stay
+ *   top_p < 1: of those, an entry stays while the ones before it weigh less
+ *     than top_p of what top_k kept (the first always stays)
+ *   min_p > 0: of those, the ones with w_i >= min_p (the largest weighs 1)
+ *   out_idx[row] (int64): the first column at which the running sum of the
+ *     weights that stayed, in column order, exceeds u times their total
+ *   out_logprob[row] (fp32): ln(w_out_idx / total), the log of the probability
+ *     it was drawn with
+ * temperature 0: the first maximum, logprob 0.  Columns of -inf or NaN are
+ * absent; a row without any other gives out_idx -1 and a NaN logprob.  Each
+ * setting is common to all rows, or given by row on the device (its _rows
+ * pointer not NULL; there a temperature, top_k, top_p or min_p outside its
+ * range acts as the nearest one inside; NaN: greedy, no top_p, the maxima).
+ * Weights are 64-bit and sums whole numbers of 2^-42, so that a result does
+ * not depend on the split of a row.  vocab <= VQ2_SAMPLE_MAX_VOCAB, rows <=
+ * VQ2_SAMPLE_MAX_ROWS.  The workspace (256-byte aligned,
+ * vq2_sample_workspace bytes) may hold anything on entry; calls that share
+ * one must not overlap.  Beside the top-1 (vq2_argmax_rows); the reference
+ * decodes greedily (legion/engine.py:288) and has no counterpart. */
+#define VQ2_SAMPLE_MAX_VOCAB (1 << 21)
+#define VQ2_SAMPLE_MAX_ROWS 65535
+size_t vq2_sample_workspace(int64_t rows, int64_t vocab);
+int vq2_sample(const void* logits, int l_dt, int64_t l_stride, int64_t rows, int64_t vocab, const float* u,
+               float temperature, const float* temperature_rows, int64_t top_k, const int32_t* top_k_rows, float top_p,
+               const float* top_p_rows, float min_p, const float* min_p_rows, int64_t* out_idx, float* out_logprob,
+               void* workspace, size_t ws_bytes, void* stream);
+
 /* First-maximum index per row (torch.argmax semantics for NaN-free rows):
  *   out_idx[r] = argmax_c v[r, c]   (int64), out_val[r] = v[r, out_idx[r]] (fp32, may be NULL)
  * Replaces torch.argmax over logits (legion/engine.py:288, vq2/generate.py:65). */

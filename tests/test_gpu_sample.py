@@ -1,0 +1,220 @@
+"""vq2_sample on the GPU against the fp64 oracle: tokens exactly, log
+probabilities to the rounding of their fp32 result plus that of the total,
+a sum of V whole numbers of 2^-42, each off by at most half of one, over a
+largest weight of 1: |lp| 2^-24 + V 2^-43 + 2^-40 for the 64-bit logarithms."""
+import numpy as np
+import pytest
+import torch
+
+from compressai_amd import kernels as K, synth
+from compressai_amd.graph import DecodeStepGraph
+from oracle import selection as S
+
+pytestmark = pytest.mark.gpu
+DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _logits(seed, B, V, dtype="fp32", steep=None):
+    """A power law over tokens, steep or flat, with noise."""
+    g = synth.gen(seed)
+    s = torch.rand(B, 1, generator=g) * 1.8 + 0.7 if steep is None else steep
+    x = 16.0 - s * (torch.rand(B, V, generator=g) * V + 2.0).log() + 0.4 * torch.randn(B, V, generator=g)
+    return x.to(DT[dtype])
+
+
+def _check(got, logits, u, **kw):
+    idx, lp = (t.cpu().numpy() for t in got)
+    host = lambda v: v.cpu().double().numpy() if torch.is_tensor(v) else np.float32(v).astype(np.float64)
+    ref_idx, ref_lp = S.sample(logits.float().cpu().numpy(), host(u), **{k: host(v) for k, v in kw.items()})
+    assert idx.dtype == np.int64 and lp.dtype == np.float32
+    assert np.array_equal(idx, ref_idx)
+    live = ref_idx >= 0
+    assert np.isnan(lp[~live]).all()
+    tol = np.abs(ref_lp[live]) * 2.0 ** -24 + logits.shape[-1] * 2.0 ** -43 + 2.0 ** -40
+    off = np.abs(lp[live] - ref_lp[live]) > tol
+    assert not off.any(), (lp[live][off][:5], ref_lp[live][off][:5])
+
+
+SETTINGS = [
+    dict(), dict(temperature=0.7), dict(top_k=1), dict(top_k=50), dict(top_k=50, top_p=0.9, temperature=0.7),
+    dict(top_p=0.95), dict(top_p=0.3, temperature=1.4), dict(min_p=0.05), dict(top_p=0.9, min_p=0.02, temperature=1.1),
+    dict(top_k=700, top_p=0.99, min_p=0.001), dict(temperature=0.0), dict(top_p=0.0), dict(min_p=1.0),
+    dict(top_k=3000, temperature=2.0), dict(top_p=0.9999), dict(temperature=1e-6), dict(temperature=50.0, top_p=0.5),
+]
+
+
+@pytest.mark.parametrize("kw", SETTINGS, ids=str)
+@pytest.mark.parametrize("B,V,dtype", [
+    (1, 5000, "fp32"), (3, 1, "bf16"), (2, 7, "fp32"), (4, 4099, "bf16"), (9, 1000, "fp16"), (2, 32000, "bf16"), (5, 64, "fp32")])
+def test_settings(dev, B, V, dtype, kw):
+    x = _logits(8000 + V, B, V, dtype)
+    u = torch.rand(B, generator=synth.gen(8001 + B))
+    _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=50, top_p=0.9, temperature=0.7), dict(top_p=0.95), dict(top_p=0.9, min_p=0.01),
+                                dict(top_k=1000), dict(top_k=100000, top_p=0.8)], ids=str)
+@pytest.mark.parametrize("dtype,steep", [("fp32", 1.2), ("bf16", 1.2), ("fp32", 0.1), ("bf16", 0.1), ("fp16", 2.5)])
+def test_whole_vocabulary(dev, dtype, steep, kw):
+    """Peaked rows and rows nearly flat, whose kept sets are long."""
+    x = _logits(8100, 2, 151936, dtype, steep)
+    u = torch.tensor([0.137, 0.861])
+    _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+@pytest.mark.parametrize("B", [1, 2, 31, 257, 700])
+def test_row_counts_and_settings_by_row(dev, B):
+    V = 1500
+    g = synth.gen(8200 + B)
+    x = _logits(8201, B, V, "bf16")
+    x[:, V - 40:] = -float("inf")
+    pick = lambda lo, hi, off: torch.where(torch.rand(B, generator=g) < 0.4, torch.tensor(off), torch.rand(B, generator=g) * (hi - lo) + lo)
+    kw = dict(temperature=pick(0.4, 1.5, 0.0), top_k=pick(1, 200, 0.0).to(torch.int32), top_p=pick(0.3, 0.99, 1.0),
+              min_p=pick(0.01, 0.2, 0.0))
+    u = torch.rand(B, generator=g)
+    _check(K.vq_sample(x.to(dev), u.to(dev), **{k: v.to(dev) for k, v in kw.items()}), x, u, **kw)
+    # one setting by row beside common ones
+    _check(K.vq_sample(x.to(dev), u.to(dev), top_k=kw["top_k"].to(dev), top_p=0.9), x, u, top_k=kw["top_k"], top_p=0.9)
+
+
+def test_settings_outside_their_range_by_row(dev):
+    """On the device nothing can refuse them: each acts as the nearest inside."""
+    x = _logits(8250, 8, 900)
+    u = torch.rand(8, generator=synth.gen(8251))
+    nan = float("nan")
+    f = lambda *v: torch.tensor(v, device=dev)
+    got = K.vq_sample(x.to(dev), u.to(dev), temperature=f(-1.0, nan, 1, 1, 1, 1, 1, 1), top_p=f(1, 1, -2.0, nan, 7.0, 1, 1, 1),
+                      min_p=f(0, 0, 0, 0, 0, -1.0, 3.0, nan), top_k=torch.tensor([0, 0, 0, 0, 0, 0, 0, -5], dtype=torch.int32, device=dev))
+    _check(got, x, u, temperature=torch.tensor([0.0, 0, 1, 1, 1, 1, 1, 1]), top_p=torch.tensor([1.0, 1, 0, 1, 1, 1, 1, 1]),
+           min_p=torch.tensor([0.0, 0, 0, 0, 0, 0, 1, 1]))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=5), dict(top_k=1), dict(top_p=0.5), dict(top_k=700, top_p=0.25), dict(min_p=0.5),
+                                dict(top_p=0.999), dict(temperature=0.0)], ids=str)
+@pytest.mark.parametrize("V", [7, 1023, 20000, 70001])
+def test_ties(dev, V, kw):
+    """Rows of one value, of two, of zeros of both signs: the lower columns
+    stay, and the draw of an even row is floor(u n).  Weights are 1 or
+    exp(-1) (rounded the same by any summation of so few values)."""
+    x = torch.zeros(5, V)
+    x[1, ::3] = 1.0
+    x[2, 1::2] = -0.0
+    x[3] = torch.finfo(torch.float32).min
+    x[4, : V // 2] = -1.0
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.999])
+    _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+def test_absent_columns(dev):
+    inf, nan = float("inf"), float("nan")
+    V = 3001
+    x = _logits(8300, 12, V)
+    x[0] = -inf
+    x[1] = nan
+    x[2, :-1] = -inf
+    x[3, 1:] = nan
+    x[4, 100] = inf
+    x[5, ::7] = inf
+    x[6, ::2] = -inf
+    x[7, ::3] = nan
+    x[8, 5:] = torch.finfo(torch.float32).min
+    x[9, : V - 1] = -inf
+    x[10] = inf
+    x[11, 17] = nan
+    u = torch.rand(12, generator=synth.gen(8301))
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.8), dict(min_p=0.1, temperature=0.5), dict(temperature=0.0), dict(top_k=2000, top_p=0.9)):
+        _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+def test_borders_of_u(dev):
+    x = _logits(8400, 6, 2000)
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, -1.0, 2.0, 2.0 ** -60])
+    for kw in (dict(), dict(top_k=30), dict(top_p=0.9), dict(min_p=0.1)):
+        _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+def test_frequencies(dev):
+    """Evenly spaced numbers draw each kept token as often as its weight
+    says, to one draw."""
+    n, V = 4096, 50
+    x = _logits(8500, 1, V)
+    u = (torch.arange(n) + 0.5) / n
+    for kw in (dict(), dict(temperature=0.6), dict(top_k=9), dict(top_p=0.8)):
+        idx, lp = K.vq_sample(x.expand(n, V).contiguous().to(dev), u.to(dev), **kw)
+        kept = S.sample_row(x[0].numpy(), 0.5, **kw)[2]
+        share = np.bincount(idx.cpu().numpy(), minlength=V) / n
+        assert np.abs(share - kept / kept.sum()).max() <= 1.0 / n + 1e-12
+        assert np.allclose(np.exp(lp.cpu().numpy()), (kept / kept.sum())[idx.cpu().numpy()], rtol=1e-5)
+
+
+def test_strides(dev):
+    B, V = 5, 4001
+    for dtype in DT:
+        wide = _logits(8600, 2 * B, V + 300, dtype).to(dev)
+        u = torch.rand(B, generator=synth.gen(8601))
+        for view in (wide[::2, 3:3 + V], wide[:B, 1:V + 1], wide[:B, :V]):
+            for kw in (dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.9)):
+                _check(K.vq_sample(view, u.to(dev), **kw), view, u, **kw)
+    x = _logits(8602, 6, 100)
+    assert torch.equal(K.vq_sample(x.view(2, 3, 100).to(dev), torch.full((6,), 0.5, device=dev))[0],
+                       K.vq_sample(x.to(dev), torch.full((6,), 0.5, device=dev))[0])
+    idx, lp = K.vq_sample(wide[:0, :V], torch.zeros(0, device=dev))
+    assert idx.shape == (0,) and lp.shape == (0,)
+
+
+def test_refusals(dev):
+    x, u = torch.zeros(4, 64, device=dev), torch.zeros(4, device=dev)
+    f = lambda n, dt=torch.float32: torch.zeros(n, dtype=dt, device=dev)
+    for b in (dict(u=f(3)), dict(u=f(4, torch.float64)), dict(u=u.cpu()), dict(temperature=-1.0), dict(top_p=-0.1),
+              dict(min_p=1.1), dict(top_k=-2), dict(temperature=f(3)), dict(top_k=f(4)), dict(top_k=f(4, torch.int64)),
+              dict(top_p=f(8)[::2]), dict(min_p=f(4).cpu()), dict(logits=x.to(torch.int32)), dict(logits=x.t()),
+              dict(logits=x[:, ::2]), dict(logits=x[:1].expand(4, 64)), dict(logits=x[:, :0]),
+              dict(temperature=float("nan"))):
+        with pytest.raises(K.Vq2Error):
+            K.vq_sample(**dict(dict(logits=x, u=u), **b))
+
+
+@pytest.mark.parametrize("B,V", [(1, 151936), (40, 9000)])
+def test_streams_graphs_and_repeats(dev, B, V):
+    """Another stream, two streams at once, a captured graph replayed among
+    eager calls: the same results, bit for bit."""
+    xs = [_logits(8700 + i, B, V, "bf16").to(dev) for i in range(3)]
+    u = torch.rand(B, generator=synth.gen(8710)).to(dev)
+    for kw in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95)):
+        refs = [K.vq_sample(x, u, **kw) for x in xs]
+        torch.cuda.synchronize(dev)
+        sides = [torch.cuda.Stream(dev) for _ in xs]
+        got = []
+        for _ in range(4):
+            for x, s in zip(xs, sides):
+                with torch.cuda.stream(s):
+                    got.append(K.vq_sample(x, u, **kw))
+        torch.cuda.synchronize(dev)
+        for i, g in enumerate(got):
+            assert torch.equal(g[0], refs[i % 3][0]) and torch.equal(g[1], refs[i % 3][1])
+        steps = [DecodeStepGraph(lambda x: K.vq_sample(x, u, **kw), [xs[0]]) for _ in range(2)]
+        for i in (0, 1, 2, 2, 0, 1):
+            for step in steps:
+                g = step(xs[i])
+                torch.cuda.synchronize(dev)
+                assert torch.equal(g[0], refs[i][0]) and torch.equal(g[1], refs[i][1])
+            K.vq_sample(xs[1], u, **kw)
+
+
+def test_head_sample(dev):
+    """PackedLMHead.sample draws from the head's fp32 logits, at every batch
+    size the head has a path for."""
+    from compressai_amd.runtime import PackedLinear, PackedLMHead
+
+    rows, n = 4000, 512
+    m = synth.vq_matrix(8800, rows, n, bpw=2)
+    lin = PackedLinear((rows, n), (16,), "head", [m["idx0"]], m["scale"], {"16": synth.codebook(8801).to(dev)}, dev)
+    head = PackedLMHead(lin)
+    for B in (1, 2, 4, 9):
+        h = synth.activations(8810 + B, (B, n)).to(dev)
+        u = torch.rand(B, generator=synth.gen(8811)).to(dev)
+        logits = lin(h, out_dtype=torch.float32)
+        for kw in (dict(), dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=torch.full((B,), 0.5, device=dev), min_p=0.1)):
+            got = head.sample(h, u, **kw)
+            _check(got, logits, u, **kw)
+        assert torch.equal(head.sample(h, u, temperature=0.0)[0], logits.argmax(-1))
