@@ -20,8 +20,6 @@ DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 S2_NONE, S2_U8, S2_U16 = 0, 1, 2
 ID_I32, ID_I64 = 0, 1
 OK, ERR_ARG, ERR_HIP, ERR_UNSUPPORTED = 0, 1, 2, 3
-SCORING = {"softmax": 0, "sigmoid": 1}      # VQ2_SCORE_*
-GROUP_SCORE = {"max": 0, "top2": 1}         # VQ2_GROUP_*
 NOALLOC_SCRATCH_BYTES = 16 << 20  # VQ2_NOALLOC_SCRATCH_BYTES
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float

@@ -1466,6 +1466,10 @@ def _on_device(dev):
     return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+SCORING = {"softmax": 0, "sigmoid": 1}  # VQ2_SCORE_*
+GROUP_SCORE = {"max": 0, "top2": 1}     # VQ2_GROUP_*
+
+
 def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, topk_groups=None, group_score="max",
                      renormalise=True, scale=1.0, h=None, shared_gate=None, shared_id=-1, ids=None, w=None):
     """The router's further forms, per token: scores s = softmax(logits) or
@@ -1482,7 +1486,7 @@ def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, t
     form without bias and groups."""
     k, n_groups, shared_id = int(k), int(n_groups), int(shared_id)
     topk_groups = n_groups if topk_groups is None else int(topk_groups)
-    if scoring not in _lib.SCORING or group_score not in _lib.GROUP_SCORE:
+    if scoring not in SCORING or group_score not in GROUP_SCORE:
         raise Vq2Error(f"vq_router_select: scoring {scoring!r} (softmax/sigmoid), group_score {group_score!r} (max/top2)")
     dev = _dev(logits, bias, h, shared_gate, ids, w)
     lg, stride = _rows2d(logits, "logits")
@@ -1507,8 +1511,8 @@ def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, t
     if w is None:
         w = torch.empty((T, slots), dtype=torch.float32, device=dev)
     with _on_device(dev):
-        _lib.call("vq2_router_select", _p(lg), _dt(lg, "logits"), stride, T, E, k, _lib.SCORING[scoring], _p(bias),
-                  n_groups, topk_groups, _lib.GROUP_SCORE[group_score], 1 if renormalise else 0, float(scale),
+        _lib.call("vq2_router_select", _p(lg), _dt(lg, "logits"), stride, T, E, k, SCORING[scoring], _p(bias),
+                  n_groups, topk_groups, GROUP_SCORE[group_score], 1 if renormalise else 0, float(scale),
                   _p(h) if gate is not None else None, _dt(h, "h") if gate is not None else 0, hid, _p(gate),
                   _dt(gate, "gate") if gate is not None else 0, shared_id, _p(ids), _p(w), _stream(dev))
     return ids, w

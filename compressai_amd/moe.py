@@ -21,7 +21,10 @@ synchronisation.
 logits) and the shared expert with its sigmoid gate (transformers 5.15.0
 ``Qwen3_5MoeTopKRouter`` / ``Qwen3_5MoeSparseMoeBlock``), the shared expert
 living in the same pool at id ``n_routed``.  The whole layer is two
-launches and no host synchronisation.
+launches and no host synchronisation.  Checkpoints that route otherwise
+(sigmoid scores, a balance bias, expert groups, weights not renormalised or
+scaled, a shared expert without a gate) have the router as a launch of its own,
+``kernels.vq_router_select``, in front of the same experts.
 
 Intermediates are fp32 by default (the parity contract); ``act_dtype`` may
 select bf16 to follow the reference's cast points instead.
@@ -235,11 +238,16 @@ class MoELayer(nn.Module):
     """Router + top-k routed experts + gated shared expert, one pool.
 
     pools: gate_up_idx [E+1, 2I, H/8], down_idx [E+1, H, I/8] (int16), scales
-    [E+1, 2I] / [E+1, H]; id E is the shared expert.  shared_gate [H]."""
+    [E+1, 2I] / [E+1, H]; id E is the shared expert.  shared_gate [H], or None
+    for a shared expert of weight 1.  ``scoring``, ``router_bias`` (fp32 [E]),
+    ``n_groups``, ``topk_groups``, ``group_score``, ``renormalise`` and
+    ``routed_scale`` are those of ``kernels.vq_router_select``; their defaults
+    are the softmax router built into the experts' launches."""
 
     def __init__(self, gate_up_idx, gate_up_scale, down_idx, down_scale, cb16, shared_gate, top_k=8,
                  n_routed=None, rot_h=None, rot_i=None, act_dtype=torch.float32, out_dtype=torch.float32,
-                 sorted_layout=None):
+                 sorted_layout=None, *, scoring="softmax", router_bias=None, n_groups=1, topk_groups=None,
+                 group_score="max", renormalise=True, routed_scale=1.0):
         super().__init__()
         self.experts_mod = ResidentMoEExperts.from_pools(gate_up_idx, gate_up_scale, down_idx, down_scale, cb16,
                                                          rot_h, rot_i, act_dtype, out_dtype, sorted_layout)
@@ -247,11 +255,27 @@ class MoELayer(nn.Module):
         self.top_k = int(top_k)
         self.shared_gate = shared_gate
         self.out_dtype = out_dtype
+        # the router's form, where it is not the built-in one
+        self.router_form = None
+        form = dict(scoring=scoring, bias=router_bias, n_groups=int(n_groups), topk_groups=topk_groups,
+                    group_score=group_score, renormalise=bool(renormalise), scale=float(routed_scale))
+        if scoring not in K.SCORING or group_score not in K.GROUP_SCORE or n_groups < 1 or self.n_routed % n_groups:
+            raise K.Vq2Error(f"scoring {scoring!r}, group_score {group_score!r} or n_groups={n_groups} of {self.n_routed} "
+                             "routed experts invalid")
+        if (shared_gate is None or scoring != "softmax" or router_bias is not None or not renormalise
+                or routed_scale != 1.0 or form["topk_groups"] not in (None, form["n_groups"])):
+            self.router_form = form
         # down projection: one launch (SwiGLU + RHT in every workgroup) or a
         # separate SwiGLU + RHT launch followed by the grouped down + combine
         self.fused_down = True
 
     def route(self, h, router_logits):
+        """ids int32, w fp32 [T, top_k + 1] of the routed experts and the shared one."""
+        if self.router_form is not None:
+            if router_logits.shape[-1] != self.n_routed:
+                raise K.Vq2Error(f"router logits of {router_logits.shape[-1]} columns for {self.n_routed} routed experts")
+            return K.vq_router_select(router_logits, self.top_k, h=h, shared_gate=self.shared_gate,
+                                      shared_id=self.n_routed, **self.router_form)
         return K.vq_router_topk(router_logits, self.top_k, h, self.shared_gate, shared_id=self.n_routed)
 
     def wait_errors(self, clear=False) -> int:
@@ -266,6 +290,8 @@ class MoELayer(nn.Module):
         m = self.experts_mod
         h2 = h.reshape(-1, m.hidden_dim).contiguous()
         T = h2.shape[0]
+        if self.router_form is not None:
+            return m.experts(h2, *self.route(h2, router_logits.reshape(T, -1)))
         if m.sorted_gu is not None and self.n_routed <= 256:
             # (calls that the sorted path refuses are left to it, and those
             # whose top_k only its built-in router takes)
