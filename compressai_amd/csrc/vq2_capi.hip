@@ -763,6 +763,7 @@ int vq2_sample(const void* logits, int l_dt, int64_t l_stride, int64_t rows, int
     CHECK(logits && u && out_idx && out_logprob, "vq2_sample: NULL pointer argument");
     CHECK(dt_ok(l_dt), "vq2_sample: bad logits dtype");
     CHECK(l_stride >= vocab || rows == 1, "vq2_sample: l_stride < vocab");
+    CHECK((uintptr_t)logits % dt_size(l_dt) == 0, "vq2_sample: logits must be aligned to their elements");
     CHECK((uintptr_t)out_idx % 8 == 0, "vq2_sample: out_idx must be 8-byte aligned");
     const size_t need = sample_workspace_bytes(rows, vocab);
     CHECK(need == 0 || (workspace && ws_bytes >= need), "vq2_sample: workspace of %zu bytes needed, got %zu", need, ws_bytes);

@@ -96,7 +96,7 @@ def _sample(**kw):
     (dict(p=-0.1), "top_p"), (dict(p=float("nan")), "top_p"), (dict(m=-0.1), "min_p"), (dict(m=1.5), "min_p"),
     (dict(m=float("nan")), "min_p"), (dict(k=-1), "top_k"), (dict(logits=None), "NULL"), (dict(u=None), "NULL"),
     (dict(idx=None), "NULL"), (dict(lp=None), "NULL"), (dict(dt=7), "dtype"), (dict(rows=2, stride=63), "l_stride"),
-    (dict(idx=12), "aligned")])
+    (dict(idx=12), "aligned"), (dict(logits=18), "aligned"), (dict(logits=17, dt=2), "aligned")])
 def test_sample_refuses(kw, msg):
     assert msg in _err(_sample(**kw))
 
