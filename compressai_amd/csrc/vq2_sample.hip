@@ -9,12 +9,12 @@
 //
 // Which token comes out hangs on sums over a whole row, and two draws differ
 // by as little as one flat row's weight, 1e-5 of the total: in 32 bits one
-// draw in some hundred would be another.  So weights are computed in 64 bits
-// (exp2_f64), and where entries are put in order they are summed as whole
-// numbers of 2^-42 of the largest (a weight below 2^-43 counts as 0), whose
-// sum is the same in any order.
+// draw in some hundred would be another.  So weights are computed in 64 bits,
+// and where entries are put in order they are summed as whole numbers of 2^-42
+// of the largest (a weight below 2^-43 counts as 0), whose sum is the same in
+// any order.
 //
-// Three launches:
+// Launches:
 //   stats    A row is cut into units, each a contiguous piece that one wave
 //            reads; every unit's maximum and weight (for top-k, the maxima of
 //            finer groups).
@@ -24,18 +24,18 @@
 //                     that large);
 //              top-p  w < (1 - p) Z / V: all such entries together weigh less
 //                     than (1 - p) Z, which the last entries may be short of;
-//              min-p  w < min_p;  always: w < 2^-45.
+//              min-p  the least logit of w >= min_p;  always: w < 2^-45.
 //            The entries above, usually some hundred to some thousand of a
-//            row, are listed in column order.
+//            row, go to the row's list, in any order.
+//   refine   Only for rows with more entries than LDS holds (flat rows): their
+//            slices (the units of a workgroup) left histograms; each workgroup
+//            adds them up to the bin that the border lies in, and lists its
+//            slice's entries of that bin.
 //   finish   One workgroup a row, on the list in LDS: up to 256 entries are
-//            ranked directly, more are narrowed down by histograms; a running
-//            sum over the list finds the token.
-// A draw without a border (no top-k, top-p or min-p) needs no list: the unit
-// whose weights' running sum passes u Z is read again (two launches).  A row
-// with too many entries for LDS (flat rows) has a histogram of each slice of
-// 8 units beside the lists: the finish adds them up, fetches the entries of
-// the border's bin alone and, at the end, the slice that the draw falls into.
-// Long ties in that bin are the one case that is finished entry by entry.
+//            ranked directly, more are narrowed down by a histogram (in the
+//            order of logits for a border, of columns for the draw).
+// A draw without a border (no top-k, top-p or min-p) is stats and finish: the
+// unit whose weights' running sum passes u Z is read again.
 #include <float.h>
 
 #include "vq2_common.hpp"
@@ -47,21 +47,36 @@ namespace vq2 {
 namespace {
 
 constexpr int NT = 512;           // threads of a workgroup
+constexpr int BITS = 9;           // NT = 2^BITS
 constexpr int NW = NT / 64;       // its waves, one unit each: a slice
 constexpr int MAX_UNITS = 1024;   // units of a row
-constexpr int MAX_SLICES = MAX_UNITS / NW;
 constexpr int LIST = 3072;        // entries of the list in LDS
+constexpr int SHORT_LIST = 8192;  // entries of the slices without a histogram
 constexpr int DIRECT = 256;       // entries that are ranked directly
 constexpr int BINS = 256;         // of a slice's histogram
 constexpr double UNIT = 4398046511104.0;  // 2^42: a weight of 1
+static_assert(NT == 1 << BITS && NT == 2 * DIRECT && NT >= MAX_UNITS / 2, "a thread a range, two an entry, for two units");
+
+// What the collect launch leaves of a row.
+struct RowInfo {
+    double z;
+    float max, cut;
+};
+// What the refine launch leaves: the border's bin and the amount ahead of it.
+struct RefineInfo {
+    uint64_t before;
+    int64_t bin;  // -1: all entries stay
+};
+enum { CNT_LONG, CNT_SHORT, CNT_BIN, CNTS };  // a row's counters
 
 struct SampleArgs {
     const void* logits;
     int64_t stride;
     int vocab;
     int units, unit_blocks;  // blocks (16 bytes) of a unit, a multiple of 64
-    int fine;                // groups of a unit whose maxima are kept: 64 lanes, or 4 rows of 16
-    int cap;                 // entries a unit can list
+    int fine;                // groups of a unit whose maxima are kept: 64 lanes, or their quads or rows of 16
+    int list_cap, short_cap; // entries of the lists
+    bool refines;            // the refine launch takes place
     const float* u;
     const float* temperature_rows;
     const int32_t* top_k_rows;
@@ -75,13 +90,18 @@ struct SampleArgs {
     double* unit_sum;      // [rows][units], of exp((l - unit's max) / temperature)
     float* unit_max;       // [rows][units]
     float* fine_max;       // [rows][units][fine]
-    uint32_t* list_len;    // [rows][units]
-    uint64_t* bin_amount;  // [rows][slices][BINS], of slices with long lists
+    uint32_t* counters;    // [rows][CNTS]
+    RowInfo* info;         // [rows]
+    RefineInfo* refined;   // [rows]
+    uint32_t* slice_n;     // [rows][slices] entries
+    uint64_t* slice_mass;  // [rows][slices] of the bins ahead of the border's
+    uint64_t* bin_amount;  // [rows][slices][BINS], of slices of more than short_slice() entries
     uint32_t* bin_count;   // [rows][slices][BINS]
-    uint64_t* list;        // [rows][units][cap]
+    uint64_t* list;        // [rows][list_cap] entries of such slices; then of the border's bin
+    uint64_t* short_list;  // [rows][short_cap] entries of the others
     __device__ __forceinline__ int slices() const { return (units + NW - 1) / NW; }
-    // a slice lists entries only up to here without a histogram: all such together fit in LDS
-    __device__ __forceinline__ uint32_t short_slice() const { return (uint32_t)(LIST / slices()); }
+    // all slices of up to so many entries together fit the short list (and one a stage)
+    __device__ __forceinline__ uint32_t short_slice() const { return (uint32_t)min(short_cap / slices(), LIST); }
 };
 
 // One row's settings.
@@ -106,43 +126,29 @@ struct Setting {
     }
     __device__ __forceinline__ bool whole_sum() const { return k == 0 && (top_p_on || !min_p_on); }
     __device__ __forceinline__ bool listed() const { return k > 1 || (k == 0 && (top_p_on || min_p_on)); }
+    // one border is enough to say what stays (besides the collect's cut)
+    __device__ __forceinline__ bool one_border() const { return k == 0 || !top_p_on; }
 };
 
-// A row in blocks of 16 bytes (the last possibly shorter), from its first
-// column on: any alignment of the elements is taken, as the memory pipeline
-// takes it.
+// A row in blocks of 16 bytes from its first column on, whatever the
+// alignment of its elements; the last block may be short.
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
 template <int LT>
 struct Row {
     static constexpr int VEC = LT == VQ2_DT_F32 ? 4 : 8;
-    const void* p;  // its first column
-    int vocab, blocks;
+    const char* p;  // its first column
+    int vocab, blocks, full;
     __device__ __forceinline__ Row(const SampleArgs& a, int b)
-        : p((const char*)a.logits + b * a.stride * (16 / VEC)), vocab(a.vocab), blocks((a.vocab + VEC - 1) / VEC)
+        : p((const char*)a.logits + b * a.stride * (16 / VEC)), vocab(a.vocab), blocks((a.vocab + VEC - 1) / VEC),
+          full(a.vocab / VEC)
     {
-    }
-    __device__ __forceinline__ u32x4 raw(int block) const
-    {
-        if ((block + 1) * VEC <= vocab) return *(const u32x4_any*)((const char*)p + (int64_t)block * 16);
-        // the last, short block, element by element
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int c = block * VEC + i * (VEC / 4);
-            if constexpr (LT == VQ2_DT_F32) {
-                w[i] = c < vocab ? ((const uint32_t*)p)[c] : 0xFF800000u;
-            } else {
-                constexpr uint32_t ABSENT = LT == VQ2_DT_F16 ? 0xFC00u : 0xFF80u;  // -inf
-                w[i] = c < vocab ? ((const uint16_t*)p)[c] : ABSENT;
-                w[i] |= (c + 1 < vocab ? ((const uint16_t*)p)[c + 1] : ABSENT) << 16;
-            }
-        }
-        return w;
     }
     // An infinite logit becomes the largest finite one (no difference of
     // infinities); NaN stays.
     static __device__ __forceinline__ float finite(float v) { return v == INFINITY ? FLT_MAX : v; }
+    __device__ __forceinline__ float at(int column) const { return finite(ld_t<LT>(p, column)); }
+    __device__ __forceinline__ u32x4 raw(int block) const { return *(const u32x4_any*)(p + (int64_t)block * 16); }
     static __device__ __forceinline__ void values(u32x4 w, float (&v)[VEC])
     {
 #pragma unroll
@@ -156,20 +162,29 @@ struct Row {
             v[i] = finite(v[i]);
         }
     }
-    __device__ __forceinline__ void load(int block, float (&v)[VEC]) const { values(raw(block), v); }
-    __device__ __forceinline__ float at(int column) const { return finite(ld_t<LT>(p, column)); }
     // f(block, values) for the blocks from `from` on in steps of `step`, the
-    // next block's load in flight meanwhile
+    // next block's load in flight meanwhile.  A short last block, padded with
+    // -inf, comes by itself: its loads in the loop's path would keep every
+    // load from being in flight.
     template <class F>
     __device__ __forceinline__ void stream(int from, int end, int step, F f) const
     {
-        if (from >= end) return;
-        u32x4 next = raw(from);
-        for (int i = from; i < end; i += step) {
-            const u32x4 w = next;
-            if (i + step < end) next = raw(i + step);
+        const int last = min(end, full);
+        int i = from;
+        if (i < last) {
+            u32x4 next = raw(i);
+            for (; i < last; i += step) {
+                const u32x4 w = next;
+                if (i + step < last) next = raw(i + step);
+                float v[VEC];
+                values(w, v);
+                f(i, v);
+            }
+        }
+        if (i == full && i < end) {
             float v[VEC];
-            values(w, v);
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[j] = i * VEC + j < vocab ? at(i * VEC + j) : -INFINITY;
             f(i, v);
         }
     }
@@ -200,43 +215,75 @@ struct Weigher {
     }
 };
 
-// The bin of a logit, 0 the highest: linear between `max` and `max` - 1 / inv
-// * BINS.  Rounded arithmetic, but monotonic: a higher logit is never in a
-// lower bin.
-__device__ __forceinline__ int bin_of(float l, float max, float inv)
-{
-    return (int)fminf((max - l) * inv, (float)(BINS - 1));
-}
-__device__ __forceinline__ float bins_inv(float max, float cut)
-{
-    const float width = max - cut;
-    return width > 0.0f && width < INFINITY ? (float)BINS / width : 0.0f;
-}
-
-// ------------------------------------------------- sums over the workgroup
-__device__ __forceinline__ double wave_sum_f64(double v)
-{
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    return v;
-}
-
-struct Scratch {
-    uint64_t wave64[NW + 2];
-    double wave_d[NW];
+// The bin of n of a logit, 0 the highest: linear between `max` and `cut`.
+// Rounded arithmetic, but monotonic: a higher logit is never in a lower bin.
+struct Binner {
+    float max, inv;
+    int n;
+    __device__ __forceinline__ Binner(float max_, float cut, int n_) : max(max_), n(n_)
+    {
+        const float width = max - cut;
+        inv = width > 0.0f && width < INFINITY ? (float)n / width : 0.0f;
+    }
+    __device__ __forceinline__ int operator()(float l) const { return (int)fminf((max - l) * inv, (float)(n - 1)); }
 };
 
+// ------------------------------------------------- sums over the workgroup
+// Lanes' values shifted within the wave, 0 where there is none: the steps of a
+// running sum (within a row of 16 by 1, 2, 4, 8, then row 0's and 2's last
+// lane to the next row, then lane 31 to the upper half).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v)
+{
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)(uint32_t)hi << 32 | (uint32_t)lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_u64(double v)
+{
+    return __builtin_bit_cast(double, dpp_u64<CTRL, ROWS>(__builtin_bit_cast(uint64_t, v)));
+}
 template <class T>
 __device__ __forceinline__ T wave_scan(T v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(v, off);
-        if (lane >= off) v += o;
-    }
+    v += dpp_u64<0x111, 0xF>(v);
+    v += dpp_u64<0x112, 0xF>(v);
+    v += dpp_u64<0x114, 0xF>(v);
+    v += dpp_u64<0x118, 0xF>(v);
+    v += dpp_u64<0x142, 0xA>(v);
+    v += dpp_u64<0x143, 0xC>(v);
     return v;
 }
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane)
+{
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ double wave_sum_f64(double v)
+{
+    return __builtin_bit_cast(double, read_lane(__builtin_bit_cast(uint64_t, wave_scan(v)), 63));
+}
+// (least of the wave, in lane 63)
+__device__ __forceinline__ uint64_t wave_min_u64(uint64_t v)
+{
+    v = ~v;  // (the shifts fill with 0, the least complement)
+    auto up = [&](uint64_t o) { v = o > v ? o : v; };
+    up(dpp_u64<0x111, 0xF>(v));
+    up(dpp_u64<0x112, 0xF>(v));
+    up(dpp_u64<0x114, 0xF>(v));
+    up(dpp_u64<0x118, 0xF>(v));
+    up(dpp_u64<0x142, 0xA>(v));
+    up(dpp_u64<0x143, 0xC>(v));
+    return ~v;
+}
+
+struct Scratch {
+    uint64_t wave64[NW];
+    uint64_t found[2];
+    double wave_d[NW];
+};
 
 // Inclusive running sum over the workgroup; total in every thread.
 __device__ __forceinline__ uint64_t block_scan(Scratch& sh, uint64_t v, uint64_t& total)
@@ -272,13 +319,9 @@ __device__ __forceinline__ float block_max(Scratch& sh, float v)
 
 __device__ __forceinline__ uint64_t block_min(Scratch& sh, uint64_t v)
 {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t o = __shfl_xor(v, off);
-        v = o < v ? o : v;
-    }
+    v = wave_min_u64(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wave64[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) sh.wave64[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t m = sh.wave64[0];
 #pragma unroll
@@ -286,8 +329,24 @@ __device__ __forceinline__ uint64_t block_min(Scratch& sh, uint64_t v)
     return m;
 }
 
-// What the units say of a row: its maximum and, of a sum over the whole row, Z
-// and each thread's running sum, thread t holding units 2 t and 2 t + 1.
+// The thread at which the running sum of `mine` over the workgroup first
+// reaches `limit` (>= 1), and the sum before it; -1 if it does not.
+__device__ __forceinline__ int block_locate(Scratch& sh, uint64_t mine, uint64_t limit, uint64_t& before)
+{
+    uint64_t all;
+    const uint64_t run = block_scan(sh, mine, all);
+    if (all < limit) return -1;
+    if (run >= limit && run - mine < limit) {
+        sh.found[0] = threadIdx.x;
+        sh.found[1] = run - mine;
+    }
+    __syncthreads();
+    before = sh.found[1];
+    return (int)(sh.found[0] & (NT - 1));
+}
+
+// What the units say of a row: its maximum and, of a sum over the whole row,
+// Z; thread t holds units 2 t and 2 t + 1.
 struct Units {
     float um[2];
     float max;
@@ -321,14 +380,40 @@ __device__ __forceinline__ Units read_units(Scratch& sh, const SampleArgs& a, co
 }
 
 // ------------------------------------------------------------------- stats
+// The sum over a whole row is an exponential of 64 bits an entry, and those,
+// not memory, bound this launch.  2^(j / 1024) comes from a table in LDS, which
+// leaves f in [-2^-11, 2^-11]: 2^f = 1 + f (ln 2 + f ln^2 2 / 2), off by 7e-12
+// at its ends (odd in f, so that it averages out of a sum), in 11 operations
+// of 64 bits and a lookup instead of 17.
+constexpr int TABLE = 1024;
+__device__ __forceinline__ double exp2_table(const double* table, double y)
+{
+    constexpr double MAGIC = 6755399441055744.0 / TABLE;  // rounds to a whole number of 1 / TABLE
+    y = fmax(y, -1000.0);
+    const double t = y + MAGIC;
+    const double f = y - (t - MAGIC);
+    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const double r = table[n & (TABLE - 1)];
+    const double g = fma(0.2402265069591007, f, 0.6931471805599453) * f;
+    const uint64_t p = __builtin_bit_cast(uint64_t, fma(r, g, r));
+    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(n >> 10) << 20);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)p);
+}
+
 template <int LT>
 __global__ void __launch_bounds__(NT) sample_stats_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
-    const int b = blockIdx.y, lane = threadIdx.x & 63;
-    const int unit = blockIdx.x * NW + (threadIdx.x >> 6);
-    if (unit >= a.units) return;
+    __shared__ double table[TABLE];
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    if (blockIdx.x == 0 && tid < CNTS) a.counters[b * CNTS + tid] = 0;
     const Setting s(a, b);
+    if (s.whole_sum()) {
+        for (int i = tid; i < TABLE; i += NT) table[i] = exp2_f64_in((double)i / TABLE);
+        __syncthreads();
+    }
+    const int unit = blockIdx.x * NW + (tid >> 6);
+    if (unit >= a.units) return;
     const Row<LT> row(a, b);
     const int from = unit * a.unit_blocks + lane, end = min(row.blocks, (unit + 1) * a.unit_blocks);
     float m = -INFINITY;
@@ -347,7 +432,7 @@ __global__ void __launch_bounds__(NT) sample_stats_kernel(SampleArgs a)
                 ref = top;
             }
 #pragma unroll
-            for (int j = 0; j < VEC; j++) sum += exp2_f64(((double)v[j] - (double)ref) * s.c);
+            for (int j = 0; j < VEC; j++) sum += exp2_table(table, ((double)v[j] - (double)ref) * s.c);
         });
         const float um = wave_max_all(m);
         sum = wave_sum_f64(sum * exp2_f64(((double)ref - (double)um) * s.c));
@@ -359,15 +444,17 @@ __global__ void __launch_bounds__(NT) sample_stats_kernel(SampleArgs a)
     }
     const int64_t at = (int64_t)b * a.units + unit;
     if (s.k > 1) {
-        if (a.fine == 4) {
-            float g = fmaxf(m, dpp_xor1(m));
+        float g = m;
+        if (a.fine < 64) {
+            g = fmaxf(g, dpp_xor1(g));
             g = fmaxf(g, dpp_xor2(g));
+        }
+        if (a.fine == 4) {
             g = fmaxf(g, dpp_half_mirror(g));
             g = fmaxf(g, dpp_row_mirror(g));
-            if ((lane & 15) == 0) a.fine_max[at * 4 + lane / 16] = g;
-        } else {
-            a.fine_max[at * 64 + lane] = m;
         }
+        const int each = 64 / a.fine;
+        if (lane % each == 0) a.fine_max[at * a.fine + lane / each] = g;
     }
     m = wave_max_all(m);
     if (lane == 0) {
@@ -377,11 +464,64 @@ __global__ void __launch_bounds__(NT) sample_stats_kernel(SampleArgs a)
 }
 
 // ----------------------------------------------------------------- collect
+// Entries of a workgroup on their way to a list.
+struct Stage {
+    uint64_t entry[LIST];
+    uint32_t n, base;
+};
+
+// Puts the `in` entries of this lane's block into the stage (those past its
+// end are counted only).
+template <int VEC>
+__device__ __forceinline__ void stage_block(Stage& st, uint32_t in, int block, const float (&v)[VEC])
+{
+    if (in == 0) return;
+    uint32_t at = atomicAdd(&st.n, (uint32_t)__popc(in));
+#pragma unroll
+    for (int j = 0; j < VEC; j++)
+        if (in >> j & 1) {
+            if (at < LIST) st.entry[at] = order_key(v[j], block * VEC + j);
+            at++;
+        }
+}
+
+// Appends the stage to a list of `cap` entries; the list's counter counts
+// entries that do not fit as well.
+__device__ __forceinline__ void flush_stage(Stage& st, uint32_t* counter, uint64_t* list, uint32_t cap)
+{
+    __syncthreads();
+    const uint32_t n = st.n;
+    if (n == 0) return;
+    if (threadIdx.x == 0) st.base = atomicAdd(counter, n);
+    __syncthreads();
+    const uint32_t base = st.base;
+    if (n > LIST || base > cap || n > cap - base) return;
+    for (uint32_t i = threadIdx.x; i < n; i += NT) list[base + i] = st.entry[i];
+}
+
+// The smallest logit of weight >= min_p, by a search of 64 steps at once.
+__device__ __forceinline__ float min_p_border(const Setting& s, const Weigher& weigh)
+{
+    uint32_t lo = 0x00800000u, hi = (uint32_t)(order_key(weigh.max, 0) >> 32);  // (-FLT_MAX's; weight 1 >= min_p)
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / 64 + 1, probe = lo + min((threadIdx.x & 63) * step, hi - lo);
+        const uint64_t yes = __ballot(weigh(key_logit((uint64_t)probe << 32)) >= s.min_p);
+        if (yes == 0) {  // (the last probe is short of hi then)
+            lo += 63 * step + 1;
+        } else {
+            const uint32_t f = (uint32_t)__ffsll((unsigned long long)yes) - 1, top = hi - lo;
+            hi = lo + min(f * step, top);
+            if (f > 0) lo += (f - 1) * step + 1;
+        }
+    }
+    return key_logit((uint64_t)hi << 32);
+}
+
 struct CollectShared {
     Scratch scratch;
+    Stage stage;
     uint64_t amount[BINS];
     uint32_t count[NT];
-    uint32_t slice_n;
 };
 
 // The logit from which on a row's entries may stay: rounded down, by more than
@@ -392,23 +532,21 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
     const double m = (double)un.max;
     double w = 2.8421709430404007e-14;  // 2^-45
     if (s.k == 0 && s.top_p_on) w = fmax(w, (1.0 - s.p) * 0.999 * un.z / (double)a.vocab);
-    if (s.min_p_on && !(s.k > 0 && s.top_p_on)) w = fmax(w, s.min_p * 0.999);
     double low = m + log2(w) / s.c;
+    low -= (fabs(m) + fabs(low)) * 1e-6;
+    float cut = (float)fmax(low, (double)-FLT_MAX);
     if (s.k > 0) {
-        // the lower end of the bin that the k-th largest maximum falls into;
+        // the lower end of the range that the k-th largest maximum falls into;
         // more groups than k are needed for it to say something
         const bool coarse = s.k * 2 <= (uint32_t)a.units;
         const int groups = coarse ? a.units : a.units * a.fine;
         if (s.k * 5 <= (uint32_t)groups * 4) {
             const int64_t u0 = (int64_t)b * a.units;
             const float* const g = coarse ? a.unit_max + u0 : a.fine_max + u0 * a.fine;
-            const float floor = (float)fmax(low, (double)-FLT_MAX);
             float least = INFINITY;
-            for (int i = tid; i < groups; i += NT) least = fminf(least, fmaxf(g[i], floor));
+            for (int i = tid; i < groups; i += NT) least = fminf(least, fmaxf(g[i], cut));
             least = -block_max(sh.scratch, -least);
-            const float width = un.max - least;
-            const float inv = width > 0.0f && width < INFINITY ? (float)NT / width : 0.0f;
-            auto bin = [&](float l) { return (int)fminf((un.max - l) * inv, (float)(NT - 1)); };
+            const Binner bin(un.max, least, NT);
             sh.count[tid] = 0;
             __syncthreads();
             for (int i = tid; i < groups; i += NT) {
@@ -416,26 +554,14 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
                 if (l >= least) atomicAdd(&sh.count[bin(l)], 1u);
             }
             __syncthreads();
-            uint64_t all;
-            const uint64_t mine = sh.count[tid], run = block_scan(sh.scratch, mine, all);
-            if (tid == 0) sh.scratch.wave64[NW] = NT;
-            __syncthreads();
-            if (run >= s.k && run - mine < s.k) sh.scratch.wave64[NW] = (uint64_t)tid;
-            __syncthreads();
-            const int r = (int)sh.scratch.wave64[NW];
-            // the least maximum of the bins up to that one: k are at least as large
-            float kth = INFINITY;
-            if (r < NT)
-                for (int i = tid; i < groups; i += NT) {
-                    const float l = g[i];
-                    if (l >= least && bin(l) <= r) kth = fminf(kth, l);
-                }
-            kth = -block_max(sh.scratch, -kth);
-            if (r < NT) return fmaxf(kth, floor - (fabsf(floor) + fabsf(un.max)) * 1e-6f);
+            uint64_t before;
+            const int r = block_locate(sh.scratch, sh.count[tid], s.k, before);
+            // (the range's end as the binner rounds it, and a range to spare)
+            if (r >= 0 && bin.inv > 0.0f) cut = fmaxf(cut, un.max - (float)(r + 2) / bin.inv);
         }
     }
-    const double slack = (fabs(m) + fabs(low)) * 1e-6;
-    return (float)fmax(low - slack, (double)-FLT_MAX);
+    if (s.min_p_on && !(s.k > 0 && s.top_p_on)) cut = fmaxf(cut, min_p_border(s, Weigher{un.max, s.c}));
+    return cut;
 }
 
 template <int LT>
@@ -449,190 +575,221 @@ __global__ void __launch_bounds__(NT) sample_collect_kernel(SampleArgs a)
     const Units un = read_units(sh.scratch, a, s, b);
     if (un.max == -INFINITY) return;
     const float cut = lowest_kept(sh, a, s, un, b);
+    if (blockIdx.x == 0 && tid == 0) a.info[b] = RowInfo{un.z, un.max, cut};
     const Row<LT> row(a, b);
-    const int64_t units0 = (int64_t)b * a.units;
     const int unit = blockIdx.x * NW + (tid >> 6);
     const int from = unit * a.unit_blocks, end = min(row.blocks, from + a.unit_blocks);
-    if (tid == 0) sh.slice_n = 0;
+    if (tid == 0) sh.stage.n = 0;
     __syncthreads();
-    if (unit < a.units) {
-        uint64_t* const list = a.list + (units0 + unit) * a.cap;
-        int n = 0;
-        // (lanes past the end keep step, without entries)
-        const int rounds = max(0, (end - from + 63) / 64);
-        u32x4 next{};
-        if (from + lane < end) next = row.raw(from + lane);
-        for (int r = 0; r < rounds; r++) {
-            const int i = from + r * 64 + lane;
-            const u32x4 w = next;
-            if (i + 64 < end) next = row.raw(i + 64);
-            float v[VEC];
-            Row<LT>::values(w, v);
-            uint32_t in = 0;
+    row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
+        uint32_t in = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; j++) in |= (uint32_t)(v[j] >= cut) << j;
-            if (i >= end) in = 0;
-            if (__ballot(in != 0) == 0) continue;
-            const int mine = __popc(in), upto = wave_scan(mine);
-            int at = n + upto - mine;
-            if (in) {
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if (in >> j & 1) {
-                        if (at < a.cap) list[at] = order_key(v[j], i * VEC + j);
-                        at++;
-                    }
-            }
-            n += __shfl(upto, 63);
-        }
-        if (lane == 0) {
-            a.list_len[units0 + unit] = (uint32_t)n;
-            atomicAdd(&sh.slice_n, (uint32_t)n);
-        }
-    }
+        for (int j = 0; j < VEC; j++) in |= (uint32_t)(v[j] >= cut) << j;
+        stage_block<VEC>(sh.stage, in, i, v);
+    });
     __syncthreads();
-    if (sh.slice_n <= a.short_slice()) return;
-    // a histogram of the slice's entries beside their lists
+    const uint32_t n = sh.stage.n;
+    const bool is_long = n > a.short_slice();
+    const int64_t slice = (int64_t)b * gridDim.x + blockIdx.x;
+    if (tid == 0) a.slice_n[slice] = n;
+    if (is_long)
+        flush_stage(sh.stage, a.counters + b * CNTS + CNT_LONG, a.list + (int64_t)b * a.list_cap, a.list_cap);
+    else
+        flush_stage(sh.stage, a.counters + b * CNTS + CNT_SHORT, a.short_list + (int64_t)b * a.short_cap, a.short_cap);
+    if (!is_long) return;
+    // a histogram of the slice's entries, in case the row has too many
     if (tid < BINS) {
         sh.amount[tid] = 0;
         sh.count[tid] = 0;
     }
     __syncthreads();
     const Weigher weigh{un.max, s.c};
-    const float inv = bins_inv(un.max, cut);
-    if (unit < a.units)
+    const Binner bin(un.max, cut, BINS);
+    auto add = [&](float l) {
+        const int r = bin(l);
+        atomicAdd((unsigned long long*)&sh.amount[r], (unsigned long long)fixed(weigh(l)));
+        atomicAdd(&sh.count[r], 1u);
+    };
+    if (n <= LIST) {
+        for (uint32_t i = tid; i < n; i += NT) add(key_logit(sh.stage.entry[i]));
+    } else {
         row.stream(from + lane, end, 64, [&](int, const float (&v)[VEC]) {
 #pragma unroll
             for (int j = 0; j < VEC; j++)
-                if (v[j] >= cut) {
-                    const int r = bin_of(v[j], un.max, inv);
-                    atomicAdd((unsigned long long*)&sh.amount[r], (unsigned long long)fixed(weigh(v[j])));
-                    atomicAdd(&sh.count[r], 1u);
-                }
+                if (v[j] >= cut) add(v[j]);
         });
+    }
     __syncthreads();
     if (tid < BINS) {
-        const int64_t at = ((int64_t)b * gridDim.x + blockIdx.x) * BINS + tid;
-        a.bin_amount[at] = sh.amount[tid];
-        a.bin_count[at] = sh.count[tid];
+        a.bin_amount[slice * BINS + tid] = sh.amount[tid];
+        a.bin_count[slice * BINS + tid] = sh.count[tid];
     }
+}
+
+// ------------------------------------------------------------------ refine
+struct RefineShared {
+    Scratch scratch;
+    Stage stage;
+    uint64_t amount[NT];
+    uint32_t count[NT];
+};
+
+template <int LT>
+__global__ void __launch_bounds__(NT) sample_refine_kernel(SampleArgs a)
+{
+    constexpr int VEC = Row<LT>::VEC;
+    __shared__ RefineShared sh;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, slices = gridDim.x;
+    const Setting s(a, b);
+    if (!s.listed() || !s.one_border()) return;
+    const uint32_t n_long = a.counters[b * CNTS + CNT_LONG], n_short = a.counters[b * CNTS + CNT_SHORT];
+    if (n_long + n_short <= LIST) return;
+    const RowInfo info = a.info[b];
+    const Weigher weigh{info.max, s.c};
+    const Binner bin(info.max, info.cut, BINS);
+    // the row's histogram: two threads a bin, then the short slices' entries
+    const int64_t slice0 = (int64_t)b * slices;
+    sh.amount[tid] = 0;
+    sh.count[tid] = 0;
+    if (tid == 0) sh.stage.n = 0;
+    __syncthreads();
+    {
+        uint64_t am = 0;
+        uint32_t ct = 0;
+#pragma unroll 4
+        for (int g = tid / BINS; g < slices; g += NT / BINS)
+            if (a.slice_n[slice0 + g] > a.short_slice()) {
+                am += a.bin_amount[(slice0 + g) * BINS + tid % BINS];
+                ct += a.bin_count[(slice0 + g) * BINS + tid % BINS];
+            }
+        atomicAdd((unsigned long long*)&sh.amount[tid % BINS], (unsigned long long)am);
+        atomicAdd(&sh.count[tid % BINS], ct);
+        for (uint32_t i = tid; i < min(n_short, (uint32_t)a.short_cap); i += NT) {
+            const float l = key_logit(a.short_list[(int64_t)b * a.short_cap + i]);
+            atomicAdd((unsigned long long*)&sh.amount[bin(l)], (unsigned long long)fixed(weigh(l)));
+            atomicAdd(&sh.count[bin(l)], 1u);
+        }
+    }
+    __syncthreads();
+    const double p_limit = ceil(s.p * info.z * UNIT);
+    const uint64_t limit = s.k > 0 ? (uint64_t)s.k : !s.top_p_on ? ~0ull : p_limit > 1.0 ? (uint64_t)p_limit : 1;
+    const uint64_t amount = tid < BINS ? (s.k > 0 ? (uint64_t)sh.count[tid] : sh.amount[tid]) : 0;
+    uint64_t before = 0;
+    const int r = block_locate(sh.scratch, amount, limit, before);
+    if (blockIdx.x == 0 && tid == 0) a.refined[b] = RefineInfo{before, r};
+    if (a.slice_n[slice0 + blockIdx.x] <= a.short_slice()) return;
+    // this slice's weight ahead of the bin, and its entries of the bin
+    uint64_t ahead = tid < BINS && (r < 0 || tid < r) ? a.bin_amount[(slice0 + blockIdx.x) * BINS + tid] : 0, all;
+    block_scan(sh.scratch, ahead, all);
+    if (tid == 0) a.slice_mass[slice0 + blockIdx.x] = all;
+    if (r < 0) return;
+    const Row<LT> row(a, b);
+    const int from = (blockIdx.x * NW + (tid >> 6)) * a.unit_blocks, end = min(row.blocks, from + a.unit_blocks);
+    row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) in |= (uint32_t)(v[j] >= info.cut && bin(v[j]) == r) << j;
+        stage_block<VEC>(sh.stage, in, i, v);
+    });
+    flush_stage(sh.stage, a.counters + b * CNTS + CNT_BIN, a.list + (int64_t)b * a.list_cap, a.list_cap);
 }
 
 // ------------------------------------------------------------------ finish
 struct FinishShared {
     Scratch scratch;
-    CollectShared cut;        // (for lowest_kept)
-    uint64_t list[LIST];      // the row's entries in column order
-    uint64_t amount[NT];      // a histogram's sums; weights of ranked entries
-    uint64_t small[NT];       // entries that are ranked
-    uint32_t count[NT];
-    uint32_t first[MAX_UNITS + 1];  // entries of the list before a unit's
-    uint64_t slice_mass[MAX_SLICES];
-    uint32_t small_n;
+    uint64_t list[LIST];  // entries
+    uint64_t mass[LIST];  // and their weights
+    uint64_t amount[NT];  // a histogram's sums, or entries that are ranked: amounts,
+    uint64_t order[NT];   // places
+    uint32_t index[NT];   // and which they are
+    uint32_t count[NT];   // a histogram's entries
+    uint64_t slice[MAX_UNITS / NW];
+    uint32_t n;
 };
 
-// The entries that a border is sought among: a list in LDS or, for a row whose
-// ties fit none, every entry of the row from `cut` on.
-template <int LT>
-struct Source {
-    const Row<LT>& row;
-    const uint64_t* list;  // null: the row
-    int n;
-    float cut;
-    template <class F>
-    __device__ __forceinline__ void each(F f) const
-    {
-        if (list) {
-            for (int i = threadIdx.x; i < n; i += NT) f(list[i]);
-        } else {
-            row.stream(threadIdx.x, row.blocks, NT, [&](int i, const float (&v)[Row<LT>::VEC]) {
-                for (int j = 0; j < Row<LT>::VEC; j++)
-                    if (v[j] >= cut) f(order_key(v[j], i * Row<LT>::VEC + j));
-            });
-        }
-    }
-};
-
-// The border of the entries in [lo, ~0]: the key of the last one that stays
-// when an entry stays while the amounts before it are below `limit` (>= 1), of
-// which `before` are ahead of them all.  Each round is a histogram of the
-// keys over NT equal ranges, whose running sum finds the range that the limit
-// falls into; keys differ, so ranges end up with few entries, which are
-// ranked directly.  lo if all stay.
-template <int LT, class F>
-__device__ uint64_t find_border(FinishShared& sh, const Source<LT>& src, uint64_t lo, uint64_t limit, uint64_t before,
-                                F amount)
+// Of entries 0 ... n - 1 with different places order(i) (ascending), the one
+// at which the running sum of amount(i), in their order, first reaches `limit`
+// (>= 1); -1 if it does not.  A histogram over ranges of the order, bin(i) <
+// NT, finds the range; while that holds more than DIRECT entries, it is cut
+// into NT equal ranges again (places differ, so that ends).  The entries left
+// are compared with each other.
+template <class Order, class Amount, class Bin>
+__device__ __forceinline__ int locate_entry(FinishShared& sh, int n, uint64_t limit, Order order, Amount amount, Bin bin)
 {
     const int tid = threadIdx.x;
-    uint64_t hi = 0;
-    for (int round = 0;; round++) {
-        // the range that the entries span
-        uint64_t least = ~0ull, most = ~0ull;  // (most: the largest key's complement)
-        src.each([&](uint64_t key) {
-            if (key >= lo && (round == 0 || key <= hi)) {
-                least = key < least ? key : least;
-                most = ~key < most ? ~key : most;
-            }
-        });
-        least = block_min(sh.scratch, least);
-        most = ~block_min(sh.scratch, most);
-        if (least == ~0ull) return lo;  // no entry
-        lo = least;
-        hi = most;
-        const uint64_t span = hi - lo;
-        constexpr int BITS = 9;
-        static_assert(NT == 1 << BITS, "one range a thread");
-        const int shift = span < NT ? 0 : 64 - __clzll(span) - BITS;
+    uint64_t lo = 0, hi = ~0ull, before = 0;
+    int shift = -1;  // (the first round: bin)
+    for (;;) {
+        auto range = [&](int i) -> int {
+            if (shift < 0) return bin(i);
+            const uint64_t o = order(i);
+            return o < lo || o > hi ? -1 : (int)((o - lo) >> shift);
+        };
         __syncthreads();
         sh.amount[tid] = 0;
         sh.count[tid] = 0;
+        if (tid == 0) sh.n = 0;
         __syncthreads();
-        src.each([&](uint64_t key) {
-            if (key >= lo && key <= hi) {
-                const int r = (int)((hi - key) >> shift);
-                atomicAdd((unsigned long long*)&sh.amount[r], (unsigned long long)amount(key));
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t x = amount(i);
+            const int r = range(i);
+            if (x && r >= 0) {
+                atomicAdd((unsigned long long*)&sh.amount[r], (unsigned long long)x);
                 atomicAdd(&sh.count[r], 1u);
             }
-        });
-        __syncthreads();
-        const uint64_t mine = sh.amount[tid];
-        uint64_t all;
-        const uint64_t run = before + block_scan(sh.scratch, mine, all);
-        if (before + all < limit) return lo;
-        if (run >= limit && run - mine < limit) {
-            sh.scratch.wave64[NW] = (uint64_t)tid;
-            sh.scratch.wave64[NW + 1] = run - mine;
         }
         __syncthreads();
-        const int r = (int)(sh.scratch.wave64[NW] & (NT - 1));
-        before = sh.scratch.wave64[NW + 1];
-        const uint32_t m = min(sh.count[r], (uint32_t)NT);
-        hi -= (uint64_t)r << shift;
-        const uint64_t width = (1ull << shift) - 1;
-        lo = hi - lo < width ? lo : hi - width;
-        if (m > DIRECT && shift > 0) continue;
-        if (tid == 0) sh.small_n = 0;
+        uint64_t ahead = 0;
+        const int at = block_locate(sh.scratch, sh.amount[tid], limit - before, ahead);
+        if (at < 0) return -1;
+        before += ahead;
+        const uint32_t m = sh.count[at];
         __syncthreads();
-        src.each([&](uint64_t key) {
-            if (key >= lo && key <= hi) {
-                const uint32_t at = atomicAdd(&sh.small_n, 1u) & (NT - 1);
-                sh.small[at] = key;
-                sh.amount[at] = amount(key);
+        if (m <= DIRECT || shift == 0) {
+            // gather, then compare
+            for (int i = tid; i < n; i += NT) {
+                const uint64_t x = amount(i);
+                if (x && range(i) == at) {
+                    const uint32_t to = atomicAdd(&sh.n, 1u) & (NT - 1);
+                    sh.amount[to] = x;
+                    sh.order[to] = order(i);
+                    sh.index[to] = (uint32_t)i;
+                }
             }
-        });
-        __syncthreads();
-        uint64_t last = ~0ull;
-        if (tid < (int)m) {
-            const uint64_t key = sh.small[tid];
-            uint64_t above = before;
-            for (int j = 0; j < (int)m; j++) above += sh.small[j] > key ? sh.amount[j] : 0;
-            if (above < limit) last = key;
+            __syncthreads();
+            if (tid < (int)min(m, (uint32_t)NT)) {
+                const uint64_t o = sh.order[tid];
+                uint64_t ahead_of = before;
+                for (uint32_t j = 0; j < m; j++) ahead_of += sh.order[j] < o ? sh.amount[j] : 0;
+                if (ahead_of < limit && ahead_of + sh.amount[tid] >= limit) sh.scratch.found[0] = sh.index[tid];
+            }
+            __syncthreads();
+            return (int)sh.scratch.found[0];
         }
-        return block_min(sh.scratch, last);
+        // the places that the range spans
+        uint64_t least = ~0ull, most = ~0ull;
+        for (int i = tid; i < n; i += NT)
+            if (amount(i) && range(i) == at) {
+                const uint64_t o = order(i);
+                least = o < least ? o : least;
+                most = ~o < most ? ~o : most;
+            }
+        least = block_min(sh.scratch, least);
+        most = ~block_min(sh.scratch, most);
+        lo = least;
+        hi = most;
+        shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
     }
 }
 
 __device__ __forceinline__ double clamped_u(const SampleArgs& a, int b) { return fmin(fmax((double)a.u[b], 0.0), 1.0); }
+
+// u of the total, plus one: the running sum that the token's reaches first.
+__device__ __forceinline__ uint64_t draw_limit(const SampleArgs& a, int b, uint64_t total)
+{
+    const uint64_t t = (uint64_t)(clamped_u(a, b) * (double)total);
+    return t < total ? t + 1 : total;
+}
 
 __device__ __forceinline__ void write_token(const SampleArgs& a, int b, int column, float l, const Weigher& weigh,
                                             double total)
@@ -641,318 +798,300 @@ __device__ __forceinline__ void write_token(const SampleArgs& a, int b, int colu
     a.out_logprob[b] = (float)(((double)l - (double)weigh.max) * weigh.c / LOG2E_F64 - log(total));
 }
 
-// The token at `target` of the kept entries of the list in column order; its
-// entries' kept weights are `kept`, `total` all of them.
-template <class F>
-__device__ void draw_from_list(Scratch& sh, const SampleArgs& a, const Weigher& weigh, const uint64_t* list, int n, F kept,
-                               uint64_t target, uint64_t total, int b)
+// Up to DIRECT entries: each one's rank and the weight ahead of it, and the
+// kept weight of lower columns, by comparing it with every other, half of
+// them by each half of the workgroup.
+__device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
+                                              int n, double z, int b)
 {
-    const int per = (n + NT - 1) / NT, i0 = threadIdx.x * per, i1 = min(n, i0 + per);
-    uint64_t mine = 0, all;
-    for (int i = i0; i < i1; i++) mine += kept(list[i]);
-    uint64_t run = block_scan(sh, mine, all);
-    if (!(run > target && run - mine <= target)) return;
-    run -= mine;
-    for (int i = i0; i < i1; i++) {
-        run += kept(list[i]);
-        if (run > target) {
-            write_token(a, b, key_column(list[i]), key_logit(list[i]), weigh, (double)total / UNIT);
-            return;
-        }
-    }
-}
-
-__device__ __forceinline__ uint64_t draw_target(const SampleArgs& a, int b, uint64_t total)
-{
-    const uint64_t t = (uint64_t)(clamped_u(a, b) * (double)total);
-    return t < total ? t : total - 1;
-}
-
-// Up to DIRECT entries: each one's rank and the weight before it by comparing
-// it with every other, half of them by each half of the workgroup.
-__device__ void finish_direct(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, int n, double z,
-                              int b)
-{
-    static_assert(NT == 2 * DIRECT, "two threads an entry");
     const int tid = threadIdx.x, i = tid & (DIRECT - 1), half = tid / DIRECT;
-    const uint64_t key = i < n ? sh.list[i] : 0;
-    const double w = weigh(key_logit(key));
-    const uint64_t mass = i < n ? fixed(w) : 0;
-    if (half == 0) sh.amount[i] = mass;
-    __syncthreads();
+    const int j0 = half ? n / 2 : 0, j1 = half ? n : n / 2;
+    const uint64_t key = i < n ? sh.list[i] : 0, mass = i < n ? sh.mass[i] : 0;
     uint32_t rank = 0;
     uint64_t before = 0;
-    if (i < n) {
-        const int mid = n / 2;
-        for (int j = half ? mid : 0; j < (half ? n : mid); j++) {
-            const bool ahead = sh.list[j] > key;
-            rank += ahead;
-            before += ahead ? sh.amount[j] : 0;
-        }
+    for (int j = j0; j < j1; j++) {
+        const bool ahead = sh.list[j] > key;
+        rank += ahead;
+        before += ahead ? sh.mass[j] : 0;
     }
-    sh.small[tid] = before;
+    sh.order[tid] = before;
     sh.count[tid] = rank;
     __syncthreads();
     rank += sh.count[tid ^ DIRECT];
-    before += sh.small[tid ^ DIRECT];
-    bool stays = half == 0 && i < n && (s.k == 0 || rank < s.k);
+    before += sh.order[tid ^ DIRECT];
+    bool stays = i < n && (s.k == 0 || rank < s.k);
     uint64_t total;
     if (s.top_p_on) {
         double all = z * UNIT;
         if (s.k > 0) {
-            block_scan(sh.scratch, stays ? mass : 0, total);
+            block_scan(sh.scratch, half == 0 && stays ? mass : 0, total);
             all = (double)total;
         }
         stays = stays && (rank == 0 || (double)before < s.p * all);
     }
-    if (s.min_p_on) stays = stays && w >= s.min_p;
-    const uint64_t mine = stays ? mass : 0;
-    const uint64_t run = block_scan(sh.scratch, mine, total);
-    const uint64_t target = draw_target(a, b, total);
-    if (run > target && run - mine <= target)
+    if (s.min_p_on) stays = stays && weigh(key_logit(key)) >= s.min_p;
+    const uint64_t kept = stays ? mass : 0;
+    if (half == 0) sh.amount[i] = kept;
+    block_scan(sh.scratch, half == 0 ? kept : 0, total);  // (its barriers are amount's as well)
+    const uint64_t limit = draw_limit(a, b, total);
+    uint64_t run = 0;
+    const uint32_t col = ~(uint32_t)key;
+    for (int j = j0; j < j1; j++) run += ~(uint32_t)sh.list[j] < col ? sh.amount[j] : 0;
+    sh.order[tid] = run;
+    __syncthreads();
+    run += sh.order[tid ^ DIRECT];
+    if (half == 0 && kept && run < limit && run + kept >= limit)
         write_token(a, b, key_column(key), key_logit(key), weigh, (double)total / UNIT);
 }
 
-// The row, all of it, by its source: borders by find_border, the draw from
-// the list or, without one, over the row in pieces of the threads.
-template <int LT>
-__device__ void finish_source(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
-                              const Source<LT>& src, double z, int b)
+// A list of more entries: a border's key by the order of logits, the draw by
+// the order of columns.
+__device__ __forceinline__ uint64_t list_border(FinishShared& sh, int n, uint64_t limit, bool by_count, uint64_t from,
+                                                const Binner& bin)
 {
-    auto mass = [&](uint64_t key) { return fixed(weigh(key_logit(key))); };
+    const int at = locate_entry(
+        sh, n, limit, [&](int i) { return ~sh.list[i]; },
+        [&](int i) -> uint64_t { return sh.list[i] < from ? 0 : by_count ? 1 : sh.mass[i]; },
+        [&](int i) { return bin(key_logit(sh.list[i])); });
+    return at < 0 ? from : sh.list[at];
+}
+
+__device__ void finish_list(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, int n, float cut,
+                            double z, int b)
+{
+    const Binner bin(weigh.max, cut, NT);
     uint64_t lo = 0, total;
-    if (s.k > 0) lo = find_border(sh, src, lo, (uint64_t)s.k, 0, [](uint64_t) { return 1ull; });
+    if (s.k > 0) lo = list_border(sh, n, s.k, true, 0, bin);
     if (s.top_p_on) {
         double all = z * UNIT;
         if (s.k > 0) {
             uint64_t part = 0;
-            src.each([&](uint64_t key) { part += key >= lo ? mass(key) : 0; });
+            for (int i = threadIdx.x; i < n; i += NT) part += sh.list[i] >= lo ? sh.mass[i] : 0;
             block_scan(sh.scratch, part, total);
             all = (double)total;
         }
         const double limit = ceil(s.p * all);
-        lo = find_border(sh, src, lo, limit > 1.0 ? (uint64_t)limit : 1, 0, mass);
+        lo = list_border(sh, n, limit > 1.0 ? (uint64_t)limit : 1, false, lo, bin);
     }
-    auto kept = [&](uint64_t key) -> uint64_t {
-        if (key < lo) return 0;
-        const double w = weigh(key_logit(key));
-        return !s.min_p_on || w >= s.min_p ? fixed(w) : 0;
-    };
-    if (src.list) {
-        uint64_t part = 0;
-        src.each([&](uint64_t key) { part += kept(key); });
-        block_scan(sh.scratch, part, total);
-        draw_from_list(sh.scratch, a, weigh, src.list, src.n, kept, draw_target(a, b, total), total, b);
-        return;
+    // what does not stay weighs nothing from here on
+    uint64_t part = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t key = sh.list[i];
+        if (key < lo || (s.min_p_on && !(weigh(key_logit(key)) >= s.min_p))) sh.mass[i] = 0;
+        part += sh.mass[i];
     }
-    const int per = (a.vocab + NT - 1) / NT, c0 = threadIdx.x * per, c1 = min(a.vocab, c0 + per);
-    auto at = [&](int c) -> uint64_t {
-        const float l = src.row.at(c);
-        return l >= src.cut ? kept(order_key(l, c)) : 0;
-    };
-    uint64_t mine = 0;
-    for (int c = c0; c < c1; c++) mine += at(c);
-    uint64_t run = block_scan(sh.scratch, mine, total);
-    const uint64_t target = draw_target(a, b, total);
-    if (!(run > target && run - mine <= target)) return;
-    run -= mine;
-    for (int c = c0; c < c1; c++) {
-        run += at(c);
-        if (run > target) {
-            write_token(a, b, c, src.row.at(c), weigh, (double)total / UNIT);
-            return;
-        }
-    }
+    block_scan(sh.scratch, part, total);
+    const int width = (a.vocab + NT - 1) / NT;
+    const int at = locate_entry(
+        sh, n, draw_limit(a, b, total), [&](int i) { return (uint64_t)(uint32_t)~(uint32_t)sh.list[i]; },
+        [&](int i) { return sh.mass[i]; }, [&](int i) { return key_column(sh.list[i]) / width; });
+    if (threadIdx.x == 0)
+        write_token(a, b, key_column(sh.list[at]), key_logit(sh.list[at]), weigh, (double)total / UNIT);
 }
 
-// The smallest key whose weight is at least min_p, by a search of 64 steps at
-// once in every wave.
-__device__ __forceinline__ uint64_t min_p_border(const Setting& s, const Weigher& weigh)
-{
-    uint32_t lo = 0x00800000u, hi = (uint32_t)(order_key(weigh.max, 0) >> 32);  // (-FLT_MAX's; weight 1 >= min_p)
-    while (lo < hi) {
-        const uint32_t step = (hi - lo) / 64 + 1, probe = lo + min((threadIdx.x & 63) * step, hi - lo);
-        const uint64_t yes = __ballot(weigh(key_logit((uint64_t)probe << 32)) >= s.min_p);
-        if (yes == 0) {
-            lo = lo + min(63 * step, hi - lo - 1) + 1;
-        } else {
-            const int f = __ffsll((unsigned long long)yes) - 1;
-            hi = lo + min((uint32_t)f * step, hi - lo);
-            if (f > 0) lo = lo + min((uint32_t)(f - 1) * step, hi - lo) + (hi > lo ? 1 : 0);
-            lo = min(lo, hi);
-        }
-    }
-    return (uint64_t)hi << 32;
-}
-
-// A row of more entries than LDS lists: slices above short_slice() entries
-// have histograms, the others' lists are in LDS.  False if a border's bin has
-// too many entries.
+// A row after the refine launch: the border among its bin's entries, then the
+// slice that the draw falls into, whose entries are read again.  False if the
+// bin has too many.
 template <int LT>
-__device__ bool finish_long(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, const Row<LT>& row,
-                            float cut, double z, const uint64_t long_slices[MAX_SLICES / 64], int n, int b)
+__device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
+                               const Row<LT>& row, const RowInfo& info, uint32_t n_short, int b)
 {
     constexpr int VEC = Row<LT>::VEC;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, slices = a.slices();
-    const int64_t hist0 = (int64_t)b * slices * BINS;
-    const int slice_blocks = NW * a.unit_blocks;
-    const float inv = bins_inv(weigh.max, cut);
+    const int tid = threadIdx.x, slices = a.slices();
+    const int64_t slice0 = (int64_t)b * slices;
+    const RefineInfo ref = a.refined[b];
+    const uint32_t n_bin = a.counters[b * CNTS + CNT_BIN];
+    if (ref.bin >= 0 && n_bin > LIST) return false;
+    const Binner bins(weigh.max, info.cut, BINS);
+    const uint64_t* const short_list = a.short_list + (int64_t)b * a.short_cap;
     auto mass = [&](uint64_t key) { return fixed(weigh(key_logit(key))); };
-    auto is_long = [&](int g) { return (long_slices[g / 64] >> (g & 63) & 1) != 0; };
-    // the row's histogram: two threads a bin, then the short slices' entries
-    uint64_t* const amount = sh.amount;
-    uint32_t* const count = sh.count;
-    __syncthreads();
-    amount[tid] = 0;
-    count[tid] = 0;
-    __syncthreads();
-    {
-        uint64_t am = 0;
-        uint32_t ct = 0;
-        for (int g = tid / BINS; g < slices; g += NT / BINS)
-            if (is_long(g)) {
-                am += a.bin_amount[hist0 + g * BINS + tid % BINS];
-                ct += a.bin_count[hist0 + g * BINS + tid % BINS];
+    uint64_t lo = 0;
+    int n = 0;
+    if (ref.bin >= 0) {
+        n = (int)n_bin;
+        for (int i = tid; i < n; i += NT) sh.list[i] = a.list[(int64_t)b * a.list_cap + i];
+        if (tid == 0) sh.n = n_bin;
+        __syncthreads();
+        for (uint32_t i = tid; i < n_short; i += NT) {
+            const uint64_t key = short_list[i];
+            if (bins(key_logit(key)) == (int)ref.bin) {
+                const uint32_t to = atomicAdd(&sh.n, 1u);
+                if (to < LIST) sh.list[to] = key;
             }
-        atomicAdd((unsigned long long*)&amount[tid % BINS], (unsigned long long)am);
-        atomicAdd(&count[tid % BINS], ct);
-        for (int i = tid; i < n; i += NT) {
-            const uint64_t key = sh.list[i];
-            const int r = bin_of(key_logit(key), weigh.max, inv);
-            atomicAdd((unsigned long long*)&amount[r], (unsigned long long)mass(key));
-            atomicAdd(&count[r], 1u);
         }
+        __syncthreads();
+        if (sh.n > LIST) return false;
+        n = (int)sh.n;
+        for (int i = tid; i < n; i += NT) sh.mass[i] = mass(sh.list[i]);
+        __syncthreads();
+        // the bin's own range in NT
+        const float top = weigh.max - (float)ref.bin / bins.inv, step = 1.0f / bins.inv;
+        const Binner bin(top, top - step, NT);
+        const double p_limit = ceil(s.p * info.z * UNIT);
+        const uint64_t limit = s.k > 0 ? (uint64_t)s.k : p_limit > 1.0 ? (uint64_t)p_limit : 1;
+        const int at = locate_entry(
+            sh, n, limit - ref.before, [&](int i) { return ~sh.list[i]; },
+            [&](int i) -> uint64_t { return s.k > 0 ? 1 : sh.mass[i]; },
+            [&](int i) { return max(0, bin(key_logit(sh.list[i]))); });
+        if (at >= 0) lo = sh.list[at];
+    }
+    // each slice's kept weight
+    const int slice_cols = NW * a.unit_blocks * VEC;
+    __syncthreads();
+    if (tid < slices) {
+        const uint32_t sn = a.slice_n[slice0 + tid];
+        sh.slice[tid] = sn > a.short_slice() ? a.slice_mass[slice0 + tid] : 0;
+        sh.count[tid] = sn > a.short_slice();
     }
     __syncthreads();
-    const uint64_t bin_mass = tid < BINS ? amount[tid] : 0, bin_n = tid < BINS ? count[tid] : 0;
-    // entries of bin r of all slices to sh.small, in any order; false if too many
-    auto fetch = [&](int r) -> bool {
-        if (tid == 0) sh.small_n = 0;
-        __syncthreads();
-        auto take = [&](uint64_t key) {
-            const uint32_t at = atomicAdd(&sh.small_n, 1u);
-            if (at < NT) sh.small[at] = key;
-        };
-        for (int g = wave; g < slices; g += NW) {
-            if (!is_long(g)) continue;
-            row.stream(g * slice_blocks + lane, min(row.blocks, (g + 1) * slice_blocks), 64, [&](int i, const float (&v)[VEC]) {
-#pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    if (v[j] >= cut && bin_of(v[j], weigh.max, inv) == r) take(order_key(v[j], i * VEC + j));
-            });
-        }
-        for (int i = tid; i < n; i += NT)
-            if (bin_of(key_logit(sh.list[i]), weigh.max, inv) == r) take(sh.list[i]);
-        __syncthreads();
-        return sh.small_n <= NT;
-    };
-    // the border of `limit` by the bins' amounts `mine`: its bin, then among the bin's entries from `from` on
-    int lo_bin = BINS;
-    auto border = [&](uint64_t mine, uint64_t limit, uint64_t from, uint64_t& lo, auto per_entry) -> bool {
-        uint64_t all;
-        const uint64_t run = block_scan(sh.scratch, mine, all);
-        if (all < limit) return true;
-        if (run >= limit && run - mine < limit) {
-            sh.scratch.wave64[NW] = (uint64_t)tid;
-            sh.scratch.wave64[NW + 1] = run - mine;
-        }
-        __syncthreads();
-        const int r = (int)(sh.scratch.wave64[NW] & (BINS - 1));
-        const uint64_t before = sh.scratch.wave64[NW + 1];
-        __syncthreads();
-        if (!fetch(r)) return false;
-        const int m = (int)sh.small_n;
-        uint64_t last = ~0ull;
-        if (tid < m && sh.small[tid] >= from) {
-            const uint64_t key = sh.small[tid];
-            uint64_t above = before;
-            for (int j = 0; j < m; j++) above += sh.small[j] > key ? per_entry(sh.small[j]) : 0;
-            if (above < limit) last = key;
-        }
-        last = block_min(sh.scratch, last);
-        lo = last > lo && last != ~0ull ? last : lo;
-        lo_bin = r;
-        return true;
-    };
-    uint64_t lo = 0, total;
-    double all_mass = z * UNIT;
-    if (s.k > 0) {
-        if (!border(bin_n, (uint64_t)s.k, 0, lo, [](uint64_t) { return 1ull; })) return false;
-        if (s.top_p_on) {  // what top-k kept: whole bins, and the border's bin's entries
-            uint64_t part = tid < lo_bin ? bin_mass : 0;
-            if (lo_bin < BINS && tid < (int)sh.small_n && sh.small[tid] >= lo) part += mass(sh.small[tid]);
-            block_scan(sh.scratch, part, total);
-            all_mass = (double)total;
-        }
-    }
-    if (s.top_p_on) {
-        const double limit = ceil(s.p * all_mass);
-        if (!border(bin_mass, limit > 1.0 ? (uint64_t)limit : 1, lo, lo, mass)) return false;
-    }
-    if (s.min_p_on) {
-        const uint64_t at = min_p_border(s, weigh);
-        if (at > lo) {
-            lo = at;
-            lo_bin = bin_of(key_logit(at), weigh.max, inv);
-            __syncthreads();
-            if (!fetch(lo_bin)) return false;
-        }
-    }
-    // each slice's kept weight: its bins above the border's, its entries in that bin
-    for (int g = tid; g < MAX_SLICES; g += NT) sh.slice_mass[g] = 0;
-    __syncthreads();
-    for (int g = wave; g < slices; g += NW) {
-        if (!is_long(g)) continue;
-        uint64_t part = 0;
-        for (int r = lane; r < min(lo_bin, BINS); r += 64) part += a.bin_amount[hist0 + g * BINS + r];
-        if (part) atomicAdd((unsigned long long*)&sh.slice_mass[g], (unsigned long long)part);
-    }
-    auto slice_of = [&](uint64_t key) { return key_column(key) / (slice_blocks * VEC); };
-    if (lo_bin < BINS && tid < (int)sh.small_n) {
-        const uint64_t key = sh.small[tid];
-        if (key >= lo && is_long(slice_of(key)))
-            atomicAdd((unsigned long long*)&sh.slice_mass[slice_of(key)], (unsigned long long)mass(key));
-    }
     for (int i = tid; i < n; i += NT) {
         const uint64_t key = sh.list[i];
-        if (key >= lo) atomicAdd((unsigned long long*)&sh.slice_mass[slice_of(key)], (unsigned long long)mass(key));
+        const int g = key_column(key) / slice_cols;
+        if (key >= lo && sh.count[g]) atomicAdd((unsigned long long*)&sh.slice[g], (unsigned long long)sh.mass[i]);
+    }
+    for (uint32_t i = tid; i < n_short; i += NT) {
+        const uint64_t key = short_list[i];
+        if (key >= lo) atomicAdd((unsigned long long*)&sh.slice[key_column(key) / slice_cols], (unsigned long long)mass(key));
     }
     __syncthreads();
-    const uint64_t mine = tid < slices ? sh.slice_mass[tid] : 0;
-    const uint64_t run = block_scan(sh.scratch, mine, total);
-    uint64_t target = draw_target(a, b, total);
-    if (run > target && run - mine <= target) {
-        sh.scratch.wave64[NW] = (uint64_t)tid;
-        sh.scratch.wave64[NW + 1] = run - mine;
-    }
-    __syncthreads();
-    const int g = (int)(sh.scratch.wave64[NW] & (MAX_SLICES - 1));
-    target -= sh.scratch.wave64[NW + 1];
-    auto kept = [&](uint64_t key) -> uint64_t { return key >= lo && slice_of(key) == g ? mass(key) : 0; };
-    if (!is_long(g)) {
-        draw_from_list(sh.scratch, a, weigh, sh.list, n, kept, target, total, b);
-        return true;
-    }
-    const int b0 = g * slice_blocks, per = (slice_blocks + NT - 1) / NT;
-    const int i0 = b0 + tid * per, i1 = min(min(row.blocks, b0 + slice_blocks), i0 + per);
-    uint64_t part = 0, all;
+    uint64_t total, before = 0, all;
+    const uint64_t mine = tid < slices ? sh.slice[tid] : 0;
+    block_scan(sh.scratch, mine, total);
+    const uint64_t limit = draw_limit(a, b, total);
+    const int g = block_locate(sh.scratch, mine, limit, before);
+    // that slice, in pieces of the threads
+    const int b0 = g * NW * a.unit_blocks, per = (NW * a.unit_blocks + NT - 1) / NT;
+    const int i0 = b0 + tid * per, i1 = min(min(row.blocks, b0 + NW * a.unit_blocks), i0 + per);
+    auto kept = [&](float l, int c) -> uint64_t { return l >= info.cut && order_key(l, c) >= lo ? fixed(weigh(l)) : 0; };
+    uint64_t part = 0;
     row.stream(i0, i1, 1, [&](int i, const float (&v)[VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++)
-            if (v[j] >= cut) part += kept(order_key(v[j], i * VEC + j));
+        for (int j = 0; j < VEC; j++) part += kept(v[j], i * VEC + j);
     });
-    uint64_t upto = block_scan(sh.scratch, part, all);
-    if (!(upto > target && upto - part <= target)) return true;
-    upto -= part;
+    uint64_t run = before + block_scan(sh.scratch, part, all);
+    if (!(run >= limit && run - part < limit)) return true;
+    run -= part;
     for (int c = i0 * VEC; c < min(a.vocab, i1 * VEC); c++) {
         const float l = row.at(c);
-        if (l >= cut) upto += kept(order_key(l, c));
-        if (upto > target) {
+        run += kept(l, c);
+        if (run >= limit) {
             write_token(a, b, c, l, weigh, (double)total / UNIT);
-            return true;
+            break;
         }
     }
     return true;
+}
+
+// A row of which nothing shorter is known (long ties in the border's bin; a
+// long row under both top-k and top-p): every round goes over all of it.
+template <int LT>
+__device__ uint64_t row_border(FinishShared& sh, const Row<LT>& row, float cut, const Weigher& weigh, uint64_t limit,
+                               bool by_count, uint64_t from)
+{
+    constexpr int VEC = Row<LT>::VEC;
+    const int tid = threadIdx.x;
+    auto each = [&](auto f) {
+        row.stream(tid, row.blocks, NT, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++)
+                if (v[j] >= cut) f(order_key(v[j], i * VEC + j));
+        });
+    };
+    uint64_t lo = from, hi = ~0ull, before = 0;
+    for (;;) {
+        uint64_t least = ~0ull, most = ~0ull;  // (most: the largest key's complement)
+        each([&](uint64_t key) {
+            if (key >= lo && key <= hi) {
+                least = key < least ? key : least;
+                most = ~key < most ? ~key : most;
+            }
+        });
+        lo = block_min(sh.scratch, least);
+        hi = ~block_min(sh.scratch, most);
+        if (lo > hi) return from;
+        const int shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
+        __syncthreads();
+        sh.amount[tid] = 0;
+        __syncthreads();
+        each([&](uint64_t key) {
+            if (key >= lo && key <= hi)
+                atomicAdd((unsigned long long*)&sh.amount[(hi - key) >> shift],
+                          by_count ? 1ull : (unsigned long long)fixed(weigh(key_logit(key))));
+        });
+        __syncthreads();
+        uint64_t ahead = 0;
+        const int r = block_locate(sh.scratch, sh.amount[tid], limit - before, ahead);
+        if (r < 0) return from;
+        before += ahead;
+        hi -= (uint64_t)r << shift;
+        lo = hi - lo < (1ull << shift) - 1 ? lo : hi - ((1ull << shift) - 1);
+        if (shift == 0) return hi;  // (one key)
+    }
+}
+
+template <int LT>
+__device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, const Row<LT>& row,
+                           float cut, double z, int b)
+{
+    constexpr int VEC = Row<LT>::VEC;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    uint64_t lo = 0, total;
+    auto kept = [&](float l, int c, bool with_min) -> uint64_t {
+        if (!(l >= cut) || order_key(l, c) < lo) return 0;
+        const double w = weigh(l);
+        return with_min && s.min_p_on && !(w >= s.min_p) ? 0 : fixed(w);
+    };
+    // the kept weight of the wave's eighth of the row, which `range` cuts out
+    const int eighth = (row.blocks + NW - 1) / NW;
+    auto sum = [&](bool with_min) {
+        uint64_t part = 0;
+        row.stream(wave * eighth + lane, min(row.blocks, (wave + 1) * eighth), 64, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) part += kept(v[j], i * VEC + j, with_min);
+        });
+        return part;
+    };
+    if (s.k > 0) lo = row_border(sh, row, cut, weigh, s.k, true, 0);
+    if (s.top_p_on) {
+        double all = z * UNIT;
+        if (s.k > 0) {
+            block_scan(sh.scratch, sum(false), total);
+            all = (double)total;
+        }
+        const double limit = ceil(s.p * all);
+        lo = row_border(sh, row, cut, weigh, limit > 1.0 ? (uint64_t)limit : 1, false, lo);
+    }
+    const uint64_t part = sum(true);
+    block_scan(sh.scratch, part, total);
+    const uint64_t limit = draw_limit(a, b, total);
+    uint64_t before = 0, all;
+    const int w = block_locate(sh.scratch, part, limit, before) >> 6;
+    // (the sum before the wave, not before its lane: the columns alternate between lanes)
+    const uint64_t wave_sum = read_lane(wave_scan(part), 63);
+    __syncthreads();
+    if (lane == 63) sh.scratch.wave64[wave] = wave_sum;
+    __syncthreads();
+    before = 0;
+    for (int i = 0; i < w; i++) before += sh.scratch.wave64[i];
+    const int per = (eighth + NT - 1) / NT, i0 = w * eighth + tid * per;
+    const int i1 = min(min(row.blocks, (w + 1) * eighth), i0 + per);
+    uint64_t mine = 0;
+    row.stream(i0, i1, 1, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) mine += kept(v[j], i * VEC + j, true);
+    });
+    uint64_t run = before + block_scan(sh.scratch, mine, all);
+    if (!(run >= limit && run - mine < limit)) return;
+    run -= mine;
+    for (int c = i0 * VEC; c < min(a.vocab, i1 * VEC); c++) {
+        const float l = row.at(c);
+        run += kept(l, c, true);
+        if (run >= limit) {
+            write_token(a, b, c, l, weigh, (double)total / UNIT);
+            break;
+        }
+    }
 }
 
 // A draw over the whole row: the unit, then the column, whose running sum is
@@ -984,12 +1123,12 @@ __device__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weighe
     // of that thread's two units
     if (tid == t) {
         const bool second = !(un.us[0] > 0.0) || (un.us[1] > 0.0 && !(before + un.us[0] > target));
-        sh.scratch.wave64[NW] = (uint64_t)(2 * t + second);
-        sh.slice_mass[0] = __builtin_bit_cast(uint64_t, second ? before + un.us[0] : before);
+        sh.scratch.found[0] = (uint64_t)(2 * t + second);
+        sh.scratch.found[1] = __builtin_bit_cast(uint64_t, second ? before + un.us[0] : before);
     }
     __syncthreads();
-    const int unit = (int)sh.scratch.wave64[NW];
-    const double base = __builtin_bit_cast(double, sh.slice_mass[0]);
+    const int unit = (int)sh.scratch.found[0];
+    const double base = __builtin_bit_cast(double, sh.scratch.found[1]);
     const int b0 = unit * a.unit_blocks, per = (a.unit_blocks + NT - 1) / NT;
     const int i0 = b0 + tid * per, i1 = min(min(row.blocks, b0 + a.unit_blocks), i0 + per);
     double mine = 0.0;
@@ -1020,99 +1159,70 @@ __global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
     const int b = blockIdx.x, tid = threadIdx.x;
     const Setting s(a, b);
     const Row<LT> row(a, b);
-    const int64_t units0 = (int64_t)b * a.units;
-    const Units un = read_units(sh.scratch, a, s, b);
-    if (un.max == -INFINITY) {
+    if (!s.listed()) {
+        const Units un = read_units(sh.scratch, a, s, b);
+        const Weigher weigh{un.max, s.c};
+        if (un.max == -INFINITY) {
+            if (tid == 0) {
+                a.out_idx[b] = -1;
+                a.out_logprob[b] = NAN;
+            }
+        } else if (s.k == 1) {  // the first maximum
+            const int mine = un.um[0] == un.max ? 2 * tid : un.um[1] == un.max ? 2 * tid + 1 : MAX_UNITS;
+            const int unit = (int)block_min(sh.scratch, (uint64_t)mine);
+            uint64_t col = ~0ull;
+            row.stream(unit * a.unit_blocks + tid, min(row.blocks, (unit + 1) * a.unit_blocks), NT,
+                       [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+                           for (int j = VEC - 1; j >= 0; j--)
+                               if (v[j] == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
+                       });
+            col = block_min(sh.scratch, col);
+            if (tid == 0) {
+                a.out_idx[b] = (int64_t)col;
+                a.out_logprob[b] = 0.0f;
+            }
+        } else {
+            finish_plain<LT>(sh, a, weigh, row, un, b);
+        }
+        return;
+    }
+    const uint32_t n_long = a.counters[b * CNTS + CNT_LONG], n_short = a.counters[b * CNTS + CNT_SHORT];
+    const uint32_t n = n_long + n_short;
+    if (n == 0) {  // (nothing collected: the row has no maximum)
         if (tid == 0) {
             a.out_idx[b] = -1;
             a.out_logprob[b] = NAN;
         }
         return;
     }
-    const Weigher weigh{un.max, s.c};
-    if (s.k == 1) {  // the first maximum
-        const int mine = un.um[0] == un.max ? 2 * tid : un.um[1] == un.max ? 2 * tid + 1 : MAX_UNITS;
-        const int unit = (int)block_min(sh.scratch, (uint64_t)mine);
-        uint64_t col = ~0ull;
-        row.stream(unit * a.unit_blocks + tid, min(row.blocks, (unit + 1) * a.unit_blocks), NT,
-                   [&](int i, const float (&v)[VEC]) {
-#pragma unroll
-                       for (int j = VEC - 1; j >= 0; j--)
-                           if (v[j] == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
-                   });
-        col = block_min(sh.scratch, col);
-        if (tid == 0) {
-            a.out_idx[b] = (int64_t)col;
-            a.out_logprob[b] = 0.0f;
-        }
-        return;
-    }
-    if (!s.listed()) {
-        finish_plain<LT>(sh, a, weigh, row, un, b);
-        return;
-    }
-    // the units' lists: all of them, or those of the slices without a histogram
-    uint32_t len[2];
-    bool over = false;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        len[i] = 2 * tid + i < a.units ? a.list_len[units0 + 2 * tid + i] : 0;
-        over |= len[i] > (uint32_t)a.cap;
-    }
-    uint64_t all;
-    block_scan(sh.scratch, (uint64_t)(len[0] + len[1]) | (over ? 1ull << 40 : 0), all);
-    const bool fits = all <= LIST;
-    uint64_t long_slices[MAX_SLICES / 64] = {};
-    if (!fits) {
-        // a slice's entries are those of the threads of its 8 units, 4 lanes
-        uint32_t n = len[0] + len[1];
-        n += __shfl_xor(n, 1);
-        n += __shfl_xor(n, 2);
-        const bool is_long = n > a.short_slice();
-        if (is_long) len[0] = len[1] = 0;
-        const uint64_t quads = __ballot(is_long && (tid & 3) == 0);
-        __syncthreads();
-        if ((tid & 63) == 0) {
-            uint32_t bits = 0;
-            for (int i = 0; i < 16; i++) bits |= (uint32_t)(quads >> (4 * i) & 1) << i;
-            sh.scratch.wave64[tid >> 6] = bits;
+    const RowInfo info = a.info[b];
+    const Weigher weigh{info.max, s.c};
+    if (n <= LIST) {
+        for (uint32_t i = tid; i < n; i += NT) {
+            const uint64_t key = i < n_long ? a.list[(int64_t)b * a.list_cap + i]
+                                            : a.short_list[(int64_t)b * a.short_cap + (i - n_long)];
+            sh.list[i] = key;
+            sh.mass[i] = fixed(weigh(key_logit(key)));
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NW; i++) long_slices[i / 4] |= sh.scratch.wave64[i] << (16 * (i % 4));
-    }
-    const uint64_t upto = block_scan(sh.scratch, len[0] + len[1], all);
-    const int n = (int)all;
-    sh.first[2 * tid + 2] = (uint32_t)upto;
-    sh.first[2 * tid + 1] = (uint32_t)upto - len[1];
-    if (tid == 0) sh.first[0] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-        int at = 0;  // the unit: first[at] <= i < first[at + 1]
-#pragma unroll
-        for (int step = MAX_UNITS / 2; step > 0; step >>= 1)
-            if (sh.first[at + step] <= (uint32_t)i) at += step;
-        sh.list[i] = a.list[(units0 + at) * a.cap + (i - sh.first[at])];
-    }
-    __syncthreads();
-    if (fits && n <= DIRECT) {
-        finish_direct(sh, a, s, weigh, n, un.z, b);
+        if (n <= DIRECT)
+            finish_direct(sh, a, s, weigh, (int)n, info.z, b);
+        else
+            finish_list(sh, a, s, weigh, (int)n, info.cut, info.z, b);
         return;
     }
-    float cut = -INFINITY;
-    if (!fits) {
-        cut = lowest_kept(sh.cut, a, s, un, b);
-        if (finish_long<LT>(sh, a, s, weigh, row, cut, un.z, long_slices, n, b)) return;
-        __syncthreads();
-    }
-    finish_source<LT>(sh, a, s, weigh, Source<LT>{row, fits ? sh.list : nullptr, n, cut}, un.z, b);
+    if (a.refines && s.one_border() && finish_refined<LT>(sh, a, s, weigh, row, info, n_short, b)) return;
+    __syncthreads();
+    finish_row<LT>(sh, a, s, weigh, row, info.cut, info.z, b);
 }
 
 // How a call is cut: units of at least 64 blocks (one load a lane), longer
-// ones where the rows alone make 1024 workgroups of 16 units.
+// ones where the rows alone make 2048 workgroups.
 struct Plan {
-    int units, unit_blocks, fine, cap;
-    size_t unit_sum, unit_max, fine_max, list_len, bin_amount, bin_count, list, bytes;
+    int units, unit_blocks, fine, list_cap, short_cap;
+    size_t unit_sum, unit_max, fine_max, counters, info, refined, slice_n, slice_mass, bin_amount, bin_count, list,
+        short_list, bytes;
 };
 
 Plan make_plan(int64_t rows, int64_t vocab, int vec)
@@ -1124,11 +1234,9 @@ Plan make_plan(int64_t rows, int64_t vocab, int vec)
     per = per > (blocks + NW - 1) / NW ? (blocks + NW - 1) / NW : per;
     p.unit_blocks = (int)((per + 63) / 64 * 64);
     p.units = (int)((blocks + p.unit_blocks - 1) / p.unit_blocks);
-    p.fine = p.units >= 512 ? 4 : 64;
-    const int entries = p.unit_blocks * vec;
-    // a list of more is not read: its slice has a histogram (short_slice())
-    const int whole = LIST / ((p.units + NW - 1) / NW) > 512 ? LIST / ((p.units + NW - 1) / NW) : 512;
-    p.cap = entries < whole ? entries : whole;
+    p.fine = p.units < 128 ? 64 : p.units < 512 ? 16 : 4;
+    p.list_cap = vocab < LIST ? (int)vocab : LIST;
+    p.short_cap = vocab < SHORT_LIST ? (int)vocab : SHORT_LIST;
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t r = at;
@@ -1139,10 +1247,15 @@ Plan make_plan(int64_t rows, int64_t vocab, int vec)
     p.unit_sum = take(n * 8);
     p.unit_max = take(n * 4);
     p.fine_max = take(n * p.fine * 4);
-    p.list_len = take(n * 4);
+    p.counters = take(rows * CNTS * 4);
+    p.info = take(rows * sizeof(RowInfo));
+    p.refined = take(rows * sizeof(RefineInfo));
+    p.slice_n = take(slices * 4);
+    p.slice_mass = take(slices * 8);
     p.bin_amount = take(slices * BINS * 8);
     p.bin_count = take(slices * BINS * 4);
-    p.list = take(n * p.cap * 8);
+    p.list = take(rows * p.list_cap * 8);
+    p.short_list = take(rows * p.short_cap * 8);
     p.bytes = at;
     return p;
 }
@@ -1152,19 +1265,25 @@ int launch(const SampleCall& c)
 {
     const Plan p = make_plan(c.rows, c.vocab, Row<LT>::VEC);
     char* const ws = (char*)c.workspace;
-    const SampleArgs a{c.logits, c.l_stride, (int)c.vocab, p.units, p.unit_blocks, p.fine, p.cap,
+    // settings common to all rows say here which launches have nothing to do:
+    // without a border nothing is listed; no list is long where the row is
+    // short or a top-k of at most LIST / 3 cuts it (but for ties, which the
+    // finish goes over by itself)
+    const bool by_row = c.temperature_rows || c.top_k_rows || c.top_p_rows || c.min_p_rows;
+    const bool listed = by_row || (c.temperature > 0.0f && c.top_k != 1 && (c.top_k > 0 || c.top_p < 1.0f || c.min_p > 0.0f));
+    const bool refine = listed && c.vocab > LIST && (by_row || c.top_k == 0 || c.top_k > LIST / 3);
+    const SampleArgs a{c.logits, c.l_stride, (int)c.vocab, p.units, p.unit_blocks, p.fine, p.list_cap, p.short_cap, refine,
                        c.u, c.temperature_rows, c.top_k_rows, c.top_p_rows, c.min_p_rows,
                        c.temperature, c.top_p, c.min_p, c.top_k, c.out_idx, c.out_logprob,
                        (double*)(ws + p.unit_sum), (float*)(ws + p.unit_max), (float*)(ws + p.fine_max),
-                       (uint32_t*)(ws + p.list_len), (uint64_t*)(ws + p.bin_amount), (uint32_t*)(ws + p.bin_count),
-                       (uint64_t*)(ws + p.list)};
-    // nothing is listed for settings, common to all rows, without a border
-    const bool listed = c.temperature_rows || c.top_k_rows || c.top_p_rows || c.min_p_rows ||
-                        (c.temperature > 0.0f && c.top_k != 1 && (c.top_k > 0 || c.top_p < 1.0f || c.min_p > 0.0f));
+                       (uint32_t*)(ws + p.counters), (RowInfo*)(ws + p.info), (RefineInfo*)(ws + p.refined),
+                       (uint32_t*)(ws + p.slice_n), (uint64_t*)(ws + p.slice_mass), (uint64_t*)(ws + p.bin_amount),
+                       (uint32_t*)(ws + p.bin_count), (uint64_t*)(ws + p.list), (uint64_t*)(ws + p.short_list)};
     hipStream_t st = (hipStream_t)c.stream;
     const dim3 grid((unsigned)((p.units + NW - 1) / NW), (unsigned)c.rows), block(NT);
     hipLaunchKernelGGL(sample_stats_kernel<LT>, grid, block, 0, st, a);
     if (listed) hipLaunchKernelGGL(sample_collect_kernel<LT>, grid, block, 0, st, a);
+    if (refine) hipLaunchKernelGGL(sample_refine_kernel<LT>, grid, block, 0, st, a);
     hipLaunchKernelGGL(sample_finish_kernel<LT>, dim3((unsigned)c.rows), block, 0, st, a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return set_hip_error(err, "vq2 sample launch");
