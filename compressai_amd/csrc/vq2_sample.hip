@@ -50,6 +50,7 @@ constexpr int NT = 512;           // threads of a workgroup
 constexpr int BITS = 9;           // NT = 2^BITS
 constexpr int NW = NT / 64;       // its waves, one unit each: a slice
 constexpr int MAX_UNITS = 1024;   // units of a row
+constexpr int MAX_GROUPS = 8192;  // groups of a row (Plan::fine)
 constexpr int LIST = 3072;        // entries of the list in LDS
 constexpr int SHORT_LIST = 8192;  // entries of the slices without a histogram
 constexpr int DIRECT = 256;       // entries that are ranked directly
@@ -134,6 +135,10 @@ struct Setting {
 // alignment of its elements; the last block may be short.
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
+// An infinite logit counts as the largest finite one (no difference of
+// infinities); NaN stays.
+__device__ __forceinline__ float finite(float v) { return v == INFINITY ? FLT_MAX : v; }
+
 template <int LT>
 struct Row {
     static constexpr int VEC = LT == VQ2_DT_F32 ? 4 : 8;
@@ -144,9 +149,6 @@ struct Row {
           full(a.vocab / VEC)
     {
     }
-    // An infinite logit becomes the largest finite one (no difference of
-    // infinities); NaN stays.
-    static __device__ __forceinline__ float finite(float v) { return v == INFINITY ? FLT_MAX : v; }
     __device__ __forceinline__ float at(int column) const { return finite(ld_t<LT>(p, column)); }
     __device__ __forceinline__ u32x4 raw(int block) const { return *(const u32x4_any*)(p + (int64_t)block * 16); }
     static __device__ __forceinline__ void values(u32x4 w, float (&v)[VEC])
@@ -159,32 +161,32 @@ struct Row {
                 const uint32_t h = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
                 v[i] = LT == VQ2_DT_F16 ? f16_bits_to_f32((uint16_t)h) : bf16_bits_to_f32(h);
             }
-            v[i] = finite(v[i]);
         }
     }
     // f(block, values) for the blocks from `from` on in steps of `step`, the
-    // next block's load in flight meanwhile.  A short last block, padded with
-    // -inf, comes by itself: its loads in the loop's path would keep every
-    // load from being in flight.
+    // next block's load in flight meanwhile; the first one's is head(from,
+    // end).  A short last block is loaded by itself and padded with -inf.
+    __device__ __forceinline__ u32x4 head(int from, int end) const
+    {
+        return from < min(end, full) ? raw(from) : u32x4{};
+    }
     template <class F>
     __device__ __forceinline__ void stream(int from, int end, int step, F f) const
     {
-        const int last = min(end, full);
-        int i = from;
-        if (i < last) {
-            u32x4 next = raw(i);
-            for (; i < last; i += step) {
-                const u32x4 w = next;
-                if (i + step < last) next = raw(i + step);
-                float v[VEC];
-                values(w, v);
-                f(i, v);
-            }
-        }
-        if (i == full && i < end) {
+        stream(from, end, step, head(from, end), f);
+    }
+    template <class F>
+    __device__ __forceinline__ void stream(int from, int end, int step, u32x4 next, F f) const
+    {
+        for (int i = from; i < end; i += step) {
+            const u32x4 w = next;
+            if (i + step < min(end, full)) next = raw(i + step);
             float v[VEC];
+            values(w, v);
+            if (i >= full) {
 #pragma unroll
-            for (int j = 0; j < VEC; j++) v[j] = i * VEC + j < vocab ? at(i * VEC + j) : -INFINITY;
+                for (int j = 0; j < VEC; j++) v[j] = i * VEC + j < vocab ? ld_t<LT>(p, i * VEC + j) : -INFINITY;
+            }
             f(i, v);
         }
     }
@@ -193,7 +195,7 @@ struct Row {
 // Order of a row's entries: larger is earlier.
 __device__ __forceinline__ uint64_t order_key(float l, int i)
 {
-    return argmax_key(l + 0.0f, i);  // (+ 0: -0 is 0)
+    return argmax_key(finite(l) + 0.0f, i);  // (+ 0: -0 is 0)
 }
 __device__ __forceinline__ float key_logit(uint64_t key)
 {
@@ -210,7 +212,7 @@ struct Weigher {
     double c;
     __device__ __forceinline__ double operator()(float l) const
     {
-        const double d = ((double)l - (double)max) * c;
+        const double d = ((double)finite(l) - (double)max) * c;
         return d > -999.0 ? exp2_f64_in(d) : 0.0;  // (NaN: 0)
     }
 };
@@ -225,7 +227,7 @@ struct Binner {
         const float width = max - cut;
         inv = width > 0.0f && width < INFINITY ? (float)n / width : 0.0f;
     }
-    __device__ __forceinline__ int operator()(float l) const { return (int)fminf((max - l) * inv, (float)(n - 1)); }
+    __device__ __forceinline__ int operator()(float l) const { return (int)fminf((max - finite(l)) * inv, (float)(n - 1)); }
 };
 
 // ------------------------------------------------- sums over the workgroup
@@ -386,61 +388,71 @@ __device__ __forceinline__ Units read_units(Scratch& sh, const SampleArgs& a, co
 // at its ends (odd in f, so that it averages out of a sum), in 11 operations
 // of 64 bits and a lookup instead of 17.
 constexpr int TABLE = 1024;
-__device__ __forceinline__ double exp2_table(const double* table, double y)
+__device__ __forceinline__ double exp2_table(const double* table, double y)  // |y| <= 1000
 {
     constexpr double MAGIC = 6755399441055744.0 / TABLE;  // rounds to a whole number of 1 / TABLE
-    y = fmax(y, -1000.0);
     const double t = y + MAGIC;
     const double f = y - (t - MAGIC);
     const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
     const double r = table[n & (TABLE - 1)];
     const double g = fma(0.2402265069591007, f, 0.6931471805599453) * f;
-    const uint64_t p = __builtin_bit_cast(uint64_t, fma(r, g, r));
-    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)(n >> 10) << 20);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)p);
+    return __builtin_amdgcn_ldexp(fma(r, g, r), n >> 10);
 }
 
 template <int LT>
-__global__ void __launch_bounds__(NT) sample_stats_kernel(SampleArgs a)
+__global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
     __shared__ double table[TABLE];
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     if (blockIdx.x == 0 && tid < CNTS) a.counters[b * CNTS + tid] = 0;
+    const Row<LT> row(a, b);
+    const int unit = blockIdx.x * NW + (tid >> 6);
+    const int from = unit * a.unit_blocks + lane, end = min(row.blocks, (unit + 1) * a.unit_blocks);
+    const u32x4 head = row.head(from, end);
     const Setting s(a, b);
     if (s.whole_sum()) {
         for (int i = tid; i < TABLE; i += NT) table[i] = exp2_f64_in((double)i / TABLE);
         __syncthreads();
     }
-    const int unit = blockIdx.x * NW + (tid >> 6);
     if (unit >= a.units) return;
-    const Row<LT> row(a, b);
-    const int from = unit * a.unit_blocks + lane, end = min(row.blocks, (unit + 1) * a.unit_blocks);
     float m = -INFINITY;
     double sum = 0.0;
     if (s.whole_sum()) {
         // sum of exp((l - ref) / temperature), ref one of the lane's logits:
-        // 64 bits hold weights of 2^1000, so it moves only where one is close
-        float ref = -INFINITY;
-        row.stream(from, end, 64, [&](int, const float (&v)[VEC]) {
+        // 64 bits hold weights of 2^1000, so it moves only where one is close.
+        // Logits are raised to `least`, whose weight is 2^-990 (absent ones
+        // too: the median of the three is the one that is no NaN); where fp32
+        // has no such number (huge logits, huge temperatures) it is -inf.
+        float ref = -INFINITY, least = -INFINITY;
+        row.stream(from, end, 64, head, [&](int, const float (&v)[VEC]) {
             float top = v[0];
 #pragma unroll
             for (int j = 1; j < VEC; j++) top = fmaxf(top, v[j]);
+            top = finite(top);
             m = fmaxf(m, top);
             if (((double)top - (double)ref) * s.c > 900.0) {
                 sum *= exp2_f64(((double)ref - (double)top) * s.c);
                 ref = top;
+                least = (float)fmax((double)ref - 990.0 / s.c, (double)-FLT_MAX);
+                if (fabs(((double)ref - (double)least) * s.c - 990.0) > 5.0) least = -INFINITY;
             }
+            if (least > -INFINITY) {
 #pragma unroll
-            for (int j = 0; j < VEC; j++) sum += exp2_table(table, ((double)v[j] - (double)ref) * s.c);
+                for (int j = 0; j < VEC; j++)
+                    sum += exp2_table(table, ((double)__builtin_amdgcn_fmed3f(v[j], least, FLT_MAX) - (double)ref) * s.c);
+            } else {
+                for (int j = 0; j < VEC; j++) sum += exp2_f64(((double)finite(v[j]) - (double)ref) * s.c);
+            }
         });
         const float um = wave_max_all(m);
         sum = wave_sum_f64(sum * exp2_f64(((double)ref - (double)um) * s.c));
     } else {
-        row.stream(from, end, 64, [&](int, const float (&v)[VEC]) {
+        row.stream(from, end, 64, head, [&](int, const float (&v)[VEC]) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) m = fmaxf(m, v[j]);
         });
+        m = finite(m);
     }
     const int64_t at = (int64_t)b * a.units + unit;
     if (s.k > 1) {
@@ -542,17 +554,19 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
         const int groups = coarse ? a.units : a.units * a.fine;
         if (s.k * 5 <= (uint32_t)groups * 4) {
             const int64_t u0 = (int64_t)b * a.units;
-            const float* const g = coarse ? a.unit_max + u0 : a.fine_max + u0 * a.fine;
-            float least = INFINITY;
-            for (int i = tid; i < groups; i += NT) least = fminf(least, fmaxf(g[i], cut));
+            const float* const from = coarse ? a.unit_max + u0 : a.fine_max + u0 * a.fine;
+            float g[MAX_GROUPS / NT], least = INFINITY;  // (all loads in flight together)
+#pragma unroll
+            for (int i = 0; i < MAX_GROUPS / NT; i++) g[i] = tid + i * NT < groups ? from[tid + i * NT] : INFINITY;
+#pragma unroll
+            for (int i = 0; i < MAX_GROUPS / NT; i++) least = fminf(least, fmaxf(g[i], cut));
             least = -block_max(sh.scratch, -least);
             const Binner bin(un.max, least, NT);
             sh.count[tid] = 0;
             __syncthreads();
-            for (int i = tid; i < groups; i += NT) {
-                const float l = g[i];
-                if (l >= least) atomicAdd(&sh.count[bin(l)], 1u);
-            }
+#pragma unroll
+            for (int i = 0; i < MAX_GROUPS / NT; i++)
+                if (tid + i * NT < groups && g[i] >= least) atomicAdd(&sh.count[bin(g[i])], 1u);
             __syncthreads();
             uint64_t before;
             const int r = block_locate(sh.scratch, sh.count[tid], s.k, before);
@@ -760,6 +774,7 @@ __device__ __forceinline__ int locate_entry(FinishShared& sh, int n, uint64_t li
             if (tid < (int)min(m, (uint32_t)NT)) {
                 const uint64_t o = sh.order[tid];
                 uint64_t ahead_of = before;
+#pragma unroll 8
                 for (uint32_t j = 0; j < m; j++) ahead_of += sh.order[j] < o ? sh.amount[j] : 0;
                 if (ahead_of < limit && ahead_of + sh.amount[tid] >= limit) sh.scratch.found[0] = sh.index[tid];
             }
@@ -809,6 +824,7 @@ __device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs
     const uint64_t key = i < n ? sh.list[i] : 0, mass = i < n ? sh.mass[i] : 0;
     uint32_t rank = 0;
     uint64_t before = 0;
+#pragma unroll 8
     for (int j = j0; j < j1; j++) {
         const bool ahead = sh.list[j] > key;
         rank += ahead;
@@ -836,6 +852,7 @@ __device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs
     const uint64_t limit = draw_limit(a, b, total);
     uint64_t run = 0;
     const uint32_t col = ~(uint32_t)key;
+#pragma unroll 8
     for (int j = j0; j < j1; j++) run += ~(uint32_t)sh.list[j] < col ? sh.amount[j] : 0;
     sh.order[tid] = run;
     __syncthreads();
@@ -844,34 +861,30 @@ __device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs
         write_token(a, b, key_column(key), key_logit(key), weigh, (double)total / UNIT);
 }
 
-// A list of more entries: a border's key by the order of logits, the draw by
-// the order of columns.
-__device__ __forceinline__ uint64_t list_border(FinishShared& sh, int n, uint64_t limit, bool by_count, uint64_t from,
-                                                const Binner& bin)
-{
-    const int at = locate_entry(
-        sh, n, limit, [&](int i) { return ~sh.list[i]; },
-        [&](int i) -> uint64_t { return sh.list[i] < from ? 0 : by_count ? 1 : sh.mass[i]; },
-        [&](int i) { return bin(key_logit(sh.list[i])); });
-    return at < 0 ? from : sh.list[at];
-}
-
-__device__ void finish_list(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, int n, float cut,
-                            double z, int b)
+// A list of more entries: the borders by the order of logits, the draw by the
+// order of columns.
+__device__ __forceinline__ void finish_list(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, int n,
+                                            float cut, double z, int b)
 {
     const Binner bin(weigh.max, cut, NT);
     uint64_t lo = 0, total;
-    if (s.k > 0) lo = list_border(sh, n, s.k, true, 0, bin);
-    if (s.top_p_on) {
-        double all = z * UNIT;
-        if (s.k > 0) {
-            uint64_t part = 0;
-            for (int i = threadIdx.x; i < n; i += NT) part += sh.list[i] >= lo ? sh.mass[i] : 0;
-            block_scan(sh.scratch, part, total);
-            all = (double)total;
+    for (int by_mass = s.k == 0; by_mass <= (int)s.top_p_on; by_mass++) {  // top-k, top-p
+        double limit = (double)s.k;
+        if (by_mass) {
+            limit = z * UNIT;
+            if (s.k > 0) {
+                uint64_t part = 0;
+                for (int i = threadIdx.x; i < n; i += NT) part += sh.list[i] >= lo ? sh.mass[i] : 0;
+                block_scan(sh.scratch, part, total);
+                limit = (double)total;
+            }
+            limit = fmax(1.0, ceil(s.p * limit));
         }
-        const double limit = ceil(s.p * all);
-        lo = list_border(sh, n, limit > 1.0 ? (uint64_t)limit : 1, false, lo, bin);
+        const int at = locate_entry(
+            sh, n, (uint64_t)limit, [&](int i) { return ~sh.list[i]; },
+            [&](int i) -> uint64_t { return sh.list[i] < lo ? 0 : by_mass ? sh.mass[i] : 1; },
+            [&](int i) { return bin(key_logit(sh.list[i])); });
+        if (at >= 0) lo = sh.list[at];
     }
     // what does not stay weighs nothing from here on
     uint64_t part = 0;
@@ -986,47 +999,48 @@ __device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Sett
 // A row of which nothing shorter is known (long ties in the border's bin; a
 // long row under both top-k and top-p): every round goes over all of it.
 template <int LT>
-__device__ uint64_t row_border(FinishShared& sh, const Row<LT>& row, float cut, const Weigher& weigh, uint64_t limit,
-                               bool by_count, uint64_t from)
+__device__ __forceinline__ uint64_t row_border(FinishShared& sh, const Row<LT>& row, float cut, const Weigher& weigh,
+                                               uint64_t limit, bool by_mass, uint64_t from)
 {
     constexpr int VEC = Row<LT>::VEC;
     const int tid = threadIdx.x;
-    auto each = [&](auto f) {
-        row.stream(tid, row.blocks, NT, [&](int i, const float (&v)[VEC]) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++)
-                if (v[j] >= cut) f(order_key(v[j], i * VEC + j));
-        });
-    };
     uint64_t lo = from, hi = ~0ull, before = 0;
+    int shift = 64;  // (64: a round that finds the range the entries span)
     for (;;) {
         uint64_t least = ~0ull, most = ~0ull;  // (most: the largest key's complement)
-        each([&](uint64_t key) {
-            if (key >= lo && key <= hi) {
-                least = key < least ? key : least;
-                most = ~key < most ? ~key : most;
-            }
-        });
-        lo = block_min(sh.scratch, least);
-        hi = ~block_min(sh.scratch, most);
-        if (lo > hi) return from;
-        const int shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
         __syncthreads();
         sh.amount[tid] = 0;
         __syncthreads();
-        each([&](uint64_t key) {
-            if (key >= lo && key <= hi)
-                atomicAdd((unsigned long long*)&sh.amount[(hi - key) >> shift],
-                          by_count ? 1ull : (unsigned long long)fixed(weigh(key_logit(key))));
+        row.stream(tid, row.blocks, NT, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+                const uint64_t key = order_key(v[j], i * VEC + j);
+                if (!(v[j] >= cut) || key < lo || key > hi) continue;
+                if (shift == 64) {
+                    least = key < least ? key : least;
+                    most = ~key < most ? ~key : most;
+                } else {
+                    atomicAdd((unsigned long long*)&sh.amount[(hi - key) >> shift],
+                              by_mass ? (unsigned long long)fixed(weigh(v[j])) : 1ull);
+                }
+            }
         });
         __syncthreads();
+        if (shift == 64) {
+            lo = block_min(sh.scratch, least);
+            hi = ~block_min(sh.scratch, most);
+            if (lo > hi) return from;
+            shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
+            continue;
+        }
         uint64_t ahead = 0;
         const int r = block_locate(sh.scratch, sh.amount[tid], limit - before, ahead);
         if (r < 0) return from;
         before += ahead;
         hi -= (uint64_t)r << shift;
-        lo = hi - lo < (1ull << shift) - 1 ? lo : hi - ((1ull << shift) - 1);
         if (shift == 0) return hi;  // (one key)
+        lo = hi - lo < (1ull << shift) - 1 ? lo : hi - ((1ull << shift) - 1);
+        shift = 64;
     }
 }
 
@@ -1036,7 +1050,7 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
 {
     constexpr int VEC = Row<LT>::VEC;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    uint64_t lo = 0, total;
+    uint64_t lo = 0, total = 0;
     auto kept = [&](float l, int c, bool with_min) -> uint64_t {
         if (!(l >= cut) || order_key(l, c) < lo) return 0;
         const double w = weigh(l);
@@ -1052,18 +1066,18 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
         });
         return part;
     };
-    if (s.k > 0) lo = row_border(sh, row, cut, weigh, s.k, true, 0);
-    if (s.top_p_on) {
-        double all = z * UNIT;
-        if (s.k > 0) {
-            block_scan(sh.scratch, sum(false), total);
-            all = (double)total;
+    uint64_t part = 0;
+    // top-k's border; the weight that it keeps, top-p's border; the kept weight
+    for (int step = s.k > 0 ? 0 : s.top_p_on ? 2 : 3; step < 4; step++) {
+        if (step == 1 || step == 3) {
+            part = sum(step == 3);
+            block_scan(sh.scratch, part, total);
+            if (step == 1 && !s.top_p_on) step = 2;
+            continue;
         }
-        const double limit = ceil(s.p * all);
-        lo = row_border(sh, row, cut, weigh, limit > 1.0 ? (uint64_t)limit : 1, false, lo);
+        const double limit = step == 0 ? (double)s.k : fmax(1.0, ceil(s.p * (s.k > 0 ? (double)total : z * UNIT)));
+        lo = row_border(sh, row, cut, weigh, (uint64_t)limit, step == 2, lo);
     }
-    const uint64_t part = sum(true);
-    block_scan(sh.scratch, part, total);
     const uint64_t limit = draw_limit(a, b, total);
     uint64_t before = 0, all;
     const int w = block_locate(sh.scratch, part, limit, before) >> 6;
@@ -1175,7 +1189,7 @@ __global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
                        [&](int i, const float (&v)[VEC]) {
 #pragma unroll
                            for (int j = VEC - 1; j >= 0; j--)
-                               if (v[j] == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
+                               if (finite(v[j]) == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
                        });
             col = block_min(sh.scratch, col);
             if (tid == 0) {
@@ -1218,7 +1232,7 @@ __global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
 }
 
 // How a call is cut: units of at least 64 blocks (one load a lane), longer
-// ones where the rows alone make 2048 workgroups.
+// ones where the rows alone fill the device, 8192 waves of up to 64 registers.
 struct Plan {
     int units, unit_blocks, fine, list_cap, short_cap;
     size_t unit_sum, unit_max, fine_max, counters, info, refined, slice_n, slice_mass, bin_amount, bin_count, list,
@@ -1229,7 +1243,7 @@ Plan make_plan(int64_t rows, int64_t vocab, int vec)
 {
     Plan p;
     const int64_t blocks = (vocab + vec - 1) / vec;
-    int64_t per = (blocks * rows + 16383) / 16384;
+    int64_t per = (blocks * rows + 8191) / 8192;
     per = per > (blocks + MAX_UNITS - 1) / MAX_UNITS ? per : (blocks + MAX_UNITS - 1) / MAX_UNITS;
     per = per > (blocks + NW - 1) / NW ? (blocks + NW - 1) / NW : per;
     p.unit_blocks = (int)((per + 63) / 64 * 64);
