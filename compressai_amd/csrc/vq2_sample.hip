@@ -542,9 +542,11 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
 {
     const int tid = threadIdx.x;
     const double m = (double)un.max;
-    double w = 2.8421709430404007e-14;  // 2^-45
-    if (s.k == 0 && s.top_p_on) w = fmax(w, (1.0 - s.p) * 0.999 * un.z / (double)a.vocab);
-    double low = m + log2(w) / s.c;
+    // (the logarithm of 32 bits is off by less than 0.001)
+    double bits = -45.0;
+    if (s.k == 0 && s.top_p_on)
+        bits = fmax(bits, (double)__builtin_amdgcn_logf((float)((1.0 - s.p) * un.z / (double)a.vocab)) - 0.002);
+    double low = m + bits / s.c;
     low -= (fabs(m) + fabs(low)) * 1e-6;
     float cut = (float)fmax(low, (double)-FLT_MAX);
     if (s.k > 0) {
@@ -654,10 +656,10 @@ __global__ void __launch_bounds__(NT) sample_refine_kernel(SampleArgs a)
     constexpr int VEC = Row<LT>::VEC;
     __shared__ RefineShared sh;
     const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, slices = gridDim.x;
-    const Setting s(a, b);
-    if (!s.listed() || !s.one_border()) return;
     const uint32_t n_long = a.counters[b * CNTS + CNT_LONG], n_short = a.counters[b * CNTS + CNT_SHORT];
     if (n_long + n_short <= LIST) return;
+    const Setting s(a, b);
+    if (!s.one_border()) return;
     const RowInfo info = a.info[b];
     const Weigher weigh{info.max, s.c};
     const Binner bin(info.max, info.cut, BINS);
