@@ -10,6 +10,8 @@
 // every pointer, shape and type is read from the arguments of the call.
 #include <torch/extension.h>
 
+#include <c10/core/impl/VirtualGuardImpl.h>
+
 #include <algorithm>
 
 #include "vq2_amd.h"
@@ -392,6 +394,105 @@ py::object sorted_moe(const at::Tensor& h, py::handle gate_up, const at::Tensor&
     return py::cast(out);
 }
 
+// Rows of unit stride on the current device, [R, n] with R * n > 0 (others:
+// the Python entry); the elements between them.
+int64_t read_rows(Check& c, const at::Tensor& t)
+{
+    c.on_gpu(t);
+    c.need(t.dim() == 2 && t.size(0) > 0 && t.size(1) > 0 && dt_code(t.scalar_type()) >= 0);
+    if (!c.ok) return 0;
+    c.need(t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= t.size(1)));
+    static const c10::impl::VirtualGuardImpl guard(at::kCUDA);
+    c.need(guard.getDevice() == t.device());
+    return t.size(0) == 1 ? t.size(1) : t.stride(0);
+}
+
+// vq_router_select without given outputs; scoring and group_score as codes
+py::object router_select(const at::Tensor& logits, int64_t k, int64_t scoring, const OptTensor& bias, int64_t n_groups,
+                         int64_t topk_groups, int64_t group_score, bool renormalise, double scale, const OptTensor& h,
+                         const OptTensor& gate, int64_t shared_id)
+{
+    Check c;
+    const int64_t stride = read_rows(c, logits);
+    if (!c.ok) return py::none();
+    const int64_t T = logits.size(0), E = logits.size(1);
+    c.table(bias, at::kFloat, E);
+    c.need(k >= 1 && k <= 4096 && n_groups >= 1 && n_groups <= 4096 && topk_groups >= 1 && topk_groups <= n_groups);
+    const bool gated = shared_id >= 0 && gate.has_value();
+    if (gated) {
+        if (!h) return py::none();
+        c.dense(*h);
+        c.dense(*gate);
+        c.need(dt_code(h->scalar_type()) >= 0 && dt_code(gate->scalar_type()) >= 0 && h->numel() == T * gate->numel());
+    } else {
+        if (h) c.on_gpu(*h);
+        if (gate) c.on_gpu(*gate);
+    }
+    if (!c.ok) return py::none();
+    const int64_t slots = k + (shared_id >= 0);
+    at::Tensor ids = at::empty({T, slots}, logits.options().dtype(at::kInt));
+    at::Tensor w = at::empty({T, slots}, logits.options().dtype(at::kFloat));
+    void* const st = stream_of(*c.dev);
+    int32_t* const io = ids.data_ptr<int32_t>();
+    float* const wo = w.data_ptr<float>();
+    check_status(unlocked([&] {
+                     return vq2_router_select(ptr(logits), dt_code(logits.scalar_type()), stride, T, E, (int)k, (int)scoring,
+                                              (const float*)ptr(bias), (int)n_groups, (int)topk_groups, (int)group_score,
+                                              renormalise, (float)scale, gated ? ptr(h) : nullptr,
+                                              gated ? dt_code(h->scalar_type()) : 0, gated ? gate->numel() : 0,
+                                              gated ? ptr(gate) : nullptr, gated ? dt_code(gate->scalar_type()) : 0, shared_id,
+                                              io, wo, st);
+                 }),
+                 "vq2_router_select");
+    return py::make_tuple(ids, w);
+}
+
+// A setting of vq_sample: a number, or a tensor of one value per row
+template <class N>
+struct RowSetting {
+    N one = 0;
+    at::Tensor rows;
+    RowSetting(Check& c, py::handle o, at::ScalarType dt, int64_t n)
+    {
+        if (THPVariable_Check(o.ptr())) {
+            rows = THPVariable_Unpack(o.ptr());
+            c.table(rows, dt, n);
+        } else if (PyLong_Check(o.ptr()) || (std::is_floating_point_v<N> && PyFloat_Check(o.ptr()))) {
+            one = py::cast<N>(o);
+        } else {
+            c.need(false);
+        }
+    }
+    const void* ptr() const { return rows.defined() ? rows.const_data_ptr() : nullptr; }
+};
+
+// vq_sample
+py::object sample(const at::Tensor& logits, const at::Tensor& u, py::handle temperature, py::handle top_k, py::handle top_p,
+                  py::handle min_p)
+{
+    Check c;
+    const int64_t stride = read_rows(c, logits);
+    if (!c.ok) return py::none();
+    const int64_t B = logits.size(0), V = logits.size(1);
+    c.table(u, at::kFloat, B);
+    const RowSetting<double> t(c, temperature, at::kFloat, B), p(c, top_p, at::kFloat, B), m(c, min_p, at::kFloat, B);
+    const RowSetting<int64_t> k(c, top_k, at::kInt, B);
+    if (!c.ok) return py::none();
+    at::Tensor idx = at::empty({B}, logits.options().dtype(at::kLong));
+    at::Tensor logprob = at::empty({B}, logits.options().dtype(at::kFloat));
+    const size_t bytes = vq2_sample_workspace(B, V);
+    const at::Tensor ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+    void* const st = stream_of(*c.dev);
+    check_status(unlocked([&] {
+                     return vq2_sample(ptr(logits), dt_code(logits.scalar_type()), stride, B, V, (const float*)ptr(u),
+                                       (float)t.one, (const float*)t.ptr(), k.one, (const int32_t*)k.ptr(), (float)p.one,
+                                       (const float*)p.ptr(), (float)m.one, (const float*)m.ptr(), idx.data_ptr<int64_t>(),
+                                       logprob.data_ptr<float>(), ws.data_ptr(), bytes, st);
+                 }),
+                 "vq2_sample");
+    return py::make_tuple(idx, logprob);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -400,6 +501,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("gemv_rht", &gemv_rht);
     m.def("rows_gemm", &rows_gemm);
     m.def("sorted_moe", &sorted_moe);
+    m.def("router_select", &router_select);
+    m.def("sample", &sample);
     m.def("sorted_slices", [](int64_t chunks, int64_t min_ipc, int64_t cu) {
         return sorted_slices(std::max<int64_t>(1, chunks), min_ipc, cu);
     });

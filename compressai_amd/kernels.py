@@ -17,7 +17,8 @@ Additive entry points: vq_gemv_16_16 (4 bpw), batched GEMV (x of shape
 vq_moe_down_combine, vq_gemv_argmax, vq_sample, vq_argmax, vq_dequant_rows, vq_decode_idx.
 
 The entries of the small calls (vq_sorted_gemv, vq_gemv_rht, vq_rows_gemm,
-vq_sorted_moe) hand the calls without given outputs to their native twins
+vq_sorted_moe, vq_router_select, vq_sample) hand the calls without given
+outputs to their native twins
 (csrc/vq2_host.cpp: the same checks and launch, ~8 us less host time each),
 which decline whatever the checks here have to look at.
 
@@ -1488,6 +1489,11 @@ def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, t
     topk_groups = n_groups if topk_groups is None else int(topk_groups)
     if scoring not in SCORING or group_score not in GROUP_SCORE:
         raise Vq2Error(f"vq_router_select: scoring {scoring!r} (softmax/sigmoid), group_score {group_score!r} (max/top2)")
+    if ids is None and w is None and logits.is_cuda:
+        out = _lib.host().router_select(logits, k, SCORING[scoring], bias, n_groups, topk_groups, GROUP_SCORE[group_score],
+                                        renormalise, scale, h, shared_gate, shared_id)
+        if out is not None:
+            return out
     dev = _dev(logits, bias, h, shared_gate, ids, w)
     lg, stride = _rows2d(logits, "logits")
     T, E = lg.shape
@@ -1530,6 +1536,10 @@ def vq_sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     logprob.  Each setting is a number for all rows or a tensor [rows] (fp32;
     top_k int32).  Returns (idx int64 [rows], logprob fp32 [rows]: the log of
     the probability the token was drawn with)."""
+    if logits.is_cuda:
+        out = _lib.host().sample(logits, u, temperature, top_k, top_p, min_p)
+        if out is not None:
+            return out
     rows_of = [t if torch.is_tensor(t) else None for t in (temperature, top_k, top_p, min_p)]
     dev = _dev(logits, u, *rows_of)
     lg, stride = _rows2d(logits, "logits")
