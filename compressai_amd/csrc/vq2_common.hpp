@@ -65,7 +65,7 @@ __device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float
         ((float*)p)[i] = v;
 }
 
-// 2^y in 64 bits, -1000 <= y <= 1000: y is split into the nearest whole
+// 2^y in 64 bits, |y| < 1023: y is split into the nearest whole
 // number, which goes into the exponent, and f in [-1/2, 1/2]; 2^f = 1 + f g(f),
 // g interpolated at the Chebyshev nodes by a polynomial of degree 8 (2^f off
 // by 4e-14 of itself over the range, and exact at 0).  15 operations, against
@@ -88,7 +88,7 @@ __device__ __forceinline__ double exp2_f64_in(double y)
     const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)p);
 }
-// any y <= 1000; below -1000, or NaN: 2^-1000
+// any y < 1023; below -1000, or NaN: 2^-1000
 __device__ __forceinline__ double exp2_f64(double y) { return exp2_f64_in(fmax(y, -1000.0)); }
 constexpr double LOG2E_F64 = 1.4426950408889634074;
 

@@ -6,7 +6,21 @@
 // their two best and the first `keep` stay; the k best c of the experts that
 // stay are taken in descending order, ties to the lower id.  Weights come from
 // s alone.  An expert whose logit is -inf or NaN (or whose choice is) is
-// masked: it ranks behind every other one and weighs 0.
+// masked: it ranks behind every other one and weighs 0.  Without a bias c
+// orders as the logits do, which are compared themselves.
+//
+// Choices that differ in the eighth digit must not trade places, so they are
+// made in 64 bits; but a sigmoid of 64 bits for each of E experts costs several
+// times what the rest does.  Two kernels:
+//   rows   16 lanes a token, four tokens a wave.  Choices of 32 bits, cut to
+//          22 to 26 bits of their range with the expert's id below them, make
+//          one word each: a lane sorts its own (a network of v_min / v_max_u32),
+//          rounds of a maximum over the 16 lanes (DPP) take the k + 4 best, and
+//          only those are computed in 64 bits and put in order by them.  The
+//          words of what was left out say whether any of it could belong among
+//          the k (or whether two groups are too close to tell): such tokens, and
+//          those with too few experts, go to
+//   token  one wave a token, all of it in 64 bits.
 #include "vq2_common.hpp"
 #include "vq2_router.hpp"
 #include "vq2_internal.hpp"
@@ -29,8 +43,84 @@ struct SelectArgs {
     int64_t shared_id;
     int32_t* ids;
     float* w;
+    __device__ __forceinline__ int slots() const { return k + (shared_id >= 0 ? 1 : 0); }
 };
 
+// Scores of 64 bits: exp for x <= 0, and the sigmoid, 0 where e^-x is none of
+// 64 bits.
+__device__ __forceinline__ double exp_f64(double x) { return exp2_f64(x * LOG2E_F64); }
+__device__ __forceinline__ double sigmoid_f64(double x)
+{
+    return x < -709.0 ? 0.0 : 1.0 / (1.0 + exp2_f64(-x * LOG2E_F64));
+}
+
+// LDS written by a wave's lanes is read by its others.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ------------------------------------------------- sigmoid(gate . h) of a token
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8])
+{
+    typedef u32x4 __attribute__((aligned(2))) any_t;
+    if constexpr (DT == VQ2_DT_F32) {
+        const u32x4 a = *(const any_t*)((const float*)p + i), b = *(const any_t*)((const float*)p + i + 4);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = __uint_as_float(a[j]);
+            v[4 + j] = __uint_as_float(b[j]);
+        }
+    } else {
+        const u32x4 a = *(const any_t*)((const uint16_t*)p + i);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t h = j & 1 ? a[j / 2] >> 16 : a[j / 2] & 0xFFFFu;
+            v[j] = DT == VQ2_DT_F16 ? f16_bits_to_f32((uint16_t)h) : bf16_bits_to_f32(h);
+        }
+    }
+}
+
+template <int GT, int HT>
+__device__ __forceinline__ float gate_dot(const SelectArgs& a, int64_t t, int lane)
+{
+    const int64_t row = t * a.hidden, whole = a.hidden / 512 * 512;
+    float d = 0.0f;
+#pragma unroll 4
+    for (int64_t i = lane * 8; i < whole; i += 512) {
+        float g[8], x[8];
+        load8<GT>(a.gate, i, g);
+        load8<HT>(a.h, row + i, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) d = fmaf(g[j], x[j], d);
+    }
+    for (int64_t i = whole + lane; i < a.hidden; i += 64) d = fmaf(ld_t<GT>(a.gate, i), ld_t<HT>(a.h, row + i), d);
+    return wave_sum_all(d);
+}
+
+// the shared expert's weight, uniform over the wave
+__device__ __forceinline__ float shared_weight(const SelectArgs& a, int64_t t, int lane)
+{
+    if (!a.gate) return 1.0f;
+    float d;
+    switch (a.g_dt * 3 + a.h_dt) {
+    case VQ2_DT_F32 * 3 + VQ2_DT_F32: d = gate_dot<VQ2_DT_F32, VQ2_DT_F32>(a, t, lane); break;
+    case VQ2_DT_F32 * 3 + VQ2_DT_F16: d = gate_dot<VQ2_DT_F32, VQ2_DT_F16>(a, t, lane); break;
+    case VQ2_DT_F32 * 3 + VQ2_DT_BF16: d = gate_dot<VQ2_DT_F32, VQ2_DT_BF16>(a, t, lane); break;
+    case VQ2_DT_F16 * 3 + VQ2_DT_F32: d = gate_dot<VQ2_DT_F16, VQ2_DT_F32>(a, t, lane); break;
+    case VQ2_DT_F16 * 3 + VQ2_DT_F16: d = gate_dot<VQ2_DT_F16, VQ2_DT_F16>(a, t, lane); break;
+    case VQ2_DT_F16 * 3 + VQ2_DT_BF16: d = gate_dot<VQ2_DT_F16, VQ2_DT_BF16>(a, t, lane); break;
+    case VQ2_DT_BF16 * 3 + VQ2_DT_F32: d = gate_dot<VQ2_DT_BF16, VQ2_DT_F32>(a, t, lane); break;
+    case VQ2_DT_BF16 * 3 + VQ2_DT_F16: d = gate_dot<VQ2_DT_BF16, VQ2_DT_F16>(a, t, lane); break;
+    default: d = gate_dot<VQ2_DT_BF16, VQ2_DT_BF16>(a, t, lane); break;
+    }
+    return 1.0f / (1.0f + __expf(-d));
+}
+
+// ------------------------------------------------------------- one wave a token
 constexpr double KEY_MASKED = -1e300;
 
 // Choice and expert in one double, so that one v_max_f64 compares both: the
@@ -65,13 +155,11 @@ __device__ __forceinline__ double wave_sum_f64(double v)
     return v;
 }
 
-// One wave per token; lane holds experts j * 64 + lane.
+// A token's choice by a whole wave; lane holds experts j * 64 + lane, s_c is
+// RPL * 64 doubles of LDS of the wave's own.
 template <int LT, int RPL>
-__global__ void __launch_bounds__(64) select_kernel(SelectArgs a)
+__device__ void select_token(const SelectArgs& a, int64_t t, int lane, double* s_c)
 {
-    __shared__ double s_c[RPL * 64];
-    const int lane = threadIdx.x;
-    const int64_t t = blockIdx.x;
     const int64_t row = t * a.stride;
     float l[RPL];
 #pragma unroll
@@ -88,9 +176,9 @@ __global__ void __launch_bounds__(64) select_kernel(SelectArgs a)
 #pragma unroll
     for (int j = 0; j < RPL; j++) {
         if (a.scoring == VQ2_SCORE_SIGMOID)
-            s[j] = 1.0 / (1.0 + exp(-(double)l[j]));
+            s[j] = sigmoid_f64((double)l[j]);
         else
-            s[j] = l[j] == m ? 1.0 : exp((double)l[j] - (double)m);
+            s[j] = l[j] == m ? 1.0 : exp_f64((double)l[j] - (double)m);
         if (l[j] == -INFINITY) s[j] = 0.0;
         z += s[j];
     }
@@ -112,7 +200,7 @@ __global__ void __launch_bounds__(64) select_kernel(SelectArgs a)
     if (a.n_groups > 1) {
 #pragma unroll
         for (int j = 0; j < RPL; j++) s_c[j * 64 + lane] = s[j];
-        __syncthreads();
+        wave_sync();
         double g1 = -INFINITY, g2 = -INFINITY;
         if (lane < a.n_groups) {
             for (int i = 0; i < a.group_size; i++) {
@@ -153,40 +241,374 @@ __global__ void __launch_bounds__(64) select_kernel(SelectArgs a)
     // the weights: lane r takes choice r's logit again
     double sw = 0.0;
     if (lane < a.k) {
-        float x = ld_t<LT>(a.logits, row + id);
+        const float x = ld_t<LT>(a.logits, row + id);
         bool masked = !(x > -INFINITY);
         if (a.bias) masked |= !(a.bias[id] > -INFINITY);
         if (a.scoring == VQ2_SCORE_SIGMOID)
-            sw = 1.0 / (1.0 + exp(-(double)x));
+            sw = sigmoid_f64((double)x);
         else
-            sw = (x == m ? 1.0 : exp((double)x - (double)m)) / z;
+            sw = (x == m ? 1.0 : exp_f64((double)x - (double)m)) / z;
         if (masked) sw = 0.0;
     }
     const double tot = a.renorm ? wave_sum_f64(sw) : 1.0;
-    const int slots = a.k + (a.shared_id >= 0 ? 1 : 0);
     if (lane < a.k) {
-        a.ids[t * slots + lane] = id;
-        a.w[t * slots + lane] = tot > 0.0 ? (float)(sw / tot * (double)a.scale) : 0.0f;
-    }
-    if (a.shared_id >= 0) {
-        const float g = a.gate ? router_shared_weight(a.gate, a.g_dt, a.h, a.h_dt, t, a.hidden, lane) : 1.0f;
-        if (lane == 0) {
-            a.ids[t * slots + a.k] = (int32_t)a.shared_id;
-            a.w[t * slots + a.k] = g;
-        }
+        a.ids[t * a.slots() + lane] = id;
+        a.w[t * a.slots() + lane] = tot > 0.0 ? (float)(sw / tot * (double)a.scale) : 0.0f;
     }
 }
 
-template <int LT>
-void launch_rpl(const SelectArgs& a, hipStream_t st)
+__device__ __forceinline__ void write_shared(const SelectArgs& a, int64_t t, int lane)
 {
+    const float g = shared_weight(a, t, lane);
+    if (lane == 0) {
+        a.ids[t * a.slots() + a.k] = (int32_t)a.shared_id;
+        a.w[t * a.slots() + a.k] = g;
+    }
+}
+
+template <int LT, int RPL>
+__global__ void __launch_bounds__(64) select_token_kernel(SelectArgs a)
+{
+    __shared__ double s_c[RPL * 64];
+    select_token<LT, RPL>(a, blockIdx.x, threadIdx.x, s_c);
+    if (a.shared_id >= 0) write_shared(a, blockIdx.x, threadIdx.x);
+}
+
+// ----------------------------------------------------------- 16 lanes a token
+constexpr int ROWS_MAX_E = 512, ROWS_MAX_K = 12, ROWS_MAX_G = 16;
+constexpr int EXTRA = 4;  // candidates beyond k
+
+template <int CTRL>
+__device__ __forceinline__ float row_f32(float v)
+{
+    return __int_as_float(dpp_mov<CTRL>(__float_as_int(v)));
+}
+// Over the 16 lanes of a row (rotations by 8, 4, 2, 1), in all of them.
+__device__ __forceinline__ float row_max(float v)
+{
+    v = fmaxf(v, row_f32<0x128>(v));
+    v = fmaxf(v, row_f32<0x124>(v));
+    v = fmaxf(v, row_f32<0x122>(v));
+    return fmaxf(v, row_f32<0x121>(v));
+}
+__device__ __forceinline__ float row_min(float v) { return -row_max(-v); }
+__device__ __forceinline__ float row_sum(float v)
+{
+    v += row_f32<0x128>(v);
+    v += row_f32<0x124>(v);
+    v += row_f32<0x122>(v);
+    return v + row_f32<0x121>(v);
+}
+__device__ __forceinline__ uint32_t row_max_u32(uint32_t v)
+{
+    v = max(v, (uint32_t)dpp_mov<0x128>((int)v));
+    v = max(v, (uint32_t)dpp_mov<0x124>((int)v));
+    v = max(v, (uint32_t)dpp_mov<0x122>((int)v));
+    return max(v, (uint32_t)dpp_mov<0x121>((int)v));
+}
+template <int CTRL>
+__device__ __forceinline__ double row_f64(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double row_sum(double v)
+{
+    v += row_f64<0x128>(v);
+    v += row_f64<0x124>(v);
+    v += row_f64<0x122>(v);
+    return v + row_f64<0x121>(v);
+}
+
+// Descending, by odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_down(uint32_t (&v)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+        for (int k = p; k >= 1; k >>= 1)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; i++)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t x = v[i + j], y = v[i + j + k];
+                        v[i + j] = max(x, y);
+                        v[i + j + k] = min(x, y);
+                    }
+}
+
+// Four tokens a wave, N experts a lane; four waves a workgroup.
+template <int LT, int N, bool GROUPS>
+__global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
+{
+    constexpr int V = LT == VQ2_DT_F32 ? 4 : (N < 8 ? N : 8);  // experts of one load
+    constexpr int IDB = N <= 4 ? 6 : N <= 8 ? 7 : N <= 16 ? 8 : 9, QB = 32 - IDB;
+    constexpr uint32_t IDS = (1u << IDB) - 1;
+    constexpr int HEADS = N < ROWS_MAX_K + EXTRA ? N : ROWS_MAX_K + EXTRA;
+    constexpr int PER_TOKEN = 16 * N + ROWS_MAX_G;  // a group's scores are one apart from the next one's
+    __shared__ uint32_t s_heads[4][HEADS * 64];
+    __shared__ union {
+        float c[4][GROUPS ? PER_TOKEN : 1];
+        double token[GROUPS ? 16 * N : 1];  // (only groups take a whole wave there)
+    } s_g[4];  // one a wave
+    __shared__ float s_score[4][4][GROUPS ? 16 : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15, quarter = lane >> 4;
+    const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * 4;
+    if (t0 >= a.tokens) return;
+    const int64_t t = t0 + quarter, tc = t < a.tokens ? t : a.tokens - 1;
+    const int64_t row = tc * a.stride;
+    const bool softmax = a.scoring == VQ2_SCORE_SOFTMAX, biased = a.bias != nullptr;
+    const bool by_score = biased || (GROUPS && a.group_score == VQ2_GROUP_TOP2);
+
+    auto expert = [&](int j) { return ((j / V) * 16 + sub) * V + j % V; };
+    const uint32_t magic = ((1u << 20) + a.group_size - 1) / a.group_size;
+    auto group = [&](int e) { return (int)((uint32_t)e * magic >> 20); };  // (e / group_size, for e < 512)
+    float l[N];
+#pragma unroll
+    for (int c = 0; c < N / V; c++) {
+        const int e0 = expert(c * V);
+        if (e0 + V <= a.n_e) {
+            if constexpr (LT == VQ2_DT_F32) {
+                typedef u32x4 __attribute__((aligned(4))) any_t;
+                const u32x4 w = *(const any_t*)((const float*)a.logits + row + e0);
+#pragma unroll
+                for (int j = 0; j < 4; j++) l[c * V + j] = __uint_as_float(w[j]);
+            } else {
+                typedef uint32_t words_t __attribute__((ext_vector_type(V / 2)));
+                typedef words_t __attribute__((aligned(2))) any_t;
+                const words_t w = *(const any_t*)((const uint16_t*)a.logits + row + e0);
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const uint32_t h = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu;
+                    l[c * V + j] = LT == VQ2_DT_F16 ? f16_bits_to_f32((uint16_t)h) : bf16_bits_to_f32(h);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                l[c * V + j] = e0 + j < a.n_e ? ld_t<LT>(a.logits, row + e0 + j) : -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        if (!(l[j] > -INFINITY)) l[j] = -INFINITY;  // (NaN)
+        m = fmaxf(m, l[j]);
+    }
+    m = row_max(m);
+
+    // c: choices of 32 bits, -inf where masked; off by less than `eps`
+    float c[N], eps = 0.0f;
+    if (by_score) {
+        if (softmax) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                c[j] = __builtin_amdgcn_exp2f((l[j] - m) * 1.44269504f);
+                z += c[j];
+            }
+            const float r = 1.0f / row_sum(z);
+#pragma unroll
+            for (int j = 0; j < N; j++) c[j] *= r;
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) c[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[j] * -1.44269504f));
+        }
+        if (biased) {
+#pragma unroll
+            for (int o = 0; o < N / V; o++) {
+                const int e0 = expert(o * V);
+#pragma unroll
+                for (int j = 0; j < V; j += 4)
+                    if (e0 + j + 4 <= a.n_e) {
+                        typedef float f32x4 __attribute__((ext_vector_type(4)));
+                        typedef f32x4 __attribute__((aligned(4))) any_t;
+                        const f32x4 b = *(const any_t*)(a.bias + e0 + j);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) c[o * V + j + i] += b[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) c[o * V + j + i] += e0 + j + i < a.n_e ? a.bias[e0 + j + i] : 0.0f;
+                    }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (l[j] == -INFINITY || !(c[j] > -INFINITY)) c[j] = -INFINITY;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) c[j] = l[j];
+    }
+    float cmax = -INFINITY, cmin = INFINITY;
+    auto limits = [&] {
+        cmax = -INFINITY;
+        cmin = INFINITY;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            cmax = fmaxf(cmax, c[j]);
+            cmin = fminf(cmin, c[j] == -INFINITY ? INFINITY : c[j]);
+        }
+        cmax = row_max(cmax);
+        cmin = row_min(cmin);
+        // a score of 32 bits: its exponential's argument, exponential, sum and quotient
+        // (the argument's error falls off with the score), and the bias's addition
+        eps = by_score ? 2e-6f * fmaxf(1.0f, fmaxf(fabsf(cmax), fabsf(cmin))) : 0.0f;
+    };
+    bool unsure = softmax && !(m < INFINITY);
+    uint32_t stays = 0xFFFFu;
+    if constexpr (GROUPS) {
+        limits();
+        float* const sc = s_g[wave].c[quarter];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int e = expert(j);
+            if (e < a.n_e) sc[e + group(e)] = c[j];
+        }
+        wave_sync();
+        // the lanes of a row share the groups: 1, 2, 4, 8 or 16 a group
+        const int shift = a.n_groups > 8 ? 0 : a.n_groups > 4 ? 1 : a.n_groups > 2 ? 2 : 3, g = sub >> shift;
+        float g1 = -INFINITY, g2 = -INFINITY;
+        if (g < a.n_groups)
+            for (int i = sub & ((1 << shift) - 1); i < a.group_size; i += 1 << shift) {
+                const float x = sc[g * (a.group_size + 1) + i];
+                g2 = fmaxf(g2, fminf(g1, x));
+                g1 = fmaxf(g1, x);
+            }
+        auto merge = [&](float o1, float o2) {
+            g2 = fmaxf(fminf(g1, o1), fmaxf(g2, o2));
+            g1 = fmaxf(g1, o1);
+        };
+        if (shift >= 1) merge(dpp_xor1(g1), dpp_xor1(g2));
+        if (shift >= 2) merge(dpp_xor2(g1), dpp_xor2(g2));
+        if (shift >= 3) merge(dpp_half_mirror(g1), dpp_half_mirror(g2));
+        if (a.group_score == VQ2_GROUP_TOP2 && g2 > -INFINITY) g1 += g2;
+        float* const scores = s_score[wave][quarter];
+        if ((sub & ((1 << shift) - 1)) == 0) scores[g] = g1;
+        wave_sync();
+        int rank = 0;
+        for (int o = 0; o < a.n_groups; o++) {
+            const float x = scores[o];
+            rank += x > g1 || (x == g1 && o < g);
+        }
+        const bool real = g < a.n_groups, in = real && rank < a.keep;
+        // groups closer than their scores are exact (logits are)
+        const float lowest_in = row_min(in ? g1 : INFINITY), highest_out = row_max(real && !in ? g1 : -INFINITY);
+        unsure |= by_score && highest_out > -INFINITY && !(lowest_in - highest_out > 4.0f * eps);
+        const uint32_t lanes = (uint32_t)(__ballot(in) >> (quarter * 16)) & 0xFFFFu;
+        stays = 0;
+        for (int o = 0; o < a.n_groups; o++) stays |= (lanes >> (o << shift) & 1) << o;
+        if (!biased) {  // the experts' own order is the logits'
+#pragma unroll
+            for (int j = 0; j < N; j++) c[j] = l[j];
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (!(stays >> group(expert(j)) & 1)) c[j] = -INFINITY;
+    }
+    limits();
+    if (!biased) eps = 0.0f;
+    const float range = cmax - cmin, scale = 0.9999f * (float)(1u << QB) / range;
+    unsure |= !(range > 0.0f && range < INFINITY && scale < INFINITY);
+
+    // words: place in the range, then the id, lower ids above
+    uint32_t key[N];
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        key[j] = c[j] == -INFINITY ? 0u : ((uint32_t)((c[j] - cmin) * scale) + 1u) << IDB | (IDS - (uint32_t)expert(j));
+    sort_down(key);
+#pragma unroll
+    for (int j = 0; j < HEADS; j++) s_heads[wave][j * 64 + lane] = key[j];
+    const int C = a.k + EXTRA;
+    uint32_t mine = 0, head = key[0], last = 0;
+    int next = 1;
+    for (int r = 0; r < C; r++) {
+        last = row_max_u32(head);
+        if (sub == r) mine = last;
+        if (head == last) {
+            head = next < HEADS ? s_heads[wave][next * 64 + lane] : 0;
+            next++;
+        }
+    }
+
+    // the candidates in 64 bits, one a lane
+    const bool has = mine != 0;
+    const int id = has ? (int)(IDS - (mine & IDS)) : 0;
+    double z = 1.0;
+    if (softmax && (biased || !a.renorm)) {
+        z = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp_f64((double)l[j] - (double)m);
+        z = row_sum(z);
+    }
+    const float x = ld_t<LT>(a.logits, row + id);
+    const double s = softmax ? exp_f64((double)x - (double)m) / z : sigmoid_f64((double)x);
+    const double choice = biased ? s + (double)a.bias[id] : (double)x;
+    int rank = 0;
+    auto compare = [&](double o, int oid, bool ohas) { rank += ohas && (o > choice || (o == choice && oid < id)); };
+    const int hid = has ? id : -1;
+#define VQ2_ROTATE(n)                                                       \
+    {                                                                       \
+        const int oid = dpp_mov<0x120 + n>(hid);                            \
+        compare(row_f64<0x120 + n>(choice), oid, oid >= 0);                 \
+    }
+    VQ2_ROTATE(1) VQ2_ROTATE(2) VQ2_ROTATE(3) VQ2_ROTATE(4) VQ2_ROTATE(5) VQ2_ROTATE(6) VQ2_ROTATE(7) VQ2_ROTATE(8)
+    VQ2_ROTATE(9) VQ2_ROTATE(10) VQ2_ROTATE(11) VQ2_ROTATE(12) VQ2_ROTATE(13) VQ2_ROTATE(14) VQ2_ROTATE(15)
+#undef VQ2_ROTATE
+    const bool wins = has && rank < a.k;
+    // `last` is the lowest candidate's word: what was left out is not above it.
+    // Places are off by the choices' error and by the rounding of the
+    // difference and the product (2^-23 of the range together, two of them).
+    const uint32_t slack = 4u + (QB > 23 ? 4u << (QB - 23) : 4u);
+    const float margin = (float)slack + 2.0f * eps * scale;
+    const float lowest = row_min(wins ? (float)(mine >> IDB) : INFINITY);
+    const float winners = row_sum(wins ? 1.0f : 0.0f);
+    unsure |= winners < (float)a.k || (last != 0 && !(lowest - (float)(last >> IDB) > margin));
+
+    const double tot = a.renorm ? row_sum(wins ? s : 0.0) : 1.0;
+    if (wins && !unsure && t < a.tokens) {
+        a.ids[t * a.slots() + rank] = id;
+        a.w[t * a.slots() + rank] = tot > 0.0 ? (float)(s / tot * (double)a.scale) : 0.0f;
+    }
+    // the tokens that are left, by the whole wave
+    const uint64_t left = __ballot(unsure && t < a.tokens);
+    for (int q = 0; q < 4; q++)
+        if (left >> (16 * q) & 1) {
+            wave_sync();
+            select_token<LT, (N + 3) / 4>(a, t0 + q, lane, s_g[wave].token);
+        }
+    if (a.shared_id >= 0)
+        for (int q = 0; q < 4 && t0 + q < a.tokens; q++) write_shared(a, t0 + q, lane);
+}
+
+template <int LT, int N>
+void launch_rows(const SelectArgs& a, hipStream_t st)
+{
+    const dim3 grid((unsigned)((a.tokens + 15) / 16)), block(256);
+    if (a.n_groups > 1)
+        hipLaunchKernelGGL((select_rows_kernel<LT, N, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((select_rows_kernel<LT, N, false>), grid, block, 0, st, a);
+}
+
+template <int LT>
+void launch(const SelectArgs& a, hipStream_t st)
+{
+    if (a.n_e <= ROWS_MAX_E && a.k <= ROWS_MAX_K && a.n_groups <= ROWS_MAX_G) {
+        if (a.n_e <= 64) return launch_rows<LT, 4>(a, st);
+        if (a.n_e <= 128) return launch_rows<LT, 8>(a, st);
+        if (a.n_e <= 256) return launch_rows<LT, 16>(a, st);
+        return launch_rows<LT, 32>(a, st);
+    }
     const dim3 grid((unsigned)a.tokens), block(64);
     if (a.n_e <= 64)
-        hipLaunchKernelGGL((select_kernel<LT, 1>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((select_token_kernel<LT, 1>), grid, block, 0, st, a);
     else if (a.n_e <= 256)
-        hipLaunchKernelGGL((select_kernel<LT, 4>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((select_token_kernel<LT, 4>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((select_kernel<LT, 16>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((select_token_kernel<LT, 16>), grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -197,13 +619,15 @@ int router_select_launch(const RouterSelectCall& c)
     SelectArgs a{c.logits, c.l_stride, c.tokens,    (int)c.n_experts, c.k, c.scoring, c.n_groups, c.keep,
                  (int)(c.n_experts / c.n_groups),   c.group_score,    c.renorm, c.scale, c.bias, c.h, c.h_dt,
                  c.hidden, c.gate, c.g_dt, c.shared_id, c.ids, c.w};
+    // all groups staying is no grouping
+    if (a.keep == a.n_groups) a.n_groups = a.keep = 1, a.group_size = a.n_e;
     hipStream_t st = (hipStream_t)c.stream;
     if (c.l_dt == VQ2_DT_F32)
-        launch_rpl<VQ2_DT_F32>(a, st);
+        launch<VQ2_DT_F32>(a, st);
     else if (c.l_dt == VQ2_DT_F16)
-        launch_rpl<VQ2_DT_F16>(a, st);
+        launch<VQ2_DT_F16>(a, st);
     else
-        launch_rpl<VQ2_DT_BF16>(a, st);
+        launch<VQ2_DT_BF16>(a, st);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return set_hip_error(err, "vq2 router select launch");
     return VQ2_OK;
