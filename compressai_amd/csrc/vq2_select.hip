@@ -49,9 +49,17 @@ struct SelectArgs {
 // Scores of 64 bits: exp for x <= 0, and the sigmoid, 0 where e^-x is none of
 // 64 bits.
 __device__ __forceinline__ double exp_f64(double x) { return exp2_f64(x * LOG2E_F64); }
+// 1 / x of a normal x whose reciprocal is normal, to 2^-51: the instruction's
+// approximation and two Newton steps
+__device__ __forceinline__ double reciprocal_f64(double x)
+{
+    double r = __builtin_amdgcn_rcp(x);
+    r = fma(fma(-x, r, 1.0), r, r);
+    return fma(fma(-x, r, 1.0), r, r);
+}
 __device__ __forceinline__ double sigmoid_f64(double x)
 {
-    return x < -709.0 ? 0.0 : 1.0 / (1.0 + exp2_f64(-x * LOG2E_F64));
+    return x < -700.0 ? (x < -709.0 ? 0.0 : exp_f64(x)) : reciprocal_f64(1.0 + exp2_f64(-x * LOG2E_F64));
 }
 
 // LDS written by a wave's lanes is read by its others.
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(64) select_token_kernel(SelectArgs a)
 
 // ----------------------------------------------------------- 16 lanes a token
 constexpr int ROWS_MAX_E = 512, ROWS_MAX_K = 12, ROWS_MAX_G = 16;
-constexpr int EXTRA = 4;  // candidates beyond k
+constexpr int EXTRA = 2;  // candidates beyond k
 
 template <int CTRL>
 __device__ __forceinline__ float row_f32(float v)
@@ -341,8 +349,8 @@ __device__ __forceinline__ void sort_down(uint32_t (&v)[N])
 }
 
 // Four tokens a wave, N experts a lane; four waves a workgroup.
-template <int LT, int N, bool GROUPS>
-__global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
+template <int LT, int N, bool GROUPS, bool GATE>
+__global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
 {
     constexpr int V = LT == VQ2_DT_F32 ? 4 : (N < 8 ? N : 8);  // experts of one load
     constexpr int IDB = N <= 4 ? 6 : N <= 8 ? 7 : N <= 16 ? 8 : 9, QB = 32 - IDB;
@@ -362,6 +370,8 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
     const int64_t row = tc * a.stride;
     const bool softmax = a.scoring == VQ2_SCORE_SOFTMAX, biased = a.bias != nullptr;
     const bool by_score = biased || (GROUPS && a.group_score == VQ2_GROUP_TOP2);
+    // unbiased logits of 16 bits and an id fit a word: no candidate is in doubt
+    const bool exact = LT != VQ2_DT_F32 && !biased;
 
     auto expert = [&](int j) { return ((j / V) * 16 + sub) * V + j % V; };
     const uint32_t magic = ((1u << 20) + a.group_size - 1) / a.group_size;
@@ -392,6 +402,22 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
                 l[c * V + j] = e0 + j < a.n_e ? ld_t<LT>(a.logits, row + e0 + j) : -INFINITY;
         }
     }
+    // adds the biases of V experts
+    auto add_bias = [&](int o, float* c) {
+        const int e0 = expert(o * V);
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+            if (e0 + j + 4 <= a.n_e) {
+                typedef float f32x4 __attribute__((ext_vector_type(4)));
+                typedef f32x4 __attribute__((aligned(4))) any_t;
+                const f32x4 b = *(const any_t*)(a.bias + e0 + j);
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[j + i] += b[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[j + i] += e0 + j + i < a.n_e ? a.bias[e0 + j + i] : 0.0f;
+            }
+    };
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -399,6 +425,13 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
         m = fmaxf(m, l[j]);
     }
     m = row_max(m);
+    double z = 1.0;
+    if (softmax && (biased || !a.renorm)) {
+        z = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp_f64((double)l[j] - (double)m);
+        z = row_sum(z);
+    }
 
     // c: choices of 32 bits, -inf where masked; off by less than `eps`
     float c[N], eps = 0.0f;
@@ -419,21 +452,7 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
         }
         if (biased) {
 #pragma unroll
-            for (int o = 0; o < N / V; o++) {
-                const int e0 = expert(o * V);
-#pragma unroll
-                for (int j = 0; j < V; j += 4)
-                    if (e0 + j + 4 <= a.n_e) {
-                        typedef float f32x4 __attribute__((ext_vector_type(4)));
-                        typedef f32x4 __attribute__((aligned(4))) any_t;
-                        const f32x4 b = *(const any_t*)(a.bias + e0 + j);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) c[o * V + j + i] += b[i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) c[o * V + j + i] += e0 + j + i < a.n_e ? a.bias[e0 + j + i] : 0.0f;
-                    }
-            }
+            for (int o = 0; o < N / V; o++) add_bias(o, c + o * V);
         }
 #pragma unroll
         for (int j = 0; j < N; j++)
@@ -442,25 +461,19 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
 #pragma unroll
         for (int j = 0; j < N; j++) c[j] = l[j];
     }
-    float cmax = -INFINITY, cmin = INFINITY;
-    auto limits = [&] {
-        cmax = -INFINITY;
-        cmin = INFINITY;
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            cmax = fmaxf(cmax, c[j]);
-            cmin = fminf(cmin, c[j] == -INFINITY ? INFINITY : c[j]);
-        }
-        cmax = row_max(cmax);
-        cmin = row_min(cmin);
-        // a score of 32 bits: its exponential's argument, exponential, sum and quotient
-        // (the argument's error falls off with the score), and the bias's addition
-        eps = by_score ? 2e-6f * fmaxf(1.0f, fmaxf(fabsf(cmax), fabsf(cmin))) : 0.0f;
-    };
+    // What a choice of 32 bits is off by, in units of its size or 1.  Sigmoid:
+    // s (1 - s) |l| 1.5 steps of 2^-24 by the exponential's argument, s (1 - s) 2 by
+    // the exponential, 3 by the sum and the reciprocal, 1 by the bias's addition:
+    // 5 together.  Softmax: 1 by the argument, 38 by the sum of up to 32 + 4
+    // terms, 4 by the rest.
+    const float EPS = softmax ? 2.6e-6f : 3.5e-7f;
     bool unsure = softmax && !(m < INFINITY);
     uint32_t stays = 0xFFFFu;
     if constexpr (GROUPS) {
-        limits();
+        float size = 1.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++) size = fmaxf(size, c[j] == -INFINITY ? 0.0f : fabsf(c[j]));
+        const float eps = EPS * row_max(size);
         float* const sc = s_g[wave].c[quarter];
 #pragma unroll
         for (int j = 0; j < N; j++) {
@@ -472,6 +485,7 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
         const int shift = a.n_groups > 8 ? 0 : a.n_groups > 4 ? 1 : a.n_groups > 2 ? 2 : 3, g = sub >> shift;
         float g1 = -INFINITY, g2 = -INFINITY;
         if (g < a.n_groups)
+#pragma unroll 4
             for (int i = sub & ((1 << shift) - 1); i < a.group_size; i += 1 << shift) {
                 const float x = sc[g * (a.group_size + 1) + i];
                 g2 = fmaxf(g2, fminf(g1, x));
@@ -489,6 +503,7 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
         if ((sub & ((1 << shift) - 1)) == 0) scores[g] = g1;
         wave_sync();
         int rank = 0;
+#pragma unroll 4
         for (int o = 0; o < a.n_groups; o++) {
             const float x = scores[o];
             rank += x > g1 || (x == g1 && o < g);
@@ -508,27 +523,44 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
         for (int j = 0; j < N; j++)
             if (!(stays >> group(expert(j)) & 1)) c[j] = -INFINITY;
     }
-    limits();
-    if (!biased) eps = 0.0f;
+    float cmax = -INFINITY, cmin = INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        cmax = fmaxf(cmax, c[j]);
+        cmin = fminf(cmin, c[j] == -INFINITY ? INFINITY : c[j]);
+    }
+    cmax = row_max(cmax);
+    cmin = row_min(cmin);
     const float range = cmax - cmin, scale = 0.9999f * (float)(1u << QB) / range;
-    unsure |= !(range > 0.0f && range < INFINITY && scale < INFINITY);
+    unsure |= !exact && !(range > 0.0f && range < INFINITY && scale < INFINITY);
 
     // words: place in the range, then the id, lower ids above
     uint32_t key[N];
 #pragma unroll
-    for (int j = 0; j < N; j++)
-        key[j] = c[j] == -INFINITY ? 0u : ((uint32_t)((c[j] - cmin) * scale) + 1u) << IDB | (IDS - (uint32_t)expert(j));
+    for (int j = 0; j < N; j++) {
+        uint32_t place;
+        if (exact) {  // the logit's own 16 bits, in their order (fp16's are fp32's top 19, zeros below)
+            uint32_t u;
+            if constexpr (LT == VQ2_DT_F16) u = __builtin_bit_cast(uint16_t, (_Float16)(c[j] + 0.0f));
+            else u = __float_as_uint(c[j] + 0.0f) >> 16;
+            place = u & 0x8000u ? 0xFFFFu - u : 0x8000u + u;
+        } else {
+            place = (uint32_t)((c[j] - cmin) * scale) + 1u;
+        }
+        key[j] = c[j] == -INFINITY ? 0u : place << IDB | (IDS - (uint32_t)expert(j));
+    }
     sort_down(key);
 #pragma unroll
     for (int j = 0; j < HEADS; j++) s_heads[wave][j * 64 + lane] = key[j];
-    const int C = a.k + EXTRA;
-    uint32_t mine = 0, head = key[0], last = 0;
-    int next = 1;
+    const int C = a.k + (exact ? 0 : EXTRA);
+    uint32_t mine = 0, head = key[0], second = key[1], last = 0;
+    int next = 2;
     for (int r = 0; r < C; r++) {
         last = row_max_u32(head);
         if (sub == r) mine = last;
         if (head == last) {
-            head = next < HEADS ? s_heads[wave][next * 64 + lane] : 0;
+            head = second;
+            second = next < HEADS ? s_heads[wave][next * 64 + lane] : 0;
             next++;
         }
     }
@@ -536,41 +568,38 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
     // the candidates in 64 bits, one a lane
     const bool has = mine != 0;
     const int id = has ? (int)(IDS - (mine & IDS)) : 0;
-    double z = 1.0;
-    if (softmax && (biased || !a.renorm)) {
-        z = 0.0;
-#pragma unroll
-        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp_f64((double)l[j] - (double)m);
-        z = row_sum(z);
-    }
     const float x = ld_t<LT>(a.logits, row + id);
-    const double s = softmax ? exp_f64((double)x - (double)m) / z : sigmoid_f64((double)x);
+    const double s = softmax ? exp_f64((double)x - (double)m) * (z == 1.0 ? 1.0 : reciprocal_f64(z)) : sigmoid_f64((double)x);
     const double choice = biased ? s + (double)a.bias[id] : (double)x;
-    int rank = 0;
-    auto compare = [&](double o, int oid, bool ohas) { rank += ohas && (o > choice || (o == choice && oid < id)); };
+    // they are nearly always in order already: then a candidate's rank is its lane
+    int rank = sub;
     const int hid = has ? id : -1;
-#define VQ2_ROTATE(n)                                                       \
-    {                                                                       \
-        const int oid = dpp_mov<0x120 + n>(hid);                            \
-        compare(row_f64<0x120 + n>(choice), oid, oid >= 0);                 \
-    }
-    VQ2_ROTATE(1) VQ2_ROTATE(2) VQ2_ROTATE(3) VQ2_ROTATE(4) VQ2_ROTATE(5) VQ2_ROTATE(6) VQ2_ROTATE(7) VQ2_ROTATE(8)
-    VQ2_ROTATE(9) VQ2_ROTATE(10) VQ2_ROTATE(11) VQ2_ROTATE(12) VQ2_ROTATE(13) VQ2_ROTATE(14) VQ2_ROTATE(15)
+    auto ahead = [&](double o, int oid) { return oid >= 0 && (o > choice || (o == choice && oid < id)); };
+    if (__ballot(has && ahead(row_f64<0x101>(choice), sub == 15 ? -1 : dpp_mov<0x101>(hid)))) {
+        rank = 0;
+#define VQ2_ROTATE(n) rank += ahead(row_f64<0x120 + n>(choice), dpp_mov<0x120 + n>(hid));
+        VQ2_ROTATE(1) VQ2_ROTATE(2) VQ2_ROTATE(3) VQ2_ROTATE(4) VQ2_ROTATE(5) VQ2_ROTATE(6) VQ2_ROTATE(7) VQ2_ROTATE(8)
+        VQ2_ROTATE(9) VQ2_ROTATE(10) VQ2_ROTATE(11) VQ2_ROTATE(12) VQ2_ROTATE(13) VQ2_ROTATE(14) VQ2_ROTATE(15)
 #undef VQ2_ROTATE
+    }
     const bool wins = has && rank < a.k;
-    // `last` is the lowest candidate's word: what was left out is not above it.
-    // Places are off by the choices' error and by the rounding of the
-    // difference and the product (2^-23 of the range together, two of them).
-    const uint32_t slack = 4u + (QB > 23 ? 4u << (QB - 23) : 4u);
-    const float margin = (float)slack + 2.0f * eps * scale;
-    const float lowest = row_min(wins ? (float)(mine >> IDB) : INFINITY);
     const float winners = row_sum(wins ? 1.0f : 0.0f);
-    unsure |= winners < (float)a.k || (last != 0 && !(lowest - (float)(last >> IDB) > margin));
+    unsure |= winners < (float)a.k;
+    if (!exact) {
+        // `last` is the lowest candidate's word: what was left out is not above it.
+        // Places are off by the choices' error and by the rounding of the
+        // difference and the product (2^-23 of the range together, two of them).
+        const float slack = 4.0f + (float)(QB > 23 ? 4u << (QB - 23) : 4u);
+        const float margin = slack + (biased ? 2.0f * EPS * fmaxf(1.0f, fmaxf(fabsf(cmax), fabsf(cmin))) * scale : 0.0f);
+        const float lowest = row_min(wins ? (float)(mine >> IDB) : INFINITY);
+        unsure |= last != 0 && !(lowest - (float)(last >> IDB) > margin);
+    }
 
     const double tot = a.renorm ? row_sum(wins ? s : 0.0) : 1.0;
+    unsure |= !(tot > 1e-290);  // (no normal reciprocal)
     if (wins && !unsure && t < a.tokens) {
         a.ids[t * a.slots() + rank] = id;
-        a.w[t * a.slots() + rank] = tot > 0.0 ? (float)(s / tot * (double)a.scale) : 0.0f;
+        a.w[t * a.slots() + rank] = (float)(s * reciprocal_f64(tot) * (double)a.scale);
     }
     // the tokens that are left, by the whole wave
     const uint64_t left = __ballot(unsure && t < a.tokens);
@@ -579,18 +608,28 @@ __global__ void __launch_bounds__(256) select_rows_kernel(SelectArgs a)
             wave_sync();
             select_token<LT, (N + 3) / 4>(a, t0 + q, lane, s_g[wave].token);
         }
-    if (a.shared_id >= 0)
+    if constexpr (GATE) {
         for (int q = 0; q < 4 && t0 + q < a.tokens; q++) write_shared(a, t0 + q, lane);
+    } else if (a.shared_id >= 0 && sub == 0 && t < a.tokens) {
+        a.ids[t * a.slots() + a.k] = (int32_t)a.shared_id;
+        a.w[t * a.slots() + a.k] = 1.0f;
+    }
+}
+
+template <int LT, int N, bool GROUPS>
+void launch_rows(const SelectArgs& a, hipStream_t st)
+{
+    const dim3 grid((unsigned)((a.tokens + 15) / 16)), block(256);
+    if (a.shared_id >= 0 && a.gate)
+        hipLaunchKernelGGL((select_rows_kernel<LT, N, GROUPS, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((select_rows_kernel<LT, N, GROUPS, false>), grid, block, 0, st, a);
 }
 
 template <int LT, int N>
 void launch_rows(const SelectArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.tokens + 15) / 16)), block(256);
-    if (a.n_groups > 1)
-        hipLaunchKernelGGL((select_rows_kernel<LT, N, true>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((select_rows_kernel<LT, N, false>), grid, block, 0, st, a);
+    return a.n_groups > 1 ? launch_rows<LT, N, true>(a, st) : launch_rows<LT, N, false>(a, st);
 }
 
 template <int LT>
