@@ -31,7 +31,7 @@
 //            slices (the units of a workgroup) left histograms; each workgroup
 //            adds them up to the bin that the border lies in, and lists its
 //            slice's entries of that bin.
-//   finish   One workgroup a row, on the list in LDS: up to 256 entries are
+//   finish   One workgroup a row, on the list in LDS: up to 128 entries are
 //            ranked directly, more are narrowed down by a histogram (in the
 //            order of logits for a border, of columns for the draw).
 // A draw without a border (no top-k, top-p or min-p) is stats and finish: the
@@ -53,10 +53,11 @@ constexpr int MAX_UNITS = 1024;   // units of a row
 constexpr int MAX_GROUPS = 8192;  // groups of a row (Plan::fine)
 constexpr int LIST = 3072;        // entries of the list in LDS
 constexpr int SHORT_LIST = 8192;  // entries of the slices without a histogram
-constexpr int DIRECT = 256;       // entries that are ranked directly
+constexpr int DIRECT = 128;       // entries that are ranked directly
+constexpr int PARTS = NT / DIRECT;  // threads an entry then
 constexpr int BINS = 256;         // of a slice's histogram
 constexpr double UNIT = 4398046511104.0;  // 2^42: a weight of 1
-static_assert(NT == 1 << BITS && NT == 2 * DIRECT && NT >= MAX_UNITS / 2, "a thread a range, two an entry, for two units");
+static_assert(NT == 1 << BITS && NT >= MAX_UNITS / 2, "a thread a range and for two units");
 
 // What the collect launch leaves of a row.
 struct RowInfo {
@@ -816,50 +817,60 @@ __device__ __forceinline__ void write_token(const SampleArgs& a, int b, int colu
 }
 
 // Up to DIRECT entries: each one's rank and the weight ahead of it, and the
-// kept weight of lower columns, by comparing it with every other, half of
-// them by each half of the workgroup.
+// kept weight of lower columns, by comparing it with every other, a part of
+// them by each of its threads.  (The comparisons are what it costs: 250 entries
+// took 5 us of them, two histograms 4.)
 __device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
                                               int n, double z, int b)
 {
-    const int tid = threadIdx.x, i = tid & (DIRECT - 1), half = tid / DIRECT;
-    const int j0 = half ? n / 2 : 0, j1 = half ? n : n / 2;
+    const int tid = threadIdx.x, i = tid & (DIRECT - 1), part = tid / DIRECT;
+    const int j0 = part * n / PARTS, j1 = (part + 1) * n / PARTS;
     const uint64_t key = i < n ? sh.list[i] : 0, mass = i < n ? sh.mass[i] : 0;
     uint32_t rank = 0;
     uint64_t before = 0;
+    if (i - (tid & 63) < n)  // (waves without an entry)
 #pragma unroll 8
-    for (int j = j0; j < j1; j++) {
-        const bool ahead = sh.list[j] > key;
-        rank += ahead;
-        before += ahead ? sh.mass[j] : 0;
-    }
+        for (int j = j0; j < j1; j++) {
+            const bool ahead = sh.list[j] > key;
+            rank += ahead;
+            before += ahead ? sh.mass[j] : 0;
+        }
     sh.order[tid] = before;
     sh.count[tid] = rank;
     __syncthreads();
-    rank += sh.count[tid ^ DIRECT];
-    before += sh.order[tid ^ DIRECT];
+    rank = 0;
+    before = 0;
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) {
+        rank += sh.count[p * DIRECT + i];
+        before += sh.order[p * DIRECT + i];
+    }
     bool stays = i < n && (s.k == 0 || rank < s.k);
     uint64_t total;
     if (s.top_p_on) {
         double all = z * UNIT;
         if (s.k > 0) {
-            block_scan(sh.scratch, half == 0 && stays ? mass : 0, total);
+            block_scan(sh.scratch, part == 0 && stays ? mass : 0, total);
             all = (double)total;
         }
         stays = stays && (rank == 0 || (double)before < s.p * all);
     }
     if (s.min_p_on) stays = stays && weigh(key_logit(key)) >= s.min_p;
     const uint64_t kept = stays ? mass : 0;
-    if (half == 0) sh.amount[i] = kept;
-    block_scan(sh.scratch, half == 0 ? kept : 0, total);  // (its barriers are amount's as well)
+    if (part == 0) sh.amount[i] = kept;
+    block_scan(sh.scratch, part == 0 ? kept : 0, total);  // (its barriers are amount's and order's as well)
     const uint64_t limit = draw_limit(a, b, total);
     uint64_t run = 0;
     const uint32_t col = ~(uint32_t)key;
+    if (i - (tid & 63) < n)
 #pragma unroll 8
-    for (int j = j0; j < j1; j++) run += ~(uint32_t)sh.list[j] < col ? sh.amount[j] : 0;
+        for (int j = j0; j < j1; j++) run += ~(uint32_t)sh.list[j] < col ? sh.amount[j] : 0;
     sh.order[tid] = run;
     __syncthreads();
-    run += sh.order[tid ^ DIRECT];
-    if (half == 0 && kept && run < limit && run + kept >= limit)
+    if (part > 0) return;
+#pragma unroll
+    for (int p = 1; p < PARTS; p++) run += sh.order[p * DIRECT + i];
+    if (kept && run < limit && run + kept >= limit)
         write_token(a, b, key_column(key), key_logit(key), weigh, (double)total / UNIT);
 }
 
