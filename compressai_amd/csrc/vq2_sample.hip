@@ -150,7 +150,6 @@ struct Row {
           full(a.vocab / VEC)
     {
     }
-    __device__ __forceinline__ float at(int column) const { return finite(ld_t<LT>(p, column)); }
     __device__ __forceinline__ u32x4 raw(int block) const { return *(const u32x4_any*)(p + (int64_t)block * 16); }
     static __device__ __forceinline__ void values(u32x4 w, float (&v)[VEC])
     {
@@ -370,8 +369,9 @@ __device__ __forceinline__ Units read_units(Scratch& sh, const SampleArgs& a, co
     r.max = block_max(sh, fmaxf(r.um[0], r.um[1]));
     r.z = 0.0;
     if (s.whole_sum()) {
+        if (2 * (threadIdx.x & ~63u) < (uint32_t)a.units)  // (not for waves without units)
 #pragma unroll
-        for (int i = 0; i < 2; i++) r.us[i] *= exp2_f64(((double)r.um[i] - (double)r.max) * s.c);
+            for (int i = 0; i < 2; i++) r.us[i] *= exp2_f64(((double)r.um[i] - (double)r.max) * s.c);
         const double w = wave_sum_f64(r.us[0] + r.us[1]);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) sh.wave_d[threadIdx.x >> 6] = w;
@@ -483,19 +483,33 @@ struct Stage {
     uint32_t n, base;
 };
 
-// Puts the `in` entries of this lane's block into the stage (those past its
-// end are counted only).
-template <int VEC>
-__device__ __forceinline__ void stage_block(Stage& st, uint32_t in, int block, const float (&v)[VEC])
+// Puts the entries of this block that pass `in` into the stage (those past its
+// end are counted only): the wave counts them by ballots and takes their places
+// at once.
+template <int VEC, class F>
+__device__ __forceinline__ void stage_block(Stage& st, int block, const float (&v)[VEC], F in)
 {
-    if (in == 0) return;
-    uint32_t at = atomicAdd(&st.n, (uint32_t)__popc(in));
+    uint64_t pass[VEC];
+    uint32_t total = 0;
 #pragma unroll
-    for (int j = 0; j < VEC; j++)
-        if (in >> j & 1) {
-            if (at < LIST) st.entry[at] = order_key(v[j], block * VEC + j);
-            at++;
-        }
+    for (int j = 0; j < VEC; j++) {
+        pass[j] = __ballot(in(v[j]));
+        total += (uint32_t)__popcll(pass[j]);
+    }
+    if (total == 0) return;
+    const uint64_t active = __ballot(true);
+    uint32_t at = 0;
+    if (__builtin_amdgcn_mbcnt_hi((uint32_t)(active >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)active, 0)) == 0)
+        at = atomicAdd(&st.n, total);
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+        if (pass[j] == 0) continue;
+        const uint32_t to =
+            at + __builtin_amdgcn_mbcnt_hi((uint32_t)(pass[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)pass[j], 0));
+        if (in(v[j]) && to < LIST) st.entry[to] = order_key(v[j], block * VEC + j);
+        at += (uint32_t)__popcll(pass[j]);
+    }
 }
 
 // Appends the stage to a list of `cap` entries; the list's counter counts
@@ -577,7 +591,15 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
             if (r >= 0 && bin.inv > 0.0f) cut = fmaxf(cut, un.max - (float)(r + 2) / bin.inv);
         }
     }
-    if (s.min_p_on && !(s.k > 0 && s.top_p_on)) cut = fmaxf(cut, min_p_border(s, Weigher{un.max, s.c}));
+    if (s.min_p_on && !(s.k > 0 && s.top_p_on)) {
+        __syncthreads();
+        if (tid < 64) {
+            const float at = min_p_border(s, Weigher{un.max, s.c});
+            if (tid == 0) sh.scratch.wave_d[0] = (double)at;
+        }
+        __syncthreads();
+        cut = fmaxf(cut, (float)sh.scratch.wave_d[0]);
+    }
     return cut;
 }
 
@@ -599,10 +621,10 @@ __global__ void __launch_bounds__(NT) sample_collect_kernel(SampleArgs a)
     if (tid == 0) sh.stage.n = 0;
     __syncthreads();
     row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
-        uint32_t in = 0;
+        float top = v[0];
 #pragma unroll
-        for (int j = 0; j < VEC; j++) in |= (uint32_t)(v[j] >= cut) << j;
-        stage_block<VEC>(sh.stage, in, i, v);
+        for (int j = 1; j < VEC; j++) top = fmaxf(top, v[j]);
+        if (__ballot(top >= cut)) stage_block<VEC>(sh.stage, i, v, [&](float l) { return l >= cut; });
     });
     __syncthreads();
     const uint32_t n = sh.stage.n;
@@ -703,10 +725,7 @@ __global__ void __launch_bounds__(NT) sample_refine_kernel(SampleArgs a)
     const Row<LT> row(a, b);
     const int from = (blockIdx.x * NW + (tid >> 6)) * a.unit_blocks, end = min(row.blocks, from + a.unit_blocks);
     row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
-        uint32_t in = 0;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) in |= (uint32_t)(v[j] >= info.cut && bin(v[j]) == r) << j;
-        stage_block<VEC>(sh.stage, in, i, v);
+        stage_block<VEC>(sh.stage, i, v, [&](float l) { return l >= info.cut && bin(l) == r; });
     });
     flush_stage(sh.stage, a.counters + b * CNTS + CNT_BIN, a.list + (int64_t)b * a.list_cap, a.list_cap);
 }
@@ -998,14 +1017,18 @@ __device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Sett
     uint64_t run = before + block_scan(sh.scratch, part, all);
     if (!(run >= limit && run - part < limit)) return true;
     run -= part;
-    for (int c = i0 * VEC; c < min(a.vocab, i1 * VEC); c++) {
-        const float l = row.at(c);
-        run += kept(l, c);
-        if (run >= limit) {
-            write_token(a, b, c, l, weigh, (double)total / UNIT);
-            break;
-        }
-    }
+    int col = 0;
+    float l = weigh.max;
+    row.stream(i0, i1, 1, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+            if (run < limit) {
+                run += kept(v[j], i * VEC + j);
+                col = i * VEC + j;
+                l = v[j];
+            }
+    });
+    write_token(a, b, col, finite(l), weigh, (double)total / UNIT);
     return true;
 }
 
@@ -1111,14 +1134,18 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
     uint64_t run = before + block_scan(sh.scratch, mine, all);
     if (!(run >= limit && run - mine < limit)) return;
     run -= mine;
-    for (int c = i0 * VEC; c < min(a.vocab, i1 * VEC); c++) {
-        const float l = row.at(c);
-        run += kept(l, c, true);
-        if (run >= limit) {
-            write_token(a, b, c, l, weigh, (double)total / UNIT);
-            break;
-        }
-    }
+    int col = 0;
+    float l = weigh.max;
+    row.stream(i0, i1, 1, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+            if (run < limit) {
+                run += kept(v[j], i * VEC + j, true);
+                col = i * VEC + j;
+                l = v[j];
+            }
+    });
+    write_token(a, b, col, finite(l), weigh, (double)total / UNIT);
 }
 
 // A draw over the whole row: the unit, then the column, whose running sum is
@@ -1166,16 +1193,19 @@ __device__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weighe
     if (tid != locate(mine, base, target, before)) return;
     int col = -1;
     float l = weigh.max;
-    for (int c = i0 * VEC; c < min(a.vocab, i1 * VEC) && (col < 0 || !(before > target)); c++) {
-        const float v = row.at(c);
-        const double w = weigh(v);
-        before += w;
-        if (w > 0.0) {
-            col = c;
-            l = v;
+    row.stream(i0, i1, 1, [&](int i, const float (&v)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            if (col >= 0 && before > target) continue;
+            const double w = weigh(v[j]);
+            before += w;
+            if (w > 0.0) {
+                col = i * VEC + j;
+                l = v[j];
+            }
         }
-    }
-    write_token(a, b, col, l, weigh, un.z);
+    });
+    write_token(a, b, col, finite(l), weigh, un.z);
 }
 
 template <int LT>
