@@ -385,19 +385,29 @@ __device__ __forceinline__ Units read_units(Scratch& sh, const SampleArgs& a, co
 // ------------------------------------------------------------------- stats
 // The sum over a whole row is an exponential of 64 bits an entry, and those,
 // not memory, bound this launch.  2^(j / 1024) comes from a table in LDS, which
-// leaves f in [-2^-11, 2^-11]: 2^f = 1 + f (ln 2 + f ln^2 2 / 2), off by 7e-12
-// at its ends (odd in f, so that it averages out of a sum), in 11 operations
-// of 64 bits and a lookup instead of 17.
+// leaves f in [-1/2, 1/2] of a step: 2^(f / 1024) = 1 + f (K + f K^2 / 2), K =
+// ln 2 / 1024, off by 7e-12 at its ends (odd in f, so that it averages out of a
+// sum).  The table's upper words lack j << 10, so that n << 10 (n in steps, j its
+// lower bits) makes index and exponent right at once.  7 operations of 64
+// bits and a lookup, against 16 of exp2_f64.
 constexpr int TABLE = 1024;
-__device__ __forceinline__ double exp2_table(const double* table, double y)  // |y| <= 1000
+__device__ __forceinline__ double table_entry(int j)
 {
-    constexpr double MAGIC = 6755399441055744.0 / TABLE;  // rounds to a whole number of 1 / TABLE
-    const double t = y + MAGIC;
-    const double f = y - (t - MAGIC);
-    const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-    const double r = table[n & (TABLE - 1)];
-    const double g = fma(0.2402265069591007, f, 0.6931471805599453) * f;
-    return __builtin_amdgcn_ldexp(fma(r, g, r), n >> 10);
+    const uint64_t b = __builtin_bit_cast(uint64_t, exp2_f64_in((double)j / TABLE));
+    return __builtin_bit_cast(double, b - ((uint64_t)(uint32_t)j << 42));
+}
+// 2^(d * steps / 1024), |d * steps| < 2^20
+__device__ __forceinline__ double exp2_table(const double* table, double d, double steps)
+{
+    constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    constexpr double K = 0.0006769015435155716;
+    const double t = fma(d, steps, MAGIC);
+    const double f = fma(d, steps, MAGIC - t);
+    const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
+    const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (TABLE - 1)]);
+    const uint32_t hi = (uint32_t)(e >> 32) + (n << 10);
+    const double r = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)e);
+    return fma(r, fma(f, K * K / 2, K) * f, r);
 }
 
 template <int LT>
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
     const u32x4 head = row.head(from, end);
     const Setting s(a, b);
     if (s.whole_sum()) {
-        for (int i = tid; i < TABLE; i += NT) table[i] = exp2_f64_in((double)i / TABLE);
+        for (int i = tid; i < TABLE; i += NT) table[i] = table_entry(i);
         __syncthreads();
     }
     if (unit >= a.units) return;
@@ -421,29 +431,46 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
     double sum = 0.0;
     if (s.whole_sum()) {
         // sum of exp((l - ref) / temperature), ref one of the lane's logits:
-        // 64 bits hold weights of 2^1000, so it moves only where one is close.
-        // Logits are raised to `least`, whose weight is 2^-990 (absent ones
-        // too: the median of the three is the one that is no NaN); where fp32
-        // has no such number (huge logits, huge temperatures) it is -inf.
-        float ref = -INFINITY, least = -INFINITY;
+        // 64 bits hold weights of 2^1000, so it moves only where one is close,
+        // past `high`.  Differences are held above -990 / c, whose weight is
+        // nothing, by a median, which drops NaN as well as -inf: of 16-bit
+        // logits in 32 bits, exact but for logits 2^-13 of ref and below; of
+        // 32-bit ones before the difference in 64.  `quick` is whether fp32
+        // has that bound (it does but for huge logits and temperatures).
+        const double steps = s.c * TABLE;
+        const float span = (float)fmin(900.0 / s.c, (double)FLT_MAX), lim = (float)fmin(990.0 / s.c, (double)FLT_MAX);
+        float ref = -INFINITY, high = -INFINITY, least = -INFINITY;
+        bool quick = false;
         row.stream(from, end, 64, head, [&](int, const float (&v)[VEC]) {
             float top = v[0];
 #pragma unroll
             for (int j = 1; j < VEC; j++) top = fmaxf(top, v[j]);
             top = finite(top);
             m = fmaxf(m, top);
-            if (((double)top - (double)ref) * s.c > 900.0) {
+            if (top > high) {
                 sum *= exp2_f64(((double)ref - (double)top) * s.c);
                 ref = top;
-                least = (float)fmax((double)ref - 990.0 / s.c, (double)-FLT_MAX);
-                if (fabs(((double)ref - (double)least) * s.c - 990.0) > 5.0) least = -INFINITY;
+                high = (float)fmin((double)ref + (double)span, (double)FLT_MAX);
+                least = (float)fmax((double)ref - (double)lim, (double)-FLT_MAX);
+                quick = LT == VQ2_DT_F32 ? fabs(((double)ref - (double)least) * s.c - 990.0) < 5.0 : lim < 1e37f && ref < FLT_MAX;
+                // (a bound that rounds past what 64 bits hold)
+                quick = quick && ((double)high - (double)ref) * s.c < 1000.0;
             }
-            if (least > -INFINITY) {
+            if (quick) {
 #pragma unroll
-                for (int j = 0; j < VEC; j++)
-                    sum += exp2_table(table, ((double)__builtin_amdgcn_fmed3f(v[j], least, FLT_MAX) - (double)ref) * s.c);
+                for (int j = 0; j < VEC; j++) {
+                    double d;
+                    if constexpr (LT == VQ2_DT_F32)
+                        d = (double)__builtin_amdgcn_fmed3f(v[j], least, FLT_MAX) - (double)ref;
+                    else
+                        d = (double)__builtin_amdgcn_fmed3f(v[j] - ref, -lim, lim);
+                    sum += exp2_table(table, d, steps);
+                }
             } else {
-                for (int j = 0; j < VEC; j++) sum += exp2_f64(((double)finite(v[j]) - (double)ref) * s.c);
+                for (int j = 0; j < VEC; j++) {
+                    const double y = ((double)finite(v[j]) - (double)ref) * s.c;
+                    sum += exp2_f64(y > 1000.0 ? 1000.0 : y);  // (NaN stays: 2^-1000)
+                }
             }
         });
         const float um = wave_max_all(m);
@@ -604,7 +631,7 @@ __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setti
 }
 
 template <int LT>
-__global__ void __launch_bounds__(NT) sample_collect_kernel(SampleArgs a)
+__global__ void __launch_bounds__(NT, 8) sample_collect_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
     __shared__ CollectShared sh;
@@ -674,7 +701,7 @@ struct RefineShared {
 };
 
 template <int LT>
-__global__ void __launch_bounds__(NT) sample_refine_kernel(SampleArgs a)
+__global__ void __launch_bounds__(NT, 8) sample_refine_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
     __shared__ RefineShared sh;
