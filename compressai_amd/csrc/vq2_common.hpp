@@ -84,9 +84,9 @@ __device__ __forceinline__ double exp2_f64_in(double y)
     g = fma(g, f, 0.055504108664760424);
     g = fma(g, f, 0.2402265069581299);
     g = fma(g, f, 0.6931471805599453);
-    const uint64_t p = __builtin_bit_cast(uint64_t, fma(g, f, 1.0));
-    const uint32_t hi = (uint32_t)(p >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)p);
+    u32x2 p = __builtin_bit_cast(u32x2, fma(g, f, 1.0));
+    p.y += (uint32_t)__builtin_bit_cast(uint64_t, t) << 20;
+    return __builtin_bit_cast(double, p);
 }
 // any y < 1023; below -1000, or NaN: 2^-1000
 __device__ __forceinline__ double exp2_f64(double y) { return exp2_f64_in(fmax(y, -1000.0)); }

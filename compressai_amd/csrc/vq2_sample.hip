@@ -404,9 +404,9 @@ __device__ __forceinline__ double exp2_table(const double* table, double d, doub
     const double t = fma(d, steps, MAGIC);
     const double f = fma(d, steps, MAGIC - t);
     const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, t);
-    const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (TABLE - 1)]);
-    const uint32_t hi = (uint32_t)(e >> 32) + (n << 10);
-    const double r = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)e);
+    u32x2 e = __builtin_bit_cast(u32x2, table[n & (TABLE - 1)]);
+    e.y += n << 10;
+    const double r = __builtin_bit_cast(double, e);
     return fma(r, fma(f, K * K / 2, K) * f, r);
 }
 
