@@ -705,7 +705,7 @@ __global__ void __launch_bounds__(NT, 8) sample_refine_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
     __shared__ RefineShared sh;
-    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, slices = gridDim.x;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, slices = a.slices();
     const uint32_t n_long = a.counters[b * CNTS + CNT_LONG], n_short = a.counters[b * CNTS + CNT_SHORT];
     if (n_long + n_short <= LIST) return;
     const Setting s(a, b);
@@ -717,7 +717,6 @@ __global__ void __launch_bounds__(NT, 8) sample_refine_kernel(SampleArgs a)
     const int64_t slice0 = (int64_t)b * slices;
     sh.amount[tid] = 0;
     sh.count[tid] = 0;
-    if (tid == 0) sh.stage.n = 0;
     __syncthreads();
     {
         uint64_t am = 0;
@@ -743,18 +742,23 @@ __global__ void __launch_bounds__(NT, 8) sample_refine_kernel(SampleArgs a)
     uint64_t before = 0;
     const int r = block_locate(sh.scratch, amount, limit, before);
     if (blockIdx.x == 0 && tid == 0) a.refined[b] = RefineInfo{before, r};
-    if (a.slice_n[slice0 + blockIdx.x] <= a.short_slice()) return;
-    // this slice's weight ahead of the bin, and its entries of the bin
-    uint64_t ahead = tid < BINS && (r < 0 || tid < r) ? a.bin_amount[(slice0 + blockIdx.x) * BINS + tid] : 0, all;
-    block_scan(sh.scratch, ahead, all);
-    if (tid == 0) a.slice_mass[slice0 + blockIdx.x] = all;
-    if (r < 0) return;
     const Row<LT> row(a, b);
-    const int from = (blockIdx.x * NW + (tid >> 6)) * a.unit_blocks, end = min(row.blocks, from + a.unit_blocks);
-    row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
-        stage_block<VEC>(sh.stage, i, v, [&](float l) { return l >= info.cut && bin(l) == r; });
-    });
-    flush_stage(sh.stage, a.counters + b * CNTS + CNT_BIN, a.list + (int64_t)b * a.list_cap, a.list_cap);
+    for (int g = blockIdx.x; g < slices; g += gridDim.x) {
+        if (a.slice_n[slice0 + g] <= a.short_slice()) continue;
+        // the slice's weight ahead of the bin, and its entries of the bin
+        const uint64_t ahead = tid < BINS && (r < 0 || tid < r) ? a.bin_amount[(slice0 + g) * BINS + tid] : 0;
+        uint64_t all;
+        block_scan(sh.scratch, ahead, all);
+        if (tid == 0) a.slice_mass[slice0 + g] = all;
+        if (r < 0) continue;
+        if (tid == 0) sh.stage.n = 0;
+        __syncthreads();
+        const int from = (g * NW + (tid >> 6)) * a.unit_blocks, end = min(row.blocks, from + a.unit_blocks);
+        row.stream(from + lane, end, 64, [&](int i, const float (&v)[VEC]) {
+            stage_block<VEC>(sh.stage, i, v, [&](float l) { return l >= info.cut && bin(l) == r; });
+        });
+        flush_stage(sh.stage, a.counters + b * CNTS + CNT_BIN, a.list + (int64_t)b * a.list_cap, a.list_cap);
+    }
 }
 
 // ------------------------------------------------------------------ finish
@@ -1367,7 +1371,10 @@ int launch(const SampleCall& c)
     const dim3 grid((unsigned)((p.units + NW - 1) / NW), (unsigned)c.rows), block(NT);
     hipLaunchKernelGGL(sample_stats_kernel<LT>, grid, block, 0, st, a);
     if (listed) hipLaunchKernelGGL(sample_collect_kernel<LT>, grid, block, 0, st, a);
-    if (refine) hipLaunchKernelGGL(sample_refine_kernel<LT>, grid, block, 0, st, a);
+    if (refine) {  // (rows mostly leave at once: no more workgroups than spread a single long row)
+        const unsigned per_row = (unsigned)(c.rows < 512 ? 512 / c.rows : 1);
+        hipLaunchKernelGGL(sample_refine_kernel<LT>, dim3(per_row < grid.x ? per_row : grid.x, grid.y), block, 0, st, a);
+    }
     hipLaunchKernelGGL(sample_finish_kernel<LT>, dim3((unsigned)c.rows), block, 0, st, a);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return set_hip_error(err, "vq2 sample launch");
