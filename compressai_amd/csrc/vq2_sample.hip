@@ -695,6 +695,7 @@ __global__ void __launch_bounds__(NT, 8) sample_collect_kernel(SampleArgs a)
 // ------------------------------------------------------------------ refine
 struct RefineShared {
     Scratch scratch;
+    uint32_t is_long[MAX_UNITS / NW];
     Stage stage;
     uint64_t amount[NT];
     uint32_t count[NT];
@@ -713,22 +714,34 @@ __global__ void __launch_bounds__(NT, 8) sample_refine_kernel(SampleArgs a)
     const RowInfo info = a.info[b];
     const Weigher weigh{info.max, s.c};
     const Binner bin(info.max, info.cut, BINS);
-    // the row's histogram: two threads a bin, then the short slices' entries
+    // the row's histogram: two bins a thread of every fourth slice, eight
+    // slices' loads in flight, then the short slices' entries
     const int64_t slice0 = (int64_t)b * slices;
     sh.amount[tid] = 0;
     sh.count[tid] = 0;
+    if (tid < slices) sh.is_long[tid] = a.slice_n[slice0 + tid] > a.short_slice();
     __syncthreads();
     {
-        uint64_t am = 0;
-        uint32_t ct = 0;
-#pragma unroll 4
-        for (int g = tid / BINS; g < slices; g += NT / BINS)
-            if (a.slice_n[slice0 + g] > a.short_slice()) {
-                am += a.bin_amount[(slice0 + g) * BINS + tid % BINS];
-                ct += a.bin_count[(slice0 + g) * BINS + tid % BINS];
-            }
-        atomicAdd((unsigned long long*)&sh.amount[tid % BINS], (unsigned long long)am);
-        atomicAdd(&sh.count[tid % BINS], ct);
+        constexpr int PAIRS = BINS / 2;
+        const int pair = tid % PAIRS;
+        uint64_t am[2] = {};
+        uint32_t ct[2] = {};
+#pragma unroll 8
+        for (int g = tid / PAIRS; g < slices; g += NT / PAIRS) {
+            // (a short slice's, which nothing wrote, are loaded and dropped: no branch keeps the loads apart)
+            const ulonglong2 x = ((const ulonglong2*)a.bin_amount)[(slice0 + g) * PAIRS + pair];
+            const uint2 y = ((const uint2*)a.bin_count)[(slice0 + g) * PAIRS + pair];
+            const bool is_long = sh.is_long[g] != 0;
+            am[0] += is_long ? x.x : 0;
+            am[1] += is_long ? x.y : 0;
+            ct[0] += is_long ? y.x : 0;
+            ct[1] += is_long ? y.y : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            atomicAdd((unsigned long long*)&sh.amount[2 * pair + i], (unsigned long long)am[i]);
+            atomicAdd(&sh.count[2 * pair + i], ct[i]);
+        }
         for (uint32_t i = tid; i < min(n_short, (uint32_t)a.short_cap); i += NT) {
             const float l = key_logit(a.short_list[(int64_t)b * a.short_cap + i]);
             atomicAdd((unsigned long long*)&sh.amount[bin(l)], (unsigned long long)fixed(weigh(l)));
