@@ -452,9 +452,8 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
                 ref = top;
                 high = (float)fmin((double)ref + (double)span, (double)FLT_MAX);
                 least = (float)fmax((double)ref - (double)lim, (double)-FLT_MAX);
+                if (((double)high - (double)ref) * s.c > 1000.0) high = ref;  // (rounded past what 64 bits hold)
                 quick = LT == VQ2_DT_F32 ? fabs(((double)ref - (double)least) * s.c - 990.0) < 5.0 : lim < 1e37f && ref < FLT_MAX;
-                // (a bound that rounds past what 64 bits hold)
-                quick = quick && ((double)high - (double)ref) * s.c < 1000.0;
             }
             if (quick) {
 #pragma unroll
