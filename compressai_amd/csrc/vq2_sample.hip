@@ -136,8 +136,8 @@ struct Setting {
 // alignment of its elements; the last block may be short.
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
-// An infinite logit counts as the largest finite one (no difference of
-// infinities); NaN stays.
+// An infinite logit as the largest finite one, for what takes no infinity; NaN
+// stays.
 __device__ __forceinline__ float finite(float v) { return v == INFINITY ? FLT_MAX : v; }
 
 template <int LT>
@@ -195,7 +195,7 @@ struct Row {
 // Order of a row's entries: larger is earlier.
 __device__ __forceinline__ uint64_t order_key(float l, int i)
 {
-    return argmax_key(finite(l) + 0.0f, i);  // (+ 0: -0 is 0)
+    return argmax_key(l + 0.0f, i);  // (+ 0: -0 is 0)
 }
 __device__ __forceinline__ float key_logit(uint64_t key)
 {
@@ -206,13 +206,16 @@ __device__ __forceinline__ int key_column(uint64_t key) { return (int)(0xFFFFFFF
 
 __device__ __forceinline__ uint64_t fixed(double w) { return (uint64_t)(w * UNIT + 0.5); }
 
-// A row's weights of 64 bits.
+// A row's weights of 64 bits.  The maximum weighs 1, also an infinite one (no
+// difference of infinities), beside which every finite logit weighs nothing.
 struct Weigher {
     float max;
     double c;
+    // log2 of the weight
+    __device__ __forceinline__ double log2_of(float l) const { return l == max ? 0.0 : ((double)l - (double)max) * c; }
     __device__ __forceinline__ double operator()(float l) const
     {
-        const double d = ((double)finite(l) - (double)max) * c;
+        const double d = log2_of(l);
         return d > -999.0 ? exp2_f64_in(d) : 0.0;  // (NaN: 0)
     }
 };
@@ -222,7 +225,7 @@ struct Weigher {
 struct Binner {
     float max, inv;
     int n;
-    __device__ __forceinline__ Binner(float max_, float cut, int n_) : max(max_), n(n_)
+    __device__ __forceinline__ Binner(float max_, float cut, int n_) : max(finite(max_)), n(n_)
     {
         const float width = max - cut;
         inv = width > 0.0f && width < INFINITY ? (float)n / width : 0.0f;
@@ -371,7 +374,7 @@ __device__ __forceinline__ Units read_units(Scratch& sh, const SampleArgs& a, co
     if (s.whole_sum()) {
         if (2 * (threadIdx.x & ~63u) < (uint32_t)a.units)  // (not for waves without units)
 #pragma unroll
-            for (int i = 0; i < 2; i++) r.us[i] *= exp2_f64(((double)r.um[i] - (double)r.max) * s.c);
+            for (int i = 0; i < 2; i++) r.us[i] *= Weigher{r.max, s.c}(r.um[i]);  // (0: none of its entries weighs)
         const double w = wave_sum_f64(r.us[0] + r.us[1]);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) sh.wave_d[threadIdx.x >> 6] = w;
@@ -445,8 +448,8 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
             float top = v[0];
 #pragma unroll
             for (int j = 1; j < VEC; j++) top = fmaxf(top, v[j]);
-            top = finite(top);
             m = fmaxf(m, top);
+            top = finite(top);
             if (top > high) {
                 sum *= exp2_f64(((double)ref - (double)top) * s.c);
                 ref = top;
@@ -473,13 +476,20 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
             }
         });
         const float um = wave_max_all(m);
-        sum = wave_sum_f64(sum * exp2_f64(((double)ref - (double)um) * s.c));
+        sum *= exp2_f64(((double)ref - (double)um) * s.c);
+        if (um == INFINITY) {  // (the infinite ones count, and nothing else)
+            sum = 0.0;
+            row.stream(from, end, 64, [&](int, const float (&v)[VEC]) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) sum += v[j] == INFINITY ? 1.0 : 0.0;
+            });
+        }
+        sum = wave_sum_f64(sum);
     } else {
         row.stream(from, end, 64, head, [&](int, const float (&v)[VEC]) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) m = fmaxf(m, v[j]);
         });
-        m = finite(m);
     }
     const int64_t at = (int64_t)b * a.units + unit;
     if (s.k > 1) {
@@ -582,6 +592,7 @@ struct CollectShared {
 __device__ float lowest_kept(CollectShared& sh, const SampleArgs& a, const Setting& s, const Units& un, int b)
 {
     const int tid = threadIdx.x;
+    if (un.max == INFINITY) return un.max;  // (no finite logit weighs anything)
     const double m = (double)un.max;
     // (the logarithm of 32 bits is off by less than 0.001)
     double bits = -45.0;
@@ -875,7 +886,7 @@ __device__ __forceinline__ void write_token(const SampleArgs& a, int b, int colu
                                             double total)
 {
     a.out_idx[b] = column;
-    a.out_logprob[b] = (float)(((double)l - (double)weigh.max) * weigh.c / LOG2E_F64 - log(total));
+    a.out_logprob[b] = (float)(weigh.log2_of(l) / LOG2E_F64 - log(total));
 }
 
 // Up to DIRECT entries: each one's rank and the weight ahead of it, and the
@@ -1071,7 +1082,7 @@ __device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Sett
                 l = v[j];
             }
     });
-    write_token(a, b, col, finite(l), weigh, (double)total / UNIT);
+    write_token(a, b, col, l, weigh, (double)total / UNIT);
     return true;
 }
 
@@ -1188,7 +1199,7 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
                 l = v[j];
             }
     });
-    write_token(a, b, col, finite(l), weigh, (double)total / UNIT);
+    write_token(a, b, col, l, weigh, (double)total / UNIT);
 }
 
 // A draw over the whole row: the unit, then the column, whose running sum is
@@ -1248,7 +1259,7 @@ __device__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weighe
             }
         }
     });
-    write_token(a, b, col, finite(l), weigh, un.z);
+    write_token(a, b, col, l, weigh, un.z);
 }
 
 template <int LT>
@@ -1275,7 +1286,7 @@ __global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
                        [&](int i, const float (&v)[VEC]) {
 #pragma unroll
                            for (int j = VEC - 1; j >= 0; j--)
-                               if (finite(v[j]) == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
+                               if (v[j] == un.max && (uint64_t)(i * VEC + j) < col) col = (uint64_t)(i * VEC + j);
                        });
             col = block_min(sh.scratch, col);
             if (tid == 0) {

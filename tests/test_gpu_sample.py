@@ -218,3 +218,115 @@ def test_head_sample(dev):
             got = head.sample(h, u, **kw)
             _check(got, logits, u, **kw)
         assert torch.equal(head.sample(h, u, temperature=0.0)[0], logits.argmax(-1))
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-9, 1e-30, 1e-44, 1e6, 1e30, float("inf")])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_extreme_temperatures(dev, dtype, temperature):
+    """Differences of logits times 1 / temperature leave the range of 64-bit
+    weights (one entry counts) or vanish in it (all count alike); logits near
+    one another, near zero and huge.  (An infinite
+    temperature counts as the largest finite one.  Beside an infinite logit
+    every finite one weighs nothing, however high the temperature.)"""
+    g = synth.gen(8900)
+    x = torch.randn(8, 5000, generator=g)
+    x[1] = 16.0 + 1e-6 * x[1]
+    x[2] *= 1e-20
+    x[3] *= 1e4
+    x[4, ::2] = -float("inf")
+    x[5, 4000] = float("inf")
+    x[6] = -60000.0
+    x = x.to(DT[dtype])
+    u = torch.rand(8, generator=g)
+    t = torch.tensor(min(temperature, torch.finfo(torch.float32).max), dtype=torch.float32)
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.7), dict(min_p=0.2), dict(top_k=4000, top_p=0.5, min_p=0.01)):
+        _check(K.vq_sample(x.to(dev), u.to(dev), temperature=temperature, **kw), x, u, temperature=t, **kw)
+
+
+@pytest.mark.parametrize("order", ["descending", "ascending"])
+@pytest.mark.parametrize("kw", [dict(top_k=50), dict(top_p=0.95), dict(min_p=0.001), dict(top_k=2500), dict()], ids=str)
+def test_sorted_vocabularies(dev, order, kw):
+    """Vocabularies sorted by frequency: the likely tokens stand side by
+    side, in the first or the last slice of the row alone."""
+    x, _ = torch.sort(_logits(8950, 3, 100003, "fp32", 1.3), dim=-1, descending=order == "descending")
+    u = torch.tensor([0.01, 0.5, 0.99])
+    _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+def test_offsets_past_32_bits(dev):
+    """Rows more than 2^31 elements apart."""
+    stride, V = (1 << 31) + 8, 3000
+    buf = torch.empty(stride + V + 1, dtype=torch.bfloat16, device=dev)
+    x = _logits(8960, 2, V, "bf16")
+    view = buf.as_strided((2, V), (stride, 1), 1)
+    view.copy_(x.to(dev))
+    u = torch.tensor([0.3, 0.7])
+    for kw in (dict(), dict(top_k=40), dict(top_p=0.9)):
+        _check(K.vq_sample(view, u.to(dev), **kw), x, u, **kw)
+
+
+def test_many_rows(dev):
+    """Rows in the last places of the grid."""
+    B, V = 65535, 24
+    x = _logits(8970, B, V, "bf16")
+    u = torch.rand(B, generator=synth.gen(8971))
+    for kw in (dict(), dict(top_k=5), dict(top_p=0.8)):
+        idx, lp = K.vq_sample(x.to(dev), u.to(dev), **kw)
+        pick = torch.randint(0, B, (300,), generator=synth.gen(8972))
+        pick[:2] = torch.tensor([0, B - 1])
+        _check((idx.cpu()[pick], lp.cpu()[pick]), x[pick], u[pick], **kw)
+    with pytest.raises(K.Vq2Error, match="rows"):
+        K.vq_sample(torch.zeros(65536, 4, device=dev), torch.zeros(65536, device=dev))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=30, top_p=0.9), dict(top_p=0.9)], ids=str)
+def test_native_and_python_entries_agree(dev, kw, monkeypatch):
+    """The native twin and the Python entry: the same launches; a call that the
+    twin declines (numpy settings) is the Python entry's."""
+    from compressai_amd import _lib
+
+    x = _logits(8980, 4, 7001, "fp16").to(dev)
+    u = torch.rand(4, generator=synth.gen(8981)).to(dev)
+    native = _lib.host().sample(x, u, *[kw.get(k, d) for k, d in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))])
+    assert native is not None
+    got = K.vq_sample(x, u, **{k: np.float32(v) if k == "top_p" else v for k, v in kw.items()})
+    assert all(torch.equal(a, b) for a, b in zip(native, got))
+    assert _lib.host().sample(x, u, np.float32(1.0), 0, 1.0, 0.0) is None
+    assert all(torch.equal(a, b) for a, b in zip(K.vq_sample(x, u, temperature=np.float32(1.0)), K.vq_sample(x, u)))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=3), dict(top_p=0.6), dict(min_p=0.5), dict(top_k=5000, top_p=0.7),
+                                dict(temperature=0.0), dict(temperature=3e38)], ids=str)
+def test_infinite_logits(dev, dtype, kw):
+    """+inf next to the type's largest finite logit, several of them, rows of
+    nothing else, and longer than the lists hold."""
+    V = 20000
+    x = torch.randn(6, V, generator=synth.gen(9000)).to(DT[dtype])
+    big = torch.finfo(DT[dtype]).max
+    x[0, 3], x[0, 9] = big, float("inf")
+    x[1, [5, 700, 19999]] = float("inf")
+    x[2, :10] = big
+    x[3] = float("inf")
+    x[4, ::2] = float("inf")
+    x[5] = -float("inf")
+    x[5, 77] = float("inf")
+    for at in (0.0, 0.4, 0.999):
+        u = torch.full((6,), at)
+        _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kw", [dict(), dict(top_p=0.9999), dict(min_p=1e-9)], ids=str)
+def test_units_without_weight(dev, dtype, kw):
+    """u = 0 is the first column with a weight: what is ahead of it lies more
+    than 64-bit weights hold below the maximum (e^-6000 in total)."""
+    V = 30000
+    x = torch.full((3, V), -6000.0)
+    x[0, 20000:] = 0.0
+    x[1, 29999] = 0.0
+    x[2, 15000:] = 1.0
+    x = x.to(DT[dtype])
+    u = torch.zeros(3)
+    _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+    assert K.vq_sample(x.to(dev), u.to(dev), **kw)[0].tolist() == [20000, 29999, 15000]
