@@ -64,7 +64,8 @@ def test_forms(dev, T, E, k, dtype, form):
 @pytest.mark.parametrize("E,G,keep,k,dtype", [
     (256, 8, 4, 8, "bf16"), (160, 8, 3, 6, "fp32"), (64, 64, 6, 6, "fp32"), (48, 3, 1, 16, "fp16"), (512, 16, 16, 10, "bf16"),
     (1024, 4, 2, 32, "bf16"), (63, 9, 2, 3, "fp32"), (72, 8, 1, 9, "fp16"), (1024, 64, 5, 20, "fp32"), (96, 2, 1, 4, "bf16"),
-    (384, 12, 2, 7, "fp32"), (128, 32, 3, 12, "bf16")])
+    (384, 12, 2, 7, "fp32"), (128, 32, 3, 12, "bf16"), (16, 16, 5, 5, "fp32"), (8, 2, 1, 3, "bf16"), (510, 15, 4, 12, "fp32"),
+    (500, 5, 4, 11, "fp16"), (33, 11, 9, 12, "bf16")])
 @pytest.mark.parametrize("group_score", ["max", "top2"])
 def test_groups(dev, E, G, keep, k, dtype, form, group_score):
     _run(dev, 7100 + E + G, 37, E, k, dtype, form, n_groups=G, topk_groups=keep, group_score=group_score)
@@ -212,3 +213,50 @@ def test_agrees_with_the_softmax_router(dev):
     ref_ids, ref_w = K.vq_router_topk(lg, 8)
     assert torch.equal(ids, ref_ids)
     assert torch.allclose(w, ref_w, rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("E,k,G", [(256, 8, 1), (256, 8, 8), (64, 6, 1), (512, 12, 16), (40, 2, 5), (700, 5, 7)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_choices_a_rounding_apart(dev, E, k, G, bias):
+    """Logits that differ in their last bits: which expert is chosen shows in
+    the eighth digit of its choice."""
+    g = synth.gen(7950 + E)
+    lg = 1.0 + torch.randint(0, 40, (50, E), generator=g).float() * 2.0 ** -23
+    lg[25:, ::3] = 0.5
+    kw = dict(scoring="sigmoid", n_groups=G, topk_groups=max(1, G // 2), group_score="top2",
+              bias=torch.randint(0, 3, (E,), generator=g).float().to(dev) * 2.0 ** -20 if bias else None)
+    _check(K.vq_router_select(lg.to(dev), k, **kw), lg, k, **kw)
+    lg16 = (1.0 + torch.randint(0, 4, (50, E), generator=g).float() / 128).to(torch.bfloat16)
+    _check(K.vq_router_select(lg16.to(dev), k, **kw), lg16, k, **kw)
+
+
+def test_offsets_past_32_bits(dev):
+    """Tokens' logits more than 2^31 elements apart."""
+    stride, E = (1 << 31) + 8, 96
+    buf = torch.empty(stride + E + 1, dtype=torch.bfloat16, device=dev)
+    lg = _logits(7960, 2, E, "bf16")
+    view = buf.as_strided((2, E), (stride, 1), 1)
+    view.copy_(lg.to(dev))
+    for k in (5, 20):
+        _check(K.vq_router_select(view, k, scoring="sigmoid"), lg, k, scoring="sigmoid")
+
+
+def test_many_tokens(dev):
+    T, E = 300001, 24
+    lg = _logits(7970, T, E, "bf16").to(dev)
+    bias = (torch.randn(E, generator=synth.gen(7971)) * 0.05).to(dev)
+    ids, w = K.vq_router_select(lg, 3, scoring="sigmoid", bias=bias)
+    pick = torch.randint(0, T, (400,), generator=synth.gen(7972))
+    pick[:2] = torch.tensor([0, T - 1])
+    _check((ids.cpu()[pick], w.cpu()[pick]), lg.cpu()[pick], 3, scoring="sigmoid", bias=bias)
+
+
+def test_native_and_python_entries_agree(dev):
+    """Given outputs take the Python entry, the same launch."""
+    lg = _logits(7980, 90, 256, "fp32").to(dev)
+    h, gate = synth.activations(7981, (90, 512)).to(dev), synth.activations(7982, 512).to(dev)
+    for kw in (dict(), dict(scoring="sigmoid", n_groups=8, topk_groups=2, scale=2.0), dict(h=h, shared_gate=gate, shared_id=256)):
+        slots = 9 if "h" in kw else 8
+        ref = K.vq_router_select(lg, 8, **kw)
+        got = K.vq_router_select(lg, 8, ids=torch.empty(90, slots, dtype=torch.int32, device=dev), **kw)
+        assert all(torch.equal(a, b) for a, b in zip(ref, got))
