@@ -51,7 +51,7 @@ constexpr int BITS = 9;           // NT = 2^BITS
 constexpr int NW = NT / 64;       // its waves, one unit each: a slice
 constexpr int MAX_UNITS = 1024;   // units of a row
 constexpr int MAX_GROUPS = 8192;  // groups of a row (Plan::fine)
-constexpr int LIST = 3072;        // entries of the list in LDS
+constexpr int LIST = 2944;        // entries of the list in LDS
 constexpr int SHORT_LIST = 8192;  // entries of the slices without a histogram
 constexpr int DIRECT = 128;       // entries that are ranked directly
 constexpr int PARTS = NT / DIRECT;  // threads an entry then

@@ -373,8 +373,9 @@ int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t to
  * setting is common to all rows, or given by row on the device (its _rows
  * pointer not NULL; there a temperature, top_k, top_p or min_p outside its
  * range acts as the nearest one inside; NaN: greedy, no top_p, the maxima).
- * Weights are 64-bit and sums whole numbers of 2^-42, so that a result does
- * not depend on the split of a row.  vocab <= VQ2_SAMPLE_MAX_VOCAB, rows <=
+ * Weights are 64-bit; sums over a whole row are too, in an order that the
+ * sizes fix, and those of entries put in order are whole numbers of 2^-42:
+ * a call gives the same results every time.  Up to four launches.  vocab <= VQ2_SAMPLE_MAX_VOCAB, rows <=
  * VQ2_SAMPLE_MAX_ROWS.  The workspace (256-byte aligned,
  * vq2_sample_workspace bytes) may hold anything on entry; calls that share
  * one must not overlap.  Beside the top-1 (vq2_argmax_rows); the reference
