@@ -190,6 +190,25 @@ struct Row {
             f(i, v);
         }
     }
+    // the same with 16 values a thread in flight
+    template <class F>
+    __device__ __forceinline__ void stream_wide(int from, int end, int step, F f) const
+    {
+        constexpr int Q = 16 / VEC;
+        int i = from;
+        for (; i + (Q - 1) * step < min(end, full); i += Q * step) {
+            u32x4 w[Q];
+#pragma unroll
+            for (int q = 0; q < Q; q++) w[q] = raw(i + q * step);
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                float v[VEC];
+                values(w[q], v);
+                f(i + q * step, v);
+            }
+        }
+        stream(i, end, step, f);
+    }
 };
 
 // Order of a row's entries: larger is earlier.
@@ -993,7 +1012,7 @@ __device__ __forceinline__ void finish_list(FinishShared& sh, const SampleArgs& 
 // slice that the draw falls into, whose entries are read again.  False if the
 // bin has too many.
 template <int LT>
-__device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
+__device__ __forceinline__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
                                const Row<LT>& row, const RowInfo& info, uint32_t n_short, int b)
 {
     constexpr int VEC = Row<LT>::VEC;
@@ -1086,63 +1105,104 @@ __device__ bool finish_refined(FinishShared& sh, const SampleArgs& a, const Sett
     return true;
 }
 
-// A row of which nothing shorter is known (long ties in the border's bin; a
-// long row under both top-k and top-p): every round goes over all of it.
+// The last key that stays of a row of which nothing shorter is known (long ties
+// in the border's bin; a long row under both top-k and top-p): a histogram
+// finds a range of the order, and once a range's entries fit the list they are
+// taken from it.  Passes over the row are what it costs: two for a range that
+// fits at once, two more for one that holds too many (to find what it spans,
+// and to cut that).  `known` is a bin of BINS that the border is already known
+// to lie in, and the amount ahead of it.
 template <int LT>
 __device__ __forceinline__ uint64_t row_border(FinishShared& sh, const Row<LT>& row, float cut, const Weigher& weigh,
-                                               uint64_t limit, bool by_mass, uint64_t from)
+                                               uint64_t limit, bool by_mass, uint64_t from, const RefineInfo& known)
 {
     constexpr int VEC = Row<LT>::VEC;
     const int tid = threadIdx.x;
-    uint64_t lo = from, hi = ~0ull, before = 0;
-    int shift = 64;  // (64: a round that finds the range the entries span)
-    for (;;) {
-        uint64_t least = ~0ull, most = ~0ull;  // (most: the largest key's complement)
-        __syncthreads();
-        sh.amount[tid] = 0;
-        __syncthreads();
-        row.stream(tid, row.blocks, NT, [&](int i, const float (&v)[VEC]) {
+    const Binner bin(weigh.max, cut, known.bin >= 0 ? BINS : NT);
+    uint64_t lo = from, hi = ~0ull, before = known.bin >= 0 ? known.before : 0;
+    int shift = -1, at = (int)known.bin;  // (the first round: bin)
+    auto mass = [&](float l) -> uint64_t { return by_mass ? fixed(weigh(l)) : 1; };
+    // f(range, key, logit) for the entries of the ranges (one compute unit's
+    // arithmetic is what a pass costs: keys only of logits in between)
+    auto entries = [&](auto f) {
+        const float least = fmaxf(cut, lo ? key_logit(lo) : -INFINITY), most = hi == ~0ull ? INFINITY : key_logit(hi);
+        row.stream_wide(tid, row.blocks, NT, [&](int i, const float (&v)[VEC]) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) {
+                if (!(v[j] >= least && v[j] <= most)) continue;
                 const uint64_t key = order_key(v[j], i * VEC + j);
-                if (!(v[j] >= cut) || key < lo || key > hi) continue;
-                if (shift == 64) {
-                    least = key < least ? key : least;
-                    most = ~key < most ? ~key : most;
-                } else {
-                    atomicAdd((unsigned long long*)&sh.amount[(hi - key) >> shift],
-                              by_mass ? (unsigned long long)fixed(weigh(v[j])) : 1ull);
-                }
+                if (key >= lo && key <= hi) f(shift < 0 ? bin(v[j]) : (int)((hi - key) >> shift), key, v[j]);
             }
         });
-        __syncthreads();
-        if (shift == 64) {
-            lo = block_min(sh.scratch, least);
-            hi = ~block_min(sh.scratch, most);
-            if (lo > hi) return from;
-            shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
-            continue;
+    };
+    for (bool find = at < 0;; find = true) {
+        if (find) {
+            __syncthreads();
+            sh.amount[tid] = 0;
+            sh.count[tid] = 0;
+            if (tid == 0) sh.n = 0;
+            __syncthreads();
+            // (runs of one range are added at once: ties would queue for it)
+            int run = -1;
+            uint64_t sum = 0;
+            uint32_t length = 0;
+            auto add = [&]() {
+                atomicAdd((unsigned long long*)&sh.amount[run], (unsigned long long)sum);
+                atomicAdd(&sh.count[run], length);
+            };
+            entries([&](int r, uint64_t, float l) {
+                if (r != run) {
+                    if (run >= 0) add();
+                    run = r;
+                    sum = 0;
+                    length = 0;
+                }
+                sum += mass(l);
+                length++;
+            });
+            if (run >= 0) add();
+            __syncthreads();
+            uint64_t ahead = 0;
+            at = block_locate(sh.scratch, sh.amount[tid], limit - before, ahead);
+            if (at < 0) return from;
+            before += ahead;
+            if (sh.count[at] <= LIST) break;
         }
-        uint64_t ahead = 0;
-        const int r = block_locate(sh.scratch, sh.amount[tid], limit - before, ahead);
-        if (r < 0) return from;
-        before += ahead;
-        hi -= (uint64_t)r << shift;
-        if (shift == 0) return hi;  // (one key)
-        lo = hi - lo < (1ull << shift) - 1 ? lo : hi - ((1ull << shift) - 1);
-        shift = 64;
+        uint64_t least = ~0ull, most = ~0ull;  // (most: the largest key's complement)
+        entries([&](int r, uint64_t key, float) {
+            if (r != at) return;
+            least = key < least ? key : least;
+            most = ~key < most ? ~key : most;
+        });
+        lo = block_min(sh.scratch, least);
+        hi = ~block_min(sh.scratch, most);
+        if (lo > hi) return from;
+        shift = hi - lo < NT ? 0 : 64 - __clzll(hi - lo) - BITS;
     }
+    entries([&](int r, uint64_t key, float l) {
+        if (r != at) return;
+        const uint32_t to = atomicAdd(&sh.n, 1u);
+        if (to >= LIST) return;
+        sh.list[to] = key;
+        sh.mass[to] = mass(l);
+    });
+    __syncthreads();
+    const int n = (int)min(sh.n, (uint32_t)LIST);
+    const int i = locate_entry(
+        sh, n, limit - before, [&](int e) { return ~sh.list[e]; }, [&](int e) { return sh.mass[e]; }, [](int) { return 0; });
+    return i >= 0 ? sh.list[i] : from;
 }
 
 template <int LT>
-__device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, const Row<LT>& row,
-                           float cut, double z, int b)
+__device__ __forceinline__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh, const Row<LT>& row,
+                           float cut, double z, const RefineInfo& known, int b)
 {
     constexpr int VEC = Row<LT>::VEC;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     uint64_t lo = 0, total = 0;
+    float least = cut;  // (and lo's logit: keys only of its ties)
     auto kept = [&](float l, int c, bool with_min) -> uint64_t {
-        if (!(l >= cut) || order_key(l, c) < lo) return 0;
+        if (!(l >= least) || (l == least && order_key(l, c) < lo)) return 0;
         const double w = weigh(l);
         return with_min && s.min_p_on && !(w >= s.min_p) ? 0 : fixed(w);
     };
@@ -1150,7 +1210,7 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
     const int eighth = (row.blocks + NW - 1) / NW;
     auto sum = [&](bool with_min) {
         uint64_t part = 0;
-        row.stream(wave * eighth + lane, min(row.blocks, (wave + 1) * eighth), 64, [&](int i, const float (&v)[VEC]) {
+        row.stream_wide(wave * eighth + lane, min(row.blocks, (wave + 1) * eighth), 64, [&](int i, const float (&v)[VEC]) {
 #pragma unroll
             for (int j = 0; j < VEC; j++) part += kept(v[j], i * VEC + j, with_min);
         });
@@ -1166,7 +1226,8 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
             continue;
         }
         const double limit = step == 0 ? (double)s.k : fmax(1.0, ceil(s.p * (s.k > 0 ? (double)total : z * UNIT)));
-        lo = row_border(sh, row, cut, weigh, (uint64_t)limit, step == 2, lo);
+        lo = row_border(sh, row, cut, weigh, (uint64_t)limit, step == 2, lo, known);
+        if (lo) least = fmaxf(cut, key_logit(lo));
     }
     const uint64_t limit = draw_limit(a, b, total);
     uint64_t before = 0, all;
@@ -1205,7 +1266,7 @@ __device__ void finish_row(FinishShared& sh, const SampleArgs& a, const Setting&
 // A draw over the whole row: the unit, then the column, whose running sum is
 // the first above u Z (the last with a weight, if rounding leaves none).
 template <int LT>
-__device__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weigher& weigh, const Row<LT>& row, const Units& un,
+__device__ __forceinline__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weigher& weigh, const Row<LT>& row, const Units& un,
                              int b)
 {
     constexpr int VEC = Row<LT>::VEC;
@@ -1263,7 +1324,7 @@ __device__ void finish_plain(FinishShared& sh, const SampleArgs& a, const Weighe
 }
 
 template <int LT>
-__global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
+__global__ void __launch_bounds__(NT, 4) sample_finish_kernel(SampleArgs a)
 {
     constexpr int VEC = Row<LT>::VEC;
     __shared__ FinishShared sh;
@@ -1323,9 +1384,10 @@ __global__ void __launch_bounds__(NT) sample_finish_kernel(SampleArgs a)
             finish_list(sh, a, s, weigh, (int)n, info.cut, info.z, b);
         return;
     }
-    if (a.refines && s.one_border() && finish_refined<LT>(sh, a, s, weigh, row, info, n_short, b)) return;
+    const bool refined = a.refines && s.one_border();
+    if (refined && finish_refined<LT>(sh, a, s, weigh, row, info, n_short, b)) return;
     __syncthreads();
-    finish_row<LT>(sh, a, s, weigh, row, info.cut, info.z, b);
+    finish_row<LT>(sh, a, s, weigh, row, info.cut, info.z, refined ? a.refined[b] : RefineInfo{0, -1}, b);
 }
 
 // How a call is cut: units of at least 64 blocks (one load a lane), longer
