@@ -36,6 +36,22 @@
 //            order of logits for a border, of columns for the draw).
 // A draw without a border (no top-k, top-p or min-p) is stats and finish: the
 // unit whose weights' running sum passes u Z is read again.
+//
+// Kernel times on MI355X, us (stats + collect + refine + finish):
+//   1 x 151936 fp32, top-k 50, top-p 0.9     3.2 + 7.0 +  -  +  5.3
+//   1 x 151936 fp32, top-p 0.95              4.1 + 6.0 + 1.9 +  8.8
+//   8 x 32000 fp16, top-k 1000               4.0 + 7.9 + 1.9 + 12.5
+//   37 x 50257 bf16, settings by row         5.9 + 9.5 + 6.7 + 13.3
+//   256 x 151936 fp32, plain                  36 +  -  +  -  + 10.2
+//   256 x 151936 bf16, top-p 0.9, min-p       29 +  17 + 4.6 +  7.2
+// Small calls are chains of launches and, within them, of loads and barriers of
+// one row.  In large ones the stats launch is most: over fp32 it reads 4.3 TB/s
+// (a large copy reaches 4.9; with the exponentials left out, 29 us), over 16
+// bits its exponentials of 64 bits bound it (38.9 M in 29 us).
+// A row whose border lies among more entries than the list holds (flat to a
+// tenth, or ties) is gone over by one workgroup: 0.25 to 0.33 ms at 151936
+// logits, bound by that compute unit's instructions, 0.47 to 0.7 ms where it
+// has both a longer top-k and a top-p.
 #include <float.h>
 
 #include "vq2_common.hpp"
@@ -910,8 +926,8 @@ __device__ __forceinline__ void write_token(const SampleArgs& a, int b, int colu
 
 // Up to DIRECT entries: each one's rank and the weight ahead of it, and the
 // kept weight of lower columns, by comparing it with every other, a part of
-// them by each of its threads.  (The comparisons are what it costs: 250 entries
-// took 5 us of them, two histograms 4.)
+// them by each of its threads.  (The comparisons are what it costs: over 250
+// entries they took 5 us, and finish_list's histograms 4, hence DIRECT.)
 __device__ __forceinline__ void finish_direct(FinishShared& sh, const SampleArgs& a, const Setting& s, const Weigher& weigh,
                                               int n, double z, int b)
 {

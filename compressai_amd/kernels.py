@@ -1533,7 +1533,7 @@ def vq_sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     column at which their running sum exceeds u times the total.  Ties go to
     the lower column; temperature 0 takes the first maximum; -inf and NaN
     columns are absent, and a row of nothing else gives token -1 and a NaN
-    logprob.  Each setting is a number for all rows or a tensor [rows] (fp32;
+    logprob; beside +inf finite logits weigh nothing.  Each setting is a number for all rows or a tensor [rows] (fp32;
     top_k int32).  Returns (idx int64 [rows], logprob fp32 [rows]: the log of
     the probability the token was drawn with)."""
     if logits.is_cuda:

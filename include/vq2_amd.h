@@ -337,7 +337,8 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
  *     descending order (ties toward the lower id)
  *   w[t, j] (fp32) = s_ids[t, j] / (renormalise ? sum_j s_ids[t, j] : 1) * scale
  * Without a bias c orders as the logits do, which are compared themselves;
- * else choices are made in 64-bit arithmetic, c that agree to 42 bits as ties.
+ * else choices are made in 64-bit arithmetic, and c that agree to 42 bits may
+ * count as ties.
  * An expert whose logit is -inf or NaN, or whose bias is, is masked: behind
  * every other of its group, weight 0 (a token whose experts are all masked
  * gets ids of weight 0).  If shared_id >= 0, slot k of each row is the shared
@@ -368,14 +369,17 @@ int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t to
  *     weights that stayed, in column order, exceeds u times their total
  *   out_logprob[row] (fp32): ln(w_out_idx / total), the log of the probability
  *     it was drawn with
- * temperature 0: the first maximum, logprob 0.  Columns of -inf or NaN are
- * absent; a row without any other gives out_idx -1 and a NaN logprob.  Each
+ * temperature 0: the first maximum, logprob 0; an infinite one is taken as
+ * the largest finite one.  Columns of -inf or NaN are absent; a row without any
+ * other gives out_idx -1 and a NaN logprob.  Beside a column of +inf every
+ * finite one weighs 0.  u outside [0, 1] acts as the nearest end (NaN: 0).  Each
  * setting is common to all rows, or given by row on the device (its _rows
  * pointer not NULL; there a temperature, top_k, top_p or min_p outside its
  * range acts as the nearest one inside; NaN: greedy, no top_p, the maxima).
  * Weights are 64-bit; sums over a whole row are too, in an order that the
- * sizes fix, and those of entries put in order are whole numbers of 2^-42:
- * a call gives the same results every time.  Up to four launches.  vocab <= VQ2_SAMPLE_MAX_VOCAB, rows <=
+ * sizes fix, and those of entries put in order are whole numbers of 2^-42
+ * (weights below half of that count as 0 there): a call gives the same results
+ * every time.  Two to four launches.  vocab <= VQ2_SAMPLE_MAX_VOCAB, rows <=
  * VQ2_SAMPLE_MAX_ROWS.  The workspace (256-byte aligned,
  * vq2_sample_workspace bytes) may hold anything on entry; calls that share
  * one must not overlap.  Beside the top-1 (vq2_argmax_rows); the reference

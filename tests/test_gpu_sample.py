@@ -330,3 +330,60 @@ def test_units_without_weight(dev, dtype, kw):
     u = torch.zeros(3)
     _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
     assert K.vq_sample(x.to(dev), u.to(dev), **kw)[0].tolist() == [20000, 29999, 15000]
+
+
+def test_u_of_nan_is_zero(dev):
+    x = _logits(9100, 2, 5000, "fp32").to(dev)
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.9)):
+        got = K.vq_sample(x, torch.tensor([float("nan"), 0.5], device=dev), **kw)
+        ref = K.vq_sample(x, torch.tensor([0.0, 0.5], device=dev), **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.parametrize("top_k", [50, 5000])
+def test_long_ties_under_every_border(dev, top_k):
+    """Rows whose border lies among more ties than the list holds, one slice's
+    ties, and ties behind a few larger logits."""
+    V = 30011
+    x = torch.zeros(4, V)
+    x[1, ::2] = 1.0
+    x[2, 9000:16000] = 2.0
+    x[3, ::1000] = 3.0
+    u = torch.tensor([0.2, 0.5, 0.8, 0.97])
+    for dtype in DT.values():
+        for kw in (dict(top_k=top_k), dict(top_p=0.7), dict(top_k=top_k, top_p=0.5), dict(top_k=top_k, top_p=0.5, min_p=0.3),
+                   dict(top_p=0.999, temperature=4.0)):
+            _check(K.vq_sample(x.to(dtype).to(dev), u.to(dev), **kw), x.to(dtype), u, **kw)
+
+
+def test_calls_side_by_side(dev):
+    """Two streams with a call each, again and again, and two graphs replayed in
+    turn with eager calls between: every result is the one of a call alone."""
+    a, b = _logits(9200, 3, 151936, "bf16", 0.1).to(dev), _logits(9201, 40, 9000, "fp32").to(dev)
+    ua, ub = torch.rand(3, generator=synth.gen(9202)).to(dev), torch.rand(40, generator=synth.gen(9203)).to(dev)
+    calls = [lambda: K.vq_sample(a, ua, top_p=0.95), lambda: K.vq_sample(b, ub, top_k=700, top_p=0.9)]
+    ref = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(10):
+        for i, (c, st) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(c())
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(c())
+    for _ in range(4):
+        for i in (0, 1):
+            for o in outs[i]:
+                o.zero_()
+            graphs[i].replay()
+            got[1 - i].append(calls[1 - i]())
+            got[i].append([o.clone() for o in outs[i]])
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for g in got[i]:
+            assert torch.equal(g[0], ref[i][0]) and torch.equal(g[1], ref[i][1])
