@@ -49,9 +49,10 @@
 // (a large copy reaches 4.9; with the exponentials left out, 29 us), over 16
 // bits its exponentials of 64 bits bound it (38.9 M in 29 us).
 // A row whose border lies among more entries than the list holds (flat to a
-// tenth, or ties) is gone over by one workgroup: 0.25 to 0.33 ms at 151936
-// logits, bound by that compute unit's instructions, 0.47 to 0.7 ms where it
-// has both a longer top-k and a top-p.
+// tenth, or ties) is gone over by one workgroup, bound by that compute unit's
+// instructions: 0.25 to 0.33 ms at 151936 logits, 0.48 with ties of which every
+// second column is one, 0.47 to 0.7 ms where it has both a longer top-k and a
+// top-p.
 #include <float.h>
 
 #include "vq2_common.hpp"
