@@ -146,24 +146,6 @@ __device__ __forceinline__ float shared_weight(const SelectArgs& a, int64_t t, i
 // ------------------------------------------------------------- one wave a token
 constexpr double KEY_MASKED = -1e300;
 
-// Choice and expert in one double, so that one v_max_f64 compares both: the
-// low 10 bits of the mantissa carry the id, such that the lower one wins among
-// equal choices.  Choices are compared to 42 bits then; fp32 logits, compared
-// themselves where scores order alike, have 24 and stay exact.
-__device__ __forceinline__ double choice_key(double c, int e)
-{
-    // (+ 0.0: -0 is 0; no infinity, whose low bits make a NaN)
-    uint64_t b = __builtin_bit_cast(uint64_t, fmin(c, 1e300) + 0.0) & ~1023ull;
-    b |= (b >> 63) ? (uint64_t)e : (uint64_t)(1023 - e);
-    return __builtin_bit_cast(double, b);
-}
-
-__device__ __forceinline__ int key_expert(double key)
-{
-    const uint64_t b = __builtin_bit_cast(uint64_t, key);
-    return (b >> 63) ? (int)(b & 1023) : 1023 - (int)(b & 1023);
-}
-
 __device__ __forceinline__ double wave_max_f64(double v)
 {
 #pragma unroll
@@ -246,20 +228,26 @@ __device__ void select_token(const SelectArgs& a, int64_t t, int lane, double* s
         }
     }
 #pragma unroll
-    for (int j = 0; j < RPL; j++) {
-        const int e = j * 64 + lane;
-        key[j] = e < a.n_e && key[j] > -INFINITY ? choice_key(key[j], e) : -INFINITY;
-    }
+    for (int j = 0; j < RPL; j++)
+        if (j * 64 + lane >= a.n_e) key[j] = -INFINITY;
+    // the largest choice, and of its experts the lowest (choices that differ in
+    // their last bit alone are told apart: sigmoids close to 1 do)
     int id = 0;
     for (int r = 0; r < a.k; r++) {
         double best = key[0];
 #pragma unroll
         for (int j = 1; j < RPL; j++) best = fmax(best, key[j]);
         best = wave_max_f64(best);
+        int at = 0;
+#pragma unroll
+        for (int j = RPL - 1; j >= 0; j--) {
+            const uint64_t equal = __ballot(key[j] == best);
+            if (equal) at = j * 64 + __builtin_ctzll(equal);
+        }
 #pragma unroll
         for (int j = 0; j < RPL; j++)
-            if (key[j] == best) key[j] = -INFINITY;
-        if (lane == r) id = key_expert(best);
+            if (j * 64 + lane == at) key[j] = -INFINITY;
+        if (lane == r) id = at;
     }
     // the weights: lane r takes choice r's logit again
     double sw = 0.0;

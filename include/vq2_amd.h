@@ -337,8 +337,8 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
  *     descending order (ties toward the lower id)
  *   w[t, j] (fp32) = s_ids[t, j] / (renormalise ? sum_j s_ids[t, j] : 1) * scale
  * Without a bias c orders as the logits do, which are compared themselves;
- * else choices are made in 64-bit arithmetic, and c that agree to 42 bits may
- * count as ties.
+ * else choices are made and compared in 64-bit arithmetic, whose scores are off
+ * by less than 2^-44 of themselves.
  * An expert whose logit is -inf or NaN, or whose bias is, is masked: behind
  * every other of its group, weight 0 (a token whose experts are all masked
  * gets ids of weight 0).  If shared_id >= 0, slot k of each row is the shared

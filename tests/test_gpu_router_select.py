@@ -260,3 +260,15 @@ def test_native_and_python_entries_agree(dev):
         ref = K.vq_router_select(lg, 8, **kw)
         got = K.vq_router_select(lg, 8, ids=torch.empty(90, slots, dtype=torch.int32, device=dev), **kw)
         assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+@pytest.mark.parametrize("E,k,G", [(64, 6, 1), (256, 8, 8), (512, 12, 1), (100, 20, 5), (1024, 32, 1)])
+@pytest.mark.parametrize("bias", [0.0, 0.125, -3.0])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_choices_that_differ_in_their_last_bits(dev, E, k, G, bias, dtype):
+    """Sigmoids close to 1 under one bias for all (a balance bias that has not
+    moved yet): choices differ from the 43rd bit on and are still in order."""
+    lg = (27.0 + 9.0 * torch.rand(30, E, generator=synth.gen(7995))).to(DT[dtype])
+    for gs in ("max", "top2"):
+        more = dict(scoring="sigmoid", bias=torch.full((E,), bias, device=dev), n_groups=G, topk_groups=max(1, G // 2), group_score=gs)
+        _check(K.vq_router_select(lg.to(dev), k, **more), lg, k, **more)
