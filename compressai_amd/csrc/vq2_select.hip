@@ -62,8 +62,14 @@ struct SelectArgs {
 };
 
 // Scores of 64 bits: exp for x <= 0, and the sigmoid, 0 where e^-x is none of
-// 64 bits.
-__device__ __forceinline__ double exp_f64(double x) { return exp2_f64(x * LOG2E_F64); }
+// 64 bits.  Below 2^-1000, which exp2_f64 does not pass, the power is taken 128
+// binary orders higher, and the product with 2^-128 rounds it to what 64 bits
+// have there.
+__device__ __forceinline__ double exp_f64(double x)
+{
+    const double y = fmax(x * LOG2E_F64, -1100.0);
+    return y < -1000.0 ? exp2_f64_in(y + 128.0) * 0x1p-128 : exp2_f64_in(y);
+}
 // 1 / x of a normal x whose reciprocal is normal, to 2^-51: the instruction's
 // approximation and two Newton steps
 __device__ __forceinline__ double reciprocal_f64(double x)
@@ -74,7 +80,8 @@ __device__ __forceinline__ double reciprocal_f64(double x)
 }
 __device__ __forceinline__ double sigmoid_f64(double x)
 {
-    return x < -700.0 ? (x < -709.0 ? 0.0 : exp_f64(x)) : reciprocal_f64(1.0 + exp2_f64(-x * LOG2E_F64));
+    if (x < -700.0) return x < -709.78271289338397 ? 0.0 : exp_f64(x);
+    return reciprocal_f64(1.0 + exp2_f64(-x * LOG2E_F64));
 }
 
 // LDS written by a wave's lanes is read by its others.
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
     if (softmax && (biased || !a.renorm)) {
         z = 0.0;
 #pragma unroll
-        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp_f64((double)l[j] - (double)m);
+        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp2_f64(((double)l[j] - (double)m) * LOG2E_F64);
         z = row_sum(z);
     }
 

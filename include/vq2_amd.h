@@ -328,7 +328,8 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
 
 /* The router's further forms, per token, on given logits [tokens, l_stride]
  * (n_experts of each row used):
- *   s_e = softmax(l)_e over the n_experts, or sigmoid(l_e)   (scoring)
+ *   s_e = softmax(l)_e over the n_experts, or sigmoid(l_e)   (scoring; a
+ *     sigmoid is 0 where e^-l is past 64 bits, l < -709.78)
  *   c_e = s_e + bias[e]                    (bias fp32 [n_experts] or NULL)
  * The experts are cut into n_groups groups of n_experts / n_groups consecutive
  * ones (1: no groups); the topk_groups groups of the largest group score --
@@ -338,7 +339,7 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
  *   w[t, j] (fp32) = s_ids[t, j] / (renormalise ? sum_j s_ids[t, j] : 1) * scale
  * Without a bias c orders as the logits do, which are compared themselves;
  * else choices are made and compared in 64-bit arithmetic, whose scores are off
- * by less than 2^-44 of themselves.
+ * by less than 2^-43 of themselves.
  * An expert whose logit is -inf or NaN, or whose bias is, is masked: behind
  * every other of its group, weight 0 (a token whose experts are all masked
  * gets ids of weight 0).  If shared_id >= 0, slot k of each row is the shared

@@ -272,3 +272,25 @@ def test_choices_that_differ_in_their_last_bits(dev, E, k, G, bias, dtype):
     for gs in ("max", "top2"):
         more = dict(scoring="sigmoid", bias=torch.full((E,), bias, device=dev), n_groups=G, topk_groups=max(1, G // 2), group_score=gs)
         _check(K.vq_router_select(lg.to(dev), k, **more), lg, k, **more)
+
+
+@pytest.mark.parametrize("E,k,G", [(16, 12, 1), (24, 10, 2), (100, 20, 1), (700, 5, 7)])
+@pytest.mark.parametrize("low,high", [(-708.0, -690.0), (-709.7, -699.0), (-745.0, -700.0)])
+@pytest.mark.parametrize("form", [dict(scoring="sigmoid"), dict(scoring="sigmoid", bias=0.0), dict(bias=0.0)], ids=str)
+def test_scores_near_the_end_of_64_bits(dev, E, k, G, low, high, form):
+    """Sigmoids and softmax terms of e^-690 and below are in order and weighed
+    against each other, down to the steps of 2^-1074 that 64 bits end in; a
+    sigmoid is 0 from -709.78 on.  (Softmax: one expert far above, which its
+    bias keeps from being chosen.)"""
+    lg = low + (high - low) * torch.rand(24, E, generator=synth.gen(7990))
+    if low < -740.0 and "scoring" in form:
+        lg[:, ::2] += 9.0
+    kw = dict(form)
+    if "bias" in kw:
+        kw["bias"] = torch.zeros(E)
+    if "scoring" not in kw:
+        lg[:, E // 2] = 0.0
+        kw["bias"][E // 2] = -2.0
+    kw["bias"] = kw["bias"].to(dev) if "bias" in kw else None
+    more = dict(n_groups=G, topk_groups=max(1, G // 2), **kw)
+    _check(K.vq_router_select(lg.to(dev), k, **more), lg, k, **more)
