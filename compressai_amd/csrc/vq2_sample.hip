@@ -258,13 +258,16 @@ struct Weigher {
 
 // The bin of n of a logit, 0 the highest: linear between `max` and `cut`.
 // Rounded arithmetic, but monotonic: a higher logit is never in a lower bin.
+// `inv` is 0, and all are in bin 0, where bins have no width in 32 bits or no
+// reciprocal (logits closer than n / FLT_MAX).
 struct Binner {
     float max, inv;
     int n;
     __device__ __forceinline__ Binner(float max_, float cut, int n_) : max(finite(max_)), n(n_)
     {
         const float width = max - cut;
-        inv = width > 0.0f && width < INFINITY ? (float)n / width : 0.0f;
+        const float r = (float)n / width;
+        inv = width > 0.0f && r < INFINITY ? r : 0.0f;
     }
     __device__ __forceinline__ int operator()(float l) const { return (int)fminf((max - finite(l)) * inv, (float)(n - 1)); }
 };

@@ -387,3 +387,18 @@ def test_calls_side_by_side(dev):
     for i in (0, 1):
         for g in got[i]:
             assert torch.equal(g[0], ref[i][0]) and torch.equal(g[1], ref[i][1])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-36, 1e-37, 1e-39, 1e-43])
+@pytest.mark.parametrize("V", [5000, 5120])
+def test_logits_a_tiny_way_apart(dev, dtype, scale, V):
+    """Rows whose logits lie so close that their range has no reciprocal of 32
+    bits, subnormal ones among them (5120 columns fill every group of the
+    row): every entry weighs 1, and the order is still the logits'."""
+    x = (torch.rand(4, V, generator=synth.gen(9300)).double() * scale).to(DT[dtype])
+    x[1] = 2 * scale + x[1]
+    u = torch.tensor([0.05, 0.4, 0.75, 0.999])
+    for kw in (dict(top_k=3), dict(top_k=20), dict(top_k=300), dict(top_k=20, top_p=0.5), dict(top_p=0.6), dict(min_p=0.5),
+               dict(top_k=4000, top_p=0.9), dict()):
+        _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
