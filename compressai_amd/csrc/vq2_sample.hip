@@ -474,7 +474,9 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
     if (s.whole_sum()) {
         // sum of exp((l - ref) / temperature), ref one of the lane's logits:
         // 64 bits hold weights of 2^1000, so it moves only where one is close,
-        // past `high`.  Differences are held above -990 / c, whose weight is
+        // past `high`, 900 binary orders above: a sum of weights up to there,
+        // moved by the most that exp2_f64 takes away, 2^-1000, is nothing
+        // beside a weight of 1.  Differences are held above -990 / c, whose weight is
         // nothing, by a median, which drops NaN as well as -inf: of 16-bit
         // logits in 32 bits, exact but for logits 2^-13 of ref and below; of
         // 32-bit ones before the difference in 64.  `quick` is whether fp32
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(NT, 8) sample_stats_kernel(SampleArgs a)
                 ref = top;
                 high = (float)fmin((double)ref + (double)span, (double)FLT_MAX);
                 least = (float)fmax((double)ref - (double)lim, (double)-FLT_MAX);
-                if (((double)high - (double)ref) * s.c > 1000.0) high = ref;  // (rounded past what 64 bits hold)
+                if (((double)high - (double)ref) * s.c > 910.0) high = ref;  // (rounded further up than that)
                 quick = LT == VQ2_DT_F32 ? fabs(((double)ref - (double)least) * s.c - 990.0) < 5.0 : lim < 1e37f && ref < FLT_MAX;
             }
             if (quick) {

@@ -402,3 +402,26 @@ def test_logits_a_tiny_way_apart(dev, dtype, scale, V):
     for kw in (dict(top_k=3), dict(top_k=20), dict(top_k=300), dict(top_k=20, top_p=0.5), dict(top_p=0.6), dict(min_p=0.5),
                dict(top_k=4000, top_p=0.9), dict()):
         _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+
+
+@pytest.mark.parametrize("orders", [850, 905, 950, 995, 1005])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_logits_one_step_apart_a_range_of_weights_apart(dev, dtype, orders):
+    """Temperatures at which neighbouring logits of the type differ by about
+    as many binary orders as a sum of 64-bit weights can hold, in rows that
+    ascend under each lane: all but the maxima weigh nothing."""
+    B, V = 64, 151936
+    step = 16.0 * torch.finfo(DT[dtype]).eps
+    col = torch.arange(V)
+    rows = []
+    for r in range(4):
+        rise = (col // (256 * (r + 1))) % 4 if r < 3 else torch.randint(0, 4, (V,), generator=synth.gen(9310))
+        rows.append(16.0 + step * rise)
+    x = torch.stack(rows).to(DT[dtype])
+    u = torch.tensor([0.1, 0.45, 0.7, 0.95])
+    t = float(np.float32(step * np.log2(np.e) / orders))
+    logits, us = x.to(dev).repeat(B // 4, 1), u.to(dev).repeat(B // 4)
+    for kw in (dict(), dict(top_p=0.5)):
+        idx, lp = K.vq_sample(logits, us, temperature=t, **kw)
+        assert torch.equal(idx, idx[:4].repeat(B // 4)) and torch.equal(lp, lp[:4].repeat(B // 4))
+        _check((idx[:4], lp[:4]), x, u, temperature=t, **kw)
