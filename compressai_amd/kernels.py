@@ -1471,6 +1471,25 @@ SCORING = {"softmax": 0, "sigmoid": 1}  # VQ2_SCORE_*
 GROUP_SCORE = {"max": 0, "top2": 1}     # VQ2_GROUP_*
 
 
+def _router_bias(bias, n):
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
+        raise Vq2Error(f"bias must be a contiguous float32 [{n}]")
+
+
+def check_router_form(n_experts, k, *, scoring="softmax", bias=None, n_groups=1, topk_groups=None, group_score="max",
+                      renormalise=True, scale=1.0, shared_id=-1):
+    """Raises what ``vq_router_select`` raises for these arguments with logits
+    of n_experts columns, without any logits."""
+    if scoring not in SCORING or group_score not in GROUP_SCORE:
+        raise Vq2Error(f"vq_router_select: scoring {scoring!r} (softmax/sigmoid), group_score {group_score!r} (max/top2)")
+    _router_bias(bias, n_experts)
+    topk_groups = n_groups if topk_groups is None else topk_groups
+    # (no tokens: the library checks the rest and launches nothing)
+    _lib.call("vq2_router_select", None, _lib.DT_F32, n_experts, 0, n_experts, int(k), SCORING[scoring], _p(bias), int(n_groups),
+              int(topk_groups), GROUP_SCORE[group_score], 1 if renormalise else 0, float(scale), None, 0, 0, None, 0,
+              int(shared_id), None, None, None)
+
+
 def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, topk_groups=None, group_score="max",
                      renormalise=True, scale=1.0, h=None, shared_gate=None, shared_id=-1, ids=None, w=None):
     """The router's further forms, per token: scores s = softmax(logits) or
@@ -1497,8 +1516,7 @@ def vq_router_select(logits, k=8, *, scoring="softmax", bias=None, n_groups=1, t
     dev = _dev(logits, bias, h, shared_gate, ids, w)
     lg, stride = _rows2d(logits, "logits")
     T, E = lg.shape
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != E or not bias.is_contiguous()):
-        raise Vq2Error(f"bias must be a contiguous float32 [{E}]")
+    _router_bias(bias, E)
     slots = k + (1 if shared_id >= 0 else 0)
     gate, hid = None, 0
     if shared_id >= 0 and shared_gate is not None:

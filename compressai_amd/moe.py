@@ -241,8 +241,10 @@ class MoELayer(nn.Module):
     [E+1, 2I] / [E+1, H]; id E is the shared expert.  shared_gate [H], or None
     for a shared expert of weight 1.  ``scoring``, ``router_bias`` (fp32 [E]),
     ``n_groups``, ``topk_groups``, ``group_score``, ``renormalise`` and
-    ``routed_scale`` are those of ``kernels.vq_router_select``; their defaults
-    are the softmax router built into the experts' launches."""
+    ``routed_scale`` are those of ``kernels.vq_router_select``, checked here;
+    their defaults are the softmax router built into the experts' launches.
+    The bias, like the pools and the gate, is held as given, on the pools'
+    device: no buffer that ``to()`` or ``state_dict()`` would take."""
 
     def __init__(self, gate_up_idx, gate_up_scale, down_idx, down_scale, cb16, shared_gate, top_k=8,
                  n_routed=None, rot_h=None, rot_i=None, act_dtype=torch.float32, out_dtype=torch.float32,
@@ -264,6 +266,9 @@ class MoELayer(nn.Module):
                              "routed experts invalid")
         if (shared_gate is None or scoring != "softmax" or router_bias is not None or not renormalise
                 or routed_scale != 1.0 or form["topk_groups"] not in (None, form["n_groups"])):
+            K.check_router_form(self.n_routed, self.top_k, shared_id=self.n_routed, **form)
+            if router_bias is not None and router_bias.device != gate_up_idx.device:
+                raise K.Vq2Error(f"router_bias is on {router_bias.device}, the pools are on {gate_up_idx.device}")
             self.router_form = form
         # down projection: one launch (SwiGLU + RHT in every workgroup) or a
         # separate SwiGLU + RHT launch followed by the grouped down + combine

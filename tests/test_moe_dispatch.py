@@ -77,3 +77,21 @@ def test_token_count_of_activations_with_more_dims(calls):
         n = h.numel() // H
         m.experts(h, torch.zeros(n, 1, dtype=torch.int32), torch.zeros(n, 1))
         assert calls[-1] == entry, h.shape
+
+
+def _routed(top_k=4, **kw):
+    gu, dn = synth.indices16(8620, (E, 2 * I, H // 8)), synth.indices16(8621, (E, H, I // 8))
+    return MoELayer(gu, synth.scales(8622, (E, 2 * I)), dn, synth.scales(8623, (E, H)), synth.codebook(8624),
+                    torch.zeros(H), top_k=top_k, sorted_layout=False, **kw)
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(scoring="sigmoid", router_bias=torch.zeros(E)), "bias"), (dict(router_bias=torch.zeros(E - 1).half()), "bias"),
+    (dict(router_bias=torch.zeros(2 * E - 2)[::2]), "bias"), (dict(router_bias=torch.zeros(E - 1, device="meta")), "router_bias"),
+    (dict(n_groups=8, topk_groups=0), "topk_groups"), (dict(n_groups=8, topk_groups=9), "topk_groups"),
+    (dict(n_groups=32, topk_groups=1), "topk_groups"), (dict(scoring="sigmoid", top_k=33), "k=33"),
+    (dict(scoring="sigmoid", top_k=0), "k=0"), (dict(routed_scale=float("nan")), "scale")])
+def test_router_forms_are_checked_when_the_layer_is_made(kw, msg):
+    with pytest.raises(K.Vq2Error, match=msg):
+        _routed(**kw)
+    assert _routed(scoring="sigmoid", router_bias=torch.zeros(E - 1), n_groups=8, topk_groups=2).router_form is not None
