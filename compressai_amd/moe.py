@@ -267,6 +267,9 @@ class MoELayer(nn.Module):
         if (shared_gate is None or scoring != "softmax" or router_bias is not None or not renormalise
                 or routed_scale != 1.0 or form["topk_groups"] not in (None, form["n_groups"])):
             K.check_router_form(self.n_routed, self.top_k, shared_id=self.n_routed, **form)
+            if self.n_routed >= self.experts_mod.num_experts:
+                raise K.Vq2Error(f"the shared expert, id n_routed={self.n_routed}, is outside the pool of "
+                                 f"{self.experts_mod.num_experts}")
             if router_bias is not None and router_bias.device != gate_up_idx.device:
                 raise K.Vq2Error(f"router_bias is on {router_bias.device}, the pools are on {gate_up_idx.device}")
             self.router_form = form

@@ -95,3 +95,12 @@ def test_router_forms_are_checked_when_the_layer_is_made(kw, msg):
     with pytest.raises(K.Vq2Error, match=msg):
         _routed(**kw)
     assert _routed(scoring="sigmoid", router_bias=torch.zeros(E - 1), n_groups=8, topk_groups=2).router_form is not None
+
+
+@pytest.mark.parametrize("n_routed", [E, E + 3])
+def test_a_shared_expert_outside_the_pool_is_refused(n_routed):
+    """The built-in router refuses it at the call; a router in front of the
+    experts hands them ids, and an id outside the pool computes NaN."""
+    with pytest.raises(K.Vq2Error, match="pool"):
+        _routed(scoring="sigmoid", n_routed=n_routed)
+    assert _routed(scoring="sigmoid", n_routed=E - 5).n_routed == E - 5
