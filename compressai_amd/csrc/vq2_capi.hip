@@ -733,6 +733,7 @@ int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t to
     CHECK(logits && ids && w, "vq2_router_select: NULL pointer argument");
     CHECK(dt_ok(l_dt), "vq2_router_select: bad logits dtype");
     CHECK(l_stride >= n_experts || tokens == 1, "vq2_router_select: l_stride < n_experts");
+    CHECK((uintptr_t)logits % dt_size(l_dt) == 0, "vq2_router_select: logits must be aligned to their elements");
     if (shared_id >= 0 && gate) {
         CHECK(h && hidden > 0, "vq2_router_select: shared gate needs h and hidden");
         CHECK(dt_ok(h_dt) && dt_ok(g_dt), "vq2_router_select: bad h/gate dtype");

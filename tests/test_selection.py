@@ -132,3 +132,8 @@ def test_rows_of_any_stride():
     for bad in (x[:, ::2], x.t(), x[:1].expand(5, 40), torch.zeros(2, 0), torch.tensor(1.0), x[:, 3:9].unsqueeze(0)):
         with pytest.raises(K.Vq2Error):
             K._rows2d(bad, "x")
+
+
+@pytest.mark.parametrize("kw", [dict(logits=18), dict(logits=17, dt=1), dict(logits=17, dt=2)])
+def test_router_select_refuses_logits_between_elements(kw):
+    assert "aligned" in _err(_select(**kw))
