@@ -6,6 +6,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <cmath>
 #include <mutex>
 #include <vector>
 
@@ -726,7 +727,7 @@ int vq2_router_select(const void* logits, int l_dt, int64_t l_stride, int64_t to
           "vq2_router_select: topk_groups=%d out of range (1..%d, with k=%d experts among them)", topk_groups, n_groups, k);
     CHECK(group_score == VQ2_GROUP_MAX || group_score == VQ2_GROUP_TOP2, "vq2_router_select: group_score %d invalid",
           group_score);
-    CHECK(scale == scale, "vq2_router_select: scale is NaN");
+    CHECK(std::isfinite(scale), "vq2_router_select: scale %g is not finite", (double)scale);
     CHECK(shared_id <= 0x7FFFFFFF, "vq2_router_select: shared_id does not fit int32");
     if (tokens == 0) return VQ2_OK;
     if (tokens > 0x7FFFFFFF) return set_error(VQ2_ERR_UNSUPPORTED, "vq2_router_select: too many tokens");

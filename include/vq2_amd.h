@@ -337,6 +337,7 @@ int vq2_router_topk(const void* logits, int l_dt, int64_t tokens, int64_t n_expe
  *   ids[t, j] (int32), j < k: the k largest c of the groups that stay, in
  *     descending order (ties toward the lower id)
  *   w[t, j] (fp32) = s_ids[t, j] / (renormalise ? sum_j s_ids[t, j] : 1) * scale
+ *     (scale finite; a sum of 0 gives weights of 0)
  * Without a bias c orders as the logits do, which are compared themselves;
  * else choices are made and compared in 64-bit arithmetic, whose scores are off
  * by less than 2^-43 of themselves.

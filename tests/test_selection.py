@@ -137,3 +137,9 @@ def test_rows_of_any_stride():
 @pytest.mark.parametrize("kw", [dict(logits=18), dict(logits=17, dt=1), dict(logits=17, dt=2)])
 def test_router_select_refuses_logits_between_elements(kw):
     assert "aligned" in _err(_select(**kw))
+
+
+@pytest.mark.parametrize("scale", [float("inf"), -float("inf")])
+def test_router_select_refuses_an_infinite_scale(scale):
+    """A masked expert's weight, 0, would be 0 times infinity."""
+    assert "scale" in _err(_select(scale=scale))
