@@ -83,6 +83,26 @@ def sample_row(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return token, float(np.log(stayed[token] / run[-1])), stayed
 
 
+def sample_long_row(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, fp64 logprob) of sample_row for a long row of finite logits and a
+    temperature above 0, by sorting and running sums of whole arrays."""
+    x = np.asarray(logits, np.float64)
+    order = np.argsort(-x, kind="stable")
+    if top_k > 0:
+        order = order[:top_k]
+    w = np.exp((x[order] - x[order[0]]) / temperature)
+    if top_p < 1.0:
+        before = np.concatenate([[0.0], np.cumsum(w)[:-1]])
+        n = max(1, int(np.count_nonzero(before < top_p * w[::-1].sum())))
+        order, w = order[:n], w[:n]
+    order, w = order[w >= min(min_p, 1.0)], w[w >= min(min_p, 1.0)]
+    by_column = np.argsort(order, kind="stable")
+    order, w = order[by_column], w[by_column]
+    run = np.cumsum(w)
+    at = min(int(np.searchsorted(run, min(max(u, 0.0), 1.0) * run[-1], side="right")), len(order) - 1)
+    return int(order[at]), float(np.log(w[at] / run[-1]))
+
+
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Rows of sample_row; each setting a number or one value per row."""
     x = np.atleast_2d(np.asarray(logits, np.float64))

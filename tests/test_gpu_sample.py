@@ -425,3 +425,51 @@ def test_logits_one_step_apart_a_range_of_weights_apart(dev, dtype, orders):
         idx, lp = K.vq_sample(logits, us, temperature=t, **kw)
         assert torch.equal(idx, idx[:4].repeat(B // 4)) and torch.equal(lp, lp[:4].repeat(B // 4))
         _check((idx[:4], lp[:4]), x, u, temperature=t, **kw)
+
+
+def _check_long(got, logits, u, rows, **kw):
+    """_check for picked rows of a long vocabulary, whose draw and logprob are
+    the sorted arrays' (settings are held in 32 bits)."""
+    idx, lp = (t.cpu() for t in got)
+    kw = {k: v if k == "top_k" else float(np.float32(v)) for k, v in kw.items()}
+    for r in rows:
+        ref_idx, ref_lp = S.sample_long_row(logits[r].float().cpu().numpy(), float(u[r]), **kw)
+        assert int(idx[r]) == ref_idx, r
+        assert abs(float(lp[r]) - ref_lp) <= abs(ref_lp) * 2.0 ** -24 + logits.shape[-1] * 2.0 ** -43 + 2.0 ** -40, r
+
+
+def _long_logits(dev, B, V, dtype, steep):
+    """_logits made on the device."""
+    g = torch.Generator(device=dev).manual_seed(9400 + V % 1000)
+    rank = torch.rand(B, V, generator=g, device=dev) * V + 2.0
+    return (16.0 - steep * rank.log() + 0.4 * steep * torch.randn(B, V, generator=g, device=dev)).to(DT[dtype])
+
+
+LONG = [dict(), dict(top_p=0.9, min_p=0.01), dict(top_k=50, top_p=0.9, temperature=0.7), dict(min_p=0.3), dict(top_k=700),
+        dict(top_k=20000), dict(top_k=20000, top_p=0.5, min_p=0.02)]
+
+
+@pytest.mark.parametrize("kw", LONG, ids=str)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("steep", [1.3, 0.1])
+def test_large_batches_of_a_whole_vocabulary(dev, dtype, steep, kw):
+    """256 rows cut into units that a wave reads in many steps (19 over fp32, 10
+    over bf16), peaked and nearly flat."""
+    B, V = 256, 151936
+    x = _long_logits(dev, B, V, dtype, steep)
+    u = torch.rand(B, generator=synth.gen(9401))
+    rows = [0, 101, 255]
+    u[101], u[255] = 1.0 - 2.0 ** -24, 0.0
+    _check_long(K.vq_sample(x, u.to(dev), **kw), x, u, rows, **kw)
+
+
+@pytest.mark.parametrize("kw", LONG, ids=str)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,steep", [(1 << 21, 1.3), ((1 << 21) - 3, 0.1)])
+def test_the_longest_vocabulary(dev, V, steep, dtype, kw):
+    """Rows of as many units and slices as there can be."""
+    x = _long_logits(dev, 3, V, dtype, steep)
+    u = torch.tensor([0.0, 0.5, 1.0 - 2.0 ** -24])
+    _check_long(K.vq_sample(x, u.to(dev), **kw), x, u, range(3), **kw)
+    one = K.vq_sample(x[1:2], u[1:2].to(dev), **kw)
+    _check_long(one, x[1:2], u[1:2], [0], **kw)

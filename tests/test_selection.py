@@ -53,6 +53,18 @@ def test_sample_oracle_frequencies_and_filters():
     assert S.sample_row([np.inf, 1.0, np.inf], 0.6)[:2] == (2, np.log(0.5))
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.6), dict(top_k=9), dict(top_p=0.7), dict(top_p=0.0), dict(min_p=0.2),
+                                dict(top_k=40, top_p=0.8, min_p=0.05, temperature=1.3), dict(top_k=1000)], ids=str)
+def test_sample_oracle_of_long_rows_is_the_other_one(kw):
+    g = np.random.default_rng(2)
+    for n in (1, 2, 50, 301):
+        x = np.round(g.normal(size=n) * 2, 1)  # (ties among them)
+        for u in (0.0, 0.3, 0.8, 1.0):
+            token, lp = S.sample_long_row(x, u, **kw)
+            ref_token, ref_lp, _ = S.sample_row(x, u, **kw)
+            assert token == ref_token and abs(lp - ref_lp) < 1e-12
+
+
 # ----------------------------------------------------------------- refusals
 def _err(code):
     assert code != _lib.OK
