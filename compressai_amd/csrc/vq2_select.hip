@@ -13,7 +13,7 @@
 // made in 64 bits; but a sigmoid of 64 bits for each of E experts costs several
 // times what the rest does.  Two kernels:
 //   rows   16 lanes a token, four tokens a wave.  Choices of 32 bits, cut to
-//          22 to 26 bits of their range with the expert's id below them, make
+//          23 to 26 bits of their range with the expert's id below them, make
 //          one word each: a lane sorts its own (a network of v_min / v_max_u32),
 //          rounds of a maximum over the 16 lanes (DPP) take the k + 2 best, and
 //          only those are computed in 64 bits and put in order by them.  The
@@ -443,8 +443,8 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
         z = row_sum(z);
     }
 
-    // c: choices of 32 bits, -inf where masked; off by less than `eps`
-    float c[N], eps = 0.0f;
+    // c: choices of 32 bits, -inf where masked
+    float c[N];
     if (by_score) {
         if (softmax) {
             float z = 0.0f;
