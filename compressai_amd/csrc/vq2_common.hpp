@@ -69,11 +69,13 @@ __device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float
 // number, which goes into the exponent, and f in [-1/2, 1/2]; 2^f = 1 + f g(f),
 // g interpolated at the Chebyshev nodes by a polynomial of degree 8 (2^f off
 // by 4e-14 of itself over the range, and exact at 0).  15 operations, against
-// some fifty of the library's exp().
-__device__ __forceinline__ double exp2_f64_in(double y)
+// some fifty of the library's exp().  The first function leaves the whole number
+// to its caller.
+__device__ __forceinline__ double exp2_f64_fraction(double y, uint32_t& whole)
 {
     constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
     const double t = y + MAGIC;
+    whole = (uint32_t)__builtin_bit_cast(uint64_t, t);
     const double f = y - (t - MAGIC);
     double g = 1.0203121156603192e-07;
     g = fma(g, f, 1.325522487537687e-06);
@@ -84,8 +86,13 @@ __device__ __forceinline__ double exp2_f64_in(double y)
     g = fma(g, f, 0.055504108664760424);
     g = fma(g, f, 0.2402265069581299);
     g = fma(g, f, 0.6931471805599453);
-    u32x2 p = __builtin_bit_cast(u32x2, fma(g, f, 1.0));
-    p.y += (uint32_t)__builtin_bit_cast(uint64_t, t) << 20;
+    return fma(g, f, 1.0);
+}
+__device__ __forceinline__ double exp2_f64_in(double y)
+{
+    uint32_t whole;
+    u32x2 p = __builtin_bit_cast(u32x2, exp2_f64_fraction(y, whole));
+    p.y += whole << 20;
     return __builtin_bit_cast(double, p);
 }
 // any y < 1023; below -1000, or NaN: 2^-1000

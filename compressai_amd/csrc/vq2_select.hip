@@ -61,14 +61,13 @@ struct SelectArgs {
     __device__ __forceinline__ int slots() const { return k + (shared_id >= 0 ? 1 : 0); }
 };
 
-// Scores of 64 bits: exp for x <= 0, and the sigmoid, 0 where e^-x is none of
-// 64 bits.  Below 2^-1000, which exp2_f64 does not pass, the power is taken 128
-// binary orders higher, and the product with 2^-128 rounds it to what 64 bits
-// have there.
+// Scores of 64 bits: exp for x <= 0, down to the steps of 2^-1074 that 64 bits
+// end in, and the sigmoid, 0 where e^-x is none of 64 bits.
 __device__ __forceinline__ double exp_f64(double x)
 {
-    const double y = fmax(x * LOG2E_F64, -1100.0);
-    return y < -1000.0 ? exp2_f64_in(y + 128.0) * 0x1p-128 : exp2_f64_in(y);
+    uint32_t whole;
+    const double p = exp2_f64_fraction(fmax(x * LOG2E_F64, -1100.0), whole);
+    return __builtin_amdgcn_ldexp(p, (int)whole);
 }
 // 1 / x of a normal x whose reciprocal is normal, to 2^-51: the instruction's
 // approximation and two Newton steps
@@ -80,8 +79,8 @@ __device__ __forceinline__ double reciprocal_f64(double x)
 }
 __device__ __forceinline__ double sigmoid_f64(double x)
 {
-    if (x < -700.0) return x < -709.78271289338397 ? 0.0 : exp_f64(x);
-    return reciprocal_f64(1.0 + exp2_f64(-x * LOG2E_F64));
+    const double e = exp_f64(-fabs(x)), r = reciprocal_f64(1.0 + e);
+    return x >= 0.0 ? r : x >= -709.78271289338397 ? e * r : 0.0;
 }
 
 // LDS written by a wave's lanes is read by its others.
@@ -238,18 +237,27 @@ __device__ void select_token(const SelectArgs& a, int64_t t, int lane, double* s
     for (int j = 0; j < RPL; j++)
         if (j * 64 + lane >= a.n_e) key[j] = -INFINITY;
     // the largest choice, and of its experts the lowest (choices that differ in
-    // their last bit alone are told apart: sigmoids close to 1 do)
+    // their last bit alone are told apart: sigmoids close to 1 do); `mine` is
+    // the lane's first expert with it
     int id = 0;
     for (int r = 0; r < a.k; r++) {
         double best = key[0];
 #pragma unroll
         for (int j = 1; j < RPL; j++) best = fmax(best, key[j]);
         best = wave_max_f64(best);
-        int at = 0;
+        int mine = RPL;
 #pragma unroll
-        for (int j = RPL - 1; j >= 0; j--) {
-            const uint64_t equal = __ballot(key[j] == best);
-            if (equal) at = j * 64 + __builtin_ctzll(equal);
+        for (int j = RPL - 1; j >= 0; j--)
+            if (key[j] == best) mine = j;
+        const uint64_t equal = __ballot(mine < RPL);
+        const int first = __builtin_ctzll(equal);
+        int at = __builtin_amdgcn_readlane(mine, first) * 64 + first;
+        if (equal & (equal - 1)) {
+#pragma unroll
+            for (int j = RPL - 1; j >= 0; j--) {
+                const uint64_t here = __ballot(mine == j);
+                if (here) at = j * 64 + __builtin_ctzll(here);
+            }
         }
 #pragma unroll
         for (int j = 0; j < RPL; j++)
@@ -374,10 +382,10 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
     } s_g[4];  // one a wave
     __shared__ float s_score[4][4][GROUPS ? 16 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15, quarter = lane >> 4;
-    const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * 4;
-    if (t0 >= a.tokens) return;
-    const int64_t t = t0 + quarter, tc = t < a.tokens ? t : a.tokens - 1;
-    const int64_t row = tc * a.stride;
+    const uint32_t tokens = (uint32_t)a.tokens, t0 = (blockIdx.x * 4 + wave) * 4;
+    if (t0 >= tokens) return;
+    const uint32_t t = t0 + quarter;
+    const int64_t row = min(t, tokens - 1) * a.stride;
     const bool softmax = a.scoring == VQ2_SCORE_SOFTMAX, biased = a.bias != nullptr;
     const bool by_score = biased || (GROUPS && a.group_score == VQ2_GROUP_TOP2);
     // unbiased logits of 16 bits and an id fit a word: no candidate is in doubt
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
     if (softmax && (biased || !a.renorm)) {
         z = 0.0;
 #pragma unroll
-        for (int j = 0; j < N; j++) z += l[j] == -INFINITY ? 0.0 : exp2_f64(((double)l[j] - (double)m) * LOG2E_F64);
+        for (int j = 0; j < N; j++) z += exp_f64((double)l[j] - (double)m);  // (-inf and NaN: 0)
         z = row_sum(z);
     }
 
@@ -607,22 +615,22 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
 
     const double tot = a.renorm ? row_sum(wins ? s : 0.0) : 1.0;
     unsure |= !(tot > 1e-290);  // (no normal reciprocal)
-    if (wins && !unsure && t < a.tokens) {
-        a.ids[t * a.slots() + rank] = id;
-        a.w[t * a.slots() + rank] = (float)(s * reciprocal_f64(tot) * (double)a.scale);
+    if (wins && !unsure && t < tokens) {
+        a.ids[(int64_t)t * a.slots() + rank] = id;
+        a.w[(int64_t)t * a.slots() + rank] = (float)(s * reciprocal_f64(tot) * (double)a.scale);
     }
     // the tokens that are left, by the whole wave
-    const uint64_t left = __ballot(unsure && t < a.tokens);
+    const uint64_t left = __ballot(unsure && t < tokens);
     for (int q = 0; q < 4; q++)
         if (left >> (16 * q) & 1) {
             wave_sync();
             select_token<LT, (N + 3) / 4>(a, t0 + q, lane, s_g[wave].token);
         }
     if constexpr (GATE) {
-        for (int q = 0; q < 4 && t0 + q < a.tokens; q++) write_shared(a, t0 + q, lane);
-    } else if (a.shared_id >= 0 && sub == 0 && t < a.tokens) {
-        a.ids[t * a.slots() + a.k] = (int32_t)a.shared_id;
-        a.w[t * a.slots() + a.k] = 1.0f;
+        for (int q = 0; q < 4 && t0 + q < tokens; q++) write_shared(a, t0 + q, lane);
+    } else if (a.shared_id >= 0 && sub == 0 && t < tokens) {
+        a.ids[(int64_t)t * a.slots() + a.k] = (int32_t)a.shared_id;
+        a.w[(int64_t)t * a.slots() + a.k] = 1.0f;
     }
 }
 
