@@ -137,7 +137,7 @@ struct Setting {
         const float mm = a.min_p_rows ? a.min_p_rows[b] : a.min_p;
         const bool greedy = !(t > 0.0f);
         c = greedy ? LOG2E_F64 : LOG2E_F64 / (double)fminf(t, FLT_MAX);
-        k = greedy ? 1u : kk > 0 && kk < a.vocab ? (uint32_t)kk : 0u;
+        k = greedy || kk == 1 ? 1u : kk > 0 && kk < a.vocab ? (uint32_t)kk : 0u;  // (1 also of one column, as launch() has it)
         top_p_on = pp < 1.0f;
         p = (double)fmaxf(pp, 0.0f);
         min_p_on = !(mm <= 0.0f);

@@ -473,3 +473,17 @@ def test_the_longest_vocabulary(dev, V, steep, dtype, kw):
     _check_long(K.vq_sample(x, u.to(dev), **kw), x, u, range(3), **kw)
     one = K.vq_sample(x[1:2], u[1:2].to(dev), **kw)
     _check_long(one, x[1:2], u[1:2], [0], **kw)
+
+
+@pytest.mark.parametrize("V", [1, 2, 3])
+@pytest.mark.parametrize("top_k", [1, 2, 3, 9])
+def test_a_top_k_of_the_whole_row(dev, V, top_k):
+    """top_k at the number of columns, one column's among them, beside the
+    other settings, common and by row."""
+    x = torch.tensor([[0.5, 2.0, 1.0], [float("nan"), 0.0, -1.0]])[:, :V].contiguous()
+    u = torch.tensor([0.3, 0.8])
+    for kw in (dict(), dict(top_p=0.5), dict(min_p=0.5), dict(top_p=0.0, min_p=1.0), dict(temperature=0.0), dict(temperature=1e-4, top_p=0.9)):
+        kw = dict(kw, top_k=top_k)
+        _check(K.vq_sample(x.to(dev), u.to(dev), **kw), x, u, **kw)
+        by_row = {k: torch.full((2,), v, dtype=torch.int32 if k == "top_k" else torch.float32) for k, v in kw.items()}
+        _check(K.vq_sample(x.to(dev), u.to(dev), **{k: v.to(dev) for k, v in by_row.items()}), x, u, **by_row)
