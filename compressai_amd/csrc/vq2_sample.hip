@@ -45,14 +45,17 @@
 //   256 x 151936 fp32, plain                  36 +  -  +  -  + 10.2
 //   256 x 151936 bf16, top-p 0.9, min-p       29 +  17 + 4.6 +  7.2
 // Small calls are chains of launches and, within them, of loads and barriers of
-// one row.  In large ones the stats launch is most: over fp32 it reads 4.3 TB/s
-// (a large copy reaches 4.9; with the exponentials left out, 29 us), over 16
-// bits its exponentials of 64 bits bound it (38.9 M in 29 us).
-// A row whose border lies among more entries than the list holds (flat to a
-// tenth, or ties) is gone over by one workgroup, bound by that compute unit's
-// instructions: 0.25 to 0.33 ms at 151936 logits, 0.48 with ties of which every
-// second column is one, 0.47 to 0.7 ms where it has both a longer top-k and a
-// top-p.
+// one row.  In large ones the stats launch is most.  Over fp32 it reads 4.3 TB/s
+// (a large copy reaches 4.9; with the exponentials left out, 29 us).  Over 16
+// bits vector instructions bound it: 21 a logit, issuing in 92 % of the busy
+// cycles (76 % over fp32); the table's lookups conflict in 20 % of them, hidden.
+// A row whose border lies among more entries than the list holds is gone over by
+// one workgroup, bound by that compute unit's instructions.  Those are rows flat
+// to a tenth, long ties, and rows whose top-p border is far down their tail (0.98
+// of a power law at a temperature of 1.15, 126731 entries of bf16 above the
+// border, 4000 in its bin): 0.25 to 0.33 ms at 151936 logits, 0.48 with ties of
+// which every second column is one, 0.47 to 0.7 ms where it has both a longer
+// top-k and a top-p.
 #include <float.h>
 
 #include "vq2_common.hpp"
