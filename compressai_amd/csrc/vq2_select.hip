@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(256, 4) select_rows_kernel(SelectArgs a)
         double token[GROUPS ? 16 * N : 1];  // (only groups take a whole wave there)
     } s_g[4];  // one a wave
     __shared__ float s_score[4][4][GROUPS ? 16 : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 15, quarter = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), sub = lane & 15, quarter = lane >> 4;
     const uint32_t tokens = (uint32_t)a.tokens, t0 = (blockIdx.x * 4 + wave) * 4;
     if (t0 >= tokens) return;
     const uint32_t t = t0 + quarter;
