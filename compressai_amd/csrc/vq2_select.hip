@@ -159,11 +159,23 @@ __device__ __forceinline__ float shared_weight(const SelectArgs& a, int64_t t, i
 // ------------------------------------------------------------- one wave a token
 constexpr double KEY_MASKED = -1e300;
 
+template <int CTRL>
+__device__ __forceinline__ double row_f64(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// (a round's chain is mostly this: within a row of 16 by rotations, then two
+// shuffles)
 __device__ __forceinline__ double wave_max_f64(double v)
 {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmax(v, __shfl_xor(v, off));
-    return v;
+    v = fmax(v, row_f64<0x128>(v));
+    v = fmax(v, row_f64<0x124>(v));
+    v = fmax(v, row_f64<0x122>(v));
+    v = fmax(v, row_f64<0x121>(v));
+    v = fmax(v, __shfl_xor(v, 16));
+    return fmax(v, __shfl_xor(v, 32));
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v)
@@ -338,13 +350,6 @@ __device__ __forceinline__ uint32_t row_max_u32(uint32_t v)
     v = max(v, (uint32_t)dpp_mov<0x124>((int)v));
     v = max(v, (uint32_t)dpp_mov<0x122>((int)v));
     return max(v, (uint32_t)dpp_mov<0x121>((int)v));
-}
-template <int CTRL>
-__device__ __forceinline__ double row_f64(double v)
-{
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_mov<CTRL>((int)(uint32_t)(b >> 32));
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 __device__ __forceinline__ double row_sum(double v)
 {
