@@ -23,25 +23,29 @@
 //   token  one wave a token, all of it in 64 bits.
 //
 // Kernel times on MI355X, us, of the rows kernel | the token kernel:
-//   1 token, 256 experts fp32, sigmoid, bias, 4 of 8 groups, gate    7.7 |   8.1
-//   64 tokens, 64 experts bf16, softmax                              3.8 |   5.0
-//   333 tokens, 160 experts fp32, softmax, 3 of 8 groups             7.9 |   7.7
-//   4096 tokens, 256 experts fp16, sigmoid, gate over 2048 (19 MB)   9.8 |    12
-//   16384 tokens, 256 experts bf16, sigmoid, bias, 4 of 8 groups    15.1 |    41
-//   32768 tokens, 512 experts fp32, sigmoid, bias (67 MB)           33.5 |   175
-// so the rows kernel takes every call it has room for (512 experts, 12 of them
-// chosen, 16 groups: candidates, groups and a lane's words in 16 lanes), some
-// hundred grouped tokens among them, where the two are equal to 3 %.  Few tokens
-// are bound by the chain of a wave (loads, sort, k + 2 rounds, 64-bit candidates:
-// 4 to 8 us); many by its vector instructions, which issue in 77 % of the cycles
-// of the last line and in 74 % of the one above: 51 an expert in the last line,
-// of which the sorting network of 32 words a lane is 10, and 2.0 TB/s of the 4.9
-// that a large copy reaches.
+//   1 token, 256 experts fp32, sigmoid, bias, 4 of 8 groups, gate    7.7 |   7.4
+//   64 tokens, 64 experts bf16, softmax                              3.9 |   4.3
+//   333 tokens, 160 experts fp32, softmax, 3 of 8 groups             8.0 |   7.2
+//   4096 tokens, 256 experts fp16, sigmoid, gate over 2048 (19 MB)  10.0 |    11
+//   16384 tokens, 256 experts bf16, sigmoid, bias, 4 of 8 groups    15.0 |    36
+//   32768 tokens, 512 experts fp32, sigmoid, bias (67 MB)           30.3 |   164
+// The rows kernel takes every call it has room for (512 experts, 12 of them
+// chosen, 16 groups: candidates, groups and a lane's words in 16 lanes).  Up to
+// some 500 tokens the token kernel is the faster one where there is a bias or a
+// gate (16 tokens of 256 experts bf16: 6.0 | 5.5, 7.7 | 5.8) and the slower one
+// without (4.8 | 5.4) or with 512 experts (7.3 | 11); but the two round weights
+// differently, and a limit between them would make a token's last bits depend on
+// how many others are routed with it.
+// Few tokens are bound by the chain of a wave (loads, sort, k + 2 rounds, 64-bit
+// candidates: 4 to 8 us); many by its vector instructions, which issue in 84 % of
+// the cycles of the last line and in 74 % of the one above: 51 an expert in the
+// last line, of which the sorting network of 32 words a lane is 10, and 2.2 TB/s
+// of the 4.9 that a large copy reaches.
 // Choices of 32 bits tell little apart where one expert's lies far from all
 // others: unbiased fp32 logits masked by a large finite number (-1e9, the type's
 // lowest) share one place, and every token goes on to 64 bits, four in turn in a
-// wave.  4096 tokens of 256 experts, half of them masked so: 27 us, against 5.7
-// with -inf or without masks and 10.8 by the token kernel alone.  (So does a bias
+// wave.  4096 tokens of 256 experts, half of them masked so: 24 us, against 5.7
+// with -inf or without masks and 9.8 by the token kernel alone.  (So does a bias
 // far below all others; 16-bit logits without a bias order exactly.)
 #include "vq2_common.hpp"
 #include "vq2_router.hpp"

@@ -294,3 +294,17 @@ def test_scores_near_the_end_of_64_bits(dev, E, k, G, low, high, form):
     kw["bias"] = kw["bias"].to(dev) if "bias" in kw else None
     more = dict(n_groups=G, topk_groups=max(1, G // 2), **kw)
     _check(K.vq_router_select(lg.to(dev), k, **more), lg, k, **more)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+@pytest.mark.parametrize("E,k,G", [(256, 8, 1), (160, 6, 8), (700, 20, 1)])
+def test_a_token_does_not_depend_on_the_others(dev, E, k, G, form):
+    """The same logits alone, among a few and among many: the same bits."""
+    lg = _logits(7999, 700, E, "fp32").to(dev)
+    kw = dict(form, n_groups=G, topk_groups=max(1, G // 2))
+    if kw.get("bias") is not None:
+        kw["bias"] = (torch.randn(E, generator=synth.gen(8000)) * kw["bias"]).to(dev)
+    ids, w = K.vq_router_select(lg, k, **kw)
+    for a, b in ((0, 1), (3, 9), (500, 700), (699, 700)):
+        part = K.vq_router_select(lg[a:b], k, **kw)
+        assert torch.equal(part[0], ids[a:b]) and torch.equal(part[1], w[a:b])
