@@ -17,6 +17,8 @@ LIB_PATH = PKG_DIR / "libvq2_amd.so"
 HEADER_PATH = PKG_DIR.parent / "include" / "vq2_amd.h"
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+DT_I8, DT_E4M3 = 3, 4
+ACT_SILU, ACT_GELU_TANH = 0, 1
 S2_NONE, S2_U8, S2_U16 = 0, 1, 2
 ID_I32, ID_I64 = 0, 1
 OK, ERR_ARG, ERR_HIP, ERR_UNSUPPORTED = 0, 1, 2, 3
@@ -102,6 +104,26 @@ SIGNATURES = {
     "vq2_dequant_rows": ([_vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _vp], _i32),
     "vq2_decode_idx": ([_vp, _i32, _i64, _vp, _vp], _i32),
     "vq2_unpack_fixed": ([_vp, _i64, _i32, _i64, _vp, _vp], _i32),
+    "vq2_add_rms_norm": ([_vp, _i32, _vp, _i64, _i64, _vp, _i32, _i32, _f32, _vp, _vp, _i64, _f32, _vp, _i32, _vp, _vp,
+                          _vp], _i32),
+    "vq2_add_rms_norm_backward_workspace": ([_i64, _i64], ctypes.c_size_t),
+    "vq2_add_rms_norm_backward": ([_vp, _i32, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _i32, _f32, _vp, _vp, _i64, _f32,
+                                   _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "vq2_head_loss_workspace": ([_i64, _i64, _i64, _i32, _i32], ctypes.c_size_t),
+    "vq2_head_loss": ([_vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _f32, _vp,
+                       _vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "vq2_head_loss_backward_workspace": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32], ctypes.c_size_t),
+    "vq2_head_loss_backward": ([_vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i64,
+                                _i64, _f32, _vp, _i32, _vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "vq2_gated_rows_workspace": ([_i64, _i64, _i64, _i32, _i32, _i32], ctypes.c_size_t),
+    "vq2_gated_rows": ([_vp, _i32, _vp, _i64, _vp, _i32, _vp, _vp, _i32, _i32, _i64, _f32, _i32, _vp, _i32, _vp,
+                        ctypes.c_size_t, _vp], _i32),
+    "vq2_gated_rows_backward_workspace": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32], ctypes.c_size_t),
+    "vq2_gated_rows_backward": ([_vp, _i32, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, _i32, _i64, _f32, _i32, _vp,
+                                 _i32, _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
+    "vq2_gemm_backward_workspace": ([_i64, _i64, _i64, _i32, _i32, _i32, _i32], ctypes.c_size_t),
+    "vq2_gemm_backward": ([_vp, _i32, _vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _f32, _vp,
+                           _i32, _vp, _vp, ctypes.c_size_t, _vp], _i32),
 }
 
 _lib = None

@@ -1138,4 +1138,341 @@ int vq2_unpack_fixed(const uint8_t* buf, int64_t nbytes, int bits, int64_t n, in
     return unpack_fixed_launch(buf, nbytes, bits, n, out, stream);
 }
 
+// --------------------------------------- the norm in front of packed products
+static int check_norm(const char* who, const NormCall& c, int64_t rows, int64_t n, int64_t hb)
+{
+    CHECK(rows >= 0 && rows <= VQ2_NORM_MAX_ROWS, "%s: rows=%lld not in [0, %lld]", who, (long long)rows,
+          (long long)VQ2_NORM_MAX_ROWS);
+    CHECK(n >= 1 && n <= VQ2_NORM_MAX_N, "%s: n=%lld not in [1, %d]", who, (long long)n, VQ2_NORM_MAX_N);
+    CHECK(dt_ok(c.x_dt) && dt_ok(c.w_dt), "%s: bad dtype", who);
+    CHECK(c.eps >= 0.0f, "%s: eps=%g is negative or NaN", who, (double)c.eps);
+    CHECK(c.weight, "%s: weight is NULL", who);
+    CHECK((uintptr_t)c.weight % dt_size(c.w_dt) == 0, "%s: weight must be aligned to its elements", who);
+    if (hb == 0) {
+        CHECK(!c.perm && !c.sign, "%s: perm / sign without hb", who);
+        return VQ2_OK;
+    }
+    CHECK(hb >= 64 && (hb & (hb - 1)) == 0 && n % hb == 0, "%s: hb=%lld must be a power of two from 64 on that divides n=%lld",
+          who, (long long)hb, (long long)n);
+    CHECK(((uintptr_t)c.x | (uintptr_t)c.residual | (uintptr_t)c.weight | (uintptr_t)c.y | (uintptr_t)c.h | (uintptr_t)c.dy |
+           (uintptr_t)c.dh) % 16 == 0, "%s: a rotated call's arrays must be 16-byte aligned", who);
+    CHECK((uintptr_t)c.perm % 4 == 0, "%s: perm must be aligned to its elements", who);
+    return VQ2_OK;
+}
+
+int vq2_add_rms_norm(const void* x, int x_dt, const void* residual, int64_t rows, int64_t n, const void* weight, int w_dt,
+                     int zero_centred, float eps, const int32_t* perm, const int8_t* sign, int64_t hb, float rht_scale,
+                     void* y, int y_dt, float* y_scale, void* h, void* stream)
+{
+    clear_error();
+    const NormCall c{x, residual, x_dt, rows, (int)n, weight, w_dt, zero_centred != 0, eps, perm, sign, (int)hb, rht_scale,
+                     y, y_dt, y_scale, h, nullptr, nullptr, stream};
+    const int r = check_norm("vq2_add_rms_norm", c, rows, n, hb);
+    if (r) return r;
+    const bool bits8 = y_dt == VQ2_DT_I8 || y_dt == VQ2_DT_E4M3;
+    CHECK(dt_ok(y_dt) || bits8, "vq2_add_rms_norm: bad y dtype");
+    CHECK(bits8 == (y_scale != nullptr), "vq2_add_rms_norm: y_scale must be given iff y has 8 bits");
+    if (rows == 0) return VQ2_OK;
+    CHECK(x && y, "vq2_add_rms_norm: NULL pointer argument");
+    CHECK(h || !residual, "vq2_add_rms_norm: h must be given with a residual");
+    CHECK(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)h) % dt_size(x_dt) == 0 &&
+          (bits8 || (uintptr_t)y % dt_size(y_dt) == 0) && (uintptr_t)y_scale % 4 == 0,
+          "vq2_add_rms_norm: arrays must be aligned to their elements");
+    return norm_launch(c);
+}
+
+size_t vq2_add_rms_norm_backward_workspace(int64_t rows, int64_t n)
+{
+    return rows < 0 || rows > VQ2_NORM_MAX_ROWS || n < 1 || n > VQ2_NORM_MAX_N ? 0 : norm_workspace_bytes(rows, n);
+}
+
+int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt, const void* dh, int64_t rows, int64_t n,
+                              const void* weight, int w_dt, int zero_centred, float eps, const int32_t* perm,
+                              const int8_t* sign, int64_t hb, float rht_scale, void* dx, float* dweight, void* workspace,
+                              size_t ws_bytes, void* stream)
+{
+    clear_error();
+    const NormCall c{h, nullptr, h_dt, rows, (int)n, weight, w_dt, zero_centred != 0, eps, perm, sign, (int)hb, rht_scale,
+                     dx, dy_dt, nullptr, nullptr, dy, dh, stream};
+    const int r = check_norm("vq2_add_rms_norm_backward", c, rows, n, hb);
+    if (r) return r;
+    CHECK(dt_ok(dy_dt), "vq2_add_rms_norm_backward: bad dy dtype");
+    CHECK((uintptr_t)dweight % 4 == 0, "vq2_add_rms_norm_backward: dweight must be aligned to its elements");
+    if (rows == 0 && !dweight) return VQ2_OK;
+    if (rows) {
+        CHECK(dy && h && dx, "vq2_add_rms_norm_backward: NULL pointer argument");
+        CHECK(((uintptr_t)h | (uintptr_t)dh | (uintptr_t)dx) % dt_size(h_dt) == 0 && (uintptr_t)dy % dt_size(dy_dt) == 0,
+              "vq2_add_rms_norm_backward: arrays must be aligned to their elements");
+    }
+    const size_t need = dweight ? norm_workspace_bytes(rows, n) : 0;
+    CHECK(need == 0 || (workspace && ws_bytes >= need), "vq2_add_rms_norm_backward: workspace of %zu bytes needed, got %zu", need,
+          ws_bytes);
+    CHECK((uintptr_t)workspace % 256 == 0, "vq2_add_rms_norm_backward: workspace must be 256-byte aligned");
+    return norm_grad_launch(c, dweight, workspace);
+}
+
+// ------------------------------------------- many-row products on panels
+// (what leaves through an fp16 panel has 16 bits)
+static bool grad_dt(int dt) { return dt == VQ2_DT_F16 || dt == VQ2_DT_BF16; }
+
+static bool bits8_dt(int dt) { return dt == VQ2_DT_I8 || dt == VQ2_DT_E4M3; }
+
+static PanelCall panel_sizes(int what, int64_t tokens, int64_t rows, int nmat, int64_t n, int s2, int cb_dt, int y_dt,
+                             bool scale_grad)
+{
+    PanelCall c{};
+    c.what = what;
+    c.tokens = tokens;
+    c.rows = rows;
+    c.nmat = nmat;
+    c.n = n;
+    c.s2 = s2;
+    c.cb_dt = cb_dt;
+    c.y_dt = y_dt;
+    c.ds[0] = scale_grad ? (float*)1 : nullptr;
+    return c;
+}
+
+static bool panel_sizes_ok(int64_t tokens, int64_t rows, int64_t n)
+{
+    return tokens >= 0 && tokens <= VQ2_PANEL_MAX_TOKENS && rows >= 1 && rows <= VQ2_PANEL_MAX_ROWS && n >= 64 && n % 64 == 0 &&
+           n <= VQ2_PANEL_MAX_N;
+}
+
+static size_t panel_workspace(int what, int64_t tokens, int64_t rows, int nmat, int64_t n, int s2, int cb_dt, int y_dt,
+                              int scale_grad)
+{
+    if (!panel_sizes_ok(tokens, rows, n)) return 0;
+    return panel_workspace_bytes(panel_sizes(what, tokens, rows, nmat, n, s2, cb_dt, y_dt, scale_grad != 0));
+}
+
+// the checks all panel entries share; x is not read where x_used is false
+static int check_panel(const PanelCall& c, bool x_used, bool x8)
+{
+    const char* who = c.who;
+    CHECK(c.tokens >= 0 && c.tokens <= VQ2_PANEL_MAX_TOKENS, "%s: tokens=%lld not in [0, %lld]", who, (long long)c.tokens,
+          (long long)VQ2_PANEL_MAX_TOKENS);
+    CHECK(c.rows >= 1 && c.rows <= VQ2_PANEL_MAX_ROWS, "%s: out_rows=%lld not in [1, %d]", who, (long long)c.rows,
+          VQ2_PANEL_MAX_ROWS);
+    CHECK(c.n >= 64 && c.n % 64 == 0 && c.n <= VQ2_PANEL_MAX_N, "%s: n=%lld must be a multiple of 64 up to %d", who,
+          (long long)c.n, VQ2_PANEL_MAX_N);
+    int r = check_codebooks(c.s2, c.cb0, c.cb1, c.cb_dt);
+    if (r) return r;
+    CHECK(dt_ok(c.s_dt), "%s: bad scale dtype", who);
+    for (int k = 0; k < c.nmat; k++) {
+        CHECK(c.mat[k].i0 && c.mat[k].scale, "%s: NULL planes or scales", who);
+        CHECK((c.s2 == VQ2_S2_NONE) == (c.mat[k].i1 == nullptr), "%s: idx1 must be given iff s2_kind != NONE", who);
+        CHECK((uintptr_t)c.mat[k].i0 % 2 == 0 && (c.s2 != VQ2_S2_U16 || (uintptr_t)c.mat[k].i1 % 2 == 0) &&
+              (uintptr_t)c.mat[k].scale % dt_size(c.s_dt) == 0, "%s: planes and scales must be aligned to their elements", who);
+    }
+    for (int k = 0; k < 2; k++) CHECK((uintptr_t)c.ds[k] % 4 == 0, "%s: gradients of scales must be aligned to their elements", who);
+    if (c.tokens == 0) return VQ2_OK;
+    if (x_used) {
+        CHECK(c.x, "%s: x is NULL", who);
+        CHECK(c.x_dt == VQ2_DT_F16 || c.x_dt == VQ2_DT_BF16 || (x8 && bits8_dt(c.x_dt)),
+              "%s: x must hold fp16 or bf16%s values", who, x8 ? ", or 8-bit" : "");
+        CHECK(bits8_dt(c.x_dt) == (c.x_scale != nullptr), "%s: x_scale must be given iff x has 8 bits", who);
+        CHECK((uintptr_t)c.x % 16 == 0, "%s: x must be 16-byte aligned", who);
+        CHECK((uintptr_t)c.x_scale % 4 == 0, "%s: x_scale must be aligned to its elements", who);
+    }
+    const size_t need = panel_workspace_bytes(c);
+    CHECK(c.workspace && c.ws_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, c.ws_bytes);
+    CHECK((uintptr_t)c.workspace % 256 == 0, "%s: workspace must be 256-byte aligned", who);
+    return VQ2_OK;
+}
+
+static void set_head(PanelCall& c, const int16_t* idx0, const void* idx1, const void* cb0, const void* cb1, const void* scale,
+                     int s_dt, float rs)
+{
+    c.mat[0] = PanelMatCall{idx0, idx1, scale};
+    c.cb0 = cb0;
+    c.cb1 = cb1;
+    c.s_dt = s_dt;
+    c.rs = rs;
+}
+
+size_t vq2_head_loss_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt)
+{
+    return panel_workspace(PANEL_STATS, tokens, out_rows, 1, n, s2_kind, cb_dt, VQ2_DT_F32, 0);
+}
+
+int vq2_head_loss(const void* x, int x_dt, const float* x_scale, int64_t tokens, const int64_t* targets, int64_t ignore_index,
+                  const int16_t* idx0, const void* idx1, int s2_kind, const void* cb0, const void* cb1, int cb_dt,
+                  const void* scale, int s_dt, int64_t out_rows, int64_t n, float rs, float* loss, float* lse, void* workspace,
+                  size_t ws_bytes, void* stream)
+{
+    clear_error();
+    PanelCall c = panel_sizes(PANEL_STATS, tokens, out_rows, 1, n, s2_kind, cb_dt, VQ2_DT_F32, false);
+    c.who = "vq2_head_loss";
+    c.x = x;
+    c.x_dt = x_dt;
+    c.x_scale = x_scale;
+    set_head(c, idx0, idx1, cb0, cb1, scale, s_dt, rs);
+    c.target = targets;
+    c.ignore = ignore_index;
+    c.loss = loss;
+    c.lse_out = lse;
+    c.workspace = workspace;
+    c.ws_bytes = ws_bytes;
+    c.stream = stream;
+    const int r = check_panel(c, true, true);
+    if (r) return r;
+    if (tokens == 0) return VQ2_OK;
+    CHECK(targets && loss && lse, "vq2_head_loss: NULL pointer argument");
+    CHECK((uintptr_t)targets % 8 == 0 && ((uintptr_t)loss | (uintptr_t)lse) % 4 == 0,
+          "vq2_head_loss: arrays must be aligned to their elements");
+    return panel_launch(c);
+}
+
+size_t vq2_head_loss_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                        int scale_grad)
+{
+    return panel_workspace(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, scale_grad);
+}
+
+int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_t* targets, int64_t ignore_index,
+                           const float* lse, const float* dloss, const int16_t* idx0, const void* idx1, int s2_kind,
+                           const void* cb0, const void* cb1, int cb_dt, const void* scale, int s_dt, int64_t out_rows, int64_t n,
+                           float rs, void* dx, int dx_dt, float* dscale, void* workspace, size_t ws_bytes, void* stream)
+{
+    clear_error();
+    PanelCall c = panel_sizes(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, false);
+    c.who = "vq2_head_loss_backward";
+    c.x = x;
+    c.x_dt = x_dt;
+    set_head(c, idx0, idx1, cb0, cb1, scale, s_dt, rs);
+    c.target = targets;
+    c.ignore = ignore_index;
+    c.lse = lse;
+    c.dloss = dloss;
+    c.y = dx;
+    c.ds[0] = dscale;
+    c.workspace = workspace;
+    c.ws_bytes = ws_bytes;
+    c.stream = stream;
+    const int r = check_panel(c, true, false);
+    if (r) return r;
+    CHECK(grad_dt(dx_dt), "vq2_head_loss_backward: dx must hold fp16 or bf16 values");
+    if (tokens) {
+        CHECK(targets && lse && dloss && dx, "vq2_head_loss_backward: NULL pointer argument");
+        CHECK((uintptr_t)targets % 8 == 0 && ((uintptr_t)lse | (uintptr_t)dloss) % 4 == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
+              "vq2_head_loss_backward: arrays must be aligned to their elements");
+    }
+    return panel_launch(c);
+}
+
+static int set_gated(PanelCall& c, const vq2_seg* mats, const void* cb0, const void* cb1, int s_dt, float rs, int act)
+{
+    for (int k = 0; k < 2; k++) c.mat[k] = PanelMatCall{mats[k].idx0, mats[k].idx1, mats[k].scale};
+    c.cb0 = cb0;
+    c.cb1 = cb1;
+    c.s_dt = s_dt;
+    c.rs = rs;
+    c.act = act;
+    CHECK(mats[0].out_rows == mats[1].out_rows, "%s: gate has %lld rows, up %lld", c.who, (long long)mats[0].out_rows,
+          (long long)mats[1].out_rows);
+    CHECK(act == VQ2_ACT_SILU || act == VQ2_ACT_GELU_TANH, "%s: unknown activation %d", c.who, act);
+    return VQ2_OK;
+}
+
+size_t vq2_gated_rows_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int y_dt)
+{
+    return panel_workspace(PANEL_GATED, tokens, out_rows, 2, n, s2_kind, cb_dt, y_dt, 0);
+}
+
+int vq2_gated_rows(const void* x, int x_dt, const float* x_scale, int64_t tokens, const vq2_seg* mats, int s2_kind,
+                   const void* cb0, const void* cb1, int cb_dt, int s_dt, int64_t n, float rs, int act, void* y, int y_dt,
+                   void* workspace, size_t ws_bytes, void* stream)
+{
+    clear_error();
+    CHECK(mats, "vq2_gated_rows: mats is NULL");
+    PanelCall c = panel_sizes(PANEL_GATED, tokens, mats[0].out_rows, 2, n, s2_kind, cb_dt, y_dt, false);
+    c.who = "vq2_gated_rows";
+    c.x = x;
+    c.x_dt = x_dt;
+    c.x_scale = x_scale;
+    c.y = y;
+    c.workspace = workspace;
+    c.ws_bytes = ws_bytes;
+    c.stream = stream;
+    int r = set_gated(c, mats, cb0, cb1, s_dt, rs, act);
+    if (r) return r;
+    CHECK(dt_ok(y_dt), "vq2_gated_rows: bad y dtype");
+    r = check_panel(c, true, true);
+    if (r) return r;
+    if (tokens == 0) return VQ2_OK;
+    CHECK(y && (uintptr_t)y % dt_size(y_dt) == 0, "vq2_gated_rows: y is NULL or not aligned to its elements");
+    return panel_launch(c);
+}
+
+size_t vq2_gated_rows_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                         int scale_grad)
+{
+    return panel_workspace(PANEL_DGATED, tokens, out_rows, 2, n, s2_kind, cb_dt, dx_dt, scale_grad);
+}
+
+int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens, const vq2_seg* mats, int s2_kind,
+                            const void* cb0, const void* cb1, int cb_dt, int s_dt, int64_t n, float rs, int act, void* dx,
+                            int dx_dt, float* dgate, float* dup, void* workspace, size_t ws_bytes, void* stream)
+{
+    clear_error();
+    CHECK(mats, "vq2_gated_rows_backward: mats is NULL");
+    PanelCall c = panel_sizes(PANEL_DGATED, tokens, mats[0].out_rows, 2, n, s2_kind, cb_dt, dx_dt, false);
+    c.who = "vq2_gated_rows_backward";
+    c.x = x;
+    c.x_dt = x_dt;
+    c.y = dx;
+    c.dy = dy;
+    c.dy_dt = dy_dt;
+    c.ds[0] = dgate;
+    c.ds[1] = dup;
+    c.workspace = workspace;
+    c.ws_bytes = ws_bytes;
+    c.stream = stream;
+    int r = set_gated(c, mats, cb0, cb1, s_dt, rs, act);
+    if (r) return r;
+    CHECK(dt_ok(dy_dt), "vq2_gated_rows_backward: bad dy dtype");
+    CHECK(grad_dt(dx_dt), "vq2_gated_rows_backward: dx must hold fp16 or bf16 values");
+    CHECK((dgate == nullptr) == (dup == nullptr), "vq2_gated_rows_backward: dgate and dup must be given both or neither");
+    r = check_panel(c, true, false);
+    if (r) return r;
+    if (tokens)
+        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
+              "vq2_gated_rows_backward: dy or dx is NULL or not aligned to its elements");
+    return panel_launch(c);
+}
+
+size_t vq2_gemm_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                   int scale_grad)
+{
+    return panel_workspace(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, scale_grad);
+}
+
+int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens, const int16_t* idx0, const void* idx1,
+                      int s2_kind, const void* cb0, const void* cb1, int cb_dt, const void* scale, int s_dt, int64_t out_rows,
+                      int64_t n, float rs, void* dx, int dx_dt, float* dscale, void* workspace, size_t ws_bytes, void* stream)
+{
+    clear_error();
+    PanelCall c = panel_sizes(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, false);
+    c.who = "vq2_gemm_backward";
+    c.x = x;
+    c.x_dt = x_dt;
+    set_head(c, idx0, idx1, cb0, cb1, scale, s_dt, rs);
+    c.y = dx;
+    c.dy = dy;
+    c.dy_dt = dy_dt;
+    c.ds[0] = dscale;
+    c.workspace = workspace;
+    c.ws_bytes = ws_bytes;
+    c.stream = stream;
+    const int r = check_panel(c, dscale != nullptr, false);
+    if (r) return r;
+    CHECK(dt_ok(dy_dt), "vq2_gemm_backward: bad dy dtype");
+    CHECK(grad_dt(dx_dt), "vq2_gemm_backward: dx must hold fp16 or bf16 values");
+    if (tokens)
+        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
+              "vq2_gemm_backward: dy or dx is NULL or not aligned to its elements");
+    return panel_launch(c);
+}
+
 }  // extern "C"

@@ -409,6 +409,75 @@ int decode_launch(const void* in, int is_u8, int64_t count, int32_t* out, void* 
 
 int unpack_fixed_launch(const uint8_t* buf, int64_t nbytes, int bits, int64_t n, int16_t* out, void* stream);
 
+// The norm in front of packed products, and its backward pass (vq2_norm.hip).
+struct NormCall {
+    const void* x;         // backward: the forward's h
+    const void* residual;  // or null
+    int x_dt;              // of x, residual and h (backward: of h, dh and dx)
+    int64_t rows;
+    int n;
+    const void* weight;
+    int w_dt;
+    int zero_centred;
+    float eps;
+    const int32_t* perm;
+    const int8_t* sign;
+    int hb;  // 0: not rotated
+    float rht_scale;
+    void* y;  // backward: dx
+    int y_dt;  // of y (backward: of dy)
+    float* y_scale;
+    void* h;         // or null
+    const void* dy;  // backward
+    const void* dh;
+    void* stream;
+};
+size_t norm_workspace_bytes(int64_t rows, int64_t n);
+int norm_launch(const NormCall& c);
+int norm_grad_launch(const NormCall& c, float* dw, void* workspace);
+
+// Many-row products on panels (vq2_panel.hip): the gated block, the head's
+// loss, and the gradients through packed matrices.
+struct PanelMatCall {
+    const int16_t* i0;
+    const void* i1;
+    const void* scale;
+};
+struct PanelCall {
+    const char* who;  // entry, for messages
+    int what;         // PANEL_*
+    const void* x;    // [tokens][n], rotated
+    int x_dt;         // also VQ2_DT_I8 / VQ2_DT_E4M3, with x_scale
+    const float* x_scale;
+    int64_t tokens, n;
+    PanelMatCall mat[2];
+    int nmat;
+    int64_t rows;  // of each matrix
+    int s2;
+    const void* cb0;
+    const void* cb1;
+    int cb_dt, s_dt;
+    float rs;
+    int act;
+    void* y;  // the block's activation, or the gradient of x
+    int y_dt;
+    const void* dy;  // upstream gradient [tokens][rows]
+    int dy_dt;
+    const int64_t* target;
+    int64_t ignore;
+    const float* lse;
+    const float* dloss;
+    float* loss;
+    float* lse_out;
+    float* ds[2];  // the row scales' gradients, or null
+    void* workspace;
+    size_t ws_bytes;
+    void* stream;
+};
+enum { PANEL_STATS, PANEL_DLOGIT, PANEL_GATED, PANEL_DGATED, PANEL_PRODUCT };
+size_t panel_workspace_bytes(const PanelCall& c);
+int panel_launch(const PanelCall& c);
+
 inline bool dt_ok(int dt) { return dt == VQ2_DT_F32 || dt == VQ2_DT_F16 || dt == VQ2_DT_BF16; }
 inline int64_t dt_size(int dt) { return dt == VQ2_DT_F32 ? 4 : 2; }
 

@@ -1,0 +1,518 @@
+// vq2_norm.hip -- the norm in front of packed products: residual addition,
+// root mean square, weight, and the rotation the product wants, in one pass
+// over the rows; and its backward pass.
+//
+//   h = x + residual,  r = (mean(h^2) + eps)^-1/2,  u = h r w
+//   y = u, or R u with R = blockdiag(H_hb) S P scale (vq2_rht), in 16 or 32 bits,
+//       or in 8 bits under a scale for each row
+//
+//   g = R^T dy,  dx = dh + r g w - h r^3 mean(g w h),  dw = sum over rows of g h r
+//
+// Bound by HBM: every element is read once and written once, the row stays in
+// registers between.  A thread holds 8 neighbouring values (16-byte loads) of each
+// 2048: the transform's first 3 stages are in its registers, the next 6 are
+// exchanges between lanes, the ones above (blocks of 1024 and 2048) one pass
+// through LDS between the waves, blocks above 2048 in registers again.  The
+// permutation goes through LDS, too.  A workgroup takes rows in turn and loads
+// its part of the weights and tables once.  All
+// arithmetic is fp32; h is rounded where it is stored, y is made from the
+// unrounded sum.
+#include <algorithm>
+
+#include "vq2_internal.hpp"
+#include "vq2_panel.hpp"
+
+namespace vq2 {
+
+namespace {
+
+constexpr int NT = 256;  // threads of a workgroup
+
+// lane i <- lane i ^ 4, i ^ 8 within a row of 16
+__device__ __forceinline__ float dpp_xor4(float v)
+{
+    // row_half_mirror is i ^ 7, quad_perm [3,2,1,0] i ^ 3
+    return __int_as_float(dpp_mov<0x1B>(dpp_mov<0x141>(__float_as_int(v))));
+}
+__device__ __forceinline__ float dpp_xor8(float v) { return __int_as_float(dpp_mov<0x128>(__float_as_int(v))); }  // row_ror:8
+
+// One butterfly stage between lanes: the lane whose bit is clear takes the
+// sum, the other the difference.
+template <class X>
+__device__ __forceinline__ void lane_stage(float (&v)[8], bool high, X other)
+{
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float o = other(v[k]);
+        v[k] = high ? o - v[k] : v[k] + o;
+    }
+}
+
+// Hadamard transform of blocks of hb values; the row's value 8 (c TPR + id) + k
+// is v[c][k] of its thread id.  s: V * 8 * TPR floats of the row (TPR == 256).
+template <int V, int TPR>
+__device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float* s)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+#pragma unroll
+        for (int st = 1; st < 8; st *= 2)
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (!(k & st)) {
+                    const float a = v[c][k], b = v[c][k + st];
+                    v[c][k] = a + b;
+                    v[c][k + st] = a - b;
+                }
+        // (blocks have 64 values or more)
+        lane_stage(v[c], lane & 1, [](float a) { return dpp_xor1(a); });
+        lane_stage(v[c], lane & 2, [](float a) { return dpp_xor2(a); });
+        lane_stage(v[c], lane & 4, [](float a) { return dpp_xor4(a); });
+        if (hb >= 128) lane_stage(v[c], lane & 8, [](float a) { return dpp_xor8(a); });
+        if (hb >= 256) lane_stage(v[c], lane & 16, [](float a) { return swz_xor16(a); });
+        if (hb >= 512) lane_stage(v[c], lane & 32, [](float a) { return xor32(a); });
+    }
+    if (TPR == 64 || hb < 1024) return;
+    // between the waves: value of wave w gets sum over w' of +- theirs
+    const int w = id >> 6;
+    f32x4_t* p = (f32x4_t*)s;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        p[(c * 2 + 0) * TPR + id] = f32x4_t{v[c][0], v[c][1], v[c][2], v[c][3]};
+        p[(c * 2 + 1) * TPR + id] = f32x4_t{v[c][4], v[c][5], v[c][6], v[c][7]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < V; c++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f32x4_t* q = p + (c * 2 + h) * TPR + (id & 63);
+            f32x4_t o;
+            if (hb == 1024) {
+                const f32x4_t a = q[(w & ~1) * 64], b = q[(w | 1) * 64];
+                o = w & 1 ? a - b : a + b;
+            } else {
+                const f32x4_t a = q[0], b = q[64], d = q[128], e = q[192];
+                const f32x4_t lo = w & 1 ? a - b : a + b, hi = w & 1 ? d - e : d + e;
+                o = w & 2 ? lo - hi : lo + hi;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[c][4 * h + k] = o[k];
+        }
+    // blocks above 2048: between a thread's own parts
+#pragma unroll
+    for (int st = 1; st < V; st *= 2) {
+        if (hb < 4096 * st) break;
+#pragma unroll
+        for (int c = 0; c < V; c++)
+            if (!(c & st) && c + st < V)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float a = v[c][k], b = v[c + st][k];
+                    v[c][k] = a + b;
+                    v[c + st][k] = a - b;
+                }
+    }
+}
+
+// a value every thread of the row has a part of; s: one word for each wave
+template <int TPR, class Op>
+__device__ __forceinline__ float row_reduce(float v, float* s, Op op)
+{
+    v = op(v, dpp_xor1(v));
+    v = op(v, dpp_xor2(v));
+    v = op(v, dpp_half_mirror(v));
+    v = op(v, dpp_row_mirror(v));
+    v = op(v, swz_xor16(v));
+    v = op(v, xor32(v));
+    if (TPR == 64) return v;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = op(op(s[0], s[1]), op(s[2], s[3]));
+    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ float add_op(float a, float b) { return a + b; }
+// maximum of magnitudes by their bits: a NaN is above everything and stays
+__device__ __forceinline__ float bits_op(float a, float b)
+{
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+}
+
+// A thread's part of a row.  VEC: 8 neighbouring values in each of the V parts,
+// by 16-byte accesses; otherwise value (8 c + k) TPR + id, one by one.
+template <int V, int TPR, bool VEC>
+__device__ __forceinline__ int place(int c, int k, int id)
+{
+    return VEC ? (c * TPR + id) * 8 + k : (c * 8 + k) * TPR + id;
+}
+
+template <int V, int TPR, bool VEC>
+__device__ __forceinline__ void load_row(float (&v)[V][8], const void* p, int dt, int64_t row, int n, int id)
+{
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        if constexpr (VEC) {
+            Eight e = {{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}};
+            if (place<V, TPR, VEC>(c, 0, id) < n) e = load8(p, dt, row * n + place<V, TPR, VEC>(c, 0, id));
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[c][k] = e.v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = place<V, TPR, VEC>(c, k, id);
+                v[c][k] = i < n ? load_as_f32(p, dt, row * n + i) : 0.0f;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (&v)[8])
+{
+    if (dt == VQ2_DT_F32) {
+        *(f32x4_t*)((float*)p + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *(f32x4_t*)((float*)p + i + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else if (dt == VQ2_DT_F16) {
+        half8_t h;
+#pragma unroll
+        for (int k = 0; k < 8; k++) h[k] = (_Float16)v[k];
+        *(half8_t*)((uint16_t*)p + i) = h;
+    } else {
+        u32x4 u;
+#pragma unroll
+        for (int k = 0; k < 4; k++) u[k] = f32_to_bf16_bits(v[2 * k]) | (uint32_t)f32_to_bf16_bits(v[2 * k + 1]) << 16;
+        *(u32x4*)((uint16_t*)p + i) = u;
+    }
+}
+
+// q = v * inv rounded to the nearest (ties to even), 8 bits each
+__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, int dt)
+{
+    if (dt == VQ2_DT_I8) {
+        auto q = [](float v) { return (uint32_t)(int)fminf(fmaxf(rintf(v), -127.0f), 127.0f) & 0xFFu; };
+        return q(a) | q(b) << 8 | q(c) << 16 | q(d) << 24;
+    }
+    auto cl = [](float v) { return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f); };
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), r, true);
+    return (uint32_t)r;
+}
+
+template <int V, int TPR, bool VEC>
+__device__ __forceinline__ void store_row(const float (&v)[V][8], void* p, int dt, int64_t row, int n, int id, float inv)
+{
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        if constexpr (VEC) {
+            const int i = place<V, TPR, VEC>(c, 0, id);
+            if (i >= n) continue;
+            if (dt <= VQ2_DT_BF16) store8(p, dt, row * n + i, v[c]);
+            else
+                *(u32x2*)((uint8_t*)p + row * n + i) =
+                    u32x2{quant4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv, dt),
+                          quant4(v[c][4] * inv, v[c][5] * inv, v[c][6] * inv, v[c][7] * inv, dt)};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = place<V, TPR, VEC>(c, k, id);
+                if (i >= n) continue;
+                if (dt <= VQ2_DT_BF16) store_from_f32(p, dt, row * n + i, v[c][k]);
+                else ((uint8_t*)p)[row * n + i] = (uint8_t)quant4(v[c][k] * inv, 0.0f, 0.0f, 0.0f, dt);
+            }
+        }
+    }
+}
+
+// Rotation tables of a thread's values (VEC), two entries a word: the place
+// the value comes from (13 bits) and its sign above; no place of the row
+// where the permutation's entry is none, which gives NaN as in vq2_rht.
+constexpr uint32_t NO_PLACE = 0x7FFF;
+template <int V, int TPR>
+__device__ __forceinline__ void load_tables(uint32_t (&tab)[V][4], const NormCall& a, int id)
+{
+#pragma unroll
+    for (int c = 0; c < V; c++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = (c * TPR + id) * 8 + k;
+            uint32_t p = NO_PLACE, neg = 0;
+            if (i < a.n) {
+                p = a.perm ? (uint32_t)a.perm[i] : (uint32_t)i;
+                if (p >= (uint32_t)a.n) p = NO_PLACE;
+                neg = a.sign && a.sign[i] < 0 ? 0x8000u : 0u;
+            }
+            tab[c][k >> 1] = (k & 1 ? tab[c][k >> 1] : 0) | (p | neg) << (16 * (k & 1));
+        }
+}
+__device__ __forceinline__ uint32_t entry(const uint32_t (&tab)[4], int k) { return tab[k >> 1] >> (16 * (k & 1)) & 0xFFFFu; }
+
+template <int DT, int V, int TPR, bool VEC, bool ROT>
+__global__ void __launch_bounds__(NT) norm_kernel(const NormCall a, int64_t row_step)
+{
+    constexpr int RW = NT / TPR;  // rows of a workgroup
+    __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
+    __shared__ float s_red[8];
+    const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
+    float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
+    float w[V][8];
+    uint32_t tab[V][4];
+    const float off = a.zero_centred ? 1.0f : 0.0f;
+    load_row<V, TPR, VEC>(w, a.weight, a.w_dt, 0, a.n, id);
+    if constexpr (ROT) load_tables<V, TPR>(tab, a, id);
+    for (int64_t r0 = (int64_t)blockIdx.x * RW; r0 < a.rows; r0 += row_step) {
+        const int64_t row = r0 + rw;
+        const bool live = row < a.rows;  // (rows of a workgroup: whole waves)
+        const int64_t at = live ? row : a.rows - 1;
+        float h[V][8], e[V][8];
+        load_row<V, TPR, VEC>(h, a.x, DT, at, a.n, id);
+        if (a.residual) {
+            load_row<V, TPR, VEC>(e, a.residual, DT, at, a.n, id);
+#pragma unroll
+            for (int c = 0; c < V; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) h[c][k] += e[c][k];
+        }
+        if (a.h && live) store_row<V, TPR, VEC>(h, a.h, DT, row, a.n, id, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum += h[c][k] * h[c][k];
+        sum = row_reduce<TPR>(sum, s_red, add_op);
+        const float r = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+#pragma unroll
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) h[c][k] = h[c][k] * r * (w[c][k] + off);
+        if constexpr (ROT) {
+#pragma unroll
+            for (int c = 0; c < V; c++) {
+                f32x4_t* p = (f32x4_t*)(s + (c * TPR + id) * 8);
+                p[0] = f32x4_t{h[c][0], h[c][1], h[c][2], h[c][3]};
+                p[1] = f32x4_t{h[c][4], h[c][5], h[c][6], h[c][7]};
+            }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < V; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t e = entry(tab[c], k), p = e & NO_PLACE;
+                    const float v = s[p == NO_PLACE ? 0 : p];
+                    h[c][k] = p == NO_PLACE ? __builtin_nanf("") : e & 0x8000u ? -v : v;
+                }
+            hadamard<V, TPR>(h, a.hb, id, s);
+#pragma unroll
+            for (int c = 0; c < V; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) h[c][k] *= a.rht_scale;
+            __syncthreads();  // the next row's values go where these were
+        }
+        float inv = 0.0f;
+        if (a.y_dt > VQ2_DT_BF16) {
+            float m = 0.0f;
+#pragma unroll
+            for (int c = 0; c < V; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (place<V, TPR, VEC>(c, k, id) < a.n) m = bits_op(m, fabsf(h[c][k]));
+            m = row_reduce<TPR>(m, s_red, bits_op);
+            const float top = a.y_dt == VQ2_DT_I8 ? 127.0f : 448.0f;
+            inv = m > 0.0f ? top / m : 0.0f;
+            if (live && id == 0) a.y_scale[row] = m / top;
+        }
+        if (live) store_row<V, TPR, VEC>(h, a.y, a.y_dt, row, a.n, id, inv);
+    }
+}
+
+template <int DT, int V, int TPR, bool VEC, bool ROT>
+__global__ void __launch_bounds__(NT) norm_grad_kernel(const NormCall a, int64_t row_step, float* part)
+{
+    constexpr int RW = NT / TPR;
+    __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
+    __shared__ float s_red[8];
+    const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
+    float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
+    float w[V][8], dw[V][8];
+    uint32_t tab[V][4];
+    const float off = a.zero_centred ? 1.0f : 0.0f;
+    load_row<V, TPR, VEC>(w, a.weight, a.w_dt, 0, a.n, id);
+    if constexpr (ROT) load_tables<V, TPR>(tab, a, id);
+#pragma unroll
+    for (int c = 0; c < V; c++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) dw[c][k] = 0.0f;
+    for (int64_t r0 = (int64_t)blockIdx.x * RW; r0 < a.rows; r0 += row_step) {
+        const int64_t row = r0 + rw;
+        const bool live = row < a.rows;
+        const int64_t at = live ? row : a.rows - 1;
+        float h[V][8], g[V][8];
+        if (a.y_dt == DT) load_row<V, TPR, VEC>(g, a.dy, DT, at, a.n, id);
+        else load_row<V, TPR, VEC>(g, a.dy, a.y_dt, at, a.n, id);
+        load_row<V, TPR, VEC>(h, a.x, DT, at, a.n, id);
+        float e[V][8];
+        if (a.dh) load_row<V, TPR, VEC>(e, a.dh, DT, at, a.n, id);
+        if constexpr (ROT) {
+            hadamard<V, TPR>(g, a.hb, id, s);
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < V; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float v = g[c][k] * a.rht_scale;
+                    const uint32_t e = entry(tab[c], k), p = e & NO_PLACE;
+                    if (p != NO_PLACE) s[p] = e & 0x8000u ? -v : v;
+                }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < V; c++) {
+                const f32x4_t* p = (const f32x4_t*)(s + (c * TPR + id) * 8);
+                const f32x4_t lo = p[0], hi = p[1];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    // (past the row nothing was written)
+                    g[c][k] = (c * TPR + id) * 8 < a.n ? lo[k] : 0.0f;
+                    g[c][4 + k] = (c * TPR + id) * 8 < a.n ? hi[k] : 0.0f;
+                }
+            }
+        }
+        float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                sum += h[c][k] * h[c][k];
+                dot += g[c][k] * (w[c][k] + off) * h[c][k];
+            }
+        sum = row_reduce<TPR>(sum, s_red, add_op);
+        dot = row_reduce<TPR>(dot, s_red, add_op);
+        const float r = 1.0f / sqrtf(sum / (float)a.n + a.eps), b = r * r * r * (dot / (float)a.n);
+#pragma unroll
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (live) dw[c][k] += g[c][k] * (h[c][k] * r);
+                const float d = r * (g[c][k] * (w[c][k] + off)) - h[c][k] * b;
+                e[c][k] = a.dh ? e[c][k] + d : d;
+            }
+        if (live) store_row<V, TPR, VEC>(e, a.y, DT, row, a.n, id, 0.0f);
+    }
+    if (!part) return;
+    float* o = part + (int64_t)(blockIdx.x * RW + rw) * a.n;
+#pragma unroll
+    for (int c = 0; c < V; c++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int i = place<V, TPR, VEC>(c, k, id);
+            if (i < a.n) o[i] = dw[c][k];
+        }
+}
+
+// dw: the sums of the workgroups, 64 columns a workgroup, 16 threads a column
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int chunks, int n, float* dw)
+{
+    __shared__ float s[16][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
+    float v = 0.0f;
+    if (col < n)
+        for (int k = y; k < chunks; k += 16) v += part[(int64_t)k * n + col];
+    s[y][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (y || col >= n) return;
+    for (int k = 1; k < 16; k++) v += s[k][threadIdx.x];
+    dw[col] = v;
+}
+
+struct Shape {
+    int v, tpr, vec, rot;
+    int64_t groups;  // workgroups
+};
+
+Shape shape_of(const NormCall& c, bool grad)
+{
+    Shape s;
+    s.rot = c.hb > 0;
+    const uintptr_t ptrs = (uintptr_t)c.x | (uintptr_t)c.residual | (uintptr_t)c.weight | (uintptr_t)c.y | (uintptr_t)c.h |
+                           (uintptr_t)c.dy | (uintptr_t)c.dh;
+    s.vec = c.n % 8 == 0 && ptrs % 16 == 0;
+    s.tpr = c.n <= 512 ? 64 : 256;
+    const int v = (int)((c.n + s.tpr * 8 - 1) / (s.tpr * 8));
+    s.v = v;  // up to 4: VQ2_NORM_MAX_N
+    const int64_t rows = (c.rows + NT / s.tpr - 1) / (NT / s.tpr);
+    // forward: enough workgroups to hide each other's loads; backward: fewer,
+    // each leaves a row of sums
+    s.groups = std::min<int64_t>(rows, (int64_t)device_cu_count() * (grad ? 3 : s.v <= 2 ? 8 : 4));
+    return s;
+}
+
+template <int DT, int V, int TPR>
+hipError_t launch(const NormCall& c, const Shape& s, bool grad, float* part)
+{
+    const dim3 grid((unsigned)s.groups), block(NT);
+    const hipStream_t st = (hipStream_t)c.stream;
+    const int64_t step = s.groups * (NT / TPR);
+    if (grad) {
+        if (s.rot) hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, true, true>), grid, block, 0, st, c, step, part);
+        else if (s.vec) hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, true, false>), grid, block, 0, st, c, step, part);
+        else hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, false, false>), grid, block, 0, st, c, step, part);
+        return hipGetLastError();
+    }
+    if (s.rot) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, true>), grid, block, 0, st, c, step);
+    else if (s.vec) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, false>), grid, block, 0, st, c, step);
+    else hipLaunchKernelGGL((norm_kernel<DT, V, TPR, false, false>), grid, block, 0, st, c, step);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_shape(const NormCall& c, const Shape& s, bool grad, float* part)
+{
+    if (s.tpr == 64) return launch<DT, 1, 64>(c, s, grad, part);
+    switch (s.v) {
+    case 1: return launch<DT, 1, 256>(c, s, grad, part);
+    case 2: return launch<DT, 2, 256>(c, s, grad, part);
+    case 3: return launch<DT, 3, 256>(c, s, grad, part);
+    default: return launch<DT, 4, 256>(c, s, grad, part);
+    }
+}
+
+hipError_t launch_dt(const NormCall& c, const Shape& s, bool grad, float* part)
+{
+    if (c.x_dt == VQ2_DT_F16) return launch_shape<VQ2_DT_F16>(c, s, grad, part);
+    if (c.x_dt == VQ2_DT_BF16) return launch_shape<VQ2_DT_BF16>(c, s, grad, part);
+    return launch_shape<VQ2_DT_F32>(c, s, grad, part);
+}
+
+}  // namespace
+
+size_t norm_workspace_bytes(int64_t rows, int64_t n)
+{
+    NormCall c{};
+    c.rows = rows;
+    c.n = (int)n;
+    const Shape s = shape_of(c, true);
+    return rows == 0 ? 0 : (size_t)(s.groups * (NT / s.tpr)) * n * 4;
+}
+
+int norm_launch(const NormCall& c)
+{
+    const Shape s = shape_of(c, false);
+    const hipError_t e = launch_dt(c, s, false, nullptr);
+    return e == hipSuccess ? VQ2_OK : set_hip_error(e, "vq2_add_rms_norm");
+}
+
+int norm_grad_launch(const NormCall& c, float* dw, void* workspace)
+{
+    const Shape s = shape_of(c, true);
+    if (c.rows) {
+        const hipError_t e = launch_dt(c, s, true, dw ? (float*)workspace : nullptr);
+        if (e != hipSuccess) return set_hip_error(e, "vq2_add_rms_norm_backward");
+    }
+    if (!dw) return VQ2_OK;
+    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((c.n + 63) / 64)), dim3(1024), 0, (hipStream_t)c.stream,
+                       (const float*)workspace, c.rows ? (int)(s.groups * (NT / s.tpr)) : 0, c.n, dw);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? VQ2_OK : set_hip_error(e, "vq2_add_rms_norm_backward");
+}
+
+}  // namespace vq2

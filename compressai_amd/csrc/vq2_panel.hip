@@ -1,0 +1,1054 @@
+// vq2_panel.hip -- many-row products of packed matrices on the matrix cores,
+// with what follows them in their epilogues, and the gradients through the
+// frozen codes:
+//
+//   gated block   act = f(s_g Wg x) (s_u Wu x), and its backward pass
+//   head's loss   lse_t = log sum_v exp(s_v W_v x_t), loss = lse - logit of
+//                 the target, and its backward pass
+//   product       dx = (s dy) W and ds_v = sum_t dy_tv W_v x_t
+//
+// A call packs the token rows into a panel (vq2_panel.hpp), and takes the
+// matrix in pieces of rows: a piece's codes are turned into panels of fp16
+// weights in a workspace (rows of n values; for a gradient also columns of
+// piece values), which the products then read.  Logits and their gradients
+// exist for one piece at a time.
+//
+// Rounding.  A token row is held in fp16 under a power of two of its own (11
+// bits: exact for fp16, bf16 and 8-bit rows but for values 2^-28 below the
+// row's largest).  A weight is the fp32 sum of its stages' centroids, exact
+// in fp16 for one stage of fp16 codebooks; otherwise it is rounded to fp16
+// where only bf16 results depend on it (half a step is 2^-12 of a weight,
+// against 2^-9 of the result), and held as two fp16 parts, multiplied one
+// after the other, where an fp16 or fp32 result does.  Row scales stay outside, in fp32.  A gradient is
+// rounded to fp16 once between its two products (half a step is 2^-12 of each
+// term; what comes of it has 16 bits); everything else is fp32.
+#include <algorithm>
+#include <mutex>
+
+#include "vq2_internal.hpp"
+#include "vq2_panel.hpp"
+
+namespace vq2 {
+
+namespace {
+
+// ------------------------------------------------------------- conversions
+constexpr float NEG_INF = -__builtin_inff();
+
+// 2^e, |e| <= 126
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// exponent e with |v| < 2^(e+1); 0 for 0, infinities and NaN
+__device__ __forceinline__ int exponent_of(float v)
+{
+    const int b = (int)(__float_as_uint(v) >> 23 & 0xFF);
+    return b == 0xFF || (__float_as_uint(v) & 0x7FFFFFFFu) == 0 ? 0 : b - 127;
+}
+
+// exponent of a power of two not below any row scale (bits of their largest
+// magnitude); bounded so that 2^(15 - e) and 2^e are normal numbers
+__device__ __forceinline__ int scale_exponent(uint32_t bits)
+{
+    const int b = (int)(bits >> 23);
+    return b == 0xFF ? 0 : min(max(b - 126, -100), 100);
+}
+
+// -------------------------------------------------------------- token rows
+struct PackArgs {
+    const void* x;
+    int x_dt;
+    int tokens, n;  // rows past the last token are zeros
+    const float* x_scale;
+    half8_t* panel;     // [tiles][n / 32][64]
+    float* fac;         // a product of the panel times fac[t] is one of the row
+    uint32_t* amax;     // largest row scale, cleared here for prep_kernel
+};
+
+// One workgroup a tile of 16 rows: the rows' largest magnitudes, then fp16
+// under a power of two that brings it into [2^13, 2^14).
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs a)
+{
+    __shared__ float s_f[16];
+    const int tid = threadIdx.x, tile = blockIdx.x;
+    if (tile == 0 && tid == 0 && a.amax) *a.amax = 0;
+    {
+        const int r = tid >> 4, row = tile * 16 + r;
+        float m = 0.0f;
+        if (a.x_dt <= VQ2_DT_BF16 && row < a.tokens) {
+            for (int i = (tid & 15) * 8; i < a.n; i += 128) {
+                const Eight e = load8(a.x, a.x_dt, (int64_t)row * a.n + i);
+#pragma unroll
+                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
+            }
+        }
+        m = fmaxf(m, dpp_xor1(m));
+        m = fmaxf(m, dpp_xor2(m));
+        m = fmaxf(m, dpp_half_mirror(m));
+        m = fmaxf(m, dpp_row_mirror(m));
+        if ((tid & 15) == 0) {
+            const int e = m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
+            s_f[r] = pow2(-e);
+            a.fac[row] = row < a.tokens ? pow2(e) * (a.x_scale ? a.x_scale[row] : 1.0f) : 0.0f;
+        }
+    }
+    __syncthreads();
+    const int lane = tid & 63, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
+    const float f = s_f[lane & 15];
+    for (int k = tid >> 6; k < kt; k += 4) {
+        half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (row < a.tokens) {
+            const Eight e = load8(a.x, a.x_dt, (int64_t)row * a.n + k * 32 + q * 8);
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[j] = (_Float16)(e.v[j] * f);
+        }
+        a.panel[((int64_t)tile * kt + k) * 64 + lane] = h;
+    }
+}
+
+// ------------------------------------------------------------ packed rows
+// Rows of the matrices in tiles of 16: one matrix in order; two (gate, up)
+// in turn, so that a wave finds both products of a row in its registers.
+struct PanelMat {
+    const int16_t* i0;
+    const void* i1;
+    const void* scale;
+};
+struct MatArgs {
+    PanelMat m[2];
+    int nmat;
+    int64_t rows;  // of each
+    int ng;        // groups of 8 values
+    int s_dt;
+    const void* cb0;
+    const void* cb1;
+};
+__device__ __forceinline__ int64_t mat_row(const MatArgs& a, int64_t tile, int r, int& mat)
+{
+    mat = a.nmat == 2 ? (int)(tile & 1) : 0;
+    return (a.nmat == 2 ? tile >> 1 : tile) * 16 + r;
+}
+
+// Order of a panel's 16 rows.  Plain: as they come.  Turned: row 4 i + c at
+// place 4 c + i; a lane of a product then holds rows c, 4 + c, 8 + c, 12 + c
+// (c = lane / 16), and two tiles' values are the 8 values of operand chunk c
+// of the panel that the next product reads: the lane stores them as they are.
+__device__ __forceinline__ int turned(int r) { return (r & 3) * 4 + (r >> 2); }
+
+struct PrepArgs {
+    MatArgs m;
+    float rs;
+    int turn;
+    int64_t places;   // 16 * tiles
+    float* sc;        // scale * rs of each place, 0 past the last row
+    uint32_t* amax;   // largest magnitude among them, as bits
+};
+__global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a)
+{
+    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    float v = 0.0f;
+    if (p < a.places) {
+        int mat;
+        const int place = (int)(p & 15);
+        const int64_t row = mat_row(a.m, p >> 4, a.turn ? turned(place) : place, mat);
+        if (row < a.m.rows) v = load_as_f32(a.m.m[mat].scale, a.m.s_dt, row) * a.rs;
+        a.sc[p] = v;
+    }
+    if (!a.amax) return;
+    // (magnitudes as bits are ordered like the numbers, and a maximum does
+    // not depend on the order of its parts)
+    const float m = wave_max_all(fabsf(v));
+    if ((threadIdx.x & 63) == 0) atomicMax(a.amax, __float_as_uint(m));
+}
+
+template <int CBT>
+__device__ __forceinline__ void centroid_f32(const void* cb, uint32_t c, float (&w)[8])
+{
+    const Eight e = load8(cb, CBT, (int64_t)c * 8);
+#pragma unroll
+    for (int k = 0; k < 8; k++) w[k] = e.v[k];
+}
+
+// fp16 weight of a code pair; PARTS == 2: what its rounding leaves, too
+template <int CBT, int S2, int PARTS>
+__device__ __forceinline__ void weight_of(const MatArgs& a, uint32_t c0, uint32_t c1, half8_t& hi, half8_t& lo)
+{
+    if constexpr (CBT == VQ2_DT_F16 && S2 == VQ2_S2_NONE) {
+        hi = ((const half8_t*)a.cb0)[c0];
+    } else {
+        float w[8], u[8];
+        centroid_f32<CBT>(a.cb0, c0, w);
+        if constexpr (S2 != VQ2_S2_NONE) {
+            centroid_f32<CBT>(a.cb1, c1, u);
+#pragma unroll
+            for (int k = 0; k < 8; k++) w[k] += u[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            hi[k] = (_Float16)w[k];
+            if constexpr (PARTS == 2) lo[k] = (_Float16)(w[k] - (float)hi[k]);
+        }
+    }
+}
+
+template <int S2>
+__device__ __forceinline__ uint32_t code1(const void* i1, int64_t i)
+{
+    if constexpr (S2 == VQ2_S2_U8) return ((const uint8_t*)i1)[i];
+    if constexpr (S2 == VQ2_S2_U16) return ((const uint16_t*)i1)[i];
+    return 0;
+}
+
+struct DequantArgs {
+    MatArgs m;
+    int64_t tile0;  // the piece's first tile
+    half8_t* w;     // [tiles][PARTS * ng / 4][64]
+    half8_t* wt;    // [columns / 16][parts * tiles / 2][64], or null
+    int vkt;        // tiles / 2
+};
+
+// Forward: rows in plain order.  A wave takes a tile of 16 rows and 8 k
+// tiles: lane (row, q) gathers group 4 k + q, and each k tile is one KiB.
+template <int CBT, int S2, int PARTS>
+__global__ void __launch_bounds__(256) dequant_plain_kernel(const DequantArgs a)
+{
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int kt = a.m.ng / 4;
+    int mat;
+    const int64_t row = mat_row(a.m, a.tile0 + tile, lane & 15, mat);
+    const bool ok = row < a.m.rows;
+    const int64_t off = (ok ? row : 0) * a.m.ng;
+    uint32_t c0[8], c1[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int64_t i = off + min((int)blockIdx.y * 8 + k, kt - 1) * 4 + q;
+        c0[k] = ((const uint16_t*)a.m.m[mat].i0)[i];
+        c1[k] = code1<S2>(a.m.m[mat].i1, i);
+    }
+    const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    half8_t hi[8], lo[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) weight_of<CBT, S2, PARTS>(a.m, c0[k], c1[k], hi[k], lo[k]);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int t = (int)blockIdx.y * 8 + k;
+        if (t >= kt) break;
+        half8_t* w = a.w + (tile * (PARTS * kt) + t) * 64 + lane;
+        w[0] = ok ? hi[k] : zero;
+        if constexpr (PARTS == 2) w[(int64_t)kt * 64] = ok ? lo[k] : zero;
+    }
+}
+
+// Backward: rows in turned order, and the columns' panel.  A wave takes 32
+// rows (two tiles) and 16 groups: lane (c, g) gathers the 8 rows 16 (m / 4) +
+// 4 (m % 4) + c of group g.  Column j of the 8 centroids is then one operand
+// of the columns' panel, whose block j holds columns j, 8 + j, ... of the 16
+// groups: one KiB a block, and a lane of the next product holds 8 neighbouring
+// columns in its 8 row tiles.
+template <int CBT, int S2, int WP, int TP>
+__global__ void __launch_bounds__(256) dequant_turned_kernel(const DequantArgs a)
+{
+    const int lane = threadIdx.x & 63, c = lane >> 4, g = blockIdx.y * 16 + (lane & 15);
+    const int pair = blockIdx.x * 4 + (threadIdx.x >> 6);  // of the piece
+    const int kt = a.m.ng / 4;
+    const bool g_ok = g < a.m.ng;
+    uint32_t c0[8], c1[8];
+    bool ok[8];
+#pragma unroll
+    for (int m = 0; m < 8; m++) {
+        int mat;
+        const int64_t row = mat_row(a.m, a.tile0 + 2 * pair + m / 4, 4 * (m % 4) + c, mat);
+        ok[m] = g_ok && row < a.m.rows;
+        const int64_t i = ok[m] ? row * a.m.ng + g : 0;
+        c0[m] = ((const uint16_t*)a.m.m[mat].i0)[i];
+        c1[m] = code1<S2>(a.m.m[mat].i1, i);
+    }
+    const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    constexpr int PARTS = WP == 2 || TP == 2 ? 2 : 1;
+    half8_t hi[8], lo[8];
+#pragma unroll
+    for (int m = 0; m < 8; m++) weight_of<CBT, S2, PARTS>(a.m, c0[m], c1[m], hi[m], lo[m]);
+#pragma unroll
+    for (int m = 0; m < 8; m++) {
+        hi[m] = ok[m] ? hi[m] : zero;
+        if constexpr (PARTS == 2) lo[m] = ok[m] ? lo[m] : zero;
+    }
+    if (WP && g_ok) {
+#pragma unroll
+        for (int m = 0; m < 8; m++) {
+            half8_t* w = a.w + ((int64_t)(2 * pair + m / 4) * (WP * kt) + g / 4) * 64 + (g & 3) * 16 + 4 * c + m % 4;
+            w[0] = hi[m];
+            if constexpr (WP == 2) w[(int64_t)kt * 64] = lo[m];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        half8_t* t = a.wt + ((int64_t)(blockIdx.y * 8 + j) * (TP * a.vkt) + pair) * 64 + lane;
+        half8_t v;
+#pragma unroll
+        for (int m = 0; m < 8; m++) v[m] = hi[m][j];
+        t[0] = v;
+        if constexpr (TP == 2) {
+#pragma unroll
+            for (int m = 0; m < 8; m++) v[m] = lo[m][j];
+            t[(int64_t)a.vkt * 64] = v;
+        }
+    }
+}
+
+// -------------------------------------------------------------- epilogues
+// What a product of weights (panel a) and tokens (panel b) is made into.
+// `tile` is the first weight tile of the wave, counted over all pieces, `tok`
+// its first token.
+
+// over the four lanes that hold a token's rows
+__device__ __forceinline__ float max_rows(float v)
+{
+    v = fmaxf(v, swz_xor16(v));
+    return fmaxf(v, xor32(v));
+}
+__device__ __forceinline__ float sum_rows(float v)
+{
+    v += swz_xor16(v);
+    return v + xor32(v);
+}
+
+constexpr int64_t TARGET_SKIP = -1, TARGET_BAD = -2;
+// the token's target, TARGET_SKIP for a token that does not count, TARGET_BAD
+// for one outside the vocabulary
+__device__ __forceinline__ int64_t target_of(const int64_t* t, int64_t i, int64_t ignore, int64_t rows)
+{
+    const int64_t v = t[i];
+    return v == ignore ? TARGET_SKIP : v < 0 || v >= rows ? TARGET_BAD : v;
+}
+
+struct StatsEpi {
+    const float* sc;
+    const float* fac;
+    const int64_t* target;
+    int64_t rows, ignore;
+    int tokens, tp;
+    f32x2_t* part;  // [waves of rows][tp]: largest logit and sum of exp(l - largest)
+    float* at;      // [tp]: the target's logit
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+        f32x4_t s[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) s[i] = *(const f32x4_t*)(sc + (tile + i) * 16 + q * 4);
+        const bool tail = (tile + MT) * 16 > rows;
+#pragma unroll
+        for (int j = 0; j < PG_NT; j++) {
+            const int t = tok + j * 16 + nl;
+            const float f = fac[t];
+            float m = NEG_INF;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float z = acc[i][j][e] * f * s[i][e];
+                    if (tail && (tile + i) * 16 + q * 4 + e >= rows) z = NEG_INF;
+                    acc[i][j][e] = z;
+                    m = fmaxf(m, z);
+                }
+            m = max_rows(m);
+            const float base = m == NEG_INF ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += __expf(acc[i][j][e] - base);
+            sum = sum_rows(sum);
+            if (q == 0) part[(tile / MT) * tp + t] = f32x2_t{m, sum};
+            const int64_t v = t < tokens ? target_of(target, t, ignore, rows) : TARGET_SKIP;
+            const int64_t rel = v - tile * 16;
+            if (rel >= 0 && rel < MT * 16) {  // (few lanes of a launch)
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (rel == i * 16 + q * 4 + e) at[t] = acc[i][j][e];
+            }
+        }
+    }
+};
+
+struct DlogitEpi {
+    const float* sc;
+    const float* fac;
+    const float* lse;
+    const float* dloss;
+    const int64_t* target;
+    const uint32_t* amax;
+    int64_t rows, ignore, tile0;  // tile0: the piece's first tile
+    int tokens, tp, vkt;
+    half8_t* p;    // the next product's panel of tokens, [tp / 16][vkt][64]
+    float* ds;     // [tp / 64][16 * all tiles]: sums over 64 tokens, or null
+    int64_t ds_ld;
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+        const float c = pow2(14 - scale_exponent(*amax));
+        float l[PG_NT], up[PG_NT], f[PG_NT];
+        int rel[PG_NT];  // the target's row of the wave's, or none; SKIP: the token does not count
+        constexpr int SKIP = -2, NONE = -1;
+#pragma unroll
+        for (int j = 0; j < PG_NT; j++) {
+            const int t = tok + j * 16 + nl;
+            int64_t v = TARGET_SKIP;
+            l[j] = up[j] = 0.0f;
+            if (t < tokens) {
+                v = target_of(target, t, ignore, rows);
+                l[j] = lse[t];
+                up[j] = v == TARGET_BAD ? __builtin_nanf("") : dloss[t];
+            }
+            f[j] = fac[t];
+            const int64_t r = v - tile * 16;
+            rel[j] = v == TARGET_SKIP ? SKIP : r >= 0 && r < MT * 16 ? (int)r : NONE;
+        }
+        const int left = (int)min(rows - tile * 16, (int64_t)MT * 16);  // rows of the wave that exist
+#pragma unroll
+        for (int i = 0; i < MT; i += 2) {
+            f32x4_t s[2], d[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                s[k] = *(const f32x4_t*)(sc + (tile + i + k) * 16 + q * 4);
+                d[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) {
+                half8_t h;
+#pragma unroll
+                for (int m = 0; m < 8; m++) {
+                    const int e = m & 3, k = m >> 2, r = (i + k) * 16 + 4 * e + q;
+                    const float raw = acc[i + k][j][e] * f[j];
+                    float v = __expf(raw * s[k][e] - l[j]) - (rel[j] == r ? 1.0f : 0.0f);
+                    if (rel[j] == SKIP || r >= left) v = 0.0f;
+                    h[m] = (_Float16)(v * (s[k][e] * c));
+                    if (ds && rel[j] != SKIP) d[k][e] += up[j] * v * raw;
+                }
+                p[((int64_t)((tok >> 4) + j) * vkt + (tile - tile0 + i) / 2) * 64 + lane] = h;
+            }
+            if (ds) {
+#pragma unroll
+                for (int m = 0; m < 8; m++) {
+                    const float v = group_sum(d[m >> 2][m & 3], 16);
+                    if (nl == 0) ds[(tok / (16 * PG_NT)) * ds_ld + (tile + i + (m >> 2)) * 16 + q * 4 + (m & 3)] = v;
+                }
+            }
+        }
+    }
+};
+
+// f(g), and its derivative
+template <int ACT>
+__device__ __forceinline__ void gate_act(float g, float& f, float& df)
+{
+    if constexpr (ACT == VQ2_ACT_SILU) {
+        const float s = 1.0f / (1.0f + __expf(-g));
+        f = g * s;
+        df = s * (1.0f + g * (1.0f - s));
+        if (g < -80.0f) f = df = 0.0f;  // (also -inf; the true values are below 1e-32)
+    } else {
+        // g / (1 + exp(-2 u)), u the tanh form's argument
+        const float g2 = g * g, u2 = 1.5957691216057308f * g * (1.0f + 0.044715f * g2);
+        const float s = 1.0f / (1.0f + __expf(-u2));
+        f = g * s;
+        df = s * (1.0f + g * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * g2)));
+        if (g < -12.0f) f = df = 0.0f;
+        if (g > 12.0f) { f = g; df = 1.0f; }
+    }
+}
+
+struct GatedEpi {
+    const float* sc;
+    const float* fac;
+    void* y;
+    int y_dt, tokens;
+    int64_t rows;
+    int vec;  // rows a multiple of 4, y aligned: 4 values a store
+    int act;
+    template <int ACT, int MT>
+    __device__ __forceinline__ void run_act(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+#pragma unroll
+        for (int i = 0; i < MT; i += 2) {
+            const f32x4_t sg = *(const f32x4_t*)(sc + (tile + i) * 16 + q * 4);
+            const f32x4_t su = *(const f32x4_t*)(sc + (tile + i + 1) * 16 + q * 4);
+            const int64_t r0 = (tile + i) / 2 * 16 + q * 4;
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) {
+                const int t = tok + j * 16 + nl;
+                if (t >= tokens || r0 >= rows) continue;
+                const float x = fac[t];
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float f, df;
+                    gate_act<ACT>(acc[i][j][e] * x * sg[e], f, df);
+                    o[e] = f * (acc[i + 1][j][e] * x * su[e]);
+                }
+                const int64_t at = (int64_t)t * rows + r0;
+                if (!vec) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (r0 + e < rows) store_from_f32(y, y_dt, at + e, o[e]);
+                } else if (y_dt == VQ2_DT_F32) {
+                    *(f32x4_t*)((float*)y + at) = f32x4_t{o[0], o[1], o[2], o[3]};
+                } else if (y_dt == VQ2_DT_F16) {
+                    *(half4_t*)((uint16_t*)y + at) = half4_t{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+                } else {
+                    *(u32x2*)((uint16_t*)y + at) = u32x2{f32_to_bf16_bits(o[0]) | (uint32_t)f32_to_bf16_bits(o[1]) << 16,
+                                                         f32_to_bf16_bits(o[2]) | (uint32_t)f32_to_bf16_bits(o[3]) << 16};
+                }
+            }
+        }
+    }
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
+    {
+        if (act == VQ2_ACT_SILU) run_act<VQ2_ACT_SILU>(acc, tile, tok);
+        else run_act<VQ2_ACT_GELU_TANH>(acc, tile, tok);
+    }
+};
+
+struct DgatedEpi {
+    const float* sc;
+    const float* fac;
+    const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_factor_kernel)
+    const void* dy;     // [tokens][rows]
+    const uint32_t* amax;
+    int dy_dt, tokens, tp, vkt;
+    int64_t rows, tile0;
+    half8_t* p;
+    float* ds;
+    int64_t ds_ld;
+    int act;
+    template <int ACT, int MT>
+    __device__ __forceinline__ void run_act(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+        const float c = pow2(-scale_exponent(*amax));
+#pragma unroll
+        for (int i = 0; i < MT; i += 2) {
+            const f32x4_t sg = *(const f32x4_t*)(sc + (tile + i) * 16 + q * 4);
+            const f32x4_t su = *(const f32x4_t*)(sc + (tile + i + 1) * 16 + q * 4);
+            const int64_t r0 = (tile + i) / 2 * 16 + q;
+            f32x4_t dsg = {0.0f, 0.0f, 0.0f, 0.0f}, dsu = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) {
+                const int t = tok + j * 16 + nl;
+                const float x = fac[t], k = t < tokens ? dfac[t] : 0.0f;
+                half8_t h;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float d = t < tokens && r0 + 4 * e < rows
+                                        ? load_as_f32(dy, dy_dt, (int64_t)t * rows + r0 + 4 * e) : 0.0f;
+                    const float rg = acc[i][j][e] * x, ru = acc[i + 1][j][e] * x;
+                    float f, df;
+                    gate_act<ACT>(rg * sg[e], f, df);
+                    const float dg = d * (ru * su[e]) * df, du = d * f;
+                    h[e] = (_Float16)(dg * k * (sg[e] * c));
+                    h[4 + e] = (_Float16)(du * k * (su[e] * c));
+                    if (ds) {
+                        dsg[e] += dg * rg;
+                        dsu[e] += du * ru;
+                    }
+                }
+                p[((int64_t)((tok >> 4) + j) * vkt + (tile - tile0 + i) / 2) * 64 + lane] = h;
+            }
+            if (ds) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float a = group_sum(dsg[e], 16), b = group_sum(dsu[e], 16);
+                    if (nl == 0) {
+                        float* o = ds + (tok / (16 * PG_NT)) * ds_ld + (tile + i) * 16 + q * 4 + e;
+                        o[0] = a;
+                        o[16] = b;
+                    }
+                }
+            }
+        }
+    }
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
+    {
+        if (act == VQ2_ACT_SILU) run_act<VQ2_ACT_SILU>(acc, tile, tok);
+        else run_act<VQ2_ACT_GELU_TANH>(acc, tile, tok);
+    }
+};
+
+// sums over 64 tokens of upstream times product: the row scales' gradient
+struct ColsumEpi {
+    const float* fac;
+    const void* dy;
+    int dy_dt, tokens;
+    int64_t rows;
+    float* ds;
+    int64_t ds_ld;
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int64_t r0 = (tile + i) * 16 + q;
+            f32x4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) {
+                const int t = tok + j * 16 + nl;
+                const float x = fac[t];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float u = t < tokens && r0 + 4 * e < rows
+                                        ? load_as_f32(dy, dy_dt, (int64_t)t * rows + r0 + 4 * e) : 0.0f;
+                    d[e] += u * (acc[i][j][e] * x);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float v = group_sum(d[e], 16);
+                if (nl == 0) ds[(tok / (16 * PG_NT)) * ds_ld + (tile + i) * 16 + q * 4 + e] = v;
+            }
+        }
+    }
+};
+
+// Columns' product, added to what earlier pieces left: tile i of the wave
+// holds columns i, 8 + i, ... of its 128 (MT == 8) or the 64 of parity h.
+struct GradEpi {
+    float* out;  // [slices][tp][np]
+    int64_t np;
+    int tp, add;
+    template <int MT>
+    __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int bz)
+    {
+        const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+        const int64_t c0 = tile / 8 * 128 + tile % 8;
+#pragma unroll
+        for (int j = 0; j < PG_NT; j++) {
+            float* o = out + ((int64_t)bz * tp + tok + j * 16 + nl) * np + c0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < MT; i += 4) {
+                    f32x4_t v = {acc[i][j][e], acc[i + 1][j][e], acc[i + 2][j][e], acc[i + 3][j][e]};
+                    f32x4_t* a = (f32x4_t*)(o + (q * 4 + e) * 8 + i);
+                    if (add) v += *a;
+                    *a = v;
+                }
+        }
+    }
+};
+
+template <int MT, class Epi>
+__global__ void __launch_bounds__(PG_THREADS, MT == 8 ? 2 : 3) panel_gemm_kernel(const PanelGemmArgs g, Epi epi, int64_t tile0)
+{
+    int bm, bn, bz;
+    panel_tile(g, bm, bn, bz);
+    f32x4_t acc[MT][PG_NT];
+    panel_product<MT>(g, bm, bn, bz, acc);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % PG_WM, wn = wave / PG_WM;
+    epi.template run<MT>(acc, tile0 + (bm * PG_WM + wm) * MT, (bn * PG_WN + wn) * PG_NT * 16, bz);
+}
+
+// ------------------------------------------------- upstream rows of a product
+struct DyArgs {
+    const void* dy;
+    int dy_dt, tokens;
+    int64_t rows, row0;  // row0: the piece's first
+    const float* sc;     // turned order
+    const uint32_t* amax;
+    half8_t* p;          // [tp / 16][vkt][64], or null: only the factors
+    int vkt, head;    // head: bits left above the row's largest value
+    float* dfac;      // [tp]: 2^-e; the panel holds dy 2^-e (scale 2^-es)
+};
+
+// One workgroup a tile of 16 tokens: the rows' largest magnitudes, then the
+// panel of dy * scale in the order of the columns' panel.
+__global__ void __launch_bounds__(256) dy_rows_kernel(const DyArgs a)
+{
+    __shared__ float s_f[16];
+    const int tid = threadIdx.x, tile = blockIdx.x;
+    {
+        const int r = tid >> 4, t = tile * 16 + r;
+        float m = 0.0f;
+        if (t < a.tokens)
+            for (int64_t i = tid & 15; i < a.rows; i += 16) m = fmaxf(m, fabsf(load_as_f32(a.dy, a.dy_dt, t * a.rows + i)));
+        m = fmaxf(m, dpp_xor1(m));
+        m = fmaxf(m, dpp_xor2(m));
+        m = fmaxf(m, dpp_half_mirror(m));
+        m = fmaxf(m, dpp_row_mirror(m));
+        if ((tid & 15) == 0) {
+            const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
+            s_f[r] = pow2(-e);
+            a.dfac[t] = pow2(-e);
+        }
+    }
+    if (!a.p) return;
+    __syncthreads();
+    const int lane = tid & 63, c = lane >> 4, t = tile * 16 + (lane & 15);
+    const float f = s_f[lane & 15] * pow2(-scale_exponent(*a.amax));
+    for (int k = tid >> 6; k < a.vkt; k += 4) {
+        half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < 8; m++) {
+            const int64_t row = a.row0 + (int64_t)k * 32 + 16 * (m >> 2) + 4 * (m & 3) + c;
+            if (t < a.tokens && row < a.rows)
+                h[m] = (_Float16)(load_as_f32(a.dy, a.dy_dt, t * a.rows + row) *
+                                  (a.sc[(row >> 4) * 16 + 4 * c + (m & 3)] * f));
+        }
+        a.p[((int64_t)tile * a.vkt + k) * 64 + lane] = h;
+    }
+}
+
+// ---------------------------------------------------------------- last steps
+struct LseArgs {
+    const f32x2_t* part;
+    int64_t chunks;
+    int tokens, tp;
+    const int64_t* target;
+    int64_t rows, ignore;
+    const float* at;
+    float* loss;
+    float* lse;
+};
+// 16 tokens a workgroup, 16 threads a token over the chunks
+__global__ void __launch_bounds__(256) lse_kernel(const LseArgs a)
+{
+    __shared__ f32x2_t s_p[16][17];
+    const int tid = threadIdx.x, tl = tid & 15, t = blockIdx.x * 16 + tl;
+    float m = NEG_INF, s = 0.0f;
+    auto add = [&](float om, float os) {
+        const float n = fmaxf(m, om), b = n == NEG_INF ? 0.0f : n;
+        s = s * __expf(m - b) + os * __expf(om - b);
+        m = n;
+    };
+    for (int64_t k = tid >> 4; k < a.chunks; k += 16) {
+        const f32x2_t p = a.part[k * a.tp + t];
+        add(p.x, p.y);
+    }
+    s_p[tid >> 4][tl] = f32x2_t{m, s};
+    __syncthreads();
+    if (tid >= 16 || t >= a.tokens) return;
+    for (int k = 1; k < 16; k++) add(s_p[k][tl].x, s_p[k][tl].y);
+    const float lse = m + logf(s);
+    const int64_t v = target_of(a.target, t, a.ignore, a.rows);
+    a.lse[t] = lse;
+    a.loss[t] = v == TARGET_SKIP ? 0.0f : v == TARGET_BAD ? __builtin_nanf("") : lse - a.at[t];
+}
+
+struct DxArgs {
+    const float* part;  // [slices][tp][np]
+    int slices, tp, n;
+    int64_t np;
+    const uint32_t* amax;
+    const float* dfac;      // the panel's factors, or null: the loss's
+    const float* dloss;
+    const int64_t* target;
+    int64_t rows, ignore;
+    void* dx;
+    int dx_dt;
+};
+__global__ void __launch_bounds__(256) dx_kernel(const DxArgs a)
+{
+    const int t = blockIdx.y, i = ((int)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= a.n) return;
+    const int es = scale_exponent(*a.amax);
+    float f, g = 1.0f;
+    bool skip = false;
+    if (a.dfac) {
+        f = pow2(es);
+        g = 1.0f / a.dfac[t];
+    } else {
+        const int64_t v = target_of(a.target, t, a.ignore, a.rows);
+        skip = v == TARGET_SKIP;
+        f = pow2(es - 14);
+        g = v == TARGET_BAD ? __builtin_nanf("") : a.dloss[t];
+    }
+    f32x4_t v = *(const f32x4_t*)(a.part + (int64_t)t * a.np + i);
+    for (int z = 1; z < a.slices; z++) v += *(const f32x4_t*)(a.part + ((int64_t)z * a.tp + t) * a.np + i);
+#pragma unroll
+    for (int k = 0; k < 4; k++) store_from_f32(a.dx, a.dx_dt, (int64_t)t * a.n + i + k, skip ? 0.0f : v[k] * f * g);
+}
+
+struct DsArgs {
+    MatArgs m;
+    const float* part;  // [chunks][ld] in turned order
+    int chunks;
+    int64_t ld;
+    float rs;
+    float* ds[2];
+    int add;
+};
+__global__ void __launch_bounds__(256) ds_kernel(const DsArgs a)
+{
+    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (p >= a.ld) return;
+    int mat;
+    const int64_t row = mat_row(a.m, p >> 4, turned((int)(p & 15)), mat);
+    if (row >= a.m.rows) return;
+    float s = 0.0f;
+    for (int k = 0; k < a.chunks; k++) s += a.part[k * a.ld + p];
+    float* d = a.ds[mat] + row;
+    *d = (a.add ? *d : 0.0f) + s * a.rs;
+}
+
+__global__ void __launch_bounds__(256) zero_kernel(float* p, int64_t n)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0.0f;
+}
+
+// ------------------------------------------------------------------- host
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+struct Bump {
+    size_t at = 0;
+    size_t take(size_t bytes)
+    {
+        const size_t o = at;
+        at += (bytes + 255) / 256 * 256;
+        return o;
+    }
+};
+
+// Tokens are taken PANEL_TOKENS at a time, and the matrix in pieces whose
+// panel of gradients (2 bytes a token and row) stays near PIECE_BYTES.
+constexpr int64_t PANEL_TOKENS = 8192;
+constexpr int64_t PIECE_BYTES = 128 << 20;
+constexpr int64_t PIECE_MAX_ROWS = 16384, PIECE_MIN_ROWS = 4096;
+
+struct Plan {
+    int64_t chunk;       // tokens of a chunk (the last may be shorter)
+    int64_t tp;          // of them, padded
+    int64_t tiles;       // 16-row tiles of all matrices, padded to whole workgroups
+    int64_t piece;       // tiles of a piece
+    int parts, tparts, kt;  // parts of a weight in the rows' panel, and the columns'
+    int64_t np;          // columns, padded
+    int slices;
+    size_t fac, amax, sc, xp, w, wt, p, acc, stats, at, ds, dfac, total;
+};
+
+enum { STATS = PANEL_STATS, DLOGIT = PANEL_DLOGIT, GATED = PANEL_GATED, DGATED = PANEL_DGATED, PRODUCT = PANEL_PRODUCT };
+
+Plan plan_of(const PanelCall& c)
+{
+    Plan p{};
+    const bool grad = c.what == DLOGIT || c.what == DGATED || c.what == PRODUCT;
+    p.chunk = std::min(c.tokens, PANEL_TOKENS);
+    p.tp = up(p.chunk, PG_N);
+    p.tiles = up((c.rows + 15) / 16 * c.nmat, pg_m(8) / 16);
+    p.kt = (int)(c.n / 32);
+    const bool exact = c.cb_dt != VQ2_DT_F32 && c.s2 == VQ2_S2_NONE;
+    const bool fine = c.y_dt != VQ2_DT_BF16;
+    const bool wide = c.what == STATS || c.what == DLOGIT || c.ds[0] != nullptr || fine;
+    p.parts = !exact && wide ? 2 : 1;
+    p.tparts = !exact && fine ? 2 : 1;
+    int64_t rows = PIECE_MAX_ROWS;
+    while (grad && rows > PIECE_MIN_ROWS && rows * p.tp * 2 > PIECE_BYTES) rows /= 2;
+    p.piece = std::min(p.tiles, rows / 16);
+    p.np = up(c.n, pg_m(8));
+    p.slices = 1;
+    Bump b;
+    p.fac = b.take(p.tp * 4);
+    p.amax = b.take(4);
+    p.sc = b.take(p.tiles * 16 * 4);
+    p.xp = b.take(p.tp * c.n * 2);
+    const bool w = c.what != PRODUCT || c.ds[0];
+    p.w = b.take(w ? p.piece * 16 * c.n * 2 * p.parts : 0);
+    if (grad) {
+        p.wt = b.take(p.piece * 16 * p.np * 2 * p.tparts);
+        p.p = b.take(p.piece * 16 * p.tp * 2);
+        // as many slices of a piece's rows as fill the device
+        const int64_t wg = p.np / pg_m(8) * (p.tp / PG_N);
+        const int64_t most = std::max<int64_t>(1, p.piece / 2 / 16);
+        while (p.slices < 64 && wg * p.slices < 512 && p.slices * 2 <= most) p.slices *= 2;
+        p.acc = b.take(p.slices * p.tp * p.np * 4);
+        if (c.ds[0]) p.ds = b.take(p.tp / (16 * PG_NT) * p.tiles * 16 * 4);
+        if (c.what != DLOGIT) p.dfac = b.take(p.tp * 4);
+    }
+    if (c.what == STATS) {
+        p.stats = b.take(p.tiles / 4 * p.tp * 8);
+        p.at = b.take(p.tp * 4);
+    }
+    p.total = b.at;
+    return p;
+}
+
+template <int MT, class Epi>
+hipError_t gemm(const PanelGemmArgs& g, const Epi& e, int64_t tile0, hipStream_t st)
+{
+    static std::once_flag once;
+    static hipError_t attr = hipSuccess;
+    std::call_once(once, [] {
+        attr = hipFuncSetAttribute((const void*)panel_gemm_kernel<MT, Epi>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   pg_lds(MT));
+    });
+    if (attr != hipSuccess) return attr;
+    hipLaunchKernelGGL((panel_gemm_kernel<MT, Epi>), dim3((unsigned)(g.gm * g.gn * g.gz)), dim3(PG_THREADS), pg_lds(MT), st, g, e,
+                       tile0);
+    return hipGetLastError();
+}
+
+template <int CBT, int S2, int WP, int TP>
+hipError_t dequant_parts(const DequantArgs& a, int64_t tiles, hipStream_t st)
+{
+    if constexpr (TP == 0)
+        hipLaunchKernelGGL((dequant_plain_kernel<CBT, S2, WP>), dim3((unsigned)(tiles / 4), (unsigned)((a.m.ng / 4 + 7) / 8)),
+                           dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((dequant_turned_kernel<CBT, S2, WP, TP>), dim3((unsigned)(tiles / 8), (unsigned)((a.m.ng + 15) / 16)),
+                           dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <int CBT, int S2>
+hipError_t dequant_typed(const DequantArgs& a, int wp, int tp, int64_t tiles, hipStream_t st)
+{
+    constexpr bool EXACT = CBT != VQ2_DT_F32 && S2 == VQ2_S2_NONE;
+    if constexpr (!EXACT) {
+        if (tp == 0 && wp == 2) return dequant_parts<CBT, S2, 2, 0>(a, tiles, st);
+        if (tp == 2 && wp == 0) return dequant_parts<CBT, S2, 0, 2>(a, tiles, st);
+        if (tp == 2) return dequant_parts<CBT, S2, 2, 2>(a, tiles, st);
+        if (wp == 2) return dequant_parts<CBT, S2, 2, 1>(a, tiles, st);
+    }
+    if (tp == 0) return dequant_parts<CBT, S2, 1, 0>(a, tiles, st);
+    if (wp == 0) return dequant_parts<CBT, S2, 0, 1>(a, tiles, st);
+    return dequant_parts<CBT, S2, 1, 1>(a, tiles, st);
+}
+
+template <int CBT>
+hipError_t dequant_s2(const DequantArgs& a, int s2, int wp, int tp, int64_t tiles, hipStream_t st)
+{
+    if (s2 == VQ2_S2_NONE) return dequant_typed<CBT, VQ2_S2_NONE>(a, wp, tp, tiles, st);
+    if (s2 == VQ2_S2_U8) return dequant_typed<CBT, VQ2_S2_U8>(a, wp, tp, tiles, st);
+    return dequant_typed<CBT, VQ2_S2_U16>(a, wp, tp, tiles, st);
+}
+
+// wp, tp: parts of the rows' and the columns' panel, 0 for none
+hipError_t dequant(const DequantArgs& a, int cb_dt, int s2, int wp, int tp, int64_t tiles, hipStream_t st)
+{
+    if (cb_dt == VQ2_DT_F16) return dequant_s2<VQ2_DT_F16>(a, s2, wp, tp, tiles, st);
+    if (cb_dt == VQ2_DT_BF16) return dequant_s2<VQ2_DT_BF16>(a, s2, wp, tp, tiles, st);
+    return dequant_s2<VQ2_DT_F32>(a, s2, wp, tp, tiles, st);
+}
+
+}  // namespace
+
+size_t panel_workspace_bytes(const PanelCall& c) { return c.tokens ? plan_of(c).total : 0; }
+
+#define TRY(call)                                               \
+    do {                                                        \
+        const hipError_t e_ = (call);                           \
+        if (e_ != hipSuccess) return set_hip_error(e_, c.who);  \
+    } while (0)
+
+int panel_launch(const PanelCall& c)
+{
+    const hipStream_t st = (hipStream_t)c.stream;
+    const MatArgs mats{{{c.mat[0].i0, c.mat[0].i1, c.mat[0].scale}, {c.mat[1].i0, c.mat[1].i1, c.mat[1].scale}},
+                       c.nmat, c.rows, (int)(c.n / 8), c.s_dt, c.cb0, c.cb1};
+    if (c.tokens == 0) {
+        for (int k = 0; k < c.nmat; k++)
+            if (c.ds[k]) {
+                hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((c.rows + 255) / 256)), dim3(256), 0, st, c.ds[k], c.rows);
+                TRY(hipGetLastError());
+            }
+        return VQ2_OK;
+    }
+    const Plan p = plan_of(c);
+    char* ws = (char*)c.workspace;
+    const bool grad = c.what == DLOGIT || c.what == DGATED || c.what == PRODUCT;
+    const bool first = c.what != PRODUCT || c.ds[0];  // the product of weights and tokens
+    float* fac = (float*)(ws + p.fac);
+    uint32_t* amax = (uint32_t*)(ws + p.amax);
+    float* sc = (float*)(ws + p.sc);
+    half8_t* xp = (half8_t*)(ws + p.xp);
+    half8_t* w = first ? (half8_t*)(ws + p.w) : nullptr;
+    half8_t* wt = grad ? (half8_t*)(ws + p.wt) : nullptr;
+    half8_t* pp = (half8_t*)(ws + p.p);
+    float* acc = (float*)(ws + p.acc);
+    float* ds = c.ds[0] ? (float*)(ws + p.ds) : nullptr;
+    float* dfac = (float*)(ws + p.dfac);
+    const int64_t xsize = c.x_dt == VQ2_DT_F32 ? 4 : c.x_dt <= VQ2_DT_BF16 ? 2 : 1;
+    for (int64_t t0 = 0; t0 < c.tokens; t0 += p.chunk) {
+        const int tokens = (int)std::min(p.chunk, c.tokens - t0);
+        const int tp = (int)up(tokens, PG_N);
+        const int64_t ds_ld = p.tiles * 16;
+        const void* dy = c.dy ? (const char*)c.dy + t0 * c.rows * dt_size(c.dy_dt) : nullptr;
+        const int64_t* target = c.target ? c.target + t0 : nullptr;
+        if (first) {
+            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
+                               PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
+                                        c.x_scale ? c.x_scale + t0 : nullptr, xp, fac, t0 == 0 ? amax : nullptr});
+            TRY(hipGetLastError());
+        } else if (t0 == 0) {
+            hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(256), 0, st, (float*)amax, (int64_t)1);
+            TRY(hipGetLastError());
+        }
+        if (t0 == 0) {
+            hipLaunchKernelGGL(prep_kernel, dim3((unsigned)((ds_ld + 255) / 256)), dim3(256), 0, st,
+                               PrepArgs{mats, c.rs, grad ? 1 : 0, ds_ld, sc, grad ? amax : nullptr});
+            TRY(hipGetLastError());
+        }
+        if (c.what == DGATED) {
+            hipLaunchKernelGGL(dy_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
+                               DyArgs{dy, c.dy_dt, tokens, c.rows, 0, sc, amax, nullptr, 0, 19, dfac});
+            TRY(hipGetLastError());
+        }
+        for (int64_t tile0 = 0; tile0 < p.tiles; tile0 += p.piece) {
+            const int64_t tiles = std::min(p.piece, p.tiles - tile0);
+            const int vkt = (int)(tiles / 2);
+            TRY(dequant(DequantArgs{mats, tile0, w, wt, vkt}, c.cb_dt, c.s2, w ? p.parts : 0, wt ? p.tparts : 0, tiles, st));
+            const PanelGemmArgs g{w, xp, p.parts * p.kt, p.kt, (int)(tiles * 16 / pg_m(8)), tp / PG_N, 1};
+            if (c.what == STATS)
+                TRY((gemm<8>(g, StatsEpi{sc, fac, target, c.rows, c.ignore, tokens, tp, (f32x2_t*)(ws + p.stats),
+                                         (float*)(ws + p.at)}, tile0, st)));
+            else if (c.what == GATED)
+                TRY((gemm<8>(g, GatedEpi{sc, fac, (char*)c.y + t0 * c.rows * dt_size(c.y_dt), c.y_dt, tokens, c.rows,
+                                         c.rows % 4 == 0 && (uintptr_t)c.y % 16 == 0, c.act}, tile0, st)));
+            else if (c.what == DLOGIT)
+                TRY((gemm<8>(g, DlogitEpi{sc, fac, c.lse + t0, c.dloss + t0, target, amax, c.rows, c.ignore, tile0, tokens, tp, vkt,
+                                          pp, ds, ds_ld}, tile0, st)));
+            else if (c.what == DGATED)
+                TRY((gemm<8>(g, DgatedEpi{sc, fac, dfac, dy, amax, c.dy_dt, tokens, tp, vkt, c.rows, tile0, pp, ds, ds_ld, c.act},
+                             tile0, st)));
+            else if (first)
+                TRY((gemm<8>(g, ColsumEpi{fac, dy, c.dy_dt, tokens, c.rows, ds, ds_ld}, tile0, st)));
+            if (!grad) continue;
+            if (c.what == PRODUCT) {
+                // (a piece's rows of dy; their largest value is taken over all rows)
+                hipLaunchKernelGGL(dy_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
+                                   DyArgs{dy, c.dy_dt, tokens, c.rows, tile0 * 16, sc, amax, pp, vkt, 0, dfac});
+                TRY(hipGetLastError());
+            }
+            const int slices = (int)std::min<int64_t>(p.slices, vkt);
+            const PanelGemmArgs g2{wt, pp, p.tparts * vkt, vkt, (int)(p.np / pg_m(8)), tp / PG_N, slices};
+            TRY((gemm<8>(g2, GradEpi{acc, p.np, tp, tile0 != 0}, 0, st)));
+        }
+        if (c.what == STATS) {
+            hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((tokens + 15) / 16)), dim3(256), 0, st,
+                               LseArgs{(const f32x2_t*)(ws + p.stats), p.tiles / 8, tokens, tp, target, c.rows, c.ignore,
+                                       (const float*)(ws + p.at), c.loss + t0, c.lse_out + t0});
+            TRY(hipGetLastError());
+        }
+        if (!grad) continue;
+        hipLaunchKernelGGL(dx_kernel, dim3((unsigned)((c.n + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st,
+                           DxArgs{acc, p.slices, tp, (int)c.n, p.np, amax, c.what == DLOGIT ? nullptr : dfac,
+                                  c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore,
+                                  (char*)c.y + t0 * c.n * dt_size(c.y_dt), c.y_dt});
+        TRY(hipGetLastError());
+        if (ds) {
+            hipLaunchKernelGGL(ds_kernel, dim3((unsigned)((ds_ld + 255) / 256)), dim3(256), 0, st,
+                               DsArgs{mats, ds, tp / (16 * PG_NT), ds_ld, c.rs, {c.ds[0], c.ds[1]}, t0 != 0});
+            TRY(hipGetLastError());
+        }
+    }
+    return VQ2_OK;
+}
+
+}  // namespace vq2

@@ -14,7 +14,9 @@ Kept names and signatures (reference: vq2/kernels.py):
 
 Additive entry points: vq_gemv_16_16 (4 bpw), batched GEMV (x of shape
 [B, n]), vq_rht, vq_swiglu_rht, vq_router_topk, vq_router_select,
-vq_moe_down_combine, vq_gemv_argmax, vq_sample, vq_argmax, vq_dequant_rows, vq_decode_idx.
+vq_moe_down_combine, vq_gemv_argmax, vq_sample, vq_argmax, vq_dequant_rows, vq_decode_idx;
+around the packed products and for tuning: vq_add_rms_norm, vq_gated_rows,
+vq_head_loss and their backward passes, vq_gemm_backward.
 
 The entries of the small calls (vq_sorted_gemv, vq_gemv_rht, vq_rows_gemm,
 vq_sorted_moe, vq_router_select, vq_sample) hand the calls without given
@@ -49,7 +51,8 @@ __all__ = [
     "vq_gemv_rht", "vq_moe_gate_up_rht", "vq_moe_down_swiglu_combine", "vq_gemm_small_m",
     "vq_moe_router_gate_up_rht", "vq_unpack_fixed", "SortedPlanes", "vq_sorted_gemv", "vq_sorted_gemv_argmax",
     "vq_rht", "vq_swiglu_rht", "vq_router_topk", "vq_router_select", "vq_sample", "vq_gemv_argmax", "vq_argmax",
-    "vq_dequant_rows", "vq_decode_idx", "patch_transformers_kernels",
+    "vq_add_rms_norm", "vq_add_rms_norm_backward", "vq_gated_rows", "vq_gated_rows_backward", "vq_head_loss",
+    "vq_head_loss_backward", "vq_gemm_backward", "vq_dequant_rows", "vq_decode_idx", "patch_transformers_kernels",
     "optimize_deltanet_layers", "Vq2Error",
 ]
 
@@ -1672,3 +1675,268 @@ def vq_unpack_fixed(buf, bits, n, *, out=None):
         raise Vq2Error("out must be int16 with at least n elements")
     _lib.call("vq2_unpack_fixed", _p(b), b.numel(), int(bits), n, _p(_contig(out, "out")), _stream(dev))
     return out
+
+
+# ------------------------------- around the packed products, and their gradients
+_DT8 = {torch.int8: _lib.DT_I8, torch.float8_e4m3fn: _lib.DT_E4M3}
+_ACTS = {"silu": _lib.ACT_SILU, "gelu_tanh": _lib.ACT_GELU_TANH}
+
+
+def _rotation_args(perm, sign, n, hb, rht_scale, what):
+    """(hb, scale) of an optional rotation: hb 0 is none."""
+    hb = int(hb or 0)
+    if hb == 0 and (perm is not None or sign is not None):
+        raise Vq2Error(f"{what}: perm and sign need the rotation's block hb")
+    _perm_sign(perm, sign, n, f"{what}: ")
+    return hb, (float(hb) ** -0.5 if hb else 1.0) if rht_scale is None else float(rht_scale)
+
+
+def _same(t, like, what, dtype=None):
+    if t.shape != like.shape or t.dtype != (dtype or like.dtype):
+        raise Vq2Error(f"{what} must be {dtype or like.dtype} {tuple(like.shape)}, got {t.dtype} {tuple(t.shape)}")
+    return _contig(t, what)
+
+
+def vq_add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, perm=None, sign=None, hb=0, rht_scale=None,
+                    out_dtype=None, h=None):
+    """The norm in front of packed products: h = x + residual, y = h / rms(h)
+    * weight over the last dim (zero_centred: 1 + weight), and where hb is
+    given its rotation, as vq_rht makes it of y, in one launch.  x [..., n],
+    n up to 8192.  Returns (y, h, y_scale): h is the sum in x's dtype (x itself
+    without a residual; given h, which may be x or residual, it goes there); y is of out_dtype (x's by default), y_scale None.
+    out_dtype int8 / float8_e4m3fn: y in 8 bits under y_scale fp32 [rows] (largest magnitude / 127 or 448),
+    which vq_gated_rows and vq_head_loss take as x and x_scale."""
+    dev = _dev(x, weight, residual, perm, sign, h)
+    n = x.shape[-1]
+    _contig(x, "x")
+    if weight.numel() != n:
+        raise Vq2Error(f"weight has {weight.numel()} entries, expected {n}")
+    _contig(weight, "weight")
+    if residual is None:
+        if h is not None:
+            raise Vq2Error("vq_add_rms_norm: h without a residual")
+    else:
+        _same(residual, x, "residual")
+        h = torch.empty_like(x) if h is None else _same(h, x, "h")
+    hb, sc = _rotation_args(perm, sign, n, hb, rht_scale, "vq_add_rms_norm")
+    rows = x.numel() // n if n else 0
+    odt = out_dtype or x.dtype
+    ydt = _DT8.get(odt)
+    y = torch.empty(x.shape, dtype=odt, device=dev)
+    y_scale = None
+    if ydt is None:
+        ydt = _dt(y, "y")
+    else:
+        y_scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        _lib.call("vq2_add_rms_norm", _p(x), _dt(x, "x"), _p(residual), rows, n, _p(weight), _dt(weight, "weight"),
+                  1 if zero_centred else 0, float(eps), _p(perm), _p(sign), hb, sc, _p(y), ydt, _p(y_scale), _p(h),
+                  _stream(dev))
+    return y, x if h is None else h, y_scale
+
+
+def vq_add_rms_norm_backward(dy, h, weight, dh=None, *, eps=1e-6, zero_centred=False, perm=None, sign=None, hb=0,
+                             rht_scale=None, weight_grad=True):
+    """Backward pass of vq_add_rms_norm from the gradient dy of its y, the
+    forward's h, and the gradient dh that reaches h elsewhere (None: none).
+    Returns (dx, dweight): dx in h's dtype is the gradient of x and of
+    residual alike; dweight fp32 [n], the sum over the rows in a fixed order
+    (None where weight_grad is False)."""
+    dev = _dev(dy, h, weight, dh, perm, sign)
+    n = h.shape[-1]
+    _contig(h, "h")
+    _same(dy, h, "dy", dy.dtype)
+    if dh is not None:
+        _same(dh, h, "dh")
+    if weight.numel() != n:
+        raise Vq2Error(f"weight has {weight.numel()} entries, expected {n}")
+    _contig(weight, "weight")
+    hb, sc = _rotation_args(perm, sign, n, hb, rht_scale, "vq_add_rms_norm_backward")
+    rows = h.numel() // n if n else 0
+    dx = torch.empty_like(h)
+    dw = ws = None
+    nbytes = 0
+    with _on_device(dev):
+        if weight_grad:
+            dw = torch.empty(n, dtype=torch.float32, device=dev)
+            nbytes = int(_lib.load().vq2_add_rms_norm_backward_workspace(rows, n))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_add_rms_norm_backward", _p(dy), _dt(dy, "dy"), _p(h), _dt(h, "h"), _p(dh), rows, n, _p(weight),
+                  _dt(weight, "weight"), 1 if zero_centred else 0, float(eps), _p(perm), _p(sign), hb, sc, _p(dx), _p(dw),
+                  _p(ws), nbytes, _stream(dev))
+    return dx, dw
+
+
+def _panel_x(xr, x_scale, n, bits8=True):
+    """(rows [T, n], dtype code) of a panel entry's activation"""
+    if xr.shape[-1] != n:
+        raise Vq2Error(f"xr must have a last dim of n={n}")
+    x2 = _contig(xr, "xr").reshape(-1, n)
+    dt = _DT8.get(xr.dtype) if bits8 else None
+    if dt is None:
+        if xr.dtype not in (torch.float16, torch.bfloat16):
+            raise Vq2Error(f"xr: unsupported dtype {xr.dtype} (float16 / bfloat16{', int8 / float8_e4m3fn' if bits8 else ''})")
+        dt = _DT[xr.dtype]
+        if x_scale is not None:
+            raise Vq2Error("x_scale is for 8-bit rows")
+    else:
+        if x_scale is None:
+            raise Vq2Error("8-bit rows need their x_scale")
+        if x_scale.dtype != torch.float32 or x_scale.numel() != x2.shape[0] or not x_scale.is_contiguous():
+            raise Vq2Error(f"x_scale must be a contiguous float32 [{x2.shape[0]}]")
+    return x2, dt
+
+
+def _token_vec(t, T, dtype, what):
+    if t.dtype != dtype or t.numel() != T or not t.is_contiguous():
+        raise Vq2Error(f"{what} must be a contiguous {dtype} [{T}]")
+    return t
+
+
+def vq_head_loss(xr, targets, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, x_scale=None, ignore_index=-100):
+    """Softmax cross entropy of the packed head over rotated rows xr [T, n]
+    (fp16 / bf16, or 8 bits under x_scale as vq_add_rms_norm gives them)
+    against targets int64 [T], in pieces of the vocabulary, the logits never
+    kept: (loss fp32 [T], lse fp32 [T]).  A target of ignore_index gives a
+    loss of 0, any other outside [0, out) NaN."""
+    dev = _dev(xr, targets, i0, i1, cb0, cb1, scale, x_scale)
+    n, out = int(n), int(out)
+    x2, xdt = _panel_x(xr, x_scale, n)
+    T = x2.shape[0]
+    i0, i1, s2 = _planes(i0, i1, cb0, cb1, scale, out, n)
+    _token_vec(targets, T, torch.int64, "targets")
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    cdt = _dt(cb0, "cb0")
+    with _on_device(dev):
+        nbytes = int(_lib.load().vq2_head_loss_workspace(T, out, n, s2, cdt))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_head_loss", _p(x2), xdt, _p(x_scale), T, _p(targets), int(ignore_index), _p(i0), _p(i1), s2, _p(cb0),
+                  _p(cb1), cdt, _p(scale), _dt(scale, "scale"), out, n, float(rs), _p(loss), _p(lse), _p(ws), nbytes,
+                  _stream(dev))
+    return loss, lse
+
+
+def vq_head_loss_backward(xr, targets, lse, dloss, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, ignore_index=-100,
+                          scale_grad=False):
+    """Backward pass of vq_head_loss from its lse and the gradient dloss fp32
+    [T] of every token's loss: (dxr in xr's shape and dtype, dscale fp32 [out]
+    or None).  Tokens of ignore_index give zeros."""
+    dev = _dev(xr, targets, lse, dloss, i0, i1, cb0, cb1, scale)
+    n, out = int(n), int(out)
+    x2, xdt = _panel_x(xr, None, n, bits8=False)
+    T = x2.shape[0]
+    i0, i1, s2 = _planes(i0, i1, cb0, cb1, scale, out, n)
+    _token_vec(targets, T, torch.int64, "targets")
+    _token_vec(lse, T, torch.float32, "lse")
+    _token_vec(dloss, T, torch.float32, "dloss")
+    dx = torch.empty_like(xr)
+    ds = torch.empty(out, dtype=torch.float32, device=dev) if scale_grad else None
+    cdt = _dt(cb0, "cb0")
+    with _on_device(dev):
+        nbytes = int(_lib.load().vq2_head_loss_backward_workspace(T, out, n, s2, cdt, xdt, 1 if scale_grad else 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_head_loss_backward", _p(x2), xdt, T, _p(targets), int(ignore_index), _p(lse), _p(dloss), _p(i0),
+                  _p(i1), s2, _p(cb0), _p(cb1), cdt, _p(scale), _dt(scale, "scale"), out, n, float(rs), _p(dx), xdt,
+                  _p(ds), _p(ws), nbytes, _stream(dev))
+    return dx, ds
+
+
+def _gated_mats(gate, up, cb0, cb1, n):
+    """(s2, segments, rows, scale dtype) of a gated block's two matrices,
+    each (i0, i1, scale)"""
+    rows = gate[2].numel()
+    s2, mats = check_gemv_rht_mats([(*gate, rows), (*up, up[2].numel())], cb0, cb1, n)
+    if up[2].numel() != rows:
+        raise Vq2Error(f"gate has {rows} rows, up {up[2].numel()}")
+    segs = (_lib.Seg * 2)()
+    for k, (i0, i1, scale, r) in enumerate(mats):
+        segs[k] = _lib.Seg(_p(i0), _p(i1), _p(scale), None, r, r)
+    return s2, segs, rows, _dt(gate[2], "scale"), mats
+
+
+def _act(activation):
+    try:
+        return _ACTS[activation]
+    except KeyError:
+        raise Vq2Error(f"unknown activation {activation!r} ({' / '.join(_ACTS)})") from None
+
+
+def vq_gated_rows(xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", x_scale=None, out_dtype=None):
+    """Gated feed-forward block over rotated rows xr [..., n] (fp16 / bf16, or
+    8 bits under x_scale): f(gate xr) * (up xr) [..., rows], f "silu" or
+    "gelu_tanh"; both products, the activation and the product of the two in
+    one pass, nothing in between stored.  gate, up: (i0, i1 or None, scale),
+    of one cfg.  out_dtype: xr's by default, bf16 for 8-bit rows."""
+    dev = _dev(xr, *gate, *up, cb0, cb1, x_scale)
+    n = int(n)
+    act = _act(activation)
+    x2, xdt = _panel_x(xr, x_scale, n)
+    T = x2.shape[0]
+    s2, segs, rows, sdt, _keep = _gated_mats(gate, up, cb0, cb1, n)
+    y = torch.empty((*xr.shape[:-1], rows), dtype=out_dtype or (xr.dtype if xr.dtype in _DT else torch.bfloat16), device=dev)
+    cdt, ydt = _dt(cb0, "cb0"), _dt(y, "y")
+    with _on_device(dev):
+        nbytes = int(_lib.load().vq2_gated_rows_workspace(T, rows, n, s2, cdt, ydt))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_gated_rows", _p(x2), xdt, _p(x_scale), T, segs, s2, _p(cb0), _p(cb1), cdt, sdt, n, float(rs), act,
+                  _p(y), ydt, _p(ws), nbytes, _stream(dev))
+    return y
+
+
+def vq_gated_rows_backward(dact, xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", scale_grad=False):
+    """Backward pass of vq_gated_rows from the gradient dact [..., rows] of its
+    result; the two products are made again.  Returns (dxr in xr's shape and
+    dtype, dgate fp32 [rows], dup fp32 [rows]): the latter are the row scales'
+    gradients, None unless scale_grad."""
+    dev = _dev(dact, xr, *gate, *up, cb0, cb1)
+    n = int(n)
+    act = _act(activation)
+    x2, xdt = _panel_x(xr, None, n, bits8=False)
+    T = x2.shape[0]
+    s2, segs, rows, sdt, _keep = _gated_mats(gate, up, cb0, cb1, n)
+    if dact.numel() != T * rows or dact.shape[-1] != rows:
+        raise Vq2Error(f"dact must be [{T}, {rows}], got {tuple(dact.shape)}")
+    _contig(dact, "dact")
+    dx = torch.empty_like(xr)
+    dg = torch.empty(rows, dtype=torch.float32, device=dev) if scale_grad else None
+    du = torch.empty(rows, dtype=torch.float32, device=dev) if scale_grad else None
+    cdt = _dt(cb0, "cb0")
+    with _on_device(dev):
+        nbytes = int(_lib.load().vq2_gated_rows_backward_workspace(T, rows, n, s2, cdt, xdt, 1 if scale_grad else 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_gated_rows_backward", _p(dact), _dt(dact, "dact"), _p(x2), xdt, T, segs, s2, _p(cb0), _p(cb1), cdt,
+                  sdt, n, float(rs), act, _p(dx), xdt, _p(dg), _p(du), _p(ws), nbytes, _stream(dev))
+    return dx, dg, du
+
+
+def vq_gemm_backward(dy, xr, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, scale_grad=False, dx_dtype=None):
+    """Backward pass of a packed product y = vq_gemv / vq_gemm_small_m /
+    vq_rows_gemm (hb=0) of rotated rows xr [..., n], from dy [..., out]:
+    (dxr [..., n], dscale fp32 [out] or None).  xr is read only for dscale and
+    may be None without it; dxr is of dx_dtype (float16 / bfloat16), by default xr's, or dy's
+    without one."""
+    dev = _dev(dy, xr, i0, i1, cb0, cb1, scale)
+    n, out = int(n), int(out)
+    i0, i1, s2 = _planes(i0, i1, cb0, cb1, scale, out, n)
+    if dy.shape[-1] != out:
+        raise Vq2Error(f"dy must have a last dim of {out}, got {tuple(dy.shape)}")
+    _contig(dy, "dy")
+    T = dy.numel() // out
+    x2, xdt = None, _lib.DT_F16
+    if xr is not None:
+        if xr.shape[:-1] != dy.shape[:-1]:
+            raise Vq2Error(f"xr {tuple(xr.shape)} and dy {tuple(dy.shape)} have different rows")
+        x2, xdt = _panel_x(xr, None, n, bits8=False)
+    elif scale_grad:
+        raise Vq2Error("vq_gemm_backward: the scales' gradient needs xr")
+    dx = torch.empty((*dy.shape[:-1], n), dtype=dx_dtype or (dy if xr is None else xr).dtype, device=dev)
+    ddt = _dt(dx, "dx")
+    ds = torch.empty(out, dtype=torch.float32, device=dev) if scale_grad else None
+    cdt = _dt(cb0, "cb0")
+    with _on_device(dev):
+        nbytes = int(_lib.load().vq2_gemm_backward_workspace(T, out, n, s2, cdt, ddt, 1 if scale_grad else 0))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("vq2_gemm_backward", _p(dy), _dt(dy, "dy"), _p(x2), xdt, T, _p(i0), _p(i1), s2, _p(cb0), _p(cb1), cdt,
+                  _p(scale), _dt(scale, "scale"), out, n, float(rs), _p(dx), ddt, _p(ds), _p(ws), nbytes, _stream(dev))
+    return dx, ds

@@ -32,6 +32,13 @@ extern "C" {
 #define VQ2_DT_F32 0
 #define VQ2_DT_F16 1
 #define VQ2_DT_BF16 2
+/* 8-bit rows under a scale for each row, where an entry says so */
+#define VQ2_DT_I8 3
+#define VQ2_DT_E4M3 4
+
+/* activations of the gated block */
+#define VQ2_ACT_SILU 0
+#define VQ2_ACT_GELU_TANH 1
 
 /* stage-2 index plane kinds */
 #define VQ2_S2_NONE 0 /* cfg (16,):   2 bpw, one int16 plane                        */
@@ -723,6 +730,101 @@ int vq2_decode_idx(const void* in, int is_u8, int64_t count, int32_t* out, void*
  * vq2/export.py:39-53 (pack_fixed).  Replaces unpack_fixed
  * (vq2/export.py:56-70) at container load time. */
 int vq2_unpack_fixed(const uint8_t* buf, int64_t nbytes, int bits, int64_t n, int16_t* out, void* stream);
+
+/* The norm in front of packed products.  Per row: h = x + residual (residual
+ * may be NULL: h = x), r = (sum h^2 / n + eps)^-1/2, u = h r w, and y = u or,
+ * where hb is not 0, its transform as by vq2_rht: blockdiag(H_hb)(sign *
+ * u[perm]) * rht_scale (perm / sign may be NULL).
+ *   x, residual, h [rows, n] of x_dt; h receives the sum (rounded; y is made
+ *     from the unrounded one), may be NULL without a residual, and may be x or
+ *     residual itself
+ *   weight [n] of w_dt; zero_centred: it holds the distance from 1
+ *   y [rows, n]: VQ2_DT_F32 / F16 / BF16, or VQ2_DT_I8 / VQ2_DT_E4M3 of y_scale [rows]
+ *     each: y_scale = largest magnitude / 127 (/ 448), y = u / y_scale to the
+ *     nearest; a row with a NaN or an infinity has that for its scale
+ * n up to VQ2_NORM_MAX_N; rotated: n a multiple of 64, hb a power of two from
+ * 64 on that divides n, and 16-byte aligned rows and tables' entries in order.
+ * The reference's counterpart is its residual + zero-centred norm kernel
+ * (vq2/kernels.py:375-395). */
+#define VQ2_NORM_MAX_N 8192
+#define VQ2_NORM_MAX_ROWS 1099511627776LL /* 2^40 */
+int vq2_add_rms_norm(const void* x, int x_dt, const void* residual, int64_t rows, int64_t n,
+                     const void* weight, int w_dt, int zero_centred, float eps,
+                     const int32_t* perm, const int8_t* sign, int64_t hb, float rht_scale,
+                     void* y, int y_dt, float* y_scale, void* h, void* stream);
+
+/* Its backward pass: dy [rows, n] of dy_dt is the gradient of y, dh (of h_dt,
+ * or NULL) the one that reaches h elsewhere, h the forward's.  dx [rows, n] of h_dt is
+ * the gradient of x and of residual alike (it may be dh itself); dweight [n] fp32, summed over
+ * the rows in a fixed order, or NULL.  perm must be a permutation. */
+size_t vq2_add_rms_norm_backward_workspace(int64_t rows, int64_t n);
+int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt, const void* dh, int64_t rows,
+                              int64_t n, const void* weight, int w_dt, int zero_centred, float eps,
+                              const int32_t* perm, const int8_t* sign, int64_t hb, float rht_scale,
+                              void* dx, float* dweight, void* workspace, size_t ws_bytes, void* stream);
+
+/* Many-row products of packed matrices with what follows them, and the
+ * gradients through the frozen codes.  Common to the entries below:
+ *   x       [tokens, n] rotated rows, 16-byte aligned: VQ2_DT_F16 / BF16, in forward
+ *           calls also VQ2_DT_I8 / VQ2_DT_E4M3 with x_scale [tokens] (NULL otherwise)
+ *   n       a multiple of 64 up to VQ2_PANEL_MAX_N; out_rows up to VQ2_PANEL_MAX_ROWS
+ *   dx      gradients of x, VQ2_DT_F16 / BF16;  dscale  of the row scales, fp32, or NULL
+ *   workspace  256-byte aligned, of the entry's _workspace bytes (scale_grad:
+ *           whether dscale is wanted); contents on entry do not matter
+ * Results do not depend on what ran before, and sums have a fixed order. */
+#define VQ2_PANEL_MAX_N 32768
+#define VQ2_PANEL_MAX_ROWS 4194304
+#define VQ2_PANEL_MAX_TOKENS 1099511627776LL /* 2^40 */
+
+/* Softmax cross entropy of a packed head without its logits: for every token
+ * lse = log sum_v exp(l_v), l_v = scale[v] * rs * (W_v . x), and loss = lse -
+ * l_target; 0 for a target of ignore_index, NaN for any other outside [0,
+ * out_rows).  The reference evaluates perplexity from whole logits
+ * (vq2/common.py:190-216). */
+size_t vq2_head_loss_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt);
+int vq2_head_loss(const void* x, int x_dt, const float* x_scale, int64_t tokens, const int64_t* targets,
+                  int64_t ignore_index, const int16_t* idx0, const void* idx1, int s2_kind,
+                  const void* cb0, const void* cb1, int cb_dt, const void* scale, int s_dt,
+                  int64_t out_rows, int64_t n, float rs, float* loss, float* lse,
+                  void* workspace, size_t ws_bytes, void* stream);
+
+/* Its backward pass, with the forward's lse and the gradient dloss [tokens]
+ * of every token's loss: dx [tokens, n] of dx_dt, dscale [out_rows].  Tokens
+ * of ignore_index give zeros whatever else they hold. */
+size_t vq2_head_loss_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                        int scale_grad);
+int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_t* targets, int64_t ignore_index,
+                           const float* lse, const float* dloss, const int16_t* idx0, const void* idx1, int s2_kind,
+                           const void* cb0, const void* cb1, int cb_dt, const void* scale, int s_dt,
+                           int64_t out_rows, int64_t n, float rs, void* dx, int dx_dt, float* dscale,
+                           void* workspace, size_t ws_bytes, void* stream);
+
+/* Gated feed-forward block: y[t, i] = f(g) u, g = gate scale * rs * (gate row
+ * i . x_t), u alike; f by act (VQ2_ACT_*).  mats[0] is gate, mats[1] up (their
+ * y and y_stride are not used), of the same out_rows. */
+size_t vq2_gated_rows_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int y_dt);
+int vq2_gated_rows(const void* x, int x_dt, const float* x_scale, int64_t tokens, const vq2_seg* mats,
+                   int s2_kind, const void* cb0, const void* cb1, int cb_dt, int s_dt, int64_t n, float rs, int act,
+                   void* y, int y_dt, void* workspace, size_t ws_bytes, void* stream);
+
+/* Its backward pass from dy [tokens, out_rows]: both products are made again.
+ * dx [tokens, n] of dx_dt; dgate / dup [out_rows], both or neither. */
+size_t vq2_gated_rows_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                         int scale_grad);
+int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens,
+                            const vq2_seg* mats, int s2_kind, const void* cb0, const void* cb1, int cb_dt,
+                            int s_dt, int64_t n, float rs, int act, void* dx, int dx_dt, float* dgate, float* dup,
+                            void* workspace, size_t ws_bytes, void* stream);
+
+/* Backward pass of a packed product y = scale * rs * (W x): dx[t] = sum_r
+ * dy[t, r] scale[r] rs W_r (dx_dt), and dscale[r] = rs sum_t dy[t, r] (W_r .
+ * x_t).  x may be NULL where dscale is. */
+size_t vq2_gemm_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
+                                   int scale_grad);
+int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens, const int16_t* idx0,
+                      const void* idx1, int s2_kind, const void* cb0, const void* cb1, int cb_dt, const void* scale,
+                      int s_dt, int64_t out_rows, int64_t n, float rs, void* dx, int dx_dt, float* dscale,
+                      void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
