@@ -37,14 +37,40 @@ __device__ __forceinline__ float dpp_xor4(float v)
 __device__ __forceinline__ float dpp_xor8(float v) { return __int_as_float(dpp_mov<0x128>(__float_as_int(v))); }  // row_ror:8
 
 // One butterfly stage between lanes: the lane whose bit is clear takes the
-// sum, the other the difference.
+// sum, the other the difference (two instructions a value: the exchange is
+// part of the addition).
 template <class X>
 __device__ __forceinline__ void lane_stage(float (&v)[8], bool high, X other)
 {
+    const float s = high ? -1.0f : 1.0f;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        const float o = other(v[k]);
-        v[k] = high ? o - v[k] : v[k] + o;
+        const float t = v[k] * s;
+        v[k] = other(v[k]) + t;
+    }
+}
+// Between rows of 16 lanes (STEP 16) or halves of the wave (32), two values
+// at a time: a swap brings both partners of one value into one lane, and
+// another puts the results back.
+template <int STEP>
+__device__ __forceinline__ void swap2(float& a, float& b)
+{
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    const auto r = STEP == 16 ? __builtin_amdgcn_permlane16_swap(x, y, false, false)
+                              : __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+template <int STEP>
+__device__ __forceinline__ void swap_stage(float (&v)[8])
+{
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+        swap2<STEP>(v[k], v[k + 1]);
+        const float s = v[k] + v[k + 1], d = v[k] - v[k + 1];
+        v[k] = s;
+        v[k + 1] = d;
+        swap2<STEP>(v[k], v[k + 1]);
     }
 }
 
@@ -69,10 +95,16 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
         lane_stage(v[c], lane & 1, [](float a) { return dpp_xor1(a); });
         lane_stage(v[c], lane & 2, [](float a) { return dpp_xor2(a); });
         lane_stage(v[c], lane & 4, [](float a) { return dpp_xor4(a); });
-        if (hb >= 128) lane_stage(v[c], lane & 8, [](float a) { return dpp_xor8(a); });
-        if (hb >= 256) lane_stage(v[c], lane & 16, [](float a) { return swz_xor16(a); });
-        if (hb >= 512) lane_stage(v[c], lane & 32, [](float a) { return xor32(a); });
     }
+    if (hb >= 128)
+#pragma unroll
+        for (int c = 0; c < V; c++) lane_stage(v[c], lane & 8, [](float a) { return dpp_xor8(a); });
+    if (hb >= 256)
+#pragma unroll
+        for (int c = 0; c < V; c++) swap_stage<16>(v[c]);
+    if (hb >= 512)
+#pragma unroll
+        for (int c = 0; c < V; c++) swap_stage<32>(v[c]);
     if (TPR == 64 || hb < 1024) return;
     // between the waves: value of wave w gets sum over w' of +- theirs
     const int w = id >> 6;
@@ -84,6 +116,7 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
         p[(c * 2 + 1) * TPR + id] = f32x4_t{v[c][4], v[c][5], v[c][6], v[c][7]};
     }
     __syncthreads();
+    const float s1 = w & 1 ? -1.0f : 1.0f, s2 = w & 2 ? -1.0f : 1.0f;
 #pragma unroll
     for (int c = 0; c < V; c++)
 #pragma unroll
@@ -92,11 +125,10 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
             f32x4_t o;
             if (hb == 1024) {
                 const f32x4_t a = q[(w & ~1) * 64], b = q[(w | 1) * 64];
-                o = w & 1 ? a - b : a + b;
+                o = a + b * s1;
             } else {
                 const f32x4_t a = q[0], b = q[64], d = q[128], e = q[192];
-                const f32x4_t lo = w & 1 ? a - b : a + b, hi = w & 1 ? d - e : d + e;
-                o = w & 2 ? lo - hi : lo + hi;
+                o = (a + b * s1) + (d + e * s1) * s2;
             }
 #pragma unroll
             for (int k = 0; k < 4; k++) v[c][4 * h + k] = o[k];
@@ -117,22 +149,27 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
     }
 }
 
-// a value every thread of the row has a part of; s: one word for each wave
-template <int TPR, class Op>
-__device__ __forceinline__ float row_reduce(float v, float* s, Op op)
+// N values that every thread of the row has a part of; s: N words for each wave
+template <int TPR, int N, class Op>
+__device__ __forceinline__ void row_reduce(float (&v)[N], float* s, Op op)
 {
-    v = op(v, dpp_xor1(v));
-    v = op(v, dpp_xor2(v));
-    v = op(v, dpp_half_mirror(v));
-    v = op(v, dpp_row_mirror(v));
-    v = op(v, swz_xor16(v));
-    v = op(v, xor32(v));
-    if (TPR == 64) return v;
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        v[i] = op(v[i], dpp_xor1(v[i]));
+        v[i] = op(v[i], dpp_xor2(v[i]));
+        v[i] = op(v[i], dpp_half_mirror(v[i]));
+        v[i] = op(v[i], dpp_row_mirror(v[i]));
+        v[i] = op(v[i], swz_xor16(v[i]));
+        v[i] = op(v[i], xor32(v[i]));
+    }
+    if (TPR == 64) return;
+    __syncthreads();  // (the last call's values have been read)
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if ((threadIdx.x & 63) == 0) s[i * 4 + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
-    v = op(op(s[0], s[1]), op(s[2], s[3]));
-    __syncthreads();
-    return v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = op(op(s[i * 4], s[i * 4 + 1]), op(s[i * 4 + 2], s[i * 4 + 3]));
 }
 __device__ __forceinline__ float add_op(float a, float b) { return a + b; }
 // maximum of magnitudes by their bits: a NaN is above everything and stays
@@ -149,24 +186,79 @@ __device__ __forceinline__ int place(int c, int k, int id)
     return VEC ? (c * TPR + id) * 8 + k : (c * 8 + k) * TPR + id;
 }
 
-template <int V, int TPR, bool VEC>
-__device__ __forceinline__ void load_row(float (&v)[V][8], const void* p, int dt, int64_t row, int n, int id)
+// A row's values as they are loaded (VEC: 16 or 32 bytes of type DT; else the
+// values in fp32), and as numbers.
+template <int DT, int V, bool VEC>
+struct Raw {
+    u32x4 w[V][VEC && DT != VQ2_DT_F32 ? 1 : 2];
+};
+template <int DT, int V, int TPR, bool VEC>
+__device__ __forceinline__ void load_raw(Raw<DT, V, VEC>& r, const void* p, int64_t row, int n, int id)
 {
 #pragma unroll
     for (int c = 0; c < V; c++) {
         if constexpr (VEC) {
-            Eight e = {{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}};
-            if (place<V, TPR, VEC>(c, 0, id) < n) e = load8(p, dt, row * n + place<V, TPR, VEC>(c, 0, id));
+            const int i = place<V, TPR, VEC>(c, 0, id);
+            constexpr int N = DT == VQ2_DT_F32 ? 2 : 1;
+            const u32x4* q = (const u32x4*)((const char*)p + (row * n + (i < n ? i : 0)) * (DT == VQ2_DT_F32 ? 4 : 2));
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[c][k] = e.v[k];
+            for (int k = 0; k < N; k++) r.w[c][k] = q[k];
+            if (i >= n)
+#pragma unroll
+                for (int k = 0; k < N; k++) r.w[c][k] = u32x4{0, 0, 0, 0};
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int i = place<V, TPR, VEC>(c, k, id);
-                v[c][k] = i < n ? load_as_f32(p, dt, row * n + i) : 0.0f;
+                r.w[c][k / 4][k % 4] = i < n ? __float_as_uint(load_as_f32(p, DT, row * n + i)) : 0;
             }
         }
     }
+}
+template <int DT, int V, bool VEC>
+__device__ __forceinline__ void numbers(float (&v)[V][8], const Raw<DT, V, VEC>& r)
+{
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        if constexpr (!VEC || DT == VQ2_DT_F32) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[c][k] = __uint_as_float(r.w[c][k / 4][k % 4]);
+        } else if constexpr (DT == VQ2_DT_F16) {
+            const half8_t h = __builtin_bit_cast(half8_t, r.w[c][0]);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[c][k] = (float)h[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                v[c][2 * k] = __uint_as_float(r.w[c][0][k] << 16);
+                v[c][2 * k + 1] = __uint_as_float(r.w[c][0][k] & 0xFFFF0000u);
+            }
+        }
+    }
+}
+template <int V, int TPR, bool VEC>
+__device__ __forceinline__ void load_row(float (&v)[V][8], const void* p, int dt, int64_t row, int n, int id)
+{
+    if (dt == VQ2_DT_F16) {
+        Raw<VQ2_DT_F16, V, VEC> r;
+        load_raw<VQ2_DT_F16, V, TPR, VEC>(r, p, row, n, id);
+        numbers(v, r);
+    } else if (dt == VQ2_DT_BF16) {
+        Raw<VQ2_DT_BF16, V, VEC> r;
+        load_raw<VQ2_DT_BF16, V, TPR, VEC>(r, p, row, n, id);
+        numbers(v, r);
+    } else {
+        Raw<VQ2_DT_F32, V, VEC> r;
+        load_raw<VQ2_DT_F32, V, TPR, VEC>(r, p, row, n, id);
+        numbers(v, r);
+    }
+}
+
+// two values rounded to bf16, one instruction
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b)
+{
+    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf2_t{(__bf16)a, (__bf16)b});
 }
 
 __device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (&v)[8])
@@ -182,7 +274,7 @@ __device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (
     } else {
         u32x4 u;
 #pragma unroll
-        for (int k = 0; k < 4; k++) u[k] = f32_to_bf16_bits(v[2 * k]) | (uint32_t)f32_to_bf16_bits(v[2 * k + 1]) << 16;
+        for (int k = 0; k < 4; k++) u[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
         *(u32x4*)((uint16_t*)p + i) = u;
     }
 }
@@ -225,68 +317,103 @@ __device__ __forceinline__ void store_row(const float (&v)[V][8], void* p, int d
     }
 }
 
-// Rotation tables of a thread's values (VEC), two entries a word: the place
-// the value comes from (13 bits) and its sign above; no place of the row
-// where the permutation's entry is none, which gives NaN as in vq2_rht.
-constexpr uint32_t NO_PLACE = 0x7FFF;
+// Rotation tables of a thread's values (VEC), two entries a word: four times
+// the place the value comes from (15 bits), its sign above.  A part with an entry
+// that is no place of the row gets a NaN added, which the transform spreads
+// over its block, as in vq2_rht.
+template <int V>
+struct Tables {
+    uint32_t w[V][4];
+    float nan[V];
+};
 template <int V, int TPR>
-__device__ __forceinline__ void load_tables(uint32_t (&tab)[V][4], const NormCall& a, int id)
+__device__ __forceinline__ void load_tables(Tables<V>& t, const NormCall& a, int id)
 {
 #pragma unroll
-    for (int c = 0; c < V; c++)
+    for (int c = 0; c < V; c++) {
+        t.nan[c] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int i = (c * TPR + id) * 8 + k;
-            uint32_t p = NO_PLACE, neg = 0;
+            uint32_t p = 0, neg = 0;
             if (i < a.n) {
                 p = a.perm ? (uint32_t)a.perm[i] : (uint32_t)i;
-                if (p >= (uint32_t)a.n) p = NO_PLACE;
+                if (p >= (uint32_t)a.n) {
+                    p = 0;
+                    t.nan[c] = __builtin_nanf("");
+                }
                 neg = a.sign && a.sign[i] < 0 ? 0x8000u : 0u;
             }
-            tab[c][k >> 1] = (k & 1 ? tab[c][k >> 1] : 0) | (p | neg) << (16 * (k & 1));
+            t.w[c][k >> 1] = (k & 1 ? t.w[c][k >> 1] : 0) | (p * 4 | neg) << (16 * (k & 1));
         }
+    }
 }
-__device__ __forceinline__ uint32_t entry(const uint32_t (&tab)[4], int k) { return tab[k >> 1] >> (16 * (k & 1)) & 0xFFFFu; }
+template <int V>
+__device__ __forceinline__ float& table_place(float* s, const Tables<V>& t, int c, int k)
+{
+    const uint32_t w = t.w[c][k >> 1];
+    return *(float*)((char*)s + ((k & 1 ? w >> 16 : w) & 0x7FFCu));
+}
+template <int V>
+__device__ __forceinline__ float table_sign(float v, const Tables<V>& t, int c, int k)
+{
+    const uint32_t w = t.w[c][k >> 1];
+    return __uint_as_float(__float_as_uint(v) ^ ((k & 1 ? w : w << 16) & 0x80000000u));
+}
 
 template <int DT, int V, int TPR, bool VEC, bool ROT>
-__global__ void __launch_bounds__(NT) norm_kernel(const NormCall a, int64_t row_step)
+__global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t row_step)
 {
     constexpr int RW = NT / TPR;  // rows of a workgroup
     __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
-    __shared__ float s_red[8];
+    __shared__ float s_red[4];
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
+    // the next row's values are on their way while this one is worked on
+    Raw<DT, V, VEC> rx, rr;
+    auto fetch = [&](int64_t r0) {
+        const int64_t at = min(r0 + rw, a.rows - 1);
+        load_raw<DT, V, TPR, VEC>(rx, a.x, at, a.n, id);
+        if (a.residual) load_raw<DT, V, TPR, VEC>(rr, a.residual, at, a.n, id);
+    };
+    fetch((int64_t)blockIdx.x * RW);
     float w[V][8];
-    uint32_t tab[V][4];
-    const float off = a.zero_centred ? 1.0f : 0.0f;
+    Tables<V> tab;
     load_row<V, TPR, VEC>(w, a.weight, a.w_dt, 0, a.n, id);
     if constexpr (ROT) load_tables<V, TPR>(tab, a, id);
+    if (a.zero_centred)
+#pragma unroll
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) w[c][k] += 1.0f;
     for (int64_t r0 = (int64_t)blockIdx.x * RW; r0 < a.rows; r0 += row_step) {
         const int64_t row = r0 + rw;
         const bool live = row < a.rows;  // (rows of a workgroup: whole waves)
-        const int64_t at = live ? row : a.rows - 1;
-        float h[V][8], e[V][8];
-        load_row<V, TPR, VEC>(h, a.x, DT, at, a.n, id);
+        float h[V][8];
+        numbers(h, rx);
         if (a.residual) {
-            load_row<V, TPR, VEC>(e, a.residual, DT, at, a.n, id);
+            float e[V][8];
+            numbers(e, rr);
 #pragma unroll
             for (int c = 0; c < V; c++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) h[c][k] += e[c][k];
         }
+        if (r0 + row_step < a.rows) fetch(r0 + row_step);
         if (a.h && live) store_row<V, TPR, VEC>(h, a.h, DT, row, a.n, id, 0.0f);
-        float sum = 0.0f;
+        float sum[1] = {0.0f};
 #pragma unroll
         for (int c = 0; c < V; c++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) sum += h[c][k] * h[c][k];
-        sum = row_reduce<TPR>(sum, s_red, add_op);
-        const float r = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+            for (int k = 0; k < 8; k++) sum[0] += h[c][k] * h[c][k];
+        row_reduce<TPR>(sum, s_red, add_op);
+        const float r = 1.0f / sqrtf(sum[0] / (float)a.n + a.eps);
 #pragma unroll
         for (int c = 0; c < V; c++)
 #pragma unroll
-            for (int k = 0; k < 8; k++) h[c][k] = h[c][k] * r * (w[c][k] + off);
+            for (int k = 0; k < 8; k++) h[c][k] = h[c][k] * r * w[c][k];
         if constexpr (ROT) {
+            __syncthreads();  // the last row's values have been read
 #pragma unroll
             for (int c = 0; c < V; c++) {
                 f32x4_t* p = (f32x4_t*)(s + (c * TPR + id) * 8);
@@ -295,105 +422,112 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormCall a, int64_t row_
             }
             __syncthreads();
 #pragma unroll
-            for (int c = 0; c < V; c++)
+            for (int c = 0; c < V; c++) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const uint32_t e = entry(tab[c], k), p = e & NO_PLACE;
-                    const float v = s[p == NO_PLACE ? 0 : p];
-                    h[c][k] = p == NO_PLACE ? __builtin_nanf("") : e & 0x8000u ? -v : v;
-                }
+                for (int k = 0; k < 8; k++) h[c][k] = table_sign(table_place(s, tab, c, k), tab, c, k);
+                h[c][0] += tab.nan[c];
+            }
             hadamard<V, TPR>(h, a.hb, id, s);
 #pragma unroll
             for (int c = 0; c < V; c++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) h[c][k] *= a.rht_scale;
-            __syncthreads();  // the next row's values go where these were
         }
         float inv = 0.0f;
         if (a.y_dt > VQ2_DT_BF16) {
-            float m = 0.0f;
+            float m[1] = {0.0f};
 #pragma unroll
             for (int c = 0; c < V; c++)
 #pragma unroll
                 for (int k = 0; k < 8; k++)
-                    if (place<V, TPR, VEC>(c, k, id) < a.n) m = bits_op(m, fabsf(h[c][k]));
-            m = row_reduce<TPR>(m, s_red, bits_op);
+                    if (place<V, TPR, VEC>(c, k, id) < a.n) m[0] = bits_op(m[0], fabsf(h[c][k]));
+            row_reduce<TPR>(m, s_red, bits_op);
             const float top = a.y_dt == VQ2_DT_I8 ? 127.0f : 448.0f;
-            inv = m > 0.0f ? top / m : 0.0f;
-            if (live && id == 0) a.y_scale[row] = m / top;
+            inv = m[0] > 0.0f ? top / m[0] : 0.0f;
+            if (live && id == 0) a.y_scale[row] = m[0] / top;
         }
         if (live) store_row<V, TPR, VEC>(h, a.y, a.y_dt, row, a.n, id, inv);
     }
 }
 
 template <int DT, int V, int TPR, bool VEC, bool ROT>
-__global__ void __launch_bounds__(NT) norm_grad_kernel(const NormCall a, int64_t row_step, float* part)
+__global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int64_t row_step, float* part)
 {
     constexpr int RW = NT / TPR;
     __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
     __shared__ float s_red[8];
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
+    const bool same = a.y_dt == DT;  // dy of h's type
+    Raw<DT, V, VEC> rh, rg;
+    auto fetch = [&](int64_t r0) {
+        const int64_t at = min(r0 + rw, a.rows - 1);
+        if (same) load_raw<DT, V, TPR, VEC>(rg, a.dy, at, a.n, id);
+        load_raw<DT, V, TPR, VEC>(rh, a.x, at, a.n, id);
+    };
+    fetch((int64_t)blockIdx.x * RW);
     float w[V][8], dw[V][8];
-    uint32_t tab[V][4];
-    const float off = a.zero_centred ? 1.0f : 0.0f;
+    Tables<V> tab;
     load_row<V, TPR, VEC>(w, a.weight, a.w_dt, 0, a.n, id);
     if constexpr (ROT) load_tables<V, TPR>(tab, a, id);
 #pragma unroll
     for (int c = 0; c < V; c++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) dw[c][k] = 0.0f;
+        for (int k = 0; k < 8; k++) {
+            if (a.zero_centred) w[c][k] += 1.0f;
+            dw[c][k] = 0.0f;
+        }
     for (int64_t r0 = (int64_t)blockIdx.x * RW; r0 < a.rows; r0 += row_step) {
-        const int64_t row = r0 + rw;
+        const int64_t row = r0 + rw, at = min(row, a.rows - 1);
         const bool live = row < a.rows;
-        const int64_t at = live ? row : a.rows - 1;
         float h[V][8], g[V][8];
-        if (a.y_dt == DT) load_row<V, TPR, VEC>(g, a.dy, DT, at, a.n, id);
+        if (same) numbers(g, rg);
         else load_row<V, TPR, VEC>(g, a.dy, a.y_dt, at, a.n, id);
-        load_row<V, TPR, VEC>(h, a.x, DT, at, a.n, id);
-        float e[V][8];
-        if (a.dh) load_row<V, TPR, VEC>(e, a.dh, DT, at, a.n, id);
+        numbers(h, rh);
+        Raw<DT, V, VEC> re;
+        if (a.dh) load_raw<DT, V, TPR, VEC>(re, a.dh, at, a.n, id);
+        if (r0 + row_step < a.rows) fetch(r0 + row_step);
         if constexpr (ROT) {
             hadamard<V, TPR>(g, a.hb, id, s);
             __syncthreads();
 #pragma unroll
-            for (int c = 0; c < V; c++)
+            for (int c = 0; c < V; c++) {
+                g[c][0] += tab.nan[c];
+                if ((c * TPR + id) * 8 < a.n)
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float v = g[c][k] * a.rht_scale;
-                    const uint32_t e = entry(tab[c], k), p = e & NO_PLACE;
-                    if (p != NO_PLACE) s[p] = e & 0x8000u ? -v : v;
-                }
+                    for (int k = 0; k < 8; k++) table_place(s, tab, c, k) = table_sign(g[c][k] * a.rht_scale, tab, c, k);
+            }
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < V; c++) {
                 const f32x4_t* p = (const f32x4_t*)(s + (c * TPR + id) * 8);
                 const f32x4_t lo = p[0], hi = p[1];
+                const bool in = (c * TPR + id) * 8 < a.n;  // (past the row nothing was written)
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    // (past the row nothing was written)
-                    g[c][k] = (c * TPR + id) * 8 < a.n ? lo[k] : 0.0f;
-                    g[c][4 + k] = (c * TPR + id) * 8 < a.n ? hi[k] : 0.0f;
+                    g[c][k] = in ? lo[k] : 0.0f;
+                    g[c][4 + k] = in ? hi[k] : 0.0f;
                 }
             }
         }
-        float sum = 0.0f, dot = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < V; c++)
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                sum += h[c][k] * h[c][k];
-                dot += g[c][k] * (w[c][k] + off) * h[c][k];
+                sum[0] += h[c][k] * h[c][k];
+                sum[1] += g[c][k] * w[c][k] * h[c][k];
             }
-        sum = row_reduce<TPR>(sum, s_red, add_op);
-        dot = row_reduce<TPR>(dot, s_red, add_op);
-        const float r = 1.0f / sqrtf(sum / (float)a.n + a.eps), b = r * r * r * (dot / (float)a.n);
+        row_reduce<TPR>(sum, s_red, add_op);
+        const float r = 1.0f / sqrtf(sum[0] / (float)a.n + a.eps), b = r * r * r * (sum[1] / (float)a.n);
+        float e[V][8];
+        if (a.dh) numbers(e, re);
 #pragma unroll
         for (int c = 0; c < V; c++)
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 if (live) dw[c][k] += g[c][k] * (h[c][k] * r);
-                const float d = r * (g[c][k] * (w[c][k] + off)) - h[c][k] * b;
+                const float d = r * (g[c][k] * w[c][k]) - h[c][k] * b;
                 e[c][k] = a.dh ? e[c][k] + d : d;
             }
         if (live) store_row<V, TPR, VEC>(e, a.y, DT, row, a.n, id, 0.0f);
@@ -401,12 +535,15 @@ __global__ void __launch_bounds__(NT) norm_grad_kernel(const NormCall a, int64_t
     if (!part) return;
     float* o = part + (int64_t)(blockIdx.x * RW + rw) * a.n;
 #pragma unroll
-    for (int c = 0; c < V; c++)
+    for (int c = 0; c < V; c++) {
+        if (VEC && place<V, TPR, VEC>(c, 0, id) < a.n) {
+            store8(o, VQ2_DT_F32, place<V, TPR, VEC>(c, 0, id), dw[c]);
+        } else if (!VEC) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int i = place<V, TPR, VEC>(c, k, id);
-            if (i < a.n) o[i] = dw[c][k];
+            for (int k = 0; k < 8; k++)
+                if (place<V, TPR, VEC>(c, k, id) < a.n) o[place<V, TPR, VEC>(c, k, id)] = dw[c][k];
         }
+    }
 }
 
 // dw: the sums of the workgroups, 64 columns a workgroup, 16 threads a column
@@ -442,7 +579,7 @@ Shape shape_of(const NormCall& c, bool grad)
     const int64_t rows = (c.rows + NT / s.tpr - 1) / (NT / s.tpr);
     // forward: enough workgroups to hide each other's loads; backward: fewer,
     // each leaves a row of sums
-    s.groups = std::min<int64_t>(rows, (int64_t)device_cu_count() * (grad ? 3 : s.v <= 2 ? 8 : 4));
+    s.groups = std::min<int64_t>(rows, (int64_t)device_cu_count() * (grad ? (s.v <= 2 ? 4 : 2) : s.v <= 2 ? 8 : 4));
     return s;
 }
 

@@ -53,6 +53,18 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits)
     return b == 0xFF ? 0 : min(max(b - 126, -100), 100);
 }
 
+// over the four lanes that hold a token's rows
+__device__ __forceinline__ float max_rows(float v)
+{
+    v = fmaxf(v, swz_xor16(v));
+    return fmaxf(v, xor32(v));
+}
+__device__ __forceinline__ float sum_rows(float v)
+{
+    v += swz_xor16(v);
+    return v + xor32(v);
+}
+
 // -------------------------------------------------------------- token rows
 struct PackArgs {
     const void* x;
@@ -64,44 +76,69 @@ struct PackArgs {
     uint32_t* amax;     // largest row scale, cleared here for prep_kernel
 };
 
-// One workgroup a tile of 16 rows: the rows' largest magnitudes, then fp16
-// under a power of two that brings it into [2^13, 2^14).
-__global__ void __launch_bounds__(256) pack_rows_kernel(const PackArgs a)
+// One workgroup a tile of 16 rows, its 16 waves a share of the k tiles each:
+// the rows' largest magnitudes, then fp16 under a power of two that brings
+// them into [2^13, 2^14).  Rows of up to 4096 values stay in registers in
+// between (4096 rows of 2048: 21 us with 4 waves that read twice).
+constexpr int PK_WAVES = 16, PK_HELD = 8;
+__global__ void __launch_bounds__(64 * PK_WAVES) pack_rows_kernel(const PackArgs a)
 {
-    __shared__ float s_f[16];
+    __shared__ float s_m[PK_WAVES][16];
     const int tid = threadIdx.x, tile = blockIdx.x;
     if (tile == 0 && tid == 0 && a.amax) *a.amax = 0;
-    {
-        const int r = tid >> 4, row = tile * 16 + r;
-        float m = 0.0f;
-        if (a.x_dt <= VQ2_DT_BF16 && row < a.tokens) {
-            for (int i = (tid & 15) * 8; i < a.n; i += 128) {
-                const Eight e = load8(a.x, a.x_dt, (int64_t)row * a.n + i);
+    const int lane = tid & 63, wave = tid >> 6, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
+    const int per = (kt + PK_WAVES - 1) / PK_WAVES, k0 = wave * per, k1 = min(k0 + per, kt);
+    const bool live = row < a.tokens, held = per <= PK_HELD;
+    const int64_t at = (int64_t)row * a.n + q * 8;
+    Eight x[PK_HELD];
+    float m = 0.0f;
+    if (held) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
-            }
-        }
-        m = fmaxf(m, dpp_xor1(m));
-        m = fmaxf(m, dpp_xor2(m));
-        m = fmaxf(m, dpp_half_mirror(m));
-        m = fmaxf(m, dpp_row_mirror(m));
-        if ((tid & 15) == 0) {
-            const int e = m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
-            s_f[r] = pow2(-e);
-            a.fac[row] = row < a.tokens ? pow2(e) * (a.x_scale ? a.x_scale[row] : 1.0f) : 0.0f;
+        for (int i = 0; i < PK_HELD; i++)
+            if (live && k0 + i < k1) x[i] = load8(a.x, a.x_dt, at + (k0 + i) * 32);
+            else
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[i].v[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PK_HELD; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(x[i].v[k]));
+    } else if (live) {
+        for (int k = k0; k < k1; k++) {
+            const Eight e = load8(a.x, a.x_dt, at + k * 32);
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(e.v[j]));
         }
     }
+    m = max_rows(m);
+    if (q == 0) s_m[wave][lane & 15] = m;
     __syncthreads();
-    const int lane = tid & 63, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
-    const float f = s_f[lane & 15];
-    for (int k = tid >> 6; k < kt; k += 4) {
-        half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (row < a.tokens) {
-            const Eight e = load8(a.x, a.x_dt, (int64_t)row * a.n + k * 32 + q * 8);
 #pragma unroll
-            for (int j = 0; j < 8; j++) h[j] = (_Float16)(e.v[j] * f);
+    for (int w = 0; w < PK_WAVES; w++) m = fmaxf(m, s_m[w][lane & 15]);
+    // (8-bit values are exact as they are)
+    const int e = a.x_dt <= VQ2_DT_BF16 && m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
+    if (tid < 16) a.fac[row] = live ? pow2(e) * (a.x_scale ? a.x_scale[row] : 1.0f) : 0.0f;
+    const float f = pow2(-e);
+    half8_t* out = a.panel + (int64_t)tile * kt * 64 + lane;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < PK_HELD; i++) {
+            if (k0 + i >= k1) break;
+            half8_t h;
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[j] = (_Float16)(x[i].v[j] * f);
+            out[(k0 + i) * 64] = h;
         }
-        a.panel[((int64_t)tile * kt + k) * 64 + lane] = h;
+    } else {
+        for (int k = k0; k < k1; k++) {
+            half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (live) {
+                const Eight v = load8(a.x, a.x_dt, at + k * 32);
+#pragma unroll
+                for (int j = 0; j < 8; j++) h[j] = (_Float16)(v.v[j] * f);
+            }
+            out[k * 64] = h;
+        }
     }
 }
 
@@ -156,8 +193,11 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a)
     if (!a.amax) return;
     // (magnitudes as bits are ordered like the numbers, and a maximum does
     // not depend on the order of its parts)
+    __shared__ float s_m[4];
     const float m = wave_max_all(fabsf(v));
-    if ((threadIdx.x & 63) == 0) atomicMax(a.amax, __float_as_uint(m));
+    if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) atomicMax(a.amax, __float_as_uint(fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]))));
 }
 
 template <int CBT>
@@ -300,18 +340,6 @@ __global__ void __launch_bounds__(256) dequant_turned_kernel(const DequantArgs a
 // What a product of weights (panel a) and tokens (panel b) is made into.
 // `tile` is the first weight tile of the wave, counted over all pieces, `tok`
 // its first token.
-
-// over the four lanes that hold a token's rows
-__device__ __forceinline__ float max_rows(float v)
-{
-    v = fmaxf(v, swz_xor16(v));
-    return fmaxf(v, xor32(v));
-}
-__device__ __forceinline__ float sum_rows(float v)
-{
-    v += swz_xor16(v);
-    return v + xor32(v);
-}
 
 constexpr int64_t TARGET_SKIP = -1, TARGET_BAD = -2;
 // the token's target, TARGET_SKIP for a token that does not count, TARGET_BAD
@@ -518,7 +546,7 @@ struct GatedEpi {
 struct DgatedEpi {
     const float* sc;
     const float* fac;
-    const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_factor_kernel)
+    const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_max_kernel)
     const void* dy;     // [tokens][rows]
     const uint32_t* amax;
     int dy_dt, tokens, tp, vkt;
@@ -655,53 +683,86 @@ __global__ void __launch_bounds__(PG_THREADS, MT == 8 ? 2 : 3) panel_gemm_kernel
     epi.template run<MT>(acc, tile0 + (bm * PG_WM + wm) * MT, (bn * PG_WN + wn) * PG_NT * 16, bz);
 }
 
-// ------------------------------------------------- upstream rows of a product
+// ------------------------------------------------------------ upstream rows
+struct DyMaxArgs {
+    const void* dy;
+    int dy_dt, tokens, vec;  // vec: rows a multiple of 8, 16-byte aligned
+    int64_t rows;
+    int head;     // bits left above the row's largest value
+    float* dfac;  // [tp]: 2^-e, which brings the row's largest into [2^(14 - head), 2^(15 - head))
+};
+// a wave a row
+__global__ void __launch_bounds__(256) dy_max_kernel(const DyMaxArgs a)
+{
+    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    float m = 0.0f;
+    if (t < a.tokens) {
+        const int64_t at = t * a.rows;
+        if (a.vec) {
+#pragma unroll 4
+            for (int64_t i = lane * 8; i < a.rows; i += 512) {
+                const Eight e = load8(a.dy, a.dy_dt, at + i);
+#pragma unroll
+                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t i = lane; i < a.rows; i += 64) m = fmaxf(m, fabsf(load_as_f32(a.dy, a.dy_dt, at + i)));
+        }
+    }
+    m = wave_max_all(m);
+    const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
+    if (lane == 0) a.dfac[t] = pow2(-e);
+}
+
 struct DyArgs {
     const void* dy;
-    int dy_dt, tokens;
+    int dy_dt, tokens, vec;
     int64_t rows, row0;  // row0: the piece's first
     const float* sc;     // turned order
     const uint32_t* amax;
-    half8_t* p;          // [tp / 16][vkt][64], or null: only the factors
-    int vkt, head;    // head: bits left above the row's largest value
-    float* dfac;      // [tp]: 2^-e; the panel holds dy 2^-e (scale 2^-es)
+    const float* dfac;
+    half8_t* p;          // [tp / 16][vkt][64]
+    int vkt;
 };
-
-// One workgroup a tile of 16 tokens: the rows' largest magnitudes, then the
-// panel of dy * scale in the order of the columns' panel.
-__global__ void __launch_bounds__(256) dy_rows_kernel(const DyArgs a)
+// The panel of dy * scale * 2^-e in the order of the columns' panel: 16 tokens
+// by 256 rows a workgroup, through LDS (an operand's 8 values lie 4 apart).
+constexpr int DY_ROWS = 256, DY_LD = DY_ROWS + 4;
+__global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 {
-    __shared__ float s_f[16];
-    const int tid = threadIdx.x, tile = blockIdx.x;
-    {
-        const int r = tid >> 4, t = tile * 16 + r;
-        float m = 0.0f;
-        if (t < a.tokens)
-            for (int64_t i = tid & 15; i < a.rows; i += 16) m = fmaxf(m, fabsf(load_as_f32(a.dy, a.dy_dt, t * a.rows + i)));
-        m = fmaxf(m, dpp_xor1(m));
-        m = fmaxf(m, dpp_xor2(m));
-        m = fmaxf(m, dpp_half_mirror(m));
-        m = fmaxf(m, dpp_row_mirror(m));
-        if ((tid & 15) == 0) {
-            const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
-            s_f[r] = pow2(-e);
-            a.dfac[t] = pow2(-e);
+    __shared__ __align__(16) float s_dy[16][DY_LD];
+    const int tid = threadIdx.x, tile = blockIdx.x, k0 = blockIdx.y * (DY_ROWS / 32);
+    const int64_t r0 = a.row0 + k0 * 32;
+    if (a.vec) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int f = tid + 256 * i, r = f / 32, c = f % 32 * 8, t = tile * 16 + r;
+            Eight e = {{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}};
+            if (t < a.tokens && r0 + c < a.rows) e = load8(a.dy, a.dy_dt, t * a.rows + r0 + c);
+            *(f32x4_t*)&s_dy[r][c] = f32x4_t{e.v[0], e.v[1], e.v[2], e.v[3]};
+            *(f32x4_t*)&s_dy[r][c + 4] = f32x4_t{e.v[4], e.v[5], e.v[6], e.v[7]};
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int t = tile * 16 + r;
+            s_dy[r][tid] = t < a.tokens && r0 + tid < a.rows ? load_as_f32(a.dy, a.dy_dt, t * a.rows + r0 + tid) : 0.0f;
         }
     }
-    if (!a.p) return;
     __syncthreads();
-    const int lane = tid & 63, c = lane >> 4, t = tile * 16 + (lane & 15);
-    const float f = s_f[lane & 15] * pow2(-scale_exponent(*a.amax));
-    for (int k = tid >> 6; k < a.vkt; k += 4) {
-        half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+    const int lane = tid & 63, c = lane >> 4, r = lane & 15;
+    const float f = a.dfac[tile * 16 + r] * pow2(-scale_exponent(*a.amax));
+#pragma unroll
+    for (int i = 0; i < DY_ROWS / 32 / 4; i++) {
+        const int k = (tid >> 6) + 4 * i;
+        if (k0 + k >= a.vkt) break;
+        half8_t h;
 #pragma unroll
         for (int m = 0; m < 8; m++) {
-            const int64_t row = a.row0 + (int64_t)k * 32 + 16 * (m >> 2) + 4 * (m & 3) + c;
-            if (t < a.tokens && row < a.rows)
-                h[m] = (_Float16)(load_as_f32(a.dy, a.dy_dt, t * a.rows + row) *
-                                  (a.sc[(row >> 4) * 16 + 4 * c + (m & 3)] * f));
+            const int col = k * 32 + 16 * (m >> 2) + 4 * (m & 3) + c;
+            h[m] = (_Float16)(s_dy[r][col] * (a.sc[r0 + k * 32 + 16 * (m >> 2) + 4 * c + (m & 3)] * f));
         }
-        a.p[((int64_t)tile * a.vkt + k) * 64 + lane] = h;
+        a.p[((int64_t)tile * a.vkt + k0 + k) * 64 + lane] = h;
     }
 }
 
@@ -716,10 +777,11 @@ struct LseArgs {
     float* loss;
     float* lse;
 };
-// 16 tokens a workgroup, 16 threads a token over the chunks
-__global__ void __launch_bounds__(256) lse_kernel(const LseArgs a)
+// 16 tokens a workgroup, 64 threads a token over the chunks
+constexpr int LSE_LANES = 64;
+__global__ void __launch_bounds__(16 * LSE_LANES) lse_kernel(const LseArgs a)
 {
-    __shared__ f32x2_t s_p[16][17];
+    __shared__ f32x2_t s_p[LSE_LANES][17];
     const int tid = threadIdx.x, tl = tid & 15, t = blockIdx.x * 16 + tl;
     float m = NEG_INF, s = 0.0f;
     auto add = [&](float om, float os) {
@@ -727,14 +789,24 @@ __global__ void __launch_bounds__(256) lse_kernel(const LseArgs a)
         s = s * __expf(m - b) + os * __expf(om - b);
         m = n;
     };
-    for (int64_t k = tid >> 4; k < a.chunks; k += 16) {
-        const f32x2_t p = a.part[k * a.tp + t];
-        add(p.x, p.y);
+    for (int64_t k = tid >> 4; k < a.chunks; k += 4 * LSE_LANES) {
+        f32x2_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int64_t c = k + i * LSE_LANES;
+            p[i] = a.part[min(c, a.chunks - 1) * a.tp + t];
+            if (c >= a.chunks) p[i] = f32x2_t{NEG_INF, 0.0f};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) add(p[i].x, p[i].y);
     }
-    s_p[tid >> 4][tl] = f32x2_t{m, s};
-    __syncthreads();
+    for (int w = LSE_LANES; w > 1; w /= 2) {
+        s_p[tid >> 4][tl] = f32x2_t{m, s};
+        __syncthreads();
+        if ((tid >> 4) < w / 2) add(s_p[(tid >> 4) + w / 2][tl].x, s_p[(tid >> 4) + w / 2][tl].y);
+        __syncthreads();
+    }
     if (tid >= 16 || t >= a.tokens) return;
-    for (int k = 1; k < 16; k++) add(s_p[k][tl].x, s_p[k][tl].y);
     const float lse = m + logf(s);
     const int64_t v = target_of(a.target, t, a.ignore, a.rows);
     a.lse[t] = lse;
@@ -784,15 +856,23 @@ struct DsArgs {
     float* ds[2];
     int add;
 };
+// 32 rows a workgroup, 8 threads a row over the chunks
 __global__ void __launch_bounds__(256) ds_kernel(const DsArgs a)
 {
-    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (p >= a.ld) return;
+    __shared__ float s_s[8][32];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t p = (int64_t)blockIdx.x * 32 + x;  // (a whole number of workgroups)
+    float s = 0.0f;
+#pragma unroll 8
+    for (int k = y; k < a.chunks; k += 8) s += a.part[k * a.ld + p];
+    s_s[y][x] = s;
+    __syncthreads();
+    if (y) return;
     int mat;
     const int64_t row = mat_row(a.m, p >> 4, turned((int)(p & 15)), mat);
     if (row >= a.m.rows) return;
-    float s = 0.0f;
-    for (int k = 0; k < a.chunks; k++) s += a.part[k * a.ld + p];
+#pragma unroll
+    for (int k = 1; k < 8; k++) s += s_s[k][x];
     float* d = a.ds[mat] + row;
     *d = (a.add ? *d : 0.0f) + s * a.rs;
 }
@@ -982,7 +1062,7 @@ int panel_launch(const PanelCall& c)
         const void* dy = c.dy ? (const char*)c.dy + t0 * c.rows * dt_size(c.dy_dt) : nullptr;
         const int64_t* target = c.target ? c.target + t0 : nullptr;
         if (first) {
-            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
+            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(tp / 16)), dim3(64 * PK_WAVES), 0, st,
                                PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
                                         c.x_scale ? c.x_scale + t0 : nullptr, xp, fac, t0 == 0 ? amax : nullptr});
             TRY(hipGetLastError());
@@ -995,9 +1075,10 @@ int panel_launch(const PanelCall& c)
                                PrepArgs{mats, c.rs, grad ? 1 : 0, ds_ld, sc, grad ? amax : nullptr});
             TRY(hipGetLastError());
         }
-        if (c.what == DGATED) {
-            hipLaunchKernelGGL(dy_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
-                               DyArgs{dy, c.dy_dt, tokens, c.rows, 0, sc, amax, nullptr, 0, 19, dfac});
+        const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;
+        if (c.what == DGATED || c.what == PRODUCT) {
+            hipLaunchKernelGGL(dy_max_kernel, dim3((unsigned)(tp / 4)), dim3(256), 0, st,
+                               DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, c.what == DGATED ? 19 : 0, dfac});
             TRY(hipGetLastError());
         }
         for (int64_t tile0 = 0; tile0 < p.tiles; tile0 += p.piece) {
@@ -1021,9 +1102,8 @@ int panel_launch(const PanelCall& c)
                 TRY((gemm<8>(g, ColsumEpi{fac, dy, c.dy_dt, tokens, c.rows, ds, ds_ld}, tile0, st)));
             if (!grad) continue;
             if (c.what == PRODUCT) {
-                // (a piece's rows of dy; their largest value is taken over all rows)
-                hipLaunchKernelGGL(dy_rows_kernel, dim3((unsigned)(tp / 16)), dim3(256), 0, st,
-                                   DyArgs{dy, c.dy_dt, tokens, c.rows, tile0 * 16, sc, amax, pp, vkt, 0, dfac});
+                hipLaunchKernelGGL(dy_panel_kernel, dim3((unsigned)(tp / 16), (unsigned)((vkt + 7) / 8)), dim3(256), 0, st,
+                                   DyArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, tile0 * 16, sc, amax, dfac, pp, vkt});
                 TRY(hipGetLastError());
             }
             const int slices = (int)std::min<int64_t>(p.slices, vkt);
@@ -1031,7 +1111,7 @@ int panel_launch(const PanelCall& c)
             TRY((gemm<8>(g2, GradEpi{acc, p.np, tp, tile0 != 0}, 0, st)));
         }
         if (c.what == STATS) {
-            hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((tokens + 15) / 16)), dim3(256), 0, st,
+            hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((tokens + 15) / 16)), dim3(16 * LSE_LANES), 0, st,
                                LseArgs{(const f32x2_t*)(ws + p.stats), p.tiles / 8, tokens, tp, target, c.rows, c.ignore,
                                        (const float*)(ws + p.at), c.loss + t0, c.lse_out + t0});
             TRY(hipGetLastError());
@@ -1043,7 +1123,7 @@ int panel_launch(const PanelCall& c)
                                   (char*)c.y + t0 * c.n * dt_size(c.y_dt), c.y_dt});
         TRY(hipGetLastError());
         if (ds) {
-            hipLaunchKernelGGL(ds_kernel, dim3((unsigned)((ds_ld + 255) / 256)), dim3(256), 0, st,
+            hipLaunchKernelGGL(ds_kernel, dim3((unsigned)(ds_ld / 32)), dim3(256), 0, st,
                                DsArgs{mats, ds, tp / (16 * PG_NT), ds_ld, c.rs, {c.ds[0], c.ds[1]}, t0 != 0});
             TRY(hipGetLastError());
         }
