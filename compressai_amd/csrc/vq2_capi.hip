@@ -1156,7 +1156,7 @@ static int check_norm(const char* who, const NormCall& c, int64_t rows, int64_t 
           who, (long long)hb, (long long)n);
     CHECK(((uintptr_t)c.x | (uintptr_t)c.residual | (uintptr_t)c.weight | (uintptr_t)c.y | (uintptr_t)c.h | (uintptr_t)c.dy |
            (uintptr_t)c.dh) % 16 == 0, "%s: a rotated call's arrays must be 16-byte aligned", who);
-    CHECK((uintptr_t)c.perm % 4 == 0, "%s: perm must be aligned to its elements", who);
+    CHECK((uintptr_t)c.perm % 16 == 0 && (uintptr_t)c.sign % 8 == 0, "%s: perm must be 16-byte aligned, sign 8-byte", who);
     return VQ2_OK;
 }
 

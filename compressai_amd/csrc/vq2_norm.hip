@@ -254,13 +254,6 @@ __device__ __forceinline__ void load_row(float (&v)[V][8], const void* p, int dt
     }
 }
 
-// two values rounded to bf16, one instruction
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b)
-{
-    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, bf2_t{(__bf16)a, (__bf16)b});
-}
-
 __device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (&v)[8])
 {
     if (dt == VQ2_DT_F32) {
@@ -331,20 +324,26 @@ __device__ __forceinline__ void load_tables(Tables<V>& t, const NormCall& a, int
 {
 #pragma unroll
     for (int c = 0; c < V; c++) {
+        const int i = (c * TPR + id) * 8, at = i < a.n ? i : 0;
+        u32x4 p[2];
+        u32x2 sg = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; k++) p[k / 4][k % 4] = at + k;
+        if (a.perm) {
+            p[0] = *(const u32x4*)(a.perm + at);
+            p[1] = *(const u32x4*)(a.perm + at + 4);
+        }
+        if (a.sign) sg = *(const u32x2*)(a.sign + at);
         t.nan[c] = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int i = (c * TPR + id) * 8 + k;
-            uint32_t p = 0, neg = 0;
-            if (i < a.n) {
-                p = a.perm ? (uint32_t)a.perm[i] : (uint32_t)i;
-                if (p >= (uint32_t)a.n) {
-                    p = 0;
-                    t.nan[c] = __builtin_nanf("");
-                }
-                neg = a.sign && a.sign[i] < 0 ? 0x8000u : 0u;
+            uint32_t q = p[k / 4][k % 4];
+            if (q >= (uint32_t)a.n) {
+                q = 0;
+                t.nan[c] = __builtin_nanf("");
             }
-            t.w[c][k >> 1] = (k & 1 ? t.w[c][k >> 1] : 0) | (p * 4 | neg) << (16 * (k & 1));
+            const uint32_t e = q * 4 | (sg[k / 4] >> (8 * (k % 4) + 7) & 1) << 15;
+            t.w[c][k >> 1] = k & 1 ? t.w[c][k >> 1] | e << 16 : e;
         }
     }
 }
@@ -369,12 +368,16 @@ __global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t r
     __shared__ float s_red[4];
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
-    // the next row's values are on their way while this one is worked on
+    // The next row's values are on their way while this one is worked on.  The
+    // loads are unconditional (the last row again, x for a residual that is
+    // not there): behind a branch the compiler waits for all of them at the
+    // next use of any (norm_grad_kernel, 8192 rows of 6144: 200 us so).
+    const void* res = a.residual ? a.residual : a.x;
     Raw<DT, V, VEC> rx, rr;
     auto fetch = [&](int64_t r0) {
         const int64_t at = min(r0 + rw, a.rows - 1);
         load_raw<DT, V, TPR, VEC>(rx, a.x, at, a.n, id);
-        if (a.residual) load_raw<DT, V, TPR, VEC>(rr, a.residual, at, a.n, id);
+        load_raw<DT, V, TPR, VEC>(rr, res, at, a.n, id);
     };
     fetch((int64_t)blockIdx.x * RW);
     float w[V][8];
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t r
 #pragma unroll
                 for (int k = 0; k < 8; k++) h[c][k] += e[c][k];
         }
-        if (r0 + row_step < a.rows) fetch(r0 + row_step);
+        fetch(r0 + row_step);
         if (a.h && live) store_row<V, TPR, VEC>(h, a.h, DT, row, a.n, id, 0.0f);
         float sum[1] = {0.0f};
 #pragma unroll
@@ -459,10 +462,12 @@ __global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int6
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
     const bool same = a.y_dt == DT;  // dy of h's type
+    const void* gsrc = same ? a.dy : a.x;
+    const void* esrc = a.dh ? a.dh : a.x;
     Raw<DT, V, VEC> rh, rg;
     auto fetch = [&](int64_t r0) {
         const int64_t at = min(r0 + rw, a.rows - 1);
-        if (same) load_raw<DT, V, TPR, VEC>(rg, a.dy, at, a.n, id);
+        load_raw<DT, V, TPR, VEC>(rg, gsrc, at, a.n, id);
         load_raw<DT, V, TPR, VEC>(rh, a.x, at, a.n, id);
     };
     fetch((int64_t)blockIdx.x * RW);
@@ -485,8 +490,8 @@ __global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int6
         else load_row<V, TPR, VEC>(g, a.dy, a.y_dt, at, a.n, id);
         numbers(h, rh);
         Raw<DT, V, VEC> re;
-        if (a.dh) load_raw<DT, V, TPR, VEC>(re, a.dh, at, a.n, id);
-        if (r0 + row_step < a.rows) fetch(r0 + row_step);
+        load_raw<DT, V, TPR, VEC>(re, esrc, at, a.n, id);
+        fetch(r0 + row_step);
         if constexpr (ROT) {
             hadamard<V, TPR>(g, a.hb, id, s);
             __syncthreads();
@@ -521,7 +526,7 @@ __global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int6
         row_reduce<TPR>(sum, s_red, add_op);
         const float r = 1.0f / sqrtf(sum[0] / (float)a.n + a.eps), b = r * r * r * (sum[1] / (float)a.n);
         float e[V][8];
-        if (a.dh) numbers(e, re);
+        numbers(e, re);
 #pragma unroll
         for (int c = 0; c < V; c++)
 #pragma unroll

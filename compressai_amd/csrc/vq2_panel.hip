@@ -350,14 +350,44 @@ __device__ __forceinline__ int64_t target_of(const int64_t* t, int64_t i, int64_
     return v == ignore ? TARGET_SKIP : v < 0 || v >= rows ? TARGET_BAD : v;
 }
 
+// row scale * rs of row r of matrix `mat`; 0 past the last row
+__device__ __forceinline__ float row_scale(const MatArgs& m, float rs, int mat, int64_t r)
+{
+    return r < m.rows ? load_as_f32(m.m[mat].scale, m.s_dt, r) * rs : 0.0f;
+}
+
 struct StatsEpi {
     const float* sc;
     const float* fac;
     const int64_t* target;
     int64_t rows, ignore;
     int tokens, tp;
-    f32x2_t* part;  // [waves of rows][tp]: largest logit and sum of exp(l - largest)
+    f32x2_t* part;  // [parts of rows][tp]: largest logit and sum of exp(l - largest)
     float* at;      // [tp]: the target's logit
+    // two tiles' products of a token (few_kernel): a part of 32 rows
+    __device__ __forceinline__ void few(const MatArgs& m, float rs, f32x4_t a, f32x4_t b, int64_t pair, int t) const
+    {
+        const int q = (threadIdx.x & 63) >> 4;
+        const int64_t r0 = pair * 32 + q * 4;
+        float z[8], top = NEG_INF;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int64_t r = r0 + (k >> 2) * 16 + (k & 3);
+            z[k] = r < m.rows ? (k < 4 ? a[k & 3] : b[k & 3]) * row_scale(m, rs, 0, r) : NEG_INF;
+            top = fmaxf(top, z[k]);
+        }
+        top = max_rows(top);
+        const float base = top == NEG_INF ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum += __expf(z[k] - base);
+        sum = sum_rows(sum);
+        if (q == 0) part[pair * tp + t] = f32x2_t{top, sum};
+        const int64_t rel = (t < tokens ? target_of(target, t, ignore, rows) : TARGET_SKIP) - r0;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (rel == (k >> 2) * 16 + (k & 3)) at[t] = z[k];
+    }
     template <int MT>
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
     {
@@ -498,6 +528,37 @@ struct GatedEpi {
     int64_t rows;
     int vec;  // rows a multiple of 4, y aligned: 4 values a store
     int act;
+    __device__ __forceinline__ void store(int t, int64_t r0, const float (&o)[4]) const
+    {
+        const int64_t at = (int64_t)t * rows + r0;
+        if (!vec) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (r0 + e < rows) store_from_f32(y, y_dt, at + e, o[e]);
+        } else if (y_dt == VQ2_DT_F32) {
+            *(f32x4_t*)((float*)y + at) = f32x4_t{o[0], o[1], o[2], o[3]};
+        } else if (y_dt == VQ2_DT_F16) {
+            *(half4_t*)((uint16_t*)y + at) = half4_t{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+        } else {
+            *(u32x2*)((uint16_t*)y + at) = u32x2{bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3])};
+        }
+    }
+    __device__ __forceinline__ void few(const MatArgs& m, float rs, f32x4_t g, f32x4_t u, int64_t pair, int t) const
+    {
+        const int q = (threadIdx.x & 63) >> 4;
+        const int64_t r0 = pair * 16 + q * 4;
+        if (t >= tokens || r0 >= rows) return;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float v = g[e] * row_scale(m, rs, 0, r0 + e);
+            float f, df;
+            if (act == VQ2_ACT_SILU) gate_act<VQ2_ACT_SILU>(v, f, df);
+            else gate_act<VQ2_ACT_GELU_TANH>(v, f, df);
+            o[e] = f * (u[e] * row_scale(m, rs, 1, r0 + e));
+        }
+        store(t, r0, o);
+    }
     template <int ACT, int MT>
     __device__ __forceinline__ void run_act(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok)
     {
@@ -519,19 +580,7 @@ struct GatedEpi {
                     gate_act<ACT>(acc[i][j][e] * x * sg[e], f, df);
                     o[e] = f * (acc[i + 1][j][e] * x * su[e]);
                 }
-                const int64_t at = (int64_t)t * rows + r0;
-                if (!vec) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (r0 + e < rows) store_from_f32(y, y_dt, at + e, o[e]);
-                } else if (y_dt == VQ2_DT_F32) {
-                    *(f32x4_t*)((float*)y + at) = f32x4_t{o[0], o[1], o[2], o[3]};
-                } else if (y_dt == VQ2_DT_F16) {
-                    *(half4_t*)((uint16_t*)y + at) = half4_t{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
-                } else {
-                    *(u32x2*)((uint16_t*)y + at) = u32x2{f32_to_bf16_bits(o[0]) | (uint32_t)f32_to_bf16_bits(o[1]) << 16,
-                                                         f32_to_bf16_bits(o[2]) | (uint32_t)f32_to_bf16_bits(o[3]) << 16};
-                }
+                store(t, r0, o);
             }
         }
     }
@@ -766,6 +815,189 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
     }
 }
 
+// ------------------------------------------------------------- few tokens
+// Up to 128 tokens: every centroid is gathered once, straight into the
+// operand it is (lane (row, q): group q of a k tile), and nothing is written in
+// between.  The gathers bound it: 240 G a second over the device, whatever
+// their size (a request of a line each).  A wave takes two tiles of 16 rows
+// (for the block: gate and up).  Up to 64 tokens the 4 waves of a workgroup
+// share the k tiles of one pair and meet in LDS, so that small matrices fill the device;
+// above, each has a pair of its own and they share the tokens' lines.
+//
+// k tiles in groups of 8: lane q takes the groups 8 q + j (j = tile of the 8)
+// of 32, so its 8 codes are one load, and the tokens' operand is read from
+// there, too.  Up to 16 tokens are read as they are (no packing launch): a wave
+// brings its share of a token's row to fp16 under a power of two of its own.
+struct FewArgs {
+    MatArgs m;
+    int64_t pairs;
+    const half8_t* xp;  // packed tokens (TT > 1)
+    const float* fac;
+    const void* x;      // TT == 1
+    int x_dt;
+    const float* x_scale;
+    int tokens, n;
+    float rs;
+};
+
+// a gathered centroid in fp16
+template <int CBT>
+__device__ __forceinline__ half8_t centroid_f16(half8_t h)
+{
+    if constexpr (CBT == VQ2_DT_BF16) {
+        const u32x4 u = __builtin_bit_cast(u32x4, h);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            h[2 * k] = (_Float16)__uint_as_float(u[k] << 16);
+            h[2 * k + 1] = (_Float16)__uint_as_float(u[k] & 0xFFFF0000u);
+        }
+    }
+    return h;
+}
+
+template <int CBT, int S2, int TT, int KW, class Epi>
+__global__ void __launch_bounds__(256, TT == 8 ? 2 : 3) few_kernel(const FewArgs a, Epi epi)
+{
+    static_assert(KW == 4 || KW == 1, "");
+    constexpr int JU = S2 == VQ2_S2_NONE && TT <= 4 ? 8 : 4;  // k tiles whose centroids are on their way together
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, nl = lane & 15;
+    const int64_t pair = KW == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    if (KW == 1 && pair >= a.pairs) return;
+    const int ng = a.m.ng, kt = ng / 4, sups = (ng + 31) / 32, part = KW == 4 ? wave : 0;
+    const int s0 = sups * part / KW, s1 = sups * (part + 1) / KW;
+    const int16_t* p0[2];
+    const char* p1[2];
+    constexpr int B1 = S2 == VQ2_S2_U8 ? 1 : 2;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        int mat;
+        const int64_t row = mat_row(a.m, 2 * pair + i, nl, mat), off = (row < a.m.rows ? row : 0) * ng;
+        p0[i] = a.m.m[mat].i0 + off;
+        p1[i] = S2 == VQ2_S2_NONE ? nullptr : (const char*)a.m.m[mat].i1 + off * B1;
+    }
+    struct Codes {
+        u32x4 a[2], b[S2 == VQ2_S2_NONE ? 1 : 2];
+    };
+    auto load_codes = [&](int sup, Codes& c) {
+        const int g = min(sup, sups - 1) * 32 + q * 8, at = g < ng ? g : 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            c.a[i] = *(const u32x4*)(p0[i] + at);
+            if constexpr (S2 == VQ2_S2_U16) c.b[i] = *(const u32x4*)(p1[i] + at * 2);
+            if constexpr (S2 == VQ2_S2_U8) {
+                const u32x2 u = *(const u32x2*)(p1[i] + at);
+                c.b[i].x = u.x;
+                c.b[i].y = u.y;
+            }
+        }
+    };
+    auto code = [](const u32x4& w, int j) { return w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu; };
+    Codes cur, next;
+    load_codes(s0, cur);
+
+    // the tokens of a wave that reads them itself: their largest values first
+    float up = 1.0f, down = 1.0f;  // 2^e, 2^-e of token nl
+    const bool own = TT == 1;
+    if (own && a.x_dt <= VQ2_DT_BF16) {
+        float m = 0.0f;
+        if (nl < a.tokens)
+            for (int s = s0; s < s1; s++)
+                if (s * 32 + q * 8 < ng)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const Eight e = load8(a.x, a.x_dt, (int64_t)nl * a.n + (s * 32 + q * 8 + j) * 8);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
+                    }
+        m = max_rows(m);
+        const int e = m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
+        up = pow2(e);
+        down = pow2(-e);
+    }
+
+    f32x4_t acc[2][TT];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < TT; j++) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int s = s0; s < s1; s++) {
+        const bool ok = s * 32 + q * 8 < ng;
+        load_codes(s + 1, next);
+#pragma unroll
+        for (int j0 = 0; j0 < 8; j0 += JU) {
+            half8_t w0[2][JU], w1[2][S2 == VQ2_S2_NONE ? 1 : JU];
+#pragma unroll
+            for (int u = 0; u < JU; u++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int j = j0 + u;
+                    w0[i][u] = ((const half8_t*)a.m.cb0)[code(cur.a[i], j)];
+                    if constexpr (S2 == VQ2_S2_U16) w1[i][u] = ((const half8_t*)a.m.cb1)[code(cur.b[i], j)];
+                    if constexpr (S2 == VQ2_S2_U8) w1[i][u] = ((const half8_t*)a.m.cb1)[cur.b[i][j >> 2] >> (8 * (j & 3)) & 0xFFu];
+                }
+#pragma unroll
+            for (int u = 0; u < JU; u++) {
+                const int g = ok ? s * 32 + q * 8 + j0 + u : 0;
+                half8_t b[TT];
+                if constexpr (TT == 1) {
+                    b[0] = zero;
+                    if (nl < a.tokens) {
+                        const Eight e = load8(a.x, a.x_dt, (int64_t)nl * a.n + g * 8);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) b[0][k] = (_Float16)(e.v[k] * down);
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < TT; t++) b[t] = a.xp[((int64_t)t * kt + (g >> 2)) * 64 + (g & 3) * 16 + nl];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const half8_t w = ok ? centroid_f16<CBT>(w0[i][u]) : zero;
+#pragma unroll
+                    for (int t = 0; t < TT; t++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, b[t], acc[i][t], 0, 0, 0);
+                    if constexpr (S2 != VQ2_S2_NONE) {
+                        const half8_t v = ok ? centroid_f16<CBT>(w1[i][u]) : zero;
+#pragma unroll
+                        for (int t = 0; t < TT; t++)
+                            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, b[t], acc[i][t], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        cur = next;
+    }
+    if constexpr (KW == 4) {
+        __shared__ f32x4_t s_acc[4][2 * TT][64];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int t = 0; t < TT; t++) s_acc[wave][i * TT + t][lane] = acc[i][t] * up;
+        __syncthreads();
+        for (int t = wave; t < TT; t += 4) {
+            if (t * 16 >= a.tokens) break;
+            f32x4_t o[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                o[i] = s_acc[0][i * TT + t][lane];
+#pragma unroll
+                for (int k = 1; k < 4; k++) o[i] += s_acc[k][i * TT + t][lane];
+            }
+            const int tok = t * 16 + nl;
+            const float f = own ? (a.x_scale && tok < a.tokens ? a.x_scale[tok] : 1.0f) : a.fac[tok];
+            epi.few(a.m, a.rs, o[0] * f, o[1] * f, pair, tok);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < TT; t++) {
+            if (t * 16 >= a.tokens) break;
+            const int tok = t * 16 + nl;
+            const float f = a.fac[tok];
+            epi.few(a.m, a.rs, acc[0][t] * f, acc[1][t] * f, pair, tok);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- last steps
 struct LseArgs {
     const f32x2_t* part;
@@ -902,11 +1134,15 @@ constexpr int64_t PANEL_TOKENS = 8192;
 constexpr int64_t PIECE_BYTES = 128 << 20;
 constexpr int64_t PIECE_MAX_ROWS = 16384, PIECE_MIN_ROWS = 4096;
 
+// up to here few_kernel; 128 tokens of a 151936 x 2048 head: @@FEW@@
+constexpr int FEW_TOKENS = 128;
+
 struct Plan {
     int64_t chunk;       // tokens of a chunk (the last may be shorter)
     int64_t tp;          // of them, padded
     int64_t tiles;       // 16-row tiles of all matrices, padded to whole workgroups
     int64_t piece;       // tiles of a piece
+    bool few;            // few_kernel
     int parts, tparts, kt;  // parts of a weight in the rows' panel, and the columns'
     int64_t np;          // columns, padded
     int slices;
@@ -923,6 +1159,8 @@ Plan plan_of(const PanelCall& c)
     p.tp = up(p.chunk, PG_N);
     p.tiles = up((c.rows + 15) / 16 * c.nmat, pg_m(8) / 16);
     p.kt = (int)(c.n / 32);
+    // (codes are loaded 8 at a time; fp32 centroids would take two products each)
+    p.few = !grad && c.tokens <= FEW_TOKENS && c.cb_dt != VQ2_DT_F32;
     const bool exact = c.cb_dt != VQ2_DT_F32 && c.s2 == VQ2_S2_NONE;
     const bool fine = c.y_dt != VQ2_DT_BF16;
     const bool wide = c.what == STATS || c.what == DLOGIT || c.ds[0] != nullptr || fine;
@@ -952,7 +1190,7 @@ Plan plan_of(const PanelCall& c)
         if (c.what != DLOGIT) p.dfac = b.take(p.tp * 4);
     }
     if (c.what == STATS) {
-        p.stats = b.take(p.tiles / 4 * p.tp * 8);
+        p.stats = b.take(p.tiles / 2 * p.tp * 8);  // parts of 32 rows (few tokens) or 128
         p.at = b.take(p.tp * 4);
     }
     p.total = b.at;
@@ -1017,6 +1255,30 @@ hipError_t dequant(const DequantArgs& a, int cb_dt, int s2, int wp, int tp, int6
     return dequant_s2<VQ2_DT_F32>(a, s2, wp, tp, tiles, st);
 }
 
+template <int CBT, int S2, class Epi>
+hipError_t few_typed(const FewArgs& a, const Epi& e, hipStream_t st)
+{
+    const dim3 one((unsigned)a.pairs), four((unsigned)((a.pairs + 3) / 4)), block(256);
+    if (a.tokens <= 16) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, Epi>), one, block, 0, st, a, e);
+    else if (a.tokens <= 32) hipLaunchKernelGGL((few_kernel<CBT, S2, 2, 4, Epi>), one, block, 0, st, a, e);
+    else if (a.tokens <= 64) hipLaunchKernelGGL((few_kernel<CBT, S2, 4, 4, Epi>), one, block, 0, st, a, e);
+    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, Epi>), four, block, 0, st, a, e);
+    return hipGetLastError();
+}
+
+template <class Epi>
+hipError_t few(const FewArgs& a, const Epi& e, int cb_dt, int s2, hipStream_t st)
+{
+    if (cb_dt == VQ2_DT_F16) {
+        if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_F16, VQ2_S2_NONE>(a, e, st);
+        if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_F16, VQ2_S2_U8>(a, e, st);
+        return few_typed<VQ2_DT_F16, VQ2_S2_U16>(a, e, st);
+    }
+    if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_BF16, VQ2_S2_NONE>(a, e, st);
+    if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_BF16, VQ2_S2_U8>(a, e, st);
+    return few_typed<VQ2_DT_BF16, VQ2_S2_U16>(a, e, st);
+}
+
 }  // namespace
 
 size_t panel_workspace_bytes(const PanelCall& c) { return c.tokens ? plan_of(c).total : 0; }
@@ -1041,6 +1303,9 @@ int panel_launch(const PanelCall& c)
         return VQ2_OK;
     }
     const Plan p = plan_of(c);
+    bool few_call = p.few;
+    for (int k = 0; k < c.nmat; k++)
+        few_call = few_call && (uintptr_t)c.mat[k].i0 % 16 == 0 && (uintptr_t)c.mat[k].i1 % 16 == 0;
     char* ws = (char*)c.workspace;
     const bool grad = c.what == DLOGIT || c.what == DGATED || c.what == PRODUCT;
     const bool first = c.what != PRODUCT || c.ds[0];  // the product of weights and tokens
@@ -1061,7 +1326,9 @@ int panel_launch(const PanelCall& c)
         const int64_t ds_ld = p.tiles * 16;
         const void* dy = c.dy ? (const char*)c.dy + t0 * c.rows * dt_size(c.dy_dt) : nullptr;
         const int64_t* target = c.target ? c.target + t0 : nullptr;
-        if (first) {
+        if (few_call && tokens <= 16) {
+            // (few_kernel reads the rows itself)
+        } else if (first) {
             hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(tp / 16)), dim3(64 * PK_WAVES), 0, st,
                                PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
                                         c.x_scale ? c.x_scale + t0 : nullptr, xp, fac, t0 == 0 ? amax : nullptr});
@@ -1069,6 +1336,25 @@ int panel_launch(const PanelCall& c)
         } else if (t0 == 0) {
             hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(256), 0, st, (float*)amax, (int64_t)1);
             TRY(hipGetLastError());
+        }
+        auto lse_launch = [&](int64_t chunks) {
+            hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((tokens + 15) / 16)), dim3(16 * LSE_LANES), 0, st,
+                               LseArgs{(const f32x2_t*)(ws + p.stats), chunks, tokens, tp, target, c.rows, c.ignore,
+                                       (const float*)(ws + p.at), c.loss + t0, c.lse_out + t0});
+            return hipGetLastError();
+        };
+        const StatsEpi stats{sc, fac, target, c.rows, c.ignore, tokens, tp, (f32x2_t*)(ws + p.stats), (float*)(ws + p.at)};
+        const GatedEpi gated{sc, fac, c.y ? (char*)c.y + t0 * c.rows * dt_size(c.y_dt) : nullptr, c.y_dt, tokens, c.rows,
+                             c.rows % 4 == 0 && (uintptr_t)c.y % 16 == 0, c.act};
+        if (few_call) {
+            const FewArgs f{mats, ((c.rows + 15) / 16 * c.nmat + 1) / 2, xp, fac, c.x, c.x_dt, c.x_scale, tokens, (int)c.n, c.rs};
+            if (c.what == GATED) {
+                TRY(few(f, gated, c.cb_dt, c.s2, st));
+            } else {
+                TRY(few(f, stats, c.cb_dt, c.s2, st));
+                TRY(lse_launch(f.pairs));
+            }
+            continue;
         }
         if (t0 == 0) {
             hipLaunchKernelGGL(prep_kernel, dim3((unsigned)((ds_ld + 255) / 256)), dim3(256), 0, st,
@@ -1087,11 +1373,9 @@ int panel_launch(const PanelCall& c)
             TRY(dequant(DequantArgs{mats, tile0, w, wt, vkt}, c.cb_dt, c.s2, w ? p.parts : 0, wt ? p.tparts : 0, tiles, st));
             const PanelGemmArgs g{w, xp, p.parts * p.kt, p.kt, (int)(tiles * 16 / pg_m(8)), tp / PG_N, 1};
             if (c.what == STATS)
-                TRY((gemm<8>(g, StatsEpi{sc, fac, target, c.rows, c.ignore, tokens, tp, (f32x2_t*)(ws + p.stats),
-                                         (float*)(ws + p.at)}, tile0, st)));
+                TRY((gemm<8>(g, stats, tile0, st)));
             else if (c.what == GATED)
-                TRY((gemm<8>(g, GatedEpi{sc, fac, (char*)c.y + t0 * c.rows * dt_size(c.y_dt), c.y_dt, tokens, c.rows,
-                                         c.rows % 4 == 0 && (uintptr_t)c.y % 16 == 0, c.act}, tile0, st)));
+                TRY((gemm<8>(g, gated, tile0, st)));
             else if (c.what == DLOGIT)
                 TRY((gemm<8>(g, DlogitEpi{sc, fac, c.lse + t0, c.dloss + t0, target, amax, c.rows, c.ignore, tile0, tokens, tp, vkt,
                                           pp, ds, ds_ld}, tile0, st)));
@@ -1110,12 +1394,7 @@ int panel_launch(const PanelCall& c)
             const PanelGemmArgs g2{wt, pp, p.tparts * vkt, vkt, (int)(p.np / pg_m(8)), tp / PG_N, slices};
             TRY((gemm<8>(g2, GradEpi{acc, p.np, tp, tile0 != 0}, 0, st)));
         }
-        if (c.what == STATS) {
-            hipLaunchKernelGGL(lse_kernel, dim3((unsigned)((tokens + 15) / 16)), dim3(16 * LSE_LANES), 0, st,
-                               LseArgs{(const f32x2_t*)(ws + p.stats), p.tiles / 8, tokens, tp, target, c.rows, c.ignore,
-                                       (const float*)(ws + p.at), c.loss + t0, c.lse_out + t0});
-            TRY(hipGetLastError());
-        }
+        if (c.what == STATS) TRY(lse_launch(p.tiles / 8));
         if (!grad) continue;
         hipLaunchKernelGGL(dx_kernel, dim3((unsigned)((c.n + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st,
                            DxArgs{acc, p.slices, tp, (int)c.n, p.np, amax, c.what == DLOGIT ? nullptr : dfac,

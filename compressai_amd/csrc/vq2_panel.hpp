@@ -61,6 +61,13 @@ __device__ __forceinline__ Eight load8(const void* p, int dt, int64_t i)
     return r;
 }
 
+// two values rounded to bf16, one instruction
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b)
+{
+    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf2_t{(__bf16)a, (__bf16)b});
+}
+
 // 1 KiB of a panel straight into LDS (no registers); l is wave-uniform, the
 // lanes' 16 bytes land in order behind it.
 __device__ __forceinline__ void panel_to_lds(const half8_t* g, half8_t* l)

@@ -743,7 +743,7 @@ int vq2_unpack_fixed(const uint8_t* buf, int64_t nbytes, int bits, int64_t n, in
  *     each: y_scale = largest magnitude / 127 (/ 448), y = u / y_scale to the
  *     nearest; a row with a NaN or an infinity has that for its scale
  * n up to VQ2_NORM_MAX_N; rotated: n a multiple of 64, hb a power of two from
- * 64 on that divides n, and 16-byte aligned rows and tables' entries in order.
+ * 64 on that divides n, rows and perm 16-byte and sign 8-byte aligned.
  * The reference's counterpart is its residual + zero-centred norm kernel
  * (vq2/kernels.py:375-395). */
 #define VQ2_NORM_MAX_N 8192
