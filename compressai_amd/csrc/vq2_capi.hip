@@ -1355,8 +1355,8 @@ int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_
     CHECK(grad_dt(dx_dt), "vq2_head_loss_backward: dx must hold fp16 or bf16 values");
     if (tokens) {
         CHECK(targets && lse && dloss && dx, "vq2_head_loss_backward: NULL pointer argument");
-        CHECK((uintptr_t)targets % 8 == 0 && ((uintptr_t)lse | (uintptr_t)dloss) % 4 == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
-              "vq2_head_loss_backward: arrays must be aligned to their elements");
+        CHECK((uintptr_t)targets % 8 == 0 && ((uintptr_t)lse | (uintptr_t)dloss) % 4 == 0 && (uintptr_t)dx % 16 == 0,
+              "vq2_head_loss_backward: arrays must be aligned to their elements, dx to 16 bytes");
     }
     return panel_launch(c);
 }
@@ -1437,8 +1437,8 @@ int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, 
     r = check_panel(c, true, false);
     if (r) return r;
     if (tokens)
-        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
-              "vq2_gated_rows_backward: dy or dx is NULL or not aligned to its elements");
+        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % 16 == 0,
+              "vq2_gated_rows_backward: dy or dx is NULL or not aligned (dy to its elements, dx to 16 bytes)");
     return panel_launch(c);
 }
 
@@ -1470,8 +1470,8 @@ int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_
     CHECK(dt_ok(dy_dt), "vq2_gemm_backward: bad dy dtype");
     CHECK(grad_dt(dx_dt), "vq2_gemm_backward: dx must hold fp16 or bf16 values");
     if (tokens)
-        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % dt_size(dx_dt) == 0,
-              "vq2_gemm_backward: dy or dx is NULL or not aligned to its elements");
+        CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % 16 == 0,
+              "vq2_gemm_backward: dy or dx is NULL or not aligned (dy to its elements, dx to 16 bytes)");
     return panel_launch(c);
 }
 

@@ -13,6 +13,7 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "vq2_amd.h"
 
@@ -493,6 +494,176 @@ py::object sample(const at::Tensor& logits, const at::Tensor& u, py::handle temp
     return py::make_tuple(idx, logprob);
 }
 
+// A call's workspace, 256-byte aligned as the allocator's blocks are.
+at::Tensor workspace_of(const at::Tensor& like, size_t bytes)
+{
+    return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+bool on_current_device(const at::Tensor& t)
+{
+    static const c10::impl::VirtualGuardImpl guard(at::kCUDA);
+    return guard.getDevice() == t.device();
+}
+
+int dt8_code(at::ScalarType t) { return t == at::kChar ? VQ2_DT_I8 : t == at::kFloat8_e4m3fn ? VQ2_DT_E4M3 : -1; }
+
+// the rotation of the norm's entries: tables, block and scale; ok as in Python
+struct NormRotation {
+    int64_t hb;
+    float scale;
+    NormRotation(Check& c, const OptTensor& perm, const OptTensor& sign, int64_t n, std::optional<int64_t> block,
+                 std::optional<double> rht_scale)
+        : hb(block.value_or(0))
+    {
+        c.table(perm, at::kInt, n);
+        c.table(sign, at::kChar, n);
+        c.need(hb != 0 || (!perm && !sign));
+        scale = rht_scale ? (float)*rht_scale : hb > 0 ? (float)(1.0 / std::sqrt((double)hb)) : 1.0f;
+    }
+};
+
+// vq_add_rms_norm without a given h
+py::object add_rms_norm(const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool zero_centred,
+                        const OptTensor& perm, const OptTensor& sign, std::optional<int64_t> block,
+                        std::optional<double> rht_scale, std::optional<at::ScalarType> out_dtype)
+{
+    Check c;
+    c.dense(x);
+    c.need(x.dim() >= 1 && x.numel() > 0 && dt_code(x.scalar_type()) >= 0);
+    if (!c.ok || !on_current_device(x)) return py::none();
+    const int64_t n = x.size(-1), rows = x.numel() / n;
+    c.scales(weight, n);
+    if (residual) {
+        c.dense(*residual);
+        c.need(residual->scalar_type() == x.scalar_type() && residual->sizes() == x.sizes());
+    }
+    const NormRotation rot(c, perm, sign, n, block, rht_scale);
+    const at::ScalarType odt = out_dtype.value_or(x.scalar_type());
+    const int d8 = dt8_code(odt), ydt = d8 >= 0 ? d8 : dt_code(odt);
+    c.need(ydt >= 0);
+    if (!c.ok) return py::none();
+    at::Tensor y = at::empty(x.sizes(), x.options().dtype(odt));
+    at::Tensor h = residual ? at::empty_like(x) : x;
+    at::Tensor s;
+    if (d8 >= 0) s = at::empty({rows}, x.options().dtype(at::kFloat));
+    void* const st = stream_of(*c.dev);
+    check_status(unlocked([&] {
+                     return vq2_add_rms_norm(ptr(x), dt_code(x.scalar_type()), ptr(residual), rows, n, ptr(weight),
+                                             dt_code(weight.scalar_type()), zero_centred, (float)eps, (const int32_t*)ptr(perm),
+                                             (const int8_t*)ptr(sign), rot.hb, rot.scale, y.data_ptr(), ydt,
+                                             d8 >= 0 ? s.data_ptr<float>() : nullptr, residual ? h.data_ptr() : nullptr, st);
+                 }),
+                 "vq2_add_rms_norm");
+    if (d8 < 0) return py::make_tuple(y, h, py::none());
+    return py::make_tuple(y, h, s);
+}
+
+// Token rows of a panel entry: [.., n] in 16 bits, or in 8 with their scales
+int panel_rows(Check& c, const at::Tensor& x, const OptTensor& x_scale, int64_t n)
+{
+    c.dense(x);
+    c.need(x.dim() >= 1 && x.numel() > 0 && x.size(-1) == n);
+    const int d8 = dt8_code(x.scalar_type());
+    c.need(d8 >= 0 || x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16);
+    c.need((d8 >= 0) == x_scale.has_value());
+    if (c.ok) c.table(x_scale, at::kFloat, x.numel() / n);
+    return d8 >= 0 ? d8 : dt_code(x.scalar_type());
+}
+
+// A matrix's planes and scales; the stage-2 kind, or -1 for what Python looks at
+int panel_mat(Check& c, const at::Tensor& i0, const OptTensor& i1, const at::Tensor& scale, const at::Tensor& cb0,
+              const OptTensor& cb1, int64_t rows, int64_t n)
+{
+    c.dense(i0);
+    c.need(n >= 8 && n % 8 == 0 && i0.scalar_type() == at::kShort && i0.numel() == rows * (n / 8));
+    c.scales(scale, rows);
+    c.book(cb0, CB_ROWS);
+    c.need(dt_code(cb0.scalar_type()) >= 0);
+    if (!i1) {
+        if (cb1) c.on_gpu(*cb1);
+        return VQ2_S2_NONE;
+    }
+    if (!cb1) return -1;
+    c.dense(*i1);
+    const bool u8 = i1->scalar_type() == at::kByte;
+    c.need((u8 || i1->scalar_type() == at::kShort) && i1->numel() == i0.numel());
+    c.book(*cb1, u8 ? 256 : CB_ROWS);
+    c.need(cb1->scalar_type() == cb0.scalar_type());
+    return u8 ? VQ2_S2_U8 : VQ2_S2_U16;
+}
+
+// vq_head_loss
+py::object head_loss(const at::Tensor& x, const at::Tensor& targets, const at::Tensor& i0, const OptTensor& i1,
+                     const at::Tensor& cb0, const OptTensor& cb1, const at::Tensor& scale, int64_t out, int64_t n, double rs,
+                     const OptTensor& x_scale, int64_t ignore_index)
+{
+    Check c;
+    const int xdt = panel_rows(c, x, x_scale, n);
+    if (!c.ok || !on_current_device(x)) return py::none();
+    const int64_t T = x.numel() / n;
+    c.dense(targets);
+    c.need(targets.scalar_type() == at::kLong && targets.numel() == T);
+    const int s2 = panel_mat(c, i0, i1, scale, cb0, cb1, out, n);
+    if (!c.ok || s2 < 0) return py::none();
+    at::Tensor loss = at::empty({T}, x.options().dtype(at::kFloat)), lse = at::empty({T}, x.options().dtype(at::kFloat));
+    const int cdt = dt_code(cb0.scalar_type());
+    const size_t bytes = vq2_head_loss_workspace(T, out, n, s2, cdt);
+    const at::Tensor ws = workspace_of(x, bytes);
+    void* const st = stream_of(*c.dev);
+    check_status(unlocked([&] {
+                     return vq2_head_loss(ptr(x), xdt, (const float*)ptr(x_scale), T, (const int64_t*)ptr(targets), ignore_index,
+                                          (const int16_t*)ptr(i0), ptr(i1), s2, ptr(cb0), s2 ? ptr(cb1) : nullptr, cdt, ptr(scale),
+                                          dt_code(scale.scalar_type()), out, n, (float)rs, loss.data_ptr<float>(),
+                                          lse.data_ptr<float>(), ws.data_ptr(), bytes, st);
+                 }),
+                 "vq2_head_loss");
+    return py::make_tuple(loss, lse);
+}
+
+// vq_gated_rows; the activation as a code
+py::object gated_rows(const at::Tensor& x, const py::sequence& gate, const py::sequence& up, const at::Tensor& cb0,
+                      const OptTensor& cb1, int64_t n, double rs, int64_t act, const OptTensor& x_scale,
+                      std::optional<at::ScalarType> out_dtype)
+{
+    Check c;
+    const int xdt = panel_rows(c, x, x_scale, n);
+    if (!c.ok || !on_current_device(x) || gate.size() != 3 || up.size() != 3) return py::none();
+    vq2_seg seg[2] = {};
+    at::Tensor scales[2];
+    int s2 = -1;
+    int64_t rows = 0;
+    for (int k = 0; k < 2; k++) {
+        const py::sequence& m = k ? up : gate;
+        const at::Tensor i0 = py::cast<at::Tensor>(m[0]);
+        const OptTensor i1 = py::cast<OptTensor>(m[1]);
+        scales[k] = py::cast<at::Tensor>(m[2]);
+        if (k == 0) rows = scales[0].numel();
+        const int kind = panel_mat(c, i0, i1, scales[k], cb0, cb1, rows, n);
+        if (!c.ok || kind < 0 || rows == 0 || (k && (kind != s2 || scales[1].scalar_type() != scales[0].scalar_type())))
+            return py::none();
+        s2 = kind;
+        seg[k] = vq2_seg{(const int16_t*)ptr(i0), ptr(i1), ptr(scales[k]), nullptr, rows, rows};
+    }
+    const at::ScalarType odt = out_dtype.value_or(dt_code(x.scalar_type()) >= 0 ? x.scalar_type() : at::kBFloat16);
+    const int ydt = dt_code(odt), cdt = dt_code(cb0.scalar_type());
+    if (ydt < 0) return py::none();
+    const int64_t T = x.numel() / n;
+    auto shape = x.sizes().vec();
+    shape.back() = rows;
+    at::Tensor y = at::empty(shape, x.options().dtype(odt));
+    const size_t bytes = vq2_gated_rows_workspace(T, rows, n, s2, cdt, ydt);
+    const at::Tensor ws = workspace_of(x, bytes);
+    void* const st = stream_of(*c.dev);
+    check_status(unlocked([&] {
+                     return vq2_gated_rows(ptr(x), xdt, (const float*)ptr(x_scale), T, seg, s2, ptr(cb0), s2 ? ptr(cb1) : nullptr,
+                                           cdt, dt_code(scales[0].scalar_type()), n, (float)rs, (int)act, y.data_ptr(), ydt,
+                                           ws.data_ptr(), bytes, st);
+                 }),
+                 "vq2_gated_rows");
+    return py::cast(y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -503,6 +674,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("sorted_moe", &sorted_moe);
     m.def("router_select", &router_select);
     m.def("sample", &sample);
+    m.def("add_rms_norm", &add_rms_norm);
+    m.def("head_loss", &head_loss);
+    m.def("gated_rows", &gated_rows);
     m.def("sorted_slices", [](int64_t chunks, int64_t min_ipc, int64_t cu) {
         return sorted_slices(std::max<int64_t>(1, chunks), min_ipc, cu);
     });

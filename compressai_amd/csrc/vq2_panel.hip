@@ -45,11 +45,18 @@ __device__ __forceinline__ int exponent_of(float v)
     return b == 0xFF || (__float_as_uint(v) & 0x7FFFFFFFu) == 0 ? 0 : b - 127;
 }
 
-// exponent of a power of two not below any row scale (bits of their largest
-// magnitude); bounded so that 2^(15 - e) and 2^e are normal numbers
-__device__ __forceinline__ int scale_exponent(uint32_t bits)
+// Exponent of a power of two not below any row scale, from the largest
+// magnitudes of the prologue's workgroups; bounded so that 2^(15 - e) and 2^e
+// are normal numbers.  Called by whole waves.
+struct RowTop {
+    const float* part;
+    int n;
+};
+__device__ __forceinline__ int scale_exponent(const RowTop& t)
 {
-    const int b = (int)(bits >> 23);
+    float m = 0.0f;
+    for (int i = threadIdx.x & 63; i < t.n; i += 64) m = fmaxf(m, t.part[i]);
+    const int b = (int)(__float_as_uint(wave_max_all(m)) >> 23);
     return b == 0xFF ? 0 : min(max(b - 126, -100), 100);
 }
 
@@ -63,83 +70,6 @@ __device__ __forceinline__ float sum_rows(float v)
 {
     v += swz_xor16(v);
     return v + xor32(v);
-}
-
-// -------------------------------------------------------------- token rows
-struct PackArgs {
-    const void* x;
-    int x_dt;
-    int tokens, n;  // rows past the last token are zeros
-    const float* x_scale;
-    half8_t* panel;     // [tiles][n / 32][64]
-    float* fac;         // a product of the panel times fac[t] is one of the row
-    uint32_t* amax;     // largest row scale, cleared here for prep_kernel
-};
-
-// One workgroup a tile of 16 rows, its 16 waves a share of the k tiles each:
-// the rows' largest magnitudes, then fp16 under a power of two that brings
-// them into [2^13, 2^14).  Rows of up to 4096 values stay in registers in
-// between (4096 rows of 2048: 21 us with 4 waves that read twice).
-constexpr int PK_WAVES = 16, PK_HELD = 8;
-__global__ void __launch_bounds__(64 * PK_WAVES) pack_rows_kernel(const PackArgs a)
-{
-    __shared__ float s_m[PK_WAVES][16];
-    const int tid = threadIdx.x, tile = blockIdx.x;
-    if (tile == 0 && tid == 0 && a.amax) *a.amax = 0;
-    const int lane = tid & 63, wave = tid >> 6, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
-    const int per = (kt + PK_WAVES - 1) / PK_WAVES, k0 = wave * per, k1 = min(k0 + per, kt);
-    const bool live = row < a.tokens, held = per <= PK_HELD;
-    const int64_t at = (int64_t)row * a.n + q * 8;
-    Eight x[PK_HELD];
-    float m = 0.0f;
-    if (held) {
-#pragma unroll
-        for (int i = 0; i < PK_HELD; i++)
-            if (live && k0 + i < k1) x[i] = load8(a.x, a.x_dt, at + (k0 + i) * 32);
-            else
-#pragma unroll
-                for (int k = 0; k < 8; k++) x[i].v[k] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PK_HELD; i++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(x[i].v[k]));
-    } else if (live) {
-        for (int k = k0; k < k1; k++) {
-            const Eight e = load8(a.x, a.x_dt, at + k * 32);
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(e.v[j]));
-        }
-    }
-    m = max_rows(m);
-    if (q == 0) s_m[wave][lane & 15] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < PK_WAVES; w++) m = fmaxf(m, s_m[w][lane & 15]);
-    // (8-bit values are exact as they are)
-    const int e = a.x_dt <= VQ2_DT_BF16 && m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
-    if (tid < 16) a.fac[row] = live ? pow2(e) * (a.x_scale ? a.x_scale[row] : 1.0f) : 0.0f;
-    const float f = pow2(-e);
-    half8_t* out = a.panel + (int64_t)tile * kt * 64 + lane;
-    if (held) {
-#pragma unroll
-        for (int i = 0; i < PK_HELD; i++) {
-            if (k0 + i >= k1) break;
-            half8_t h;
-#pragma unroll
-            for (int j = 0; j < 8; j++) h[j] = (_Float16)(x[i].v[j] * f);
-            out[(k0 + i) * 64] = h;
-        }
-    } else {
-        for (int k = k0; k < k1; k++) {
-            half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (live) {
-                const Eight v = load8(a.x, a.x_dt, at + k * 32);
-#pragma unroll
-                for (int j = 0; j < 8; j++) h[j] = (_Float16)(v.v[j] * f);
-            }
-            out[k * 64] = h;
-        }
-    }
 }
 
 // ------------------------------------------------------------ packed rows
@@ -165,39 +95,176 @@ __device__ __forceinline__ int64_t mat_row(const MatArgs& a, int64_t tile, int r
     return (a.nmat == 2 ? tile >> 1 : tile) * 16 + r;
 }
 
-// Order of a panel's 16 rows.  Plain: as they come.  Turned: row 4 i + c at
-// place 4 c + i; a lane of a product then holds rows c, 4 + c, 8 + c, 12 + c
-// (c = lane / 16), and two tiles' values are the 8 values of operand chunk c
-// of the panel that the next product reads: the lane stores them as they are.
-__device__ __forceinline__ int turned(int r) { return (r & 3) * 4 + (r >> 2); }
+// What a wave finds of two row tiles in its registers is the operand of the
+// next product: lane (q, t) holds rows 4 q .. + 3 of both, 8 values, and that is
+// its chunk q of a k tile of 32 rows as long as the columns' panel has the
+// same order (value m of chunk q: row 16 (m / 4) + 4 q + m % 4).  So a
+// gradient is stored as it is made, a KiB a tile.
+__device__ __forceinline__ int chunk_row(int q, int m) { return 16 * (m >> 2) + 4 * q + (m & 3); }
+
+// -------------------------------------------------------------- prologue
+// One launch: token rows, upstream rows' factors, row scales.
+struct PackArgs {
+    const void* x;
+    int x_dt;
+    int tokens, n;  // rows past the last token are zeros
+    const float* x_scale;
+    half8_t* panel;     // [tiles][n / 32][64]
+    float* fac;         // a product of the panel times fac[t] is one of the row
+    int tiles;          // 0: no rows to pack
+};
+
+// One workgroup a tile of 16 rows, its 16 waves a share of the k tiles each:
+// the rows' largest magnitudes, then fp16 under a power of two that brings
+// them into [2^13, 2^14).  Rows of up to 4096 values stay in registers in
+// between (4096 rows of 2048: 21 us with 4 waves that read twice).
+constexpr int PK_WAVES = 16, PK_HELD = 8;
+template <int DT>
+__device__ __forceinline__ void pack_rows(const PackArgs& a, int tile, float (*s_m)[16])
+{
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, wave = tid >> 6, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
+    const int per = (kt + PK_WAVES - 1) / PK_WAVES, k0 = wave * per, k1 = min(k0 + per, kt);
+    const bool live = row < a.tokens, held = per <= PK_HELD;
+    const int64_t at = (int64_t)row * a.n + q * 8;
+    Eight x[PK_HELD];
+    float m = 0.0f;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < PK_HELD; i++)
+            if (live && k0 + i < k1) x[i] = load8(a.x, DT, at + (k0 + i) * 32);
+            else
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[i].v[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PK_HELD; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(x[i].v[k]));
+    } else if (live) {
+        for (int k = k0; k < k1; k++) {
+            const Eight e = load8(a.x, DT, at + k * 32);
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(e.v[j]));
+        }
+    }
+    m = max_rows(m);
+    if (q == 0) s_m[wave][lane & 15] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < PK_WAVES; w++) m = fmaxf(m, s_m[w][lane & 15]);
+    // (8-bit values are exact as they are)
+    const int e = DT <= VQ2_DT_BF16 && m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
+    if (tid < 16) a.fac[row] = live ? pow2(e) * (a.x_scale ? a.x_scale[row] : 1.0f) : 0.0f;
+    const float f = pow2(-e);
+    half8_t* out = a.panel + (int64_t)tile * kt * 64 + lane;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < PK_HELD; i++) {
+            if (k0 + i >= k1) break;
+            half8_t h;
+#pragma unroll
+            for (int j = 0; j < 8; j++) h[j] = (_Float16)(x[i].v[j] * f);
+            out[(k0 + i) * 64] = h;
+        }
+    } else {
+        for (int k = k0; k < k1; k++) {
+            half8_t h = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (live) {
+                const Eight v = load8(a.x, DT, at + k * 32);
+#pragma unroll
+                for (int j = 0; j < 8; j++) h[j] = (_Float16)(v.v[j] * f);
+            }
+            out[k * 64] = h;
+        }
+    }
+}
+
+struct DyMaxArgs {
+    const void* dy;
+    int dy_dt, tokens, vec;  // vec: rows a multiple of 8, 16-byte aligned
+    int64_t rows;
+    int head;     // bits left above the row's largest value
+    float* dfac;  // [tp]: 2^-e, which brings the row's largest into [2^(14 - head), 2^(15 - head))
+    int groups;   // of 16 rows
+};
+// a wave a row
+template <int DT>
+__device__ __forceinline__ void dy_max(const DyMaxArgs& a, int group)
+{
+    const int lane = threadIdx.x & 63, t = group * PK_WAVES + (threadIdx.x >> 6);
+    float m = 0.0f;
+    if (t < a.tokens) {
+        const int64_t at = t * a.rows;
+        if (a.vec) {
+#pragma unroll 4
+            for (int64_t i = lane * 8; i < a.rows; i += 512) {
+                const Eight e = load8(a.dy, DT, at + i);
+#pragma unroll
+                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t i = lane; i < a.rows; i += 64) m = fmaxf(m, fabsf(load_as_f32(a.dy, DT, at + i)));
+        }
+    }
+    m = wave_max_all(m);
+    const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
+    if (lane == 0) a.dfac[t] = pow2(-e);
+}
 
 struct PrepArgs {
     MatArgs m;
     float rs;
-    int turn;
-    int64_t places;   // 16 * tiles
-    float* sc;        // scale * rs of each place, 0 past the last row
-    uint32_t* amax;   // largest magnitude among them, as bits
+    int64_t places;  // 16 * tiles
+    float* sc;       // scale * rs of each place, 0 past the last row
+    float* top;      // largest magnitude of each workgroup's
+    int groups;      // of PREP_ROWS places
 };
-__global__ void __launch_bounds__(256) prep_kernel(const PrepArgs a)
+constexpr int PREP_ROWS = 4 * 64 * PK_WAVES;
+__device__ __forceinline__ void prep_scales(const PrepArgs& a, int group, float* s_top)
 {
-    const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    float v = 0.0f;
-    if (p < a.places) {
+    float m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int64_t p = (int64_t)group * PREP_ROWS + k * 64 * PK_WAVES + threadIdx.x;
+        if (p >= a.places) continue;
         int mat;
-        const int place = (int)(p & 15);
-        const int64_t row = mat_row(a.m, p >> 4, a.turn ? turned(place) : place, mat);
-        if (row < a.m.rows) v = load_as_f32(a.m.m[mat].scale, a.m.s_dt, row) * a.rs;
+        const int64_t row = mat_row(a.m, p >> 4, (int)(p & 15), mat);
+        const float v = row < a.m.rows ? load_as_f32(a.m.m[mat].scale, a.m.s_dt, row) * a.rs : 0.0f;
         a.sc[p] = v;
+        m = fmaxf(m, fabsf(v));
     }
-    if (!a.amax) return;
-    // (magnitudes as bits are ordered like the numbers, and a maximum does
-    // not depend on the order of its parts)
-    __shared__ float s_m[4];
-    const float m = wave_max_all(fabsf(v));
-    if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
+    m = wave_max_all(m);
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) atomicMax(a.amax, __float_as_uint(fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]))));
+    if (threadIdx.x) return;
+    for (int k = 0; k < PK_WAVES; k++) m = fmaxf(m, s_top[k]);
+    a.top[group] = m;
+}
+
+struct PrologueArgs {
+    PackArgs pack;
+    DyMaxArgs dy;
+    PrepArgs prep;
+};
+__global__ void __launch_bounds__(64 * PK_WAVES) prologue_kernel(const PrologueArgs a)
+{
+    __shared__ float s_m[PK_WAVES][16];
+    int b = blockIdx.x;
+    // (types apart: behind a branch on the type every load is waited for)
+    if (b < a.pack.tiles) {
+        if (a.pack.x_dt == VQ2_DT_F16) return pack_rows<VQ2_DT_F16>(a.pack, b, s_m);
+        if (a.pack.x_dt == VQ2_DT_BF16) return pack_rows<VQ2_DT_BF16>(a.pack, b, s_m);
+        if (a.pack.x_dt == VQ2_DT_I8) return pack_rows<VQ2_DT_I8>(a.pack, b, s_m);
+        return pack_rows<VQ2_DT_E4M3>(a.pack, b, s_m);
+    }
+    b -= a.pack.tiles;
+    if (b < a.dy.groups) {
+        if (a.dy.dy_dt == VQ2_DT_F16) return dy_max<VQ2_DT_F16>(a.dy, b);
+        if (a.dy.dy_dt == VQ2_DT_BF16) return dy_max<VQ2_DT_BF16>(a.dy, b);
+        return dy_max<VQ2_DT_F32>(a.dy, b);
+    }
+    prep_scales(a.prep, b - a.dy.groups, s_m[0]);
 }
 
 template <int CBT>
@@ -244,26 +311,66 @@ struct DequantArgs {
     half8_t* w;     // [tiles][PARTS * ng / 4][64]
     half8_t* wt;    // [columns / 16][parts * tiles / 2][64], or null
     int vkt;        // tiles / 2
+    int vec;        // planes of 16-byte aligned rows
 };
 
+// 8 codes of consecutive groups as words of two 16-bit codes (uint8 planes:
+// of four)
+template <int B>
+__device__ __forceinline__ u32x4 codes8(const void* p, int64_t i)
+{
+    if constexpr (B == 2) return *(const u32x4*)((const uint16_t*)p + i);
+    const u32x2 u = *(const u32x2*)((const uint8_t*)p + i);
+    return u32x4{u.x, u.y, 0, 0};
+}
+// lane (row, q)'s code of k tile k of a wave's 8, group 4 k + q: lane (row,
+// k / 2) holds it at 4 (k % 2) + q of its 8
+template <int B>
+__device__ __forceinline__ uint32_t code_of(const u32x4& w, int k, int lane)
+{
+    const int q = lane >> 4, src = ((lane & 15) + 16 * (k >> 1)) * 4;
+    if constexpr (B == 2) {
+        const uint32_t a = __builtin_amdgcn_ds_bpermute(src, (int)w[2 * (k & 1)]);
+        const uint32_t b = __builtin_amdgcn_ds_bpermute(src, (int)w[2 * (k & 1) + 1]);
+        return (q & 2 ? b : a) >> (16 * (q & 1)) & 0xFFFFu;
+    }
+    return (uint32_t)__builtin_amdgcn_ds_bpermute(src, (int)w[k & 1]) >> (8 * q) & 0xFFu;
+}
+
 // Forward: rows in plain order.  A wave takes a tile of 16 rows and 8 k
-// tiles: lane (row, q) gathers group 4 k + q, and each k tile is one KiB.
+// tiles: lane (row, q) gathers group 4 k + q, and each k tile is one KiB.  The
+// codes come 8 a lane where their rows are aligned (vec), and change lanes in
+// the LDS unit: loaded one by one they cost a request for each 4 gathers.
 template <int CBT, int S2, int PARTS>
 __global__ void __launch_bounds__(256) dequant_plain_kernel(const DequantArgs a)
 {
+    constexpr int B1 = S2 == VQ2_S2_U8 ? 1 : 2;
     const int lane = threadIdx.x & 63, q = lane >> 4;
     const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int kt = a.m.ng / 4;
+    const int kt = a.m.ng / 4, k0 = blockIdx.y * 8;
     int mat;
     const int64_t row = mat_row(a.m, a.tile0 + tile, lane & 15, mat);
     const bool ok = row < a.m.rows;
     const int64_t off = (ok ? row : 0) * a.m.ng;
+    const void *i0 = a.m.m[mat].i0, *i1 = a.m.m[mat].i1;
     uint32_t c0[8], c1[8];
+    if (a.vec) {
+        const int g = k0 * 4 + q * 8, at = g < a.m.ng ? g : 0;
+        const u32x4 w = codes8<2>(i0, off + at);
+        u32x4 v = {0, 0, 0, 0};
+        if constexpr (S2 != VQ2_S2_NONE) v = codes8<B1>(i1, off + at);
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const int64_t i = off + min((int)blockIdx.y * 8 + k, kt - 1) * 4 + q;
-        c0[k] = ((const uint16_t*)a.m.m[mat].i0)[i];
-        c1[k] = code1<S2>(a.m.m[mat].i1, i);
+        for (int k = 0; k < 8; k++) {
+            c0[k] = code_of<2>(w, k, lane);
+            c1[k] = S2 == VQ2_S2_NONE ? 0 : code_of<B1>(v, k, lane);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int64_t i = off + min(k0 + k, kt - 1) * 4 + q;
+            c0[k] = ((const uint16_t*)i0)[i];
+            c1[k] = code1<S2>(i1, i);
+        }
     }
     const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
     half8_t hi[8], lo[8];
@@ -271,22 +378,20 @@ __global__ void __launch_bounds__(256) dequant_plain_kernel(const DequantArgs a)
     for (int k = 0; k < 8; k++) weight_of<CBT, S2, PARTS>(a.m, c0[k], c1[k], hi[k], lo[k]);
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-        const int t = (int)blockIdx.y * 8 + k;
-        if (t >= kt) break;
-        half8_t* w = a.w + (tile * (PARTS * kt) + t) * 64 + lane;
+        if (k0 + k >= kt) break;
+        half8_t* w = a.w + (tile * (PARTS * kt) + k0 + k) * 64 + lane;
         w[0] = ok ? hi[k] : zero;
         if constexpr (PARTS == 2) w[(int64_t)kt * 64] = ok ? lo[k] : zero;
     }
 }
 
-// Backward: rows in turned order, and the columns' panel.  A wave takes 32
-// rows (two tiles) and 16 groups: lane (c, g) gathers the 8 rows 16 (m / 4) +
-// 4 (m % 4) + c of group g.  Column j of the 8 centroids is then one operand
-// of the columns' panel, whose block j holds columns j, 8 + j, ... of the 16
-// groups: one KiB a block, and a lane of the next product holds 8 neighbouring
-// columns in its 8 row tiles.
+// Backward: the rows' panel (WP), and the columns'.  A wave takes 32 rows (two
+// tiles) and 16 groups: lane (q, g) gathers the 8 rows of chunk q of group g.
+// Column j of the 8 centroids is then one operand of the columns' panel, whose
+// block j holds columns j, 8 + j, ... of the 16 groups: one KiB a block, and a
+// lane of the next product holds 8 neighbouring columns in its 8 row tiles.
 template <int CBT, int S2, int WP, int TP>
-__global__ void __launch_bounds__(256) dequant_turned_kernel(const DequantArgs a)
+__global__ void __launch_bounds__(256) dequant_both_kernel(const DequantArgs a)
 {
     const int lane = threadIdx.x & 63, c = lane >> 4, g = blockIdx.y * 16 + (lane & 15);
     const int pair = blockIdx.x * 4 + (threadIdx.x >> 6);  // of the piece
@@ -297,7 +402,7 @@ __global__ void __launch_bounds__(256) dequant_turned_kernel(const DequantArgs a
 #pragma unroll
     for (int m = 0; m < 8; m++) {
         int mat;
-        const int64_t row = mat_row(a.m, a.tile0 + 2 * pair + m / 4, 4 * (m % 4) + c, mat);
+        const int64_t row = mat_row(a.m, a.tile0 + 2 * pair + m / 4, 4 * c + m % 4, mat);
         ok[m] = g_ok && row < a.m.rows;
         const int64_t i = ok[m] ? row * a.m.ng + g : 0;
         c0[m] = ((const uint16_t*)a.m.m[mat].i0)[i];
@@ -313,12 +418,20 @@ __global__ void __launch_bounds__(256) dequant_turned_kernel(const DequantArgs a
         hi[m] = ok[m] ? hi[m] : zero;
         if constexpr (PARTS == 2) lo[m] = ok[m] ? lo[m] : zero;
     }
-    if (WP && g_ok) {
+    if constexpr (WP != 0) {
+        // the wave's 2 row tiles by 4 k tiles, a KiB each, put in order in LDS
+        __shared__ half8_t s_w[4][8][64];
+        half8_t(*sw)[64] = s_w[threadIdx.x >> 6];
+        const int gi = lane & 15, k0 = blockIdx.y * 4;
 #pragma unroll
-        for (int m = 0; m < 8; m++) {
-            half8_t* w = a.w + ((int64_t)(2 * pair + m / 4) * (WP * kt) + g / 4) * 64 + (g & 3) * 16 + 4 * c + m % 4;
-            w[0] = hi[m];
-            if constexpr (WP == 2) w[(int64_t)kt * 64] = lo[m];
+        for (int part = 0; part < WP; part++) {
+#pragma unroll
+            for (int m = 0; m < 8; m++) sw[(m / 4) * 4 + gi / 4][(gi & 3) * 16 + 4 * c + m % 4] = part ? lo[m] : hi[m];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int f = 0; f < 8; f++)
+                if (k0 + f % 4 < kt) a.w[((int64_t)(2 * pair + f / 4) * (WP * kt) + part * kt + k0 + f % 4) * 64 + lane] = sw[f][lane];
+            __builtin_amdgcn_wave_barrier();
         }
     }
 #pragma unroll
@@ -364,29 +477,36 @@ struct StatsEpi {
     int tokens, tp;
     f32x2_t* part;  // [parts of rows][tp]: largest logit and sum of exp(l - largest)
     float* at;      // [tp]: the target's logit
-    // two tiles' products of a token (few_kernel): a part of 32 rows
-    __device__ __forceinline__ void few(const MatArgs& m, float rs, f32x4_t a, f32x4_t b, int64_t pair, int t) const
+    // few_kernel: a lane's running maximum and sum for its token
+    struct State {
+        float m = NEG_INF, s = 0.0f;
+    };
+    __device__ __forceinline__ void few(State& st, const MatArgs& m, float rs, f32x4_t a, f32x4_t b, int64_t pair, int t) const
     {
         const int q = (threadIdx.x & 63) >> 4;
         const int64_t r0 = pair * 32 + q * 4;
-        float z[8], top = NEG_INF;
+        float z[8], top = st.m;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const int64_t r = r0 + (k >> 2) * 16 + (k & 3);
             z[k] = r < m.rows ? (k < 4 ? a[k & 3] : b[k & 3]) * row_scale(m, rs, 0, r) : NEG_INF;
             top = fmaxf(top, z[k]);
         }
-        top = max_rows(top);
         const float base = top == NEG_INF ? 0.0f : top;
-        float sum = 0.0f;
+        st.s *= __expf(st.m - base);
+        st.m = top;
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum += __expf(z[k] - base);
-        sum = sum_rows(sum);
-        if (q == 0) part[pair * tp + t] = f32x2_t{top, sum};
+        for (int k = 0; k < 8; k++) st.s += __expf(z[k] - base);
         const int64_t rel = (t < tokens ? target_of(target, t, ignore, rows) : TARGET_SKIP) - r0;
 #pragma unroll
         for (int k = 0; k < 8; k++)
             if (rel == (k >> 2) * 16 + (k & 3)) at[t] = z[k];
+    }
+    __device__ __forceinline__ void few_end(const State& st, int64_t chunk, int t) const
+    {
+        const float top = max_rows(st.m), base = top == NEG_INF ? 0.0f : top;
+        const float sum = sum_rows(st.s * __expf(st.m - base));
+        if ((threadIdx.x & 63) < 16) part[chunk * tp + t] = f32x2_t{top, sum};
     }
     template <int MT>
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
@@ -438,7 +558,7 @@ struct DlogitEpi {
     const float* lse;
     const float* dloss;
     const int64_t* target;
-    const uint32_t* amax;
+    RowTop amax;
     int64_t rows, ignore, tile0;  // tile0: the piece's first tile
     int tokens, tp, vkt;
     half8_t* p;    // the next product's panel of tokens, [tp / 16][vkt][64]
@@ -448,7 +568,7 @@ struct DlogitEpi {
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
-        const float c = pow2(14 - scale_exponent(*amax));
+        const float c = pow2(14 - scale_exponent(amax));
         float l[PG_NT], up[PG_NT], f[PG_NT];
         int rel[PG_NT];  // the target's row of the wave's, or none; SKIP: the token does not count
         constexpr int SKIP = -2, NONE = -1;
@@ -480,7 +600,7 @@ struct DlogitEpi {
                 half8_t h;
 #pragma unroll
                 for (int m = 0; m < 8; m++) {
-                    const int e = m & 3, k = m >> 2, r = (i + k) * 16 + 4 * e + q;
+                    const int e = m & 3, k = m >> 2, r = (i + k) * 16 + 4 * q + e;
                     const float raw = acc[i + k][j][e] * f[j];
                     float v = __expf(raw * s[k][e] - l[j]) - (rel[j] == r ? 1.0f : 0.0f);
                     if (rel[j] == SKIP || r >= left) v = 0.0f;
@@ -543,7 +663,9 @@ struct GatedEpi {
             *(u32x2*)((uint16_t*)y + at) = u32x2{bf16_pair(o[0], o[1]), bf16_pair(o[2], o[3])};
         }
     }
-    __device__ __forceinline__ void few(const MatArgs& m, float rs, f32x4_t g, f32x4_t u, int64_t pair, int t) const
+    struct State {};
+    __device__ __forceinline__ void few_end(const State&, int64_t, int) const {}
+    __device__ __forceinline__ void few(State&, const MatArgs& m, float rs, f32x4_t g, f32x4_t u, int64_t pair, int t) const
     {
         const int q = (threadIdx.x & 63) >> 4;
         const int64_t r0 = pair * 16 + q * 4;
@@ -592,14 +714,65 @@ struct GatedEpi {
     }
 };
 
+// Upstream values of 4 neighbouring rows of a token, as loaded (16 bits: vec
+// rows in 8 bytes) and as numbers.
+struct Upstream {
+    const void* dy;  // [tokens][rows]
+    int dt, tokens, vec;
+    int64_t rows;
+    __device__ __forceinline__ u32x2 raw(int t, int64_t r) const
+    {
+        // (past the tokens or rows: anything of the row; numbers() drops it)
+        const int64_t at = (int64_t)min(t, tokens - 1) * rows + (r < rows ? r : 0);
+        return *(const u32x2*)((const uint16_t*)dy + at);
+    }
+    __device__ __forceinline__ f32x4_t numbers(u32x2 w, int t, int64_t r) const
+    {
+        f32x4_t v;
+        if (dt == VQ2_DT_F16) {
+            const half4_t h = __builtin_bit_cast(half4_t, w);
+            v = f32x4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        } else {
+            v = f32x4_t{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+                        __uint_as_float(w.y & 0xFFFF0000u)};
+        }
+        const bool in = t < tokens && r < rows;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = in ? v[e] : 0.0f;
+        return v;
+    }
+    __device__ __forceinline__ f32x4_t slow(int t, int64_t r) const
+    {
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (t < tokens && r + e < rows) v[e] = load_as_f32(dy, dt, (int64_t)t * rows + r + e);
+        return v;
+    }
+    // of PG_NT token tiles
+    __device__ __forceinline__ void load(f32x4_t (&d)[PG_NT], int t, int64_t r) const
+    {
+        if (vec) {
+            u32x2 w[PG_NT];
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) w[j] = raw(t + j * 16, r);
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) d[j] = numbers(w[j], t + j * 16, r);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) d[j] = slow(t + j * 16, r);
+        }
+    }
+};
+
 struct DgatedEpi {
     const float* sc;
     const float* fac;
-    const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_max_kernel)
-    const void* dy;     // [tokens][rows]
-    const uint32_t* amax;
-    int dy_dt, tokens, tp, vkt;
-    int64_t rows, tile0;
+    const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_max)
+    Upstream up;
+    RowTop amax;
+    int tp, vkt;
+    int64_t tile0;
     half8_t* p;
     float* ds;
     int64_t ds_ld;
@@ -608,28 +781,31 @@ struct DgatedEpi {
     __device__ __forceinline__ void run_act(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok)
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
-        const float c = pow2(-scale_exponent(*amax));
+        const float c = pow2(-scale_exponent(amax));
+        float x[PG_NT], k[PG_NT];
+#pragma unroll
+        for (int j = 0; j < PG_NT; j++) {
+            x[j] = fac[tok + j * 16 + nl];
+            k[j] = dfac[tok + j * 16 + nl];
+        }
 #pragma unroll
         for (int i = 0; i < MT; i += 2) {
             const f32x4_t sg = *(const f32x4_t*)(sc + (tile + i) * 16 + q * 4);
             const f32x4_t su = *(const f32x4_t*)(sc + (tile + i + 1) * 16 + q * 4);
-            const int64_t r0 = (tile + i) / 2 * 16 + q;
+            f32x4_t d[PG_NT];
+            up.load(d, tok + nl, (tile + i) / 2 * 16 + q * 4);
             f32x4_t dsg = {0.0f, 0.0f, 0.0f, 0.0f}, dsu = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int j = 0; j < PG_NT; j++) {
-                const int t = tok + j * 16 + nl;
-                const float x = fac[t], k = t < tokens ? dfac[t] : 0.0f;
                 half8_t h;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float d = t < tokens && r0 + 4 * e < rows
-                                        ? load_as_f32(dy, dy_dt, (int64_t)t * rows + r0 + 4 * e) : 0.0f;
-                    const float rg = acc[i][j][e] * x, ru = acc[i + 1][j][e] * x;
+                    const float rg = acc[i][j][e] * x[j], ru = acc[i + 1][j][e] * x[j];
                     float f, df;
                     gate_act<ACT>(rg * sg[e], f, df);
-                    const float dg = d * (ru * su[e]) * df, du = d * f;
-                    h[e] = (_Float16)(dg * k * (sg[e] * c));
-                    h[4 + e] = (_Float16)(du * k * (su[e] * c));
+                    const float dg = d[j][e] * (ru * su[e]) * df, du = d[j][e] * f;
+                    h[e] = (_Float16)(dg * k[j] * (sg[e] * c));
+                    h[4 + e] = (_Float16)(du * k[j] * (su[e] * c));
                     if (ds) {
                         dsg[e] += dg * rg;
                         dsu[e] += du * ru;
@@ -661,30 +837,22 @@ struct DgatedEpi {
 // sums over 64 tokens of upstream times product: the row scales' gradient
 struct ColsumEpi {
     const float* fac;
-    const void* dy;
-    int dy_dt, tokens;
-    int64_t rows;
+    Upstream up;
     float* ds;
     int64_t ds_ld;
     template <int MT>
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int)
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
+        float x[PG_NT];
+#pragma unroll
+        for (int j = 0; j < PG_NT; j++) x[j] = fac[tok + j * 16 + nl];
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const int64_t r0 = (tile + i) * 16 + q;
-            f32x4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
+            f32x4_t u[PG_NT], d = {0.0f, 0.0f, 0.0f, 0.0f};
+            up.load(u, tok + nl, (tile + i) * 16 + q * 4);
 #pragma unroll
-            for (int j = 0; j < PG_NT; j++) {
-                const int t = tok + j * 16 + nl;
-                const float x = fac[t];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float u = t < tokens && r0 + 4 * e < rows
-                                        ? load_as_f32(dy, dy_dt, (int64_t)t * rows + r0 + 4 * e) : 0.0f;
-                    d[e] += u * (acc[i][j][e] * x);
-                }
-            }
+            for (int j = 0; j < PG_NT; j++) d += u[j] * (acc[i][j] * x[j]);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float v = group_sum(d[e], 16);
@@ -694,17 +862,68 @@ struct ColsumEpi {
     }
 };
 
-// Columns' product, added to what earlier pieces left: tile i of the wave
-// holds columns i, 8 + i, ... of its 128 (MT == 8) or the 64 of parity h.
+// What makes a row of the columns' product one of dx: the factors that its
+// panel left out, and of the loss the upstream value (zero rows: exactly zero).
+struct DxFactor {
+    RowTop amax;
+    const float* dfac;  // [tp], or null: the loss's
+    const float* dloss;
+    const int64_t* target;
+    int64_t rows, ignore;
+    float base;         // by init(), called by whole waves
+    __device__ __forceinline__ void init() { base = pow2(scale_exponent(amax) - (dfac ? 0 : 14)); }
+    // (two factors: their product may leave fp32's range)
+    __device__ __forceinline__ float apply(float v, float f, bool skip) const { return skip ? 0.0f : v * base * f; }
+    __device__ __forceinline__ float of(int t, bool& skip) const
+    {
+        skip = false;
+        if (dfac) return 1.0f / dfac[t];
+        const int64_t v = target_of(target, t, ignore, rows);
+        skip = v == TARGET_SKIP;
+        return v == TARGET_BAD ? __builtin_nanf("") : dloss[t];
+    }
+};
+
+// Columns' product, added to what earlier pieces left, or (dx) finished: tile i
+// of the wave holds columns i, 8 + i, ... of its 128 (MT == 8), or of the half
+// of them that starts at tile % 8.
 struct GradEpi {
     float* out;  // [slices][tp][np]
     int64_t np;
     int tp, add;
+    void* dx;    // [tokens][n], or null
+    int dx_dt, tokens, n;
+    DxFactor fac;
     template <int MT>
     __device__ __forceinline__ void run(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok, int bz)
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
         const int64_t c0 = tile / 8 * 128 + tile % 8;
+        if (dx) {
+            fac.init();
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) {
+                const int t = tok + j * 16 + nl;
+                if (t >= tokens) continue;
+                bool skip;
+                const float f = fac.of(t, skip);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int64_t col = c0 + (q * 4 + e) * 8;
+                    if (col >= n) continue;
+                    uint32_t w[MT / 2];
+#pragma unroll
+                    for (int i = 0; i < MT; i += 2) {
+                        const float a = fac.apply(acc[i][j][e], f, skip), b = fac.apply(acc[i + 1][j][e], f, skip);
+                        w[i / 2] = dx_dt == VQ2_DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : bf16_pair(a, b);
+                    }
+                    uint32_t* o = (uint32_t*)((uint16_t*)dx + (int64_t)t * n + col);
+                    if constexpr (MT == 8) *(u32x4*)o = u32x4{w[0], w[1], w[2], w[3]};
+                    else *(u32x2*)o = u32x2{w[0], w[1]};
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < PG_NT; j++) {
             float* o = out + ((int64_t)bz * tp + tok + j * 16 + nl) * np + c0;
@@ -733,85 +952,44 @@ __global__ void __launch_bounds__(PG_THREADS, MT == 8 ? 2 : 3) panel_gemm_kernel
 }
 
 // ------------------------------------------------------------ upstream rows
-struct DyMaxArgs {
-    const void* dy;
-    int dy_dt, tokens, vec;  // vec: rows a multiple of 8, 16-byte aligned
-    int64_t rows;
-    int head;     // bits left above the row's largest value
-    float* dfac;  // [tp]: 2^-e, which brings the row's largest into [2^(14 - head), 2^(15 - head))
-};
-// a wave a row
-__global__ void __launch_bounds__(256) dy_max_kernel(const DyMaxArgs a)
-{
-    const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
-    float m = 0.0f;
-    if (t < a.tokens) {
-        const int64_t at = t * a.rows;
-        if (a.vec) {
-#pragma unroll 4
-            for (int64_t i = lane * 8; i < a.rows; i += 512) {
-                const Eight e = load8(a.dy, a.dy_dt, at + i);
-#pragma unroll
-                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
-            }
-        } else {
-#pragma unroll 4
-            for (int64_t i = lane; i < a.rows; i += 64) m = fmaxf(m, fabsf(load_as_f32(a.dy, a.dy_dt, at + i)));
-        }
-    }
-    m = wave_max_all(m);
-    const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
-    if (lane == 0) a.dfac[t] = pow2(-e);
-}
-
 struct DyArgs {
-    const void* dy;
-    int dy_dt, tokens, vec;
-    int64_t rows, row0;  // row0: the piece's first
-    const float* sc;     // turned order
-    const uint32_t* amax;
+    Upstream up;
+    int64_t row0;     // the piece's first
+    const float* sc;
+    RowTop amax;
     const float* dfac;
-    half8_t* p;          // [tp / 16][vkt][64]
+    half8_t* p;       // [tp / 16][vkt][64]
     int vkt;
 };
-// The panel of dy * scale * 2^-e in the order of the columns' panel: 16 tokens
-// by 256 rows a workgroup, through LDS (an operand's 8 values lie 4 apart).
-constexpr int DY_ROWS = 256, DY_LD = DY_ROWS + 4;
+// The panel of dy * scale * 2^-e in the order of the columns' panel (chunk_row):
+// two runs of 4 rows a lane.  A wave 4 k tiles of 16 tokens.
 __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 {
-    __shared__ __align__(16) float s_dy[16][DY_LD];
-    const int tid = threadIdx.x, tile = blockIdx.x, k0 = blockIdx.y * (DY_ROWS / 32);
-    const int64_t r0 = a.row0 + k0 * 32;
-    if (a.vec) {
+    constexpr int N = 4;
+    const int lane = threadIdx.x & 63, q = lane >> 4, tile = blockIdx.x, t = tile * 16 + (lane & 15);
+    const int k0 = ((int)blockIdx.y * 4 + (threadIdx.x >> 6)) * N;
+    const float f = a.dfac[t] * pow2(-scale_exponent(a.amax));
+    f32x4_t v[N][2], s[N][2];
+    if (a.up.vec) {
+        u32x2 w[N][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int f = tid + 256 * i, r = f / 32, c = f % 32 * 8, t = tile * 16 + r;
-            Eight e = {{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}};
-            if (t < a.tokens && r0 + c < a.rows) e = load8(a.dy, a.dy_dt, t * a.rows + r0 + c);
-            *(f32x4_t*)&s_dy[r][c] = f32x4_t{e.v[0], e.v[1], e.v[2], e.v[3]};
-            *(f32x4_t*)&s_dy[r][c + 4] = f32x4_t{e.v[4], e.v[5], e.v[6], e.v[7]};
-        }
+        for (int i = 0; i < 2 * N; i++) w[i / 2][i % 2] = a.up.raw(t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
+#pragma unroll
+        for (int i = 0; i < 2 * N; i++)
+            v[i / 2][i % 2] = a.up.numbers(w[i / 2][i % 2], t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int t = tile * 16 + r;
-            s_dy[r][tid] = t < a.tokens && r0 + tid < a.rows ? load_as_f32(a.dy, a.dy_dt, t * a.rows + r0 + tid) : 0.0f;
-        }
+        for (int i = 0; i < 2 * N; i++) v[i / 2][i % 2] = a.up.slow(t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
     }
-    __syncthreads();
-    const int lane = tid & 63, c = lane >> 4, r = lane & 15;
-    const float f = a.dfac[tile * 16 + r] * pow2(-scale_exponent(*a.amax));
 #pragma unroll
-    for (int i = 0; i < DY_ROWS / 32 / 4; i++) {
-        const int k = (tid >> 6) + 4 * i;
-        if (k0 + k >= a.vkt) break;
+    for (int i = 0; i < 2 * N; i++) s[i / 2][i % 2] = *(const f32x4_t*)(a.sc + a.row0 + min(k0 + i / 2, a.vkt - 1) * 32 + i % 2 * 16 + q * 4);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (k0 + i >= a.vkt) break;
         half8_t h;
 #pragma unroll
-        for (int m = 0; m < 8; m++) {
-            const int col = k * 32 + 16 * (m >> 2) + 4 * (m & 3) + c;
-            h[m] = (_Float16)(s_dy[r][col] * (a.sc[r0 + k * 32 + 16 * (m >> 2) + 4 * c + (m & 3)] * f));
-        }
-        a.p[((int64_t)tile * a.vkt + k0 + k) * 64 + lane] = h;
+        for (int m = 0; m < 8; m++) h[m] = (_Float16)(v[i][m >> 2][m & 3] * (s[i][m >> 2][m & 3] * f));
+        a.p[((int64_t)tile * a.vkt + k0 + i) * 64 + lane] = h;
     }
 }
 
@@ -826,17 +1004,16 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 //
 // k tiles in groups of 8: lane q takes the groups 8 q + j (j = tile of the 8)
 // of 32, so its 8 codes are one load, and the tokens' operand is read from
-// there, too.  Up to 16 tokens are read as they are (no packing launch): a wave
+// there, too.  Up to 4 tokens are read as they are (no launch before): a wave
 // brings its share of a token's row to fp16 under a power of two of its own.
 struct FewArgs {
     MatArgs m;
     int64_t pairs;
-    const half8_t* xp;  // packed tokens (TT > 1)
+    const half8_t* xp;  // packed tokens
     const float* fac;
-    const void* x;      // TT == 1
+    const void* x;      // OWN: 16-bit rows as they are
     int x_dt;
-    const float* x_scale;
-    int tokens, n;
+    int tokens, n;  // tokens of the chunk; workgroups (., y) take 16 TT of them from 16 TT y on
     float rs;
 };
 
@@ -855,26 +1032,31 @@ __device__ __forceinline__ half8_t centroid_f16(half8_t h)
     return h;
 }
 
-template <int CBT, int S2, int TT, int KW, class Epi>
-__global__ void __launch_bounds__(256, TT == 8 ? 2 : 3) few_kernel(const FewArgs a, Epi epi)
+template <int CBT, int S2, int TT, int KW, bool OWN, class Epi>
+__global__ void __launch_bounds__(256, TT == 8 || OWN ? 2 : 3) few_kernel(const FewArgs a, Epi epi)
 {
-    static_assert(KW == 4 || KW == 1, "");
+    static_assert((KW == 4 || KW == 1) && (!OWN || (TT == 1 && KW == 4)), "");
     constexpr int JU = S2 == VQ2_S2_NONE && TT <= 4 ? 8 : 4;  // k tiles whose centroids are on their way together
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, nl = lane & 15;
-    const int64_t pair = KW == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-    if (KW == 1 && pair >= a.pairs) return;
+    const int tok0 = blockIdx.y * (16 * TT), left = a.tokens - tok0;
     const int ng = a.m.ng, kt = ng / 4, sups = (ng + 31) / 32, part = KW == 4 ? wave : 0;
     const int s0 = sups * part / KW, s1 = sups * (part + 1) / KW;
+    const half8_t* xp = a.xp + (int64_t)(tok0 / 16) * kt * 64;
+    const int64_t step = (int64_t)gridDim.x * (4 / KW);
+    int64_t pair = KW == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     const int16_t* p0[2];
     const char* p1[2];
     constexpr int B1 = S2 == VQ2_S2_U8 ? 1 : 2;
+    auto set_pair = [&] {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        int mat;
-        const int64_t row = mat_row(a.m, 2 * pair + i, nl, mat), off = (row < a.m.rows ? row : 0) * ng;
-        p0[i] = a.m.m[mat].i0 + off;
-        p1[i] = S2 == VQ2_S2_NONE ? nullptr : (const char*)a.m.m[mat].i1 + off * B1;
-    }
+        for (int i = 0; i < 2; i++) {
+            int mat;
+            const int64_t row = mat_row(a.m, 2 * min(pair, a.pairs - 1) + i, nl, mat), off = (row < a.m.rows ? row : 0) * ng;
+            p0[i] = a.m.m[mat].i0 + off;
+            p1[i] = S2 == VQ2_S2_NONE ? nullptr : (const char*)a.m.m[mat].i1 + off * B1;
+        }
+    };
+    set_pair();
     struct Codes {
         u32x4 a[2], b[S2 == VQ2_S2_NONE ? 1 : 2];
     };
@@ -893,37 +1075,68 @@ __global__ void __launch_bounds__(256, TT == 8 ? 2 : 3) few_kernel(const FewArgs
     };
     auto code = [](const u32x4& w, int j) { return w[j >> 1] >> (16 * (j & 1)) & 0xFFFFu; };
     Codes cur, next;
-    load_codes(s0, cur);
+    load_codes(min(s0, sups - 1), cur);
 
     // the tokens of a wave that reads them itself: their largest values first
     float up = 1.0f, down = 1.0f;  // 2^e, 2^-e of token nl
-    const bool own = TT == 1;
-    if (own && a.x_dt <= VQ2_DT_BF16) {
+    auto raw_x = [&](int s, u32x4 (&w)[8]) {  // 16-bit values of token nl, the lane's 8 groups
+        const int g = s * 32 + q * 8 < ng ? s * 32 + q * 8 : 0;
+        const u32x4* p = (const u32x4*)((const uint16_t*)a.x + (int64_t)min(nl, a.tokens - 1) * a.n + g * 8);
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = p[j];
+    };
+    auto eight = [&](const u32x4& w) {
+        Eight e;
+        if (a.x_dt == VQ2_DT_F16) {
+            const half8_t h = __builtin_bit_cast(half8_t, w);
+#pragma unroll
+            for (int k = 0; k < 8; k++) e.v[k] = (float)h[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                e.v[2 * k] = __uint_as_float(w[k] << 16);
+                e.v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+            }
+        }
+        return e;
+    };
+    u32x4 xw[OWN ? 8 : 1];
+    if constexpr (OWN) {
         float m = 0.0f;
-        if (nl < a.tokens)
-            for (int s = s0; s < s1; s++)
-                if (s * 32 + q * 8 < ng)
+        for (int s = s1 - 1; s >= s0; s--) {  // the first last: it is used first
+            raw_x(s, xw);
+            if (s * 32 + q * 8 < ng)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const Eight e = load8(a.x, a.x_dt, (int64_t)nl * a.n + (s * 32 + q * 8 + j) * 8);
+                for (int j = 0; j < 8; j++) {
+                    const Eight e = eight(xw[j]);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
-                    }
+                    for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(e.v[k]));
+                }
+        }
         m = max_rows(m);
         const int e = m > 0.0f ? min(max(exponent_of(m) - 13, -110), 110) : 0;
         up = pow2(e);
         down = pow2(-e);
     }
 
+    const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
+    constexpr int TS = KW == 4 ? (TT + 3) / 4 : TT;  // token tiles that this wave finishes: wave, wave + 4, ...
+    typename Epi::State state[TS];
+    for (; pair < a.pairs;) {
     f32x4_t acc[2][TT];
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int j = 0; j < TT; j++) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int s = s0; s < s1; s++) {
         const bool ok = s * 32 + q * 8 < ng;
-        load_codes(s + 1, next);
+        if constexpr (OWN)
+            if (s1 - s0 > 1) raw_x(s, xw);
+        if (s + 1 == s1) {  // the next pair's first codes
+            pair += step;
+            set_pair();
+        }
+        load_codes(s + 1 == s1 ? s0 : s + 1, next);
 #pragma unroll
         for (int j0 = 0; j0 < 8; j0 += JU) {
             half8_t w0[2][JU], w1[2][S2 == VQ2_S2_NONE ? 1 : JU];
@@ -940,16 +1153,13 @@ __global__ void __launch_bounds__(256, TT == 8 ? 2 : 3) few_kernel(const FewArgs
             for (int u = 0; u < JU; u++) {
                 const int g = ok ? s * 32 + q * 8 + j0 + u : 0;
                 half8_t b[TT];
-                if constexpr (TT == 1) {
-                    b[0] = zero;
-                    if (nl < a.tokens) {
-                        const Eight e = load8(a.x, a.x_dt, (int64_t)nl * a.n + g * 8);
+                if constexpr (OWN) {
+                    const Eight e = eight(xw[j0 + u]);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) b[0][k] = (_Float16)(e.v[k] * down);
-                    }
+                    for (int k = 0; k < 8; k++) b[0][k] = (_Float16)(e.v[k] * down);
                 } else {
 #pragma unroll
-                    for (int t = 0; t < TT; t++) b[t] = a.xp[((int64_t)t * kt + (g >> 2)) * 64 + (g & 3) * 16 + nl];
+                    for (int t = 0; t < TT; t++) b[t] = xp[((int64_t)t * kt + (g >> 2)) * 64 + (g & 3) * 16 + nl];
                 }
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
@@ -967,34 +1177,45 @@ __global__ void __launch_bounds__(256, TT == 8 ? 2 : 3) few_kernel(const FewArgs
         }
         cur = next;
     }
+    const int64_t done = s1 > s0 ? pair - step : pair;
     if constexpr (KW == 4) {
+        if (s1 <= s0) pair += step;  // (a wave without k tiles: rows below 128 values)
         __shared__ f32x4_t s_acc[4][2 * TT][64];
+        __syncthreads();  // the last pair's have been read
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int t = 0; t < TT; t++) s_acc[wave][i * TT + t][lane] = acc[i][t] * up;
         __syncthreads();
-        for (int t = wave; t < TT; t += 4) {
-            if (t * 16 >= a.tokens) break;
+#pragma unroll
+        for (int k = 0; k < TS; k++) {
+            const int t = wave + 4 * k;
+            if (t >= TT || t * 16 >= left) break;
             f32x4_t o[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 o[i] = s_acc[0][i * TT + t][lane];
 #pragma unroll
-                for (int k = 1; k < 4; k++) o[i] += s_acc[k][i * TT + t][lane];
+                for (int w = 1; w < 4; w++) o[i] += s_acc[w][i * TT + t][lane];
             }
-            const int tok = t * 16 + nl;
-            const float f = own ? (a.x_scale && tok < a.tokens ? a.x_scale[tok] : 1.0f) : a.fac[tok];
-            epi.few(a.m, a.rs, o[0] * f, o[1] * f, pair, tok);
+            const int tok = tok0 + t * 16 + nl;
+            const float f = OWN ? 1.0f : a.fac[tok];
+            epi.few(state[k], a.m, a.rs, o[0] * f, o[1] * f, done, tok);
         }
     } else {
 #pragma unroll
         for (int t = 0; t < TT; t++) {
-            if (t * 16 >= a.tokens) break;
-            const int tok = t * 16 + nl;
+            if (t * 16 >= left) break;
+            const int tok = tok0 + t * 16 + nl;
             const float f = a.fac[tok];
-            epi.few(a.m, a.rs, acc[0][t] * f, acc[1][t] * f, pair, tok);
+            epi.few(state[t], a.m, a.rs, acc[0][t] * f, acc[1][t] * f, done, tok);
         }
+    }
+    }
+#pragma unroll
+    for (int k = 0; k < TS; k++) {
+        const int t = KW == 4 ? wave + 4 * k : k;
+        if (t < TT && t * 16 < left) epi.few_end(state[k], KW == 4 ? blockIdx.x : blockIdx.x * 4 + wave, tok0 + t * 16 + nl);
     }
 }
 
@@ -1049,39 +1270,27 @@ struct DxArgs {
     const float* part;  // [slices][tp][np]
     int slices, tp, n;
     int64_t np;
-    const uint32_t* amax;
-    const float* dfac;      // the panel's factors, or null: the loss's
-    const float* dloss;
-    const int64_t* target;
-    int64_t rows, ignore;
+    DxFactor fac;
     void* dx;
     int dx_dt;
 };
 __global__ void __launch_bounds__(256) dx_kernel(const DxArgs a)
 {
     const int t = blockIdx.y, i = ((int)blockIdx.x * 256 + threadIdx.x) * 4;
+    DxFactor fac = a.fac;
+    fac.init();
     if (i >= a.n) return;
-    const int es = scale_exponent(*a.amax);
-    float f, g = 1.0f;
-    bool skip = false;
-    if (a.dfac) {
-        f = pow2(es);
-        g = 1.0f / a.dfac[t];
-    } else {
-        const int64_t v = target_of(a.target, t, a.ignore, a.rows);
-        skip = v == TARGET_SKIP;
-        f = pow2(es - 14);
-        g = v == TARGET_BAD ? __builtin_nanf("") : a.dloss[t];
-    }
+    bool skip;
+    const float f = fac.of(t, skip);
     f32x4_t v = *(const f32x4_t*)(a.part + (int64_t)t * a.np + i);
     for (int z = 1; z < a.slices; z++) v += *(const f32x4_t*)(a.part + ((int64_t)z * a.tp + t) * a.np + i);
 #pragma unroll
-    for (int k = 0; k < 4; k++) store_from_f32(a.dx, a.dx_dt, (int64_t)t * a.n + i + k, skip ? 0.0f : v[k] * f * g);
+    for (int k = 0; k < 4; k++) store_from_f32(a.dx, a.dx_dt, (int64_t)t * a.n + i + k, fac.apply(v[k], f, skip));
 }
 
 struct DsArgs {
     MatArgs m;
-    const float* part;  // [chunks][ld] in turned order
+    const float* part;  // [chunks][ld]
     int chunks;
     int64_t ld;
     float rs;
@@ -1101,7 +1310,7 @@ __global__ void __launch_bounds__(256) ds_kernel(const DsArgs a)
     __syncthreads();
     if (y) return;
     int mat;
-    const int64_t row = mat_row(a.m, p >> 4, turned((int)(p & 15)), mat);
+    const int64_t row = mat_row(a.m, p >> 4, (int)(p & 15), mat);
     if (row >= a.m.rows) return;
 #pragma unroll
     for (int k = 1; k < 8; k++) s += s_s[k][x];
@@ -1132,21 +1341,62 @@ struct Bump {
 // panel of gradients (2 bytes a token and row) stays near PIECE_BYTES.
 constexpr int64_t PANEL_TOKENS = 8192;
 constexpr int64_t PIECE_BYTES = 128 << 20;
-constexpr int64_t PIECE_MAX_ROWS = 16384, PIECE_MIN_ROWS = 4096;
+constexpr int64_t PIECE_MAX_ROWS = 16384, PIECE_MIN_ROWS = 4096, PIECE_FORWARD_ROWS = 32768;
 
-// up to here few_kernel; 128 tokens of a 151936 x 2048 head: @@FEW@@
-constexpr int FEW_TOKENS = 128;
+// few_kernel: up to here it reads 16-bit rows as they are.  A lane's 8 loads are
+// a line each; 16 tokens of a 151936-row head took 245 us so, 48 packed ones 215.
+bool few_own(int64_t tokens, int x_dt) { return tokens <= 4 && x_dt <= VQ2_DT_BF16; }
+
+int64_t few_pairs(const PanelCall& c) { return ((c.rows + 15) / 16 * c.nmat + 1) / 2; }
+
+// Its token tiles a workgroup.  128 tokens at once, for which a wave has its
+// rows to itself, only where the rows are many (65 to 128 tokens of 151936 rows: 260 us,
+// 64 at a time 430; of 512 + 512 rows 66, 64 at a time 23).
+int few_tiles(const PanelCall& c, int64_t tokens)
+{
+    if (tokens <= 32) return tokens <= 16 ? 1 : 2;
+    return tokens > 64 && tokens <= 128 && few_pairs(c) >= 1024 ? 8 : 4;
+}
+
+// and its workgroups along the pairs of tiles: for the loss as many as are
+// resident, each keeps running sums over its pairs.
+int few_groups(const PanelCall& c, int64_t tokens)
+{
+    const int tt = few_tiles(c, tokens);
+    const int64_t units = tt == 8 ? (few_pairs(c) + 3) / 4 : few_pairs(c);
+    if (c.what != PANEL_STATS) return (int)units;
+    return (int)std::min<int64_t>(units, (int64_t)device_cu_count() * (tt == 8 || few_own(tokens, c.x_dt) ? 2 : 3));
+}
+
+// Whether few_kernel is ahead of panels: it gathers every centroid once for
+// each block of tokens, panels once, but they store and read it again, and take two
+// launches more.  Times of both (us; rows x n, bits, tokens: few / panels):
+// @@FEW@@
+bool few_ahead(const PanelCall& c, int64_t tokens)
+{
+    if (c.cb_dt == VQ2_DT_F32) return false;  // (its centroids would take two products each)
+#ifdef FORCE_FEW
+    return FORCE_FEW && tokens <= 2048;
+#endif
+    const double gathers = (double)c.rows * c.nmat * (double)(c.n / 8) * (c.s2 == VQ2_S2_U16 ? 2 : 1);
+    const int tt = few_tiles(c, tokens);
+    const double blocks = tt == 8 ? 1.4 : (double)((tokens + 63) / 64);
+    return blocks <= 1.5 || blocks * (gathers + 3e4) <= 1.5 * gathers + 2.5e6;
+}
 
 struct Plan {
     int64_t chunk;       // tokens of a chunk (the last may be shorter)
     int64_t tp;          // of them, padded
     int64_t tiles;       // 16-row tiles of all matrices, padded to whole workgroups
     int64_t piece;       // tiles of a piece
-    bool few;            // few_kernel
+    bool direct;         // the gradient's product writes dx
+    bool few[2];         // few_kernel for a whole chunk, and for the last one
+    int mt, gmt;         // tiles of a wave: the first product's, the gradient's
+    int tops;            // workgroups of prep_scales
     int parts, tparts, kt;  // parts of a weight in the rows' panel, and the columns'
     int64_t np;          // columns, padded
     int slices;
-    size_t fac, amax, sc, xp, w, wt, p, acc, stats, at, ds, dfac, total;
+    size_t fac, top, sc, xp, w, wt, p, acc, stats, at, ds, dfac, total;
 };
 
 enum { STATS = PANEL_STATS, DLOGIT = PANEL_DLOGIT, GATED = PANEL_GATED, DGATED = PANEL_DGATED, PRODUCT = PANEL_PRODUCT };
@@ -1159,38 +1409,50 @@ Plan plan_of(const PanelCall& c)
     p.tp = up(p.chunk, PG_N);
     p.tiles = up((c.rows + 15) / 16 * c.nmat, pg_m(8) / 16);
     p.kt = (int)(c.n / 32);
-    // (codes are loaded 8 at a time; fp32 centroids would take two products each)
-    p.few = !grad && c.tokens <= FEW_TOKENS && c.cb_dt != VQ2_DT_F32;
+    // (each chunk as a call of its own would take it)
+    const int64_t rest = c.tokens % p.chunk;
+    p.few[0] = !grad && few_ahead(c, p.chunk);
+    p.few[1] = rest ? !grad && few_ahead(c, rest) : p.few[0];
     const bool exact = c.cb_dt != VQ2_DT_F32 && c.s2 == VQ2_S2_NONE;
     const bool fine = c.y_dt != VQ2_DT_BF16;
     const bool wide = c.what == STATS || c.what == DLOGIT || c.ds[0] != nullptr || fine;
     p.parts = !exact && wide ? 2 : 1;
     p.tparts = !exact && fine ? 2 : 1;
-    int64_t rows = PIECE_MAX_ROWS;
+    int64_t rows = grad ? PIECE_MAX_ROWS : PIECE_FORWARD_ROWS;
     while (grad && rows > PIECE_MIN_ROWS && rows * p.tp * 2 > PIECE_BYTES) rows /= 2;
     p.piece = std::min(p.tiles, rows / 16);
     p.np = up(c.n, pg_m(8));
     p.slices = 1;
+    // Wave tiles of 128 rows, two workgroups a CU, where that many are there;
+    // of 64 otherwise, which keep up with them three a CU.
+    const int64_t slots = 2 * (int64_t)device_cu_count();
+    p.mt = p.piece * 16 / pg_m(8) * (p.tp / PG_N) >= slots ? 8 : 4;
     Bump b;
     p.fac = b.take(p.tp * 4);
-    p.amax = b.take(4);
+    p.tops = (int)((p.tiles * 16 + PREP_ROWS - 1) / PREP_ROWS);
+    p.top = b.take(p.tops * 4);
     p.sc = b.take(p.tiles * 16 * 4);
     p.xp = b.take(p.tp * c.n * 2);
-    const bool w = c.what != PRODUCT || c.ds[0];
+    const bool w = c.what != PRODUCT || c.ds[0];  // (also where few_kernel is ahead: it needs aligned planes)
     p.w = b.take(w ? p.piece * 16 * c.n * 2 * p.parts : 0);
     if (grad) {
         p.wt = b.take(p.piece * 16 * p.np * 2 * p.tparts);
         p.p = b.take(p.piece * 16 * p.tp * 2);
-        // as many slices of a piece's rows as fill the device
-        const int64_t wg = p.np / pg_m(8) * (p.tp / PG_N);
-        const int64_t most = std::max<int64_t>(1, p.piece / 2 / 16);
-        while (p.slices < 64 && wg * p.slices < 512 && p.slices * 2 <= most) p.slices *= 2;
-        p.acc = b.take(p.slices * p.tp * p.np * 4);
+        // As few slices of a piece's rows as fill the device (each adds a pass
+        // over the sums), of at least 8 k tiles.
+        const int64_t wg = p.np / pg_m(8) * (p.tp / PG_N), most = std::max<int64_t>(1, p.piece / 2 / 8);
+        // One piece in one slice is written as dx at once.
+        const bool one = p.piece == p.tiles;
+        p.gmt = wg >= slots || (2 * wg >= slots && !one) ? 8 : 4;
+        while (p.slices < 64 && wg * (8 / p.gmt) * p.slices < slots && p.slices * 2 <= most) p.slices *= 2;
+        p.direct = one && p.slices == 1;
+        p.acc = b.take(p.direct ? 0 : p.slices * p.tp * p.np * 4);
         if (c.ds[0]) p.ds = b.take(p.tp / (16 * PG_NT) * p.tiles * 16 * 4);
         if (c.what != DLOGIT) p.dfac = b.take(p.tp * 4);
     }
     if (c.what == STATS) {
-        p.stats = b.take(p.tiles / 2 * p.tp * 8);  // parts of 32 rows (few tokens) or 128
+        // parts: a wave's rows, or (few_kernel) a workgroup's, or a wave's
+        p.stats = b.take(std::max<int64_t>(p.tiles / 4, p.few[0] || p.few[1] ? 12 * device_cu_count() : 0) * p.tp * 8);
         p.at = b.take(p.tp * 4);
     }
     p.total = b.at;
@@ -1198,7 +1460,7 @@ Plan plan_of(const PanelCall& c)
 }
 
 template <int MT, class Epi>
-hipError_t gemm(const PanelGemmArgs& g, const Epi& e, int64_t tile0, hipStream_t st)
+hipError_t gemm_typed(const PanelGemmArgs& g, const Epi& e, int64_t tile0, hipStream_t st)
 {
     static std::once_flag once;
     static hipError_t attr = hipSuccess;
@@ -1212,6 +1474,15 @@ hipError_t gemm(const PanelGemmArgs& g, const Epi& e, int64_t tile0, hipStream_t
     return hipGetLastError();
 }
 
+// rows of panel a in g.gm * pg_m(8)
+template <class Epi>
+hipError_t gemm(PanelGemmArgs g, int mt, const Epi& e, int64_t tile0, hipStream_t st)
+{
+    if (mt == 8) return gemm_typed<8>(g, e, tile0, st);
+    g.gm *= 2;
+    return gemm_typed<4>(g, e, tile0, st);
+}
+
 template <int CBT, int S2, int WP, int TP>
 hipError_t dequant_parts(const DequantArgs& a, int64_t tiles, hipStream_t st)
 {
@@ -1219,7 +1490,7 @@ hipError_t dequant_parts(const DequantArgs& a, int64_t tiles, hipStream_t st)
         hipLaunchKernelGGL((dequant_plain_kernel<CBT, S2, WP>), dim3((unsigned)(tiles / 4), (unsigned)((a.m.ng / 4 + 7) / 8)),
                            dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((dequant_turned_kernel<CBT, S2, WP, TP>), dim3((unsigned)(tiles / 8), (unsigned)((a.m.ng + 15) / 16)),
+        hipLaunchKernelGGL((dequant_both_kernel<CBT, S2, WP, TP>), dim3((unsigned)(tiles / 8), (unsigned)((a.m.ng + 15) / 16)),
                            dim3(256), 0, st, a);
     return hipGetLastError();
 }
@@ -1256,27 +1527,28 @@ hipError_t dequant(const DequantArgs& a, int cb_dt, int s2, int wp, int tp, int6
 }
 
 template <int CBT, int S2, class Epi>
-hipError_t few_typed(const FewArgs& a, const Epi& e, hipStream_t st)
+hipError_t few_typed(const FewArgs& a, const Epi& e, int tt, int groups, hipStream_t st)
 {
-    const dim3 one((unsigned)a.pairs), four((unsigned)((a.pairs + 3) / 4)), block(256);
-    if (a.tokens <= 16) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, Epi>), one, block, 0, st, a, e);
-    else if (a.tokens <= 32) hipLaunchKernelGGL((few_kernel<CBT, S2, 2, 4, Epi>), one, block, 0, st, a, e);
-    else if (a.tokens <= 64) hipLaunchKernelGGL((few_kernel<CBT, S2, 4, 4, Epi>), one, block, 0, st, a, e);
-    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, Epi>), four, block, 0, st, a, e);
+    const dim3 grid((unsigned)groups, (unsigned)((a.tokens + 16 * tt - 1) / (16 * tt))), block(256);
+    if (tt == 1 && few_own(a.tokens, a.x_dt)) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, true, Epi>), grid, block, 0, st, a, e);
+    else if (tt == 1) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, false, Epi>), grid, block, 0, st, a, e);
+    else if (tt == 2) hipLaunchKernelGGL((few_kernel<CBT, S2, 2, 4, false, Epi>), grid, block, 0, st, a, e);
+    else if (tt == 4) hipLaunchKernelGGL((few_kernel<CBT, S2, 4, 4, false, Epi>), grid, block, 0, st, a, e);
+    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, false, Epi>), grid, block, 0, st, a, e);
     return hipGetLastError();
 }
 
 template <class Epi>
-hipError_t few(const FewArgs& a, const Epi& e, int cb_dt, int s2, hipStream_t st)
+hipError_t few(const FewArgs& a, const Epi& e, int tt, int groups, int cb_dt, int s2, hipStream_t st)
 {
     if (cb_dt == VQ2_DT_F16) {
-        if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_F16, VQ2_S2_NONE>(a, e, st);
-        if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_F16, VQ2_S2_U8>(a, e, st);
-        return few_typed<VQ2_DT_F16, VQ2_S2_U16>(a, e, st);
+        if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_F16, VQ2_S2_NONE>(a, e, tt, groups, st);
+        if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_F16, VQ2_S2_U8>(a, e, tt, groups, st);
+        return few_typed<VQ2_DT_F16, VQ2_S2_U16>(a, e, tt, groups, st);
     }
-    if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_BF16, VQ2_S2_NONE>(a, e, st);
-    if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_BF16, VQ2_S2_U8>(a, e, st);
-    return few_typed<VQ2_DT_BF16, VQ2_S2_U16>(a, e, st);
+    if (s2 == VQ2_S2_NONE) return few_typed<VQ2_DT_BF16, VQ2_S2_NONE>(a, e, tt, groups, st);
+    if (s2 == VQ2_S2_U8) return few_typed<VQ2_DT_BF16, VQ2_S2_U8>(a, e, tt, groups, st);
+    return few_typed<VQ2_DT_BF16, VQ2_S2_U16>(a, e, tt, groups, st);
 }
 
 }  // namespace
@@ -1303,14 +1575,14 @@ int panel_launch(const PanelCall& c)
         return VQ2_OK;
     }
     const Plan p = plan_of(c);
-    bool few_call = p.few;
-    for (int k = 0; k < c.nmat; k++)
-        few_call = few_call && (uintptr_t)c.mat[k].i0 % 16 == 0 && (uintptr_t)c.mat[k].i1 % 16 == 0;
+    bool aligned = true;  // (rows are n / 8 codes, a multiple of 8)
+    for (int k = 0; k < c.nmat; k++) aligned = aligned && (uintptr_t)c.mat[k].i0 % 16 == 0 && (uintptr_t)c.mat[k].i1 % 16 == 0;
     char* ws = (char*)c.workspace;
     const bool grad = c.what == DLOGIT || c.what == DGATED || c.what == PRODUCT;
     const bool first = c.what != PRODUCT || c.ds[0];  // the product of weights and tokens
     float* fac = (float*)(ws + p.fac);
-    uint32_t* amax = (uint32_t*)(ws + p.amax);
+    float* top = (float*)(ws + p.top);
+    const RowTop amax{top, p.tops};
     float* sc = (float*)(ws + p.sc);
     half8_t* xp = (half8_t*)(ws + p.xp);
     half8_t* w = first ? (half8_t*)(ws + p.w) : nullptr;
@@ -1319,22 +1591,30 @@ int panel_launch(const PanelCall& c)
     float* acc = (float*)(ws + p.acc);
     float* ds = c.ds[0] ? (float*)(ws + p.ds) : nullptr;
     float* dfac = (float*)(ws + p.dfac);
+    bool prepared = false;  // the row scales
     const int64_t xsize = c.x_dt == VQ2_DT_F32 ? 4 : c.x_dt <= VQ2_DT_BF16 ? 2 : 1;
     for (int64_t t0 = 0; t0 < c.tokens; t0 += p.chunk) {
         const int tokens = (int)std::min(p.chunk, c.tokens - t0);
         const int tp = (int)up(tokens, PG_N);
         const int64_t ds_ld = p.tiles * 16;
+        const bool few_call = aligned && p.few[tokens < p.chunk];
         const void* dy = c.dy ? (const char*)c.dy + t0 * c.rows * dt_size(c.dy_dt) : nullptr;
         const int64_t* target = c.target ? c.target + t0 : nullptr;
-        if (few_call && tokens <= 16) {
-            // (few_kernel reads the rows itself)
-        } else if (first) {
-            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)(tp / 16)), dim3(64 * PK_WAVES), 0, st,
-                               PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
-                                        c.x_scale ? c.x_scale + t0 : nullptr, xp, fac, t0 == 0 ? amax : nullptr});
-            TRY(hipGetLastError());
-        } else if (t0 == 0) {
-            hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(256), 0, st, (float*)amax, (int64_t)1);
+        const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;
+        void* dx = c.y && grad ? (char*)c.y + t0 * c.n * dt_size(c.y_dt) : nullptr;
+        const DxFactor dxf{amax, c.what == DLOGIT ? nullptr : dfac, c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore, 0.0f};
+        const Upstream upstream{dy, c.dy_dt, tokens,
+                                c.dy_dt != VQ2_DT_F32 && c.rows % 4 == 0 && (uintptr_t)dy % 8 == 0, c.rows};
+        const bool prep = !few_call && !prepared;
+        prepared = prepared || prep;
+        const PrologueArgs pro{
+            PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n, c.x_scale ? c.x_scale + t0 : nullptr, xp, fac,
+                     first && !(few_call && few_own(tokens, c.x_dt)) ? tp / 16 : 0},
+            DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, c.what == DGATED ? 19 : 0, dfac,
+                      c.what == DGATED || c.what == PRODUCT ? tp / 16 : 0},
+            PrepArgs{mats, c.rs, ds_ld, sc, top, prep ? p.tops : 0}};
+        if (const int groups = pro.pack.tiles + pro.dy.groups + pro.prep.groups) {
+            hipLaunchKernelGGL(prologue_kernel, dim3((unsigned)groups), dim3(64 * PK_WAVES), 0, st, pro);
             TRY(hipGetLastError());
         }
         auto lse_launch = [&](int64_t chunks) {
@@ -1344,63 +1624,54 @@ int panel_launch(const PanelCall& c)
             return hipGetLastError();
         };
         const StatsEpi stats{sc, fac, target, c.rows, c.ignore, tokens, tp, (f32x2_t*)(ws + p.stats), (float*)(ws + p.at)};
-        const GatedEpi gated{sc, fac, c.y ? (char*)c.y + t0 * c.rows * dt_size(c.y_dt) : nullptr, c.y_dt, tokens, c.rows,
+        const GatedEpi gated{sc, fac, c.y && !grad ? (char*)c.y + t0 * c.rows * dt_size(c.y_dt) : nullptr, c.y_dt, tokens, c.rows,
                              c.rows % 4 == 0 && (uintptr_t)c.y % 16 == 0, c.act};
         if (few_call) {
-            const FewArgs f{mats, ((c.rows + 15) / 16 * c.nmat + 1) / 2, xp, fac, c.x, c.x_dt, c.x_scale, tokens, (int)c.n, c.rs};
+            const FewArgs f{mats, few_pairs(c), xp, fac, (const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
+                            c.rs};
+            const int tt = few_tiles(c, tokens), groups = few_groups(c, tokens);
             if (c.what == GATED) {
-                TRY(few(f, gated, c.cb_dt, c.s2, st));
+                TRY(few(f, gated, tt, groups, c.cb_dt, c.s2, st));
             } else {
-                TRY(few(f, stats, c.cb_dt, c.s2, st));
-                TRY(lse_launch(f.pairs));
+                TRY(few(f, stats, tt, groups, c.cb_dt, c.s2, st));
+                TRY(lse_launch(tt == 8 ? groups * 4 : groups));
             }
             continue;
-        }
-        if (t0 == 0) {
-            hipLaunchKernelGGL(prep_kernel, dim3((unsigned)((ds_ld + 255) / 256)), dim3(256), 0, st,
-                               PrepArgs{mats, c.rs, grad ? 1 : 0, ds_ld, sc, grad ? amax : nullptr});
-            TRY(hipGetLastError());
-        }
-        const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;
-        if (c.what == DGATED || c.what == PRODUCT) {
-            hipLaunchKernelGGL(dy_max_kernel, dim3((unsigned)(tp / 4)), dim3(256), 0, st,
-                               DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, c.what == DGATED ? 19 : 0, dfac});
-            TRY(hipGetLastError());
         }
         for (int64_t tile0 = 0; tile0 < p.tiles; tile0 += p.piece) {
             const int64_t tiles = std::min(p.piece, p.tiles - tile0);
             const int vkt = (int)(tiles / 2);
-            TRY(dequant(DequantArgs{mats, tile0, w, wt, vkt}, c.cb_dt, c.s2, w ? p.parts : 0, wt ? p.tparts : 0, tiles, st));
+            TRY(dequant(DequantArgs{mats, tile0, w, wt, vkt, aligned}, c.cb_dt, c.s2, w ? p.parts : 0, wt ? p.tparts : 0, tiles, st));
             const PanelGemmArgs g{w, xp, p.parts * p.kt, p.kt, (int)(tiles * 16 / pg_m(8)), tp / PG_N, 1};
             if (c.what == STATS)
-                TRY((gemm<8>(g, stats, tile0, st)));
+                TRY(gemm(g, p.mt, stats, tile0, st));
             else if (c.what == GATED)
-                TRY((gemm<8>(g, gated, tile0, st)));
+                TRY(gemm(g, p.mt, gated, tile0, st));
             else if (c.what == DLOGIT)
-                TRY((gemm<8>(g, DlogitEpi{sc, fac, c.lse + t0, c.dloss + t0, target, amax, c.rows, c.ignore, tile0, tokens, tp, vkt,
-                                          pp, ds, ds_ld}, tile0, st)));
+                TRY(gemm(g, p.mt, DlogitEpi{sc, fac, c.lse + t0, c.dloss + t0, target, amax, c.rows, c.ignore, tile0, tokens, tp, vkt,
+                                          pp, ds, ds_ld}, tile0, st));
             else if (c.what == DGATED)
-                TRY((gemm<8>(g, DgatedEpi{sc, fac, dfac, dy, amax, c.dy_dt, tokens, tp, vkt, c.rows, tile0, pp, ds, ds_ld, c.act},
-                             tile0, st)));
+                TRY(gemm(g, p.mt, DgatedEpi{sc, fac, dfac, upstream, amax, tp, vkt, tile0, pp, ds, ds_ld, c.act},
+                         tile0, st));
             else if (first)
-                TRY((gemm<8>(g, ColsumEpi{fac, dy, c.dy_dt, tokens, c.rows, ds, ds_ld}, tile0, st)));
+                TRY(gemm(g, p.mt, ColsumEpi{fac, upstream, ds, ds_ld}, tile0, st));
             if (!grad) continue;
             if (c.what == PRODUCT) {
-                hipLaunchKernelGGL(dy_panel_kernel, dim3((unsigned)(tp / 16), (unsigned)((vkt + 7) / 8)), dim3(256), 0, st,
-                                   DyArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, tile0 * 16, sc, amax, dfac, pp, vkt});
+                hipLaunchKernelGGL(dy_panel_kernel, dim3((unsigned)(tp / 16), (unsigned)((vkt + 15) / 16)), dim3(256), 0, st,
+                                   DyArgs{upstream, tile0 * 16, sc, amax, dfac, pp, vkt});
                 TRY(hipGetLastError());
             }
             const int slices = (int)std::min<int64_t>(p.slices, vkt);
             const PanelGemmArgs g2{wt, pp, p.tparts * vkt, vkt, (int)(p.np / pg_m(8)), tp / PG_N, slices};
-            TRY((gemm<8>(g2, GradEpi{acc, p.np, tp, tile0 != 0}, 0, st)));
+            TRY(gemm(g2, p.gmt, GradEpi{acc, p.np, tp, tile0 != 0, p.direct ? dx : nullptr, c.y_dt, tokens, (int)c.n, dxf}, 0, st));
         }
-        if (c.what == STATS) TRY(lse_launch(p.tiles / 8));
+        if (c.what == STATS) TRY(lse_launch(p.tiles / p.mt));
         if (!grad) continue;
-        hipLaunchKernelGGL(dx_kernel, dim3((unsigned)((c.n + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st,
-                           DxArgs{acc, p.slices, tp, (int)c.n, p.np, amax, c.what == DLOGIT ? nullptr : dfac,
-                                  c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore,
-                                  (char*)c.y + t0 * c.n * dt_size(c.y_dt), c.y_dt});
-        TRY(hipGetLastError());
+        if (!p.direct) {
+            hipLaunchKernelGGL(dx_kernel, dim3((unsigned)((c.n + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st,
+                               DxArgs{acc, p.slices, tp, (int)c.n, p.np, dxf, dx, c.y_dt});
+            TRY(hipGetLastError());
+        }
         if (ds) {
             hipLaunchKernelGGL(ds_kernel, dim3((unsigned)(ds_ld / 32)), dim3(256), 0, st,
                                DsArgs{mats, ds, tp / (16 * PG_NT), ds_ld, c.rs, {c.ds[0], c.ds[1]}, t0 != 0});

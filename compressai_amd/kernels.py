@@ -19,7 +19,8 @@ around the packed products and for tuning: vq_add_rms_norm, vq_gated_rows,
 vq_head_loss and their backward passes, vq_gemm_backward.
 
 The entries of the small calls (vq_sorted_gemv, vq_gemv_rht, vq_rows_gemm,
-vq_sorted_moe, vq_router_select, vq_sample) hand the calls without given
+vq_sorted_moe, vq_router_select, vq_sample, vq_add_rms_norm, vq_gated_rows,
+vq_head_loss) hand the calls without given
 outputs to their native twins
 (csrc/vq2_host.cpp: the same checks and launch, ~8 us less host time each),
 which decline whatever the checks here have to look at.
@@ -1706,6 +1707,10 @@ def vq_add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, p
     without a residual; given h, which may be x or residual, it goes there); y is of out_dtype (x's by default), y_scale None.
     out_dtype int8 / float8_e4m3fn: y in 8 bits under y_scale fp32 [rows] (largest magnitude / 127 or 448),
     which vq_gated_rows and vq_head_loss take as x and x_scale."""
+    if h is None:
+        out = _lib.host().add_rms_norm(x, weight, residual, eps, bool(zero_centred), perm, sign, hb, rht_scale, out_dtype)
+        if out is not None:
+            return out
     dev = _dev(x, weight, residual, perm, sign, h)
     n = x.shape[-1]
     _contig(x, "x")
@@ -1799,6 +1804,9 @@ def vq_head_loss(xr, targets, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, x_scal
     against targets int64 [T], in pieces of the vocabulary, the logits never
     kept: (loss fp32 [T], lse fp32 [T]).  A target of ignore_index gives a
     loss of 0, any other outside [0, out) NaN."""
+    res = _lib.host().head_loss(xr, targets, i0, i1, cb0, cb1, scale, int(out), int(n), rs, x_scale, int(ignore_index))
+    if res is not None:
+        return res
     dev = _dev(xr, targets, i0, i1, cb0, cb1, scale, x_scale)
     n, out = int(n), int(out)
     x2, xdt = _panel_x(xr, x_scale, n)
@@ -1868,9 +1876,12 @@ def vq_gated_rows(xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", x_sca
     "gelu_tanh"; both products, the activation and the product of the two in
     one pass, nothing in between stored.  gate, up: (i0, i1 or None, scale),
     of one cfg.  out_dtype: xr's by default, bf16 for 8-bit rows."""
-    dev = _dev(xr, *gate, *up, cb0, cb1, x_scale)
     n = int(n)
     act = _act(activation)
+    y = _lib.host().gated_rows(xr, gate, up, cb0, cb1, n, rs, act, x_scale, out_dtype)
+    if y is not None:
+        return y
+    dev = _dev(xr, *gate, *up, cb0, cb1, x_scale)
     x2, xdt = _panel_x(xr, x_scale, n)
     T = x2.shape[0]
     s2, segs, rows, sdt, _keep = _gated_mats(gate, up, cb0, cb1, n)

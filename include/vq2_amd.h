@@ -768,7 +768,7 @@ int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt
  *   x       [tokens, n] rotated rows, 16-byte aligned: VQ2_DT_F16 / BF16, in forward
  *           calls also VQ2_DT_I8 / VQ2_DT_E4M3 with x_scale [tokens] (NULL otherwise)
  *   n       a multiple of 64 up to VQ2_PANEL_MAX_N; out_rows up to VQ2_PANEL_MAX_ROWS
- *   dx      gradients of x, VQ2_DT_F16 / BF16;  dscale  of the row scales, fp32, or NULL
+ *   dx      gradients of x, VQ2_DT_F16 / BF16, 16-byte aligned;  dscale  of the row scales, fp32, or NULL
  *   workspace  256-byte aligned, of the entry's _workspace bytes (scale_grad:
  *           whether dscale is wanted); contents on entry do not matter
  * Results do not depend on what ran before, and sums have a fixed order. */
