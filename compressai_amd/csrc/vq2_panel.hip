@@ -884,11 +884,27 @@ struct DxFactor {
     }
 };
 
+// 8 (4) neighbouring columns of dx in 16 bits: element e of N tiles' values
+template <int N>
+__device__ __forceinline__ void store_run(void* dx, int dt, int64_t at, const f32x4_t (&v)[N], int e, float f, const DxFactor& fac,
+                                          bool skip)
+{
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float a = fac.apply(v[i][e], f, skip), b = fac.apply(v[i + 1][e], f, skip);
+        w[i / 2] = dt == VQ2_DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : bf16_pair(a, b);
+    }
+    uint32_t* o = (uint32_t*)((uint16_t*)dx + at);
+    if constexpr (N == 8) *(u32x4*)o = u32x4{w[0], w[1], w[2], w[3]};
+    else *(u32x2*)o = u32x2{w[0], w[1]};
+}
+
 // Columns' product, added to what earlier pieces left, or (dx) finished: tile i
 // of the wave holds columns i, 8 + i, ... of its 128 (MT == 8), or of the half
 // of them that starts at tile % 8.
 struct GradEpi {
-    float* out;  // [slices][tp][np]
+    f32x4_t* out;  // as the lanes hold them: [slices][tp / 16][np / 128][8][64] (dx_kernel)
     int64_t np;
     int tp, add;
     void* dx;    // [tokens][n], or null
@@ -911,31 +927,21 @@ struct GradEpi {
                 for (int e = 0; e < 4; e++) {
                     const int64_t col = c0 + (q * 4 + e) * 8;
                     if (col >= n) continue;
-                    uint32_t w[MT / 2];
+                    f32x4_t v[MT];
 #pragma unroll
-                    for (int i = 0; i < MT; i += 2) {
-                        const float a = fac.apply(acc[i][j][e], f, skip), b = fac.apply(acc[i + 1][j][e], f, skip);
-                        w[i / 2] = dx_dt == VQ2_DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : bf16_pair(a, b);
-                    }
-                    uint32_t* o = (uint32_t*)((uint16_t*)dx + (int64_t)t * n + col);
-                    if constexpr (MT == 8) *(u32x4*)o = u32x4{w[0], w[1], w[2], w[3]};
-                    else *(u32x2*)o = u32x2{w[0], w[1]};
+                    for (int i = 0; i < MT; i++) v[i] = acc[i][j];
+                    store_run(dx, dx_dt, (int64_t)t * n + col, v, e, f, fac, skip);
                 }
             }
             return;
         }
+        // (in rows, 16 bytes a lane and line, the loss's 4096 x 2048 sums cost 25
+        // us a piece more)
 #pragma unroll
         for (int j = 0; j < PG_NT; j++) {
-            float* o = out + ((int64_t)bz * tp + tok + j * 16 + nl) * np + c0;
+            f32x4_t* o = out + ((((int64_t)bz * (tp / 16) + (tok >> 4) + j) * (np / 128) + tile / 8) * 8 + tile % 8) * 64 + lane;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int i = 0; i < MT; i += 4) {
-                    f32x4_t v = {acc[i][j][e], acc[i + 1][j][e], acc[i + 2][j][e], acc[i + 3][j][e]};
-                    f32x4_t* a = (f32x4_t*)(o + (q * 4 + e) * 8 + i);
-                    if (add) v += *a;
-                    *a = v;
-                }
+            for (int i = 0; i < MT; i++) o[i * 64] = add ? o[i * 64] + acc[i][j] : acc[i][j];
         }
     }
 };
@@ -994,13 +1000,15 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 }
 
 // ------------------------------------------------------------- few tokens
-// Up to 128 tokens: every centroid is gathered once, straight into the
+// Every centroid is gathered once for up to 128 tokens, straight into the
 // operand it is (lane (row, q): group q of a k tile), and nothing is written in
 // between.  The gathers bound it: 240 G a second over the device, whatever
-// their size (a request of a line each).  A wave takes two tiles of 16 rows
-// (for the block: gate and up).  Up to 64 tokens the 4 waves of a workgroup
-// share the k tiles of one pair and meet in LDS, so that small matrices fill the device;
-// above, each has a pair of its own and they share the tokens' lines.
+// their size (a request of a line each): one token of a 151936 x 2048 head (38.9 M
+// codes, 162 us by them) takes 170 us, of the block of 2 x 6144 x 2048 at 4 bits (6.3 M,
+// 26 us) 34.  A wave takes two tiles of 16 rows (for the block: gate and up).
+// The 4 waves of a workgroup share the k tiles of one pair and meet in LDS, so
+// that small matrices fill the device; with many rows and more than 64 tokens
+// each has a pair of its own (few_alone), and they share the tokens' lines.
 //
 // k tiles in groups of 8: lane q takes the groups 8 q + j (j = tile of the 8)
 // of 32, so its 8 codes are one load, and the tokens' operand is read from
@@ -1180,27 +1188,29 @@ __global__ void __launch_bounds__(256, TT == 8 || OWN ? 2 : 3) few_kernel(const 
     const int64_t done = s1 > s0 ? pair - step : pair;
     if constexpr (KW == 4) {
         if (s1 <= s0) pair += step;  // (a wave without k tiles: rows below 128 values)
-        __shared__ f32x4_t s_acc[4][2 * TT][64];
-        __syncthreads();  // the last pair's have been read
+        __shared__ f32x4_t s_acc[4][TT][64];
+        f32x4_t o[TS][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+        for (int i = 0; i < 2; i++) {
+            __syncthreads();  // what was there has been read
 #pragma unroll
-            for (int t = 0; t < TT; t++) s_acc[wave][i * TT + t][lane] = acc[i][t] * up;
-        __syncthreads();
+            for (int t = 0; t < TT; t++) s_acc[wave][t][lane] = acc[i][t] * up;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < TS; k++) {
+                const int t = min(wave + 4 * k, TT - 1);
+                o[k][i] = s_acc[0][t][lane];
+#pragma unroll
+                for (int w = 1; w < 4; w++) o[k][i] += s_acc[w][t][lane];
+            }
+        }
 #pragma unroll
         for (int k = 0; k < TS; k++) {
             const int t = wave + 4 * k;
             if (t >= TT || t * 16 >= left) break;
-            f32x4_t o[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                o[i] = s_acc[0][i * TT + t][lane];
-#pragma unroll
-                for (int w = 1; w < 4; w++) o[i] += s_acc[w][i * TT + t][lane];
-            }
             const int tok = tok0 + t * 16 + nl;
             const float f = OWN ? 1.0f : a.fac[tok];
-            epi.few(state[k], a.m, a.rs, o[0] * f, o[1] * f, done, tok);
+            epi.few(state[k], a.m, a.rs, o[k][0] * f, o[k][1] * f, done, tok);
         }
     } else {
 #pragma unroll
@@ -1267,25 +1277,54 @@ __global__ void __launch_bounds__(16 * LSE_LANES) lse_kernel(const LseArgs a)
 }
 
 struct DxArgs {
-    const float* part;  // [slices][tp][np]
-    int slices, tp, n;
+    const f32x4_t* part;  // of GradEpi
+    int slices, tp, n, tokens;
     int64_t np;
     DxFactor fac;
     void* dx;
     int dx_dt;
 };
+// A wave 16 tokens by 128 columns, a lane 4 runs of 8 neighbouring columns.
+// SPLIT: the 4 waves of a workgroup take the slices in turn and meet in LDS
+// (8 slices of 200 x 2048 sums: @@SPLIT@@).
+template <bool SPLIT>
 __global__ void __launch_bounds__(256) dx_kernel(const DxArgs a)
 {
-    const int t = blockIdx.y, i = ((int)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, tile = blockIdx.y, t = tile * 16 + (lane & 15);
+    const int64_t g = SPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    if (!SPLIT && g * 128 >= a.n) return;
     DxFactor fac = a.fac;
     fac.init();
-    if (i >= a.n) return;
+    f32x4_t v[8];
+    const f32x4_t* p = a.part + ((int64_t)tile * (a.np / 128) + g) * 512 + lane;
+    const int64_t ld = (int64_t)(a.tp / 16) * (a.np / 128) * 512;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = p[(SPLIT ? wave : 0) * ld + i * 64];
+    for (int z = SPLIT ? wave + 4 : 1; z < a.slices; z += SPLIT ? 4 : 1)
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] += p[z * ld + i * 64];
+    if constexpr (SPLIT) {
+        __shared__ f32x4_t s_v[4][8][64];
+#pragma unroll
+        for (int i = 0; i < 8; i++) s_v[wave][i][lane] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // (the wave finishes element `wave` of every lane)
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) s += ((const float*)&s_v[w][i][lane])[wave];
+            v[i][0] = s;
+        }
+    }
+    if (t >= a.tokens) return;
     bool skip;
     const float f = fac.of(t, skip);
-    f32x4_t v = *(const f32x4_t*)(a.part + (int64_t)t * a.np + i);
-    for (int z = 1; z < a.slices; z++) v += *(const f32x4_t*)(a.part + ((int64_t)z * a.tp + t) * a.np + i);
 #pragma unroll
-    for (int k = 0; k < 4; k++) store_from_f32(a.dx, a.dx_dt, (int64_t)t * a.n + i + k, fac.apply(v[k], f, skip));
+    for (int e = 0; e < (SPLIT ? 1 : 4); e++) {
+        const int64_t col = g * 128 + (q * 4 + (SPLIT ? wave : e)) * 8;
+        if (col < a.n) store_run(a.dx, a.dx_dt, (int64_t)t * a.n + col, v, e, f, fac, skip);
+    }
 }
 
 struct DsArgs {
@@ -1349,39 +1388,34 @@ bool few_own(int64_t tokens, int x_dt) { return tokens <= 4 && x_dt <= VQ2_DT_BF
 
 int64_t few_pairs(const PanelCall& c) { return ((c.rows + 15) / 16 * c.nmat + 1) / 2; }
 
-// Its token tiles a workgroup.  128 tokens at once, for which a wave has its
-// rows to itself, only where the rows are many (65 to 128 tokens of 151936 rows: 260 us,
-// 64 at a time 430; of 512 + 512 rows 66, 64 at a time 23).
-int few_tiles(const PanelCall& c, int64_t tokens)
-{
-    if (tokens <= 32) return tokens <= 16 ? 1 : 2;
-    return tokens > 64 && tokens <= 128 && few_pairs(c) >= 1024 ? 8 : 4;
-}
+// Its token tiles a workgroup, and whether a wave of 128 tokens has its rows to
+// itself.
+int few_tiles(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : tokens <= 64 ? 4 : 8; }
+bool few_alone(int64_t pairs) { return pairs >= 1024; }
 
-// and its workgroups along the pairs of tiles: for the loss as many as are
+// Its workgroups along the pairs of tiles: for the loss as many as are
 // resident, each keeps running sums over its pairs.
 int few_groups(const PanelCall& c, int64_t tokens)
 {
-    const int tt = few_tiles(c, tokens);
-    const int64_t units = tt == 8 ? (few_pairs(c) + 3) / 4 : few_pairs(c);
+    const int tt = few_tiles(tokens);
+    const int64_t pairs = few_pairs(c), units = tt == 8 && few_alone(pairs) ? (pairs + 3) / 4 : pairs;
     if (c.what != PANEL_STATS) return (int)units;
     return (int)std::min<int64_t>(units, (int64_t)device_cu_count() * (tt == 8 || few_own(tokens, c.x_dt) ? 2 : 3));
 }
 
 // Whether few_kernel is ahead of panels: it gathers every centroid once for
-// each block of tokens, panels once, but they store and read it again, and take two
-// launches more.  Times of both (us; rows x n, bits, tokens: few / panels):
-// @@FEW@@
+// each block of 128 tokens, panels once, but they store and read it again, and
+// take two launches more.  In gathers: a block costs them and 10^5, panels 1.3
+// times as many and 2.8 * 10^6.  Measured (us a call; codes of the call, tokens: few /
+// panels): 65 k, 512 15 / 24; 262 k, 1024 31 / 39, 2048 45 / 42; 512 k, 333 26 / 37, 1024 43 / 41;
+// 3.1 M, 128 33 / 51, 256 54 / 52, 512 96 / 59; 6.3 M, 128 51 / 61, 192 82 / 62; 12.9 M, 128
+// 108 / 128, 160 190 / 140; 38.9 M, 1 174 / 335, 128 270 / 335, 160 478 / 367.
 bool few_ahead(const PanelCall& c, int64_t tokens)
 {
     if (c.cb_dt == VQ2_DT_F32) return false;  // (its centroids would take two products each)
-#ifdef FORCE_FEW
-    return FORCE_FEW && tokens <= 2048;
-#endif
     const double gathers = (double)c.rows * c.nmat * (double)(c.n / 8) * (c.s2 == VQ2_S2_U16 ? 2 : 1);
-    const int tt = few_tiles(c, tokens);
-    const double blocks = tt == 8 ? 1.4 : (double)((tokens + 63) / 64);
-    return blocks <= 1.5 || blocks * (gathers + 3e4) <= 1.5 * gathers + 2.5e6;
+    const double blocks = (double)((tokens + 127) / 128);
+    return tokens <= 64 || blocks * (gathers + 1e5) <= 1.3 * gathers + 2.8e6;
 }
 
 struct Plan {
@@ -1469,8 +1503,8 @@ hipError_t gemm_typed(const PanelGemmArgs& g, const Epi& e, int64_t tile0, hipSt
                                    pg_lds(MT));
     });
     if (attr != hipSuccess) return attr;
-    hipLaunchKernelGGL((panel_gemm_kernel<MT, Epi>), dim3((unsigned)(g.gm * g.gn * g.gz)), dim3(PG_THREADS), pg_lds(MT), st, g, e,
-                       tile0);
+    hipLaunchKernelGGL((panel_gemm_kernel<MT, Epi>), dim3((unsigned)(g.gm * g.gn * g.gz)), dim3(PG_THREADS),
+                       pg_lds(MT), st, g, e, tile0);
     return hipGetLastError();
 }
 
@@ -1534,7 +1568,8 @@ hipError_t few_typed(const FewArgs& a, const Epi& e, int tt, int groups, hipStre
     else if (tt == 1) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, false, Epi>), grid, block, 0, st, a, e);
     else if (tt == 2) hipLaunchKernelGGL((few_kernel<CBT, S2, 2, 4, false, Epi>), grid, block, 0, st, a, e);
     else if (tt == 4) hipLaunchKernelGGL((few_kernel<CBT, S2, 4, 4, false, Epi>), grid, block, 0, st, a, e);
-    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, false, Epi>), grid, block, 0, st, a, e);
+    else if (few_alone(a.pairs)) hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, false, Epi>), grid, block, 0, st, a, e);
+    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 4, false, Epi>), grid, block, 0, st, a, e);
     return hipGetLastError();
 }
 
@@ -1588,7 +1623,7 @@ int panel_launch(const PanelCall& c)
     half8_t* w = first ? (half8_t*)(ws + p.w) : nullptr;
     half8_t* wt = grad ? (half8_t*)(ws + p.wt) : nullptr;
     half8_t* pp = (half8_t*)(ws + p.p);
-    float* acc = (float*)(ws + p.acc);
+    f32x4_t* acc = (f32x4_t*)(ws + p.acc);
     float* ds = c.ds[0] ? (float*)(ws + p.ds) : nullptr;
     float* dfac = (float*)(ws + p.dfac);
     bool prepared = false;  // the row scales
@@ -1629,12 +1664,12 @@ int panel_launch(const PanelCall& c)
         if (few_call) {
             const FewArgs f{mats, few_pairs(c), xp, fac, (const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n,
                             c.rs};
-            const int tt = few_tiles(c, tokens), groups = few_groups(c, tokens);
+            const int tt = few_tiles(tokens), groups = few_groups(c, tokens);
             if (c.what == GATED) {
                 TRY(few(f, gated, tt, groups, c.cb_dt, c.s2, st));
             } else {
                 TRY(few(f, stats, tt, groups, c.cb_dt, c.s2, st));
-                TRY(lse_launch(tt == 8 ? groups * 4 : groups));
+                TRY(lse_launch(tt == 8 && few_alone(few_pairs(c)) ? groups * 4 : groups));
             }
             continue;
         }
@@ -1668,8 +1703,10 @@ int panel_launch(const PanelCall& c)
         if (c.what == STATS) TRY(lse_launch(p.tiles / p.mt));
         if (!grad) continue;
         if (!p.direct) {
-            hipLaunchKernelGGL(dx_kernel, dim3((unsigned)((c.n + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st,
-                               DxArgs{acc, p.slices, tp, (int)c.n, p.np, dxf, dx, c.y_dt});
+            const DxArgs d{acc, p.slices, tp, (int)c.n, tokens, p.np, dxf, dx, c.y_dt};
+            const unsigned rows = (unsigned)((tokens + 15) / 16);
+            if (p.slices >= 4) hipLaunchKernelGGL(dx_kernel<true>, dim3((unsigned)((c.n + 127) / 128), rows), dim3(256), 0, st, d);
+            else hipLaunchKernelGGL(dx_kernel<false>, dim3((unsigned)((c.n + 511) / 512), rows), dim3(256), 0, st, d);
             TRY(hipGetLastError());
         }
         if (ds) {

@@ -82,6 +82,8 @@ constexpr int PG_WM = 2, PG_WN = 2, PG_NT = 4, PG_BUF = 3;
 constexpr int PG_THREADS = 64 * PG_WM * PG_WN;
 constexpr int PG_N = 16 * PG_WN * PG_NT;  // tokens of a workgroup
 constexpr int pg_m(int MT) { return 16 * PG_WM * MT; }
+// PG_BUF stages of one k tile in LDS (with 8 stages and a workgroup a CU, short
+// products were no faster)
 constexpr int pg_lds(int MT) { return (PG_WM * MT + PG_WN * PG_NT) * PG_BUF * 1024; }
 
 struct PanelGemmArgs {
