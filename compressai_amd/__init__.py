@@ -7,7 +7,8 @@ Hand-written HIP kernels behind the C ABI of ``include/vq2_amd.h``
 * ``compressai_amd.kernels``  VQ GEMV (2/3/4 bpw), grouped per-expert GEMV,
   RHT, router top-k, top-1, dequant and index-decode entry points;
 * ``compressai_amd.rot``      ``Rot`` / ``get_rot`` / ``FastRot`` on the RHT kernel;
-* ``compressai_amd.runtime``  ``PackedLinear`` / ``PackedLMHead`` callers;
+* ``compressai_amd.runtime``  ``PackedLinear`` / ``PackedMLP`` / ``PackedLMHead`` callers;
+* ``compressai_amd.tuning``   gradients through packed layers;
 * ``compressai_amd.moe``      resident expert pool module and full MoE layer;
 * ``compressai_amd.synth``    seeded synthetic workloads.
 """

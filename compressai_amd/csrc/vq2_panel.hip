@@ -1286,7 +1286,7 @@ struct DxArgs {
 };
 // A wave 16 tokens by 128 columns, a lane 4 runs of 8 neighbouring columns.
 // SPLIT: the 4 waves of a workgroup take the slices in turn and meet in LDS
-// (8 slices of 200 x 2048 sums: @@SPLIT@@).
+// (8 slices of 200 x 2048 sums: 8.4 us without, 5.0).
 template <bool SPLIT>
 __global__ void __launch_bounds__(256) dx_kernel(const DxArgs a)
 {
@@ -1477,7 +1477,7 @@ Plan plan_of(const PanelCall& c)
         const int64_t wg = p.np / pg_m(8) * (p.tp / PG_N), most = std::max<int64_t>(1, p.piece / 2 / 8);
         // One piece in one slice is written as dx at once.
         const bool one = p.piece == p.tiles;
-        p.gmt = wg >= slots || (2 * wg >= slots && !one) ? 8 : 4;
+        p.gmt = 2 * wg >= slots ? 8 : 4;
         while (p.slices < 64 && wg * (8 / p.gmt) * p.slices < slots && p.slices * 2 <= most) p.slices *= 2;
         p.direct = one && p.slices == 1;
         p.acc = b.take(p.direct ? 0 : p.slices * p.tp * p.np * 4);

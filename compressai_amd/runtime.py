@@ -9,10 +9,12 @@ runs the fused VQ GEMV (batch <= 2) or the matrix-core product of all rows
 (batch >= 3, ``kernels.vq_rows_gemm``) for every cfg in (16,), (16, 8), (16, 16) -- the reference
 fuses only batch 1 of (16,) and (16, 8) and otherwise re-materialises the
 dequantized matrix (runtime.py:91-110).
-``PackedLMHead`` (runtime.py:136-144) wraps it and adds ``argmax`` and
-``sample`` (the next token under temperature, top-k, top-p and min-p).
+``PackedLMHead`` (runtime.py:136-144) wraps it and adds ``argmax``,
+``sample`` (the next token under temperature, top-k, top-p and min-p) and ``loss``
+(of given tokens, without the logits).
 ``PackedProjections`` runs projections of one activation (q, k, v) in one
-launch.
+launch, ``PackedMLP`` the gated feed-forward block; the latter and ``loss`` are
+differentiable (``tuning``).
 
 Large matrices (``SORTED_MIN_CODES`` codes or more, 2 and 4 bpw) also keep
 a code-sorted copy of their index planes (``kernels.SortedPlanes``, packed
@@ -310,6 +312,65 @@ class PackedProjections(nn.Module):
         return [y.view(*x.shape[:-1], m.out) for y, m in zip(ys, lins)]
 
 
+class PackedMLP(nn.Module):
+    """Gated feed-forward block of packed matrices: down(f(gate x) * (up x)),
+    f "silu" or "gelu_tanh".  gate and up are ``PackedLinear``s of one width,
+    cfg, codebooks, rotation tag and scale dtype, down takes their rows.  One rotation, gate,
+    up, activation and product in one pass (``kernels.vq_gated_rows``), and
+    down; a single row of SiLU matrices with the sorted layout goes through it
+    instead (three launches: gate + up, SwiGLU with down's rotation, down).
+    Activations are held in x's type (fp32: fp16).  Differentiable in x and in
+    the three ``scale``s that require it."""
+
+    def __init__(self, gate, up, down, activation="silu"):
+        super().__init__()
+        if gate.n != up.n or gate.out != up.out or gate.cfg != up.cfg or gate.tag != up.tag or gate._cbs[0] is not up._cbs[0]:
+            raise K.Vq2Error("PackedMLP: gate and up must share shape, cfg, codebooks and tag")
+        if gate.scale.dtype != up.scale.dtype:
+            raise K.Vq2Error("PackedMLP: gate and up must share the scale dtype")
+        if down.n != gate.out:
+            raise K.Vq2Error(f"PackedMLP: down takes {down.n} values, gate and up give {gate.out}")
+        if gate.n % 64:
+            raise K.Vq2Error(f"PackedMLP: width {gate.n} must be a multiple of 64")
+        K._act(activation)
+        self.gate, self.up, self.down, self.activation = gate, up, down, activation
+
+    def forward(self, x, out_dtype=None):
+        gate, up, down = self.gate, self.up, self.down
+        od = out_dtype or x.dtype
+        xt = _row_type(x)
+        mats = (gate, up, down)
+        if torch.is_grad_enabled() and (x.requires_grad or any(m.scale.requires_grad for m in mats)):
+            from . import tuning as T
+
+            act = T.gated(gate, up, T.rotate(x, gate.rot, xt), self.activation)
+            return T.linear(down, T.rotate(act, down.rot)).to(od)
+        x2 = x.reshape(-1, gate.n).contiguous()
+        g0, g1, cb0, cb1 = gate._planes()
+        if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], cb0) for m in mats):
+            I = gate.out
+            gu = torch.empty(2 * I, dtype=torch.float32, device=x.device)
+            xs, perm, sign, hb, sc = gate._sorted_args(x2.reshape(-1))
+            K.vq_sorted_gemv(xs, [(gate.sorted, gate.scale), (up.sorted, up.scale)], cb0, cb1, gate.n, perm, sign, hb, sc,
+                             ys=[gu[:I], gu[I:]])
+            r = down.rot
+            act = K.vq_swiglu_rht(gu, I, r._perm32, r._sign8, r.hb, r.scale)
+            _, _, d0, d1 = down._planes()
+            y = K.vq_sorted_gemv(act, [(down.sorted, down.scale)], d0, d1, I, hb=0, out_dtype=od)[0]
+            return y.view(*x.shape[:-1], down.out)
+        if gate.planes_released or up.planes_released:
+            raise K.Vq2Error("PackedMLP: the index planes, which more than one row needs, were released")
+        u0, u1, _, _ = up._planes()
+        xr = gate.rot.fwd(x2, out_dtype=xt)
+        act = K.vq_gated_rows(xr, (g0, g1, gate.scale), (u0, u1, up.scale), cb0, cb1, gate.n, activation=self.activation)
+        return down(act, out_dtype=od).view(*x.shape[:-1], down.out)
+
+
+def _row_type(x):
+    """the type that rotated rows of x are held in: its own, fp16 for fp32"""
+    return torch.float16 if x.dtype == torch.float32 else x.dtype
+
+
 class PackedLMHead(nn.Module):
     """lm_head sharing the packed weights of a PackedLinear."""
 
@@ -326,6 +387,21 @@ class PackedLMHead(nn.Module):
         these are): (idx int64 [B], logprob fp32 [B])."""
         logits = self.lin(x.reshape(-1, self.lin.n), out_dtype=torch.float32)
         return K.vq_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+    def loss(self, x, targets, *, ignore_index=-100):
+        """Negative log-likelihood of targets (int64, one per row of x) under
+        the head's softmax, fp32 [rows], in pieces of the vocabulary
+        (kernels.vq_head_loss, whose targets these are); 0 where the target
+        is ignore_index.  Differentiable in x and, where it requires a
+        gradient, the head's ``scale``.  The rotated rows are held in x's type
+        (fp32: fp16)."""
+        from . import tuning as T
+
+        lin = self.lin
+        x2 = x.reshape(-1, lin.n)
+        if lin.planes_released:
+            raise K.Vq2Error("loss needs the head's index planes, which were released")
+        return T.head_loss(lin, T.rotate(x2, lin.rot, _row_type(x)), targets, ignore_index)
 
     def argmax(self, x):
         """Top-1 token per row of x without materialising bf16 logits:

@@ -1,0 +1,170 @@
+"""Gradients through packed layers, for tuning around frozen codes.
+
+What a packed model learns without touching its codes: the norms' weights, the
+row scales (make ``PackedLinear.scale`` a leaf: ``lin.scale.requires_grad_()``, in
+fp32 for small steps), and whatever produces the activations (adapters, other
+layers).  The functions here are differentiable once in all of these; each is
+one entry of ``kernels`` forward and one backward:
+
+  rotate(x, rot)                the RHT (orthogonal: its gradient is its inverse)
+  add_rms_norm(x, weight, residual, rot=...)  (y, h), y rotated where rot is given
+  linear(lin, xr)               a PackedLinear on rotated rows
+  gated(gate, up, xr)           f(gate xr) * (up xr)
+  head_loss(lin, xr, targets)   the loss of every token
+
+``xr`` are rotated rows in fp16 or bf16 (``rotate`` or ``add_rms_norm`` give
+them).  ``runtime.PackedMLP`` and ``PackedLMHead.loss`` are built on them.  The
+reference distils and tunes with dequantized weights in torch (vq2/kd.py); here
+no dequantized matrix is kept.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import kernels as K
+
+__all__ = ["rotate", "add_rms_norm", "linear", "gated", "head_loss"]
+
+
+def _rows16(xr, what):
+    if xr.dtype not in (torch.float16, torch.bfloat16):
+        raise K.Vq2Error(f"{what}: rotated rows in float16 or bfloat16, got {xr.dtype}")
+    return xr.contiguous()
+
+
+def _planes(lin):
+    if lin.planes_released:
+        raise K.Vq2Error("gradients need the index planes, which were released")
+    return lin._planes()
+
+
+def _to(t, like):
+    return None if t is None else t.to(like.dtype)
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rot, out_dtype):
+        ctx.rot, ctx.dtype = rot, x.dtype
+        return rot.fwd(x, out_dtype=out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return ctx.rot.inv(dy.contiguous(), out_dtype=ctx.dtype), None, None
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, kw, out_dtype):
+        ctx.set_materialize_grads(False)
+        y, h, _ = K.vq_add_rms_norm(x, weight, residual, out_dtype=out_dtype, **kw)
+        ctx.save_for_backward(h, weight)
+        ctx.kw, ctx.residual = kw, residual is not None
+        return (y, h) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        if dy is None:  # the norm itself was not used
+            return dh, None, dh, None, None
+        dx, dw = K.vq_add_rms_norm_backward(dy.contiguous(), h, weight, None if dh is None else dh.contiguous(),
+                                            weight_grad=ctx.needs_input_grad[1], **ctx.kw)
+        return dx, _to(dw, weight), dx if ctx.residual else None, None, None
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, xr, scale, lin):
+        from .runtime import vq_matmul
+
+        ctx.save_for_backward(xr, scale)
+        ctx.lin = lin
+        i0, i1, cb0, cb1 = _planes(lin)
+        x2 = xr.reshape(-1, lin.n)
+        if x2.shape[0] >= 3 and lin.n % 64 == 0 and lin.n <= K.ROWS_GEMM_MAX_N:
+            y = K.vq_rows_gemm(x2, [(i0, i1, scale, lin.out)], cb0, cb1, lin.n, hb=0, act_dtype=xr.dtype, out_dtype=xr.dtype)[0]
+        else:
+            y = vq_matmul(x2, i0, i1, cb0, cb1, scale, lin.out, lin.n, xr.dtype)
+        return y.view(*xr.shape[:-1], lin.out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xr, scale = ctx.saved_tensors
+        lin = ctx.lin
+        i0, i1, cb0, cb1 = _planes(lin)
+        dx, ds = K.vq_gemm_backward(dy.contiguous(), xr, i0, i1, cb0, cb1, scale, lin.out, lin.n,
+                                    scale_grad=ctx.needs_input_grad[1])
+        return dx, _to(ds, scale), None
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, xr, gate_scale, up_scale, gate, up, activation):
+        ctx.save_for_backward(xr, gate_scale, up_scale)
+        ctx.mats, ctx.activation = (gate, up), activation
+        (g0, g1, cb0, cb1), (u0, u1, _, _) = _planes(gate), _planes(up)
+        return K.vq_gated_rows(xr, (g0, g1, gate_scale), (u0, u1, up_scale), cb0, cb1, gate.n, activation=activation)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dact):
+        xr, gate_scale, up_scale = ctx.saved_tensors
+        gate, up = ctx.mats
+        (g0, g1, cb0, cb1), (u0, u1, _, _) = _planes(gate), _planes(up)
+        dx, dg, du = K.vq_gated_rows_backward(dact.contiguous(), xr, (g0, g1, gate_scale), (u0, u1, up_scale), cb0, cb1,
+                                              gate.n, activation=ctx.activation,
+                                              scale_grad=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return dx, _to(dg, gate_scale), _to(du, up_scale), None, None, None
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, xr, scale, lin, targets, ignore_index):
+        i0, i1, cb0, cb1 = _planes(lin)
+        loss, lse = K.vq_head_loss(xr, targets, i0, i1, cb0, cb1, scale, lin.out, lin.n, ignore_index=ignore_index)
+        ctx.save_for_backward(xr, scale, targets, lse)
+        ctx.lin, ctx.ignore_index = lin, ignore_index
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        xr, scale, targets, lse = ctx.saved_tensors
+        lin = ctx.lin
+        i0, i1, cb0, cb1 = _planes(lin)
+        dx, ds = K.vq_head_loss_backward(xr, targets, lse, dloss.contiguous(), i0, i1, cb0, cb1, scale, lin.out, lin.n,
+                                         ignore_index=ctx.ignore_index, scale_grad=ctx.needs_input_grad[1])
+        return dx, _to(ds, scale), None, None, None
+
+
+def rotate(x, rot, out_dtype=None):
+    """rot.fwd(x): rows in the basis that packed matrices of this rotation take."""
+    return _Rotate.apply(x.contiguous(), rot, out_dtype)
+
+
+def add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, rot=None, out_dtype=None):
+    """(y, h) of kernels.vq_add_rms_norm; y is rotated where a ``rot.Rot`` is given."""
+    kw = dict(eps=eps, zero_centred=zero_centred)
+    if rot is not None:
+        kw.update(perm=rot._perm32, sign=rot._sign8, hb=rot.hb, rht_scale=rot.scale)
+    out = _Norm.apply(x.contiguous(), weight, None if residual is None else residual.contiguous(), kw, out_dtype)
+    return out if residual is not None else (out, x)
+
+
+def linear(lin, xr):
+    """A PackedLinear's product with rotated rows, in their type."""
+    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin)
+
+
+def gated(gate, up, xr, activation="silu"):
+    """f(gate xr) * (up xr) of two PackedLinears of one width, cfg, codebooks and rotation."""
+    return _Gated.apply(_rows16(xr, "gated"), gate.scale, up.scale, gate, up, activation)
+
+
+def head_loss(lin, xr, targets, ignore_index=-100):
+    """kernels.vq_head_loss of a head's PackedLinear: the loss of every row, fp32."""
+    return _HeadLoss.apply(_rows16(xr, "head_loss").reshape(-1, lin.n), lin.scale, lin, targets.reshape(-1).contiguous(), ignore_index)
