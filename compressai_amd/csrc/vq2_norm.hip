@@ -9,15 +9,17 @@
 //   g = R^T dy,  dx = dh + r g w - h r^3 mean(g w h),  dw = sum over rows of g h r
 //
 // Bound by HBM: every element is read once and written once, the row stays in
-// registers between.  A thread holds 8 neighbouring values (16-byte loads) of each
+// registers between.  16384 rows of 2048 (bf16, residual: 268 MB) 41.5 us, 6.5 TB/s;
+// rotated 51; backward 42, rotated 67.  Rows that are no multiple of 8 values are loaded one
+// by one (16000 x 2047: 49 us).  A thread holds 8 neighbouring values (16-byte loads) of each
 // 2048: the transform's first 3 stages are in its registers, the next 6 are
-// exchanges between lanes, the ones above (blocks of 1024 and 2048) one pass
-// through LDS between the waves, blocks above 2048 in registers again.  The
-// permutation goes through LDS, too.  A workgroup takes rows in turn and loads
-// its part of the weights and tables once.  All
-// arithmetic is fp32; h is rounded where it is stored, y is made from the
-// unrounded sum.
+// exchanges between lanes, the ones above one pass through LDS between the waves
+// of a row, and what is left in registers again.  The permutation goes through
+// LDS, too.  A workgroup takes rows in turn, the next one's loads ahead, and
+// loads its part of the weights and tables once.  All arithmetic is fp32; h is
+// rounded where it is stored, y is made from the unrounded sum.
 #include <algorithm>
+#include <type_traits>
 
 #include "vq2_internal.hpp"
 #include "vq2_panel.hpp"
@@ -26,7 +28,10 @@ namespace vq2 {
 
 namespace {
 
-constexpr int NT = 256;  // threads of a workgroup
+// Threads of a workgroup: 256, or backward 512 that share one row above 6144
+// values (4096 x 8192: 95 us; with 256, 32 values a thread, 184, spilled.
+// Forward 256 threads take 65 us, 512 87).
+constexpr int threads_of(int TPR) { return TPR > 256 ? TPR : 256; }
 
 // lane i <- lane i ^ 4, i ^ 8 within a row of 16
 __device__ __forceinline__ float dpp_xor4(float v)
@@ -75,7 +80,7 @@ __device__ __forceinline__ void swap_stage(float (&v)[8])
 }
 
 // Hadamard transform of blocks of hb values; the row's value 8 (c TPR + id) + k
-// is v[c][k] of its thread id.  s: V * 8 * TPR floats of the row (TPR == 256).
+// is v[c][k] of its thread id.  s: V * 8 * TPR floats of the row.
 template <int V, int TPR>
 __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float* s)
 {
@@ -105,8 +110,9 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
     if (hb >= 512)
 #pragma unroll
         for (int c = 0; c < V; c++) swap_stage<32>(v[c]);
-    if (TPR == 64 || hb < 1024) return;
-    // between the waves: value of wave w gets sum over w' of +- theirs
+    if (TPR <= 64 || hb < 1024) return;
+    // between the waves of a row: that of wave w is the sum over the m of its
+    // block of +- theirs, minus where w and the other share an odd number of bits
     const int w = id >> 6;
     f32x4_t* p = (f32x4_t*)s;
     __syncthreads();
@@ -116,27 +122,33 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
         p[(c * 2 + 1) * TPR + id] = f32x4_t{v[c][4], v[c][5], v[c][6], v[c][7]};
     }
     __syncthreads();
-    const float s1 = w & 1 ? -1.0f : 1.0f, s2 = w & 2 ? -1.0f : 1.0f;
+    auto exchange = [&](auto count) {
+        constexpr int M = decltype(count)::value;
+        float sg[M];
 #pragma unroll
-    for (int c = 0; c < V; c++)
+        for (int j = 0; j < M; j++) sg[j] = __builtin_popcount(w & j) & 1 ? -1.0f : 1.0f;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const f32x4_t* q = p + (c * 2 + h) * TPR + (id & 63);
-            f32x4_t o;
-            if (hb == 1024) {
-                const f32x4_t a = q[(w & ~1) * 64], b = q[(w | 1) * 64];
-                o = a + b * s1;
-            } else {
-                const f32x4_t a = q[0], b = q[64], d = q[128], e = q[192];
-                o = (a + b * s1) + (d + e * s1) * s2;
+        for (int c = 0; c < V; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const f32x4_t* q = p + (c * 2 + h) * TPR + (w & ~(M - 1)) * 64 + (id & 63);
+                f32x4_t o = q[0];
+#pragma unroll
+                for (int j = 1; j < M; j++) o += q[j * 64] * sg[j];
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[c][4 * h + k] = o[k];
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[c][4 * h + k] = o[k];
-        }
-    // blocks above 2048: between a thread's own parts
+    };
+    if (hb == 1024) exchange(std::integral_constant<int, 2>());
+    else if (TPR == 256 || hb == 2048) {
+        if constexpr (TPR >= 256) exchange(std::integral_constant<int, 4>());
+    } else {
+        if constexpr (TPR >= 512) exchange(std::integral_constant<int, 8>());
+    }
+    // blocks above 8 TPR: between a thread's own parts
 #pragma unroll
     for (int st = 1; st < V; st *= 2) {
-        if (hb < 4096 * st) break;
+        if (hb < 16 * TPR * st) break;
 #pragma unroll
         for (int c = 0; c < V; c++)
             if (!(c & st) && c + st < V)
@@ -149,7 +161,8 @@ __device__ __forceinline__ void hadamard(float (&v)[V][8], int hb, int id, float
     }
 }
 
-// N values that every thread of the row has a part of; s: N words for each wave
+// N values that every thread of the row has a part of; s: N words for each
+// wave of the workgroup
 template <int TPR, int N, class Op>
 __device__ __forceinline__ void row_reduce(float (&v)[N], float* s, Op op)
 {
@@ -159,17 +172,25 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float* s, Op op)
         v[i] = op(v[i], dpp_xor2(v[i]));
         v[i] = op(v[i], dpp_half_mirror(v[i]));
         v[i] = op(v[i], dpp_row_mirror(v[i]));
-        v[i] = op(v[i], swz_xor16(v[i]));
-        v[i] = op(v[i], xor32(v[i]));
+        if (TPR >= 64) {
+            v[i] = op(v[i], swz_xor16(v[i]));
+            v[i] = op(v[i], xor32(v[i]));
+        }
     }
-    if (TPR == 64) return;
+    if (TPR <= 64) return;
+    constexpr int W = TPR / 64;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
     __syncthreads();  // (the last call's values have been read)
 #pragma unroll
     for (int i = 0; i < N; i++)
-        if ((threadIdx.x & 63) == 0) s[i * 4 + (threadIdx.x >> 6)] = v[i];
+        if ((threadIdx.x & 63) == 0) s[i * 8 + wave] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = op(op(s[i * 4], s[i * 4 + 1]), op(s[i * 4 + 2], s[i * 4 + 3]));
+    for (int i = 0; i < N; i++) {
+        v[i] = s[i * 8 + first];
+#pragma unroll
+        for (int k = 1; k < W; k++) v[i] = op(v[i], s[i * 8 + first + k]);
+    }
 }
 __device__ __forceinline__ float add_op(float a, float b) { return a + b; }
 // maximum of magnitudes by their bits: a NaN is above everything and stays
@@ -186,8 +207,9 @@ __device__ __forceinline__ int place(int c, int k, int id)
     return VEC ? (c * TPR + id) * 8 + k : (c * 8 + k) * TPR + id;
 }
 
-// A row's values as they are loaded (VEC: 16 or 32 bytes of type DT; else the
-// values in fp32), and as numbers.
+// A row's values as they are loaded (VEC: 16 or 32 bytes of type DT; else a word
+// each), and as numbers.  No load is behind a branch: past the row's end the
+// first value is loaded, and dropped.
 template <int DT, int V, bool VEC>
 struct Raw {
     u32x4 w[V][VEC && DT != VQ2_DT_F32 ? 1 : 2];
@@ -195,12 +217,13 @@ struct Raw {
 template <int DT, int V, int TPR, bool VEC>
 __device__ __forceinline__ void load_raw(Raw<DT, V, VEC>& r, const void* p, int64_t row, int n, int id)
 {
+    const char* base = (const char*)p + row * n * (DT == VQ2_DT_F32 ? 4 : 2);
 #pragma unroll
     for (int c = 0; c < V; c++) {
         if constexpr (VEC) {
             const int i = place<V, TPR, VEC>(c, 0, id);
             constexpr int N = DT == VQ2_DT_F32 ? 2 : 1;
-            const u32x4* q = (const u32x4*)((const char*)p + (row * n + (i < n ? i : 0)) * (DT == VQ2_DT_F32 ? 4 : 2));
+            const u32x4* q = (const u32x4*)(base + (i < n ? i : 0) * (DT == VQ2_DT_F32 ? 4 : 2));
 #pragma unroll
             for (int k = 0; k < N; k++) r.w[c][k] = q[k];
             if (i >= n)
@@ -209,9 +232,12 @@ __device__ __forceinline__ void load_raw(Raw<DT, V, VEC>& r, const void* p, int6
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int i = place<V, TPR, VEC>(c, k, id);
-                r.w[c][k / 4][k % 4] = i < n ? __float_as_uint(load_as_f32(p, DT, row * n + i)) : 0;
+                const int i = place<V, TPR, VEC>(c, k, id), at = i < n ? i : 0;
+                r.w[c][k / 4][k % 4] = DT == VQ2_DT_F32 ? ((const uint32_t*)base)[at] : (uint32_t)((const uint16_t*)base)[at];
             }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (place<V, TPR, VEC>(c, k, id) >= n) r.w[c][k / 4][k % 4] = 0;
         }
     }
 }
@@ -222,7 +248,7 @@ __device__ __forceinline__ void numbers(float (&v)[V][8], const Raw<DT, V, VEC>&
     for (int c = 0; c < V; c++) {
         if constexpr (!VEC || DT == VQ2_DT_F32) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[c][k] = __uint_as_float(r.w[c][k / 4][k % 4]);
+            for (int k = 0; k < 8; k++) v[c][k] = raw_as_f32(r.w[c][k / 4][k % 4], DT);
         } else if constexpr (DT == VQ2_DT_F16) {
             const half8_t h = __builtin_bit_cast(half8_t, r.w[c][0]);
 #pragma unroll
@@ -272,14 +298,17 @@ __device__ __forceinline__ void store8(void* p, int dt, int64_t i, const float (
     }
 }
 
-// q = v * inv rounded to the nearest (ties to even), 8 bits each
-__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, int dt)
+// v * inv rounded to the nearest (ties to even), 8 bits each; |v * inv| <= 127
+// (448) but for its rounding
+__device__ __forceinline__ uint32_t quant4(float a, float b, float c, float d, float inv, int dt)
 {
     if (dt == VQ2_DT_I8) {
-        auto q = [](float v) { return (uint32_t)(int)fminf(fmaxf(rintf(v), -127.0f), 127.0f) & 0xFFu; };
-        return q(a) | q(b) << 8 | q(c) << 16 | q(d) << 24;
+        // adding 1.5 * 2^23 rounds to a whole number in the low bits
+        auto q = [&](float v) { return __float_as_uint(fmaf(v, inv, 12582912.0f)); };
+        const uint32_t lo = __builtin_amdgcn_perm(q(b), q(a), 0x0C0C0400u), hi = __builtin_amdgcn_perm(q(d), q(c), 0x0C0C0400u);
+        return lo | hi << 16;
     }
-    auto cl = [](float v) { return v != v ? v : fminf(fmaxf(v, -448.0f), 448.0f); };
+    auto cl = [&](float v) { return v * inv != v * inv ? v * inv : fminf(fmaxf(v * inv, -448.0f), 448.0f); };
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(cl(a), cl(b), 0, false);
     r = __builtin_amdgcn_cvt_pk_fp8_f32(cl(c), cl(d), r, true);
     return (uint32_t)r;
@@ -296,15 +325,14 @@ __device__ __forceinline__ void store_row(const float (&v)[V][8], void* p, int d
             if (dt <= VQ2_DT_BF16) store8(p, dt, row * n + i, v[c]);
             else
                 *(u32x2*)((uint8_t*)p + row * n + i) =
-                    u32x2{quant4(v[c][0] * inv, v[c][1] * inv, v[c][2] * inv, v[c][3] * inv, dt),
-                          quant4(v[c][4] * inv, v[c][5] * inv, v[c][6] * inv, v[c][7] * inv, dt)};
+                    u32x2{quant4(v[c][0], v[c][1], v[c][2], v[c][3], inv, dt), quant4(v[c][4], v[c][5], v[c][6], v[c][7], inv, dt)};
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int i = place<V, TPR, VEC>(c, k, id);
                 if (i >= n) continue;
                 if (dt <= VQ2_DT_BF16) store_from_f32(p, dt, row * n + i, v[c][k]);
-                else ((uint8_t*)p)[row * n + i] = (uint8_t)quant4(v[c][k] * inv, 0.0f, 0.0f, 0.0f, dt);
+                else ((uint8_t*)p)[row * n + i] = (uint8_t)quant4(v[c][k], 0.0f, 0.0f, 0.0f, inv, dt);
             }
         }
     }
@@ -361,11 +389,11 @@ __device__ __forceinline__ float table_sign(float v, const Tables<V>& t, int c, 
 }
 
 template <int DT, int V, int TPR, bool VEC, bool ROT>
-__global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t row_step)
+__global__ void __launch_bounds__(threads_of(TPR), 2) norm_kernel(const NormCall a, int64_t row_step)
 {
-    constexpr int RW = NT / TPR;  // rows of a workgroup
-    __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
-    __shared__ float s_red[4];
+    constexpr int RW = threads_of(TPR) / TPR;  // rows of a workgroup
+    __shared__ __align__(16) float s_row[ROT ? V * 8 * threads_of(TPR) : 1];
+    __shared__ float s_red[8];
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
     // The next row's values are on their way while this one is worked on.  The
@@ -391,7 +419,7 @@ __global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t r
             for (int k = 0; k < 8; k++) w[c][k] += 1.0f;
     for (int64_t r0 = (int64_t)blockIdx.x * RW; r0 < a.rows; r0 += row_step) {
         const int64_t row = r0 + rw;
-        const bool live = row < a.rows;  // (rows of a workgroup: whole waves)
+        const bool live = row < a.rows;
         float h[V][8];
         numbers(h, rx);
         if (a.residual) {
@@ -454,11 +482,11 @@ __global__ void __launch_bounds__(NT, 2) norm_kernel(const NormCall a, int64_t r
 }
 
 template <int DT, int V, int TPR, bool VEC, bool ROT>
-__global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int64_t row_step, float* part)
+__global__ void __launch_bounds__(threads_of(TPR), 2) norm_grad_kernel(const NormCall a, int64_t row_step, float* part)
 {
-    constexpr int RW = NT / TPR;
-    __shared__ __align__(16) float s_row[ROT ? V * 8 * NT : 1];
-    __shared__ float s_red[8];
+    constexpr int RW = threads_of(TPR) / TPR;
+    __shared__ __align__(16) float s_row[ROT || RW > 1 ? V * 8 * threads_of(TPR) : 1];
+    __shared__ float s_red[16];
     const int id = threadIdx.x % TPR, rw = threadIdx.x / TPR;
     float* s = s_row + (ROT ? rw * V * 8 * TPR : 0);
     const bool same = a.y_dt == DT;  // dy of h's type
@@ -538,7 +566,17 @@ __global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int6
         if (live) store_row<V, TPR, VEC>(e, a.y, DT, row, a.n, id, 0.0f);
     }
     if (!part) return;
-    float* o = part + (int64_t)(blockIdx.x * RW + rw) * a.n;
+    if constexpr (RW > 1) {  // the workgroup's rows, added in order
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; k++) s_row[(rw * 8 + k) * TPR + id] = dw[0][k];
+        __syncthreads();
+        if (rw) return;
+        for (int y = 1; y < RW; y++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) dw[0][k] += s_row[(y * 8 + k) * TPR + id];
+    }
+    float* o = part + (int64_t)blockIdx.x * a.n;
 #pragma unroll
     for (int c = 0; c < V; c++) {
         if (VEC && place<V, TPR, VEC>(c, 0, id) < a.n) {
@@ -551,19 +589,22 @@ __global__ void __launch_bounds__(NT, 2) norm_grad_kernel(const NormCall a, int6
     }
 }
 
-// dw: the sums of the workgroups, 64 columns a workgroup, 16 threads a column
+// dw: the sums of the workgroups, 16 columns a workgroup, 64 threads a column
 __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* part, int chunks, int n, float* dw)
 {
-    __shared__ float s[16][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
+    __shared__ float s[64][17];
+    const int x = threadIdx.x & 15, col = blockIdx.x * 16 + x, y = threadIdx.x >> 4;
     float v = 0.0f;
     if (col < n)
-        for (int k = y; k < chunks; k += 16) v += part[(int64_t)k * n + col];
-    s[y][threadIdx.x & 63] = v;
+#pragma unroll 8
+        for (int k = y; k < chunks; k += 64) v += part[(int64_t)k * n + col];
+    s[y][x] = v;
     __syncthreads();
-    if (y || col >= n) return;
-    for (int k = 1; k < 16; k++) v += s[k][threadIdx.x];
-    dw[col] = v;
+    for (int w = 32; w; w /= 2) {
+        if (y < w) s[y][x] += s[y + w][x];
+        __syncthreads();
+    }
+    if (y == 0 && col < n) dw[col] = s[0][x];
 }
 
 struct Shape {
@@ -578,51 +619,54 @@ Shape shape_of(const NormCall& c, bool grad)
     const uintptr_t ptrs = (uintptr_t)c.x | (uintptr_t)c.residual | (uintptr_t)c.weight | (uintptr_t)c.y | (uintptr_t)c.h |
                            (uintptr_t)c.dy | (uintptr_t)c.dh;
     s.vec = c.n % 8 == 0 && ptrs % 16 == 0;
-    s.tpr = c.n <= 512 ? 64 : 256;
-    const int v = (int)((c.n + s.tpr * 8 - 1) / (s.tpr * 8));
-    s.v = v;  // up to 4: VQ2_NORM_MAX_N
-    const int64_t rows = (c.rows + NT / s.tpr - 1) / (NT / s.tpr);
+    // 8 values a thread of a row where that many threads are there (a row of 1024
+    // with 256 threads took twice its time), up to 32
+    s.tpr = c.n <= 128 ? 16 : c.n <= 512 ? 64 : c.n <= 1024 ? 128 : c.n <= 6144 || !grad ? 256 : 512;
+    s.v = (c.n + s.tpr * 8 - 1) / (s.tpr * 8);
+    const int64_t per = threads_of(s.tpr) / s.tpr, rows = (c.rows + per - 1) / per;
     // forward: enough workgroups to hide each other's loads; backward: fewer,
     // each leaves a row of sums
     s.groups = std::min<int64_t>(rows, (int64_t)device_cu_count() * (grad ? (s.v <= 2 ? 4 : 2) : s.v <= 2 ? 8 : 4));
     return s;
 }
 
-template <int DT, int V, int TPR>
-hipError_t launch(const NormCall& c, const Shape& s, bool grad, float* part)
+template <bool GRAD, int DT, int V, int TPR>
+hipError_t launch(const NormCall& c, const Shape& s, float* part)
 {
-    const dim3 grid((unsigned)s.groups), block(NT);
+    const dim3 grid((unsigned)s.groups), block(threads_of(TPR));
     const hipStream_t st = (hipStream_t)c.stream;
-    const int64_t step = s.groups * (NT / TPR);
-    if (grad) {
+    const int64_t step = s.groups * (threads_of(TPR) / TPR);
+    if constexpr (GRAD) {
         if (s.rot) hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, true, true>), grid, block, 0, st, c, step, part);
         else if (s.vec) hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, true, false>), grid, block, 0, st, c, step, part);
         else hipLaunchKernelGGL((norm_grad_kernel<DT, V, TPR, false, false>), grid, block, 0, st, c, step, part);
-        return hipGetLastError();
+    } else {
+        if (s.rot) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, true>), grid, block, 0, st, c, step);
+        else if (s.vec) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, false>), grid, block, 0, st, c, step);
+        else hipLaunchKernelGGL((norm_kernel<DT, V, TPR, false, false>), grid, block, 0, st, c, step);
     }
-    if (s.rot) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, true>), grid, block, 0, st, c, step);
-    else if (s.vec) hipLaunchKernelGGL((norm_kernel<DT, V, TPR, true, false>), grid, block, 0, st, c, step);
-    else hipLaunchKernelGGL((norm_kernel<DT, V, TPR, false, false>), grid, block, 0, st, c, step);
     return hipGetLastError();
 }
 
-template <int DT>
-hipError_t launch_shape(const NormCall& c, const Shape& s, bool grad, float* part)
+template <bool GRAD, int DT>
+hipError_t launch_shape(const NormCall& c, const Shape& s, float* part)
 {
-    if (s.tpr == 64) return launch<DT, 1, 64>(c, s, grad, part);
-    switch (s.v) {
-    case 1: return launch<DT, 1, 256>(c, s, grad, part);
-    case 2: return launch<DT, 2, 256>(c, s, grad, part);
-    case 3: return launch<DT, 3, 256>(c, s, grad, part);
-    default: return launch<DT, 4, 256>(c, s, grad, part);
-    }
+    if (s.tpr == 16) return launch<GRAD, DT, 1, 16>(c, s, part);
+    if (s.tpr == 64) return launch<GRAD, DT, 1, 64>(c, s, part);
+    if (s.tpr == 128) return launch<GRAD, DT, 1, 128>(c, s, part);
+    if (s.v == 1) return launch<GRAD, DT, 1, 256>(c, s, part);
+    if (s.tpr == 256 && s.v == 2) return launch<GRAD, DT, 2, 256>(c, s, part);
+    if (s.v == 3) return launch<GRAD, DT, 3, 256>(c, s, part);
+    if constexpr (GRAD) return launch<GRAD, DT, 2, 512>(c, s, part);
+    else return launch<GRAD, DT, 4, 256>(c, s, part);
 }
 
-hipError_t launch_dt(const NormCall& c, const Shape& s, bool grad, float* part)
+template <bool GRAD>
+hipError_t launch_dt(const NormCall& c, const Shape& s, float* part)
 {
-    if (c.x_dt == VQ2_DT_F16) return launch_shape<VQ2_DT_F16>(c, s, grad, part);
-    if (c.x_dt == VQ2_DT_BF16) return launch_shape<VQ2_DT_BF16>(c, s, grad, part);
-    return launch_shape<VQ2_DT_F32>(c, s, grad, part);
+    if (c.x_dt == VQ2_DT_F16) return launch_shape<GRAD, VQ2_DT_F16>(c, s, part);
+    if (c.x_dt == VQ2_DT_BF16) return launch_shape<GRAD, VQ2_DT_BF16>(c, s, part);
+    return launch_shape<GRAD, VQ2_DT_F32>(c, s, part);
 }
 
 }  // namespace
@@ -633,13 +677,13 @@ size_t norm_workspace_bytes(int64_t rows, int64_t n)
     c.rows = rows;
     c.n = (int)n;
     const Shape s = shape_of(c, true);
-    return rows == 0 ? 0 : (size_t)(s.groups * (NT / s.tpr)) * n * 4;
+    return rows == 0 ? 0 : (size_t)s.groups * n * 4;
 }
 
 int norm_launch(const NormCall& c)
 {
     const Shape s = shape_of(c, false);
-    const hipError_t e = launch_dt(c, s, false, nullptr);
+    const hipError_t e = launch_dt<false>(c, s, nullptr);
     return e == hipSuccess ? VQ2_OK : set_hip_error(e, "vq2_add_rms_norm");
 }
 
@@ -647,12 +691,12 @@ int norm_grad_launch(const NormCall& c, float* dw, void* workspace)
 {
     const Shape s = shape_of(c, true);
     if (c.rows) {
-        const hipError_t e = launch_dt(c, s, true, dw ? (float*)workspace : nullptr);
+        const hipError_t e = launch_dt<true>(c, s, dw ? (float*)workspace : nullptr);
         if (e != hipSuccess) return set_hip_error(e, "vq2_add_rms_norm_backward");
     }
     if (!dw) return VQ2_OK;
-    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((c.n + 63) / 64)), dim3(1024), 0, (hipStream_t)c.stream,
-                       (const float*)workspace, c.rows ? (int)(s.groups * (NT / s.tpr)) : 0, c.n, dw);
+    hipLaunchKernelGGL(norm_dw_kernel, dim3((unsigned)((c.n + 15) / 16)), dim3(1024), 0, (hipStream_t)c.stream,
+                       (const float*)workspace, c.rows ? (int)s.groups : 0, c.n, dw);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? VQ2_OK : set_hip_error(e, "vq2_add_rms_norm_backward");
 }
