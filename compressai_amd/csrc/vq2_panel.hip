@@ -17,11 +17,13 @@
 // bits: exact for fp16, bf16 and 8-bit rows but for values 2^-28 below the
 // row's largest).  A weight is the fp32 sum of its stages' centroids, exact
 // in fp16 for one stage of fp16 codebooks; otherwise it is rounded to fp16
-// where only bf16 results depend on it (half a step is 2^-12 of a weight,
-// against 2^-9 of the result), and held as two fp16 parts, multiplied one
-// after the other, where an fp16 or fp32 result does.  Row scales stay outside, in fp32.  A gradient is
-// rounded to fp16 once between its two products (half a step is 2^-12 of each
-// term; what comes of it has 16 bits); everything else is fp32.
+// where only bf16 results depend on it (half a step is 2^-11 of a weight,
+// against 2^-8 of the result), and held as two fp16 parts, multiplied one
+// after the other, where an fp16 or fp32 result does.  Row scales stay outside,
+// in fp32.  A gradient is rounded to fp16 once between its two products (2^-11
+// of each term; what comes of it has 16 bits), under powers of two that hold the
+// largest; in the block's backward pass that leaves 20 bits for |u f'(g)| and |f(g)|
+// above an upstream value, past which dx overflows.  Everything else is fp32.
 #include <algorithm>
 #include <mutex>
 
@@ -100,7 +102,6 @@ __device__ __forceinline__ int64_t mat_row(const MatArgs& a, int64_t tile, int r
 // its chunk q of a k tile of 32 rows as long as the columns' panel has the
 // same order (value m of chunk q: row 16 (m / 4) + 4 q + m % 4).  So a
 // gradient is stored as it is made, a KiB a tile.
-__device__ __forceinline__ int chunk_row(int q, int m) { return 16 * (m >> 2) + 4 * q + (m & 3); }
 
 // -------------------------------------------------------------- prologue
 // One launch: token rows, upstream rows' factors, row scales.
@@ -967,7 +968,7 @@ struct DyArgs {
     half8_t* p;       // [tp / 16][vkt][64]
     int vkt;
 };
-// The panel of dy * scale * 2^-e in the order of the columns' panel (chunk_row):
+// The panel of dy * scale * 2^-e in the order of the columns' panel:
 // two runs of 4 rows a lane.  A wave 4 k tiles of 16 tokens.
 __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 {

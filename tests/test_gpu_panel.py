@@ -7,8 +7,8 @@ A product of K terms takes K / 32 steps of the matrix core (twice as many
 where weights are held in two parts), each rounding the running sum a few
 times: it is off by at most (K / 4) 2^-24 of the sum of its terms' magnitudes,
 M = sum |x_k w_k|, to which the second part's own rounding adds 2^-22 of them.
-A weight that is rounded to fp16 once (results in bf16) is off by 2^-12 of
-itself: 2^-12 M.  Rounding a result adds half a step.  A gradient is rounded to fp16 between
+A weight that is rounded to fp16 once (results in bf16) is off by 2^-11 of
+itself: 2^-11 M.  Rounding a result adds half a step.  A gradient is rounded to fp16 between
 its two products: 2^-11 of each term (and 2^-25 of the largest scale's), so
 2^-11 of the sum of the terms' magnitudes.  exp and log are good to 2^-20 of
 their results over these ranges (__expf: a rounded product with log2 e, so
@@ -80,7 +80,7 @@ def rows_of(seed, T, n, dtype):
 def product_err(x64, m, rounded):
     """bound of a raw product's error (before its scale)"""
     mag = x64.abs() @ m.w.abs().t()
-    return mag * (x64.shape[1] / 4 * E + 2.0 ** -22 + (2.0 ** -12 if rounded and not m.exact else 0))
+    return mag * (x64.shape[1] / 4 * E + 2.0 ** -22 + (2.0 ** -11 if rounded and not m.exact else 0))
 
 
 def act64(a, g):
@@ -146,8 +146,8 @@ def test_gated_backward(dev, T, rows, n, xdt, stages, cdt, sdt):
         floor = 2.0 ** -19 * d64.abs().amax(-1, keepdim=True) if rows else 0
         top = torch.maximum(g.s.max(), u.s.max())
         pg, pu = (t.abs() * 2.0 ** -11 * m.s + floor * top * 2 for t, m in ((tg, g), (tu, u)))
-        w12 = 2.0 ** -12 if x.dtype == torch.bfloat16 and not g.exact else 0.0
-        rel = (2 * rows / 4) * E + 2.0 ** -22 + w12
+        w11 = 2.0 ** -11 if x.dtype == torch.bfloat16 and not g.exact else 0.0
+        rel = (2 * rows / 4) * E + 2.0 ** -22 + w11
         tol = 1.25 * ((etg * g.s + pg + rel * (tg * g.s).abs()) @ g.w.abs() + (etu * u.s + pu + rel * (tu * u.s).abs()) @ u.w.abs())
         off = (got.cpu().double() - want).abs() - tol - half(x.dtype, want)
         assert off.numel() == 0 or off.max() <= 0, float(off.max())
@@ -177,8 +177,8 @@ def test_gemm_backward(dev, T, rows, n, xdt, stages, cdt, sdt):
     want = t @ m.w
     # the row's largest value lies in [2^14, 2^15) before its scale: what fp16 cannot hold is below 2^-39 of it
     p = t.abs() * 2.0 ** -11 + 2.0 ** -38 * d64.abs().amax(-1, keepdim=True) * m.s.max() if rows and T else t.abs()
-    w12 = 2.0 ** -12 if x.dtype == torch.bfloat16 and not m.exact else 0.0
-    tol = (p + (rows / 4 * E + 2.0 ** -22 + w12) * t.abs()) @ m.w.abs()
+    w11 = 2.0 ** -11 if x.dtype == torch.bfloat16 and not m.exact else 0.0
+    tol = (p + (rows / 4 * E + 2.0 ** -22 + w11) * t.abs()) @ m.w.abs()
     off = (dx.cpu().double() - want).abs() - tol - half(dx.dtype, want)
     assert off.numel() == 0 or off.max() <= 0, float(off.max())
     raw = x64 @ m.w.t()
@@ -241,9 +241,9 @@ def test_head_loss_backward(dev, T, rows, n, xdt, stages, cdt, sdt):
     elog = ez + (ez.amax(-1, keepdim=True) if rows else 0) + 2.0 ** -19 + 4 * E * (lse64.abs()[:, None] + z.abs())
     ep = torch.exp(z - lse64[:, None]) * (elog + 2.0 ** -20)
     want = up * ((p * m.s * 2.0) @ m.w)
-    w12 = 2.0 ** -12 if x.dtype == torch.bfloat16 and not m.exact else 0.0
+    w11 = 2.0 ** -11 if x.dtype == torch.bfloat16 and not m.exact else 0.0
     # fp16 of p s / 2^e 2^14: 2^-11 of it, and 2^-25 2^-14 of the largest scale
-    tp = p.abs() * m.s * 2.0 * (2.0 ** -11 + rows / 4 * E + 2.0 ** -22 + w12) + ep * m.s * 2.0 + 2.0 ** -38 * 2 * m.s.max()
+    tp = p.abs() * m.s * 2.0 * (2.0 ** -11 + rows / 4 * E + 2.0 ** -22 + w11) + ep * m.s * 2.0 + 2.0 ** -38 * 2 * m.s.max()
     tol = up.abs() * (tp @ m.w.abs()) + 4 * E * want.abs()
     off = (dx.cpu().double() - want).abs() - tol - half(x.dtype, want)
     assert off.numel() == 0 or off.max() <= 0, float(off.max())
@@ -398,6 +398,171 @@ def test_graph_streams_and_runs(dev):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def _views(t, off, dev):
+    """the tensor at an address that is only aligned to its elements"""
+    buf = torch.empty(t.numel() + off, dtype=t.dtype, device=dev)
+    v = buf[off:].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("T", [1, 5, 100, 300])
+@pytest.mark.parametrize("stages", [1, 2, 3])
+def test_planes_and_rows_at_any_address(dev, T, stages):
+    """planes, scales and upstream rows aligned to their elements alone, and rows no multiple of 4: the aligned call's
+    results up to the order of sums (2^-20 of the largest).  Few aligned tokens go through a kernel that multiplies the stages one by
+    one, unaligned ones through panels, whose weights of two stages are rounded to fp16 for the block's bf16 result (2^-11 of
+    each): its g and u are then 2^-11 of M apart, M the sum of their terms' magnitudes, and f(g) u |f'| <= 1.13 times that by
+    |u|, and |f| times it"""
+    n, rows = 128, 203
+    cb = books("fp16")
+    a, b = Mat(300, rows, n, stages, cb), Mat(303, rows, n, stages, cb)
+    x = rows_of(T, T, n, "bf16")[0].to(dev)
+    d = (synth.activations(5, (T, rows), torch.float32) * 1e-2).to(torch.bfloat16)
+    t = torch.randint(0, rows, (T,), generator=synth.gen(T)).to(dev)
+    dl = torch.ones(T, device=dev)
+
+    def all_of(put, dy):
+        (a0, a1, c0, c1, sa), (b0, b1, _, _, sb) = ((put(m.i0), None if m.i1 is None else put(m.i1), m.cb0.to(dev),
+                                                    None if m.cb1 is None else m.cb1.to(dev), put(m.scale)) for m in (a, b))
+        gate, up, head = (a0, a1, sa), (b0, b1, sb), (a0, a1, c0, c1, sa, rows, n)
+        loss, lse = K.vq_head_loss(x, t, *head)
+        return (loss, lse, K.vq_gated_rows(x, gate, up, c0, c1, n), *K.vq_head_loss_backward(x, t, lse, dl, *head, scale_grad=True),
+                *K.vq_gated_rows_backward(dy, x, gate, up, c0, c1, n, scale_grad=True), *K.vq_gemm_backward(dy, x, *head, scale_grad=True))
+
+    want = all_of(lambda v: v.to(dev), d.to(dev))
+    got = all_of(lambda v: _views(v, 1, dev), _views(d, 1, dev))
+    for k, (p, q) in enumerate(zip(got, want)):
+        step = 0 if p.dtype == torch.float32 else 2.0 ** -7  # (a sum near a border may round the other way)
+        tol = step * q.double().abs() + 2.0 ** -20 * q.double().abs().max()
+        if k == 2 and stages > 1:
+            x64 = x.double().cpu()
+            g, v = x64 @ a.w.t() * a.s, x64 @ b.w.t() * b.s
+            eg, ev = (2.0 ** -11 * (x64.abs() @ w.w.abs().t()) * w.s for w in (a, b))
+            tol = tol + (1.13 * eg * (v.abs() + ev) + act64("silu", g)[0].abs() * ev).to(dev)
+        assert ((p.double() - q.double()).abs() <= tol).all(), k
+
+
+LARGE = [  # sizes that fill the device: wave tiles of 128 rows, several pieces of a matrix, one and more slices
+    ("loss", 1100, 17000, 64), ("loss", 2500, 40000, 64), ("gated", 2050, 4100, 64), ("gated", 300, 9000, 64),
+    ("product", 2048, 100, 4096), ("product", 2048, 600, 4096), ("product", 4100, 300, 2048), ("product", 130, 40000, 64)]
+
+
+@pytest.mark.parametrize("kind,T,rows,n", LARGE)
+@pytest.mark.parametrize("stages", [1, 2])
+def test_large(dev, kind, T, rows, n, stages):
+    """as the tests above, the 64-bit side on the GPU"""
+    x, _, _ = rows_of(T + 9, T, n, "bf16")
+    x = x.to(dev)
+    x64 = x.double()
+    cb = books("fp16")
+    m, u = Mat(400 + rows, rows, n, stages, cb, "fp32"), Mat(403 + rows, rows, n, stages, cb, "fp32")
+    for k in (m, u):
+        k.w, k.s = k.w.to(dev), k.s.to(dev)
+    i0, i1, cb0, cb1, sc = m.on(dev)
+    head = (i0, i1, cb0, cb1, sc, rows, n)
+    gen = torch.Generator(device=dev).manual_seed(T)
+    if kind == "loss":
+        t = torch.randint(0, rows, (T,), generator=gen, device=dev)
+        t[::3] = -100
+        dl = torch.rand(T, generator=gen, device=dev)
+        loss, lse = K.vq_head_loss(x, t, *head)
+        dx, ds = K.vq_head_loss_backward(x, t, lse, dl, *head, scale_grad=True)
+        z, lse64, want, used = loss64(x64, m, t, 1.0, -100)
+        ez = product_err(x64, m, False) * m.s + 4 * E * z.abs()
+        el = ez.amax(-1) + 2.0 ** -19 + 4 * E * lse64.abs()
+        assert ((lse.double() - lse64).abs() <= el).all()
+        assert ((loss.double() - want).abs() <= torch.where(used, 2 * el + 2 * E * (want.abs() + lse64.abs()), 0.0)).all()
+        p = torch.exp(z - lse64[:, None])
+        ep = p * (ez + el[:, None] + 2.0 ** -18 + 4 * E * z.abs())
+        p[torch.arange(T, device=dev)[used], t[used]] -= 1
+        p[~used] = 0
+        up = torch.where(used, dl.double(), 0.0)[:, None]
+        want = up * ((p * m.s) @ m.w)
+        tp = p.abs() * m.s * (2.0 ** -11 + rows / 4 * E + 2.0 ** -22 + (0 if m.exact else 2.0 ** -11)) + ep * m.s + 2.0 ** -38 * m.s.max()
+        assert ((dx.double() - want).abs() <= up.abs() * (tp @ m.w.abs()) + half(x.dtype, want) + 4 * E * want.abs()).all()
+        raw = z / m.s
+        eds = (up.abs() * (ep * raw.abs() + (p.abs() + ep) * ez / m.s + (T + 8) * E * (p * raw).abs())).sum(0) + 1e-30
+        assert ((ds.double() - (up * p * raw).sum(0)).abs() <= eds).all()
+        return
+    d = (torch.randn(T, rows, generator=gen, device=dev) * 1e-3).to(torch.bfloat16)
+    d64 = d.double()
+    if kind == "product":
+        dx, ds = K.vq_gemm_backward(d, x, *head, scale_grad=True)
+        t = d64 * m.s
+        w11 = 0.0 if m.exact else 2.0 ** -11
+        tol = (t.abs() * (2.0 ** -11 + rows / 4 * E + 2.0 ** -22 + w11) + 2.0 ** -38 * d64.abs().amax(-1, keepdim=True) * m.s.max()) @ m.w.abs()
+        assert ((dx.double() - t @ m.w).abs() <= tol + half(x.dtype, t @ m.w)).all()
+        raw = x64 @ m.w.t()
+        tol = (d64.abs() * product_err(x64, m, False) + (T + 8) * E * (d64 * raw).abs()).sum(0) + 1e-30
+        assert ((ds.double() - (d64 * raw).sum(0)).abs() <= tol).all()
+        return
+    gate, up = (i0, i1, sc), (u.i0.to(dev), None if u.i1 is None else u.i1.to(dev), u.scale.to(dev))
+    y = K.vq_gated_rows(x, gate, up, cb0, cb1, n)
+    dx, _, _ = K.vq_gated_rows_backward(d, x, gate, up, cb0, cb1, n)
+    g64, u64 = (x64 @ k.w.t() * k.s for k in (m, u))
+    eg, eu = (product_err(x64, k, True) * k.s + 4 * E * v.abs() for k, v in ((m, g64), (u, u64)))
+    f, df = act64("silu", g64)
+    tol = (1.13 * eg + 2.0 ** -20 * f.abs() + 2.0 ** -22 * g64.abs()) * (u64.abs() + eu) + f.abs() * eu
+    assert ((y.double() - f * u64).abs() <= tol + half(y.dtype, f * u64)).all()
+    tg, tu = d64 * u64 * df, d64 * f
+    want = (tg * m.s) @ m.w + (tu * u.s) @ u.w
+    etg = d64.abs() * (eu * (df.abs() + 1.2 * eg) + u64.abs() * (1.2 * eg + 2.0 ** -19 * (1 + g64.abs())))
+    etu = d64.abs() * (1.13 * eg + 2.0 ** -20 * f.abs() + 2.0 ** -22 * g64.abs())
+    floor = 2.0 ** -18 * d64.abs().amax(-1, keepdim=True) * max(m.s.max(), u.s.max())
+    rel = 2.0 ** -11 * (1 if m.exact else 2) + 2 * rows / 4 * E + 2.0 ** -22
+    tol = ((etg + rel * tg.abs()) * m.s + floor) @ m.w.abs() + ((etu + rel * tu.abs()) * u.s + floor) @ u.w.abs()
+    assert ((dx.double() - want).abs() <= tol + half(x.dtype, want)).all()
+
+
+def test_small_values(dev):
+    """rows, upstream rows and scales far below and above 1: powers of two scale results and nothing else"""
+    T, rows, n = 40, 96, 128
+    m, u = Mat(500, rows, n, 1, books("fp16"), "fp32"), Mat(503, rows, n, 1, books("fp16"), "fp32")
+    x = rows_of(7, T, n, "bf16")[0].to(dev)
+    d = synth.activations(8, (T, rows), torch.bfloat16).to(dev)
+    i0, _, cb0, _, sc = m.on(dev)
+    base = K.vq_gemm_backward(d, x, i0, None, cb0, None, sc, rows, n, scale_grad=True)
+    for e, f in ((-60, 0), (60, 0), (0, -50), (0, 50), (-40, 30)):
+        got = K.vq_gemm_backward(d * 2.0 ** e, x, i0, None, cb0, None, sc * 2.0 ** f, rows, n, scale_grad=True)
+        assert torch.equal(got[0].double(), base[0].double() * 2.0 ** (e + f))
+        assert torch.equal(got[1].double(), base[1].double() * 2.0 ** e)
+    # fp16 rows below fp16's normal numbers
+    tiny = (x.float() * 2.0 ** -18).half()
+    y = K.vq_gated_rows(tiny, (i0, None, sc * 2.0 ** 18), (u.i0.to(dev), None, u.scale.to(dev) * 2.0 ** 18), cb0, None, n, out_dtype=torch.float32)
+    x64 = tiny.double().cpu() * 2.0 ** 18
+    g, v = x64 @ m.w.t() * m.s, x64 @ u.w.t() * u.s
+    want = act64("silu", g)[0] * v
+    eg, eu = product_err(x64, m, False) * m.s, product_err(x64, u, False) * u.s
+    tol = (1.13 * eg + 2.0 ** -20 * g.abs()) * (v.abs() + eu) + act64("silu", g)[0].abs() * eu + 2.0 ** -22 * want.abs()
+    assert ((y.cpu().double() - want).abs() <= tol).all()
+    one = K.vq_gated_rows(tiny[:1], (i0, None, sc * 2.0 ** 18), (u.i0.to(dev), None, u.scale.to(dev) * 2.0 ** 18), cb0, None, n,
+                          out_dtype=torch.float32)
+    assert ((one.cpu().double() - want[:1]).abs() <= tol[:1]).all()
+
+
+def test_nan_and_infinity_stay_in_their_rows(dev):
+    T, rows, n = 150, 64, 64
+    m, u = Mat(510, rows, n, 1, books("fp16")), Mat(513, rows, n, 1, books("fp16"))
+    i0, _, cb0, _, sc = m.on(dev)
+    gate, up = (i0, None, sc), (u.i0.to(dev), None, u.scale.to(dev))
+    x = rows_of(11, T, n, "bf16")[0].to(dev)
+    d = synth.activations(12, (T, rows), torch.bfloat16).to(dev)
+    bx, bd = x.clone(), d.clone()
+    bx[3, 5], bx[70, 0], bd[9, 1], bd[140, 63] = math.nan, math.inf, math.nan, -math.inf
+    hit = torch.zeros(T, dtype=torch.bool, device=dev)
+    hit[[3, 70, 9, 140]] = True
+    for few in (T, 20):
+        a, b = K.vq_gated_rows(x[:few], gate, up, cb0, None, n), K.vq_gated_rows(bx[:few], gate, up, cb0, None, n)
+        keep = ~hit[:few]
+        assert torch.equal(a[keep], b[keep]) and not torch.isfinite(b[3]).all()
+    for f in (lambda p, q: K.vq_gated_rows_backward(q, p, gate, up, cb0, None, n)[0],
+              lambda p, q: K.vq_gemm_backward(q, p, i0, None, cb0, None, sc, rows, n)[0]):
+        a, b = f(x, d), f(bx, bd)
+        assert torch.equal(a[~hit], b[~hit])
+        assert not torch.isfinite(b[9]).any() and not torch.isfinite(b[140]).all()
 
 
 def test_refusals(dev):
