@@ -1042,7 +1042,7 @@ __device__ __forceinline__ half8_t centroid_f16(half8_t h)
 }
 
 template <int CBT, int S2, int TT, int KW, bool OWN, class Epi>
-__global__ void __launch_bounds__(256, TT == 8 || OWN ? 2 : 3) few_kernel(const FewArgs a, Epi epi)
+__global__ void __launch_bounds__(256, TT >= 6 || OWN ? 2 : 3) few_kernel(const FewArgs a, Epi epi)
 {
     static_assert((KW == 4 || KW == 1) && (!OWN || (TT == 1 && KW == 4)), "");
     constexpr int JU = S2 == VQ2_S2_NONE && TT <= 4 ? 8 : 4;  // k tiles whose centroids are on their way together
@@ -1391,17 +1391,21 @@ int64_t few_pairs(const PanelCall& c) { return ((c.rows + 15) / 16 * c.nmat + 1)
 
 // Its token tiles a workgroup, and whether a wave of 128 tokens has its rows to
 // itself.
-int few_tiles(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : tokens <= 64 ? 4 : 8; }
-bool few_alone(int64_t pairs) { return pairs >= 1024; }
+int few_tiles(int64_t tokens)
+{
+    if (tokens <= 64) return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4;
+    return tokens <= (tokens + 127) / 128 * 96 ? 6 : 8;  // as many blocks as of 8, but no larger than they have to be
+}
+bool few_alone(int tt, int64_t pairs) { return tt >= 6 && pairs >= 1024; }
 
 // Its workgroups along the pairs of tiles: for the loss as many as are
 // resident, each keeps running sums over its pairs.
 int few_groups(const PanelCall& c, int64_t tokens)
 {
     const int tt = few_tiles(tokens);
-    const int64_t pairs = few_pairs(c), units = tt == 8 && few_alone(pairs) ? (pairs + 3) / 4 : pairs;
+    const int64_t pairs = few_pairs(c), units = few_alone(tt, pairs) ? (pairs + 3) / 4 : pairs;
     if (c.what != PANEL_STATS) return (int)units;
-    return (int)std::min<int64_t>(units, (int64_t)device_cu_count() * (tt == 8 || few_own(tokens, c.x_dt) ? 2 : 3));
+    return (int)std::min<int64_t>(units, (int64_t)device_cu_count() * (tt >= 6 || few_own(tokens, c.x_dt) ? 2 : 3));
 }
 
 // Whether few_kernel is ahead of panels: it gathers every centroid once for
@@ -1569,8 +1573,13 @@ hipError_t few_typed(const FewArgs& a, const Epi& e, int tt, int groups, hipStre
     else if (tt == 1) hipLaunchKernelGGL((few_kernel<CBT, S2, 1, 4, false, Epi>), grid, block, 0, st, a, e);
     else if (tt == 2) hipLaunchKernelGGL((few_kernel<CBT, S2, 2, 4, false, Epi>), grid, block, 0, st, a, e);
     else if (tt == 4) hipLaunchKernelGGL((few_kernel<CBT, S2, 4, 4, false, Epi>), grid, block, 0, st, a, e);
-    else if (few_alone(a.pairs)) hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, false, Epi>), grid, block, 0, st, a, e);
-    else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 4, false, Epi>), grid, block, 0, st, a, e);
+    else if (few_alone(tt, a.pairs)) {
+        if (tt == 6) hipLaunchKernelGGL((few_kernel<CBT, S2, 6, 1, false, Epi>), grid, block, 0, st, a, e);
+        else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 1, false, Epi>), grid, block, 0, st, a, e);
+    } else {
+        if (tt == 6) hipLaunchKernelGGL((few_kernel<CBT, S2, 6, 4, false, Epi>), grid, block, 0, st, a, e);
+        else hipLaunchKernelGGL((few_kernel<CBT, S2, 8, 4, false, Epi>), grid, block, 0, st, a, e);
+    }
     return hipGetLastError();
 }
 
@@ -1670,7 +1679,7 @@ int panel_launch(const PanelCall& c)
                 TRY(few(f, gated, tt, groups, c.cb_dt, c.s2, st));
             } else {
                 TRY(few(f, stats, tt, groups, c.cb_dt, c.s2, st));
-                TRY(lse_launch(tt == 8 && few_alone(few_pairs(c)) ? groups * 4 : groups));
+                TRY(lse_launch(few_alone(tt, few_pairs(c)) ? groups * 4 : groups));
             }
             continue;
         }
