@@ -22,8 +22,9 @@
 // after the other, where an fp16 or fp32 result does.  Row scales stay outside,
 // in fp32.  A gradient is rounded to fp16 once between its two products (2^-11
 // of each term; what comes of it has 16 bits), under powers of two that hold the
-// largest; in the block's backward pass that leaves 20 bits for |u f'(g)| and |f(g)|
-// above an upstream value, past which dx overflows.  Everything else is fp32.
+// largest: of a token's upstream values, of the row scales, and in the block's
+// backward pass of |u f'(g)| and |f(g)|, which a bound on the products holds
+// (BlockBound).  Everything else is fp32.
 #include <algorithm>
 #include <mutex>
 
@@ -61,6 +62,26 @@ __device__ __forceinline__ int scale_exponent(const RowTop& t)
     const int b = (int)(__float_as_uint(wave_max_all(m)) >> 23);
     return b == 0xFF ? 0 : min(max(b - 126, -100), 100);
 }
+
+// The block's backward pass: exponent of a power of two above 1.13 |u| and 1.13 |g| of a
+// token, which bounds |u f'(g)| and |f(g)|, from the largest of its row, of the
+// codebooks and of the scales, and the row's length.  Of random rows the largest of them
+// is some 2^10 smaller, which fp16's 30 binades hold.
+struct BlockBound {
+    RowTop amax, books;
+    const float* fac;  // of the token rows: |x| < 2^14 fac
+    int bits;          // 14 + log2(n), rounded up, + 1, + 1 for a second stage
+    // the part that tokens share; called by whole waves
+    __device__ __forceinline__ int common() const
+    {
+        float m = 0.0f;
+        for (int i = threadIdx.x & 63; i < books.n; i += 64) m = fmaxf(m, books.part[i]);
+        return bits + scale_exponent(amax) + exponent_of(wave_max_all(m)) + 1;
+    }
+    __device__ __forceinline__ int of(int common, int t) const { return common + exponent_of(fac[t]); }
+};
+// 2^e as far as it is a normal number
+__device__ __forceinline__ float pow2_near(int e) { return pow2(min(max(e, -126), 126)); }
 
 // over the four lanes that hold a token's rows
 __device__ __forceinline__ float max_rows(float v)
@@ -184,8 +205,7 @@ struct DyMaxArgs {
     const void* dy;
     int dy_dt, tokens, vec;  // vec: rows a multiple of 8, 16-byte aligned
     int64_t rows;
-    int head;     // bits left above the row's largest value
-    float* dfac;  // [tp]: 2^-e, which brings the row's largest into [2^(14 - head), 2^(15 - head))
+    float* dfac;  // [tp]: 2^-e, which brings the row's largest into [2^14, 2^15)
     int groups;   // of 16 rows
 };
 // a wave a row
@@ -209,7 +229,7 @@ __device__ __forceinline__ void dy_max(const DyMaxArgs& a, int group)
         }
     }
     m = wave_max_all(m);
-    const int e = m > 0.0f ? min(max(exponent_of(m) - 14 + a.head, -110), 110) : 0;
+    const int e = m > 0.0f ? min(max(exponent_of(m) - 14, -110), 110) : 0;
     if (lane == 0) a.dfac[t] = pow2(-e);
 }
 
@@ -243,10 +263,39 @@ __device__ __forceinline__ void prep_scales(const PrepArgs& a, int group, float*
     a.top[group] = m;
 }
 
+// The codebooks' largest magnitudes, BOOK_VALUES values a workgroup.
+struct BookArgs {
+    const void* cb[2];
+    int cb_dt, n0;          // workgroups of the first
+    int64_t values[2];      // multiples of 8
+    float* top;             // of each workgroup
+    int groups;
+};
+constexpr int BOOK_VALUES = 8 * 64 * PK_WAVES;
+template <int CBT>
+__device__ __forceinline__ void book_max(const BookArgs& a, int group, float* s_top)
+{
+    const int k = group >= a.n0;
+    const int64_t at = (int64_t)(group - (k ? a.n0 : 0)) * BOOK_VALUES + threadIdx.x * 8;
+    float m = 0.0f;
+    if (at < a.values[k]) {
+        const Eight e = load8(a.cb[k], CBT, at);
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(e.v[j]));
+    }
+    m = wave_max_all(m);
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 0; w < PK_WAVES; w++) m = fmaxf(m, s_top[w]);
+    a.top[group] = m;
+}
+
 struct PrologueArgs {
     PackArgs pack;
     DyMaxArgs dy;
     PrepArgs prep;
+    BookArgs book;
 };
 __global__ void __launch_bounds__(64 * PK_WAVES) prologue_kernel(const PrologueArgs a)
 {
@@ -265,7 +314,12 @@ __global__ void __launch_bounds__(64 * PK_WAVES) prologue_kernel(const PrologueA
         if (a.dy.dy_dt == VQ2_DT_BF16) return dy_max<VQ2_DT_BF16>(a.dy, b);
         return dy_max<VQ2_DT_F32>(a.dy, b);
     }
-    prep_scales(a.prep, b - a.dy.groups, s_m[0]);
+    b -= a.dy.groups;
+    if (b < a.prep.groups) return prep_scales(a.prep, b, s_m[0]);
+    b -= a.prep.groups;
+    if (a.book.cb_dt == VQ2_DT_F16) return book_max<VQ2_DT_F16>(a.book, b, s_m[0]);
+    if (a.book.cb_dt == VQ2_DT_BF16) return book_max<VQ2_DT_BF16>(a.book, b, s_m[0]);
+    book_max<VQ2_DT_F32>(a.book, b, s_m[0]);
 }
 
 template <int CBT>
@@ -771,7 +825,7 @@ struct DgatedEpi {
     const float* fac;
     const float* dfac;  // [tp]: 2^-e of the token's upstream row (dy_max)
     Upstream up;
-    RowTop amax;
+    BlockBound bound;
     int tp, vkt;
     int64_t tile0;
     half8_t* p;
@@ -782,12 +836,14 @@ struct DgatedEpi {
     __device__ __forceinline__ void run_act(f32x4_t (&acc)[MT][PG_NT], int64_t tile, int tok)
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
-        const float c = pow2(-scale_exponent(amax));
-        float x[PG_NT], k[PG_NT];
+        const float c = pow2(-scale_exponent(bound.amax));
+        const int common = bound.common();
+        float x[PG_NT], k[PG_NT], b[PG_NT];  // (two factors: their product may leave fp32's range)
 #pragma unroll
         for (int j = 0; j < PG_NT; j++) {
             x[j] = fac[tok + j * 16 + nl];
             k[j] = dfac[tok + j * 16 + nl];
+            b[j] = pow2_near(-bound.of(common, tok + j * 16 + nl));
         }
 #pragma unroll
         for (int i = 0; i < MT; i += 2) {
@@ -805,8 +861,8 @@ struct DgatedEpi {
                     float f, df;
                     gate_act<ACT>(rg * sg[e], f, df);
                     const float dg = d[j][e] * (ru * su[e]) * df, du = d[j][e] * f;
-                    h[e] = (_Float16)(dg * k[j] * (sg[e] * c));
-                    h[4 + e] = (_Float16)(du * k[j] * (su[e] * c));
+                    h[e] = (_Float16)(dg * k[j] * b[j] * (sg[e] * c));
+                    h[4 + e] = (_Float16)(du * k[j] * b[j] * (su[e] * c));
                     if (ds) {
                         dsg[e] += dg * rg;
                         dsu[e] += du * ru;
@@ -871,29 +927,35 @@ struct DxFactor {
     const float* dloss;
     const int64_t* target;
     int64_t rows, ignore;
-    float base;         // by init(), called by whole waves
-    __device__ __forceinline__ void init() { base = pow2(scale_exponent(amax) - (dfac ? 0 : 14)); }
+    BlockBound bound;   // of the block; bits 0: none
+    int e;              // by init(), called by whole waves
     // (two factors: their product may leave fp32's range)
-    __device__ __forceinline__ float apply(float v, float f, bool skip) const { return skip ? 0.0f : v * base * f; }
-    __device__ __forceinline__ float of(int t, bool& skip) const
+    struct Of {
+        float a, b;
+        bool skip;
+        __device__ __forceinline__ float operator()(float v) const { return skip ? 0.0f : v * b * a; }
+    };
+    __device__ __forceinline__ void init()
     {
-        skip = false;
-        if (dfac) return 1.0f / dfac[t];
+        e = scale_exponent(amax) - (dfac ? 0 : 14);
+        if (bound.bits) e += bound.common();
+    }
+    __device__ __forceinline__ Of of(int t) const
+    {
+        if (dfac) return Of{1.0f / dfac[t], pow2_near(bound.bits ? bound.of(e, t) : e), false};
         const int64_t v = target_of(target, t, ignore, rows);
-        skip = v == TARGET_SKIP;
-        return v == TARGET_BAD ? __builtin_nanf("") : dloss[t];
+        return Of{v == TARGET_BAD ? __builtin_nanf("") : dloss[t], pow2(e), v == TARGET_SKIP};
     }
 };
 
 // 8 (4) neighbouring columns of dx in 16 bits: element e of N tiles' values
 template <int N>
-__device__ __forceinline__ void store_run(void* dx, int dt, int64_t at, const f32x4_t (&v)[N], int e, float f, const DxFactor& fac,
-                                          bool skip)
+__device__ __forceinline__ void store_run(void* dx, int dt, int64_t at, const f32x4_t (&v)[N], int e, const DxFactor::Of& f)
 {
     uint32_t w[N / 2];
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float a = fac.apply(v[i][e], f, skip), b = fac.apply(v[i + 1][e], f, skip);
+        const float a = f(v[i][e]), b = f(v[i + 1][e]);
         w[i / 2] = dt == VQ2_DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16 : bf16_pair(a, b);
     }
     uint32_t* o = (uint32_t*)((uint16_t*)dx + at);
@@ -922,8 +984,7 @@ struct GradEpi {
             for (int j = 0; j < PG_NT; j++) {
                 const int t = tok + j * 16 + nl;
                 if (t >= tokens) continue;
-                bool skip;
-                const float f = fac.of(t, skip);
+                const DxFactor::Of f = fac.of(t);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int64_t col = c0 + (q * 4 + e) * 8;
@@ -931,7 +992,7 @@ struct GradEpi {
                     f32x4_t v[MT];
 #pragma unroll
                     for (int i = 0; i < MT; i++) v[i] = acc[i][j];
-                    store_run(dx, dx_dt, (int64_t)t * n + col, v, e, f, fac, skip);
+                    store_run(dx, dx_dt, (int64_t)t * n + col, v, e, f);
                 }
             }
             return;
@@ -1319,12 +1380,11 @@ __global__ void __launch_bounds__(256) dx_kernel(const DxArgs a)
         }
     }
     if (t >= a.tokens) return;
-    bool skip;
-    const float f = fac.of(t, skip);
+    const DxFactor::Of f = fac.of(t);
 #pragma unroll
     for (int e = 0; e < (SPLIT ? 1 : 4); e++) {
         const int64_t col = g * 128 + (q * 4 + (SPLIT ? wave : e)) * 8;
-        if (col < a.n) store_run(a.dx, a.dx_dt, (int64_t)t * a.n + col, v, e, f, fac, skip);
+        if (col < a.n) store_run(a.dx, a.dx_dt, (int64_t)t * a.n + col, v, e, f);
     }
 }
 
@@ -1432,13 +1492,20 @@ struct Plan {
     bool few[2];         // few_kernel for a whole chunk, and for the last one
     int mt, gmt;         // tiles of a wave: the first product's, the gradient's
     int tops;            // workgroups of prep_scales
+    int books;           // of book_max
     int parts, tparts, kt;  // parts of a weight in the rows' panel, and the columns'
     int64_t np;          // columns, padded
     int slices;
-    size_t fac, top, sc, xp, w, wt, p, acc, stats, at, ds, dfac, total;
+    size_t fac, top, book, sc, xp, w, wt, p, acc, stats, at, ds, dfac, total;
 };
 
 enum { STATS = PANEL_STATS, DLOGIT = PANEL_DLOGIT, GATED = PANEL_GATED, DGATED = PANEL_DGATED, PRODUCT = PANEL_PRODUCT };
+
+// values of a stage's codebook
+int64_t book_values(const PanelCall& c, int stage)
+{
+    return stage == 0 || c.s2 == VQ2_S2_U16 ? 65536 * 8 : c.s2 == VQ2_S2_U8 ? 256 * 8 : 0;
+}
 
 Plan plan_of(const PanelCall& c)
 {
@@ -1470,6 +1537,8 @@ Plan plan_of(const PanelCall& c)
     p.fac = b.take(p.tp * 4);
     p.tops = (int)((p.tiles * 16 + PREP_ROWS - 1) / PREP_ROWS);
     p.top = b.take(p.tops * 4);
+    p.books = c.what == DGATED ? (int)((book_values(c, 0) + book_values(c, 1) + BOOK_VALUES - 1) / BOOK_VALUES) : 0;
+    p.book = b.take(p.books * 4);
     p.sc = b.take(p.tiles * 16 * 4);
     p.xp = b.take(p.tp * c.n * 2);
     const bool w = c.what != PRODUCT || c.ds[0];  // (also where few_kernel is ahead: it needs aligned planes)
@@ -1636,6 +1705,12 @@ int panel_launch(const PanelCall& c)
     f32x4_t* acc = (f32x4_t*)(ws + p.acc);
     float* ds = c.ds[0] ? (float*)(ws + p.ds) : nullptr;
     float* dfac = (float*)(ws + p.dfac);
+    BlockBound bound{amax, {(const float*)(ws + p.book), p.books}, fac, 0};
+    if (c.what == DGATED) {
+        int lg = 0;
+        while ((int64_t)1 << lg < c.n) lg++;
+        bound.bits = 14 + lg + 1 + (c.s2 != VQ2_S2_NONE);
+    }
     bool prepared = false;  // the row scales
     const int64_t xsize = c.x_dt == VQ2_DT_F32 ? 4 : c.x_dt <= VQ2_DT_BF16 ? 2 : 1;
     for (int64_t t0 = 0; t0 < c.tokens; t0 += p.chunk) {
@@ -1647,7 +1722,7 @@ int panel_launch(const PanelCall& c)
         const int64_t* target = c.target ? c.target + t0 : nullptr;
         const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;
         void* dx = c.y && grad ? (char*)c.y + t0 * c.n * dt_size(c.y_dt) : nullptr;
-        const DxFactor dxf{amax, c.what == DLOGIT ? nullptr : dfac, c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore, 0.0f};
+        const DxFactor dxf{amax, c.what == DLOGIT ? nullptr : dfac, c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore, bound, 0};
         const Upstream upstream{dy, c.dy_dt, tokens,
                                 c.dy_dt != VQ2_DT_F32 && c.rows % 4 == 0 && (uintptr_t)dy % 8 == 0, c.rows};
         const bool prep = !few_call && !prepared;
@@ -1655,10 +1730,12 @@ int panel_launch(const PanelCall& c)
         const PrologueArgs pro{
             PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n, c.x_scale ? c.x_scale + t0 : nullptr, xp, fac,
                      first && !(few_call && few_own(tokens, c.x_dt)) ? tp / 16 : 0},
-            DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, c.what == DGATED ? 19 : 0, dfac,
+            DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, dfac,
                       c.what == DGATED || c.what == PRODUCT ? tp / 16 : 0},
-            PrepArgs{mats, c.rs, ds_ld, sc, top, prep ? p.tops : 0}};
-        if (const int groups = pro.pack.tiles + pro.dy.groups + pro.prep.groups) {
+            PrepArgs{mats, c.rs, ds_ld, sc, top, prep ? p.tops : 0},
+            BookArgs{{c.cb0, c.cb1}, c.cb_dt, (int)(book_values(c, 0) / BOOK_VALUES), {book_values(c, 0), book_values(c, 1)},
+                     (float*)(ws + p.book), prep ? p.books : 0}};
+        if (const int groups = pro.pack.tiles + pro.dy.groups + pro.prep.groups + pro.book.groups) {
             hipLaunchKernelGGL(prologue_kernel, dim3((unsigned)groups), dim3(64 * PK_WAVES), 0, st, pro);
             TRY(hipGetLastError());
         }
@@ -1696,7 +1773,7 @@ int panel_launch(const PanelCall& c)
                 TRY(gemm(g, p.mt, DlogitEpi{sc, fac, c.lse + t0, c.dloss + t0, target, amax, c.rows, c.ignore, tile0, tokens, tp, vkt,
                                           pp, ds, ds_ld}, tile0, st));
             else if (c.what == DGATED)
-                TRY(gemm(g, p.mt, DgatedEpi{sc, fac, dfac, upstream, amax, tp, vkt, tile0, pp, ds, ds_ld, c.act},
+                TRY(gemm(g, p.mt, DgatedEpi{sc, fac, dfac, upstream, bound, tp, vkt, tile0, pp, ds, ds_ld, c.act},
                          tile0, st));
             else if (first)
                 TRY(gemm(g, p.mt, ColsumEpi{fac, upstream, ds, ds_ld}, tile0, st));

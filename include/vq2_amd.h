@@ -808,8 +808,7 @@ int vq2_gated_rows(const void* x, int x_dt, const float* x_scale, int64_t tokens
                    void* y, int y_dt, void* workspace, size_t ws_bytes, void* stream);
 
 /* Its backward pass from dy [tokens, out_rows]: both products are made again.
- * dx [tokens, n] of dx_dt; dgate / dup [out_rows], both or neither.  A token
- * with |u f'(g)| or |f(g)| above 2^19 may give an infinite dx. */
+ * dx [tokens, n] of dx_dt; dgate / dup [out_rows], both or neither. */
 size_t vq2_gated_rows_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
                                          int scale_grad);
 int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens,

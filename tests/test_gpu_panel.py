@@ -543,6 +543,47 @@ def test_small_values(dev):
     assert ((one.cpu().double() - want[:1]).abs() <= tol[:1]).all()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("stages", [1, 3])
+@pytest.mark.parametrize("xf,sf,df", [(0, 0, 0), (-20, 0, 0), (0, -20, 0), (-30, -30, 30), (0, 14, 0), (10, 14, -40), (40, -36, -60)])
+def test_gated_backward_of_any_activations(dev, act, stages, xf, sf, df):
+    """The panel between the products is fp16 (steps of 2^-24 at its smallest)
+    under powers of two that bring a token's largest upstream value into [2^14,
+    2^15), and a bound B = 1.13 n max|x| max|w| max|s| of the activations to 1:
+    each of its factors is rounded up to a power of two, so by at most 2 (the
+    codebooks' as often as there are stages, the scales' twice: once more in
+    front of the second product).  That is half a step of 2^-25 2^-14 2^6 (2^7)
+    max|dy| B max|s| of a term."""
+    T, rows, n = 40, 96, 192
+    b = books("fp16")
+    g, u = Mat(520, rows, n, stages, b, "fp32"), Mat(523, rows, n, stages, b, "fp32")
+    for m in (g, u):
+        m.scale = m.scale * 2.0 ** sf
+        m.s = m.scale.double()
+    x = (rows_of(13, T, n, "bf16")[0].float() * 2.0 ** xf).bfloat16()
+    d = (synth.activations(14, (T, rows), torch.float32) * 2.0 ** df).bfloat16()
+    x64, d64 = x.double(), d.double()
+    dg, du = g.on(dev), u.on(dev)
+    dx, _, _ = K.vq_gated_rows_backward(d.to(dev), x.to(dev), (dg[0], dg[1], dg[4]), (du[0], du[1], du[4]), dg[2], dg[3], n, activation=act)
+    gv, uv = (x64 @ m.w.t() * m.s for m in (g, u))
+    f, dv = act64(act, gv)
+    tg, tu = d64 * uv * dv, d64 * f
+    want = (tg * g.s) @ g.w + (tu * u.s) @ u.w
+    eg, eu = (product_err(x64, m, True) * m.s + 4 * E * v.abs() for m, v in ((g, gv), (u, uv)))
+    # f' moves by at most 1.2 a unit, and lies in [-0.13, 1.13]
+    edf = torch.clamp(1.2 * eg, max=1.3) + 2.0 ** -19
+    etg = d64.abs() * (eu * (dv.abs() + edf) + uv.abs() * edf)
+    etu = d64.abs() * (1.13 * eg + 2.0 ** -20 * f.abs() + 2.0 ** -22 * gv.abs())
+    wmax = b[0].double().abs().max() + (b[2].double().abs().max() if stages == 3 else 0)
+    top = torch.maximum(g.s.max(), u.s.max())
+    floor = 2.0 ** (-33 if stages == 1 else -32) * d64.abs().amax(-1, keepdim=True) * 1.13 * n * x64.abs().amax(-1, keepdim=True) * wmax * top * top
+    w11 = 2.0 ** -11 if stages > 1 else 0.0
+    rel = (2 * rows / 4) * E + 2.0 ** -22 + w11 + 2.0 ** -11
+    tol = (etg * g.s + floor + rel * (tg * g.s).abs()) @ g.w.abs() + (etu * u.s + floor + rel * (tu * u.s).abs()) @ u.w.abs()
+    off = (dx.cpu().double() - want).abs() - tol - half(torch.bfloat16, want) - 2.0 ** -133
+    assert off.max() <= 0, float(off.max())
+
+
 def test_nan_and_infinity_stay_in_their_rows(dev):
     T, rows, n = 150, 64, 64
     m, u = Mat(510, rows, n, 1, books("fp16")), Mat(513, rows, n, 1, books("fp16"))
