@@ -474,8 +474,10 @@ __global__ void __launch_bounds__(threads_of(TPR), 2) norm_kernel(const NormCall
                     if (place<V, TPR, VEC>(c, k, id) < a.n) m[0] = bits_op(m[0], fabsf(h[c][k]));
             row_reduce<TPR>(m, s_red, bits_op);
             const float top = a.y_dt == VQ2_DT_I8 ? 127.0f : 448.0f;
-            inv = m[0] > 0.0f ? top / m[0] : 0.0f;
-            if (live && id == 0) a.y_scale[row] = m[0] / top;
+            // (a scale below 2^-126 would have no reciprocal)
+            const bool low = m[0] > 0.0f && m[0] < top * 0x1p-126f;
+            inv = low ? 0x1p126f : m[0] > 0.0f ? top / m[0] : 0.0f;
+            if (live && id == 0) a.y_scale[row] = low ? 0x1p-126f : m[0] / top;
         }
         if (live) store_row<V, TPR, VEC>(h, a.y, a.y_dt, row, a.n, id, inv);
     }

@@ -740,7 +740,8 @@ int vq2_unpack_fixed(const uint8_t* buf, int64_t nbytes, int bits, int64_t n, in
  *     residual itself
  *   weight [n] of w_dt; zero_centred: it holds the distance from 1
  *   y [rows, n]: VQ2_DT_F32 / F16 / BF16, or VQ2_DT_I8 / VQ2_DT_E4M3 of y_scale [rows]
- *     each: y_scale = largest magnitude / 127 (/ 448), y = u / y_scale to the
+ *     each: y_scale = largest magnitude / 127 (/ 448), 2^-126 where that is below it
+ *     and the row not zero, y = u / y_scale to the
  *     nearest; a row with a NaN or an infinity has that for its scale
  * n up to VQ2_NORM_MAX_N; rotated: n a multiple of 64, hb a power of two from
  * 64 on that divides n, rows and perm 16-byte and sign 8-byte aligned.

@@ -120,6 +120,30 @@ def test_8bit(dev, T, n, hb, odt):
         assert int(y.cpu().int().abs().max()) == 127
 
 
+@pytest.mark.parametrize("hb", [0, 64])
+@pytest.mark.parametrize("odt", [torch.int8, torch.float8_e4m3fn])
+def test_8bit_of_tiny_rows(dev, hb, odt):
+    """rows whose largest magnitude has a scale below 2^-126: that is their
+    scale, and half a step of it (e4m3: half a step of a value, 2^-10 of the
+    scale among its smallest numbers) is what y is off by, but for fp32's own
+    subnormal steps before"""
+    x = synth.activations(3, (5, 128), torch.float32) * 2.0 ** -134
+    x[4] = 0
+    y, _, sc = K.vq_add_rms_norm(x.to(dev), torch.ones(128, device=dev), out_dtype=odt, hb=hb, eps=1e-6)
+    u = x.double() * 1e-6 ** -0.5
+    if hb:
+        h = torch.ones(1, 1, dtype=torch.float64)
+        while h.shape[0] < hb:
+            h = torch.cat([torch.cat([h, h], 1), torch.cat([h, -h], 1)], 0)
+        u = (u.view(5, 2, hb) @ h * hb ** -0.5).reshape(5, 128)
+    assert (sc[:4].cpu() == 2.0 ** -126).all() and sc[4] == 0
+    got = y.cpu().float().double() * sc.cpu().double()[:, None]
+    step = 2.0 ** -127 if odt == torch.int8 else torch.maximum(2.0 ** -4 * u.abs(), torch.tensor(2.0 ** -136, dtype=torch.float64))
+    # 128 values of up to 2^-149 of rounding each, and 2^-20 of the value
+    assert ((got - u).abs() <= step + 2.0 ** -141 + 2.0 ** -20 * u.abs()).all()
+    assert (y[4].float() == 0).all()
+
+
 def test_8bit_odd_rows(dev):
     """a row of zeros has scale 0 and gives zeros; a NaN or an infinity shows in the row's scale, not in others"""
     x = torch.randn(4, 128, generator=synth.gen(5))
