@@ -16,6 +16,11 @@ one entry of ``kernels`` forward and one backward:
 them).  ``runtime.PackedMLP`` and ``PackedLMHead.loss`` are built on them.  The
 reference distils and tunes with dequantized weights in torch (vq2/kd.py); here
 no dequantized matrix is kept.
+
+A step that is captured into a graph makes its leaves inside (``detach()``,
+``requires_grad_()``) and takes their gradients with ``torch.autograd.grad``: a
+``backward()`` that is captured while an eager graph of the same leaves lives would
+wait for that graph's stream, which a capture does not allow.
 """
 from __future__ import annotations
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from compressai_amd import kernels as K, synth, tuning as T
+from compressai_amd.graph import DecodeStepGraph
 from compressai_amd.runtime import PackedLinear, PackedLMHead, PackedMLP
 from compressai_amd.rot import get_rot
 
@@ -188,3 +189,37 @@ def test_training_step(dev):
     for k, (p, q) in enumerate(zip(a, b)):
         assert torch.isfinite(p).all() and p.abs().max() > 0
         assert k == 0 or torch.equal(p, q)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_captured_step(dev, rows):
+    """a block and the head's loss, forward and backward, captured: every replay
+    gives the eager result, also with eager steps of the same layers in between"""
+    gate, up = _lin(110, I, H, "mlp.in", dev), _lin(111, I, H, "mlp.in", dev)
+    mlp = PackedMLP(gate, up, _lin(112, H, I, "mlp.down", dev))
+    head = PackedLMHead(_lin(113, V, H, "head", dev))
+    gate.scale, up.scale = gate.scale.float(), up.scale.float()
+    w = torch.ones(H, device=dev)
+
+    def step(x, r, tok, up_):
+        leaves = [t.detach().requires_grad_() for t in (x, w, gate.scale)]
+        gate.scale, keep = leaves[2], gate.scale
+        y, h = T.add_rms_norm(leaves[0], leaves[1], r)
+        z, _ = T.add_rms_norm(mlp(y), leaves[1], h)
+        loss = head.loss(z, tok)
+        gate.scale = keep
+        return [loss.detach(), *torch.autograd.grad(loss, leaves, up_)]
+
+    def inputs(k):
+        return (synth.activations(120 + k, (rows, H), torch.bfloat16).to(dev), synth.activations(130 + k, (rows, H), torch.bfloat16).to(dev),
+                torch.randint(0, V, (rows,), generator=synth.gen(140 + k)).to(dev),
+                synth.activations(150 + k, (rows,), torch.float32).to(dev))
+
+    graph = DecodeStepGraph(step, inputs(0))
+    for k in range(4):
+        a = inputs(k)
+        got = [t.clone() for t in graph(*a)]
+        want = step(*a)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        assert all(torch.isfinite(p).all() for p in got)
