@@ -131,6 +131,8 @@ struct PackArgs {
     int x_dt;
     int tokens, n;  // rows past the last token are zeros
     const float* x_scale;
+    const int64_t* target;  // or null: rows whose target is `ignore` are zeros, too
+    int64_t ignore;
     half8_t* panel;     // [tiles][n / 32][64]
     float* fac;         // a product of the panel times fac[t] is one of the row
     int tiles;          // 0: no rows to pack
@@ -147,7 +149,7 @@ __device__ __forceinline__ void pack_rows(const PackArgs& a, int tile, float (*s
     const int tid = threadIdx.x;
     const int lane = tid & 63, wave = tid >> 6, row = tile * 16 + (lane & 15), q = lane >> 4, kt = a.n / 32;
     const int per = (kt + PK_WAVES - 1) / PK_WAVES, k0 = wave * per, k1 = min(k0 + per, kt);
-    const bool live = row < a.tokens, held = per <= PK_HELD;
+    const bool live = row < a.tokens && !(a.target && a.target[row] == a.ignore), held = per <= PK_HELD;
     const int64_t at = (int64_t)row * a.n + q * 8;
     Eight x[PK_HELD];
     float m = 0.0f;
@@ -624,24 +626,29 @@ struct DlogitEpi {
     {
         const int lane = threadIdx.x & 63, q = lane >> 4, nl = lane & 15;
         const float c = pow2(14 - scale_exponent(amax));
-        float l[PG_NT], up[PG_NT], f[PG_NT];
-        int rel[PG_NT];  // the target's row of the wave's, or none; SKIP: the token does not count
-        constexpr int SKIP = -2, NONE = -1;
+        // A token that does not count has a row of zeros and an infinite l: no term
+        // of it is anything but 0.
+        float l[PG_NT], upf[PG_NT], f[PG_NT];
+        int rel[PG_NT];   // the target's row of the wave's, or none
+        bool hit[PG_NT];  // some lane's
 #pragma unroll
         for (int j = 0; j < PG_NT; j++) {
             const int t = tok + j * 16 + nl;
             int64_t v = TARGET_SKIP;
-            l[j] = up[j] = 0.0f;
-            if (t < tokens) {
-                v = target_of(target, t, ignore, rows);
-                l[j] = lse[t];
-                up[j] = v == TARGET_BAD ? __builtin_nanf("") : dloss[t];
-            }
+            l[j] = __builtin_inff();
+            upf[j] = 0.0f;
             f[j] = fac[t];
+            if (t < tokens) v = target_of(target, t, ignore, rows);
+            if (v != TARGET_SKIP) {
+                l[j] = lse[t];
+                upf[j] = v == TARGET_BAD ? __builtin_nanf("") : dloss[t] * f[j];
+            }
             const int64_t r = v - tile * 16;
-            rel[j] = v == TARGET_SKIP ? SKIP : r >= 0 && r < MT * 16 ? (int)r : NONE;
+            rel[j] = r >= 0 && r < MT * 16 ? (int)r : -1;
+            hit[j] = __any(rel[j] >= 0);
         }
         const int left = (int)min(rows - tile * 16, (int64_t)MT * 16);  // rows of the wave that exist
+        const bool tail = left < MT * 16;
 #pragma unroll
         for (int i = 0; i < MT; i += 2) {
             f32x4_t s[2], d[2];
@@ -652,15 +659,24 @@ struct DlogitEpi {
             }
 #pragma unroll
             for (int j = 0; j < PG_NT; j++) {
+                float v[8];
+#pragma unroll
+                for (int m = 0; m < 8; m++) v[m] = __expf(acc[i + (m >> 2)][j][m & 3] * f[j] * s[m >> 2][m & 3] - l[j]);
+                if (hit[j]) {  // (few waves)
+#pragma unroll
+                    for (int m = 0; m < 8; m++) v[m] -= rel[j] == (i + (m >> 2)) * 16 + 4 * q + (m & 3) ? 1.0f : 0.0f;
+                }
+                if (tail) {
+#pragma unroll
+                    for (int m = 0; m < 8; m++)
+                        if ((i + (m >> 2)) * 16 + 4 * q + (m & 3) >= left) v[m] = 0.0f;
+                }
                 half8_t h;
 #pragma unroll
                 for (int m = 0; m < 8; m++) {
-                    const int e = m & 3, k = m >> 2, r = (i + k) * 16 + 4 * q + e;
-                    const float raw = acc[i + k][j][e] * f[j];
-                    float v = __expf(raw * s[k][e] - l[j]) - (rel[j] == r ? 1.0f : 0.0f);
-                    if (rel[j] == SKIP || r >= left) v = 0.0f;
-                    h[m] = (_Float16)(v * (s[k][e] * c));
-                    if (ds && rel[j] != SKIP) d[k][e] += up[j] * v * raw;
+                    const int e = m & 3, k = m >> 2;
+                    h[m] = (_Float16)(v[m] * (s[k][e] * c));
+                    if (ds) d[k][e] += v[m] * (acc[i + k][j][e] * upf[j]);
                 }
                 p[((int64_t)((tok >> 4) + j) * vkt + (tile - tile0 + i) / 2) * 64 + lane] = h;
             }
@@ -680,14 +696,14 @@ template <int ACT>
 __device__ __forceinline__ void gate_act(float g, float& f, float& df)
 {
     if constexpr (ACT == VQ2_ACT_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-g));
+        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));  // (2^-23 of it; a division's 10 instructions show)
         f = g * s;
         df = s * (1.0f + g * (1.0f - s));
         if (g < -80.0f) f = df = 0.0f;  // (also -inf; the true values are below 1e-32)
     } else {
         // g / (1 + exp(-2 u)), u the tanh form's argument
         const float g2 = g * g, u2 = 1.5957691216057308f * g * (1.0f + 0.044715f * g2);
-        const float s = 1.0f / (1.0f + __expf(-u2));
+        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-u2));
         f = g * s;
         df = s * (1.0f + g * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * g2)));
         if (g < -12.0f) f = df = 0.0f;
@@ -1728,7 +1744,8 @@ int panel_launch(const PanelCall& c)
         const bool prep = !few_call && !prepared;
         prepared = prepared || prep;
         const PrologueArgs pro{
-            PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n, c.x_scale ? c.x_scale + t0 : nullptr, xp, fac,
+            PackArgs{(const char*)c.x + t0 * c.n * xsize, c.x_dt, tokens, (int)c.n, c.x_scale ? c.x_scale + t0 : nullptr,
+                     c.what == DLOGIT ? target : nullptr, c.ignore, xp, fac,
                      first && !(few_call && few_own(tokens, c.x_dt)) ? tp / 16 : 0},
             DyMaxArgs{dy, c.dy_dt, tokens, dy_vec, c.rows, dfac,
                       c.what == DGATED || c.what == PRODUCT ? tp / 16 : 0},
