@@ -398,6 +398,7 @@ __device__ __forceinline__ uint32_t code_of(const u32x4& w, int k, int lane)
 // tiles: lane (row, q) gathers group 4 k + q, and each k tile is one KiB.  The
 // codes come 8 a lane where their rows are aligned (vec), and change lanes in
 // the LDS unit: loaded one by one they cost a request for each 4 gathers.
+// 32768 x 2048 at 2 bits: 50 us, 168 G gathers a second beside 134 MB written.
 template <int CBT, int S2, int PARTS>
 __global__ void __launch_bounds__(256) dequant_plain_kernel(const DequantArgs a)
 {
@@ -447,6 +448,9 @@ __global__ void __launch_bounds__(256) dequant_plain_kernel(const DequantArgs a)
 // Column j of the 8 centroids is then one operand of the columns' panel, whose
 // block j holds columns j, 8 + j, ... of the 16 groups: one KiB a block, and a
 // lane of the next product holds 8 neighbouring columns in its 8 row tiles.
+// 16384 x 2048 at 2 bits: 40 us, 105 G gathers a second beside 134 MB written (27 us at
+// a large copy's rate); the conflicts of its LDS writes (82 % of its LDS cycles) cost
+// nothing, 40 us without them, too.
 template <int CBT, int S2, int WP, int TP>
 __global__ void __launch_bounds__(256) dequant_both_kernel(const DequantArgs a)
 {

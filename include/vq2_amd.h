@@ -772,6 +772,9 @@ int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt
  *   dx      gradients of x, VQ2_DT_F16 / BF16, 16-byte aligned;  dscale  of the row scales, fp32, or NULL
  *   workspace  256-byte aligned, of the entry's _workspace bytes (scale_grad:
  *           whether dscale is wanted); contents on entry do not matter
+ * Weights are multiplied in fp16 (where an fp16 or fp32 result depends on more bits, as
+ * two addends of it): bf16 / fp32 codebooks hold values up to 65504, and what is below
+ * 2^-14 in them is held in steps of 2^-24.
  * Results do not depend on what ran before, and sums have a fixed order. */
 #define VQ2_PANEL_MAX_N 32768
 #define VQ2_PANEL_MAX_ROWS 4194304
