@@ -1212,6 +1212,21 @@ __global__ void __launch_bounds__(256, TT >= 6 || OWN ? 2 : 3) few_kernel(const 
     const half8_t zero = {0, 0, 0, 0, 0, 0, 0, 0};
     constexpr int TS = KW == 4 ? (TT + 3) / 4 : TT;  // token tiles that this wave finishes: wave, wave + 4, ...
     typename Epi::State state[TS];
+    // The tokens' operand of the next k tile is on its way while one is multiplied,
+    // where a wave is often alone on its SIMD (333 tokens of 2 x 1000 x 2048: 26.9 us
+    // without, 25.0; 3 ahead 29.5).  With rows of its own, or two stages' centroids beside
+    // it, it would take registers that loads in flight need (96 tokens of 50257 rows
+    // 99.1 -> 100.5, 64 of 2 x 1000 at 3 bits 19.9 -> 21.1).
+    constexpr int R = OWN || KW == 1 || S2 != VQ2_S2_NONE ? 1 : 2;
+    half8_t b[R][TT];
+    auto load_b = [&](int s, int j, half8_t (&o)[TT]) {
+        const int g = s * 32 + q * 8 < ng ? s * 32 + q * 8 + j : 0;
+#pragma unroll
+        for (int t = 0; t < TT; t++) o[t] = xp[((int64_t)t * kt + (g >> 2)) * 64 + (g & 3) * 16 + nl];
+    };
+    if constexpr (!OWN)
+#pragma unroll
+        for (int j = 0; j < R - 1; j++) load_b(s0, j, b[j]);
     for (; pair < a.pairs;) {
     f32x4_t acc[2][TT];
 #pragma unroll
@@ -1241,26 +1256,24 @@ __global__ void __launch_bounds__(256, TT >= 6 || OWN ? 2 : 3) few_kernel(const 
                 }
 #pragma unroll
             for (int u = 0; u < JU; u++) {
-                const int g = ok ? s * 32 + q * 8 + j0 + u : 0;
-                half8_t b[TT];
+                const int j = j0 + u, at = j % R;
                 if constexpr (OWN) {
-                    const Eight e = eight(xw[j0 + u]);
+                    const Eight e = eight(xw[j]);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) b[0][k] = (_Float16)(e.v[k] * down);
+                    for (int k = 0; k < 8; k++) b[at][0][k] = (_Float16)(e.v[k] * down);
                 } else {
-#pragma unroll
-                    for (int t = 0; t < TT; t++) b[t] = xp[((int64_t)t * kt + (g >> 2)) * 64 + (g & 3) * 16 + nl];
+                    load_b(j + R - 1 < 8 ? s : s + 1 == s1 ? s0 : s + 1, (j + R - 1) % 8, b[(j + R - 1) % R]);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const half8_t w = ok ? centroid_f16<CBT>(w0[i][u]) : zero;
 #pragma unroll
-                    for (int t = 0; t < TT; t++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, b[t], acc[i][t], 0, 0, 0);
+                    for (int t = 0; t < TT; t++) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, b[at][t], acc[i][t], 0, 0, 0);
                     if constexpr (S2 != VQ2_S2_NONE) {
                         const half8_t v = ok ? centroid_f16<CBT>(w1[i][u]) : zero;
 #pragma unroll
                         for (int t = 0; t < TT; t++)
-                            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, b[t], acc[i][t], 0, 0, 0);
+                            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, b[at][t], acc[i][t], 0, 0, 0);
                     }
                 }
             }
@@ -1492,7 +1505,7 @@ int few_groups(const PanelCall& c, int64_t tokens)
 // each block of 128 tokens, panels once, but they store and read it again, and
 // take two launches more.  In gathers: a block costs them and 10^5, panels 1.3
 // times as many and 2.8 * 10^6.  Measured (us a call; codes of the call, tokens: few /
-// panels): 65 k, 512 15 / 24; 262 k, 1024 31 / 39, 2048 45 / 42; 512 k, 333 26 / 37, 1024 43 / 41;
+// panels): 65 k, 512 15 / 24; 262 k, 1024 31 / 39, 2048 45 / 42; 512 k, 333 25 / 37, 1024 43 / 41;
 // 3.1 M, 128 33 / 51, 256 54 / 52, 512 96 / 59; 6.3 M, 128 51 / 61, 192 82 / 62; 12.9 M, 128
 // 108 / 128, 160 190 / 140; 38.9 M, 1 174 / 335, 128 270 / 335, 160 478 / 367.
 bool few_ahead(const PanelCall& c, int64_t tokens)
