@@ -1056,7 +1056,8 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
     constexpr int N = 4;
     const int lane = threadIdx.x & 63, q = lane >> 4, tile = blockIdx.x, t = tile * 16 + (lane & 15);
     const int k0 = ((int)blockIdx.y * 4 + (threadIdx.x >> 6)) * N;
-    const float f = a.dfac[t] * pow2(-scale_exponent(a.amax));
+    // (two factors: their product may leave fp32's range)
+    const float f = a.dfac[t], c = pow2(-scale_exponent(a.amax));
     f32x4_t v[N][2], s[N][2];
     if (a.up.vec) {
         u32x2 w[N][2];
@@ -1076,7 +1077,7 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
         if (k0 + i >= a.vkt) break;
         half8_t h;
 #pragma unroll
-        for (int m = 0; m < 8; m++) h[m] = (_Float16)(v[i][m >> 2][m & 3] * (s[i][m >> 2][m & 3] * f));
+        for (int m = 0; m < 8; m++) h[m] = (_Float16)(v[i][m >> 2][m & 3] * f * (s[i][m >> 2][m & 3] * c));
         a.p[((int64_t)tile * a.vkt + k0 + i) * 64 + lane] = h;
     }
 }

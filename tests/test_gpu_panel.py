@@ -543,6 +543,21 @@ def test_small_values(dev):
     assert ((one.cpu().double() - want[:1]).abs() <= tol[:1]).all()
 
 
+def test_gradient_of_tiny_rows_and_scales(dev):
+    """upstream rows and scales whose powers of two together leave fp32's range:
+    the gradient of the same rows at ordinary size, times both, as far as bf16
+    holds it (steps of 2^-133 at its smallest)"""
+    T, rows, n = 20, 96, 128
+    m = Mat(530, rows, n, 1, books("fp16"), "fp32")
+    d = synth.activations(15, (T, rows), torch.bfloat16).to(dev)
+    i0, _, cb0, _, sc = m.on(dev)
+    base = K.vq_gemm_backward(d, None, i0, None, cb0, None, sc, rows, n)[0].double()
+    for e, f in ((-64, -64), (-70, -58), (64, -64), (-90, 60), (60, 60)):
+        got = K.vq_gemm_backward(d * 2.0 ** e, None, i0, None, cb0, None, sc * 2.0 ** f, rows, n)[0].double()
+        want = base * 2.0 ** (e + f)
+        assert torch.isfinite(got).all() and ((got - want).abs() <= 2.0 ** -133).logical_or(got == want).all()
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
 @pytest.mark.parametrize("stages", [1, 3])
 @pytest.mark.parametrize("xf,sf,df", [(0, 0, 0), (-20, 0, 0), (0, -20, 0), (-30, -30, 30), (0, 14, 0), (10, 14, -40), (40, -36, -60)])
