@@ -344,7 +344,7 @@ class PackedMLP(nn.Module):
             from . import tuning as T
 
             act = T.gated(gate, up, T.rotate(x, gate.rot, xt), self.activation)
-            return T.linear(down, T.rotate(act, down.rot)).to(od)
+            return T.linear(down, T.rotate(act, down.rot), od)
         x2 = x.reshape(-1, gate.n).contiguous()
         g0, g1, cb0, cb1 = gate._planes()
         if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], cb0) for m in mats):

@@ -8,7 +8,7 @@ one entry of ``kernels`` forward and one backward:
 
   rotate(x, rot)                the RHT (orthogonal: its gradient is its inverse)
   add_rms_norm(x, weight, residual, rot=...)  (y, h), y rotated where rot is given
-  linear(lin, xr)               a PackedLinear on rotated rows
+  linear(lin, xr, out_dtype)    a PackedLinear on rotated rows
   gated(gate, up, xr)           f(gate xr) * (up xr)
   head_loss(lin, xr, targets)   the loss of every token
 
@@ -82,7 +82,7 @@ class _Norm(torch.autograd.Function):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, xr, scale, lin):
+    def forward(ctx, xr, scale, lin, out_dtype):
         from .runtime import vq_matmul
 
         ctx.save_for_backward(xr, scale)
@@ -90,9 +90,9 @@ class _Linear(torch.autograd.Function):
         i0, i1, cb0, cb1 = _planes(lin)
         x2 = xr.reshape(-1, lin.n)
         if x2.shape[0] >= 3 and lin.n % 64 == 0 and lin.n <= K.ROWS_GEMM_MAX_N:
-            y = K.vq_rows_gemm(x2, [(i0, i1, scale, lin.out)], cb0, cb1, lin.n, hb=0, act_dtype=xr.dtype, out_dtype=xr.dtype)[0]
+            y = K.vq_rows_gemm(x2, [(i0, i1, scale, lin.out)], cb0, cb1, lin.n, hb=0, act_dtype=xr.dtype, out_dtype=out_dtype)[0]
         else:
-            y = vq_matmul(x2, i0, i1, cb0, cb1, scale, lin.out, lin.n, xr.dtype)
+            y = vq_matmul(x2, i0, i1, cb0, cb1, scale, lin.out, lin.n, out_dtype)
         return y.view(*xr.shape[:-1], lin.out)
 
     @staticmethod
@@ -103,7 +103,7 @@ class _Linear(torch.autograd.Function):
         i0, i1, cb0, cb1 = _planes(lin)
         dx, ds = K.vq_gemm_backward(dy.contiguous(), xr, i0, i1, cb0, cb1, scale, lin.out, lin.n,
                                     scale_grad=ctx.needs_input_grad[1])
-        return dx, _to(ds, scale), None
+        return dx, _to(ds, scale), None, None
 
 
 class _Gated(torch.autograd.Function):
@@ -160,9 +160,9 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, rot=
     return out if residual is not None else (out, x)
 
 
-def linear(lin, xr):
-    """A PackedLinear's product with rotated rows, in their type."""
-    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin)
+def linear(lin, xr, out_dtype=None):
+    """A PackedLinear's product with rotated rows, in their type or out_dtype."""
+    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype)
 
 
 def gated(gate, up, xr, activation="silu"):
