@@ -18,6 +18,7 @@ HEADER_PATH = PKG_DIR.parent / "include" / "vq2_amd.h"
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 DT_I8, DT_E4M3 = 3, 4
+DT_F32_RANGE = 5
 ACT_SILU, ACT_GELU_TANH = 0, 1
 S2_NONE, S2_U8, S2_U16 = 0, 1, 2
 ID_I32, ID_I64 = 0, 1

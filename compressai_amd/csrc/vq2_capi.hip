@@ -1212,8 +1212,9 @@ int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt
 }
 
 // ------------------------------------------- many-row products on panels
-// (what leaves through an fp16 panel has 16 bits)
-static bool grad_dt(int dt) { return dt == VQ2_DT_F16 || dt == VQ2_DT_BF16; }
+// (what leaves through an fp16 panel has 11 bits: fp32 is taken for its range alone, under a name that says so)
+static bool grad_dt(int dt) { return dt == VQ2_DT_F16 || dt == VQ2_DT_BF16 || dt == VQ2_DT_F32_RANGE; }
+static int grad_store_dt(int dt) { return dt == VQ2_DT_F32_RANGE ? VQ2_DT_F32 : dt; }
 
 static bool bits8_dt(int dt) { return dt == VQ2_DT_I8 || dt == VQ2_DT_E4M3; }
 
@@ -1327,7 +1328,7 @@ int vq2_head_loss(const void* x, int x_dt, const float* x_scale, int64_t tokens,
 size_t vq2_head_loss_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
                                         int scale_grad)
 {
-    return panel_workspace(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, scale_grad);
+    return panel_workspace(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, grad_store_dt(dx_dt), scale_grad);
 }
 
 int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_t* targets, int64_t ignore_index,
@@ -1336,7 +1337,7 @@ int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_
                            float rs, void* dx, int dx_dt, float* dscale, void* workspace, size_t ws_bytes, void* stream)
 {
     clear_error();
-    PanelCall c = panel_sizes(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, false);
+    PanelCall c = panel_sizes(PANEL_DLOGIT, tokens, out_rows, 1, n, s2_kind, cb_dt, grad_store_dt(dx_dt), false);
     c.who = "vq2_head_loss_backward";
     c.x = x;
     c.x_dt = x_dt;
@@ -1352,7 +1353,7 @@ int vq2_head_loss_backward(const void* x, int x_dt, int64_t tokens, const int64_
     c.stream = stream;
     const int r = check_panel(c, true, false);
     if (r) return r;
-    CHECK(grad_dt(dx_dt), "vq2_head_loss_backward: dx must hold fp16 or bf16 values");
+    CHECK(grad_dt(dx_dt), "vq2_head_loss_backward: dx must hold fp16 or bf16 values, or fp32 ones as VQ2_DT_F32_RANGE");
     if (tokens) {
         CHECK(targets && lse && dloss && dx, "vq2_head_loss_backward: NULL pointer argument");
         CHECK((uintptr_t)targets % 8 == 0 && ((uintptr_t)lse | (uintptr_t)dloss) % 4 == 0 && (uintptr_t)dx % 16 == 0,
@@ -1408,7 +1409,7 @@ int vq2_gated_rows(const void* x, int x_dt, const float* x_scale, int64_t tokens
 size_t vq2_gated_rows_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
                                          int scale_grad)
 {
-    return panel_workspace(PANEL_DGATED, tokens, out_rows, 2, n, s2_kind, cb_dt, dx_dt, scale_grad);
+    return panel_workspace(PANEL_DGATED, tokens, out_rows, 2, n, s2_kind, cb_dt, grad_store_dt(dx_dt), scale_grad);
 }
 
 int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens, const vq2_seg* mats, int s2_kind,
@@ -1417,7 +1418,7 @@ int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, 
 {
     clear_error();
     CHECK(mats, "vq2_gated_rows_backward: mats is NULL");
-    PanelCall c = panel_sizes(PANEL_DGATED, tokens, mats[0].out_rows, 2, n, s2_kind, cb_dt, dx_dt, false);
+    PanelCall c = panel_sizes(PANEL_DGATED, tokens, mats[0].out_rows, 2, n, s2_kind, cb_dt, grad_store_dt(dx_dt), false);
     c.who = "vq2_gated_rows_backward";
     c.x = x;
     c.x_dt = x_dt;
@@ -1432,7 +1433,7 @@ int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, 
     int r = set_gated(c, mats, cb0, cb1, s_dt, rs, act);
     if (r) return r;
     CHECK(dt_ok(dy_dt), "vq2_gated_rows_backward: bad dy dtype");
-    CHECK(grad_dt(dx_dt), "vq2_gated_rows_backward: dx must hold fp16 or bf16 values");
+    CHECK(grad_dt(dx_dt), "vq2_gated_rows_backward: dx must hold fp16 or bf16 values, or fp32 ones as VQ2_DT_F32_RANGE");
     CHECK((dgate == nullptr) == (dup == nullptr), "vq2_gated_rows_backward: dgate and dup must be given both or neither");
     r = check_panel(c, true, false);
     if (r) return r;
@@ -1445,7 +1446,7 @@ int vq2_gated_rows_backward(const void* dy, int dy_dt, const void* x, int x_dt, 
 size_t vq2_gemm_backward_workspace(int64_t tokens, int64_t out_rows, int64_t n, int s2_kind, int cb_dt, int dx_dt,
                                    int scale_grad)
 {
-    return panel_workspace(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, scale_grad);
+    return panel_workspace(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, grad_store_dt(dx_dt), scale_grad);
 }
 
 int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_t tokens, const int16_t* idx0, const void* idx1,
@@ -1453,7 +1454,7 @@ int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_
                       int64_t n, float rs, void* dx, int dx_dt, float* dscale, void* workspace, size_t ws_bytes, void* stream)
 {
     clear_error();
-    PanelCall c = panel_sizes(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, dx_dt, false);
+    PanelCall c = panel_sizes(PANEL_PRODUCT, tokens, out_rows, 1, n, s2_kind, cb_dt, grad_store_dt(dx_dt), false);
     c.who = "vq2_gemm_backward";
     c.x = x;
     c.x_dt = x_dt;
@@ -1468,7 +1469,7 @@ int vq2_gemm_backward(const void* dy, int dy_dt, const void* x, int x_dt, int64_
     const int r = check_panel(c, dscale != nullptr, false);
     if (r) return r;
     CHECK(dt_ok(dy_dt), "vq2_gemm_backward: bad dy dtype");
-    CHECK(grad_dt(dx_dt), "vq2_gemm_backward: dx must hold fp16 or bf16 values");
+    CHECK(grad_dt(dx_dt), "vq2_gemm_backward: dx must hold fp16 or bf16 values, or fp32 ones as VQ2_DT_F32_RANGE");
     if (tokens)
         CHECK(dy && dx && (uintptr_t)dy % dt_size(dy_dt) == 0 && (uintptr_t)dx % 16 == 0,
               "vq2_gemm_backward: dy or dx is NULL or not aligned (dy to its elements, dx to 16 bytes)");

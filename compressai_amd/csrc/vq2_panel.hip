@@ -790,16 +790,25 @@ struct GatedEpi {
 };
 
 // Upstream values of 4 neighbouring rows of a token, as loaded (16 bits: vec
-// rows in 8 bytes) and as numbers.
+// rows in 8 bytes; fp32: in 16) and as numbers.
+enum { ONE_BY_ONE, VEC16, VEC32 };
 struct Upstream {
     const void* dy;  // [tokens][rows]
     int dt, tokens, vec;
     int64_t rows;
-    __device__ __forceinline__ u32x2 raw(int t, int64_t r) const
+    // (past the tokens or rows: anything of the row, which is dropped)
+    __device__ __forceinline__ int64_t place(int t, int64_t r) const
     {
-        // (past the tokens or rows: anything of the row; numbers() drops it)
-        const int64_t at = (int64_t)min(t, tokens - 1) * rows + (r < rows ? r : 0);
-        return *(const u32x2*)((const uint16_t*)dy + at);
+        return (int64_t)min(t, tokens - 1) * rows + (r < rows ? r : 0);
+    }
+    __device__ __forceinline__ u32x2 raw(int t, int64_t r) const { return *(const u32x2*)((const uint16_t*)dy + place(t, r)); }
+    __device__ __forceinline__ f32x4_t words(int t, int64_t r) const { return *(const f32x4_t*)((const float*)dy + place(t, r)); }
+    __device__ __forceinline__ f32x4_t kept(f32x4_t v, int t, int64_t r) const
+    {
+        const bool in = t < tokens && r < rows;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = in ? v[e] : 0.0f;
+        return v;
     }
     __device__ __forceinline__ f32x4_t numbers(u32x2 w, int t, int64_t r) const
     {
@@ -811,10 +820,7 @@ struct Upstream {
             v = f32x4_t{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
                         __uint_as_float(w.y & 0xFFFF0000u)};
         }
-        const bool in = t < tokens && r < rows;
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = in ? v[e] : 0.0f;
-        return v;
+        return kept(v, t, r);
     }
     __device__ __forceinline__ f32x4_t slow(int t, int64_t r) const
     {
@@ -827,12 +833,17 @@ struct Upstream {
     // of PG_NT token tiles
     __device__ __forceinline__ void load(f32x4_t (&d)[PG_NT], int t, int64_t r) const
     {
-        if (vec) {
+        if (vec == VEC16) {
             u32x2 w[PG_NT];
 #pragma unroll
             for (int j = 0; j < PG_NT; j++) w[j] = raw(t + j * 16, r);
 #pragma unroll
             for (int j = 0; j < PG_NT; j++) d[j] = numbers(w[j], t + j * 16, r);
+        } else if (vec == VEC32) {
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) d[j] = words(t + j * 16, r);
+#pragma unroll
+            for (int j = 0; j < PG_NT; j++) d[j] = kept(d[j], t + j * 16, r);
         } else {
 #pragma unroll
             for (int j = 0; j < PG_NT; j++) d[j] = slow(t + j * 16, r);
@@ -968,10 +979,16 @@ struct DxFactor {
     }
 };
 
-// 8 (4) neighbouring columns of dx in 16 bits: element e of N tiles' values
+// 8 (4) neighbouring columns of dx: element e of N tiles' values
 template <int N>
 __device__ __forceinline__ void store_run(void* dx, int dt, int64_t at, const f32x4_t (&v)[N], int e, const DxFactor::Of& f)
 {
+    if (dt == VQ2_DT_F32) {
+        f32x4_t* o = (f32x4_t*)((float*)dx + at);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) o[i / 4] = f32x4_t{f(v[i][e]), f(v[i + 1][e]), f(v[i + 2][e]), f(v[i + 3][e])};
+        return;
+    }
     uint32_t w[N / 2];
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
@@ -1059,13 +1076,19 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
     // (two factors: their product may leave fp32's range)
     const float f = a.dfac[t], c = pow2(-scale_exponent(a.amax));
     f32x4_t v[N][2], s[N][2];
-    if (a.up.vec) {
+    if (a.up.vec == VEC16) {
         u32x2 w[N][2];
 #pragma unroll
         for (int i = 0; i < 2 * N; i++) w[i / 2][i % 2] = a.up.raw(t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
 #pragma unroll
         for (int i = 0; i < 2 * N; i++)
             v[i / 2][i % 2] = a.up.numbers(w[i / 2][i % 2], t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
+    } else if (a.up.vec == VEC32) {
+#pragma unroll
+        for (int i = 0; i < 2 * N; i++) v[i / 2][i % 2] = a.up.words(t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
+#pragma unroll
+        for (int i = 0; i < 2 * N; i++)
+            v[i / 2][i % 2] = a.up.kept(v[i / 2][i % 2], t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
     } else {
 #pragma unroll
         for (int i = 0; i < 2 * N; i++) v[i / 2][i % 2] = a.up.slow(t, a.row0 + (k0 + i / 2) * 32 + i % 2 * 16 + q * 4);
@@ -1757,8 +1780,8 @@ int panel_launch(const PanelCall& c)
         const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;
         void* dx = c.y && grad ? (char*)c.y + t0 * c.n * dt_size(c.y_dt) : nullptr;
         const DxFactor dxf{amax, c.what == DLOGIT ? nullptr : dfac, c.dloss ? c.dloss + t0 : nullptr, target, c.rows, c.ignore, bound, 0};
-        const Upstream upstream{dy, c.dy_dt, tokens,
-                                c.dy_dt != VQ2_DT_F32 && c.rows % 4 == 0 && (uintptr_t)dy % 8 == 0, c.rows};
+        const bool dy32 = c.dy_dt == VQ2_DT_F32, fours = c.rows % 4 == 0 && (uintptr_t)dy % (dy32 ? 16 : 8) == 0;
+        const Upstream upstream{dy, c.dy_dt, tokens, !fours ? ONE_BY_ONE : dy32 ? VEC32 : VEC16, c.rows};
         const bool prep = !few_call && !prepared;
         prepared = prepared || prep;
         const PrologueArgs pro{

@@ -1825,11 +1825,19 @@ def vq_head_loss(xr, targets, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, x_scal
     return loss, lse
 
 
+def _dx_type(dtype, wide):
+    """(dtype, code) of a backward entry's dx: ``dtype``, or fp32 where it is wide"""
+    if not wide:
+        return dtype, _DT.get(dtype, -1)
+    return torch.float32, _lib.DT_F32_RANGE
+
+
 def vq_head_loss_backward(xr, targets, lse, dloss, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, ignore_index=-100,
-                          scale_grad=False):
+                          scale_grad=False, wide=False):
     """Backward pass of vq_head_loss from its lse and the gradient dloss fp32
     [T] of every token's loss: (dxr in xr's shape and dtype, dscale fp32 [out]
-    or None).  Tokens of ignore_index give zeros."""
+    or None).  Tokens of ignore_index give zeros.  wide: dxr in fp32, for
+    activations that are fp32 themselves (its range; the terms have 11 bits)."""
     dev = _dev(xr, targets, lse, dloss, i0, i1, cb0, cb1, scale)
     n, out = int(n), int(out)
     x2, xdt = _panel_x(xr, None, n, bits8=False)
@@ -1838,14 +1846,15 @@ def vq_head_loss_backward(xr, targets, lse, dloss, i0, i1, cb0, cb1, scale, out,
     _token_vec(targets, T, torch.int64, "targets")
     _token_vec(lse, T, torch.float32, "lse")
     _token_vec(dloss, T, torch.float32, "dloss")
-    dx = torch.empty_like(xr)
+    dtype, ddt = _dx_type(xr.dtype, wide)
+    dx = torch.empty_like(xr, dtype=dtype)
     ds = torch.empty(out, dtype=torch.float32, device=dev) if scale_grad else None
     cdt = _dt(cb0, "cb0")
     with _on_device(dev):
-        nbytes = int(_lib.load().vq2_head_loss_backward_workspace(T, out, n, s2, cdt, xdt, 1 if scale_grad else 0))
+        nbytes = int(_lib.load().vq2_head_loss_backward_workspace(T, out, n, s2, cdt, ddt, 1 if scale_grad else 0))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("vq2_head_loss_backward", _p(x2), xdt, T, _p(targets), int(ignore_index), _p(lse), _p(dloss), _p(i0),
-                  _p(i1), s2, _p(cb0), _p(cb1), cdt, _p(scale), _dt(scale, "scale"), out, n, float(rs), _p(dx), xdt,
+                  _p(i1), s2, _p(cb0), _p(cb1), cdt, _p(scale), _dt(scale, "scale"), out, n, float(rs), _p(dx), ddt,
                   _p(ds), _p(ws), nbytes, _stream(dev))
     return dx, ds
 
@@ -1895,11 +1904,11 @@ def vq_gated_rows(xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", x_sca
     return y
 
 
-def vq_gated_rows_backward(dact, xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", scale_grad=False):
+def vq_gated_rows_backward(dact, xr, gate, up, cb0, cb1, n, rs=1.0, *, activation="silu", scale_grad=False, wide=False):
     """Backward pass of vq_gated_rows from the gradient dact [..., rows] of its
     result; the two products are made again.  Returns (dxr in xr's shape and
-    dtype, dgate fp32 [rows], dup fp32 [rows]): the latter are the row scales'
-    gradients, None unless scale_grad."""
+    dtype (wide: fp32, as in vq_head_loss_backward), dgate fp32 [rows], dup fp32
+    [rows]): the latter are the row scales' gradients, None unless scale_grad."""
     dev = _dev(dact, xr, *gate, *up, cb0, cb1)
     n = int(n)
     act = _act(activation)
@@ -1909,24 +1918,25 @@ def vq_gated_rows_backward(dact, xr, gate, up, cb0, cb1, n, rs=1.0, *, activatio
     if dact.numel() != T * rows or dact.shape[-1] != rows:
         raise Vq2Error(f"dact must be [{T}, {rows}], got {tuple(dact.shape)}")
     _contig(dact, "dact")
-    dx = torch.empty_like(xr)
+    dtype, ddt = _dx_type(xr.dtype, wide)
+    dx = torch.empty_like(xr, dtype=dtype)
     dg = torch.empty(rows, dtype=torch.float32, device=dev) if scale_grad else None
     du = torch.empty(rows, dtype=torch.float32, device=dev) if scale_grad else None
     cdt = _dt(cb0, "cb0")
     with _on_device(dev):
-        nbytes = int(_lib.load().vq2_gated_rows_backward_workspace(T, rows, n, s2, cdt, xdt, 1 if scale_grad else 0))
+        nbytes = int(_lib.load().vq2_gated_rows_backward_workspace(T, rows, n, s2, cdt, ddt, 1 if scale_grad else 0))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("vq2_gated_rows_backward", _p(dact), _dt(dact, "dact"), _p(x2), xdt, T, segs, s2, _p(cb0), _p(cb1), cdt,
-                  sdt, n, float(rs), act, _p(dx), xdt, _p(dg), _p(du), _p(ws), nbytes, _stream(dev))
+                  sdt, n, float(rs), act, _p(dx), ddt, _p(dg), _p(du), _p(ws), nbytes, _stream(dev))
     return dx, dg, du
 
 
-def vq_gemm_backward(dy, xr, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, scale_grad=False, dx_dtype=None):
+def vq_gemm_backward(dy, xr, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, scale_grad=False, dx_dtype=None, wide=False):
     """Backward pass of a packed product y = vq_gemv / vq_gemm_small_m /
     vq_rows_gemm (hb=0) of rotated rows xr [..., n], from dy [..., out]:
     (dxr [..., n], dscale fp32 [out] or None).  xr is read only for dscale and
     may be None without it; dxr is of dx_dtype (float16 / bfloat16), by default xr's, or dy's
-    without one."""
+    without one (wide: fp32, as in vq_head_loss_backward)."""
     dev = _dev(dy, xr, i0, i1, cb0, cb1, scale)
     n, out = int(n), int(out)
     i0, i1, s2 = _planes(i0, i1, cb0, cb1, scale, out, n)
@@ -1941,8 +1951,8 @@ def vq_gemm_backward(dy, xr, i0, i1, cb0, cb1, scale, out, n, rs=1.0, *, scale_g
         x2, xdt = _panel_x(xr, None, n, bits8=False)
     elif scale_grad:
         raise Vq2Error("vq_gemm_backward: the scales' gradient needs xr")
-    dx = torch.empty((*dy.shape[:-1], n), dtype=dx_dtype or (dy if xr is None else xr).dtype, device=dev)
-    ddt = _dt(dx, "dx")
+    dtype, ddt = _dx_type(dx_dtype or (dy if xr is None else xr).dtype, wide)
+    dx = torch.empty((*dy.shape[:-1], n), dtype=dtype, device=dev)
     ds = torch.empty(out, dtype=torch.float32, device=dev) if scale_grad else None
     cdt = _dt(cb0, "cb0")
     with _on_device(dev):

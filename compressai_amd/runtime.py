@@ -27,6 +27,7 @@ import torch
 import torch.nn as nn
 
 from . import kernels as K
+from . import tuning as T
 from .rot import get_rot
 
 
@@ -338,13 +339,9 @@ class PackedMLP(nn.Module):
     def forward(self, x, out_dtype=None):
         gate, up, down = self.gate, self.up, self.down
         od = out_dtype or x.dtype
-        xt = _row_type(x)
         mats = (gate, up, down)
         if torch.is_grad_enabled() and (x.requires_grad or any(m.scale.requires_grad for m in mats)):
-            from . import tuning as T
-
-            act = T.gated(gate, up, T.rotate(x, gate.rot, xt), self.activation)
-            return T.linear(down, T.rotate(act, down.rot), od)
+            return T.product_of(down, T.gated_of(gate, up, x, self.activation), od)
         x2 = x.reshape(-1, gate.n).contiguous()
         g0, g1, cb0, cb1 = gate._planes()
         if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], cb0) for m in mats):
@@ -361,14 +358,9 @@ class PackedMLP(nn.Module):
         if gate.planes_released or up.planes_released:
             raise K.Vq2Error("PackedMLP: the index planes, which more than one row needs, were released")
         u0, u1, _, _ = up._planes()
-        xr = gate.rot.fwd(x2, out_dtype=xt)
+        xr = gate.rot.fwd(x2, out_dtype=T._row_type(x))
         act = K.vq_gated_rows(xr, (g0, g1, gate.scale), (u0, u1, up.scale), cb0, cb1, gate.n, activation=self.activation)
         return down(act, out_dtype=od).view(*x.shape[:-1], down.out)
-
-
-def _row_type(x):
-    """the type that rotated rows of x are held in: its own, fp16 for fp32"""
-    return torch.float16 if x.dtype == torch.float32 else x.dtype
 
 
 class PackedLMHead(nn.Module):
@@ -395,13 +387,11 @@ class PackedLMHead(nn.Module):
         is ignore_index.  Differentiable in x and, where it requires a
         gradient, the head's ``scale``.  The rotated rows are held in x's type
         (fp32: fp16)."""
-        from . import tuning as T
-
         lin = self.lin
         x2 = x.reshape(-1, lin.n)
         if lin.planes_released:
             raise K.Vq2Error("loss needs the head's index planes, which were released")
-        return T.head_loss(lin, T.rotate(x2, lin.rot, _row_type(x)), targets, ignore_index)
+        return T.head_loss_of(lin, x2, targets, ignore_index)
 
     def argmax(self, x):
         """Top-1 token per row of x without materialising bf16 logits:

@@ -13,7 +13,9 @@ one entry of ``kernels`` forward and one backward:
   head_loss(lin, xr, targets)   the loss of every token
 
 ``xr`` are rotated rows in fp16 or bf16 (``rotate`` or ``add_rms_norm`` give
-them).  ``runtime.PackedMLP`` and ``PackedLMHead.loss`` are built on them.  The
+them), and their gradients are of that type: fp16 rows want a scaled loss.
+``runtime.PackedMLP`` and ``PackedLMHead.loss`` rotate inside the same functions;
+theirs are of the activations' type, in fp32 with its range (terms of 11 bits).  The
 reference distils and tunes with dequantized weights in torch (vq2/kd.py); here
 no dequantized matrix is kept.
 
@@ -46,6 +48,27 @@ def _planes(lin):
 
 def _to(t, like):
     return None if t is None else t.to(like.dtype)
+
+
+def _row_type(x):
+    """the type that rotated rows of x are held in: its own, fp16 for fp32"""
+    return torch.float16 if x.dtype == torch.float32 else x.dtype
+
+
+def _rows_of(ctx, x, rot):
+    """The rotated rows of an operator's input: x itself, or x turned by rot.
+    Inside one autograd function, so that the gradient of fp32 activations is
+    fp32 all the way back, and never that of the fp16 rows: most gradients of
+    a mean over many tokens lie below fp16's numbers."""
+    ctx.rot, ctx.dtype = rot, x.dtype
+    ctx.wide = rot is not None and x.dtype == torch.float32
+    return x if rot is None else rot.fwd(x, out_dtype=_row_type(x))
+
+
+def _input_grad(ctx, dxr):
+    if ctx.rot is None or not ctx.needs_input_grad[0]:
+        return dxr
+    return ctx.rot.inv(dxr, out_dtype=ctx.dtype)
 
 
 class _Rotate(torch.autograd.Function):
@@ -82,9 +105,10 @@ class _Norm(torch.autograd.Function):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, xr, scale, lin, out_dtype):
+    def forward(ctx, x, scale, lin, out_dtype, rot):
         from .runtime import vq_matmul
 
+        xr = _rows_of(ctx, x, rot)
         ctx.save_for_backward(xr, scale)
         ctx.lin = lin
         i0, i1, cb0, cb1 = _planes(lin)
@@ -102,17 +126,19 @@ class _Linear(torch.autograd.Function):
         lin = ctx.lin
         i0, i1, cb0, cb1 = _planes(lin)
         dx, ds = K.vq_gemm_backward(dy.contiguous(), xr, i0, i1, cb0, cb1, scale, lin.out, lin.n,
-                                    scale_grad=ctx.needs_input_grad[1])
-        return dx, _to(ds, scale), None, None
+                                    scale_grad=ctx.needs_input_grad[1], wide=ctx.wide)
+        return _input_grad(ctx, dx), _to(ds, scale), None, None, None
 
 
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, xr, gate_scale, up_scale, gate, up, activation):
+    def forward(ctx, x, gate_scale, up_scale, gate, up, activation, rot):
+        xr = _rows_of(ctx, x, rot)
         ctx.save_for_backward(xr, gate_scale, up_scale)
         ctx.mats, ctx.activation = (gate, up), activation
         (g0, g1, cb0, cb1), (u0, u1, _, _) = _planes(gate), _planes(up)
-        return K.vq_gated_rows(xr, (g0, g1, gate_scale), (u0, u1, up_scale), cb0, cb1, gate.n, activation=activation)
+        act = K.vq_gated_rows(xr, (g0, g1, gate_scale), (u0, u1, up_scale), cb0, cb1, gate.n, activation=activation)
+        return act.float() if ctx.wide else act  # (its gradient takes its type)
 
     @staticmethod
     @once_differentiable
@@ -122,13 +148,14 @@ class _Gated(torch.autograd.Function):
         (g0, g1, cb0, cb1), (u0, u1, _, _) = _planes(gate), _planes(up)
         dx, dg, du = K.vq_gated_rows_backward(dact.contiguous(), xr, (g0, g1, gate_scale), (u0, u1, up_scale), cb0, cb1,
                                               gate.n, activation=ctx.activation,
-                                              scale_grad=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
-        return dx, _to(dg, gate_scale), _to(du, up_scale), None, None, None
+                                              scale_grad=ctx.needs_input_grad[1] or ctx.needs_input_grad[2], wide=ctx.wide)
+        return _input_grad(ctx, dx), _to(dg, gate_scale), _to(du, up_scale), None, None, None, None
 
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, xr, scale, lin, targets, ignore_index):
+    def forward(ctx, x, scale, lin, targets, ignore_index, rot):
+        xr = _rows_of(ctx, x, rot)
         i0, i1, cb0, cb1 = _planes(lin)
         loss, lse = K.vq_head_loss(xr, targets, i0, i1, cb0, cb1, scale, lin.out, lin.n, ignore_index=ignore_index)
         ctx.save_for_backward(xr, scale, targets, lse)
@@ -142,8 +169,8 @@ class _HeadLoss(torch.autograd.Function):
         lin = ctx.lin
         i0, i1, cb0, cb1 = _planes(lin)
         dx, ds = K.vq_head_loss_backward(xr, targets, lse, dloss.contiguous(), i0, i1, cb0, cb1, scale, lin.out, lin.n,
-                                         ignore_index=ctx.ignore_index, scale_grad=ctx.needs_input_grad[1])
-        return dx, _to(ds, scale), None, None, None
+                                         ignore_index=ctx.ignore_index, scale_grad=ctx.needs_input_grad[1], wide=ctx.wide)
+        return _input_grad(ctx, dx), _to(ds, scale), None, None, None, None
 
 
 def rotate(x, rot, out_dtype=None):
@@ -162,14 +189,29 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, rot=
 
 def linear(lin, xr, out_dtype=None):
     """A PackedLinear's product with rotated rows, in their type or out_dtype."""
-    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype)
+    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype, None)
+
+
+def product_of(lin, x, out_dtype):
+    """A PackedLinear's product with rows that are not rotated, for the modules."""
+    return _Linear.apply(x.contiguous(), lin.scale, lin, out_dtype, lin.rot)
 
 
 def gated(gate, up, xr, activation="silu"):
     """f(gate xr) * (up xr) of two PackedLinears of one width, cfg, codebooks and rotation."""
-    return _Gated.apply(_rows16(xr, "gated"), gate.scale, up.scale, gate, up, activation)
+    return _Gated.apply(_rows16(xr, "gated"), gate.scale, up.scale, gate, up, activation, None)
+
+
+def gated_of(gate, up, x, activation):
+    """The same of rows that are not rotated, in x's type, for the modules."""
+    return _Gated.apply(x.contiguous(), gate.scale, up.scale, gate, up, activation, gate.rot)
 
 
 def head_loss(lin, xr, targets, ignore_index=-100):
     """kernels.vq_head_loss of a head's PackedLinear: the loss of every row, fp32."""
-    return _HeadLoss.apply(_rows16(xr, "head_loss").reshape(-1, lin.n), lin.scale, lin, targets.reshape(-1).contiguous(), ignore_index)
+    return _HeadLoss.apply(_rows16(xr, "head_loss").reshape(-1, lin.n), lin.scale, lin, targets.reshape(-1).contiguous(), ignore_index, None)
+
+
+def head_loss_of(lin, x, targets, ignore_index):
+    """The same of rows that are not rotated, for the modules."""
+    return _HeadLoss.apply(x.reshape(-1, lin.n).contiguous(), lin.scale, lin, targets.reshape(-1).contiguous(), ignore_index, lin.rot)

@@ -35,6 +35,9 @@ extern "C" {
 /* 8-bit rows under a scale for each row, where an entry says so */
 #define VQ2_DT_I8 3
 #define VQ2_DT_E4M3 4
+/* dx of the backward entries of packed products for fp32 activations: words of fp32, for its
+ * range; the terms they are sums of are rounded to 11 bits, so VQ2_DT_F32 is refused there */
+#define VQ2_DT_F32_RANGE 5
 
 /* activations of the gated block */
 #define VQ2_ACT_SILU 0
@@ -769,7 +772,8 @@ int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt
  *   x       [tokens, n] rotated rows, 16-byte aligned: VQ2_DT_F16 / BF16, in forward
  *           calls also VQ2_DT_I8 / VQ2_DT_E4M3 with x_scale [tokens] (NULL otherwise)
  *   n       a multiple of 64 up to VQ2_PANEL_MAX_N; out_rows up to VQ2_PANEL_MAX_ROWS
- *   dx      gradients of x, VQ2_DT_F16 / BF16, 16-byte aligned;  dscale  of the row scales, fp32, or NULL
+ *   dx      gradients of x, VQ2_DT_F16 / BF16 / F32_RANGE, 16-byte aligned;  dscale  of the row scales, fp32,
+ *           or NULL
  *   workspace  256-byte aligned, of the entry's _workspace bytes (scale_grad:
  *           whether dscale is wanted); contents on entry do not matter
  * Weights are multiplied in fp16 (where an fp16 or fp32 result depends on more bits, as

@@ -68,3 +68,82 @@ def test_mlp_result_type_under_grad(dev, rows):
         # (in fp16, too, the gradient of 2^20 W comes back in range)
         (y * 2.0 ** -20).sum().backward()
         assert torch.isfinite(x.grad).all() and x.grad.abs().max() > 0
+
+
+def _fp32_mlp(dev):
+    cbs = books(dev)
+    mlp = PackedMLP(*(lin(40 + k, I, H, "mlp.in", cbs, (16, 16)) for k in range(2)), lin(42, H, I, "mlp.down", cbs, (16, 16)))
+    for m in (mlp.gate, mlp.up, mlp.down):
+        m.scale = m.scale.float().requires_grad_()
+    return mlp
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("f", [1.0, 2.0 ** -40, 2.0 ** 40])
+def test_fp32_gradients_of_the_block(dev, rows, f):
+    """fp32 activations: gradients of any size in fp32's range, dx and the scales', from fp32 upstream values.  Their
+    roundings to 11 bits (x rotated, act, act rotated, the terms between the two products, twice) are those of gradients
+    near 1, each as often again for what it does to the values it meets"""
+    mlp = _fp32_mlp(dev)
+    x = synth.activations(43, (rows, H), torch.float32).to(dev).requires_grad_()
+    dy = (synth.activations(44, (rows, H), torch.float32) * f).to(dev)
+    y = mlp(x)
+    y.backward(dy)
+    x64 = x.detach().double().requires_grad_()
+    s64 = [m.scale.detach().double().requires_grad_() for m in (mlp.gate, mlp.up, mlp.down)]
+    act = torch.nn.functional.silu(linear64(mlp.gate, x64, s64[0])) * linear64(mlp.up, x64, s64[1])
+    want = linear64(mlp.down, act, s64[2])
+    want.backward(dy.double())
+    assert y.dtype == x.grad.dtype == torch.float32
+    close(y, want, 10 * 2.0 ** -11)
+    close(x.grad, x64.grad, 10 * 2.0 ** -11)
+    for m, s in zip((mlp.gate, mlp.up, mlp.down), s64):
+        close(m.scale.grad, s.grad, 10 * 2.0 ** -11)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("f", [1.0, 2.0 ** -40, 2.0 ** 40])
+def test_fp32_gradients_of_the_loss(dev, rows, f):
+    """as above; roundings: x rotated (in the logits, and so in every probability), the terms between the products"""
+    head = PackedLMHead(lin(45, V, H, "head", books(dev), (16, 16)))
+    head.lin.scale = head.lin.scale.float().requires_grad_()
+    x = synth.activations(46, (rows, H), torch.float32).to(dev).requires_grad_()
+    t = torch.randint(0, V, (rows,), generator=synth.gen(47)).to(dev)
+    dl = (torch.rand(rows, generator=synth.gen(48)) * f).to(dev)
+    head.loss(x, t).backward(dl)
+    x64, s64 = x.detach().double().requires_grad_(), head.lin.scale.detach().double().requires_grad_()
+    want = torch.nn.functional.cross_entropy(linear64(head.lin, x64, s64), t, reduction="none")
+    want.backward(dl.double())
+    assert x.grad.dtype == torch.float32
+    close(x.grad, x64.grad, 10 * 2.0 ** -11)
+    close(head.lin.scale.grad, s64.grad, 10 * 2.0 ** -11)
+
+
+@pytest.mark.parametrize("rows,n", [(96, 128), (203, 128), (1000, 2048), (100, 4096)])
+@pytest.mark.parametrize("tokens", [1, 130, 2100])
+def test_wide_gradients_are_the_same_sums(dev, rows, n, tokens):
+    """dx in fp32, rounded to fp16, is dx in fp16; upstream values in fp32 (by vectors, and one by one from another
+    address) give what the same values give in fp16, the scales' gradients, too"""
+    cbs = books(dev)
+    a, b = lin(50, rows, n, "x", cbs, (16, 16)) if n < 4096 else lin(50, rows, n, "x", cbs), None
+    b = lin(53, rows, n, "x", cbs, a.cfg)
+    a.scale, b.scale = a.scale.float(), b.scale.float()
+    i0, i1, cb0, cb1 = a._planes()
+    j0, j1, _, _ = b._planes()
+    gate, up, head = (i0, i1, a.scale), (j0, j1, b.scale), (i0, i1, cb0, cb1, a.scale, rows, n)
+    x = synth.activations(54, (tokens, n), torch.float16).to(dev)
+    d = (synth.activations(55, (tokens, rows), torch.float32) * 1e-2).to(torch.float16).to(dev)
+    t = torch.randint(0, rows, (tokens,), generator=synth.gen(56)).to(dev)
+    dl = torch.ones(tokens, device=dev)
+    _, lse = K.vq_head_loss(x, t, *head)
+    off = torch.empty(tokens * rows + 1, device=dev)[1:].view(tokens, rows).copy_(d)
+    calls = [lambda dy, **kw: K.vq_gemm_backward(dy, x, *head, scale_grad=True, **kw),
+             lambda dy, **kw: K.vq_gated_rows_backward(dy, x, gate, up, cb0, cb1, n, scale_grad=True, **kw),
+             lambda dy, **kw: K.vq_head_loss_backward(x, t, lse, dl, *head, scale_grad=True, **kw)]
+    for call in calls:
+        want = call(d)
+        assert want[0].dtype == torch.float16
+        for dy in (d, d.float(), off):
+            got = call(dy, wide=True)
+            assert got[0].dtype == torch.float32 and torch.equal(got[0].half(), want[0])
+            assert all(torch.equal(p, q) for p, q in zip(got[1:], want[1:]))

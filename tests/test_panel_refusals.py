@@ -100,3 +100,18 @@ def test_gated_and_product():
     assert "x is NULL" in _err(p(x=None))
     assert "dy dtype" in _err(p(dy_dt=3))
     assert "dy or dx" in _err(p())
+
+
+def test_fp32_gradients_have_a_name_of_their_own():
+    """dx in fp32 is for its range: the plain type is refused, the name for it is taken (up to the next check)"""
+    L = _lib.load()
+    assert _lib.DT_F32_RANGE == 5
+    call = lambda dx_dt, size=1 << 40: L.vq2_gemm_backward(P, 2, None, 2, 3, P, None, 0, P, None, 1, P, 2, 100, 128, 1.0, P, dx_dt, None, P,
+                                                           size, None)
+    assert "F32_RANGE" in _err(call(0)) and "fp16 or bf16" in _err(call(3))
+    need = L.vq2_gemm_backward_workspace(3, 100, 128, 0, 1, _lib.DT_F32_RANGE, 0)
+    assert need > 0 and "workspace" in _err(call(_lib.DT_F32_RANGE, need - 256))
+    # two parts of a weight, as for fp16, where its stages' sum has more bits
+    for entry, sizes in (("head_loss", (3, 100, 128, 2, 1)), ("gated_rows", (3, 100, 128, 2, 1)), ("gemm", (3, 100, 128, 2, 1))):
+        ws = getattr(L, f"vq2_{entry}_backward_workspace")
+        assert ws(*sizes, _lib.DT_F32_RANGE, 0) == ws(*sizes, 1, 0) > ws(*sizes, 2, 0) > 0
