@@ -179,7 +179,11 @@ def rotate(x, rot, out_dtype=None):
 
 
 def add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, rot=None, out_dtype=None):
-    """(y, h) of kernels.vq_add_rms_norm; y is rotated where a ``rot.Rot`` is given."""
+    """(y, h) of kernels.vq_add_rms_norm; y is rotated where a ``rot.Rot`` is given.
+    out_dtype: 16 or 32 bits (8-bit rows, which are numbers only with their
+    scales and have no gradient, are the kernel entry's alone)."""
+    if out_dtype in K._DT8:
+        raise K.Vq2Error("add_rms_norm: y in 8 bits has no gradient (kernels.vq_add_rms_norm gives it with its scales)")
     kw = dict(eps=eps, zero_centred=zero_centred)
     if rot is not None:
         kw.update(perm=rot._perm32, sign=rot._sign8, hb=rot.hb, rht_scale=rot.scale)

@@ -147,3 +147,12 @@ def test_wide_gradients_are_the_same_sums(dev, rows, n, tokens):
             got = call(dy, wide=True)
             assert got[0].dtype == torch.float32 and torch.equal(got[0].half(), want[0])
             assert all(torch.equal(p, q) for p, q in zip(got[1:], want[1:]))
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_norm_refuses_8_bits(dev, dtype):
+    """8-bit rows are numbers only with their scales, and have no gradient"""
+    x, w = torch.ones(3, H, device=dev, dtype=torch.bfloat16), torch.ones(H, device=dev)
+    for kw in (dict(), dict(residual=x), dict(rot=lin(1, 8, H, "head", books(dev)).rot)):
+        with pytest.raises(K.Vq2Error, match="8 bits"):
+            T.add_rms_norm(x, w, out_dtype=dtype, **kw)
