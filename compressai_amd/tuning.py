@@ -47,7 +47,7 @@ def _planes(lin):
 
 
 def _to(t, like):
-    return None if t is None else t.to(like.dtype)
+    return None if t is None else t.view(like.shape).to(like.dtype)
 
 
 def _row_type(x):

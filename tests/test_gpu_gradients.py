@@ -156,3 +156,26 @@ def test_norm_refuses_8_bits(dev, dtype):
     for kw in (dict(), dict(residual=x), dict(rot=lin(1, 8, H, "head", books(dev)).rot)):
         with pytest.raises(K.Vq2Error, match="8 bits"):
             T.add_rms_norm(x, w, out_dtype=dtype, **kw)
+
+
+def test_gradients_have_their_leaves_shapes(dev):
+    """weights and scales of any shape that holds as many values"""
+    x = synth.activations(60, (5, H), torch.bfloat16).to(dev)
+    w = torch.ones(1, H, device=dev, requires_grad=True)
+    y, _ = T.add_rms_norm(x, w)
+    flat = torch.ones(H, device=dev, requires_grad=True)
+    z, _ = T.add_rms_norm(x, flat)
+    g = torch.autograd.grad(y.sum(), w)[0]
+    assert g.shape == w.shape and torch.equal(g.view(-1), torch.autograd.grad(z.sum(), flat)[0])
+    cbs = books(dev)
+    gate, up, head = lin(61, I, H, "mlp.in", cbs), lin(62, I, H, "mlp.in", cbs), lin(63, V, H, "head", cbs)
+    t = torch.zeros(5, dtype=torch.int64, device=dev)
+    for m, call in ((head, lambda: T.linear(head, x)), (head, lambda: T.head_loss(head, x, t)), (gate, lambda: T.gated(gate, up, x))):
+        s = m.scale
+        grads = []
+        for shape in ((-1,), (-1, 1)):
+            m.scale = s.detach().view(shape).requires_grad_()
+            grads.append(torch.autograd.grad(call().sum(), m.scale)[0])
+            assert grads[-1].shape == m.scale.shape
+        assert torch.equal(grads[0], grads[1].view(-1))
+        m.scale = s
