@@ -1679,6 +1679,7 @@ def vq_unpack_fixed(buf, bits, n, *, out=None):
 
 
 # ------------------------------- around the packed products, and their gradients
+PANEL_MAX_N = 32768  # widest rows of the entries below, as VQ2_PANEL_MAX_N
 _DT8 = {torch.int8: _lib.DT_I8, torch.float8_e4m3fn: _lib.DT_E4M3}
 _ACTS = {"silu": _lib.ACT_SILU, "gelu_tanh": _lib.ACT_GELU_TANH}
 

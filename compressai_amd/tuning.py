@@ -193,6 +193,8 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, zero_centred=False, rot=
 
 def linear(lin, xr, out_dtype=None):
     """A PackedLinear's product with rotated rows, in their type or out_dtype."""
+    if (lin.n % 64 or lin.n > K.PANEL_MAX_N) and torch.is_grad_enabled() and (xr.requires_grad or lin.scale.requires_grad):
+        raise K.Vq2Error(f"linear: a gradient needs a width that is a multiple of 64 up to {K.PANEL_MAX_N}, got {lin.n}")
     return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype, None)
 
 

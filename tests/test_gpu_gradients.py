@@ -179,3 +179,20 @@ def test_gradients_have_their_leaves_shapes(dev):
             assert grads[-1].shape == m.scale.shape
         assert torch.equal(grads[0], grads[1].view(-1))
         m.scale = s
+
+
+@pytest.mark.parametrize("n,out", [(32, 24), (17 * 2048, 16)])
+def test_linear_refuses_widths_without_a_gradient(dev, n, out):
+    """widths that the backward pass does not take are refused where a gradient is asked for, and multiplied where none is"""
+    m = lin(64, out, n, "wide", books(dev))
+    x = synth.activations(65, (4, n), torch.bfloat16).to(dev)
+    y = T.linear(m, x)
+    want = x.double() @ (weight64(m) * m.scale.double()[:, None]).t()
+    close(y, want, 4 * 2.0 ** -8)
+    with pytest.raises(K.Vq2Error, match="multiple of 64 up to 32768"):
+        T.linear(m, x.clone().requires_grad_())
+    m.scale.requires_grad_()
+    with pytest.raises(K.Vq2Error, match="multiple of 64 up to 32768"):
+        T.linear(m, x)
+    with torch.no_grad():
+        assert torch.equal(T.linear(m, x), y)
