@@ -344,7 +344,7 @@ class PackedMLP(nn.Module):
             return T.product_of(down, T.gated_of(gate, up, x, self.activation), od)
         x2 = x.reshape(-1, gate.n).contiguous()
         g0, g1, cb0, cb1 = gate._planes()
-        if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], cb0) for m in mats):
+        if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], m._planes()[2]) for m in mats):
             I = gate.out
             gu = torch.empty(2 * I, dtype=torch.float32, device=x.device)
             xs, perm, sign, hb, sc = gate._sorted_args(x2.reshape(-1))

@@ -196,3 +196,15 @@ def test_linear_refuses_widths_without_a_gradient(dev, n, out):
         T.linear(m, x)
     with torch.no_grad():
         assert torch.equal(T.linear(m, x), y)
+
+
+def test_mlp_down_of_other_codebooks(dev):
+    """gate and up on the sorted layout, down with one of its own whose fp32 codebooks that layout does not take: one row
+    goes the way that more rows go.  Roundings to bf16: x rotated, act, act rotated, y, each as often again"""
+    cbs, fine = books(dev), books(dev, torch.float32)
+    mlp = PackedMLP(*(lin(66 + k, I, H, "mlp.in", cbs, sorted_layout=True) for k in range(2)),
+                    lin(68, H, I, "mlp.down", fine, sorted_layout=True))
+    x = synth.activations(69, (1, H), torch.bfloat16).to(dev)
+    x64 = x.double()
+    want = linear64(mlp.down, torch.nn.functional.silu(linear64(mlp.gate, x64)) * linear64(mlp.up, x64))
+    close(mlp(x), want, 8 * 2.0 ** -8)
