@@ -13,6 +13,8 @@
 // i.e. two LDS round trips and no cross-lane shuffles.  The permutation
 // gather, the sign flip, the optional SwiGLU of the MoE epilogue, the scale
 // and the dtype conversion are fused into the first and last passes.
+#include <algorithm>
+
 #include "vq2_common.hpp"
 #include "vq2_internal.hpp"
 
@@ -318,7 +320,7 @@ int rht_launch(const void* x, int x_dt, int64_t x_stride, void* y, int y_dt, int
     if (L < 1 || L > 13 || (1LL << L) != hb)
         return set_error(VQ2_ERR_ARG, "vq2 rht: hb=%lld must be a power of two in [2, 8192]", (long long)hb);
     if (n % hb) return set_error(VQ2_ERR_ARG, "vq2 rht: n=%lld is not a multiple of hb=%lld", (long long)n, (long long)hb);
-    if (batch > 65535 || n / hb > 0x7FFFFFFF) return set_error(VQ2_ERR_UNSUPPORTED, "vq2 rht: grid too large");
+    if (n / hb > 0x7FFFFFFF) return set_error(VQ2_ERR_UNSUPPORTED, "vq2 rht: grid too large");
     const int64_t esz = dt_size(x_dt);
     const bool stage = !inverse && !swiglu && perm && (uintptr_t)x % 16 == 0 && (x_stride * esz) % 16 == 0 &&
                        (n * esz) % 16 == 0 && n * esz <= RHT_STAGE_BYTES && (uintptr_t)perm % 16 == 0 &&
@@ -327,20 +329,26 @@ int rht_launch(const void* x, int x_dt, int64_t x_stride, void* y, int y_dt, int
     hipStream_t st = (hipStream_t)stream;
     const int64_t nblk = n / hb;
     const size_t shm = stage ? (size_t)(n * esz) : 0;
-    switch (L) {
-    case 1: launch_rht_l<1>(a, nblk, batch, shm, st); break;
-    case 2: launch_rht_l<2>(a, nblk, batch, shm, st); break;
-    case 3: launch_rht_l<3>(a, nblk, batch, shm, st); break;
-    case 4: launch_rht_l<4>(a, nblk, batch, shm, st); break;
-    case 5: launch_rht_l<5>(a, nblk, batch, shm, st); break;
-    case 6: launch_rht_l<6>(a, nblk, batch, shm, st); break;
-    case 7: launch_rht_l<7>(a, nblk, batch, shm, st); break;
-    case 8: launch_rht_l<8>(a, nblk, batch, shm, st); break;
-    case 9: launch_rht_l<9>(a, nblk, batch, shm, st); break;
-    case 10: launch_rht_l<10>(a, nblk, batch, shm, st); break;
-    case 11: launch_rht_l<11>(a, nblk, batch, shm, st); break;
-    case 12: launch_rht_l<12>(a, nblk, batch, shm, st); break;
-    default: launch_rht_l<13>(a, nblk, batch, shm, st); break;
+    // (a grid holds 65535 rows)
+    for (int64_t b0 = 0; b0 < batch; b0 += 65535) {
+        const int64_t rows = std::min<int64_t>(65535, batch - b0);
+        a.x = (const char*)x + b0 * x_stride * esz;
+        a.y = (char*)y + b0 * y_stride * dt_size(y_dt);
+        switch (L) {
+        case 1: launch_rht_l<1>(a, nblk, rows, shm, st); break;
+        case 2: launch_rht_l<2>(a, nblk, rows, shm, st); break;
+        case 3: launch_rht_l<3>(a, nblk, rows, shm, st); break;
+        case 4: launch_rht_l<4>(a, nblk, rows, shm, st); break;
+        case 5: launch_rht_l<5>(a, nblk, rows, shm, st); break;
+        case 6: launch_rht_l<6>(a, nblk, rows, shm, st); break;
+        case 7: launch_rht_l<7>(a, nblk, rows, shm, st); break;
+        case 8: launch_rht_l<8>(a, nblk, rows, shm, st); break;
+        case 9: launch_rht_l<9>(a, nblk, rows, shm, st); break;
+        case 10: launch_rht_l<10>(a, nblk, rows, shm, st); break;
+        case 11: launch_rht_l<11>(a, nblk, rows, shm, st); break;
+        case 12: launch_rht_l<12>(a, nblk, rows, shm, st); break;
+        default: launch_rht_l<13>(a, nblk, rows, shm, st); break;
+        }
     }
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return set_hip_error(err, "vq2 rht launch");

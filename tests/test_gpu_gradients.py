@@ -208,3 +208,31 @@ def test_mlp_down_of_other_codebooks(dev):
     x64 = x.double()
     want = linear64(mlp.down, torch.nn.functional.silu(linear64(mlp.gate, x64)) * linear64(mlp.up, x64))
     close(mlp(x), want, 8 * 2.0 ** -8)
+
+
+def test_more_rows_than_a_grid(dev):
+    """the rotation in front of the block and the loss takes any number of rows"""
+    cbs = books(dev)
+    head = PackedLMHead(lin(92, 40, 64, "head", cbs))
+    mlp = PackedMLP(lin(93, 64, 64, "mlp.in", cbs), lin(94, 64, 64, "mlp.in", cbs), lin(95, 64, 64, "mlp.down", cbs))
+    n = 65535 + 70
+    x = synth.activations(96, (n, 64), torch.bfloat16).to(dev)
+    t = torch.randint(0, 40, (n,), generator=synth.gen(97)).to(dev)
+    loss, y, g = [], [], []
+    for s in (slice(0, n), slice(0, 40000), slice(40000, n)):
+        leaf = x[s].clone().requires_grad_()
+        loss.append(head.loss(leaf, t[s]))
+        y.append(mlp(leaf))
+        g.append(torch.autograd.grad((loss[-1].sum(), y[-1]), leaf, (None, torch.ones_like(y[-1])))[0])
+    for v in (loss, y, g):
+        a, b = v[0].detach().double(), torch.cat(v[1:]).detach().double()
+        # (tokens are taken 8192 at a time: others share a launch, and its order of sums)
+        assert ((a - b).abs() <= 2.0 ** -6 * b.abs() + 2.0 ** -6 * b.abs().max()).all()
+    r = mlp.gate.rot
+    z = r.fwd(x)
+    assert torch.equal(z[65535:], r.fwd(x[65535:])) and torch.equal(z[:40], r.fwd(x[:40]))
+    # half a step of bf16, there and back
+    assert ((r.inv(z) - x).abs().float() <= 2.0 ** -7 * x.float().abs().max()).all()
+    gu = synth.activations(98, (n, 128), torch.bfloat16).to(dev)
+    a = K.vq_swiglu_rht(gu, 64)
+    assert torch.equal(a[65535:], K.vq_swiglu_rht(gu[65535:], 64))
