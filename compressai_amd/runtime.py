@@ -13,8 +13,8 @@ dequantized matrix (runtime.py:91-110).
 ``sample`` (the next token under temperature, top-k, top-p and min-p) and ``loss``
 (of given tokens, without the logits).
 ``PackedProjections`` runs projections of one activation (q, k, v) in one
-launch, ``PackedMLP`` the gated feed-forward block; the latter and ``loss`` are
-differentiable (``tuning``).
+launch, ``PackedMLP`` the gated feed-forward block.  All of them, and ``loss``, are
+differentiable in x and the row scales (``tuning``).
 
 Large matrices (``SORTED_MIN_CODES`` codes or more, 2 and 4 bpw) also keep
 a code-sorted copy of their index planes (``kernels.SortedPlanes``, packed
@@ -103,8 +103,21 @@ def _rows_ok(x2, n, rot):
     return x2.shape[0] >= 3 and n % 64 == 0 and n <= K.ROWS_GEMM_MAX_N and rot.hb >= 64
 
 
+def _grad_wanted(x, lins):
+    if not torch.is_grad_enabled():
+        return False
+    if x.requires_grad:
+        return True
+    for m in lins:
+        if m.scale.requires_grad:
+            return True
+    return False
+
+
 class PackedLinear(nn.Module):
-    """``scale_dtype``: the row scales are held in bf16 by default, as the
+    """Differentiable in x, and in ``scale`` where it is made a leaf (in fp32
+    for small steps; it is a buffer that ``state_dict`` leaves out, so a tuned
+    one is stored by its owner).  ``scale_dtype``: the row scales are held in bf16 by default, as the
     reference rounds them at construction (vq2/runtime.py:78); ``None`` keeps
     the given dtype (e.g. the container's fp16 scales, one rounding fewer)."""
 
@@ -196,6 +209,11 @@ class PackedLinear(nn.Module):
         return r.fwd(x1, out_dtype=torch.float32), None, None, 0, 1.0
 
     def forward(self, x, out_dtype=None):
+        if _grad_wanted(x, (self,)):
+            return T.module_products(x, lambda x: [self._product(x, out_dtype)], (self,))[0]
+        return self._product(x, out_dtype)
+
+    def _product(self, x, out_dtype):
         x2 = x.reshape(-1, self.n).contiguous()
         i0, i1, cb0, cb1 = self._planes()
         od = out_dtype or x.dtype
@@ -278,6 +296,11 @@ class PackedProjections(nn.Module):
                 self.sorted.append(sp)
 
     def forward(self, x, out_dtype=None):
+        if _grad_wanted(x, self.lins):
+            return list(T.module_products(x, lambda x: self._products(x, out_dtype), tuple(self.lins)))
+        return self._products(x, out_dtype)
+
+    def _products(self, x, out_dtype):
         lins = list(self.lins)
         a = lins[0]
         x2 = x.reshape(-1, a.n).contiguous()
@@ -340,8 +363,8 @@ class PackedMLP(nn.Module):
         gate, up, down = self.gate, self.up, self.down
         od = out_dtype or x.dtype
         mats = (gate, up, down)
-        if torch.is_grad_enabled() and (x.requires_grad or any(m.scale.requires_grad for m in mats)):
-            return T.product_of(down, T.gated_of(gate, up, x, self.activation), od)
+        if _grad_wanted(x, mats):
+            return down(T.gated_of(gate, up, x, self.activation), out_dtype=od)
         x2 = x.reshape(-1, gate.n).contiguous()
         g0, g1, cb0, cb1 = gate._planes()
         if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], m._planes()[2]) for m in mats):

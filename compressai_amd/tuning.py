@@ -14,8 +14,11 @@ one entry of ``kernels`` forward and one backward:
 
 ``xr`` are rotated rows in fp16 or bf16 (``rotate`` or ``add_rms_norm`` give
 them), and their gradients are of that type: fp16 rows want a scaled loss.
-``runtime.PackedMLP`` and ``PackedLMHead.loss`` rotate inside the same functions;
-theirs are of the activations' type, in fp32 with its range (terms of 11 bits).  The
+``runtime``'s modules (``PackedLinear``, ``PackedProjections``, ``PackedMLP``,
+``PackedLMHead`` and its ``loss``) are differentiable by themselves, with the
+results that they have without a gradient (``PackedMLP``'s single rows: up to
+rounding); they rotate inside, and their gradients are of the activations' type, in
+fp32 with its range (terms of 11 bits).  Expert pools (``moe``, ``paged``) have no gradient.  The
 reference distils and tunes with dequantized weights in torch (vq2/kd.py); here
 no dequantized matrix is kept.
 
@@ -48,6 +51,11 @@ def _planes(lin):
 
 def _to(t, like):
     return None if t is None else t.view(like.shape).to(like.dtype)
+
+
+def _own(y):
+    """y as no view of another tensor: a function's result may then be written over (y += residual)"""
+    return y.new_empty(0).set_(y) if y._is_view() else y
 
 
 def _row_type(x):
@@ -105,10 +113,9 @@ class _Norm(torch.autograd.Function):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, scale, lin, out_dtype, rot):
+    def forward(ctx, xr, scale, lin, out_dtype):
         from .runtime import vq_matmul
 
-        xr = _rows_of(ctx, x, rot)
         ctx.save_for_backward(xr, scale)
         ctx.lin = lin
         i0, i1, cb0, cb1 = _planes(lin)
@@ -126,8 +133,43 @@ class _Linear(torch.autograd.Function):
         lin = ctx.lin
         i0, i1, cb0, cb1 = _planes(lin)
         dx, ds = K.vq_gemm_backward(dy.contiguous(), xr, i0, i1, cb0, cb1, scale, lin.out, lin.n,
-                                    scale_grad=ctx.needs_input_grad[1], wide=ctx.wide)
-        return _input_grad(ctx, dx), _to(ds, scale), None, None, None
+                                    scale_grad=ctx.needs_input_grad[1])
+        return dx, _to(ds, scale), None, None
+
+
+class _Modules(torch.autograd.Function):
+    """Products of PackedLinears that share their input x and its rotation: the
+    results are run(x), whatever kernels that takes; rotated rows in 16 bits are
+    made again for the scales' gradients alone."""
+
+    @staticmethod
+    def forward(ctx, x, run, lins, *scales):
+        ctx.set_materialize_grads(False)
+        # (without scales to tune x is not needed, and may be written over, as residual streams are)
+        ctx.save_for_backward(x if any(ctx.needs_input_grad[3:]) else None, *scales)
+        ctx.lins, ctx.shape, ctx.dtype = lins, x.shape, x.dtype
+        return tuple(_own(y) for y in run(x))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        x, *scales = ctx.saved_tensors
+        need_x, _, _, *need = ctx.needs_input_grad
+        a, wide = ctx.lins[0], ctx.dtype == torch.float32
+        rows = torch.float16 if wide else ctx.dtype
+        xr = a.rot.fwd(x.reshape(-1, a.n), out_dtype=rows) if any(need) else None
+        dx, ds = None, []
+        for lin, s, dy, n in zip(ctx.lins, scales, dys, need):
+            d = None
+            if dy is not None:
+                i0, i1, cb0, cb1 = _planes(lin)
+                part, d = K.vq_gemm_backward(dy.reshape(-1, lin.out).contiguous(), xr if n else None, i0, i1, cb0, cb1, s, lin.out,
+                                             lin.n, scale_grad=n, dx_dtype=rows, wide=wide)
+                dx = part if dx is None else dx + part
+            ds.append(_to(d, s))
+        if dx is not None:
+            dx = a.rot.inv(dx, out_dtype=ctx.dtype).view(ctx.shape) if need_x else None
+        return dx, None, None, *ds
 
 
 class _Gated(torch.autograd.Function):
@@ -195,12 +237,12 @@ def linear(lin, xr, out_dtype=None):
     """A PackedLinear's product with rotated rows, in their type or out_dtype."""
     if (lin.n % 64 or lin.n > K.PANEL_MAX_N) and torch.is_grad_enabled() and (xr.requires_grad or lin.scale.requires_grad):
         raise K.Vq2Error(f"linear: a gradient needs a width that is a multiple of 64 up to {K.PANEL_MAX_N}, got {lin.n}")
-    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype, None)
+    return _Linear.apply(_rows16(xr, "linear"), lin.scale, lin, out_dtype or xr.dtype)
 
 
-def product_of(lin, x, out_dtype):
-    """A PackedLinear's product with rows that are not rotated, for the modules."""
-    return _Linear.apply(x.contiguous(), lin.scale, lin, out_dtype, lin.rot)
+def module_products(x, run, lins):
+    """run(x), results of PackedLinears of one rotation, differentiable in x and the scales."""
+    return _Modules.apply(x, run, lins, *[m.scale for m in lins])
 
 
 def gated(gate, up, xr, activation="silu"):

@@ -236,3 +236,87 @@ def test_more_rows_than_a_grid(dev):
     gu = synth.activations(98, (n, 128), torch.bfloat16).to(dev)
     a = K.vq_swiglu_rht(gu, 64)
     assert torch.equal(a[65535:], K.vq_swiglu_rht(gu[65535:], 64))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 2, 40])
+@pytest.mark.parametrize("cfg", [(16,), (16, 16)])
+def test_modules_have_gradients(dev, dtype, rows, cfg):
+    """PackedLinear, PackedLMHead and PackedProjections: the results they give without a gradient, with those of x and of
+    the scales.  Half a step (fp32: of fp16) at x rotated, dx rotated, the terms between, y and dx, each as often again;
+    three projections add theirs in x's type"""
+    half = torch.finfo(torch.float16 if dtype == torch.float32 else dtype).eps / 2
+    cbs = books(dev)
+    lins = [lin(70 + k, out, H, "attn", cbs, cfg, sorted_layout=False) for k, out in enumerate((H, 72, 40))]
+    x = synth.activations(75, (rows, H), dtype).to(dev)
+    dys = [synth.activations(76 + k, (rows, m.out), dtype).to(dev) for k, m in enumerate(lins)]
+    calls = [(lins[:1], lambda x: [lins[0](x)]), (lins[:1], lambda x: [PackedLMHead(lins[0])(x)]), (lins, PackedProjections(lins))]
+    for mats, call in calls:
+        for tuned in (0, 1, len(mats)):  # scales that take a gradient
+            plain = call(x)
+            assert not any(y.requires_grad for y in plain)
+            leaf = x.clone().requires_grad_()
+            for m in mats[:tuned]:
+                m.scale = m.scale.float().requires_grad_()
+            for m in mats[tuned:]:
+                m.scale = m.scale.float()
+            with torch.no_grad():
+                plain = call(x)
+            ys = call(leaf)
+            assert all(torch.equal(a, b) for a, b in zip(ys, plain))
+            scales = [m.scale for m in mats[:tuned]]
+            got = torch.autograd.grad(ys, [leaf, *scales], dys[:len(mats)])
+            x64 = x.double().requires_grad_()
+            s64 = [m.scale.detach().double().requires_grad_() for m in mats]
+            want = torch.autograd.grad([linear64(m, x64, s) for m, s in zip(mats, s64)], [x64, *s64], [d.double() for d in dys[:len(mats)]])
+            for g, w in zip(got, want):
+                close(g, w, 10 * half)
+            assert got[0].dtype == dtype and got[0].shape == x.shape
+            for m in mats:
+                m.scale = m.scale.detach().to(torch.bfloat16)
+
+
+def test_modules_without_a_gradient_pass(dev):
+    """a module whose backward pass is not there runs as before, and says so when it is asked for"""
+    m = lin(80, 2048, 2048, "big", books(dev), sorted_layout=True)
+    x = synth.activations(81, (3, 2048), torch.bfloat16).to(dev)
+    m.release_planes()
+    with torch.no_grad():
+        plain = m(x)
+    leaf = x.clone().requires_grad_()
+    y = m(leaf)
+    assert torch.equal(y, plain)
+    with pytest.raises(K.Vq2Error, match="released"):
+        y.sum().backward()
+    narrow = lin(82, 16, 32, "narrow", books(dev))
+    x = synth.activations(83, (3, 32), torch.bfloat16).to(dev).requires_grad_()
+    with pytest.raises(K.Vq2Error, match="multiple of 64"):
+        narrow(x).sum().backward()
+
+
+def test_gradient_reaches_through_a_residual_stream(dev):
+    """x + B(A(x)): both ways count"""
+    cbs = books(dev)
+    a, b = lin(84, H, H, "attn", cbs), lin(85, H, H, "attn", cbs)
+    x = synth.activations(86, (9, H), torch.float32).to(dev).requires_grad_()
+    d = synth.activations(87, (9, H), torch.float32).to(dev)
+    h = a(x)
+    y = b(h)
+    h += 1  # (written over: the products with frozen scales do not need it again)
+    (x + y).backward(d)
+    x64 = x.detach().double().requires_grad_()
+    (x64 + linear64(b, linear64(a, x64))).backward(d.double())
+    close(x.grad, x64.grad, 10 * 2.0 ** -11)
+
+
+def test_mlp_calls_its_down_module(dev):
+    """hooks of the down projection see the same calls with and without a gradient"""
+    cbs = books(dev)
+    mlp = PackedMLP(lin(88, I, H, "mlp.in", cbs), lin(89, I, H, "mlp.in", cbs), lin(90, H, I, "mlp.down", cbs))
+    seen = []
+    mlp.down.register_forward_hook(lambda m, a, y: seen.append((a[0].shape, y.shape, y.dtype)))
+    x = synth.activations(91, (4, H), torch.bfloat16).to(dev)
+    with torch.no_grad():
+        mlp(x)
+    mlp(x.requires_grad_()).sum().backward()
+    assert len(seen) == 2 and seen[0] == seen[1]
