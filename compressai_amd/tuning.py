@@ -124,7 +124,7 @@ class _Linear(torch.autograd.Function):
             y = K.vq_rows_gemm(x2, [(i0, i1, scale, lin.out)], cb0, cb1, lin.n, hb=0, act_dtype=xr.dtype, out_dtype=out_dtype)[0]
         else:
             y = vq_matmul(x2, i0, i1, cb0, cb1, scale, lin.out, lin.n, out_dtype)
-        return y.view(*xr.shape[:-1], lin.out)
+        return _own(y.view(*xr.shape[:-1], lin.out))
 
     @staticmethod
     @once_differentiable

@@ -320,3 +320,30 @@ def test_mlp_calls_its_down_module(dev):
         mlp(x)
     mlp(x.requires_grad_()).sum().backward()
     assert len(seen) == 2 and seen[0] == seen[1]
+
+
+def test_results_may_be_written_over(dev):
+    """y += 1 of every result that its own backward pass does not need (the norm's h it does)"""
+    cbs = books(dev)
+    gate, up, down, head = (lin(130 + k, o, n, tag, cbs) for k, (o, n, tag) in enumerate(((I, H, "mlp.in"), (I, H, "mlp.in"),
+                                                                                         (H, I, "mlp.down"), (V, H, "head"))))
+    w = torch.ones(H, device=dev)
+    for rows in (1, 2, 5):
+        for shape in ((rows, H), (1, rows, H)):
+            x = synth.activations(134, shape, torch.bfloat16).to(dev)
+            t = torch.zeros(rows, dtype=torch.int64, device=dev)
+            for call in (lambda x: T.linear(gate, x), lambda x: T.gated(gate, up, x), lambda x: T.rotate(x, gate.rot),
+                         lambda x: T.add_rms_norm(x, w)[0], lambda x: T.head_loss(head, x, t),
+                         gate, PackedProjections([gate, up]), PackedMLP(gate, up, down), PackedLMHead(head),
+                         lambda x: PackedLMHead(head).loss(x, t)):
+                grads = []
+                for change in (0, 1):
+                    leaf = x.clone().requires_grad_()
+                    ys = call(leaf)
+                    ys = ys if isinstance(ys, list) else [ys]
+                    for y in ys:
+                        if change:
+                            y += 1
+                        assert y.shape[-1] in (rows, H, I, V) and y.requires_grad
+                    grads.append(torch.autograd.grad(ys, leaf, [torch.ones_like(y) for y in ys])[0])
+                assert torch.equal(*grads)
