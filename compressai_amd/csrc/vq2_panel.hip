@@ -1117,9 +1117,11 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs a)
 // each has a pair of its own (few_alone), and they share the tokens' lines.
 //
 // k tiles in groups of 8: lane q takes the groups 8 q + j (j = tile of the 8)
-// of 32, so its 8 codes are one load, and the tokens' operand is read from
-// there, too.  Up to 4 tokens are read as they are (no launch before): a wave
+// of 32, so its 8 codes are one load (from any address: vector loads take
+// those), and the tokens' operand is read from there, too.  Up to 4 tokens are read as they are (no launch before): a wave
 // brings its share of a token's row to fp16 under a power of two of its own.
+typedef uint32_t codes16_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t codes8_t __attribute__((ext_vector_type(2), aligned(1)));
 struct FewArgs {
     MatArgs m;
     int64_t pairs;
@@ -1178,10 +1180,10 @@ __global__ void __launch_bounds__(256, TT >= 6 || OWN ? 2 : 3) few_kernel(const 
         const int g = min(sup, sups - 1) * 32 + q * 8, at = g < ng ? g : 0;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            c.a[i] = *(const u32x4*)(p0[i] + at);
-            if constexpr (S2 == VQ2_S2_U16) c.b[i] = *(const u32x4*)(p1[i] + at * 2);
+            c.a[i] = *(const codes16_t*)(p0[i] + at);
+            if constexpr (S2 == VQ2_S2_U16) c.b[i] = *(const codes16_t*)(p1[i] + at * 2);
             if constexpr (S2 == VQ2_S2_U8) {
-                const u32x2 u = *(const u32x2*)(p1[i] + at);
+                const u32x2 u = *(const codes8_t*)(p1[i] + at);
                 c.b[i].x = u.x;
                 c.b[i].y = u.y;
             }
@@ -1598,7 +1600,8 @@ Plan plan_of(const PanelCall& c)
     p.book = b.take(p.books * 4);
     p.sc = b.take(p.tiles * 16 * 4);
     p.xp = b.take(p.tp * c.n * 2);
-    const bool w = c.what != PRODUCT || c.ds[0];  // (also where few_kernel is ahead: it needs aligned planes)
+    // (none of a matrix is kept where few_kernel takes all chunks: one token's loss over 151936 x 2048 had 134 MB)
+    const bool w = grad ? c.what != PRODUCT || c.ds[0] : !p.few[0] || !p.few[1];
     p.w = b.take(w ? p.piece * 16 * c.n * 2 * p.parts : 0);
     if (grad) {
         p.wt = b.take(p.piece * 16 * p.np * 2 * p.tparts);
@@ -1774,7 +1777,7 @@ int panel_launch(const PanelCall& c)
         const int tokens = (int)std::min(p.chunk, c.tokens - t0);
         const int tp = (int)up(tokens, PG_N);
         const int64_t ds_ld = p.tiles * 16;
-        const bool few_call = aligned && p.few[tokens < p.chunk];
+        const bool few_call = p.few[tokens < p.chunk];
         const void* dy = c.dy ? (const char*)c.dy + t0 * c.rows * dt_size(c.dy_dt) : nullptr;
         const int64_t* target = c.target ? c.target + t0 : nullptr;
         const int dy_vec = dy && c.rows % 8 == 0 && (uintptr_t)dy % 16 == 0;

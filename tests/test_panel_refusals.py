@@ -115,3 +115,14 @@ def test_fp32_gradients_have_a_name_of_their_own():
     for entry, sizes in (("head_loss", (3, 100, 128, 2, 1)), ("gated_rows", (3, 100, 128, 2, 1)), ("gemm", (3, 100, 128, 2, 1))):
         ws = getattr(L, f"vq2_{entry}_backward_workspace")
         assert ws(*sizes, _lib.DT_F32_RANGE, 0) == ws(*sizes, 1, 0) > ws(*sizes, 2, 0) > 0
+
+
+def test_few_tokens_keep_no_weights():
+    """the workspace of calls that gather centroids as they go holds no dequantized rows: tokens, sums and no more"""
+    L = _lib.load()
+    for s2, cb in ((0, 1), (1, 1), (2, 2)):
+        assert L.vq2_head_loss_workspace(1, 151936, 2048, s2, cb) < 8 << 20
+        assert L.vq2_head_loss_workspace(64, 151936, 2048, s2, cb) < 8 << 20
+        assert L.vq2_gated_rows_workspace(1, 6144, 2048, s2, cb, 2) < 2 << 20
+    # where weights are kept they are there: 4096 tokens read 32768 rows of them at a time
+    assert L.vq2_head_loss_workspace(4096, 151936, 2048, 0, 1) > 32768 * 2048 * 2
