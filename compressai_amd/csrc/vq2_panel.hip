@@ -703,7 +703,7 @@ __device__ __forceinline__ void gate_act(float g, float& f, float& df)
         const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));  // (2^-23 of it; a division's 10 instructions show)
         f = g * s;
         df = s * (1.0f + g * (1.0f - s));
-        if (g < -80.0f) f = df = 0.0f;  // (also -inf; the true values are below 1e-32)
+        if (g == NEG_INF) f = df = 0.0f;  // (below -87 the sigmoid is no normal number: 0)
     } else {
         // g / (1 + exp(-2 u)), u the tanh form's argument
         const float g2 = g * g, u2 = 1.5957691216057308f * g * (1.0f + 0.044715f * g2);
