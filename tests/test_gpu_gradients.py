@@ -347,3 +347,62 @@ def test_results_may_be_written_over(dev):
                         assert y.shape[-1] in (rows, H, I, V) and y.requires_grad
                     grads.append(torch.autograd.grad(ys, leaf, [torch.ones_like(y) for y in ys])[0])
                 assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("dtype,roundings", [(torch.float32, 24), (torch.float16, 76)])
+def test_step_of_a_model(dev, dtype, roundings):
+    """an embedding, two blocks and a head: every gradient against the same model's in 64 bits, and the 64-bit loss changes
+    along the gradients that were given by their own squares.  Roundings to 11 bits: fp32 activations: x rotated, act, act
+    rotated in each block, x rotated in front of the head, and five terms between products on the way back; fp16 ones, also
+    the embedding's rows, each norm's y and h, the block's result, and as many on the way back; each as often again for
+    what it does to the values it meets"""
+    cbs = books(dev)
+    blocks = [PackedMLP(*(lin(100 + 10 * k + j, I, H, "mlp.in", cbs) for j in range(2)), lin(102 + 10 * k, H, I, "mlp.down", cbs)) for k in range(2)]
+    head = PackedLMHead(lin(125, V, H, "head", cbs))
+    mats = [m for b in blocks for m in (b.gate, b.up, b.down)] + [head.lin]
+    for m in mats:
+        m.scale = m.scale.float().requires_grad_()
+    emb = torch.randn(V, H, generator=synth.gen(126)).to(dev).requires_grad_()
+    norms = [(torch.rand(H, generator=synth.gen(127 + k)) + 0.5).to(dev).requires_grad_() for k in range(3)]
+    tok = torch.randint(0, V, (64,), generator=synth.gen(128)).to(dev)
+    params = [emb, *norms, *(m.scale for m in mats)]
+
+    def loss():
+        h, x = None, emb[tok[:-1]].to(dtype)
+        for w, mlp in zip(norms, blocks):
+            y, h = T.add_rms_norm(x, w, torch.zeros_like(x) if h is None else h)
+            x = mlp(y)
+        y, _ = T.add_rms_norm(x, norms[2], h)
+        return head.loss(y, tok[1:]).sum()
+
+    def loss64(emb, n0, n1, n2, *s):
+        h = emb[tok[:-1]]
+        x = torch.zeros_like(h)
+        norm = lambda h, w: h / torch.sqrt(h.pow(2).mean(-1, keepdim=True) + 1e-6) * w
+        for k, (w, b) in enumerate(zip((n0, n1), blocks)):
+            h = h + x
+            y = norm(h, w)
+            act = torch.nn.functional.silu(linear64(b.gate, y, s[3 * k])) * linear64(b.up, y, s[3 * k + 1])
+            x = linear64(b.down, act, s[3 * k + 2])
+        z = linear64(head.lin, norm(h + x, n2), s[6])
+        return torch.nn.functional.cross_entropy(z, tok[1:], reduction="sum")
+
+    rel = roundings * 2.0 ** -11
+    got = torch.autograd.grad(loss(), params)
+    p64 = [p.detach().double().requires_grad_() for p in params]
+    value = loss64(*p64)
+    want = torch.autograd.grad(value, p64)
+    assert abs(loss().item() - value.item()) <= rel * value.item()
+    for g, w in zip(got, want):
+        close(g, w, rel)
+    for k, (g, w) in enumerate(zip(got, want)):
+        g = g.double()
+        with torch.no_grad():
+            ends = []
+            step = 1e-4 / g.norm()
+            for sign in (1, -1):
+                at = [p + sign * step * g if j == k else p for j, p in enumerate(p64)]
+                ends.append(loss64(*at))
+        along = (ends[0] - ends[1]) / (2 * step)
+        # (third order: step^2 of the curvature's change, some 1e-8)
+        assert abs(along - g.pow(2).sum()) <= rel * g.norm() * w.norm() + 1e-6 * g.pow(2).sum()
