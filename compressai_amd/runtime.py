@@ -344,7 +344,8 @@ class PackedMLP(nn.Module):
     down; a single row of SiLU matrices with the sorted layout goes through it
     instead (three launches: gate + up, SwiGLU with down's rotation, down).
     Activations are held in x's type (fp32: fp16).  Differentiable in x and in
-    the three ``scale``s that require it."""
+    the three ``scale``s that require it.  gate and up are not called as modules,
+    nor is down by the three launches of one row: hooks of theirs see no call."""
 
     def __init__(self, gate, up, down, activation="silu"):
         super().__init__()

@@ -2,7 +2,8 @@
 
 What a packed model learns without touching its codes: the norms' weights, the
 row scales (make ``PackedLinear.scale`` a leaf: ``lin.scale.requires_grad_()``, in
-fp32 for small steps), and whatever produces the activations (adapters, other
+fp32 for small steps; it is no parameter of its module and not in its
+``state_dict``: keep and store what was tuned), and whatever produces the activations (adapters, other
 layers).  The functions here are differentiable once in all of these; each is
 one entry of ``kernels`` forward and one backward:
 
@@ -25,7 +26,8 @@ no dequantized matrix is kept.
 A step that is captured into a graph makes its leaves inside (``detach()``,
 ``requires_grad_()``) and takes their gradients with ``torch.autograd.grad``: a
 ``backward()`` that is captured while an eager graph of the same leaves lives would
-wait for that graph's stream, which a capture does not allow.
+wait for that graph's stream, which a capture does not allow.  The functions are
+plain ``torch.autograd.Function``s: ``torch.func``'s transforms do not take them.
 """
 from __future__ import annotations
 
