@@ -1117,7 +1117,7 @@ __global__ void __launch_bounds__(256) dy_panel_kernel(const DyArgs<V16> a)
 // operand it is (lane (row, q): group q of a k tile), and nothing is written in
 // between.  The gathers bound it: 240 G a second over the device, whatever
 // their size (a request of a line each): one token of a 151936 x 2048 head (38.9 M
-// codes, 162 us by them) takes 170 us, of the block of 2 x 6144 x 2048 at 4 bits (6.3 M,
+// codes, 162 us by them) takes 171 us, of the block of 2 x 6144 x 2048 at 4 bits (6.3 M,
 // 26 us) 34.  A wave takes two tiles of 16 rows (for the block: gate and up).
 // The 4 waves of a workgroup share the k tiles of one pair and meet in LDS, so
 // that small matrices fill the device; with many rows and more than 64 tokens
@@ -1540,7 +1540,7 @@ int few_groups(const PanelCall& c, int64_t tokens)
 // times as many and 2.8 * 10^6.  Measured (us a call; codes of the call, tokens: few /
 // panels): 65 k, 512 15 / 24; 262 k, 1024 31 / 39, 2048 45 / 42; 512 k, 333 25 / 37, 1024 43 / 41;
 // 3.1 M, 128 33 / 51, 256 54 / 52, 512 96 / 59; 6.3 M, 128 51 / 61, 192 82 / 62; 12.9 M, 128
-// 108 / 128, 160 190 / 140; 38.9 M, 1 174 / 335, 128 270 / 335, 160 478 / 367.
+// 108 / 128, 160 190 / 140; 38.9 M, 1 171 / 335, 128 270 / 335, 160 478 / 367.
 bool few_ahead(const PanelCall& c, int64_t tokens)
 {
     if (c.cb_dt == VQ2_DT_F32) return false;  // (its centroids would take two products each)

@@ -77,10 +77,11 @@ __device__ __forceinline__ void panel_to_lds(const half8_t* g, half8_t* l)
 }
 
 // Product of a workgroup of 2 x 2 waves: wave tiles of 16 MT rows of panel a
-// (weights) times 64 rows of panel b (tokens).  Bound by the matrix cores, on long
-// runs by their power: 32768 x 4096 x 2048 takes 440 us with the loss's statistics
-// behind it (1.25 PFLOP/s, matrix cores busy in 66 % of the cycles), 12288 x 4096 x
-// 2048 196 with the gated block's (1.05).  A k tile is 12 KiB of LDS reads for 32 matrix
+// (weights) times 64 rows of panel b (tokens).  Bound by the matrix cores and
+// the epilogues between their products (busy in 59 to 78 % of the cycles), on long runs
+// with lower clocks: 32768 x 4096 x 2048 takes 440 to 460 us with the loss's statistics
+// behind it (1.25 to 1.19 PFLOP/s), 12288 x 4096 x 2048 183 to 196 with the gated block's
+// (1.13 to 1.05).  A k tile is 12 KiB of LDS reads for 32 matrix
 // instructions of a wave (MT 8): larger tiles leave no registers for an epilogue.
 constexpr int PG_WM = 2, PG_WN = 2, PG_NT = 4, PG_BUF = 3;
 constexpr int PG_THREADS = 64 * PG_WM * PG_WN;

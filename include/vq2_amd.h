@@ -777,8 +777,12 @@ int vq2_add_rms_norm_backward(const void* dy, int dy_dt, const void* h, int h_dt
  *   workspace  256-byte aligned, of the entry's _workspace bytes (scale_grad:
  *           whether dscale is wanted); contents on entry do not matter
  * Weights are multiplied in fp16 (where an fp16 or fp32 result depends on more bits, as
- * two addends of it): bf16 / fp32 codebooks hold values up to 65504, and what is below
- * 2^-14 in them is held in steps of 2^-24.
+ * two addends of it): bf16 / fp32 codebooks, and the sums of two stages, hold values up to
+ * 65504, and what is below 2^-14 in them is held in steps of 2^-24.  A gradient is rounded
+ * to fp16 between its two products under the largest row scale's power of two: of the
+ * loss's softmax times its scale, what is below about 2^-39 of the largest scale is 0.
+ * A NaN or an infinity in a token's rows shows in its own results (for an infinity they
+ * may be NaN) and in the scales' gradients, the sums over all tokens, alone.
  * Results do not depend on what ran before, and sums have a fixed order. */
 #define VQ2_PANEL_MAX_N 32768
 #define VQ2_PANEL_MAX_ROWS 4194304
