@@ -117,7 +117,11 @@ def _grad_wanted(x, lins):
 class PackedLinear(nn.Module):
     """Differentiable in x, and in ``scale`` where it is made a leaf (in fp32
     for small steps; it is a buffer that ``state_dict`` leaves out, so a tuned
-    one is stored by its owner).  ``scale_dtype``: the row scales are held in bf16 by default, as the
+    one is stored by its owner), for widths that are multiples of 64 up to
+    ``kernels.PANEL_MAX_N`` whose planes were not released; the scales'
+    gradients read the rotated rows in 16 bits (fp32: fp16).
+
+    ``scale_dtype``: the row scales are held in bf16 by default, as the
     reference rounds them at construction (vq2/runtime.py:78); ``None`` keeps
     the given dtype (e.g. the container's fp16 scales, one rounding fewer)."""
 
