@@ -372,7 +372,9 @@ class PackedMLP(nn.Module):
             return down(T.gated_of(gate, up, x, self.activation), out_dtype=od)
         x2 = x.reshape(-1, gate.n).contiguous()
         g0, g1, cb0, cb1 = gate._planes()
-        if self.activation == "silu" and all(m._sorted_ok(x2.shape[0], m._planes()[2]) for m in mats):
+        B = x2.shape[0]
+        if (self.activation == "silu" and gate._sorted_ok(B, cb0) and up._sorted_ok(B, cb0)
+                and down._sorted_ok(B, (books := down._planes()[2:])[0])):
             I = gate.out
             gu = torch.empty(2 * I, dtype=torch.float32, device=x.device)
             xs, perm, sign, hb, sc = gate._sorted_args(x2.reshape(-1))
@@ -380,8 +382,7 @@ class PackedMLP(nn.Module):
                              ys=[gu[:I], gu[I:]])
             r = down.rot
             act = K.vq_swiglu_rht(gu, I, r._perm32, r._sign8, r.hb, r.scale)
-            _, _, d0, d1 = down._planes()
-            y = K.vq_sorted_gemv(act, [(down.sorted, down.scale)], d0, d1, I, hb=0, out_dtype=od)[0]
+            y = K.vq_sorted_gemv(act, [(down.sorted, down.scale)], *books, I, hb=0, out_dtype=od)[0]
             return y.view(*x.shape[:-1], down.out)
         if gate.planes_released or up.planes_released:
             raise K.Vq2Error("PackedMLP: the index planes, which more than one row needs, were released")
